@@ -484,6 +484,83 @@ int simsd_moe_ep_send(const void* x, int64_t ldx, const int32_t* send_slot, cons
 int simsd_moe_ep_return(const void* y, int64_t ldy, const int32_t* recv_expert, int H, int capacity,
                         int rank, int world, void* const* peer_back, int dtype, void* stream);
 
+/* ---- batched serving: a paged key-value cache and the verification of drafted
+ * tokens (no counterpart in the reference's kernels; its decode loop keeps one
+ * static cache per sequence, speculative_decoding/cache_aware.py:195-215, and
+ * its sampling acceptance is torch code, mrs.py:14-108).
+ *
+ * The caches are [num_pages, Hk, page_size, head_dim] with the strides ld_page,
+ * ld_head and ld_tok (elements, multiples of 8) and unit head_dim stride, on
+ * 16-byte aligned bases; slot s is token s % page_size of page s / page_size.
+ * head_dim 64 or 128, bf16 or fp16.  `err_word` (device int or NULL) receives
+ * SIMSD_DEV_ERR_BAD_INDEX for an index outside its tensor; nothing is read or
+ * written for it.  The workspaces of these calls are plain scratch: no header, no
+ * initialisation, not read after the call's kernels, so each call may bring its
+ * own. */
+
+/*
+ * Append T tokens: per token t with slot s = slots[t] >= 0,
+ *   q_out[t, h] = r(n(q)), K[s] = r(n(k)), V[s] = v
+ * with n the RMSNorm over the head with q_weight / k_weight [head_dim] (NULL: no
+ * norm) and r the rotation of the first rotary_dim elements in pairs (i, i +
+ * rotary_dim / 2) by row positions[t] of cos / sin [n_positions, rotary_dim / 2]
+ * (fp32); fp32 arithmetic, one rounding.  A negative slot writes nothing to the
+ * caches and a zero q row, and its position is not read.  qkv [T, (Hq + 2 Hk)
+ * head_dim] with row stride ldqkv (q heads, k heads, v heads), q_out [T, Hq,
+ * head_dim].  Slots of one call are distinct.  rotary_dim: a multiple of 16, <=
+ * head_dim.  Replaces, for a batch, the q/k norm, rotary embedding and cache
+ * write of sdar/modeling_sdar.py:197-302.
+ */
+int simsd_paged_append(const void* qkv, int64_t ldqkv, int T, int Hq, int Hk, int head_dim, int rotary_dim,
+                       const void* q_weight, const void* k_weight, float eps, const float* cos, const float* sin,
+                       int64_t n_positions, const int64_t* positions, const int64_t* slots, void* q_out, void* k_cache,
+                       void* v_cache, int num_pages, int page_size, int64_t ld_page, int64_t ld_head, int64_t ld_tok,
+                       int dtype, int* err_word, void* stream);
+
+/*
+ * Attention of L query tokens per sequence over its pages, native GQA (g = h /
+ * (Hq / Hk)):
+ *   o[b, t, h] = softmax_j(scale q[b, t, h] . k_j) v_j,  lse = log sum_j exp(scale q . k_j)
+ * over sequence b's visible keys j < n = seq_lens[b] (key j: token j % page_size
+ * of page page_table[b * ld_table + j / page_size], j / page_size < max_pages).
+ * The newest L keys are the queries' own: with jt = j - (n - L), keys with jt < 0
+ * are visible to every query, the others where jt <= t, or, with tail_mask, where
+ * tail_mask[b * ldm_b + t * ldm_t + jt] != 0.  A query without a visible key: o =
+ * 0, lse = -inf.  q, o [B, L, Hq, head_dim] contiguous, lse [B, L, Hq] or NULL.
+ * The lengths are read on the device only.
+ */
+size_t simsd_paged_attention_workspace_size(int B, int L, int Hq, int Hk, int head_dim);
+int simsd_paged_attention(const void* q, const void* k_cache, const void* v_cache, int num_pages, int page_size,
+                          int64_t ld_page, int64_t ld_head, int64_t ld_tok, const int32_t* page_table, int64_t ld_table,
+                          int max_pages, const int32_t* seq_lens, const uint8_t* tail_mask, int64_t ldm_b, int64_t ldm_t,
+                          int B, int L, int Hq, int Hk, int head_dim, float scale, void* o, float* lse, int dtype,
+                          void* workspace, size_t workspace_bytes, int* err_word, void* stream);
+
+/*
+ * Speculative sampling's verification from given random numbers.  For sequence b
+ * with d = n_draft[b] (K when NULL) drafted tokens x_i, p_i = softmax(target row i
+ * / T) and q_i = softmax(draft row i / T) (draft_logits NULL: one at x_i), T =
+ * temperature[b] (1 when NULL; 0: one at the row's first maximum):
+ *   x_i is kept while uniform[b, i] q_i(x_i) < p_i(x_i); at the first one refused
+ *   the next token is argmax_v max(p - q, 0)(v) / noise[b, v], after d kept ones
+ *   argmax_v p_d(v) / noise[b, v]  (noise positive, exponentially distributed;
+ *   ties to the lowest v; a residual that is nowhere positive draws from p).
+ * tokens [B, K + 1]: the kept ones, the drawn one, then -1; accepted [B]: how many
+ * were kept; logprobs [B, K + 1]: log p of each, 0 after them.  target_logits
+ * [B, K + 1, V] (strides ldt_b, ldt_r, unit last), draft_logits [B, K, V],
+ * draft_tokens [B, K] (ld_x), uniform [B, K] (ld_u), noise [B, V] (ld_n).  NaN
+ * logits count as -inf, +inf as the largest finite number.  A drafted token
+ * outside [0, V) is refused (SIMSD_DEV_ERR_BAD_INDEX), the next one drawn from p.
+ * Replaces mrs_verify (speculative_decoding/mrs.py:14-108) for a batch.
+ */
+size_t simsd_speculative_verify_workspace_size(int B, int K, int V);
+int simsd_speculative_verify(const void* target_logits, int64_t ldt_b, int64_t ldt_r, const void* draft_logits,
+                             int64_t ldd_b, int64_t ldd_r, const int64_t* draft_tokens, int64_t ld_x,
+                             const float* uniform, int64_t ld_u, const float* noise, int64_t ld_n,
+                             const float* temperature, const int32_t* n_draft, int B, int K, int V, int dtype,
+                             int64_t* tokens, int64_t* accepted, float* logprobs, void* workspace,
+                             size_t workspace_bytes, int* err_word, void* stream);
+
 #ifdef __cplusplus
 }
 #endif

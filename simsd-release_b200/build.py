@@ -18,6 +18,7 @@ PKG = Path(__file__).resolve().parent
 REPO = PKG.parent
 CSRC = PKG / "csrc"
 OUT = PKG / "kernels" / "libsimsd_b200.so"
+OBJ = PKG / "_build"
 ARCH = ["-gencode", "arch=compute_100a,code=sm_100a"]
 
 
@@ -35,17 +36,27 @@ def build(force: bool = False, verbose: bool = False) -> Path:
         newest = max(p.stat().st_mtime for p in sources())
         if OUT.stat().st_mtime >= newest:
             return OUT
-    cmd = [nvcc(), "-O3", "-std=c++17", *ARCH, "-lineinfo", "-Xcompiler", "-fPIC,-O3", "-shared",
-           "-Xptxas", "-v" if verbose else "-O3",
-           "-I", str(REPO / "include"), "-o", str(OUT) + ".tmp", str(CSRC / "capi.cu")]
-    r = subprocess.run(cmd, capture_output=True, text=True)
-    if r.returncode != 0:
-        sys.stderr.write(r.stdout + r.stderr)
-        raise RuntimeError(f"nvcc failed ({r.returncode}): {' '.join(cmd)}")
-    if verbose:
-        sys.stderr.write(r.stderr)
+    OBJ.mkdir(exist_ok=True)
+    units = sorted(CSRC.glob("*.cu"))
+    objs = [str(OBJ / (u.stem + ".o")) for u in units]
+    # the translation units compile side by side, then link into one library
+    run([[nvcc(), "-O3", "-std=c++17", *ARCH, "-lineinfo", "-Xcompiler", "-fPIC,-O3", "-Xptxas",
+          "-v" if verbose else "-O3", "-I", str(REPO / "include"), "-c", "-o", o, str(u)]
+         for u, o in zip(units, objs)], verbose)
+    run([[nvcc(), *ARCH, "-shared", "-Xcompiler", "-fPIC", "-o", str(OUT) + ".tmp", *objs]], verbose)
     os.replace(str(OUT) + ".tmp", OUT)
     return OUT
+
+
+def run(cmds: list[list[str]], verbose: bool) -> None:
+    procs = [subprocess.Popen(c, stdout=subprocess.PIPE, stderr=subprocess.STDOUT, text=True) for c in cmds]
+    outs = [p.communicate()[0] for p in procs]
+    for c, p, out in zip(cmds, procs, outs):
+        if p.returncode != 0:
+            sys.stderr.write(out)
+            raise RuntimeError(f"nvcc failed ({p.returncode}): {' '.join(c)}")
+        if verbose:
+            sys.stderr.write(out)
 
 
 if __name__ == "__main__":

@@ -1,0 +1,228 @@
+// A paged key-value cache: the append that writes tokens into it and the
+// attention that reads it.
+//
+// The cache is [pages, Hk, page size, D] with any page, head and token strides
+// (unit D stride), so a head-major and a token-major cache are the same code.
+// Slot s is token s % page_size of page s / page_size; sequence b's key j is
+// token j % page_size of page page_table[b, j / page_size].  Every offset into
+// the cache is 64-bit.
+#pragma once
+#include "sm100.cuh"
+
+namespace simsd {
+
+// ---------------------------------------------------------------- append
+// Per token t with slot s >= 0 (s < 0: nothing written to the cache, q row zero):
+//   n(x)  = w x / sqrt(mean(x^2) + eps)   (q and k heads; w == nullptr: n(x) = x)
+//   r(x)  = (x_i c_i - x_{i+R/2} s_i, x_{i+R/2} c_i + x_i s_i) for i < R/2, the
+//           rest unchanged; c, s: the rows of the position's table entry
+//   q_out[t, h] = r(n(q)), K[s] = r(n(k)), V[s] = v
+// in fp32 with one rounding at the end.
+struct PagedAppendArgs {
+  const void* qkv;        // [T, (Hq + 2 Hk) D], row stride ldqkv
+  const void* qw;         // [D] or nullptr
+  const void* kw;
+  const float* cos;       // [n_pos, R / 2]
+  const float* sin;
+  const long long* positions;
+  const long long* slots;
+  void* q_out;            // [T, Hq, D]
+  void* k_cache;
+  void* v_cache;
+  int* err;
+  long long ldqkv, n_pos, n_slots, ld_page, ld_head, ld_tok;
+  int Hq, Hk, R, page_size, dtype;
+  float eps;
+};
+
+constexpr int PA_THREADS = 256;
+
+__device__ __forceinline__ void paged_unpack8(uint4 u, int dtype, float (&v)[8]) {
+  const uint32_t w[4] = {u.x, u.y, u.z, u.w};
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    float2 f;
+    if (dtype == 0) {
+      f.x = __uint_as_float(w[i] << 16);
+      f.y = __uint_as_float(w[i] & 0xffff0000u);
+    } else {
+      f = __half22float2(*reinterpret_cast<const __half2*>(&w[i]));
+    }
+    v[2 * i] = f.x;
+    v[2 * i + 1] = f.y;
+  }
+}
+__device__ __forceinline__ uint4 paged_pack8(const float (&f)[8], int dtype) {
+  uint32_t w[4];
+#pragma unroll
+  for (int i = 0; i < 4; ++i)
+    w[i] = (uint32_t)f32_to_16bit(f[2 * i], dtype) | ((uint32_t)f32_to_16bit(f[2 * i + 1], dtype) << 16);
+  return make_uint4(w[0], w[1], w[2], w[3]);
+}
+
+// One CTA per token.  A head's D elements are D / 8 neighbouring threads of 8
+// elements (16-byte loads and stores); PA_THREADS is a multiple of D / 8, so a
+// thread keeps its place in the head over its heads and its rotary row stays in
+// registers.  The pair of element i lies R / 16 threads away.
+template <int D>
+__global__ void __launch_bounds__(PA_THREADS) paged_append_kernel(const PagedAppendArgs p) {
+  griddep_launch_dependents();
+  griddep_wait();
+  constexpr int LANES = D / 8;
+  const long long t = blockIdx.x;
+  const int tid = threadIdx.x;
+  const int i8 = tid % LANES;
+  const long long slot = p.slots[t];
+  long long pos = p.positions[t];
+  const bool bad = slot >= p.n_slots || (slot >= 0 && (pos < 0 || pos >= p.n_pos));
+  if (bad && tid == 0 && p.err) atomicOr(p.err, SIMSD_DEV_ERR_BAD_INDEX);
+  const bool live = slot >= 0 && !bad;
+  const int rl = p.R / 16;                       // threads of half a rotation
+  const bool rot = live && i8 < 2 * rl;
+  const bool low = i8 < rl;
+  float c[8], s[8];
+#pragma unroll
+  for (int e = 0; e < 8; ++e) c[e] = 1.0f, s[e] = 0.0f;
+  if (rot) {
+    const long long at = pos * (p.R / 2) + (low ? i8 : i8 - rl) * 8;
+    const float4 c0 = *reinterpret_cast<const float4*>(p.cos + at), c1 = *reinterpret_cast<const float4*>(p.cos + at + 4);
+    const float4 s0 = *reinterpret_cast<const float4*>(p.sin + at), s1 = *reinterpret_cast<const float4*>(p.sin + at + 4);
+    c[0] = c0.x, c[1] = c0.y, c[2] = c0.z, c[3] = c0.w, c[4] = c1.x, c[5] = c1.y, c[6] = c1.z, c[7] = c1.w;
+    s[0] = s0.x, s[1] = s0.y, s[2] = s0.z, s[3] = s0.w, s[4] = s1.x, s[5] = s1.y, s[6] = s1.z, s[7] = s1.w;
+    if (low) {
+#pragma unroll
+      for (int e = 0; e < 8; ++e) s[e] = -s[e];
+    }
+  }
+  const int lane = tid & 31;
+  const int partner = !rot ? lane : low ? lane + rl : lane - rl;
+  const int H = p.Hq + 2 * p.Hk;
+  const long long page = live ? slot / p.page_size : 0;
+  const long long base = live ? page * p.ld_page + (slot - page * p.page_size) * p.ld_tok + i8 * 8 : 0;
+  const uint16_t* row = reinterpret_cast<const uint16_t*>(p.qkv) + t * p.ldqkv + i8 * 8;
+  uint16_t* q = reinterpret_cast<uint16_t*>(p.q_out) + t * p.Hq * D + i8 * 8;
+  for (int h0 = 0; h0 < H; h0 += PA_THREADS / LANES) {
+    const int h = h0 + tid / LANES;
+    const bool in = h < H && live;
+    const uint4 raw = in ? *reinterpret_cast<const uint4*>(row + (long long)h * D) : make_uint4(0, 0, 0, 0);
+    float x[8];
+    paged_unpack8(raw, p.dtype, x);
+    const void* w = h < p.Hq ? p.qw : p.kw;
+    float ss = 0.0f;
+#pragma unroll
+    for (int e = 0; e < 8; ++e) ss = fmaf(x[e], x[e], ss);
+#pragma unroll
+    for (int m = LANES / 2; m > 0; m >>= 1) ss += __shfl_xor_sync(0xffffffffu, ss, m);
+    if (w != nullptr) {
+      const float inv = rsqrtf(ss * (1.0f / D) + p.eps);
+      float wf[8];
+      paged_unpack8(*reinterpret_cast<const uint4*>(reinterpret_cast<const uint16_t*>(w) + i8 * 8), p.dtype, wf);
+#pragma unroll
+      for (int e = 0; e < 8; ++e) x[e] = x[e] * inv * wf[e];
+    }
+    float o[8];
+#pragma unroll
+    for (int e = 0; e < 8; ++e) {
+      const float other = __shfl_sync(0xffffffffu, x[e], partner);
+      o[e] = rot ? fmaf(other, s[e], x[e] * c[e]) : x[e];
+    }
+    if (h >= H) continue;
+    if (h < p.Hq) {
+      *reinterpret_cast<uint4*>(q + (long long)h * D) = live ? paged_pack8(o, p.dtype) : make_uint4(0, 0, 0, 0);
+    } else if (live) {
+      const bool is_k = h < p.Hq + p.Hk;
+      uint16_t* dst = reinterpret_cast<uint16_t*>(is_k ? p.k_cache : p.v_cache) + base +
+                      (long long)(h - p.Hq - (is_k ? 0 : p.Hk)) * p.ld_head;
+      *reinterpret_cast<uint4*>(dst) = is_k ? paged_pack8(o, p.dtype) : raw;
+    }
+  }
+}
+
+// ---------------------------------------------------------------- attention
+//   o[b, t, h, :] = sum_j p_j v_j / sum_j p_j,  p_j = exp(scale q . k_j - max),
+// over the visible keys j < n = min(seq_lens[b], max_pages page_size) of KV head
+// g = h / (Hq / Hk).  The newest L keys belong to the L query tokens: with jt =
+// j - (n - L), a key with jt < 0 is visible to all of them, the others where
+// jt <= t, or where tail_mask[b, t, jt] is set.  No visible key: o = 0, lse = -inf.
+struct PagedAttnArgs {
+  const void* q;            // [B, L, Hq, D]
+  const void* k_cache;
+  const void* v_cache;
+  const int* page_table;    // [B, ld_table]
+  const int* seq_lens;      // [B]
+  const uint8_t* tail;      // [B, L, L] bytes or nullptr
+  void* o;                  // [B, L, Hq, D]
+  float* lse;               // [B, L, Hq] or nullptr
+  int* err;
+  long long ld_page, ld_head, ld_tok, ld_table, ldm_b, ldm_t;
+  int B, L, Hq, Hk, G, num_pages, page_size, max_pages, dtype;
+  float scale_log2;         // scale * log2(e)
+};
+
+constexpr int PAT_THREADS = 128;
+
+__device__ __forceinline__ int paged_len(const PagedAttnArgs& p, int b) {
+  int n = p.seq_lens[b];
+  const long long cap = (long long)p.max_pages * p.page_size;
+  if (n > cap) {
+    if (threadIdx.x == 0 && p.err) atomicOr(p.err, SIMSD_DEV_ERR_BAD_INDEX);
+    n = (int)cap;
+  }
+  return n < 0 ? 0 : n;
+}
+
+// One CTA per row; warp w takes keys w, w + 4, ..., lane l elements l, l + 32, ...
+template <int D>
+__global__ void __launch_bounds__(PAT_THREADS) paged_attention_kernel(const PagedAttnArgs p) {
+  griddep_launch_dependents();
+  griddep_wait();
+  constexpr int E = D / 32, W = PAT_THREADS / 32;
+  __shared__ float sm[W], sl[W], so[W][D];
+  const long long row = blockIdx.x;
+  const int h = (int)(row % p.Hq), t = (int)(row / p.Hq % p.L), b = (int)(row / p.Hq / p.L);
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  const int n = paged_len(p, b);
+  const long long head = (long long)(h / p.G) * p.ld_head;
+  float q[E], o[E], m = -INFINITY, l = 0.0f;
+#pragma unroll
+  for (int e = 0; e < E; ++e) q[e] = load_f(p.q, row * D + lane + 32 * e, p.dtype), o[e] = 0.0f;
+  for (int j = warp; j < n; j += W) {
+    const int jt = j - (n - p.L);
+    if (jt >= 0 && !(p.tail ? p.tail[b * p.ldm_b + t * p.ldm_t + jt] != 0 : jt <= t)) continue;
+    const int pg = p.page_table[b * p.ld_table + j / p.page_size];
+    if (pg < 0 || pg >= p.num_pages) {
+      if (lane == 0 && p.err) atomicOr(p.err, SIMSD_DEV_ERR_BAD_INDEX);
+      continue;
+    }
+    const long long at = pg * p.ld_page + head + (j % p.page_size) * p.ld_tok + lane;
+    float s = 0.0f;
+#pragma unroll
+    for (int e = 0; e < E; ++e) s = fmaf(q[e], load_f(p.k_cache, at + 32 * e, p.dtype), s);
+#pragma unroll
+    for (int d = 16; d > 0; d >>= 1) s += __shfl_xor_sync(0xffffffffu, s, d);
+    s *= p.scale_log2;
+    const float mn = fmaxf(m, s);
+    if (mn == -INFINITY) continue;
+    const float a = exp2f(m - mn), w = exp2f(s - mn);
+    m = mn;
+    l = fmaf(l, a, w);
+#pragma unroll
+    for (int e = 0; e < E; ++e) o[e] = fmaf(o[e], a, w * load_f(p.v_cache, at + 32 * e, p.dtype));
+  }
+  if (lane == 0) sm[warp] = m, sl[warp] = l;
+#pragma unroll
+  for (int e = 0; e < E; ++e) so[warp][lane + 32 * e] = o[e];
+  __syncthreads();
+  float mt = -INFINITY, lt = 0.0f;
+  for (int w = 0; w < W; ++w) mt = fmaxf(mt, sm[w]);
+  const float mu = mt == -INFINITY ? 0.0f : mt;
+  for (int w = 0; w < W; ++w) lt += sl[w] * exp2f(sm[w] - mu);
+  for (int d = threadIdx.x; d < D; d += PAT_THREADS) {
+    float v = 0.0f;
+    for (int w = 0; w < W; ++w) v += so[w][d] * exp2f(sm[w] - mu);
+    store_f(p.o, row * D + d, lt == 0.0f ? 0.0f : v / lt, p.dtype);
+  }
+  if (p.lse && threadIdx.x == 0) p.lse[row] = lt == 0.0f ? -INFINITY : 0.69314718055994531f * mt + logf(lt);
+}
+
+}  // namespace simsd

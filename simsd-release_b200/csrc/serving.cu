@@ -1,0 +1,196 @@
+// extern "C" entry points of the batched serving operators (declared in
+// include/simsd_b200.h): the paged key-value cache and draft verification.
+#include <cuda_runtime.h>
+
+#include <algorithm>
+
+#include "paged.cuh"
+#include "simsd_b200.h"
+#include "spec_verify.cuh"
+
+using namespace simsd;
+
+namespace {
+
+inline size_t align256(size_t v) { return (v + 255) & ~size_t(255); }
+inline bool al16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15) == 0; }
+
+// Launch on `s`; as a programmatic dependent of the kernel before it on the
+// stream when `dependent` (the second kernel of one call) or SIMSD_LAUNCH_PDL is
+// set.  Every kernel here starts with griddepcontrol.wait.
+template <typename... KArgs, typename... Args>
+int launch_on(void (*kern)(KArgs...), long long grid, int block, size_t smem, void* s, bool dependent, Args&&... args) {
+  if (grid > 0x7fffffffLL) return SIMSD_ERR_UNSUPPORTED;
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3((unsigned)grid);
+  cfg.blockDim = dim3((unsigned)block);
+  cfg.dynamicSmemBytes = smem;
+  cfg.stream = (cudaStream_t)s;
+  cudaLaunchAttribute attr[1];
+  if (dependent || (simsd_get_launch_flags() & SIMSD_LAUNCH_PDL)) {
+    attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr[0].val.programmaticStreamSerializationAllowed = 1;
+    cfg.attrs = attr;
+    cfg.numAttrs = 1;
+  }
+  if (cudaLaunchKernelEx(&cfg, kern, std::forward<Args>(args)...) != cudaSuccess) return SIMSD_ERR_LAUNCH;
+  return cudaGetLastError() == cudaSuccess ? SIMSD_OK : SIMSD_ERR_LAUNCH;
+}
+
+// 16-byte rows of a paged cache
+int cache_check(const void* k, const void* v, int64_t ld_page, int64_t ld_head, int64_t ld_tok) {
+  if (!al16(k) || !al16(v) || (ld_page & 7) || (ld_head & 7) || (ld_tok & 7)) return SIMSD_ERR_ALIGN;
+  return SIMSD_OK;
+}
+
+}  // namespace
+
+extern "C" {
+
+int simsd_paged_append(const void* qkv, int64_t ldqkv, int T, int Hq, int Hk, int head_dim, int rotary_dim,
+                       const void* q_weight, const void* k_weight, float eps, const float* cos, const float* sin,
+                       int64_t n_positions, const int64_t* positions, const int64_t* slots, void* q_out, void* k_cache,
+                       void* v_cache, int num_pages, int page_size, int64_t ld_page, int64_t ld_head, int64_t ld_tok,
+                       int dtype, int* err_word, void* stream) {
+  if (T < 0 || Hq < 1 || Hk < 1 || num_pages < 1 || page_size < 1 || n_positions < 1) return SIMSD_ERR_SHAPE;
+  if (dtype != SIMSD_BF16 && dtype != SIMSD_F16) return SIMSD_ERR_DTYPE;
+  if (head_dim != 64 && head_dim != 128) return SIMSD_ERR_UNSUPPORTED;
+  if (rotary_dim < 0 || rotary_dim > head_dim || rotary_dim % 16) return SIMSD_ERR_UNSUPPORTED;
+  if (T == 0) return SIMSD_OK;
+  if (!qkv || (rotary_dim > 0 && (!cos || !sin)) || !positions || !slots || !q_out || !k_cache || !v_cache) return SIMSD_ERR_SHAPE;
+  if (ldqkv < (int64_t)(Hq + 2 * Hk) * head_dim) return SIMSD_ERR_SHAPE;
+  if (!al16(qkv) || (ldqkv & 7) || !al16(q_out) || !al16(cos) || !al16(sin) || !al16(q_weight) || !al16(k_weight))
+    return SIMSD_ERR_ALIGN;
+  int rc = cache_check(k_cache, v_cache, ld_page, ld_head, ld_tok);
+  if (rc != SIMSD_OK) return rc;
+  PagedAppendArgs a;
+  a.qkv = qkv;
+  a.qw = q_weight;
+  a.kw = k_weight;
+  a.cos = cos;
+  a.sin = sin;
+  a.positions = reinterpret_cast<const long long*>(positions);
+  a.slots = reinterpret_cast<const long long*>(slots);
+  a.q_out = q_out;
+  a.k_cache = k_cache;
+  a.v_cache = v_cache;
+  a.err = err_word;
+  a.ldqkv = ldqkv;
+  a.n_pos = n_positions;
+  a.n_slots = (long long)num_pages * page_size;
+  a.ld_page = ld_page;
+  a.ld_head = ld_head;
+  a.ld_tok = ld_tok;
+  a.Hq = Hq;
+  a.Hk = Hk;
+  a.R = rotary_dim;
+  a.page_size = page_size;
+  a.dtype = dtype;
+  a.eps = eps;
+  return head_dim == 64 ? launch_on(paged_append_kernel<64>, T, PA_THREADS, 0, stream, false, a)
+                        : launch_on(paged_append_kernel<128>, T, PA_THREADS, 0, stream, false, a);
+}
+
+size_t simsd_paged_attention_workspace_size(int B, int L, int Hq, int Hk, int head_dim) {
+  (void)B, (void)L, (void)Hq, (void)Hk, (void)head_dim;
+  return 256;
+}
+
+int simsd_paged_attention(const void* q, const void* k_cache, const void* v_cache, int num_pages, int page_size,
+                          int64_t ld_page, int64_t ld_head, int64_t ld_tok, const int32_t* page_table, int64_t ld_table,
+                          int max_pages, const int32_t* seq_lens, const uint8_t* tail_mask, int64_t ldm_b, int64_t ldm_t,
+                          int B, int L, int Hq, int Hk, int head_dim, float scale, void* o, float* lse, int dtype,
+                          void* workspace, size_t workspace_bytes, int* err_word, void* stream) {
+  if (B < 0 || L < 0 || Hq < 1 || Hk < 1 || Hq % Hk || num_pages < 1 || page_size < 1 || max_pages < 0)
+    return SIMSD_ERR_SHAPE;
+  if (dtype != SIMSD_BF16 && dtype != SIMSD_F16) return SIMSD_ERR_DTYPE;
+  if (head_dim != 64 && head_dim != 128) return SIMSD_ERR_UNSUPPORTED;
+  if (B == 0 || L == 0) return SIMSD_OK;
+  if (!q || !k_cache || !v_cache || (max_pages > 0 && !page_table) || !seq_lens || !o || ld_table < 0)
+    return SIMSD_ERR_SHAPE;
+  if (!al16(q) || !al16(o)) return SIMSD_ERR_ALIGN;
+  int rc = cache_check(k_cache, v_cache, ld_page, ld_head, ld_tok);
+  if (rc != SIMSD_OK) return rc;
+  if (workspace == nullptr || workspace_bytes < simsd_paged_attention_workspace_size(B, L, Hq, Hk, head_dim))
+    return SIMSD_ERR_WORKSPACE;
+  PagedAttnArgs a;
+  a.q = q;
+  a.k_cache = k_cache;
+  a.v_cache = v_cache;
+  a.page_table = page_table;
+  a.seq_lens = seq_lens;
+  a.tail = tail_mask;
+  a.o = o;
+  a.lse = lse;
+  a.err = err_word;
+  a.ld_page = ld_page;
+  a.ld_head = ld_head;
+  a.ld_tok = ld_tok;
+  a.ld_table = ld_table;
+  a.ldm_b = ldm_b;
+  a.ldm_t = ldm_t;
+  a.B = B;
+  a.L = L;
+  a.Hq = Hq;
+  a.Hk = Hk;
+  a.G = Hq / Hk;
+  a.num_pages = num_pages;
+  a.page_size = page_size;
+  a.max_pages = max_pages;
+  a.dtype = dtype;
+  a.scale_log2 = scale * 1.4426950408889634f;
+  const long long rows = (long long)B * L * Hq;
+  return head_dim == 64 ? launch_on(paged_attention_kernel<64>, rows, PAT_THREADS, 0, stream, false, a)
+                        : launch_on(paged_attention_kernel<128>, rows, PAT_THREADS, 0, stream, false, a);
+}
+
+size_t simsd_speculative_verify_workspace_size(int B, int K, int V) {
+  (void)V;
+  if (B < 1 || K < 0) return 256;
+  return align256((size_t)B * (2 * K + 1) * 3 * sizeof(float));
+}
+
+int simsd_speculative_verify(const void* target_logits, int64_t ldt_b, int64_t ldt_r, const void* draft_logits,
+                             int64_t ldd_b, int64_t ldd_r, const int64_t* draft_tokens, int64_t ld_x,
+                             const float* uniform, int64_t ld_u, const float* noise, int64_t ld_n,
+                             const float* temperature, const int32_t* n_draft, int B, int K, int V, int dtype,
+                             int64_t* tokens, int64_t* accepted, float* logprobs, void* workspace,
+                             size_t workspace_bytes, int* err_word, void* stream) {
+  if (B < 0 || K < 0 || V < 1) return SIMSD_ERR_SHAPE;
+  if (dtype != SIMSD_BF16 && dtype != SIMSD_F16 && dtype != SIMSD_F32) return SIMSD_ERR_DTYPE;
+  if (B == 0) return SIMSD_OK;
+  if (!target_logits || !noise || !tokens || !accepted || !logprobs) return SIMSD_ERR_SHAPE;
+  if (K > 0 && (!draft_tokens || !uniform)) return SIMSD_ERR_SHAPE;
+  if (workspace == nullptr || workspace_bytes < simsd_speculative_verify_workspace_size(B, K, V))
+    return SIMSD_ERR_WORKSPACE;
+  SpecVerifyArgs a;
+  a.target = target_logits;
+  a.draft = draft_logits;
+  a.tokens = reinterpret_cast<const long long*>(draft_tokens);
+  a.uniform = uniform;
+  a.noise = noise;
+  a.temperature = temperature;
+  a.n_draft = n_draft;
+  a.out_tokens = reinterpret_cast<long long*>(tokens);
+  a.out_accepted = reinterpret_cast<long long*>(accepted);
+  a.out_logprobs = logprobs;
+  a.stat = reinterpret_cast<float*>(workspace);
+  a.err = err_word;
+  a.ldt_b = ldt_b;
+  a.ldt_r = ldt_r;
+  a.ldd_b = ldd_b;
+  a.ldd_r = ldd_r;
+  a.ld_x = ld_x;
+  a.ld_u = ld_u;
+  a.ld_n = ld_n;
+  a.B = B;
+  a.K = K;
+  a.V = V;
+  a.dtype = dtype;
+  const long long rows = (long long)B * (draft_logits ? 2 * K + 1 : K + 1);
+  int rc = launch_on(spec_stat_kernel, rows, SV_THREADS, 0, stream, false, a);
+  if (rc != SIMSD_OK) return rc;
+  return launch_on(spec_draw_kernel, B, SV_THREADS, 0, stream, true, a);
+}
+
+}  // extern "C"

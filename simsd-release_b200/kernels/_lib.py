@@ -79,6 +79,14 @@ SIGNATURES: dict[str, tuple] = {
     "simsd_qk_norm_rope": (_I, [_P, _L, _I, _I, _I, _I, _P, _P, _P, _P, _F, _P, _P, _P, _L, _I, _I, _P]),
     "simsd_verify_attention_workspace_size": (_S, [_I, _I, _I, _I]),
     "simsd_verify_attention": (_I, [_P, _P, _P, _L, _I, _I, _I, _I, _P, _L, _F, _P, _I, _P, _S, _P]),
+    "simsd_paged_append": (_I, [_P, _L, _I, _I, _I, _I, _I, _P, _P, _F, _P, _P, _L, _P, _P, _P, _P, _P, _I, _I, _L, _L,
+                                _L, _I, _P, _P]),
+    "simsd_paged_attention_workspace_size": (_S, [_I, _I, _I, _I, _I]),
+    "simsd_paged_attention": (_I, [_P, _P, _P, _I, _I, _L, _L, _L, _P, _L, _I, _P, _P, _L, _L, _I, _I, _I, _I, _I, _F,
+                                   _P, _P, _I, _P, _S, _P, _P]),
+    "simsd_speculative_verify_workspace_size": (_S, [_I, _I, _I]),
+    "simsd_speculative_verify": (_I, [_P, _L, _L, _P, _L, _L, _P, _L, _P, _L, _P, _L, _P, _P, _I, _I, _I, _I, _P, _P,
+                                      _P, _P, _S, _P, _P]),
     "simsd_allgather_wait": (_I, [_P, _I, _I, _P, _S, _P]),
     "simsd_thin_linear_allgather": (_I, [_P, _L, _L, _P, _L, _L, _P, _P, _P, _L, _I, _I, _I, _I, _I, _I, _I, _I,
                                          _I, _P, _S, _P]),
@@ -194,6 +202,12 @@ def workspace(dev: torch.device, nbytes: int) -> torch.Tensor:
         buf = torch.zeros(size, dtype=torch.uint8, device=dev)
         _WORKSPACES[dev] = buf
     return buf
+
+
+def error_ptr(dev: torch.device) -> int:
+    """Device address of the error word in `dev`'s workspace header (`device_error` reads it)."""
+    header = lib().simsd_workspace_header_bytes()
+    return workspace(dev, header).data_ptr() + header - 64
 
 
 def reset_workspace() -> None:

@@ -1,0 +1,90 @@
+"""Verification of drafted tokens by speculative sampling, on libsimsd_b200.
+
+`speculative_verify` keeps each sequence's drafted tokens while the target's
+distribution accepts them and draws the token after them, so that the emitted
+tokens are distributed as the target's own samples.  It is the batched form of
+the reference's per-block modified rejection sampling
+(speculative_decoding/mrs.py:14-108); temperature 0 is its greedy match
+(:111-145).
+
+Forward-only; CUDA tensors only (no CPU fallback).
+"""
+from __future__ import annotations
+
+import torch
+
+from . import _lib
+
+
+def speculative_verify(target_logits: torch.Tensor, draft_tokens: torch.Tensor, uniform: torch.Tensor,
+                       noise: torch.Tensor, draft_logits: torch.Tensor | None = None,
+                       temperature: torch.Tensor | None = None, n_draft: torch.Tensor | None = None):
+    """(tokens [B, K + 1] int64, accepted [B] int64, logprobs [B, K + 1] fp32).
+
+    target_logits [B, K + 1, V]: row i is the target's after i drafted tokens.
+    draft_tokens [B, K] int64.  draft_logits [B, K, V]: what they were drawn from
+    (same type as target_logits, same temperature), or None for drafts without
+    probabilities (greedy ones).  uniform [B, K] fp32 in [0, 1): accepts token i
+    where uniform * q_i < p_i.  noise [B, V] fp32, positive, exponentially
+    distributed: draws the token after the accepted ones from max(p - q, 0), or
+    from p after the last one.  temperature [B] fp32: 1 when None, 0 = greedy.
+    n_draft [B] int32: drafted tokens of each sequence (<= K; K when None); the
+    rows after them are not read.
+
+    tokens: the accepted drafts, then the drawn token, then -1.  logprobs: the
+    target's log probability of each, 0 after them.  Logits bf16, fp16 or fp32;
+    NaN counts as -inf, +inf as the largest finite number; ties go to the lowest
+    token.  A drafted token outside [0, V) is refused, the next one drawn from p,
+    and DEV_ERR_BAD_INDEX raised in `_lib.device_error()`.
+    """
+    if torch.is_grad_enabled() and (target_logits.requires_grad
+                                    or (draft_logits is not None and draft_logits.requires_grad)):
+        raise RuntimeError("speculative_verify is a forward-only inference kernel.")
+    code = _lib.dtype_code(target_logits.dtype)
+    if target_logits.ndim != 3 or target_logits.shape[1] < 1 or target_logits.shape[2] < 1:
+        raise ValueError(f"target_logits must be [B, K + 1, V], got {tuple(target_logits.shape)}")
+    B, R, V = target_logits.shape
+    K = R - 1
+    if draft_tokens.dtype != torch.int64:
+        raise TypeError("speculative_verify: draft_tokens are int64")
+    if uniform.dtype != torch.float32 or noise.dtype != torch.float32:
+        raise TypeError("speculative_verify: uniform and noise are fp32")
+    if draft_tokens.shape != (B, K) or uniform.shape != (B, K) or noise.shape != (B, V):
+        raise ValueError(f"draft_tokens and uniform must be [{B}, {K}] and noise [{B}, {V}], got "
+                         f"{tuple(draft_tokens.shape)} / {tuple(uniform.shape)} / {tuple(noise.shape)}")
+    if draft_logits is not None:
+        if draft_logits.dtype != target_logits.dtype:
+            raise TypeError(f"dtype mismatch: target {target_logits.dtype} draft {draft_logits.dtype}")
+        if draft_logits.shape != (B, K, V):
+            raise ValueError(f"draft_logits must be [{B}, {K}, {V}], got {tuple(draft_logits.shape)}")
+    if temperature is not None:
+        if temperature.dtype != torch.float32:
+            raise TypeError("speculative_verify: temperature is fp32")
+        if temperature.shape != (B,):
+            raise ValueError(f"temperature must be [{B}]")
+    if n_draft is not None:
+        if n_draft.dtype != torch.int32:
+            raise TypeError("speculative_verify: n_draft is int32")
+        if n_draft.shape != (B,):
+            raise ValueError(f"n_draft must be [{B}]")
+    dev = _lib.require_cuda(target_logits, draft_tokens, uniform, noise, draft_logits, temperature, n_draft)
+    unit = lambda t: t if t is None or t.stride(-1) == 1 else t.contiguous()  # noqa: E731
+    target_logits, draft_logits, draft_tokens, uniform, noise, temperature, n_draft = map(
+        unit, (target_logits, draft_logits, draft_tokens, uniform, noise, temperature, n_draft))
+    tokens = torch.empty((B, R), dtype=torch.int64, device=dev)
+    accepted = torch.empty((B,), dtype=torch.int64, device=dev)
+    logprobs = torch.empty((B, R), dtype=torch.float32, device=dev)
+    L = _lib.lib()
+    drafted = draft_logits is not None and K > 0
+    with _lib.device_guard(dev):
+        ws = torch.empty(L.simsd_speculative_verify_workspace_size(B, K, V), dtype=torch.uint8, device=dev)
+        rc = L.simsd_speculative_verify(
+            target_logits.data_ptr(), target_logits.stride(0), target_logits.stride(1),
+            draft_logits.data_ptr() if drafted else None, draft_logits.stride(0) if drafted else 0,
+            draft_logits.stride(1) if drafted else 0, draft_tokens.data_ptr(), draft_tokens.stride(0),
+            uniform.data_ptr(), uniform.stride(0), noise.data_ptr(), noise.stride(0),
+            temperature.data_ptr() if temperature is not None else None,
+            n_draft.data_ptr() if n_draft is not None else None, B, K, V, code, tokens.data_ptr(), accepted.data_ptr(),
+            logprobs.data_ptr(), ws.data_ptr(), ws.numel(), _lib.error_ptr(dev), _lib.stream_ptr(dev))
+    _lib.check(rc, "speculative_verify")
+    return tokens, accepted, logprobs
