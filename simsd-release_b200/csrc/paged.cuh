@@ -1,5 +1,5 @@
-// A paged key-value cache: the append that writes tokens into it and the
-// attention that reads it.
+// The append of a paged key-value cache (the attention that reads it is in
+// paged_attn.cuh).
 //
 // The cache is [pages, Hk, page size, D] with any page, head and token strides
 // (unit D stride), so a head-major and a token-major cache are the same code.
@@ -136,93 +136,6 @@ __global__ void __launch_bounds__(PA_THREADS) paged_append_kernel(const PagedApp
       *reinterpret_cast<uint4*>(dst) = is_k ? paged_pack8(o, p.dtype) : raw;
     }
   }
-}
-
-// ---------------------------------------------------------------- attention
-//   o[b, t, h, :] = sum_j p_j v_j / sum_j p_j,  p_j = exp(scale q . k_j - max),
-// over the visible keys j < n = min(seq_lens[b], max_pages page_size) of KV head
-// g = h / (Hq / Hk).  The newest L keys belong to the L query tokens: with jt =
-// j - (n - L), a key with jt < 0 is visible to all of them, the others where
-// jt <= t, or where tail_mask[b, t, jt] is set.  No visible key: o = 0, lse = -inf.
-struct PagedAttnArgs {
-  const void* q;            // [B, L, Hq, D]
-  const void* k_cache;
-  const void* v_cache;
-  const int* page_table;    // [B, ld_table]
-  const int* seq_lens;      // [B]
-  const uint8_t* tail;      // [B, L, L] bytes or nullptr
-  void* o;                  // [B, L, Hq, D]
-  float* lse;               // [B, L, Hq] or nullptr
-  int* err;
-  long long ld_page, ld_head, ld_tok, ld_table, ldm_b, ldm_t;
-  int B, L, Hq, Hk, G, num_pages, page_size, max_pages, dtype;
-  float scale_log2;         // scale * log2(e)
-};
-
-constexpr int PAT_THREADS = 128;
-
-__device__ __forceinline__ int paged_len(const PagedAttnArgs& p, int b) {
-  int n = p.seq_lens[b];
-  const long long cap = (long long)p.max_pages * p.page_size;
-  if (n > cap) {
-    if (threadIdx.x == 0 && p.err) atomicOr(p.err, SIMSD_DEV_ERR_BAD_INDEX);
-    n = (int)cap;
-  }
-  return n < 0 ? 0 : n;
-}
-
-// One CTA per row; warp w takes keys w, w + 4, ..., lane l elements l, l + 32, ...
-template <int D>
-__global__ void __launch_bounds__(PAT_THREADS) paged_attention_kernel(const PagedAttnArgs p) {
-  griddep_launch_dependents();
-  griddep_wait();
-  constexpr int E = D / 32, W = PAT_THREADS / 32;
-  __shared__ float sm[W], sl[W], so[W][D];
-  const long long row = blockIdx.x;
-  const int h = (int)(row % p.Hq), t = (int)(row / p.Hq % p.L), b = (int)(row / p.Hq / p.L);
-  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-  const int n = paged_len(p, b);
-  const long long head = (long long)(h / p.G) * p.ld_head;
-  float q[E], o[E], m = -INFINITY, l = 0.0f;
-#pragma unroll
-  for (int e = 0; e < E; ++e) q[e] = load_f(p.q, row * D + lane + 32 * e, p.dtype), o[e] = 0.0f;
-  for (int j = warp; j < n; j += W) {
-    const int jt = j - (n - p.L);
-    if (jt >= 0 && !(p.tail ? p.tail[b * p.ldm_b + t * p.ldm_t + jt] != 0 : jt <= t)) continue;
-    const int pg = p.page_table[b * p.ld_table + j / p.page_size];
-    if (pg < 0 || pg >= p.num_pages) {
-      if (lane == 0 && p.err) atomicOr(p.err, SIMSD_DEV_ERR_BAD_INDEX);
-      continue;
-    }
-    const long long at = pg * p.ld_page + head + (j % p.page_size) * p.ld_tok + lane;
-    float s = 0.0f;
-#pragma unroll
-    for (int e = 0; e < E; ++e) s = fmaf(q[e], load_f(p.k_cache, at + 32 * e, p.dtype), s);
-#pragma unroll
-    for (int d = 16; d > 0; d >>= 1) s += __shfl_xor_sync(0xffffffffu, s, d);
-    s *= p.scale_log2;
-    const float mn = fmaxf(m, s);
-    if (mn == -INFINITY) continue;
-    const float a = exp2f(m - mn), w = exp2f(s - mn);
-    m = mn;
-    l = fmaf(l, a, w);
-#pragma unroll
-    for (int e = 0; e < E; ++e) o[e] = fmaf(o[e], a, w * load_f(p.v_cache, at + 32 * e, p.dtype));
-  }
-  if (lane == 0) sm[warp] = m, sl[warp] = l;
-#pragma unroll
-  for (int e = 0; e < E; ++e) so[warp][lane + 32 * e] = o[e];
-  __syncthreads();
-  float mt = -INFINITY, lt = 0.0f;
-  for (int w = 0; w < W; ++w) mt = fmaxf(mt, sm[w]);
-  const float mu = mt == -INFINITY ? 0.0f : mt;
-  for (int w = 0; w < W; ++w) lt += sl[w] * exp2f(sm[w] - mu);
-  for (int d = threadIdx.x; d < D; d += PAT_THREADS) {
-    float v = 0.0f;
-    for (int w = 0; w < W; ++w) v += so[w][d] * exp2f(sm[w] - mu);
-    store_f(p.o, row * D + d, lt == 0.0f ? 0.0f : v / lt, p.dtype);
-  }
-  if (p.lse && threadIdx.x == 0) p.lse[row] = lt == 0.0f ? -INFINITY : 0.69314718055994531f * mt + logf(lt);
 }
 
 }  // namespace simsd

@@ -2,15 +2,20 @@
 // include/simsd_b200.h): the paged key-value cache and draft verification.
 #include <cuda_runtime.h>
 
-#include <algorithm>
+#include <mutex>
+#include <utility>
 
 #include "paged.cuh"
+#include "paged_attn.cuh"
 #include "simsd_b200.h"
 #include "spec_verify.cuh"
 
 using namespace simsd;
 
 namespace {
+
+constexpr int kMaxDev = 64;
+std::mutex g_attr_mu;
 
 inline size_t align256(size_t v) { return (v + 255) & ~size_t(255); }
 inline bool al16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15) == 0; }
@@ -41,6 +46,51 @@ int launch_on(void (*kern)(KArgs...), long long grid, int block, size_t smem, vo
 int cache_check(const void* k, const void* v, int64_t ld_page, int64_t ld_head, int64_t ld_tok) {
   if (!al16(k) || !al16(v) || (ld_page & 7) || (ld_head & 7) || (ld_tok & 7)) return SIMSD_ERR_ALIGN;
   return SIMSD_OK;
+}
+
+// What paged attention does with G L rows per KV head: 8-row tiles per CTA (all
+// rows in one pass over the keys up to 32, more in row tiles of 32), the grid, and
+// the workspace: two parts per CTA (the end of a sequence it started inside, the
+// start of one it leaves unfinished).
+struct PagedPlan {
+  int nt, grid;
+  size_t ml_at, desc_at, bytes;
+};
+PagedPlan paged_plan(int L, int G, int D) {
+  PagedPlan p;
+  const long long rows = (long long)L * G;
+  p.nt = rows <= 8 ? 1 : rows <= 16 ? 2 : 4;
+  const int sms = simsd_device_sm_count();
+  p.grid = PAT_CTAS_PER_SM * (sms > 0 ? sms : 148);
+  p.ml_at = align256((size_t)2 * p.grid * D * p.nt * 8 * sizeof(float));
+  p.desc_at = p.ml_at + align256((size_t)2 * p.grid * p.nt * 8 * 2 * sizeof(float));
+  p.bytes = p.desc_at + align256((size_t)p.grid * sizeof(int4));
+  return p;
+}
+
+// Raise a kernel's shared-memory limit once per device.
+template <typename F>
+int allow_smem(F* kern, int bytes, bool* done) {
+  int dev = -1;
+  if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= kMaxDev) return SIMSD_ERR_DEVICE;
+  std::lock_guard<std::mutex> lk(g_attr_mu);
+  if (done[dev]) return SIMSD_OK;
+  if (cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes) != cudaSuccess)
+    return SIMSD_ERR_LAUNCH;
+  done[dev] = true;
+  return SIMSD_OK;
+}
+
+template <int D, int NT, bool BF>
+int attend(const PagedAttnArgs& a, const PagedPlan& pl, void* stream) {
+  static bool done[kMaxDev];
+  constexpr int smem = PatSmem<D, NT>::BYTES;
+  int rc = allow_smem(paged_attention_kernel<D, NT, BF>, smem, done);
+  if (rc != SIMSD_OK) return rc;
+  rc = launch_on(paged_attention_kernel<D, NT, BF>, pl.grid, PAT_THREADS, smem, stream, false, a);
+  if (rc != SIMSD_OK) return rc;
+  return launch_on(paged_combine_kernel<D, NT, BF>, pl.grid, PAC_THREADS, (size_t)pl.grid * NT * 8 * sizeof(float), stream,
+                   true, a);
 }
 
 }  // namespace
@@ -92,8 +142,8 @@ int simsd_paged_append(const void* qkv, int64_t ldqkv, int T, int Hq, int Hk, in
 }
 
 size_t simsd_paged_attention_workspace_size(int B, int L, int Hq, int Hk, int head_dim) {
-  (void)B, (void)L, (void)Hq, (void)Hk, (void)head_dim;
-  return 256;
+  if (B < 1 || L < 1 || Hq < 1 || Hk < 1 || Hq % Hk || head_dim < 1) return 256;
+  return paged_plan(L, Hq / Hk, head_dim).bytes;
 }
 
 int simsd_paged_attention(const void* q, const void* k_cache, const void* v_cache, int num_pages, int page_size,
@@ -106,6 +156,7 @@ int simsd_paged_attention(const void* q, const void* k_cache, const void* v_cach
   if (dtype != SIMSD_BF16 && dtype != SIMSD_F16) return SIMSD_ERR_DTYPE;
   if (head_dim != 64 && head_dim != 128) return SIMSD_ERR_UNSUPPORTED;
   if (B == 0 || L == 0) return SIMSD_OK;
+  if ((int64_t)max_pages * page_size > 0x7fff0000LL) return SIMSD_ERR_UNSUPPORTED;
   if (!q || !k_cache || !v_cache || (max_pages > 0 && !page_table) || !seq_lens || !o || ld_table < 0)
     return SIMSD_ERR_SHAPE;
   if (!al16(q) || !al16(o)) return SIMSD_ERR_ALIGN;
@@ -137,11 +188,23 @@ int simsd_paged_attention(const void* q, const void* k_cache, const void* v_cach
   a.num_pages = num_pages;
   a.page_size = page_size;
   a.max_pages = max_pages;
-  a.dtype = dtype;
   a.scale_log2 = scale * 1.4426950408889634f;
-  const long long rows = (long long)B * L * Hq;
-  return head_dim == 64 ? launch_on(paged_attention_kernel<64>, rows, PAT_THREADS, 0, stream, false, a)
-                        : launch_on(paged_attention_kernel<128>, rows, PAT_THREADS, 0, stream, false, a);
+  const PagedPlan pl = paged_plan(L, a.G, head_dim);
+  a.rows = a.G * L;
+  a.row_tiles = (a.rows + pl.nt * 8 - 1) / (pl.nt * 8);
+  uint8_t* ws = reinterpret_cast<uint8_t*>(workspace);
+  a.part_o = reinterpret_cast<float4*>(ws);
+  a.part_ml = reinterpret_cast<float*>(ws + pl.ml_at);
+  a.desc = reinterpret_cast<int4*>(ws + pl.desc_at);
+  const bool bf = dtype == SIMSD_BF16;
+  switch (pl.nt * 1000 + head_dim) {
+    case 1064: return bf ? attend<64, 1, true>(a, pl, stream) : attend<64, 1, false>(a, pl, stream);
+    case 1128: return bf ? attend<128, 1, true>(a, pl, stream) : attend<128, 1, false>(a, pl, stream);
+    case 2064: return bf ? attend<64, 2, true>(a, pl, stream) : attend<64, 2, false>(a, pl, stream);
+    case 2128: return bf ? attend<128, 2, true>(a, pl, stream) : attend<128, 2, false>(a, pl, stream);
+    case 4064: return bf ? attend<64, 4, true>(a, pl, stream) : attend<64, 4, false>(a, pl, stream);
+    default: return bf ? attend<128, 4, true>(a, pl, stream) : attend<128, 4, false>(a, pl, stream);
+  }
 }
 
 size_t simsd_speculative_verify_workspace_size(int B, int K, int V) {
