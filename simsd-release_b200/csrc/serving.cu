@@ -81,6 +81,29 @@ int allow_smem(F* kern, int bytes, bool* done) {
   return SIMSD_OK;
 }
 
+struct SpecPlan {
+  int parts, chunks;
+  size_t cand_at, done_at, bytes;
+};
+SpecPlan spec_plan(int B, int K, int V) {
+  SpecPlan p;
+  p.parts = (V + SV_PART - 1) / SV_PART;
+  p.chunks = (V + SV_CHUNK - 1) / SV_CHUNK;
+  p.cand_at = align256((size_t)B * (2 * K + 1) * p.parts * sizeof(float2));
+  p.done_at = p.cand_at + align256((size_t)B * p.chunks * sizeof(float4));
+  p.bytes = p.done_at + align256((size_t)B * sizeof(int));
+  return p;
+}
+
+template <int DT>
+int verify_drafts(const SpecVerifyArgs& a, void* stream) {
+  const long long rows = (long long)a.B * (a.draft ? 2 * a.K + 1 : a.K + 1);
+  int rc = launch_on(spec_stat_kernel<DT>, rows * ((a.parts + SV_WARPS - 1) / SV_WARPS), SV_THREADS, 0, stream, false, a);
+  if (rc != SIMSD_OK) return rc;
+  return launch_on(spec_draw_kernel<DT>, (long long)a.B * a.chunks, SV_THREADS, (size_t)(2 * a.K + 1) * 3 * sizeof(float),
+                   stream, true, a);
+}
+
 template <int D, int NT, bool BF>
 int attend(const PagedAttnArgs& a, const PagedPlan& pl, void* stream) {
   static bool done[kMaxDev];
@@ -208,9 +231,8 @@ int simsd_paged_attention(const void* q, const void* k_cache, const void* v_cach
 }
 
 size_t simsd_speculative_verify_workspace_size(int B, int K, int V) {
-  (void)V;
-  if (B < 1 || K < 0) return 256;
-  return align256((size_t)B * (2 * K + 1) * 3 * sizeof(float));
+  if (B < 1 || K < 0 || V < 1) return 256;
+  return spec_plan(B, K, V).bytes;
 }
 
 int simsd_speculative_verify(const void* target_logits, int64_t ldt_b, int64_t ldt_r, const void* draft_logits,
@@ -220,6 +242,7 @@ int simsd_speculative_verify(const void* target_logits, int64_t ldt_b, int64_t l
                              int64_t* tokens, int64_t* accepted, float* logprobs, void* workspace,
                              size_t workspace_bytes, int* err_word, void* stream) {
   if (B < 0 || K < 0 || V < 1) return SIMSD_ERR_SHAPE;
+  if (K > 1024 || V > 0x7fff0000) return SIMSD_ERR_UNSUPPORTED;
   if (dtype != SIMSD_BF16 && dtype != SIMSD_F16 && dtype != SIMSD_F32) return SIMSD_ERR_DTYPE;
   if (B == 0) return SIMSD_OK;
   if (!target_logits || !noise || !tokens || !accepted || !logprobs) return SIMSD_ERR_SHAPE;
@@ -237,7 +260,13 @@ int simsd_speculative_verify(const void* target_logits, int64_t ldt_b, int64_t l
   a.out_tokens = reinterpret_cast<long long*>(tokens);
   a.out_accepted = reinterpret_cast<long long*>(accepted);
   a.out_logprobs = logprobs;
-  a.stat = reinterpret_cast<float*>(workspace);
+  const SpecPlan pl = spec_plan(B, K, V);
+  uint8_t* ws = reinterpret_cast<uint8_t*>(workspace);
+  a.part = reinterpret_cast<float2*>(ws);
+  a.cand = reinterpret_cast<float4*>(ws + pl.cand_at);
+  a.done = reinterpret_cast<int*>(ws + pl.done_at);
+  a.parts = pl.parts;
+  a.chunks = pl.chunks;
   a.err = err_word;
   a.ldt_b = ldt_b;
   a.ldt_r = ldt_r;
@@ -250,10 +279,9 @@ int simsd_speculative_verify(const void* target_logits, int64_t ldt_b, int64_t l
   a.K = K;
   a.V = V;
   a.dtype = dtype;
-  const long long rows = (long long)B * (draft_logits ? 2 * K + 1 : K + 1);
-  int rc = launch_on(spec_stat_kernel, rows, SV_THREADS, 0, stream, false, a);
-  if (rc != SIMSD_OK) return rc;
-  return launch_on(spec_draw_kernel, B, SV_THREADS, 0, stream, true, a);
+  if (dtype == SIMSD_BF16) return verify_drafts<0>(a, stream);
+  if (dtype == SIMSD_F16) return verify_drafts<1>(a, stream);
+  return verify_drafts<2>(a, stream);
 }
 
 }  // extern "C"
