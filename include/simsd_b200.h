@@ -494,9 +494,12 @@ int simsd_moe_ep_return(const void* y, int64_t ldy, const int32_t* recv_expert, 
  * 16-byte aligned bases; slot s is token s % page_size of page s / page_size.
  * head_dim 64 or 128, bf16 or fp16.  `err_word` (device int or NULL) receives
  * SIMSD_DEV_ERR_BAD_INDEX for an index outside its tensor; nothing is read or
- * written for it.  The workspaces of these calls are plain scratch: no header, no
- * initialisation, not read after the call's kernels, so each call may bring its
- * own. */
+ * written for it.  The workspaces of these calls have no header; they are scratch
+ * that is not read after the call's kernels, except that simsd_paged_attention
+ * keeps counters in the first SIMSD_PAGED_COUNTER_BYTES of its own: zero before the
+ * first call with it, zero again after every call.  Calls that share a workspace
+ * must be ordered on one stream. */
+#define SIMSD_PAGED_COUNTER_BYTES 4096
 
 /*
  * Append T tokens: per token t with slot s = slots[t] >= 0,
@@ -527,7 +530,8 @@ int simsd_paged_append(const void* qkv, int64_t ldqkv, int T, int Hq, int Hk, in
  * are visible to every query, the others where jt <= t, or, with tail_mask, where
  * tail_mask[b * ldm_b + t * ldm_t + jt] != 0.  A query without a visible key: o =
  * 0, lse = -inf.  q, o [B, L, Hq, head_dim] contiguous, lse [B, L, Hq] or NULL.
- * The lengths are read on the device only.
+ * The lengths are read on the device only.  B Hk ceil(G L / 32) (max_pages
+ * page_size / 64 + 1) < 2^31 (more: SIMSD_ERR_UNSUPPORTED).
  */
 size_t simsd_paged_attention_workspace_size(int B, int L, int Hq, int Hk, int head_dim);
 int simsd_paged_attention(const void* q, const void* k_cache, const void* v_cache, int num_pages, int page_size,

@@ -35,7 +35,7 @@ struct PagedAppendArgs {
   float eps;
 };
 
-constexpr int PA_THREADS = 256;
+constexpr int PA_THREADS = 256, PA_UNROLL = 4;
 
 __device__ __forceinline__ void paged_unpack8(uint4 u, int dtype, float (&v)[8]) {
   const uint32_t w[4] = {u.x, u.y, u.z, u.w};
@@ -63,17 +63,35 @@ __device__ __forceinline__ uint4 paged_pack8(const float (&f)[8], int dtype) {
 // One CTA per token.  A head's D elements are D / 8 neighbouring threads of 8
 // elements (16-byte loads and stores); PA_THREADS is a multiple of D / 8, so a
 // thread keeps its place in the head over its heads and its rotary row stays in
-// registers.  The pair of element i lies R / 16 threads away.
+// registers.  The pair of element i lies R / 16 threads away.  HBM bounds it: the
+// row's loads (PA_UNROLL vectors a thread at a time) are issued before the slot,
+// the position and the rotary row are known, so that one round of latency covers
+// them all.
 template <int D>
 __global__ void __launch_bounds__(PA_THREADS) paged_append_kernel(const PagedAppendArgs p) {
   griddep_launch_dependents();
   griddep_wait();
-  constexpr int LANES = D / 8;
+  constexpr int LANES = D / 8, HEADS = PA_THREADS / LANES;    // threads of a head, heads at a time
   const long long t = blockIdx.x;
-  const int tid = threadIdx.x;
-  const int i8 = tid % LANES;
+  const int tid = threadIdx.x, lane = tid & 31;
+  const int i8 = tid % LANES, h_at = tid / LANES;
+  const int H = p.Hq + 2 * p.Hk;
+  const uint16_t* row = reinterpret_cast<const uint16_t*>(p.qkv) + t * p.ldqkv + i8 * 8;
+  uint4 raw[PA_UNROLL];
+  auto fetch = [&](int h0) {
+#pragma unroll
+    for (int u = 0; u < PA_UNROLL; ++u) {
+      const int h = h0 + u * HEADS + h_at;
+      raw[u] = h < H ? __ldg(reinterpret_cast<const uint4*>(row + (long long)h * D)) : make_uint4(0, 0, 0, 0);
+    }
+  };
+  fetch(0);
   const long long slot = p.slots[t];
-  long long pos = p.positions[t];
+  const long long pos = p.positions[t];
+  auto weight = [&](const void* w) {
+    return w ? __ldg(reinterpret_cast<const uint4*>(reinterpret_cast<const uint16_t*>(w) + i8 * 8)) : make_uint4(0, 0, 0, 0);
+  };
+  const uint4 qw = weight(p.qw), kw = weight(p.kw);
   const bool bad = slot >= p.n_slots || (slot >= 0 && (pos < 0 || pos >= p.n_pos));
   if (bad && tid == 0 && p.err) atomicOr(p.err, SIMSD_DEV_ERR_BAD_INDEX);
   const bool live = slot >= 0 && !bad;
@@ -94,46 +112,47 @@ __global__ void __launch_bounds__(PA_THREADS) paged_append_kernel(const PagedApp
       for (int e = 0; e < 8; ++e) s[e] = -s[e];
     }
   }
-  const int lane = tid & 31;
   const int partner = !rot ? lane : low ? lane + rl : lane - rl;
-  const int H = p.Hq + 2 * p.Hk;
   const long long page = live ? slot / p.page_size : 0;
   const long long base = live ? page * p.ld_page + (slot - page * p.page_size) * p.ld_tok + i8 * 8 : 0;
-  const uint16_t* row = reinterpret_cast<const uint16_t*>(p.qkv) + t * p.ldqkv + i8 * 8;
   uint16_t* q = reinterpret_cast<uint16_t*>(p.q_out) + t * p.Hq * D + i8 * 8;
-  for (int h0 = 0; h0 < H; h0 += PA_THREADS / LANES) {
-    const int h = h0 + tid / LANES;
-    const bool in = h < H && live;
-    const uint4 raw = in ? *reinterpret_cast<const uint4*>(row + (long long)h * D) : make_uint4(0, 0, 0, 0);
-    float x[8];
-    paged_unpack8(raw, p.dtype, x);
-    const void* w = h < p.Hq ? p.qw : p.kw;
-    float ss = 0.0f;
+  for (int h0 = 0; h0 < H; h0 += HEADS * PA_UNROLL) {
+    if (h0 > 0) fetch(h0);
 #pragma unroll
-    for (int e = 0; e < 8; ++e) ss = fmaf(x[e], x[e], ss);
+    for (int u = 0; u < PA_UNROLL; ++u) {
+      const int h = h0 + u * HEADS + h_at;
+      if (h0 + u * HEADS >= H) break;              // the whole CTA
+      float x[8];
+      paged_unpack8(raw[u], p.dtype, x);
+      const bool is_q = h < p.Hq;
+      if (is_q ? p.qw != nullptr : p.kw != nullptr) {
+        float ss = 0.0f;
 #pragma unroll
-    for (int m = LANES / 2; m > 0; m >>= 1) ss += __shfl_xor_sync(0xffffffffu, ss, m);
-    if (w != nullptr) {
-      const float inv = rsqrtf(ss * (1.0f / D) + p.eps);
-      float wf[8];
-      paged_unpack8(*reinterpret_cast<const uint4*>(reinterpret_cast<const uint16_t*>(w) + i8 * 8), p.dtype, wf);
+        for (int e = 0; e < 8; ++e) ss = fmaf(x[e], x[e], ss);
+        // the head's threads all take this branch; their lanes are the mask
+        const uint32_t mask = (LANES == 32 ? 0xffffffffu : ((1u << LANES) - 1u)) << (lane & ~(LANES - 1));
 #pragma unroll
-      for (int e = 0; e < 8; ++e) x[e] = x[e] * inv * wf[e];
-    }
-    float o[8];
+        for (int m = LANES / 2; m > 0; m >>= 1) ss += __shfl_xor_sync(mask, ss, m);
+        const float inv = rsqrtf(ss * (1.0f / D) + p.eps);
+        float wf[8];
+        paged_unpack8(is_q ? qw : kw, p.dtype, wf);
 #pragma unroll
-    for (int e = 0; e < 8; ++e) {
-      const float other = __shfl_sync(0xffffffffu, x[e], partner);
-      o[e] = rot ? fmaf(other, s[e], x[e] * c[e]) : x[e];
-    }
-    if (h >= H) continue;
-    if (h < p.Hq) {
-      *reinterpret_cast<uint4*>(q + (long long)h * D) = live ? paged_pack8(o, p.dtype) : make_uint4(0, 0, 0, 0);
-    } else if (live) {
-      const bool is_k = h < p.Hq + p.Hk;
-      uint16_t* dst = reinterpret_cast<uint16_t*>(is_k ? p.k_cache : p.v_cache) + base +
-                      (long long)(h - p.Hq - (is_k ? 0 : p.Hk)) * p.ld_head;
-      *reinterpret_cast<uint4*>(dst) = is_k ? paged_pack8(o, p.dtype) : raw;
+        for (int e = 0; e < 8; ++e) x[e] = x[e] * inv * wf[e];
+      }
+      float o[8];
+#pragma unroll
+      for (int e = 0; e < 8; ++e) {
+        const float other = __shfl_sync(0xffffffffu, x[e], partner);
+        o[e] = rot ? fmaf(other, s[e], x[e] * c[e]) : x[e];
+      }
+      if (is_q) {
+        *reinterpret_cast<uint4*>(q + (long long)h * D) = live ? paged_pack8(o, p.dtype) : make_uint4(0, 0, 0, 0);
+      } else if (live && h < H) {
+        const bool is_k = h < p.Hq + p.Hk;
+        uint16_t* dst = reinterpret_cast<uint16_t*>(is_k ? p.k_cache : p.v_cache) + base +
+                        (long long)(h - p.Hq - (is_k ? 0 : p.Hk)) * p.ld_head;
+        *reinterpret_cast<uint4*>(dst) = is_k ? paged_pack8(o, p.dtype) : raw[u];
+      }
     }
   }
 }

@@ -15,17 +15,19 @@
 // CTAs per SM, from the lengths on the device (no host knowledge of them, so a
 // graph replays as sequences grow).  A range may hold many short sequences or a
 // slice of a long one; a sequence cut between CTAs leaves each part's (O, max,
-// sum) in the workspace, and paged_combine_kernel joins the parts in key order.
+// sum) in the workspace, and the last of its CTAs to finish (a counter per first
+// CTA, zero again afterwards) joins the parts, always in key order.
 //
 // In a CTA each of the 4 warps takes 16 keys of every unit through a ring of its
 // own (cp.async, no barrier between warps until the sequence ends), loading ahead
-// across sequence ends.  Products with the roles swapped, so that few rows waste
-// little: S^T = K Q^T (m16n8k16: 16 keys x 8 rows), P^T turned into the second
-// product's operand with movmatrix, O^T = V^T P^T (16 dims x 8 rows).  Softmax in
-// fp32 with exp2 of log2-scaled scores; the running maximum moves (and O is
-// rescaled) only when a score exceeds it.  P is rounded to the 16-bit type for the
-// second product: the weights are <= 1 and their sum, kept in fp32, is of the
-// unrounded ones, so the rounding errs by at most half a step per weight.
+// across sequence ends; the next sequence's queries are fetched a sequence ahead.
+// Products with the roles swapped, so that few rows waste little: S^T = K Q^T
+// (m16n8k16: 16 keys x 8 rows), P^T turned into the second product's operand with
+// movmatrix, O^T = V^T P^T (16 dims x 8 rows).  Softmax in fp32 with exp2 of
+// log2-scaled scores; the running maximum moves (and O is rescaled) only when a
+// score exceeds it.  P is rounded to the 16-bit type for the second product: the
+// weights are <= 1 and their sum, kept in fp32, is of the unrounded ones, so the
+// rounding errs by at most half a step per weight.
 //
 // Masked keys: keys past n are zero-filled in shared memory, whatever stale memory
 // holds.  A tail key that some rows of the unit see and others do not takes part
@@ -35,6 +37,13 @@
 #include "sm100.cuh"
 
 namespace simsd {
+
+// x / d for 0 <= x < 2^31: x * magic >> shift, magic the reciprocal rounded up
+struct PagedDiv {
+  uint32_t magic;
+  int shift;
+  __device__ __forceinline__ int operator()(int x) const { return (int)((uint64_t)(uint32_t)x * magic >> shift); }
+};
 
 struct PagedAttnArgs {
   const void* q;            // [B, L, Hq, D]
@@ -46,17 +55,18 @@ struct PagedAttnArgs {
   void* o;                  // [B, L, Hq, D]
   float* lse;               // [B, L, Hq] or nullptr
   int* err;
+  int* arrived;             // [grid]: parts written of the cut sequence that starts in that CTA; zero between calls
   float4* part_o;           // [2 grid][D / 16][NT][32] fragments
-  float* part_ml;           // [2 grid][NR][2] (max in log2 units, sum)
-  int4* desc;               // [grid]: the cut sequence that starts in this CTA (b, head and row tile, last CTA or -1)
+  float2* part_ml;          // [2 grid][NR] (max in log2 units, sum)
   long long ld_page, ld_head, ld_tok, ld_table, ldm_b, ldm_t;
   int B, L, Hq, Hk, G, num_pages, page_size, max_pages, rows, row_tiles;
-  float scale_log2;         // scale * log2(e)
+  PagedDiv page_div, g_div; // by page_size, by G
+  uint32_t q_sign;          // 0x80008000 flips the queries' signs (a negative scale)
+  float scale_log2;         // |scale| log2(e), positive
 };
 
 constexpr int PAT_WARPS = 4, PAT_THREADS = PAT_WARPS * 32, PAT_TK = 16 * PAT_WARPS;
 constexpr int PAT_CTAS_PER_SM = 2;
-constexpr int PAC_THREADS = 256;
 
 template <int D, int NT>
 struct PatSmem {
@@ -66,7 +76,7 @@ struct PatSmem {
   static constexpr int OBUF = PAT_WARPS * (D / 16) * 32 * 16;  // one 8-row tile of every warp's O
   static constexpr int Q = NT > 2 ? NT * 8 * D * 2 : 0;
   static constexpr int ML = 2 * PAT_WARPS * NT * 8 * 4;
-  static constexpr int BYTES = RING + OBUF + Q + ML + 64;
+  static constexpr int BYTES = RING + OBUF + Q + ML;
 };
 
 __device__ __forceinline__ void pat_ldsm(uint32_t addr, uint32_t (&r)[4]) {
@@ -99,7 +109,17 @@ __device__ __forceinline__ void pat_mma(float (&d)[4], const uint32_t (&a)[4], u
 }
 template <bool BF>
 __device__ __forceinline__ uint32_t pat_pack(float lo, float hi) {
-  return (uint32_t)f32_to_16bit(lo, BF ? 0 : 1) | ((uint32_t)f32_to_16bit(hi, BF ? 0 : 1) << 16);
+  uint32_t r;
+  if (BF)
+    asm("cvt.rn.bf16x2.f32 %0, %1, %2;" : "=r"(r) : "f"(hi), "f"(lo));
+  else
+    asm("cvt.rn.f16x2.f32 %0, %1, %2;" : "=r"(r) : "f"(hi), "f"(lo));
+  return r;
+}
+__device__ __forceinline__ float pat_exp2(float x) {
+  float y;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
 }
 // 16 bytes into shared memory, zeros where !ok (nothing is read then)
 __device__ __forceinline__ void pat_cp16(uint32_t dst, const void* src, bool ok) {
@@ -120,119 +140,236 @@ __device__ __forceinline__ int paged_len(const PagedAttnArgs& p, int b) {
 // units of one (head, row tile) of a sequence; an empty one has a unit, which writes its rows
 __device__ __forceinline__ int paged_units(int n) { return n <= PAT_TK ? 1 : (n + PAT_TK - 1) / PAT_TK; }
 
-// Position in the unit order: sequence b (length n, nu units per head and row
-// tile), hr = KV head * row_tiles + row tile, unit of it.
+// Position in the unit order: sequence b (length n, nu units per KV head and row
+// tile), KV head g, row tile rt, unit of it.
 struct PagedPos {
-  int b, hr, unit, n, nu;
+  int b, g, rt, unit, n, nu;
   __device__ __forceinline__ void next(const PagedAttnArgs& p) {
     if (++unit < nu) return;
     unit = 0;
-    if (++hr < p.Hk * p.row_tiles) return;
-    hr = 0;
-    if (++b >= p.B) return;
+    if (!next_rows(p, b, g, rt) || b >= p.B) return;
     n = paged_len(p, b);
     nu = paged_units(n);
   }
+  // the row tile, head or sequence after (b, g, rt); true for another sequence
+  __device__ static __forceinline__ bool next_rows(const PagedAttnArgs& p, int& b, int& g, int& rt) {
+    if (++rt < p.row_tiles) return false;
+    rt = 0;
+    if (++g < p.Hk) return false;
+    g = 0;
+    ++b;
+    return true;
+  }
 };
 
-// Whether row r of the sequence's rows (t = r / G) sees key j < n
-__device__ __forceinline__ bool paged_visible(const PagedAttnArgs& p, int b, int n, int j, int r) {
-  if (j >= n) return false;
-  const int jt = j - (n - p.L);
-  if (jt < 0 || r >= p.rows) return true;
-  const int t = r / p.G;
-  return p.tail ? p.tail[b * p.ldm_b + t * p.ldm_t + jt] != 0 : jt <= t;
-}
-
-// The rows of one 8-row tile from a fragment of O^T (dims d, d + 8 of rows r, r + 1)
-template <bool BF, int D>
-__device__ __forceinline__ void paged_store(const PagedAttnArgs& p, int b, int hr, int nt8, int mt, int lane, float4 v) {
-  const int g = hr / p.row_tiles;
-  const int r = nt8 + 2 * (lane & 3), d = mt * 16 + (lane >> 2);
-  uint16_t* o = reinterpret_cast<uint16_t*>(p.o);
-#pragma unroll
-  for (int e = 0; e < 2; ++e) {
-    if (r + e >= p.rows) continue;
-    const int t = (r + e) / p.G, h = g * p.G + (r + e) - t * p.G;
-    uint16_t* dst = o + (((long long)b * p.L + t) * p.Hq + h) * D + d;
-    dst[0] = f32_to_16bit(e ? v.y : v.x, BF ? 0 : 1);
-    dst[8] = f32_to_16bit(e ? v.w : v.z, BF ? 0 : 1);
+// The equal cut of `total` units over `ctas` CTAs, the first `extra` of which have one more
+struct PagedCut {
+  int ctas, base, extra;
+  __device__ __forceinline__ int first(int c) const { return c * base + min(c, extra); }
+  __device__ __forceinline__ int cta_of(int u) const {
+    const int lead = extra * (base + 1);
+    return u < lead ? u / (base + 1) : extra + (u - lead) / base;
   }
-}
-__device__ __forceinline__ void paged_store_lse(const PagedAttnArgs& p, int b, int hr, int r, float m, float l) {
-  if (p.lse == nullptr || r >= p.rows) return;
-  const int t = r / p.G, h = hr / p.row_tiles * p.G + r - t * p.G;
-  p.lse[((long long)b * p.L + t) * p.Hq + h] = l == 0.0f ? -INFINITY : fmaf(0.69314718055994531f, m, logf(l));
+};
+
+// Whether query row r (token t = r / G) sees key j, j < n or not; rows past the last
+// one count as the last token's.  No branch around the mask's byte, so that several are fetched at once.
+__device__ __forceinline__ bool paged_visible(const PagedAttnArgs& p, int b, int n, int j, int r) {
+  const int t = min(p.g_div(r), p.L - 1), jt = j - (n - p.L);
+  bool see = jt <= t;
+  if (p.tail) see = jt < 0 || p.tail[b * p.ldm_b + t * p.ldm_t + max(0, min(jt, p.L - 1))] != 0;
+  return see && j < n;
 }
 
-// The CTA's range [w0, w1) of the call's units and the position of w0, for the
-// `ctas` CTAs that take part.  False: this CTA has none.
-__device__ __forceinline__ bool paged_range(const PagedAttnArgs& p, long long& total, long long& w0, long long& w1,
-                                            int& ctas, PagedPos& pos) {
-  __shared__ long long s_sum[PAT_WARPS];
-  __shared__ long long s_total;
-  __shared__ long long s_first;
-  __shared__ int s_b;
+// Where row r of KV head g lies in o and lse, in heads
+__device__ __forceinline__ long long paged_row(const PagedAttnArgs& p, int b, int g, int r) {
+  const int t = p.g_div(r);
+  return ((long long)b * p.L + t) * p.Hq + g * p.G + (r - t * p.G);
+}
+// 16 dims (from mt * 16) of 8 rows (from r8) out of a fragment of O^T (v: dims d, d
+// + 8 of two rows): packed and transposed, so that a lane holds two dims of row
+// lane / 4 and stores 4 bytes twice.  `row`: the lane's row's place, or -1.
+template <bool BF, int D>
+__device__ __forceinline__ void paged_store(const PagedAttnArgs& p, long long row, int mt, int lane, float4 v) {
+  const uint32_t lo = pat_transpose(pat_pack<BF>(v.x, v.y)), hi = pat_transpose(pat_pack<BF>(v.z, v.w));
+  if (row < 0) return;
+  uint32_t* dst = reinterpret_cast<uint32_t*>(reinterpret_cast<uint16_t*>(p.o) + row * D + mt * 16) + (lane & 3);
+  dst[0] = lo;
+  dst[4] = hi;
+}
+__device__ __forceinline__ void paged_store_lse(const PagedAttnArgs& p, int b, int g, int r, float m, float l) {
+  if (p.lse == nullptr || r >= p.rows) return;
+  p.lse[paged_row(p, b, g, r)] = l == 0.0f ? -INFINITY : fmaf(0.69314718055994531f, m, logf(l));
+}
+
+// This CTA's place in the cut of the call's units and the position of its first
+// unit.  False: this CTA has none.
+__device__ __forceinline__ bool paged_range(const PagedAttnArgs& p, PagedCut& cut, PagedPos& pos) {
+  __shared__ int s_sum[PAT_WARPS], s_more[PAT_WARPS];
+  __shared__ int s_b, s_first;
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   const int per = p.Hk * p.row_tiles;
-  long long sum = 0;
-  for (int b = tid; b < p.B; b += PAT_THREADS) {
-    sum += (long long)paged_units(paged_len(p, b)) * per;
-    if (blockIdx.x == 0 && p.err && p.seq_lens[b] > (long long)p.max_pages * p.page_size)
-      atomicOr(p.err, SIMSD_DEV_ERR_BAD_INDEX);
+  const bool flag = blockIdx.x == 0 && p.err != nullptr;
+  auto units = [&](int b) {
+    if (b >= p.B) return 0;
+    if (flag && p.seq_lens[b] > (long long)p.max_pages * p.page_size) atomicOr(p.err, SIMSD_DEV_ERR_BAD_INDEX);
+    return paged_units(paged_len(p, b)) * per;
+  };
+  // sequences tid, tid + PAT_THREADS, ...: the first of them scanned, the others summed
+  int u = units(tid), incl = u, more = 0;
+  for (int b = tid + PAT_THREADS; b < p.B; b += PAT_THREADS) more += units(b);
+#pragma unroll
+  for (int m = 1; m < 32; m <<= 1) {
+    const int v = __shfl_up_sync(0xffffffffu, incl, m);
+    if (lane >= m) incl += v;
+    more += __shfl_xor_sync(0xffffffffu, more, m);
   }
-#pragma unroll
-  for (int m = 16; m > 0; m >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, m);
-  if (lane == 0) s_sum[warp] = sum;
+  if (lane == 31) s_sum[warp] = incl, s_more[warp] = more;
   __syncthreads();
-  total = 0;
+  int off = 0, head = 0, total = 0;
 #pragma unroll
-  for (int w = 0; w < PAT_WARPS; ++w) total += s_sum[w];
-  ctas = (int)min((long long)gridDim.x, total);
+  for (int w = 0; w < PAT_WARPS; ++w) {
+    if (w < warp) off += s_sum[w];
+    head += s_sum[w];
+    total += s_sum[w] + s_more[w];
+  }
+  cut.ctas = min((int)gridDim.x, total);
   const int c = blockIdx.x;
-  if (c >= ctas) return false;
-  w0 = total * c / ctas;
-  w1 = total * (c + 1) / ctas;
-  // the sequence that holds w0
-  long long before = 0;
-  for (int base = 0; base < p.B; base += PAT_THREADS) {
-    const int b = base + tid;
-    long long u = b < p.B ? (long long)paged_units(paged_len(p, b)) * per : 0;
-    long long incl = u;
+  if (c >= cut.ctas) return false;
+  cut.base = total / cut.ctas;
+  cut.extra = total - cut.base * cut.ctas;
+  const int w0 = cut.first(c);
+  if (off + incl - u <= w0 && w0 < off + incl) s_b = tid, s_first = off + incl - u;
+  for (int base = PAT_THREADS, before = head; before <= w0; base += PAT_THREADS) {   // past the first sequences
+    u = incl = units(base + tid);
 #pragma unroll
     for (int m = 1; m < 32; m <<= 1) {
-      const long long v = __shfl_up_sync(0xffffffffu, incl, m);
+      const int v = __shfl_up_sync(0xffffffffu, incl, m);
       if (lane >= m) incl += v;
     }
     __syncthreads();
     if (lane == 31) s_sum[warp] = incl;
     __syncthreads();
-    long long off = before;
-    for (int w = 0; w < warp; ++w) off += s_sum[w];
-    if (off + incl - u <= w0 && w0 < off + incl) s_b = b, s_first = off + incl - u;
-    if (tid == PAT_THREADS - 1) s_total = off + incl;
-    __syncthreads();
-    before = s_total;
-    if (before > w0) break;
+    off = before;
+#pragma unroll
+    for (int w = 0; w < PAT_WARPS; ++w) {
+      if (w < warp) off += s_sum[w];
+      before += s_sum[w];
+    }
+    if (off + incl - u <= w0 && w0 < off + incl) s_b = base + tid, s_first = off + incl - u;
   }
+  __syncthreads();
   pos.b = s_b;
   pos.n = paged_len(p, pos.b);
   pos.nu = paged_units(pos.n);
-  const long long rem = w0 - s_first;
-  pos.hr = (int)(rem / pos.nu);
-  pos.unit = (int)(rem - (long long)pos.hr * pos.nu);
+  const int rem = w0 - s_first, hr = rem / pos.nu;
+  pos.unit = rem - hr * pos.nu;
+  pos.g = hr / p.row_tiles;
+  pos.rt = hr - pos.g * p.row_tiles;
   return true;
 }
 
+// A cut sequence (one KV head and row tile, rows from r0): its first CTA and how many it lies in
+struct PagedPart {
+  int b, g, r0, c0, parts;
+};
+
+// Joins the parts of a cut sequence (one KV head and row tile of it) that starts
+// in CTA c0: part i's max, sum and O lie in slot 1 of CTA c0 for i = 0, in slot 0
+// of CTA c0 + i for the others.  `buf`: OBUF bytes of shared memory.
 template <int D, int NT, bool BF>
-__global__ void __launch_bounds__(PAT_THREADS, PAT_CTAS_PER_SM) paged_attention_kernel(const PagedAttnArgs p) {
+__device__ __noinline__ void paged_join(const PagedAttnArgs& p, int b, int g, int r0, int c0, int parts, float* buf) {
+  constexpr int MT = D / 16, NR = NT * 8, PER = MT * NT * 32 / PAT_THREADS;
+  constexpr int GR = PAT_THREADS / NR, KEEP = 4;              // threads of a row, parts a thread keeps
+  constexpr int CAP = PatSmem<D, NT>::OBUF / 4 / NR;          // parts whose weights fit in buf
+  const int tid = threadIdx.x, lane = tid & 31, r = tid % NR, grp = tid / NR;
+  auto slot = [&](int i) { return i == 0 ? 2 * c0 + 1 : 2 * (c0 + i); };
+  // the first two parts of O (most sequences are cut once) are on their way while the weights are made
+  float4 lead[2][PER];
+#pragma unroll
+  for (int i = 0; i < 2; ++i)
+#pragma unroll
+    for (int k = 0; k < PER; ++k)
+      lead[i][k] = __ldcg(p.part_o + (long long)slot(i) * (MT * NT * 32) + tid + k * PAT_THREADS);
+  float2 keep[KEEP];
+#pragma unroll
+  for (int k = 0; k < KEEP; ++k) {
+    const int i = grp + k * GR;
+    keep[k] = i < parts ? __ldcg(p.part_ml + slot(i) * NR + r) : make_float2(-INFINITY, 0.0f);
+  }
+  float mm = -INFINITY, ll = 0.0f;
+  auto see = [&](float2 x) {
+    const float mn = fmaxf(mm, x.x), mu = mn == -INFINITY ? 0.0f : mn;
+    ll = fmaf(ll, pat_exp2(mm - mu), x.y * pat_exp2(x.x - mu));
+    mm = mn;
+  };
+#pragma unroll
+  for (int k = 0; k < KEEP; ++k) see(keep[k]);
+  for (int i = grp + KEEP * GR; i < parts; i += GR) see(__ldcg(p.part_ml + slot(i) * NR + r));
+  float* all = buf + GR * NR;
+  buf[grp * NR + r] = mm, all[grp * NR + r] = ll;
+  __syncthreads();
+  mm = -INFINITY, ll = 0.0f;
+#pragma unroll
+  for (int k = 0; k < GR; ++k) see(make_float2(buf[k * NR + r], all[k * NR + r]));
+  if (grp == 0) paged_store_lse(p, b, g, r0 + r, mm, ll);
+  const float mu = mm == -INFINITY ? 0.0f : mm, inv = ll == 0.0f ? 0.0f : 1.0f / ll;
+  float4 a[PER];
+#pragma unroll
+  for (int k = 0; k < PER; ++k) a[k] = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+  for (int i0 = 0; i0 < parts; i0 += CAP) {
+    const int n = min(CAP, parts - i0);
+    __syncthreads();
+    for (int i = grp; i < n; i += GR) {
+      const int k = (i0 + i) / GR;
+      float x = 0.0f;
+      if (k < KEEP) {
+#pragma unroll
+        for (int q = 0; q < KEEP; ++q) x = k == q ? keep[q].x : x;
+      } else {
+        x = __ldcg(p.part_ml + slot(i0 + i) * NR + r).x;
+      }
+      buf[i * NR + r] = pat_exp2(x - mu) * inv;
+    }
+    __syncthreads();
+    auto add = [&](int i, int k, float4 v) {
+      const int rr = (tid + k * PAT_THREADS) / 32 % NT * 8 + 2 * (lane & 3);
+      const float f0 = buf[i * NR + rr], f1 = buf[i * NR + rr + 1];
+      a[k].x = fmaf(v.x, f0, a[k].x), a[k].y = fmaf(v.y, f1, a[k].y);
+      a[k].z = fmaf(v.z, f0, a[k].z), a[k].w = fmaf(v.w, f1, a[k].w);
+    };
+    int i = 0;
+    if (i0 == 0) {
+#pragma unroll
+      for (; i < 2; ++i)
+#pragma unroll
+        for (int k = 0; k < PER; ++k) add(i, k, lead[i][k]);
+    }
+#pragma unroll 4
+    for (; i < n; ++i) {
+      const float4* o = p.part_o + (long long)slot(i0 + i) * (MT * NT * 32);
+#pragma unroll
+      for (int k = 0; k < PER; ++k) add(i, k, __ldcg(o + tid + k * PAT_THREADS));
+    }
+  }
+#pragma unroll
+  for (int k = 0; k < PER; ++k) {
+    const int x = tid + k * PAT_THREADS, rr = r0 + x / 32 % NT * 8 + (lane >> 2);
+    paged_store<BF, D>(p, rr < p.rows ? paged_row(p, b, g, rr) : -1, x / (NT * 32), lane, a[k]);
+  }
+}
+
+template <int D, int NT, bool BF>
+__global__ void __launch_bounds__(PAT_THREADS, PAT_CTAS_PER_SM) paged_attention_kernel(const __grid_constant__ PagedAttnArgs p) {
   griddep_launch_dependents();
   griddep_wait();
   using S = PatSmem<D, NT>;
   constexpr int MT = D / 16, NR = NT * 8, CH = D / 8;     // 16-byte chunks of a key
   constexpr int KPI = 32 / CH;                            // keys per cp.async of the warp
   constexpr bool QREG = NT <= 2;
+  constexpr int QW = QREG ? MT * NT * 2 : NR * CH * 4 / PAT_THREADS;   // words of the queries in a thread
   extern __shared__ __align__(128) uint8_t pat_smem[];
+  __shared__ PagedPart s_cut[2];
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   const uint32_t ring = smem_u32(pat_smem) + warp * S::STAGES * 2 * S::MAT;
   float4* obuf = reinterpret_cast<float4*>(pat_smem + S::RING);
@@ -240,46 +377,73 @@ __global__ void __launch_bounds__(PAT_THREADS, PAT_CTAS_PER_SM) paged_attention_
   float* sm_m = reinterpret_cast<float*>(pat_smem + S::RING + S::OBUF + S::Q);
   float* sm_l = sm_m + PAT_WARPS * NR;
 
-  long long total, w0, w1;
-  int ctas;
+  PagedCut cut;
   PagedPos ld;
-  if (!paged_range(p, total, w0, w1, ctas, ld)) {
-    if (tid == 0) p.desc[blockIdx.x] = make_int4(0, 0, -1, 0);
-    return;
-  }
-  if (tid == 0) p.desc[blockIdx.x] = make_int4(0, 0, -1, 0);
+  if (!paged_range(p, cut, ld)) return;
+  if (tid < 2) s_cut[tid].parts = 0;
   PagedPos at = ld;
-  const int steps = (int)(w1 - w0);
+  const int w0 = cut.first(blockIdx.x), steps = cut.first(blockIdx.x + 1) - w0;
 
-  // the page of the key that this lane (< 16) places next, fetched a step ahead
+  // ---- loads: the warp's 16 keys of position `ld` into ring slot `loaded` % STAGES.
+  // Pages of a multiple of 16 tokens hold all sixteen in one page, a fixed distance
+  // apart; otherwise every key's place is looked up (by lane key % 16, handed round).
+  // The page numbers are fetched a step ahead.
+  const bool page16 = p.page_size % 16 == 0;
+  const int kc = lane % CH, khi = lane / CH;
+  const uint32_t swz = (uint32_t)(khi * (D * 2) + ((kc ^ khi) << 4));
   auto fetch_page = [&](const PagedPos& x) {
-    const int key = x.unit * PAT_TK + warp * 16 + (lane & 15);
-    return key < x.n ? p.page_table[x.b * p.ld_table + key / p.page_size] : -1;
+    const int key = x.unit * PAT_TK + warp * 16 + (page16 ? 0 : lane & 15);
+    return key < x.n ? p.page_table[x.b * p.ld_table + p.page_div(key)] : -1;
   };
   int page = fetch_page(ld);
   int loaded = 0;
+  uint32_t load_slot = ring;
   auto load = [&]() {
     if (loaded < steps) {
-      const uint32_t dst = ring + (loaded % S::STAGES) * 2 * S::MAT;
-      const int key = ld.unit * PAT_TK + warp * 16 + (lane & 15);
-      long long off = -1;
-      if (key < ld.n) {
-        if (page >= 0 && page < p.num_pages)
-          off = page * p.ld_page + (ld.hr / p.row_tiles) * p.ld_head + (key % p.page_size) * p.ld_tok;
-        else if (p.err)
-          atomicOr(p.err, SIMSD_DEV_ERR_BAD_INDEX);
-      }
-      const int c = lane % CH;
+      const uint32_t dst = load_slot + swz;
+      const int key0 = ld.unit * PAT_TK + warp * 16;
+      if (key0 < ld.n) {
+        const bool fine = page >= 0 && page < p.num_pages;
+        if (page16) {
+          if (!fine && p.err) atomicOr(p.err, SIMSD_DEV_ERR_BAD_INDEX);
+          const int in = key0 - p.page_div(key0) * p.page_size;
+          const long long off = fine ? page * p.ld_page + ld.g * p.ld_head + (in + khi) * p.ld_tok + kc * 8 : 0;
+          const char* k = reinterpret_cast<const char*>(p.k_cache) + off * 2;
+          const char* v = reinterpret_cast<const char*>(p.v_cache) + off * 2;
+          const long long step = fine ? KPI * p.ld_tok * 2 : 0;
+          const int left = fine ? ld.n - key0 - khi : 0;      // > i KPI where the key exists
 #pragma unroll
-      for (int i = 0; i < 16 / KPI; ++i) {
-        const int r = i * KPI + lane / CH;
-        const long long o = __shfl_sync(0xffffffffu, off, r);
-        const uint32_t s = dst + r * (D * 2) + ((c ^ (r & 7)) << 4);
-        const long long e = o < 0 ? 0 : o + c * 8;
-        pat_cp16(s, reinterpret_cast<const uint16_t*>(p.k_cache) + e, o >= 0);
-        pat_cp16(s + S::MAT, reinterpret_cast<const uint16_t*>(p.v_cache) + e, o >= 0);
+          for (int i = 0; i < 16 / KPI; ++i) {
+            const uint32_t s = (dst ^ ((i * KPI & 7) << 4)) + i * KPI * (D * 2);
+            const bool ok = left > i * KPI;
+            pat_cp16(s, ok ? k : reinterpret_cast<const char*>(p.k_cache), ok);
+            pat_cp16(s + S::MAT, ok ? v : reinterpret_cast<const char*>(p.v_cache), ok);
+            k += step;
+            v += step;
+          }
+        } else {
+          const int key = key0 + (lane & 15);
+          long long off = -1;
+          if (key < ld.n) {
+            if (fine)
+              off = page * p.ld_page + ld.g * p.ld_head +
+                    (key - p.page_div(key) * p.page_size) * p.ld_tok;
+            else if (p.err)
+              atomicOr(p.err, SIMSD_DEV_ERR_BAD_INDEX);
+          }
+#pragma unroll
+          for (int i = 0; i < 16 / KPI; ++i) {
+            const long long o = __shfl_sync(0xffffffffu, off, i * KPI + khi);
+            const uint32_t s = (dst ^ ((i * KPI & 7) << 4)) + i * KPI * (D * 2);
+            const long long e = o < 0 ? 0 : o + kc * 8;
+            pat_cp16(s, reinterpret_cast<const uint16_t*>(p.k_cache) + e, o >= 0);
+            pat_cp16(s + S::MAT, reinterpret_cast<const uint16_t*>(p.v_cache) + e, o >= 0);
+          }
+        }
       }
       ++loaded;
+      load_slot += 2 * S::MAT;
+      if (load_slot == ring + S::STAGES * 2 * S::MAT) load_slot = ring;
       if (loaded < steps) {
         ld.next(p);
         page = fetch_page(ld);
@@ -287,40 +451,63 @@ __global__ void __launch_bounds__(PAT_THREADS, PAT_CTAS_PER_SM) paged_attention_
     }
     pat_commit();
   };
+
+  // ---- queries of a row tile: up to 16 rows as the first product's fragments in
+  // registers, more through shared memory
+  uint32_t qnext[QW];
+  auto fetch_queries = [&](int b, int g, int rt) {
+    const int r0 = rt * NR;
+    const uint16_t* qb = reinterpret_cast<const uint16_t*>(p.q);
+    if constexpr (QREG) {
+#pragma unroll
+      for (int nt = 0; nt < NT; ++nt) {
+        const int r = r0 + nt * 8 + (lane >> 2);
+        const bool in = r < p.rows && b < p.B;
+        const uint16_t* src = qb + (in ? paged_row(p, b, g, r) * D : 0) + 2 * (lane & 3);
+#pragma unroll
+        for (int k = 0; k < MT * 2; ++k)
+          qnext[k * NT + nt] = in ? __ldg(reinterpret_cast<const uint32_t*>(src + k * 8)) ^ p.q_sign : 0u;
+      }
+    } else {
+#pragma unroll
+      for (int k = 0; k < QW / 4; ++k) {
+        const int x = tid + k * PAT_THREADS, r = r0 + x / CH;
+        const bool in = r < p.rows && b < p.B;
+        const uint4 v = in ? __ldg(reinterpret_cast<const uint4*>(qb + paged_row(p, b, g, r) * D + x % CH * 8))
+                           : make_uint4(0, 0, 0, 0);
+        const uint32_t f = in ? p.q_sign : 0u;
+        qnext[4 * k] = v.x ^ f, qnext[4 * k + 1] = v.y ^ f, qnext[4 * k + 2] = v.z ^ f, qnext[4 * k + 3] = v.w ^ f;
+      }
+    }
+  };
+  fetch_queries(at.b, at.g, at.rt);
 #pragma unroll
   for (int s = 0; s < S::STAGES - 1; ++s) load();
 
   float o[MT][NT][4], m[NT][2], l[NT][2];
-  uint32_t bq[QREG ? MT : 1][QREG ? NT : 1][2];
+  uint32_t bq[QREG ? QW : 1];
   int first_unit = at.unit;
+  uint32_t slot_at = ring;
   for (int i = 0; i < steps; ++i) {
     if (i == 0 || at.unit == 0) {
       // a new sequence, head or row tile: its queries, and empty sums
       first_unit = at.unit;
-      const int g = at.hr / p.row_tiles, r0 = (at.hr - g * p.row_tiles) * NR;
-      const uint16_t* qb = reinterpret_cast<const uint16_t*>(p.q);
       if constexpr (QREG) {
 #pragma unroll
-        for (int nt = 0; nt < NT; ++nt) {
-          const int r = r0 + nt * 8 + (lane >> 2);
-          const int t = r / p.G, h = g * p.G + r - t * p.G;
-          const uint16_t* src = qb + (((long long)at.b * p.L + t) * p.Hq + h) * D + 2 * (lane & 3);
-#pragma unroll
-          for (int ks = 0; ks < MT; ++ks)
-#pragma unroll
-            for (int e = 0; e < 2; ++e)
-              bq[ks][nt][e] = r < p.rows ? *reinterpret_cast<const uint32_t*>(src + ks * 16 + e * 8) : 0u;
-        }
+        for (int k = 0; k < QW; ++k) bq[k] = qnext[k];
       } else {
-        for (int x = tid; x < NR * CH; x += PAT_THREADS) {
-          const int rr = x / CH, c = x % CH, r = r0 + rr;
-          const int t = r / p.G, h = g * p.G + r - t * p.G;
-          const uint4 v = r < p.rows ? *reinterpret_cast<const uint4*>(
-                                           qb + (((long long)at.b * p.L + t) * p.Hq + h) * D + c * 8)
-                                     : make_uint4(0, 0, 0, 0);
-          *reinterpret_cast<uint4*>(qs + rr * (D * 2) + ((c ^ (rr & 7)) << 4)) = v;
+#pragma unroll
+        for (int k = 0; k < QW / 4; ++k) {
+          const int x = tid + k * PAT_THREADS, rr = x / CH, c = x % CH;
+          *reinterpret_cast<uint4*>(qs + rr * (D * 2) + ((c ^ (rr & 7)) << 4)) =
+              make_uint4(qnext[4 * k], qnext[4 * k + 1], qnext[4 * k + 2], qnext[4 * k + 3]);
         }
         __syncthreads();
+      }
+      if (at.nu - at.unit < steps - i) {
+        int b = at.b, g = at.g, rt = at.rt;
+        PagedPos::next_rows(p, b, g, rt);
+        fetch_queries(b, g, rt);
       }
 #pragma unroll
       for (int nt = 0; nt < NT; ++nt) {
@@ -335,7 +522,9 @@ __global__ void __launch_bounds__(PAT_THREADS, PAT_CTAS_PER_SM) paged_attention_
     load();
     pat_wait<S::STAGES - 1>();
     __syncwarp();
-    const uint32_t ks_base = ring + (i % S::STAGES) * 2 * S::MAT, vs_base = ks_base + S::MAT;
+    const uint32_t ks_base = slot_at, vs_base = ks_base + S::MAT;
+    slot_at += 2 * S::MAT;
+    if (slot_at == ring + S::STAGES * 2 * S::MAT) slot_at = ring;
     const int key0 = at.unit * PAT_TK + warp * 16;
     if (key0 < at.n) {
       // S^T = K Q^T
@@ -349,7 +538,7 @@ __global__ void __launch_bounds__(PAT_THREADS, PAT_CTAS_PER_SM) paged_attention_
         pat_ldsm(ks_base + kr * (D * 2) + (((ks * 2 + (lane >> 4)) ^ (kr & 7)) << 4), a);
         if constexpr (QREG) {
 #pragma unroll
-          for (int nt = 0; nt < NT; ++nt) pat_mma<BF>(s[nt], a, bq[ks][nt][0], bq[ks][nt][1]);
+          for (int nt = 0; nt < NT; ++nt) pat_mma<BF>(s[nt], a, bq[2 * ks * NT + nt], bq[(2 * ks + 1) * NT + nt]);
         } else {
 #pragma unroll
           for (int nt = 0; nt < NT; nt += 2) {
@@ -362,17 +551,21 @@ __global__ void __launch_bounds__(PAT_THREADS, PAT_CTAS_PER_SM) paged_attention_
           }
         }
       }
-      const int g = at.hr / p.row_tiles, r0 = (at.hr - g * p.row_tiles) * NR;
+      const int r0 = at.rt * NR;
       const bool edge = key0 + 16 > at.n - p.L;          // some key of the sixteen may be hidden from some row
+      if (edge) {
+        uint32_t see = 0;
 #pragma unroll
-      for (int nt = 0; nt < NT; ++nt)
+        for (int x = 0; x < NT * 4; ++x)
+          see |= (uint32_t)paged_visible(p, at.b, at.n, key0 + (lane >> 2) + (x & 2) * 4,
+                                         r0 + (x >> 2) * 8 + 2 * (lane & 3) + (x & 1)) << x;
 #pragma unroll
-        for (int e = 0; e < 4; ++e) {
-          s[nt][e] *= p.scale_log2;
-          if (edge && !paged_visible(p, at.b, at.n, key0 + (lane >> 2) + (e >> 1) * 8,
-                                     r0 + nt * 8 + 2 * (lane & 3) + (e & 1)))
-            s[nt][e] = -INFINITY;
-        }
+        for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+          for (int e = 0; e < 4; ++e)
+            if (!(see >> (nt * 4 + e) & 1)) s[nt][e] = -INFINITY;
+      }
+      // m: the running maximum of the unscaled scores (the scale is positive)
       bool up = false;
 #pragma unroll
       for (int nt = 0; nt < NT; ++nt)
@@ -388,7 +581,7 @@ __global__ void __launch_bounds__(PAT_THREADS, PAT_CTAS_PER_SM) paged_attention_
             x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, 8));
             x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, 16));
             x = fmaxf(x, m[nt][e]);
-            const float f = x == -INFINITY ? 1.0f : exp2f(m[nt][e] - x);
+            const float f = x == -INFINITY ? 1.0f : pat_exp2(m[nt][e] * p.scale_log2 - x * p.scale_log2);
             m[nt][e] = x;
             l[nt][e] *= f;
 #pragma unroll
@@ -399,19 +592,19 @@ __global__ void __launch_bounds__(PAT_THREADS, PAT_CTAS_PER_SM) paged_attention_
 #pragma unroll
       for (int nt = 0; nt < NT; ++nt) {
 #pragma unroll
-        for (int e = 0; e < 4; ++e) {
-          const float mm = m[nt][e & 1];
-          s[nt][e] = exp2f(s[nt][e] - (mm == -INFINITY ? 0.0f : mm));
+        for (int e = 0; e < 2; ++e) {
+          const float ms = m[nt][e] == -INFINITY ? 0.0f : m[nt][e] * p.scale_log2;
+          s[nt][e] = pat_exp2(fmaf(s[nt][e], p.scale_log2, -ms));
+          s[nt][e + 2] = pat_exp2(fmaf(s[nt][e + 2], p.scale_log2, -ms));
+          l[nt][e] += s[nt][e] + s[nt][e + 2];
         }
-        l[nt][0] += s[nt][0] + s[nt][2];
-        l[nt][1] += s[nt][1] + s[nt][3];
         pb[nt][0] = pat_transpose(pat_pack<BF>(s[nt][0], s[nt][1]));
         pb[nt][1] = pat_transpose(pat_pack<BF>(s[nt][2], s[nt][3]));
       }
       // O^T += V^T P^T
       const int vr = (lane & 7) + (lane >> 4) * 8, vc = (lane >> 3) & 1;
       bool odd = false;
-      if (edge) {   // a value that is not finite, of a key that some row may not see?
+      if (edge && (p.L > 1 || p.tail)) {   // a value that is not finite, of a key that some row does not see?
         for (int x = lane; x < 16 * CH; x += 32) {
           uint32_t w[4];
           asm volatile("ld.shared.v4.b32 {%0, %1, %2, %3}, [%4];"
@@ -461,11 +654,7 @@ __global__ void __launch_bounds__(PAT_THREADS, PAT_CTAS_PER_SM) paged_attention_
     if (ends || i + 1 == steps) {
       // join the four warps; a whole sequence is written, a part goes to the workspace
       const bool whole = ends && first_unit == 0;
-      const int slot = 2 * blockIdx.x + (first_unit == 0 ? 1 : 0);
-      if (first_unit == 0 && !ends && tid == 0) {
-        const long long last = w0 + i - at.unit + at.nu;    // one past the sequence's last unit
-        p.desc[blockIdx.x] = make_int4(at.b, at.hr, (int)((last * ctas - 1) / total), 0);
-      }
+      const int part = first_unit == 0 ? 1 : 0, slot = 2 * blockIdx.x + part, r0 = at.rt * NR;
 #pragma unroll
       for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
@@ -474,24 +663,13 @@ __global__ void __launch_bounds__(PAT_THREADS, PAT_CTAS_PER_SM) paged_attention_
           x += __shfl_xor_sync(0xffffffffu, x, 4);
           x += __shfl_xor_sync(0xffffffffu, x, 8);
           x += __shfl_xor_sync(0xffffffffu, x, 16);
+          m[nt][e] *= p.scale_log2;
           if (lane < 4) {
             sm_m[warp * NR + nt * 8 + 2 * lane + e] = m[nt][e];
             sm_l[warp * NR + nt * 8 + 2 * lane + e] = x;
           }
         }
       __syncthreads();
-      const int r0 = at.hr % p.row_tiles * NR;
-      for (int r = tid; r < NR; r += PAT_THREADS) {
-        float mm = -INFINITY, ll = 0.0f;
-        for (int w = 0; w < PAT_WARPS; ++w) mm = fmaxf(mm, sm_m[w * NR + r]);
-        for (int w = 0; w < PAT_WARPS; ++w) ll += sm_l[w * NR + r] * exp2f(sm_m[w * NR + r] - (mm == -INFINITY ? 0.0f : mm));
-        if (whole) {
-          paged_store_lse(p, at.b, at.hr, r0 + r, mm, ll);
-        } else {
-          p.part_ml[((long long)slot * NR + r) * 2] = mm;
-          p.part_ml[((long long)slot * NR + r) * 2 + 1] = ll;
-        }
-      }
 #pragma unroll
       for (int nt = 0; nt < NT; ++nt) {
         float f[2], inv[2];
@@ -499,12 +677,22 @@ __global__ void __launch_bounds__(PAT_THREADS, PAT_CTAS_PER_SM) paged_attention_
         for (int e = 0; e < 2; ++e) {
           const int r = nt * 8 + 2 * (lane & 3) + e;
           float mm = -INFINITY, ll = 0.0f;
+#pragma unroll
           for (int w = 0; w < PAT_WARPS; ++w) mm = fmaxf(mm, sm_m[w * NR + r]);
-          if (mm == -INFINITY) mm = 0.0f;
-          for (int w = 0; w < PAT_WARPS; ++w) ll += sm_l[w * NR + r] * exp2f(sm_m[w * NR + r] - mm);
-          f[e] = exp2f(m[nt][e] - mm);
+          const float mu = mm == -INFINITY ? 0.0f : mm;
+#pragma unroll
+          for (int w = 0; w < PAT_WARPS; ++w) ll = fmaf(sm_l[w * NR + r], pat_exp2(sm_m[w * NR + r] - mu), ll);
+          f[e] = pat_exp2(m[nt][e] - mu);
           inv[e] = !whole ? 1.0f : ll == 0.0f ? 0.0f : 1.0f / ll;
+          if (warp == nt % PAT_WARPS && lane < 4) {
+            if (whole)
+              paged_store_lse(p, at.b, at.g, r0 + r, mm, ll);
+            else
+              p.part_ml[slot * NR + r] = make_float2(mm, ll);
+          }
         }
+        const int r = r0 + nt * 8 + (lane >> 2);
+        const long long row = r < p.rows ? paged_row(p, at.b, at.g, r) : -1;
         if (nt > 0) __syncthreads();
 #pragma unroll
         for (int mt = 0; mt < MT; ++mt)
@@ -512,7 +700,8 @@ __global__ void __launch_bounds__(PAT_THREADS, PAT_CTAS_PER_SM) paged_attention_
               make_float4(o[mt][nt][0] * f[0], o[mt][nt][1] * f[1], o[mt][nt][2] * f[0], o[mt][nt][3] * f[1]);
         __syncthreads();
 #pragma unroll
-        for (int mt = warp; mt < MT; mt += PAT_WARPS) {
+        for (int k = 0; k < MT / PAT_WARPS; ++k) {
+          const int mt = warp + k * PAT_WARPS;
           float4 a = obuf[mt * 32 + lane];
 #pragma unroll
           for (int w = 1; w < PAT_WARPS; ++w) {
@@ -521,62 +710,35 @@ __global__ void __launch_bounds__(PAT_THREADS, PAT_CTAS_PER_SM) paged_attention_
           }
           a.x *= inv[0], a.y *= inv[1], a.z *= inv[0], a.w *= inv[1];
           if (whole)
-            paged_store<BF, D>(p, at.b, at.hr, r0 + nt * 8, mt, lane, a);
+            paged_store<BF, D>(p, row, mt, lane, a);
           else
             p.part_o[(((long long)slot * MT + mt) * NT + nt) * 32 + lane] = a;
         }
+      }
+      if (!whole && tid == 0) {
+        const int head = w0 + i - at.unit, c0 = cut.cta_of(head);      // the sequence's first unit and CTA
+        s_cut[part] = {at.b, at.g, r0, c0, cut.cta_of(head + at.nu - 1) - c0 + 1};
       }
       __syncthreads();
     }
     at.next(p);
   }
-}
-
-// One CTA per CTA of paged_attention_kernel: joins the parts of the sequence (one
-// KV head and row tile of it) that starts there and goes on in later CTAs.
-template <int D, int NT, bool BF>
-__global__ void __launch_bounds__(PAC_THREADS) paged_combine_kernel(const PagedAttnArgs p) {
-  griddep_launch_dependents();
-  griddep_wait();
-  constexpr int MT = D / 16, NR = NT * 8;
-  extern __shared__ float pac_w[];                 // [parts][NR]
-  const int c = blockIdx.x;
-  const int4 d = p.desc[c];
-  if (d.z < 0) return;
-  const int parts = d.z - c + 1, tid = threadIdx.x, lane = tid & 31;
-  const int r0 = d.y % p.row_tiles * NR;
-  auto slot = [&](int i) { return (long long)(i == 0 ? 2 * c + 1 : 2 * (c + i)); };
-  for (int r = tid >> 5; r < NR; r += PAC_THREADS / 32) {
-    float mm = -INFINITY, ll = 0.0f;
-    for (int i = lane; i < parts; i += 32) mm = fmaxf(mm, p.part_ml[(slot(i) * NR + r) * 2]);
-#pragma unroll
-    for (int k = 16; k > 0; k >>= 1) mm = fmaxf(mm, __shfl_xor_sync(0xffffffffu, mm, k));
-    const float mu = mm == -INFINITY ? 0.0f : mm;
-    for (int i = lane; i < parts; i += 32) {
-      const float2 x = *reinterpret_cast<const float2*>(p.part_ml + (slot(i) * NR + r) * 2);
-      const float f = exp2f(x.x - mu);
-      pac_w[i * NR + r] = f;
-      ll += x.y * f;
-    }
-#pragma unroll
-    for (int k = 16; k > 0; k >>= 1) ll += __shfl_xor_sync(0xffffffffu, ll, k);
-    const float inv = ll == 0.0f ? 0.0f : 1.0f / ll;
-    __syncwarp();
-    for (int i = lane; i < parts; i += 32) pac_w[i * NR + r] *= inv;
-    if (lane == 0) paged_store_lse(p, d.x, d.y, r0 + r, mm, ll);
+  // cut sequences (at most the range's first and last): the last of their CTAs to get here joins the parts
+  if (s_cut[0].parts + s_cut[1].parts == 0) return;
+  if (tid < 2 && s_cut[tid].parts > 0) {
+    __threadfence();
+    const int c0 = s_cut[tid].c0;
+    if (atomicAdd(p.arrived + c0, 1) == s_cut[tid].parts - 1)
+      p.arrived[c0] = 0;
+    else
+      s_cut[tid].parts = 0;
+    __threadfence();
   }
   __syncthreads();
-  for (int x = tid; x < MT * NT * 32; x += PAC_THREADS) {
-    const int mt = x / (NT * 32), nt = x / 32 % NT;
-    const int r = nt * 8 + 2 * (lane & 3);
-    float4 a = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-#pragma unroll 8
-    for (int i = 0; i < parts; ++i) {
-      const float4 v = p.part_o[slot(i) * (MT * NT * 32) + x];
-      const float f0 = pac_w[i * NR + r], f1 = pac_w[i * NR + r + 1];
-      a.x = fmaf(v.x, f0, a.x), a.y = fmaf(v.y, f1, a.y), a.z = fmaf(v.z, f0, a.z), a.w = fmaf(v.w, f1, a.w);
-    }
-    paged_store<BF, D>(p, d.x, d.y, r0 + nt * 8, mt, lane, a);
+  for (int k = 0; k < 2; ++k) {
+    const PagedPart x = s_cut[k];
+    if (x.parts > 0) paged_join<D, NT, BF>(p, x.b, x.g, x.r0, x.c0, x.parts, reinterpret_cast<float*>(obuf));
+    __syncthreads();
   }
 }
 

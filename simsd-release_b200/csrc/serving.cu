@@ -2,6 +2,8 @@
 // include/simsd_b200.h): the paged key-value cache and draft verification.
 #include <cuda_runtime.h>
 
+#include <algorithm>
+#include <cmath>
 #include <mutex>
 #include <utility>
 
@@ -50,22 +52,27 @@ int cache_check(const void* k, const void* v, int64_t ld_page, int64_t ld_head, 
 
 // What paged attention does with G L rows per KV head: 8-row tiles per CTA (all
 // rows in one pass over the keys up to 32, more in row tiles of 32), the grid, and
-// the workspace: two parts per CTA (the end of a sequence it started inside, the
-// start of one it leaves unfinished).
+// the workspace: the arrival counters, then two parts per CTA (the end of a sequence
+// it started inside, the start of one it leaves unfinished).
 struct PagedPlan {
   int nt, grid;
-  size_t ml_at, desc_at, bytes;
+  size_t ml_at, bytes;
 };
 PagedPlan paged_plan(int L, int G, int D) {
   PagedPlan p;
   const long long rows = (long long)L * G;
   p.nt = rows <= 8 ? 1 : rows <= 16 ? 2 : 4;
   const int sms = simsd_device_sm_count();
-  p.grid = PAT_CTAS_PER_SM * (sms > 0 ? sms : 148);
-  p.ml_at = align256((size_t)2 * p.grid * D * p.nt * 8 * sizeof(float));
-  p.desc_at = p.ml_at + align256((size_t)2 * p.grid * p.nt * 8 * 2 * sizeof(float));
-  p.bytes = p.desc_at + align256((size_t)p.grid * sizeof(int4));
+  p.grid = std::min(PAT_CTAS_PER_SM * (sms > 0 ? sms : 148), SIMSD_PAGED_COUNTER_BYTES / (int)sizeof(int));
+  p.ml_at = SIMSD_PAGED_COUNTER_BYTES + align256((size_t)2 * p.grid * D * p.nt * 8 * sizeof(float));
+  p.bytes = p.ml_at + align256((size_t)2 * p.grid * p.nt * 8 * sizeof(float2));
   return p;
+}
+
+PagedDiv paged_div(int d) {
+  int sh = 0;
+  while ((1LL << sh) < d) ++sh;
+  return {(uint32_t)(((1ULL << (31 + sh)) + d - 1) / d), 31 + sh};
 }
 
 // Raise a kernel's shared-memory limit once per device.
@@ -110,10 +117,7 @@ int attend(const PagedAttnArgs& a, const PagedPlan& pl, void* stream) {
   constexpr int smem = PatSmem<D, NT>::BYTES;
   int rc = allow_smem(paged_attention_kernel<D, NT, BF>, smem, done);
   if (rc != SIMSD_OK) return rc;
-  rc = launch_on(paged_attention_kernel<D, NT, BF>, pl.grid, PAT_THREADS, smem, stream, false, a);
-  if (rc != SIMSD_OK) return rc;
-  return launch_on(paged_combine_kernel<D, NT, BF>, pl.grid, PAC_THREADS, (size_t)pl.grid * NT * 8 * sizeof(float), stream,
-                   true, a);
+  return launch_on(paged_attention_kernel<D, NT, BF>, pl.grid, PAT_THREADS, smem, stream, false, a);
 }
 
 }  // namespace
@@ -211,14 +215,19 @@ int simsd_paged_attention(const void* q, const void* k_cache, const void* v_cach
   a.num_pages = num_pages;
   a.page_size = page_size;
   a.max_pages = max_pages;
-  a.scale_log2 = scale * 1.4426950408889634f;
+  a.page_div = paged_div(page_size);
+  a.g_div = paged_div(a.G);
+  a.q_sign = scale < 0.0f ? 0x80008000u : 0u;
+  a.scale_log2 = std::max(std::fabs(scale) * 1.4426950408889634f, 1e-30f);
   const PagedPlan pl = paged_plan(L, a.G, head_dim);
   a.rows = a.G * L;
   a.row_tiles = (a.rows + pl.nt * 8 - 1) / (pl.nt * 8);
+  if ((long long)B * Hk * a.row_tiles * ((int64_t)max_pages * page_size / PAT_TK + 1) > 0x7fffffffLL)
+    return SIMSD_ERR_UNSUPPORTED;
   uint8_t* ws = reinterpret_cast<uint8_t*>(workspace);
-  a.part_o = reinterpret_cast<float4*>(ws);
-  a.part_ml = reinterpret_cast<float*>(ws + pl.ml_at);
-  a.desc = reinterpret_cast<int4*>(ws + pl.desc_at);
+  a.arrived = reinterpret_cast<int*>(ws);
+  a.part_o = reinterpret_cast<float4*>(ws + SIMSD_PAGED_COUNTER_BYTES);
+  a.part_ml = reinterpret_cast<float2*>(ws + pl.ml_at);
   const bool bf = dtype == SIMSD_BF16;
   switch (pl.nt * 1000 + head_dim) {
     case 1064: return bf ? attend<64, 1, true>(a, pl, stream) : attend<64, 1, false>(a, pl, stream);

@@ -37,6 +37,9 @@ LAUNCH_MOE_SIZE_CLASSES = 8
 IPC_HANDLE_BYTES = 64
 SIGNAL_BYTES = 256
 
+HEADER_BYTES = 256 * 1024          # simsd_workspace_header_bytes()
+PAGED_COUNTER_BYTES = 4096
+
 DEV_ERR_TIMEOUT = 1
 DEV_ERR_BAD_INDEX = 2
 DEV_ERR_CAPACITY = 4
@@ -136,7 +139,7 @@ def check(rc: int, what: str) -> None:
 
 
 def stream_ptr(dev: torch.device) -> int:
-    return torch.cuda.current_stream(dev).cuda_stream
+    return torch._C._cuda_getCurrentRawStream(torch.cuda.current_device() if dev.index is None else dev.index)
 
 
 _SIDE_STREAMS: dict[torch.device, torch.cuda.Stream] = {}
@@ -156,8 +159,11 @@ def device_guard(dev: torch.device):
     sharded model may live elsewhere); a no-op context otherwise, which keeps the
     common call cheap."""
     if dev.index is None or dev.index == torch.cuda.current_device():
-        return contextlib.nullcontext()
+        return _NO_GUARD
     return torch.cuda.device(dev)
+
+
+_NO_GUARD = contextlib.nullcontext()
 
 
 _WS_SIZES: dict[tuple, int] = {}
@@ -206,14 +212,35 @@ def workspace(dev: torch.device, nbytes: int) -> torch.Tensor:
 
 def error_ptr(dev: torch.device) -> int:
     """Device address of the error word in `dev`'s workspace header (`device_error` reads it)."""
-    header = lib().simsd_workspace_header_bytes()
-    return workspace(dev, header).data_ptr() + header - 64
+    return workspace(dev, HEADER_BYTES).data_ptr() + HEADER_BYTES - 64
+
+
+_STREAM_SCRATCH: dict[tuple[int, int], torch.Tensor] = {}
+
+
+def stream_scratch(dev: torch.device, nbytes: int, zeroed: int) -> torch.Tensor:
+    """Scratch of at least `nbytes` for the current stream of `dev`, its first `zeroed`
+    bytes zero when new (the operators leave them zero).  Each stream has its own, so
+    calls on several streams share none; a call under graph capture gets one of the
+    graph's memory, zeroed by the graph on every replay."""
+    if torch.cuda.is_current_stream_capturing():
+        buf = torch.empty(nbytes, dtype=torch.uint8, device=dev)
+        buf[:zeroed].zero_()
+        return buf
+    key = (dev.index, stream_ptr(dev))
+    buf = _STREAM_SCRATCH.get(key)
+    if buf is None or buf.numel() < nbytes:
+        # an outgrown one goes back to torch's allocator, which hands it out again
+        # only to later work of the stream it was allocated on: this one
+        buf = _STREAM_SCRATCH[key] = torch.zeros(nbytes, dtype=torch.uint8, device=dev)
+    return buf
 
 
 def reset_workspace() -> None:
     """Drop the cached workspaces (call before re-capturing graphs in a new pool)."""
     _WORKSPACES.clear()
     _RETIRED.clear()
+    _STREAM_SCRATCH.clear()
 
 
 def device_error(dev: torch.device | None = None) -> int:

@@ -12,8 +12,8 @@ as its `.transpose(1, 2)`.  Slot s is token s % page_size of page s // page_size
 The reference keeps one static cache per sequence
 (speculative_decoding/cache_aware.py:195-215); it has no paged form.
 
-Forward-only; CUDA tensors only (no CPU fallback).  Scratch comes from torch's
-allocator on the caller's stream, so calls on several streams do not share any.
+Forward-only; CUDA tensors only (no CPU fallback).  Every stream has scratch of its
+own, so calls on several streams share none.
 Indices that the device finds out of range raise DEV_ERR_BAD_INDEX in
 `_lib.device_error()`; nothing is read or written for them.
 """
@@ -156,7 +156,7 @@ def paged_attention(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tenso
     lse = torch.empty(q.shape[:-1], dtype=torch.float32, device=dev) if return_lse else None
     L_ = _lib.lib()
     with _lib.device_guard(dev):
-        ws = torch.empty(L_.simsd_paged_attention_workspace_size(B, L, Hq, Hk, D), dtype=torch.uint8, device=dev)
+        ws = _lib.stream_scratch(dev, L_.simsd_paged_attention_workspace_size(B, L, Hq, Hk, D), _lib.PAGED_COUNTER_BYTES)
         rc = L_.simsd_paged_attention(
             q.data_ptr(), k_cache.data_ptr(), v_cache.data_ptr(), pages, page_size, k_cache.stride(0), k_cache.stride(1),
             k_cache.stride(2), page_table.data_ptr(), page_table.stride(0), page_table.shape[1], seq_lens.data_ptr(),
