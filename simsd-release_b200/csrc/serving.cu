@@ -97,7 +97,7 @@ SpecPlan spec_plan(int B, int K, int V) {
   p.parts = (V + SV_PART - 1) / SV_PART;
   p.chunks = (V + SV_CHUNK - 1) / SV_CHUNK;
   p.cand_at = align256((size_t)B * (2 * K + 1) * p.parts * sizeof(float2));
-  p.done_at = p.cand_at + align256((size_t)B * p.chunks * sizeof(float4));
+  p.done_at = p.cand_at + align256((size_t)B * p.chunks * sizeof(float2));
   p.bytes = p.done_at + align256((size_t)B * sizeof(int));
   return p;
 }
@@ -107,7 +107,7 @@ int verify_drafts(const SpecVerifyArgs& a, void* stream) {
   const long long rows = (long long)a.B * (a.draft ? 2 * a.K + 1 : a.K + 1);
   int rc = launch_on(spec_stat_kernel<DT>, rows * ((a.parts + SV_WARPS - 1) / SV_WARPS), SV_THREADS, 0, stream, false, a);
   if (rc != SIMSD_OK) return rc;
-  return launch_on(spec_draw_kernel<DT>, (long long)a.B * a.chunks, SV_THREADS, (size_t)(2 * a.K + 1) * 3 * sizeof(float),
+  return launch_on(spec_draw_kernel<DT>, (long long)a.B * a.chunks, SV_THREADS, (size_t)(2 * a.K + 1) * 2 * sizeof(float),
                    stream, true, a);
 }
 
@@ -272,7 +272,7 @@ int simsd_speculative_verify(const void* target_logits, int64_t ldt_b, int64_t l
   const SpecPlan pl = spec_plan(B, K, V);
   uint8_t* ws = reinterpret_cast<uint8_t*>(workspace);
   a.part = reinterpret_cast<float2*>(ws);
-  a.cand = reinterpret_cast<float4*>(ws + pl.cand_at);
+  a.cand = reinterpret_cast<float2*>(ws + pl.cand_at);
   a.done = reinterpret_cast<int*>(ws + pl.done_at);
   a.parts = pl.parts;
   a.chunks = pl.chunks;

@@ -19,7 +19,9 @@
 // decides how many drafts are kept (every CTA of the sequence for itself: a few KB
 // from L2) and races the one row that is drawn from; the sequence's last CTA to
 // finish writes its outputs.  HBM bounds both; the first also runs one exponential
-// per 2 bytes, about 0.7 of what the SMs' exponential units do in that time.  Rows
+// per 2 bytes, about 0.7 of what the SMs' exponential units do in that time, so the
+// rest of its arithmetic is packed: the maximum in the 16-bit type itself, the
+// differences and sums two at a time.  Rows
 // are read last to first, so that the rows drawn from, mostly early ones, are the
 // ones left in L2.
 #pragma once
@@ -38,8 +40,9 @@ struct SpecVerifyArgs {
   long long* out_tokens;    // [B, K + 1]
   long long* out_accepted;  // [B]
   float* out_logprobs;      // [B, K + 1]
-  float2* part;             // [B, 2 K + 1, parts]: maximum, sum of exp((x - max) / T) of a part of a row
-  float4* cand;             // [B, chunks]: best residual race and token, best race over p and token
+  float2* part;             // [B, 2 K + 1, parts]: maximum, sum of exp((x - max) / T) of a part of a row; in
+                            // greedy sequences the place of the maximum instead of the sum
+  float2* cand;             // [B, chunks]: best race and its token
   int* done;                // [B]: CTAs of the sequence that have finished, zeroed by the first kernel
   int* err;
   long long ldt_b, ldt_r, ldd_b, ldd_r, ld_x, ld_u, ld_n;
@@ -69,6 +72,13 @@ __device__ __forceinline__ float spec_exp2(float x) {
   return y;
 }
 
+template <int DT>
+__device__ __forceinline__ float spec_half(uint32_t w, int hi) {
+  if constexpr (DT == 0) return __uint_as_float(hi ? w & 0xffff0000u : w << 16);
+  const __half2 h = *reinterpret_cast<const __half2*>(&w);
+  return hi ? __high2float(h) : __low2float(h);
+}
+
 // 16 bytes of logits as floats
 template <int DT>
 struct SpecVec {
@@ -90,6 +100,59 @@ struct SpecVec {
     }
   }
 };
+
+// Largest of a lane's vectors, NaN ignored: 16-bit types two at a time
+template <int DT, int VL>
+__device__ __forceinline__ float spec_max(const uint4 (&raw)[VL]) {
+  if constexpr (DT == 2) {
+    float m = -INFINITY;
+#pragma unroll
+    for (int i = 0; i < VL; ++i)
+      m = fmaxf(m, fmaxf(fmaxf(__uint_as_float(raw[i].x), __uint_as_float(raw[i].y)),
+                         fmaxf(__uint_as_float(raw[i].z), __uint_as_float(raw[i].w))));
+    return m;
+  } else {
+    uint32_t m = DT == 0 ? 0xff80ff80u : 0xfc00fc00u;
+    auto see = [&](uint32_t x) {
+      if constexpr (DT == 0)
+        asm("max.bf16x2 %0, %0, %1;" : "+r"(m) : "r"(x));
+      else
+        asm("max.f16x2 %0, %0, %1;" : "+r"(m) : "r"(x));
+    };
+#pragma unroll
+    for (int i = 0; i < VL; ++i) see(raw[i].x), see(raw[i].y), see(raw[i].z), see(raw[i].w);
+    return fmaxf(spec_half<DT>(m, 0), spec_half<DT>(m, 1));
+  }
+}
+
+// Sum of exp2((x - m) c) over a lane's vectors, two values an instruction but for
+// the exponential
+template <int DT, int VL>
+__device__ __forceinline__ float spec_sum(const uint4 (&raw)[VL], float m, float c) {
+  uint64_t nm, cc, sum = 0;
+  asm("mov.b64 %0, {%1, %1};" : "=l"(nm) : "f"(-m));
+  asm("mov.b64 %0, {%1, %1};" : "=l"(cc) : "f"(c));
+  auto see = [&](float a, float b) {
+    uint64_t x;
+    asm("mov.b64 %0, {%1, %2};" : "=l"(x) : "f"(a), "f"(b));
+    asm("add.rn.f32x2 %0, %0, %1;" : "+l"(x) : "l"(nm));
+    asm("mul.rn.f32x2 %0, %0, %1;" : "+l"(x) : "l"(cc));
+    asm("mov.b64 {%0, %1}, %2;" : "=f"(a), "=f"(b) : "l"(x));
+    a = spec_exp2(a), b = spec_exp2(b);
+    asm("mov.b64 %0, {%1, %2};" : "=l"(x) : "f"(a), "f"(b));
+    asm("add.rn.f32x2 %0, %0, %1;" : "+l"(sum) : "l"(x));
+  };
+#pragma unroll
+  for (int i = 0; i < VL; ++i) {
+    float f[SpecVec<DT>::N];
+    SpecVec<DT>::unpack(raw[i], f);
+#pragma unroll
+    for (int e = 0; e < SpecVec<DT>::N; e += 2) see(f[e], f[e + 1]);
+  }
+  float a, b;
+  asm("mov.b64 {%0, %1}, %2;" : "=f"(a), "=f"(b) : "l"(sum));
+  return a + b;
+}
 
 // Where a row of V logits starts to be 16-byte aligned, and its whole vectors.
 // Part w of the row is vectors [w, w + 1) * SV_PART / N after the `head` logits,
@@ -140,102 +203,124 @@ __global__ void __launch_bounds__(SV_THREADS) spec_stat_kernel(const SpecVerifyA
     const int v = part * (SV_PART / N) + i * 32 + lane;
     raw[i] = v < row.nvec ? __ldg(xv + v) : make_uint4(NI, NI, NI, NI);
   }
-  float extra = -INFINITY;
+  float extra = -INFINITY, extra2 = -INFINITY;           // before and after the row's whole vectors
   const int tail = row.head + row.nvec * N;
   if (part == 0 && lane < row.head) extra = spec_logit(x, lane, DT);
-  float extra2 = -INFINITY;
   if (part == p.parts - 1 && lane < p.V - tail) extra2 = spec_logit(x, tail + lane, DT);
-  float m = fmaxf(extra, extra2);
-#pragma unroll
-  for (int i = 0; i < VL; ++i) {
-    float f[N];
-    SpecVec<DT>::unpack(raw[i], f);
-#pragma unroll
-    for (int e = 0; e < N; ++e) m = fmaxf(m, f[e]);      // ignores NaN
-  }
+  float m = fmaxf(fmaxf(extra, extra2), spec_max<DT, VL>(raw));
 #pragma unroll
   for (int k = 16; k > 0; k >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, k));
   float s = 0.0f;
-  if (m == INFINITY) {                                   // +inf counts as the largest finite number
-    m = spec_clean(m);
-    s = spec_exp2((extra - m) * c) + spec_exp2((extra2 - m) * c);
+  if (c == 0.0f) {
+    // greedy: where the maximum is first
+    int at = 0x7fffffff;
+    const float mc = spec_clean(m);
+    if (extra2 == mc) at = tail + lane;
 #pragma unroll
-    for (int i = 0; i < VL; ++i) {
+    for (int i = VL - 1; i >= 0; --i) {
+      const int v = part * (SV_PART / N) + i * 32 + lane;
       float f[N];
       SpecVec<DT>::unpack(raw[i], f);
 #pragma unroll
-      for (int e = 0; e < N; ++e) s += spec_exp2((spec_clean(f[e]) - m) * c);
+      for (int e = N - 1; e >= 0; --e)
+        if (v < row.nvec && spec_clean(f[e]) == mc) at = row.head + v * N + e;
     }
+    if (extra == mc && lane < row.head) at = lane;
+#pragma unroll
+    for (int k = 16; k > 0; k >>= 1) at = min(at, __shfl_xor_sync(0xffffffffu, at, k));
+    m = mc;
+    s = __int_as_float(at);
   } else if (m != -INFINITY) {
-    s = spec_exp2((extra - m) * c) + spec_exp2((extra2 - m) * c);
+    s = spec_exp2((extra - m) * c) + spec_exp2((extra2 - m) * c) + spec_sum<DT, VL>(raw, m, c);
 #pragma unroll
-    for (int i = 0; i < VL; ++i) {
-      float f[N];
-      SpecVec<DT>::unpack(raw[i], f);
+    for (int k = 16; k > 0; k >>= 1) s += __shfl_xor_sync(0xffffffffu, s, k);
+    if (!(s < INFINITY)) {                               // NaN or +inf among the logits
+      m = spec_clean(m);
+      s = spec_exp2((extra - m) * c) + spec_exp2((extra2 - m) * c);
 #pragma unroll
-      for (int e = 0; e < N; ++e) s += spec_exp2(fmaxf((f[e] - m) * c, -INFINITY));   // NaN: 0
+      for (int i = 0; i < VL; ++i) {
+        float f[N];
+        SpecVec<DT>::unpack(raw[i], f);
+#pragma unroll
+        for (int e = 0; e < N; ++e) s += spec_exp2((spec_clean(f[e]) - m) * c);
+      }
+#pragma unroll
+      for (int k = 16; k > 0; k >>= 1) s += __shfl_xor_sync(0xffffffffu, s, k);
     }
   }
-#pragma unroll
-  for (int k = 16; k > 0; k >>= 1) s += __shfl_xor_sync(0xffffffffu, s, k);
   if (lane == 0) p.part[((long long)b * (2 * p.K + 1) + r) * p.parts + part] = make_float2(m, s);
 }
 
-// Maximum, sum and, for greedy sequences, first place of the maximum of row r, by one warp
-template <int DT>
-__device__ __forceinline__ void spec_join_row(const SpecVerifyArgs& p, int b, int r, float c, float& m, float& s, int& at) {
-  constexpr int N = SpecVec<DT>::N;
+// Maximum, and sum or, for greedy sequences, first place of the maximum of row r, by one warp
+__device__ __forceinline__ void spec_join_row(const SpecVerifyArgs& p, int b, int r, float c, float& m, float& s) {
+  constexpr int HOLD = 6;                          // parts of a lane that are held (6 x 32 x 1024 logits)
   const int lane = threadIdx.x & 31;
   const float2* part = p.part + ((long long)b * (2 * p.K + 1) + r) * p.parts;
+  float2 x[HOLD];
+#pragma unroll
+  for (int k = 0; k < HOLD; ++k) {
+    const int i = lane + k * 32;
+    x[k] = i < p.parts ? __ldcg(part + i) : make_float2(-INFINITY, 0.0f);
+  }
   m = -INFINITY;
-  for (int i = lane; i < p.parts; i += 32) m = fmaxf(m, part[i].x);
+#pragma unroll
+  for (int k = 0; k < HOLD; ++k) m = fmaxf(m, x[k].x);
+  for (int i = lane + HOLD * 32; i < p.parts; i += 32) m = fmaxf(m, __ldcg(part + i).x);
 #pragma unroll
   for (int k = 16; k > 0; k >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, k));
   s = 0.0f;
-  at = 0;
   if (m == -INFINITY) return;
-  int first = 0x7fffffff;
-  for (int i = lane; i < p.parts; i += 32) {
-    const float2 x = part[i];
-    s = fmaf(x.y, spec_exp2((x.x - m) * c), s);
-    if (x.x == m) first = min(first, i);
+  if (c == 0.0f) {
+    int at = 0x7fffffff;
+#pragma unroll
+    for (int k = 0; k < HOLD; ++k)
+      if (x[k].x == m) at = min(at, __float_as_int(x[k].y));
+    for (int i = lane + HOLD * 32; i < p.parts; i += 32) {
+      const float2 y = __ldcg(part + i);
+      if (y.x == m) at = min(at, __float_as_int(y.y));
+    }
+#pragma unroll
+    for (int k = 16; k > 0; k >>= 1) at = min(at, __shfl_xor_sync(0xffffffffu, at, k));
+    s = __int_as_float(at);
+    return;
   }
 #pragma unroll
-  for (int k = 16; k > 0; k >>= 1) {
-    s += __shfl_xor_sync(0xffffffffu, s, k);
-    first = min(first, __shfl_xor_sync(0xffffffffu, first, k));
+  for (int k = 0; k < HOLD; ++k) s = fmaf(x[k].y, spec_exp2((x[k].x - m) * c), s);
+  for (int i = lane + HOLD * 32; i < p.parts; i += 32) {
+    const float2 y = __ldcg(part + i);
+    s = fmaf(y.y, spec_exp2((y.x - m) * c), s);
   }
-  if (c != 0.0f) return;
-  const void* x = spec_row_ptr(p, b, r);
-  const SpecRow row = spec_row<DT>(x, p.V);
-  const int lo = first == 0 ? 0 : row.head + first * SV_PART;
-  const int hi = first == p.parts - 1 ? p.V : min(p.V, row.head + (first + 1) * SV_PART);
-  int best = 0x7fffffff;
-  for (int v = lo + lane; v < hi && best == 0x7fffffff; v += 32)
-    if (spec_logit(x, v, DT) == m) best = v;
 #pragma unroll
-  for (int k = 16; k > 0; k >>= 1) best = min(best, __shfl_xor_sync(0xffffffffu, best, k));
-  at = best;
+  for (int k = 16; k > 0; k >>= 1) s += __shfl_xor_sync(0xffffffffu, s, k);
 }
 
-// One token's race: the residual's and p's own, in ascending order of v per thread
+// The best race so far, in ascending order of tokens per thread
 struct SpecBest {
-  float res, own;
-  int ri, oi;
-  __device__ __forceinline__ void see(float pr, float qr, float e, int v) {
-    const float a = fmaxf(pr - qr, 0.0f) / e, o = pr / e;
-    if (a > res) res = a, ri = v;
-    if (o > own) own = o, oi = v;
+  float v;
+  int at;
+  __device__ __forceinline__ void see(float x, int i) {
+    if (x > v) v = x, at = i;
   }
-  __device__ __forceinline__ void join(float r2, int ri2, float o2, int oi2) {
-    if (r2 > res || (r2 == res && ri2 < ri)) res = r2, ri = ri2;
-    if (o2 > own || (o2 == own && oi2 < oi)) own = o2, oi = oi2;
+  __device__ __forceinline__ void join(float x, int i) {
+    if (x > v || (x == v && i < at)) v = x, at = i;
   }
   __device__ __forceinline__ void join_warp() {
 #pragma unroll
-    for (int k = 16; k > 0; k >>= 1)
-      join(__shfl_xor_sync(0xffffffffu, res, k), __shfl_xor_sync(0xffffffffu, ri, k), __shfl_xor_sync(0xffffffffu, own, k),
-           __shfl_xor_sync(0xffffffffu, oi, k));
+    for (int k = 16; k > 0; k >>= 1) join(__shfl_xor_sync(0xffffffffu, v, k), __shfl_xor_sync(0xffffffffu, at, k));
+  }
+};
+
+__device__ __forceinline__ float spec_rcp(float x) {
+  float y;
+  asm("rcp.approx.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
+
+// A row's probabilities: exp2((x - m) c) inv, 0 for an empty row (inv = 0)
+struct SpecLaw {
+  float m, inv;
+  __device__ __forceinline__ float of(float x, float c) const {
+    return spec_exp2((spec_clean(x) - m) * c) * inv;
   }
 };
 
@@ -244,48 +329,52 @@ __global__ void __launch_bounds__(SV_THREADS) spec_draw_kernel(const SpecVerifyA
   griddep_launch_dependents();
   griddep_wait();
   constexpr int N = SpecVec<DT>::N;
-  extern __shared__ float sv_rows[];               // [2 K + 1][3]: maximum, 1 / sum, place of the maximum
+  extern __shared__ float sv_rows[];               // [2 K + 1][2]: maximum, sum (greedy: place of the maximum)
   __shared__ SpecBest s_best[SV_WARPS];
   __shared__ int s_kept, s_last;
   __shared__ bool s_bad;
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   const int b = blockIdx.x / p.chunks, chunk = blockIdx.x - b * p.chunks;
   const int d = spec_count(p, b);
-  const float c = spec_scale(spec_temperature(p, b));
+  const float T = spec_temperature(p, b), c = spec_scale(T);
   const long long* xs = p.tokens + b * p.ld_x;
+  // the first warp fetches what decides about the first 32 drafts while the others join the rows' parts
+  long long x0 = -1;
+  float u0 = 0.0f, t0 = 0.0f, d0 = 0.0f;
+  auto fetch = [&](int i) {
+    x0 = i < d ? xs[i] : 0;
+    if (i < d && x0 >= 0 && x0 < p.V) {
+      t0 = load_f(spec_row_ptr(p, b, i), x0, DT);
+      if (p.draft) d0 = load_f(spec_row_ptr(p, b, p.K + 1 + i), x0, DT);
+      u0 = p.uniform[b * p.ld_u + i];
+    }
+  };
+  if (warp == 0) fetch(lane);
   const int R = d + 1 + (p.draft ? d : 0);
-  for (int k = warp; k < R; k += SV_WARPS) {
+  for (int k = SV_WARPS - 1 - warp; k < R; k += SV_WARPS) {
     const int r = k <= d ? k : p.K + k - d;
     float m, s;
-    int at;
-    spec_join_row<DT>(p, b, r, c, m, s, at);
-    if (lane == 0) sv_rows[r * 3] = m, sv_rows[r * 3 + 1] = s, sv_rows[r * 3 + 2] = __int_as_float(at);
+    spec_join_row(p, b, r, c, m, s);
+    if (lane == 0) sv_rows[r * 2] = m, sv_rows[r * 2 + 1] = s;
   }
   __syncthreads();
   // the probability of token v, whose logit is x, in row r
   auto prob = [&](int r, float x, int v) {
-    const float m = sv_rows[r * 3];
+    const float m = sv_rows[r * 2], s = sv_rows[r * 2 + 1];
     if (m == -INFINITY) return 0.0f;
-    if (c == 0.0f) return v == __float_as_int(sv_rows[r * 3 + 2]) ? 1.0f : 0.0f;
-    return spec_exp2((spec_clean(x) - m) * c) / sv_rows[r * 3 + 1];
+    if (c == 0.0f) return v == __float_as_int(s) ? 1.0f : 0.0f;
+    return spec_exp2((spec_clean(x) - m) * c) / s;
   };
   if (warp == 0) {
     int kept = d;
     bool bad = false;
     for (int i0 = 0; i0 < d && kept == d; i0 += 32) {
       const int i = i0 + lane;
-      bool ok = true, out = false;
-      if (i < d) {
-        const long long x = xs[i];
-        out = x < 0 || x >= p.V;
-        if (out) {
-          ok = false;
-        } else {
-          const float pr = prob(i, load_f(spec_row_ptr(p, b, i), x, DT), (int)x);
-          const float qr = p.draft ? prob(p.K + 1 + i, load_f(spec_row_ptr(p, b, p.K + 1 + i), x, DT), (int)x) : 1.0f;
-          ok = p.uniform[b * p.ld_u + i] * qr < pr;
-        }
-      }
+      if (i0 > 0) fetch(i);
+      const bool out = i < d && (x0 < 0 || x0 >= p.V);
+      bool ok = !out;
+      if (i < d && ok)
+        ok = u0 * (p.draft ? prob(p.K + 1 + i, d0, (int)x0) : 1.0f) < prob(i, t0, (int)x0);
       const uint32_t no = __ballot_sync(0xffffffffu, !ok), ob = __ballot_sync(0xffffffffu, out);
       if (no) {
         kept = i0 + __ffs(no) - 1;
@@ -301,82 +390,97 @@ __global__ void __launch_bounds__(SV_THREADS) spec_draw_kernel(const SpecVerifyA
   __syncthreads();
   const int a = s_kept;
   const bool minus = a < d && !s_bad;
-  SpecBest best = {-1.0f, -1.0f, 0x7fffffff, 0x7fffffff};
-  if (c != 0.0f) {
-    const void* tr = spec_row_ptr(p, b, a);
-    const void* dr = minus && p.draft ? spec_row_ptr(p, b, p.K + 1 + a) : nullptr;
-    const int hit = minus && !p.draft ? (int)xs[a] : -1;
-    const float* e = p.noise + b * p.ld_n;
-    const float mt = sv_rows[a * 3], it = mt == -INFINITY ? 0.0f : 1.0f / sv_rows[a * 3 + 1];
-    const float md = dr ? sv_rows[(p.K + 1 + a) * 3] : -INFINITY, id = md == -INFINITY ? 0.0f : 1.0f / sv_rows[(p.K + 1 + a) * 3 + 1];
-    const float mtu = mt == -INFINITY ? 0.0f : mt, mdu = md == -INFINITY ? 0.0f : md;
+  // the row that is drawn from, less (minus) the draft's
+  const void* tr = spec_row_ptr(p, b, a);
+  const void* dr = minus && p.draft ? spec_row_ptr(p, b, p.K + 1 + a) : nullptr;
+  const int hit = minus && !p.draft ? (int)xs[a] : -1;
+  const float* e = p.noise + b * p.ld_n;
+  auto law = [&](int r) {
+    const float m = sv_rows[r * 2];
+    return m == -INFINITY ? SpecLaw{0.0f, 0.0f} : SpecLaw{m, 1.0f / sv_rows[r * 2 + 1]};
+  };
+  const SpecLaw pt = law(a), pd = dr ? law(p.K + 1 + a) : SpecLaw{0.0f, 0.0f};
+  SpecBest best = {-1.0f, 0x7fffffff};
+  // tokens lo .. hi - 1, a thread's in ascending order
+  auto race = [&](int lo, int hi, bool less) {
     auto see = [&](float x, float y, float noise, int v) {
-      const float pr = spec_exp2((spec_clean(x) - mtu) * c) * it;
-      const float qr = dr ? spec_exp2((spec_clean(y) - mdu) * c) * id : v == hit ? 1.0f : 0.0f;
-      best.see(pr, qr, noise, v);
+      const float q = less ? (dr ? pd.of(y, c) : v == hit ? 1.0f : 0.0f) : 0.0f;
+      best.see(fmaxf(pt.of(x, c) - q, 0.0f) * spec_rcp(noise), v);
     };
-    const int lo = chunk * SV_CHUNK, hi = min(p.V, lo + SV_CHUNK);
     auto aligned = [](const void* q) { return (reinterpret_cast<uintptr_t>(q) & 15) == 0; };
+    int vec_hi = lo;
     if (aligned(tr) && aligned(e) && (!dr || aligned(dr))) {
-      const int vec_hi = hi - (hi - lo) % N;
+      vec_hi = hi - (hi - lo) % N;
+#pragma unroll 2
       for (int v0 = lo + tid * N; v0 < vec_hi; v0 += SV_THREADS * N) {
-        float x[N], y[N];
-        SpecVec<DT>::unpack(*reinterpret_cast<const uint4*>(reinterpret_cast<const char*>(tr) + (long long)v0 * (16 / N)), x);
-        const uint4 yr = dr ? *reinterpret_cast<const uint4*>(reinterpret_cast<const char*>(dr) + (long long)v0 * (16 / N))
-                            : make_uint4(0, 0, 0, 0);
-        SpecVec<DT>::unpack(yr, y);
-        float4 n4[N / 4];
-#pragma unroll
-        for (int k = 0; k < N / 4; ++k) n4[k] = *reinterpret_cast<const float4*>(e + v0 + 4 * k);
+        float x[N], y[N], z[N];
+        SpecVec<DT>::unpack(__ldg(reinterpret_cast<const uint4*>(reinterpret_cast<const char*>(tr) + (long long)v0 * (16 / N))), x);
+        SpecVec<DT>::unpack(dr ? __ldg(reinterpret_cast<const uint4*>(reinterpret_cast<const char*>(dr) + (long long)v0 * (16 / N)))
+                               : make_uint4(0, 0, 0, 0), y);
 #pragma unroll
         for (int k = 0; k < N / 4; ++k) {
-          see(x[4 * k], y[4 * k], n4[k].x, v0 + 4 * k);
-          see(x[4 * k + 1], y[4 * k + 1], n4[k].y, v0 + 4 * k + 1);
-          see(x[4 * k + 2], y[4 * k + 2], n4[k].z, v0 + 4 * k + 2);
-          see(x[4 * k + 3], y[4 * k + 3], n4[k].w, v0 + 4 * k + 3);
+          const float4 f = __ldg(reinterpret_cast<const float4*>(e + v0) + k);
+          z[4 * k] = f.x, z[4 * k + 1] = f.y, z[4 * k + 2] = f.z, z[4 * k + 3] = f.w;
         }
+#pragma unroll
+        for (int k = 0; k < N; ++k) see(x[k], y[k], z[k], v0 + k);
       }
-      for (int v = vec_hi + tid; v < hi; v += SV_THREADS) see(load_f(tr, v, DT), dr ? load_f(dr, v, DT) : 0.0f, e[v], v);
-    } else {
-      for (int v = lo + tid; v < hi; v += SV_THREADS) see(load_f(tr, v, DT), dr ? load_f(dr, v, DT) : 0.0f, e[v], v);
     }
+#pragma unroll 4
+    for (int v = vec_hi + tid; v < hi; v += SV_THREADS) see(load_f(tr, v, DT), dr ? load_f(dr, v, DT) : 0.0f, e[v], v);
+  };
+  if (c != 0.0f) {
+    race(chunk * SV_CHUNK, min(p.V, (chunk + 1) * SV_CHUNK), minus);
     best.join_warp();
     if (lane == 0) s_best[warp] = best;
     __syncthreads();
   }
   if (tid == 0) {
     if (c != 0.0f) {
-      for (int w = 1; w < SV_WARPS; ++w) best.join(s_best[w].res, s_best[w].ri, s_best[w].own, s_best[w].oi);
-      p.cand[(long long)b * p.chunks + chunk] = make_float4(best.res, __int_as_float(best.ri), best.own, __int_as_float(best.oi));
+      for (int w = 1; w < SV_WARPS; ++w) best.join(s_best[w].v, s_best[w].at);
+      p.cand[(long long)b * p.chunks + chunk] = make_float2(best.v, __int_as_float(best.at));
     }
     __threadfence();
     s_last = atomicAdd(p.done + b, 1) == p.chunks - 1;
+    __threadfence();
   }
   __syncthreads();
-  if (!s_last || warp != 0) return;
+  if (!s_last) return;
   // the sequence's last CTA: the best of all chunks, and the outputs
-  __threadfence();
-  int drawn = __float_as_int(sv_rows[a * 3 + 2]);
-  if (c != 0.0f) {
-    best = {-1.0f, -1.0f, 0x7fffffff, 0x7fffffff};
+  int drawn = __float_as_int(sv_rows[a * 2 + 1]);
+  if (sv_rows[a * 2] == -INFINITY) {
+    drawn = 0;
+  } else if (c != 0.0f) {
+    best = {-1.0f, 0x7fffffff};
     for (int k = lane; k < p.chunks; k += 32) {
-      const float4 x = __ldcg(p.cand + (long long)b * p.chunks + k);
-      best.join(x.x, __float_as_int(x.y), x.z, __float_as_int(x.w));
+      const float2 x = __ldcg(p.cand + (long long)b * p.chunks + k);
+      best.join(x.x, __float_as_int(x.y));
     }
     best.join_warp();
-    drawn = best.res > 0.0f ? best.ri : best.oi;
+    if (minus && !(best.v > 0.0f)) {
+      // p nowhere over q: drawn from p (every thread has the same `best` here)
+      best = {-1.0f, 0x7fffffff};
+      race(0, p.V, false);
+      best.join_warp();
+      __syncthreads();
+      if (lane == 0) s_best[warp] = best;
+      __syncthreads();
+      for (int w = 0; w < SV_WARPS; ++w) best.join(s_best[w].v, s_best[w].at);
+    }
+    drawn = best.at;
   }
+  if (warp != 0) return;
   for (int i = lane; i <= p.K; i += 32) {
     const int v = i < a ? (int)xs[i] : drawn;
     float lp = 0.0f;
     if (i <= a) {
-      const float m = sv_rows[i * 3];
+      const float m = sv_rows[i * 2], s = sv_rows[i * 2 + 1];
       if (m == -INFINITY)
         lp = -INFINITY;
       else if (c == 0.0f)
-        lp = v == __float_as_int(sv_rows[i * 3 + 2]) ? 0.0f : -INFINITY;
+        lp = v == __float_as_int(s) ? 0.0f : -INFINITY;
       else
-        lp = (spec_logit(spec_row_ptr(p, b, i), v, DT) - m) / fmaxf(spec_temperature(p, b), 1e-30f) - logf(sv_rows[i * 3 + 1]);
+        lp = (spec_logit(spec_row_ptr(p, b, i), v, DT) - m) / fmaxf(T, 1e-30f) - logf(s);
     }
     p.out_tokens[(long long)b * (p.K + 1) + i] = i <= a ? v : -1;
     p.out_logprobs[(long long)b * (p.K + 1) + i] = lp;
