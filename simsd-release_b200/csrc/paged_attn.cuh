@@ -34,16 +34,9 @@
 // with weight 0 in the second product; where its value is not finite (0 x inf), the
 // unit's product runs row by row with the hidden keys zeroed instead.
 #pragma once
-#include "sm100.cuh"
+#include "paged.cuh"
 
 namespace simsd {
-
-// x / d for 0 <= x < 2^31: x * magic >> shift, magic the reciprocal rounded up
-struct PagedDiv {
-  uint32_t magic;
-  int shift;
-  __device__ __forceinline__ int operator()(int x) const { return (int)((uint64_t)(uint32_t)x * magic >> shift); }
-};
 
 struct PagedAttnArgs {
   const void* q;            // [B, L, Hq, D]

@@ -162,10 +162,13 @@ int simsd_paged_append(const void* qkv, int64_t ldqkv, int T, int Hq, int Hk, in
   a.Hk = Hk;
   a.R = rotary_dim;
   a.page_size = page_size;
-  a.dtype = dtype;
+  a.page_div = paged_div(page_size);
   a.eps = eps;
-  return head_dim == 64 ? launch_on(paged_append_kernel<64>, T, PA_THREADS, 0, stream, false, a)
-                        : launch_on(paged_append_kernel<128>, T, PA_THREADS, 0, stream, false, a);
+  if (dtype == SIMSD_BF16)
+    return head_dim == 64 ? launch_on(paged_append_kernel<64, true>, T, PA_THREADS, 0, stream, false, a)
+                          : launch_on(paged_append_kernel<128, true>, T, PA_THREADS, 0, stream, false, a);
+  return head_dim == 64 ? launch_on(paged_append_kernel<64, false>, T, PA_THREADS, 0, stream, false, a)
+                        : launch_on(paged_append_kernel<128, false>, T, PA_THREADS, 0, stream, false, a);
 }
 
 size_t simsd_paged_attention_workspace_size(int B, int L, int Hq, int Hk, int head_dim) {
