@@ -555,7 +555,8 @@ int simsd_paged_attention(const void* q, const void* k_cache, const void* v_cach
  * draft_tokens [B, K] (ld_x), uniform [B, K] (ld_u), noise [B, V] (ld_n).  NaN
  * logits count as -inf, +inf as the largest finite number.  A drafted token
  * outside [0, V) is refused (SIMSD_DEV_ERR_BAD_INDEX), the next one drawn from p.
- * Replaces mrs_verify (speculative_decoding/mrs.py:14-108) for a batch.
+ * B <= 65535, K <= 1024 (more: SIMSD_ERR_UNSUPPORTED).  Replaces mrs_verify
+ * (speculative_decoding/mrs.py:14-108) for a batch.
  */
 size_t simsd_speculative_verify_workspace_size(int B, int K, int V);
 int simsd_speculative_verify(const void* target_logits, int64_t ldt_b, int64_t ldt_r, const void* draft_logits,

@@ -20,16 +20,16 @@ constexpr int kMaxDev = 64;
 std::mutex g_attr_mu;
 
 inline size_t align256(size_t v) { return (v + 255) & ~size_t(255); }
+inline long long cdiv(long long a, long long b) { return (a + b - 1) / b; }
 inline bool al16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15) == 0; }
 
 // Launch on `s`; as a programmatic dependent of the kernel before it on the
 // stream when `dependent` (the second kernel of one call) or SIMSD_LAUNCH_PDL is
 // set.  Every kernel here starts with griddepcontrol.wait.
 template <typename... KArgs, typename... Args>
-int launch_on(void (*kern)(KArgs...), long long grid, int block, size_t smem, void* s, bool dependent, Args&&... args) {
-  if (grid > 0x7fffffffLL) return SIMSD_ERR_UNSUPPORTED;
+int launch_on(void (*kern)(KArgs...), dim3 grid, int block, size_t smem, void* s, bool dependent, Args&&... args) {
   cudaLaunchConfig_t cfg = {};
-  cfg.gridDim = dim3((unsigned)grid);
+  cfg.gridDim = grid;
   cfg.blockDim = dim3((unsigned)block);
   cfg.dynamicSmemBytes = smem;
   cfg.stream = (cudaStream_t)s;
@@ -88,14 +88,22 @@ int allow_smem(F* kern, int bytes, bool* done) {
   return SIMSD_OK;
 }
 
+// How verification splits its rows.  A warp takes 4 blocks of 1024 logits where that
+// still leaves 32 warps per SM, else one (few rows: latency).  The race runs in about
+// two CTAs per SM, each a multiple of SV_CHUNK tokens of one sequence: every CTA of a
+// sequence joins its rows' parts anew.
 struct SpecPlan {
-  int parts, chunks;
+  int blocks, parts, chunk, chunks;
   size_t cand_at, done_at, bytes;
 };
 SpecPlan spec_plan(int B, int K, int V) {
   SpecPlan p;
-  p.parts = (V + SV_PART - 1) / SV_PART;
-  p.chunks = (V + SV_CHUNK - 1) / SV_CHUNK;
+  const int sms = simsd_device_sm_count() > 0 ? simsd_device_sm_count() : 148;
+  const long long all = (long long)B * (2 * K + 1) * V;
+  p.blocks = all >= (long long)sms * 32 * 4 * SV_BLOCK ? 4 : 1;
+  p.parts = (int)cdiv(V, p.blocks * SV_BLOCK);
+  p.chunk = (int)std::min<long long>(cdiv(cdiv((long long)B * V, 2 * sms), SV_CHUNK), cdiv(V, SV_CHUNK)) * SV_CHUNK;
+  p.chunks = (int)cdiv(V, p.chunk);
   p.cand_at = align256((size_t)B * (2 * K + 1) * p.parts * sizeof(float2));
   p.done_at = p.cand_at + align256((size_t)B * p.chunks * sizeof(float2));
   p.bytes = p.done_at + align256((size_t)B * sizeof(int));
@@ -104,10 +112,10 @@ SpecPlan spec_plan(int B, int K, int V) {
 
 template <int DT>
 int verify_drafts(const SpecVerifyArgs& a, void* stream) {
-  const long long rows = (long long)a.B * (a.draft ? 2 * a.K + 1 : a.K + 1);
-  int rc = launch_on(spec_stat_kernel<DT>, rows * ((a.parts + SV_WARPS - 1) / SV_WARPS), SV_THREADS, 0, stream, false, a);
+  const dim3 grid((unsigned)cdiv(a.parts, SV_WARPS), (unsigned)a.B, (unsigned)(a.draft ? 2 * a.K + 1 : a.K + 1));
+  int rc = launch_on(spec_stat_kernel<DT>, grid, SV_THREADS, 0, stream, false, a);
   if (rc != SIMSD_OK) return rc;
-  return launch_on(spec_draw_kernel<DT>, (long long)a.B * a.chunks, SV_THREADS, (size_t)(2 * a.K + 1) * 2 * sizeof(float),
+  return launch_on(spec_draw_kernel<DT>, dim3((unsigned)(a.B * a.chunks)), SV_THREADS, (size_t)(2 * a.K + 1) * 2 * sizeof(float),
                    stream, true, a);
 }
 
@@ -117,7 +125,7 @@ int attend(const PagedAttnArgs& a, const PagedPlan& pl, void* stream) {
   constexpr int smem = PatSmem<D, NT>::BYTES;
   int rc = allow_smem(paged_attention_kernel<D, NT, BF>, smem, done);
   if (rc != SIMSD_OK) return rc;
-  return launch_on(paged_attention_kernel<D, NT, BF>, pl.grid, PAT_THREADS, smem, stream, false, a);
+  return launch_on(paged_attention_kernel<D, NT, BF>, dim3((unsigned)pl.grid), PAT_THREADS, smem, stream, false, a);
 }
 
 }  // namespace
@@ -165,10 +173,10 @@ int simsd_paged_append(const void* qkv, int64_t ldqkv, int T, int Hq, int Hk, in
   a.page_div = paged_div(page_size);
   a.eps = eps;
   if (dtype == SIMSD_BF16)
-    return head_dim == 64 ? launch_on(paged_append_kernel<64, true>, T, PA_THREADS, 0, stream, false, a)
-                          : launch_on(paged_append_kernel<128, true>, T, PA_THREADS, 0, stream, false, a);
-  return head_dim == 64 ? launch_on(paged_append_kernel<64, false>, T, PA_THREADS, 0, stream, false, a)
-                        : launch_on(paged_append_kernel<128, false>, T, PA_THREADS, 0, stream, false, a);
+    return head_dim == 64 ? launch_on(paged_append_kernel<64, true>, dim3((unsigned)T), PA_THREADS, 0, stream, false, a)
+                          : launch_on(paged_append_kernel<128, true>, dim3((unsigned)T), PA_THREADS, 0, stream, false, a);
+  return head_dim == 64 ? launch_on(paged_append_kernel<64, false>, dim3((unsigned)T), PA_THREADS, 0, stream, false, a)
+                        : launch_on(paged_append_kernel<128, false>, dim3((unsigned)T), PA_THREADS, 0, stream, false, a);
 }
 
 size_t simsd_paged_attention_workspace_size(int B, int L, int Hq, int Hk, int head_dim) {
@@ -254,7 +262,7 @@ int simsd_speculative_verify(const void* target_logits, int64_t ldt_b, int64_t l
                              int64_t* tokens, int64_t* accepted, float* logprobs, void* workspace,
                              size_t workspace_bytes, int* err_word, void* stream) {
   if (B < 0 || K < 0 || V < 1) return SIMSD_ERR_SHAPE;
-  if (K > 1024 || V > 0x7fff0000) return SIMSD_ERR_UNSUPPORTED;
+  if (B > 65535 || K > 1024 || V > 0x7fff0000) return SIMSD_ERR_UNSUPPORTED;
   if (dtype != SIMSD_BF16 && dtype != SIMSD_F16 && dtype != SIMSD_F32) return SIMSD_ERR_DTYPE;
   if (B == 0) return SIMSD_OK;
   if (!target_logits || !noise || !tokens || !accepted || !logprobs) return SIMSD_ERR_SHAPE;
@@ -274,10 +282,13 @@ int simsd_speculative_verify(const void* target_logits, int64_t ldt_b, int64_t l
   a.out_logprobs = logprobs;
   const SpecPlan pl = spec_plan(B, K, V);
   uint8_t* ws = reinterpret_cast<uint8_t*>(workspace);
+  if ((long long)B * pl.chunks > 0x7fffffffLL) return SIMSD_ERR_UNSUPPORTED;
   a.part = reinterpret_cast<float2*>(ws);
   a.cand = reinterpret_cast<float2*>(ws + pl.cand_at);
   a.done = reinterpret_cast<int*>(ws + pl.done_at);
+  a.blocks = pl.blocks;
   a.parts = pl.parts;
+  a.chunk = pl.chunk;
   a.chunks = pl.chunks;
   a.err = err_word;
   a.ldt_b = ldt_b;

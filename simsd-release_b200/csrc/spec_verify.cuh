@@ -13,9 +13,9 @@
 // Ties go to the lowest token.  A residual that is nowhere positive (p <= q
 // everywhere) draws from p.
 //
-// Two kernels.  spec_stat_kernel reads every row once: a warp takes 1024 logits,
-// keeps them in registers between their maximum and the sum of their exponentials,
-// and leaves (max, sum) as the row's partial.  spec_draw_kernel joins the partials,
+// Two kernels.  spec_stat_kernel reads every row once: a warp takes `blocks` times
+// 1024 logits, keeps each block in registers between its maximum and the sum of its
+// exponentials, the next one on its way, and leaves (max, sum) as the row's part.  spec_draw_kernel joins the partials,
 // decides how many drafts are kept (every CTA of the sequence for itself: a few KB
 // from L2) and races the one row that is drawn from; the sequence's last CTA to
 // finish writes its outputs.  HBM bounds both; the first also runs one exponential
@@ -46,12 +46,12 @@ struct SpecVerifyArgs {
   int* done;                // [B]: CTAs of the sequence that have finished, zeroed by the first kernel
   int* err;
   long long ldt_b, ldt_r, ldd_b, ldd_r, ld_x, ld_u, ld_n;
-  int B, K, V, parts, chunks, dtype;
+  int B, K, V, blocks, parts, chunk, chunks, dtype;
 };
 
 constexpr int SV_THREADS = 256, SV_WARPS = SV_THREADS / 32;
-constexpr int SV_PART = 1024;                      // logits of one partial (one warp)
-constexpr int SV_CHUNK = 8192;                     // tokens that one CTA races
+constexpr int SV_BLOCK = 1024;                     // logits that a warp holds at a time
+constexpr int SV_CHUNK = 2048;                     // tokens that a CTA races at a time
 
 __device__ __forceinline__ float spec_clean(float v) { return fminf(fmaxf(v, -INFINITY), 3.402823466e+38f); }
 __device__ __forceinline__ float spec_logit(const void* p, long long i, int dtype) {
@@ -155,8 +155,8 @@ __device__ __forceinline__ float spec_sum(const uint4 (&raw)[VL], float m, float
 }
 
 // Where a row of V logits starts to be 16-byte aligned, and its whole vectors.
-// Part w of the row is vectors [w, w + 1) * SV_PART / N after the `head` logits,
-// which belong to part 0; those after the last whole vector to the last part.
+// Part w of the row is vectors [w, w + 1) * blocks * SV_BLOCK / N after the `head`
+// logits, which belong to part 0; those after the last whole vector to the last part.
 struct SpecRow {
   int head, nvec;
 };
@@ -176,84 +176,99 @@ __device__ __forceinline__ const void* spec_row_ptr(const SpecVerifyArgs& p, int
                   : reinterpret_cast<const char*>(p.draft) + (b * p.ldd_b + (r - p.K - 1) * p.ldd_r) * es;
 }
 
+// Grid: x parts of a row, y sequences, z rows
 template <int DT>
 __global__ void __launch_bounds__(SV_THREADS) spec_stat_kernel(const SpecVerifyArgs p) {
   griddep_launch_dependents();
   griddep_wait();
-  constexpr int N = SpecVec<DT>::N, VL = SV_PART / N / 32;     // vectors per lane
-  const int lane = threadIdx.x & 31;
-  const int per_row = (p.parts + SV_WARPS - 1) / SV_WARPS;
-  const int part = (int)(blockIdx.x % per_row) * SV_WARPS + (threadIdx.x >> 5);
-  const int rest = blockIdx.x / per_row;
-  const int b = rest % p.B, back = rest / p.B;
+  constexpr int N = SpecVec<DT>::N, VL = SV_BLOCK / N / 32;    // vectors per lane
+  const int lane = threadIdx.x & 31, b = blockIdx.y, back = blockIdx.z;
+  const int part = blockIdx.x * SV_WARPS + (threadIdx.x >> 5);
   // rows last to first: target K, then target and draft K - 1, ...
   const int r = !p.draft ? p.K - back : back & 1 ? p.K - 1 - back / 2 : back == 0 ? p.K : 2 * p.K + 1 - back / 2;
-  if (blockIdx.x % per_row == 0 && threadIdx.x == 0 && r == 0) p.done[b] = 0;
+  if (blockIdx.x == 0 && threadIdx.x == 0 && r == 0) p.done[b] = 0;
   const int d = spec_count(p, b);
   if (part >= p.parts || (r <= p.K ? r > d : r - p.K - 1 >= d)) return;
   const float c = spec_scale(spec_temperature(p, b));
   const void* x = spec_row_ptr(p, b, r);
   const SpecRow row = spec_row<DT>(x, p.V);
-  const uint4* xv = reinterpret_cast<const uint4*>(reinterpret_cast<const char*>(x) + row.head * (16 / N));
-  uint4 raw[VL];
+  const uint4* xv = reinterpret_cast<const uint4*>(reinterpret_cast<const char*>(x) + row.head * (16 / N)) + lane;
   // -inf in the type's own bits, where there is no vector
   constexpr uint32_t NI = DT == 0 ? 0xff80ff80u : DT == 1 ? 0xfc00fc00u : 0xff800000u;
+  uint4 raw[VL], next[VL];
+  int v = part * p.blocks * (SV_BLOCK / N);                    // the block's first vector
+  auto fetch = [&](int v0) {
+    const uint4* src = xv + v0;
+    if (v0 + SV_BLOCK / N <= row.nvec) {
 #pragma unroll
-  for (int i = 0; i < VL; ++i) {
-    const int v = part * (SV_PART / N) + i * 32 + lane;
-    raw[i] = v < row.nvec ? __ldg(xv + v) : make_uint4(NI, NI, NI, NI);
-  }
+      for (int i = 0; i < VL; ++i) next[i] = __ldg(src + i * 32);
+    } else {
+#pragma unroll
+      for (int i = 0; i < VL; ++i) next[i] = v0 + i * 32 + lane < row.nvec ? __ldg(src + i * 32) : make_uint4(NI, NI, NI, NI);
+    }
+  };
+  fetch(v);
   float extra = -INFINITY, extra2 = -INFINITY;           // before and after the row's whole vectors
   const int tail = row.head + row.nvec * N;
   if (part == 0 && lane < row.head) extra = spec_logit(x, lane, DT);
   if (part == p.parts - 1 && lane < p.V - tail) extra2 = spec_logit(x, tail + lane, DT);
-  float m = fmaxf(fmaxf(extra, extra2), spec_max<DT, VL>(raw));
+  auto warp_max = [](float m) {
 #pragma unroll
-  for (int k = 16; k > 0; k >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, k));
-  float s = 0.0f;
-  if (c == 0.0f) {
-    // greedy: where the maximum is first
-    int at = 0x7fffffff;
-    const float mc = spec_clean(m);
-    if (extra2 == mc) at = tail + lane;
+    for (int k = 16; k > 0; k >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, k));
+    return m;
+  };
+  float m = spec_clean(warp_max(fmaxf(extra, extra2))), s = 0.0f;   // s: this lane's
+  int at = 0x7fffffff;                                   // greedy: the first place of m that this lane saw
+  if (m != -INFINITY) {
+    s = spec_exp2((extra - m) * c) + spec_exp2((extra2 - m) * c);
+    if (extra2 == m) at = tail + lane;
+    if (extra == m) at = lane;
+  }
+  for (int n = 0; n < p.blocks && v < row.nvec; ++n, v += SV_BLOCK / N) {
 #pragma unroll
-    for (int i = VL - 1; i >= 0; --i) {
-      const int v = part * (SV_PART / N) + i * 32 + lane;
-      float f[N];
-      SpecVec<DT>::unpack(raw[i], f);
+    for (int i = 0; i < VL; ++i) raw[i] = next[i];
+    if (n + 1 < p.blocks) fetch(v + SV_BLOCK / N);
+    const float m2 = warp_max(spec_max<DT, VL>(raw)), mn = fmaxf(m, spec_clean(m2));
+    if (mn == -INFINITY) continue;
+    if (mn > m) s *= spec_exp2((m - mn) * c), at = 0x7fffffff;
+    m = mn;
+    if (c == 0.0f) {
 #pragma unroll
-      for (int e = N - 1; e >= 0; --e)
-        if (v < row.nvec && spec_clean(f[e]) == mc) at = row.head + v * N + e;
+      for (int i = VL - 1; i >= 0; --i) {
+        const int vi = v + i * 32 + lane;
+        float f[N];
+        SpecVec<DT>::unpack(raw[i], f);
+#pragma unroll
+        for (int e = N - 1; e >= 0; --e)
+          if (spec_clean(f[e]) == m) at = min(at, row.head + vi * N + e);
+      }
+      continue;
     }
-    if (extra == mc && lane < row.head) at = lane;
-#pragma unroll
-    for (int k = 16; k > 0; k >>= 1) at = min(at, __shfl_xor_sync(0xffffffffu, at, k));
-    m = mc;
-    s = __int_as_float(at);
-  } else if (m != -INFINITY) {
-    s = spec_exp2((extra - m) * c) + spec_exp2((extra2 - m) * c) + spec_sum<DT, VL>(raw, m, c);
-#pragma unroll
-    for (int k = 16; k > 0; k >>= 1) s += __shfl_xor_sync(0xffffffffu, s, k);
-    if (!(s < INFINITY)) {                               // NaN or +inf among the logits
-      m = spec_clean(m);
-      s = spec_exp2((extra - m) * c) + spec_exp2((extra2 - m) * c);
+    float add = spec_sum<DT, VL>(raw, m, c);
+    if (!(add < INFINITY)) {                             // NaN or +inf among the lane's logits
+      add = 0.0f;
 #pragma unroll
       for (int i = 0; i < VL; ++i) {
         float f[N];
         SpecVec<DT>::unpack(raw[i], f);
 #pragma unroll
-        for (int e = 0; e < N; ++e) s += spec_exp2((spec_clean(f[e]) - m) * c);
+        for (int e = 0; e < N; ++e) add += spec_exp2((spec_clean(f[e]) - m) * c);
       }
-#pragma unroll
-      for (int k = 16; k > 0; k >>= 1) s += __shfl_xor_sync(0xffffffffu, s, k);
     }
+    s += add;
   }
-  if (lane == 0) p.part[((long long)b * (2 * p.K + 1) + r) * p.parts + part] = make_float2(m, s);
+#pragma unroll
+  for (int k = 16; k > 0; k >>= 1) {
+    s += __shfl_xor_sync(0xffffffffu, s, k);
+    at = min(at, __shfl_xor_sync(0xffffffffu, at, k));
+  }
+  if (lane == 0)
+    p.part[((long long)b * (2 * p.K + 1) + r) * p.parts + part] = make_float2(m, c == 0.0f ? __int_as_float(at) : s);
 }
 
 // Maximum, and sum or, for greedy sequences, first place of the maximum of row r, by one warp
 __device__ __forceinline__ void spec_join_row(const SpecVerifyArgs& p, int b, int r, float c, float& m, float& s) {
-  constexpr int HOLD = 6;                          // parts of a lane that are held (6 x 32 x 1024 logits)
+  constexpr int HOLD = 3;                          // parts that a lane holds
   const int lane = threadIdx.x & 31;
   const float2* part = p.part + ((long long)b * (2 * p.K + 1) + r) * p.parts;
   float2 x[HOLD];
@@ -426,11 +441,11 @@ __global__ void __launch_bounds__(SV_THREADS) spec_draw_kernel(const SpecVerifyA
         for (int k = 0; k < N; ++k) see(x[k], y[k], z[k], v0 + k);
       }
     }
-#pragma unroll 4
+#pragma unroll 8
     for (int v = vec_hi + tid; v < hi; v += SV_THREADS) see(load_f(tr, v, DT), dr ? load_f(dr, v, DT) : 0.0f, e[v], v);
   };
   if (c != 0.0f) {
-    race(chunk * SV_CHUNK, min(p.V, (chunk + 1) * SV_CHUNK), minus);
+    race(chunk * p.chunk, min(p.V, (chunk + 1) * p.chunk), minus);
     best.join_warp();
     if (lane == 0) s_best[warp] = best;
     __syncthreads();
