@@ -90,7 +90,7 @@ int allow_smem(F* kern, int bytes, bool* done) {
 
 // How verification splits its rows.  A warp takes 4 blocks of 1024 logits where that
 // still leaves 32 warps per SM, else one (few rows: latency).  The race runs in about
-// two CTAs per SM, each a multiple of SV_CHUNK tokens of one sequence: every CTA of a
+// four CTAs per SM, each a multiple of SV_CHUNK tokens of one sequence: every CTA of a
 // sequence joins its rows' parts anew.
 struct SpecPlan {
   int blocks, parts, chunk, chunks;
@@ -102,7 +102,7 @@ SpecPlan spec_plan(int B, int K, int V) {
   const long long all = (long long)B * (2 * K + 1) * V;
   p.blocks = all >= (long long)sms * 32 * 4 * SV_BLOCK ? 4 : 1;
   p.parts = (int)cdiv(V, p.blocks * SV_BLOCK);
-  p.chunk = (int)std::min<long long>(cdiv(cdiv((long long)B * V, 2 * sms), SV_CHUNK), cdiv(V, SV_CHUNK)) * SV_CHUNK;
+  p.chunk = (int)std::min<long long>(cdiv(cdiv((long long)B * V, 4 * sms), SV_CHUNK), cdiv(V, SV_CHUNK)) * SV_CHUNK;
   p.chunks = (int)cdiv(V, p.chunk);
   p.cand_at = align256((size_t)B * (2 * K + 1) * p.parts * sizeof(float2));
   p.done_at = p.cand_at + align256((size_t)B * p.chunks * sizeof(float2));

@@ -178,7 +178,7 @@ __device__ __forceinline__ const void* spec_row_ptr(const SpecVerifyArgs& p, int
 
 // Grid: x parts of a row, y sequences, z rows
 template <int DT>
-__global__ void __launch_bounds__(SV_THREADS) spec_stat_kernel(const SpecVerifyArgs p) {
+__global__ void __launch_bounds__(SV_THREADS, 4) spec_stat_kernel(const SpecVerifyArgs p) {
   griddep_launch_dependents();
   griddep_wait();
   constexpr int N = SpecVec<DT>::N, VL = SV_BLOCK / N / 32;    // vectors per lane
