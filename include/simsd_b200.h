@@ -533,7 +533,7 @@ int simsd_paged_append(const void* qkv, int64_t ldqkv, int T, int Hq, int Hk, in
  * The lengths are read on the device only.  B Hk ceil(G L / 32) (max_pages
  * page_size / 64 + 1) < 2^31 (more: SIMSD_ERR_UNSUPPORTED).
  */
-size_t simsd_paged_attention_workspace_size(int B, int L, int Hq, int Hk, int head_dim);
+size_t simsd_paged_attention_workspace_size(int L, int Hq, int Hk, int head_dim);
 int simsd_paged_attention(const void* q, const void* k_cache, const void* v_cache, int num_pages, int page_size,
                           int64_t ld_page, int64_t ld_head, int64_t ld_tok, const int32_t* page_table, int64_t ld_table,
                           int max_pages, const int32_t* seq_lens, const uint8_t* tail_mask, int64_t ldm_b, int64_t ldm_t,

@@ -179,8 +179,8 @@ int simsd_paged_append(const void* qkv, int64_t ldqkv, int T, int Hq, int Hk, in
                         : launch_on(paged_append_kernel<128, false>, dim3((unsigned)T), PA_THREADS, 0, stream, false, a);
 }
 
-size_t simsd_paged_attention_workspace_size(int B, int L, int Hq, int Hk, int head_dim) {
-  if (B < 1 || L < 1 || Hq < 1 || Hk < 1 || Hq % Hk || head_dim < 1) return 256;
+size_t simsd_paged_attention_workspace_size(int L, int Hq, int Hk, int head_dim) {
+  if (L < 1 || Hq < 1 || Hk < 1 || Hq % Hk || head_dim < 1) return 256;
   return paged_plan(L, Hq / Hk, head_dim).bytes;
 }
 
@@ -200,7 +200,7 @@ int simsd_paged_attention(const void* q, const void* k_cache, const void* v_cach
   if (!al16(q) || !al16(o)) return SIMSD_ERR_ALIGN;
   int rc = cache_check(k_cache, v_cache, ld_page, ld_head, ld_tok);
   if (rc != SIMSD_OK) return rc;
-  if (workspace == nullptr || workspace_bytes < simsd_paged_attention_workspace_size(B, L, Hq, Hk, head_dim))
+  if (workspace == nullptr || workspace_bytes < simsd_paged_attention_workspace_size(L, Hq, Hk, head_dim))
     return SIMSD_ERR_WORKSPACE;
   PagedAttnArgs a;
   a.q = q;

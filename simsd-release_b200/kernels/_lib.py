@@ -84,7 +84,7 @@ SIGNATURES: dict[str, tuple] = {
     "simsd_verify_attention": (_I, [_P, _P, _P, _L, _I, _I, _I, _I, _P, _L, _F, _P, _I, _P, _S, _P]),
     "simsd_paged_append": (_I, [_P, _L, _I, _I, _I, _I, _I, _P, _P, _F, _P, _P, _L, _P, _P, _P, _P, _P, _I, _I, _L, _L,
                                 _L, _I, _P, _P]),
-    "simsd_paged_attention_workspace_size": (_S, [_I, _I, _I, _I, _I]),
+    "simsd_paged_attention_workspace_size": (_S, [_I, _I, _I, _I]),
     "simsd_paged_attention": (_I, [_P, _P, _P, _I, _I, _L, _L, _L, _P, _L, _I, _P, _P, _L, _L, _I, _I, _I, _I, _I, _F,
                                    _P, _P, _I, _P, _S, _P, _P]),
     "simsd_speculative_verify_workspace_size": (_S, [_I, _I, _I]),
@@ -207,39 +207,49 @@ def workspace(dev: torch.device, nbytes: int) -> torch.Tensor:
             _RETIRED.append(buf)
         buf = torch.zeros(size, dtype=torch.uint8, device=dev)
         _WORKSPACES[dev] = buf
+        _ERROR_PTRS.pop(dev.index, None)
     return buf
 
 
-def error_ptr(dev: torch.device) -> int:
-    """Device address of the error word in `dev`'s workspace header (`device_error` reads it)."""
-    return workspace(dev, HEADER_BYTES).data_ptr() + HEADER_BYTES - 64
+# Device index -> address of the error word in that device's workspace header.
+_ERROR_PTRS: dict[int, int] = {}
 
 
-_STREAM_SCRATCH: dict[tuple[int, int], torch.Tensor] = {}
+def error_ptr(index: int) -> int:
+    """Device address of the error word in the workspace header of CUDA device `index` (`device_error` reads it)."""
+    ptr = _ERROR_PTRS.get(index)
+    if ptr is None:
+        ptr = _ERROR_PTRS[index] = workspace(torch.device("cuda", index), HEADER_BYTES).data_ptr() + HEADER_BYTES - 64
+    return ptr
 
 
-def stream_scratch(dev: torch.device, nbytes: int, zeroed: int) -> torch.Tensor:
-    """Scratch of at least `nbytes` for the current stream of `dev`, its first `zeroed`
-    bytes zero when new (the operators leave them zero).  Each stream has its own, so
-    calls on several streams share none; a call under graph capture gets one of the
-    graph's memory, zeroed by the graph on every replay."""
-    if torch.cuda.is_current_stream_capturing():
-        buf = torch.empty(nbytes, dtype=torch.uint8, device=dev)
+_STREAM_SCRATCH: dict[tuple[int, int], tuple[int, int, torch.Tensor]] = {}
+
+
+def stream_scratch(index: int, stream: int, nbytes: int, zeroed: int):
+    """(address, bytes, owner) of scratch of at least `nbytes` for `stream` of CUDA device
+    `index` (both current), its first `zeroed` bytes zero when new (the operators leave
+    them zero).  Each stream has its own, so calls on several streams share none; a call
+    under graph capture gets one of the graph's memory, zeroed by the graph on every
+    replay.  Keep the owner until the call has been issued."""
+    if torch._C._cuda_isCurrentStreamCapturing():
+        buf = torch.empty(nbytes, dtype=torch.uint8, device=torch.device("cuda", index))
         buf[:zeroed].zero_()
-        return buf
-    key = (dev.index, stream_ptr(dev))
-    buf = _STREAM_SCRATCH.get(key)
-    if buf is None or buf.numel() < nbytes:
+        return buf.data_ptr(), nbytes, buf
+    held = _STREAM_SCRATCH.get((index, stream))
+    if held is None or held[1] < nbytes:
         # an outgrown one goes back to torch's allocator, which hands it out again
         # only to later work of the stream it was allocated on: this one
-        buf = _STREAM_SCRATCH[key] = torch.zeros(nbytes, dtype=torch.uint8, device=dev)
-    return buf
+        buf = torch.zeros(nbytes, dtype=torch.uint8, device=torch.device("cuda", index))
+        held = _STREAM_SCRATCH[(index, stream)] = (buf.data_ptr(), nbytes, buf)
+    return held
 
 
 def reset_workspace() -> None:
     """Drop the cached workspaces (call before re-capturing graphs in a new pool)."""
     _WORKSPACES.clear()
     _RETIRED.clear()
+    _ERROR_PTRS.clear()
     _STREAM_SCRATCH.clear()
 
 

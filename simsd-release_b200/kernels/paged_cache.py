@@ -23,14 +23,17 @@ import torch
 
 from . import _lib
 
-HEAD_DIMS = (64, 128)
-
-
 def rope_table(n: int, dim: int, theta: float = 1e6, device=None) -> tuple[torch.Tensor, torch.Tensor]:
     """cos and sin [n, dim / 2] fp32 of positions 0 .. n - 1 (angles in fp64, rounded once)."""
     inv = theta ** (-torch.arange(0, dim, 2, device=device, dtype=torch.float64) / dim)
     a = torch.arange(n, device=device, dtype=torch.float64)[:, None] * inv
     return a.cos().float(), a.sin().float()
+
+
+# What the kernels take, in the library's codes.
+_HALF = {torch.bfloat16: _lib.SIMSD_BF16, torch.float16: _lib.SIMSD_F16}
+_current_stream = torch._C._cuda_getCurrentRawStream
+_current_device = torch._C._cuda_getDevice
 
 
 def _check_cache(what: str, k_cache: torch.Tensor, v_cache: torch.Tensor, kv_heads: int, dtype: torch.dtype) -> None:
@@ -41,6 +44,32 @@ def _check_cache(what: str, k_cache: torch.Tensor, v_cache: torch.Tensor, kv_hea
                          f"{tuple(k_cache.shape)} / {tuple(v_cache.shape)}")
     if k_cache.stride() != v_cache.stride() or k_cache.stride(3) != 1:
         raise ValueError(f"{what}: k_cache and v_cache must have the same strides, the last one 1")
+
+
+def _check_append(qkv, heads, kv_heads, k_cache, v_cache, slots, positions, cos, sin, q_weight, k_weight) -> None:
+    """Raise what is wrong with a request of paged_append."""
+    if qkv.dtype not in _HALF:
+        raise TypeError(f"paged_append takes bf16 or fp16 activations, got {qkv.dtype}")
+    _check_cache("paged_append", k_cache, v_cache, kv_heads, qkv.dtype)
+    D = k_cache.shape[3]
+    if qkv.ndim != 2 or heads < 1 or kv_heads < 1 or qkv.shape[1] != (heads + 2 * kv_heads) * D:
+        raise ValueError(f"qkv must be [T, {(heads + 2 * kv_heads) * D}], got {tuple(qkv.shape)}")
+    T = qkv.shape[0]
+    if slots.dtype != torch.int64 or positions.dtype != torch.int64:
+        raise TypeError("paged_append: slots and positions are int64")
+    if slots.shape != (T,) or positions.shape != (T,):
+        raise ValueError(f"slots and positions must be [{T}], got {tuple(slots.shape)} / {tuple(positions.shape)}")
+    if cos.dtype != torch.float32 or sin.dtype != torch.float32:
+        raise TypeError("paged_append: cos and sin are fp32")
+    if cos.ndim != 2 or cos.shape != sin.shape or not cos.is_contiguous() or not sin.is_contiguous():
+        raise ValueError("cos and sin must be contiguous [n, R / 2] tensors of the same shape")
+    for w in (q_weight, k_weight):
+        if w is not None:
+            if w.dtype != qkv.dtype:
+                raise TypeError("paged_append: the norm weights must have qkv's dtype")
+            if w.shape != (D,):
+                raise ValueError(f"the norm weights must be [{D}]")
+    _lib.require_cuda(qkv, k_cache, v_cache, slots, positions, cos, sin, q_weight, k_weight)
 
 
 def paged_append(qkv: torch.Tensor, heads: int, kv_heads: int, k_cache: torch.Tensor, v_cache: torch.Tensor,
@@ -58,45 +87,76 @@ def paged_append(qkv: torch.Tensor, heads: int, kv_heads: int, k_cache: torch.Te
     before the rotation (sdar/modeling_sdar.py:197-302), or None.  Computed in
     fp32, rounded once.  bf16 or fp16; D 64 or 128; R a multiple of 16.
     """
-    if qkv.dtype not in (torch.bfloat16, torch.float16):
-        raise TypeError(f"paged_append takes bf16 or fp16 activations, got {qkv.dtype}")
     if torch.is_grad_enabled() and (qkv.requires_grad or k_cache.requires_grad or v_cache.requires_grad):
         raise RuntimeError("paged_append is a forward-only inference kernel.")
-    _check_cache("paged_append", k_cache, v_cache, kv_heads, qkv.dtype)
-    pages, _, page_size, D = k_cache.shape
-    if qkv.ndim != 2 or heads < 1 or qkv.shape[1] != (heads + 2 * kv_heads) * D:
-        raise ValueError(f"qkv must be [T, {(heads + 2 * kv_heads) * D}], got {tuple(qkv.shape)}")
-    T = qkv.shape[0]
-    if slots.dtype != torch.int64 or positions.dtype != torch.int64:
-        raise TypeError("paged_append: slots and positions are int64")
-    if slots.shape != (T,) or positions.shape != (T,):
-        raise ValueError(f"slots and positions must be [{T}], got {tuple(slots.shape)} / {tuple(positions.shape)}")
-    if cos.dtype != torch.float32 or sin.dtype != torch.float32:
-        raise TypeError("paged_append: cos and sin are fp32")
-    if cos.ndim != 2 or cos.shape != sin.shape or not cos.is_contiguous() or not sin.is_contiguous():
-        raise ValueError("cos and sin must be contiguous [n, R / 2] tensors of the same shape")
-    for w in (q_weight, k_weight):
-        if w is not None:
-            if w.dtype != qkv.dtype:
-                raise TypeError("paged_append: the norm weights must have qkv's dtype")
-            if w.shape != (D,):
-                raise ValueError(f"the norm weights must be [{D}]")
-    dev = _lib.require_cuda(qkv, k_cache, v_cache, slots, positions, cos, sin, q_weight, k_weight)
-    if qkv.stride(1) != 1:
+    # one test of everything that a good request has; what is wrong with a bad one is said by _check_append
+    dt, dev = qkv.dtype, qkv.get_device()
+    shape, strides = k_cache.shape, k_cache.stride()
+    rows, table = slots.shape, cos.shape
+    if not (dt in _HALF and dev >= 0 and len(shape) == 4 and len(rows) == 1 and len(table) == 2
+            and k_cache.dtype is dt and v_cache.dtype is dt and v_cache.shape == shape and v_cache.stride() == strides
+            and strides[3] == 1 and shape[1] == kv_heads and heads >= 1
+            and qkv.shape == (rows[0], (heads + 2 * kv_heads) * shape[3]) and positions.shape == rows
+            and slots.dtype is torch.int64 and positions.dtype is torch.int64
+            and cos.dtype is torch.float32 and sin.dtype is torch.float32 and sin.shape == table
+            and cos.is_contiguous() and sin.is_contiguous()
+            and (q_weight is None or q_weight.dtype is dt and q_weight.shape == shape[3:] and q_weight.get_device() == dev)
+            and (k_weight is None or k_weight.dtype is dt and k_weight.shape == shape[3:] and k_weight.get_device() == dev)
+            and k_cache.get_device() == v_cache.get_device() == slots.get_device() == positions.get_device()
+            == cos.get_device() == sin.get_device() == dev):
+        _check_append(qkv, heads, kv_heads, k_cache, v_cache, slots, positions, cos, sin, q_weight, k_weight)
+    if _current_device() != dev:
+        with torch.cuda.device(dev):
+            return paged_append(qkv, heads, kv_heads, k_cache, v_cache, slots, positions, cos, sin, q_weight, k_weight, eps)
+    ldq, unit = qkv.stride()
+    if unit != 1:
         qkv = qkv.contiguous()
-    slots, positions = slots.contiguous(), positions.contiguous()
-    q_weight = q_weight.contiguous() if q_weight is not None else None
-    k_weight = k_weight.contiguous() if k_weight is not None else None
-    q = torch.empty((T, heads, D), dtype=qkv.dtype, device=dev)
-    with _lib.device_guard(dev):
-        rc = _lib.lib().simsd_paged_append(
-            qkv.data_ptr(), qkv.stride(0), T, heads, kv_heads, D, 2 * cos.shape[1],
-            q_weight.data_ptr() if q_weight is not None else None, k_weight.data_ptr() if k_weight is not None else None,
-            float(eps), cos.data_ptr(), sin.data_ptr(), cos.shape[0], positions.data_ptr(), slots.data_ptr(),
-            q.data_ptr(), k_cache.data_ptr(), v_cache.data_ptr(), pages, page_size, k_cache.stride(0),
-            k_cache.stride(1), k_cache.stride(2), _lib.dtype_code(qkv.dtype), _lib.error_ptr(dev), _lib.stream_ptr(dev))
-    _lib.check(rc, "paged_append")
+        ldq = qkv.stride(0)
+    if not slots.is_contiguous():
+        slots = slots.contiguous()
+    if not positions.is_contiguous():
+        positions = positions.contiguous()
+    qw = kw = None
+    if q_weight is not None:
+        q_weight = q_weight.contiguous()
+        qw = q_weight.data_ptr()
+    if k_weight is not None:
+        k_weight = k_weight.contiguous()
+        kw = k_weight.data_ptr()
+    q = qkv.new_empty((rows[0], heads, shape[3]))
+    rc = _lib.lib().simsd_paged_append(
+        qkv.data_ptr(), ldq, rows[0], heads, kv_heads, shape[3], 2 * table[1], qw, kw, eps, cos.data_ptr(),
+        sin.data_ptr(), table[0], positions.data_ptr(), slots.data_ptr(), q.data_ptr(), k_cache.data_ptr(),
+        v_cache.data_ptr(), shape[0], shape[2], strides[0], strides[1], strides[2], _HALF[dt], _lib.error_ptr(dev),
+        _current_stream(dev))
+    if rc:
+        _lib.check(rc, "paged_append")
     return q
+
+
+def _check_attention(q, k_cache, v_cache, page_table, seq_lens, tail_mask) -> None:
+    """Raise what is wrong with a request of paged_attention."""
+    if q.dtype not in _HALF:
+        raise TypeError(f"paged_attention takes bf16 or fp16 queries, got {q.dtype}")
+    if q.ndim not in (3, 4):
+        raise ValueError(f"q must be [B, L, heads, D] or [B, heads, D], got {tuple(q.shape)}")
+    B, Hq, D = q.shape[0], q.shape[-2], q.shape[-1]
+    L = q.shape[1] if q.ndim == 4 else 1
+    Hk = k_cache.shape[1] if k_cache.ndim == 4 else 0
+    _check_cache("paged_attention", k_cache, v_cache, Hk, q.dtype)
+    if k_cache.shape[3] != D or Hk < 1 or Hq < 1 or Hq % Hk:
+        raise ValueError(f"q heads {Hq} x {D} do not go with the cache's {Hk} x {k_cache.shape[3]}")
+    if page_table.dtype != torch.int32 or seq_lens.dtype != torch.int32:
+        raise TypeError("paged_attention: page_table and seq_lens are int32")
+    if page_table.ndim != 2 or page_table.shape[0] != B or seq_lens.shape != (B,):
+        raise ValueError(f"page_table must be [{B}, max_pages] and seq_lens [{B}], got {tuple(page_table.shape)} / "
+                         f"{tuple(seq_lens.shape)}")
+    if tail_mask is not None:
+        if tail_mask.dtype != torch.bool:
+            raise TypeError("paged_attention: tail_mask is bool")
+        if tail_mask.shape != (L, L) and tail_mask.shape != (B, L, L):
+            raise ValueError(f"tail_mask must be [{L}, {L}] or [{B}, {L}, {L}], got {tuple(tail_mask.shape)}")
+    _lib.require_cuda(q, k_cache, v_cache, page_table, seq_lens, tail_mask)
 
 
 def paged_attention(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor, page_table: torch.Tensor,
@@ -117,51 +177,61 @@ def paged_attention(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tenso
     when None.  Lengths are read on the device, so the call can be captured in a
     CUDA graph and replayed as the sequences grow.
     """
-    if q.dtype not in (torch.bfloat16, torch.float16):
-        raise TypeError(f"paged_attention takes bf16 or fp16 queries, got {q.dtype}")
     if torch.is_grad_enabled() and (q.requires_grad or k_cache.requires_grad or v_cache.requires_grad):
         raise RuntimeError("paged_attention is a forward-only inference kernel.")
-    if q.ndim not in (3, 4):
-        raise ValueError(f"q must be [B, L, heads, D] or [B, heads, D], got {tuple(q.shape)}")
-    B, Hq, D = q.shape[0], q.shape[-2], q.shape[-1]
-    L = q.shape[1] if q.ndim == 4 else 1
-    Hk = k_cache.shape[1] if k_cache.ndim == 4 else 0
-    _check_cache("paged_attention", k_cache, v_cache, Hk, q.dtype)
-    pages, _, page_size, Dk = k_cache.shape
-    if Dk != D or Hk < 1 or Hq < 1 or Hq % Hk:
-        raise ValueError(f"q heads {Hq} x {D} do not go with the cache's {Hk} x {Dk}")
-    if page_table.dtype != torch.int32 or seq_lens.dtype != torch.int32:
-        raise TypeError("paged_attention: page_table and seq_lens are int32")
-    if page_table.ndim != 2 or page_table.shape[0] != B or seq_lens.shape != (B,):
-        raise ValueError(f"page_table must be [{B}, max_pages] and seq_lens [{B}], got {tuple(page_table.shape)} / "
-                         f"{tuple(seq_lens.shape)}")
-    ldm_b = ldm_t = 0
-    if tail_mask is not None:
-        if tail_mask.dtype != torch.bool:
-            raise TypeError("paged_attention: tail_mask is bool")
-        if tail_mask.shape != (L, L) and tail_mask.shape != (B, L, L):
-            raise ValueError(f"tail_mask must be [{L}, {L}] or [{B}, {L}, {L}], got {tuple(tail_mask.shape)}")
-    dev = _lib.require_cuda(q, k_cache, v_cache, page_table, seq_lens, tail_mask)
+    # one test of everything that a good request has; what is wrong with a bad one is said by _check_attention
+    dt, dev = q.dtype, q.get_device()
+    qs, shape, strides, ts = q.shape, k_cache.shape, k_cache.stride(), page_table.shape
+    if not (dt in _HALF and dev >= 0 and 3 <= len(qs) <= 4 and len(shape) == 4 and len(ts) == 2
+            and k_cache.dtype is dt and v_cache.dtype is dt and v_cache.shape == shape and v_cache.stride() == strides
+            and strides[3] == 1 and shape[3] == qs[-1] and shape[1] > 0 and qs[-2] > 0 and qs[-2] % shape[1] == 0
+            and page_table.dtype is torch.int32 and seq_lens.dtype is torch.int32 and ts[0] == qs[0]
+            and seq_lens.shape == qs[:1]
+            and k_cache.get_device() == v_cache.get_device() == page_table.get_device() == seq_lens.get_device() == dev
+            and (tail_mask is None or tail_mask.dtype is torch.bool and tail_mask.get_device() == dev and len(qs) == 4
+                 and (tail_mask.shape == (qs[0], qs[1], qs[1]) or tail_mask.shape == (qs[1], qs[1])))):
+        _check_attention(q, k_cache, v_cache, page_table, seq_lens, tail_mask)
+    if _current_device() != dev:
+        with torch.cuda.device(dev):
+            return paged_attention(q, k_cache, v_cache, page_table, seq_lens, scale, tail_mask, return_lse)
+    B, Hq, D = qs[0], qs[-2], qs[-1]
+    L = qs[1] if len(qs) == 4 else 1
+    mask, ldm_b, ldm_t = None, 0, 0
     if tail_mask is not None:
         if tail_mask.stride(-1) != 1:
             tail_mask = tail_mask.contiguous()
-        ldm_t = tail_mask.stride(-2)
+        mask, ldm_t = tail_mask.data_ptr(), tail_mask.stride(-2)
         ldm_b = tail_mask.stride(0) if tail_mask.ndim == 3 else 0
     if not q.is_contiguous():
         q = q.contiguous()
-    if page_table.stride(1) != 1:
+    ld_table, unit = page_table.stride()
+    if unit != 1:
         page_table = page_table.contiguous()
-    seq_lens = seq_lens.contiguous()
+        ld_table = page_table.stride(0)
+    if not seq_lens.is_contiguous():
+        seq_lens = seq_lens.contiguous()
     o = torch.empty_like(q)
-    lse = torch.empty(q.shape[:-1], dtype=torch.float32, device=dev) if return_lse else None
-    L_ = _lib.lib()
-    with _lib.device_guard(dev):
-        ws = _lib.stream_scratch(dev, L_.simsd_paged_attention_workspace_size(B, L, Hq, Hk, D), _lib.PAGED_COUNTER_BYTES)
-        rc = L_.simsd_paged_attention(
-            q.data_ptr(), k_cache.data_ptr(), v_cache.data_ptr(), pages, page_size, k_cache.stride(0), k_cache.stride(1),
-            k_cache.stride(2), page_table.data_ptr(), page_table.stride(0), page_table.shape[1], seq_lens.data_ptr(),
-            tail_mask.data_ptr() if tail_mask is not None else None, ldm_b, ldm_t, B, L, Hq, Hk, D,
-            D ** -0.5 if scale is None else float(scale), o.data_ptr(), lse.data_ptr() if return_lse else None,
-            _lib.dtype_code(q.dtype), ws.data_ptr(), ws.numel(), _lib.error_ptr(dev), _lib.stream_ptr(dev))
-    _lib.check(rc, "paged_attention")
+    lse = q.new_empty(qs[:-1], dtype=torch.float32) if return_lse else None
+    lib, stream = _lib.lib(), _current_stream(dev)
+    ws, ws_bytes, owner = _lib.stream_scratch(dev, stream, _workspace_bytes(dev, L, Hq, shape[1], D),
+                                              _lib.PAGED_COUNTER_BYTES)
+    rc = lib.simsd_paged_attention(
+        q.data_ptr(), k_cache.data_ptr(), v_cache.data_ptr(), shape[0], shape[2], strides[0], strides[1], strides[2],
+        page_table.data_ptr(), ld_table, ts[1], seq_lens.data_ptr(), mask, ldm_b, ldm_t, B, L, Hq, shape[1], D,
+        D ** -0.5 if scale is None else scale, o.data_ptr(), lse.data_ptr() if return_lse else None, _HALF[dt], ws,
+        ws_bytes, _lib.error_ptr(dev), stream)
+    if rc:
+        _lib.check(rc, "paged_attention")
     return (o, lse) if return_lse else o
+
+
+_WS_SIZES: dict[tuple, int] = {}
+
+
+def _workspace_bytes(dev: int, L: int, Hq: int, Hk: int, D: int) -> int:
+    """simsd_paged_attention_workspace_size, memoised (arithmetic for a device; the batch does not enter)."""
+    key = (dev, L, Hq, Hk, D)
+    size = _WS_SIZES.get(key)
+    if size is None:
+        size = _WS_SIZES[key] = _lib.lib().simsd_paged_attention_workspace_size(L, Hq, Hk, D)
+    return size
