@@ -4,14 +4,18 @@
     python simsd-release_b200/build.py --force
 
 The library lands next to the Python package (kernels/libsimsd_b200.so), where
-kernels/_lib.py loads it.  nvcc cross-compiles without a GPU.
+kernels/_lib.py loads it, and beside it kernels/_binding.so, the short way from
+Python to the serving operators (host code only, against torch's headers).  nvcc
+cross-compiles without a GPU.
 """
 from __future__ import annotations
 
 import argparse
+import importlib.util
 import os
 import subprocess
 import sys
+import sysconfig
 from pathlib import Path
 
 PKG = Path(__file__).resolve().parent
@@ -19,6 +23,7 @@ REPO = PKG.parent
 CSRC = PKG / "csrc"
 OUT = PKG / "kernels" / "libsimsd_b200.so"
 OBJ = PKG / "_build"
+BINDING = PKG / "kernels" / "_binding.so"
 ARCH = ["-gencode", "arch=compute_100a,code=sm_100a"]
 
 
@@ -32,20 +37,31 @@ def nvcc() -> str:
 
 
 def build(force: bool = False, verbose: bool = False) -> Path:
-    if OUT.exists() and not force:
-        newest = max(p.stat().st_mtime for p in sources())
-        if OUT.stat().st_mtime >= newest:
-            return OUT
-    OBJ.mkdir(exist_ok=True)
-    units = sorted(CSRC.glob("*.cu"))
-    objs = [str(OBJ / (u.stem + ".o")) for u in units]
-    # the translation units compile side by side, then link into one library
-    run([[nvcc(), "-O3", "-std=c++17", *ARCH, "-lineinfo", "-Xcompiler", "-fPIC,-O3", "-Xptxas",
-          "-v" if verbose else "-O3", "-I", str(REPO / "include"), "-c", "-o", o, str(u)]
-         for u, o in zip(units, objs)], verbose)
-    run([[nvcc(), *ARCH, "-shared", "-Xcompiler", "-fPIC", "-o", str(OUT) + ".tmp", *objs]], verbose)
-    os.replace(str(OUT) + ".tmp", OUT)
+    if force or stale(OUT, sources()):
+        OBJ.mkdir(exist_ok=True)
+        units = sorted(CSRC.glob("*.cu"))
+        objs = [str(OBJ / (u.stem + ".o")) for u in units]
+        # the translation units compile side by side, then link into one library
+        run([[nvcc(), "-O3", "-std=c++17", *ARCH, "-lineinfo", "-Xcompiler", "-fPIC,-O3", "-Xptxas",
+              "-v" if verbose else "-O3", "-I", str(REPO / "include"), "-c", "-o", o, str(u)]
+             for u, o in zip(units, objs)], verbose)
+        run([[nvcc(), *ARCH, "-shared", "-Xcompiler", "-fPIC", "-o", str(OUT) + ".tmp", *objs]], verbose)
+        os.replace(str(OUT) + ".tmp", OUT)
+    source = CSRC / "binding.cpp"
+    if force or stale(BINDING, [source, REPO / "include" / "simsd_b200.h"]):
+        torch = Path(importlib.util.find_spec("torch").submodule_search_locations[0])
+        cuda = Path(nvcc()).resolve().parents[1]
+        run([[os.environ.get("CXX", "g++"), "-O2", "-std=c++17", "-fPIC", "-shared", "-I", str(REPO / "include"),
+              "-I", sysconfig.get_paths()["include"], "-I", str(torch / "include"),
+              "-I", str(torch / "include" / "torch" / "csrc" / "api" / "include"), "-I", str(cuda / "include"),
+              "-o", str(BINDING) + ".tmp", str(source), "-L", str(torch / "lib"), "-L", str(cuda / "lib64"),
+              "-ltorch_python", "-ltorch_cpu", "-ltorch_cuda", "-lc10", "-lc10_cuda", "-lcudart"]], verbose)
+        os.replace(str(BINDING) + ".tmp", BINDING)
     return OUT
+
+
+def stale(out: Path, srcs: list[Path]) -> bool:
+    return not out.exists() or out.stat().st_mtime < max(p.stat().st_mtime for p in srcs)
 
 
 def run(cmds: list[list[str]], verbose: bool) -> None:
@@ -54,7 +70,7 @@ def run(cmds: list[list[str]], verbose: bool) -> None:
     for c, p, out in zip(cmds, procs, outs):
         if p.returncode != 0:
             sys.stderr.write(out)
-            raise RuntimeError(f"nvcc failed ({p.returncode}): {' '.join(c)}")
+            raise RuntimeError(f"{Path(c[0]).name} failed ({p.returncode}): {' '.join(c)}")
         if verbose:
             sys.stderr.write(out)
 

@@ -120,6 +120,26 @@ def lib() -> ctypes.CDLL:
     return _lib
 
 
+_BOUND = ("simsd_paged_append", "simsd_paged_attention", "simsd_paged_attention_workspace_size",
+          "simsd_speculative_verify", "simsd_speculative_verify_workspace_size")
+_binding = None
+
+
+def binding():
+    """The native short way to the serving operators (csrc/binding.cpp), bound to this library."""
+    global _binding
+    if _binding is None:
+        try:
+            from . import _binding as native
+        except ImportError as e:
+            raise RuntimeError("kernels/_binding.so is not built for this Python and torch; run "
+                               "`python simsd-release_b200/build.py`") from e
+        L = lib()
+        native.bind({n: ctypes.cast(getattr(L, n), ctypes.c_void_p).value for n in _BOUND}, error_ptr, stream_scratch)
+        _binding = native
+    return _binding
+
+
 def dtype_code(dt: torch.dtype) -> int:
     try:
         return _DTYPE[dt]
@@ -208,6 +228,8 @@ def workspace(dev: torch.device, nbytes: int) -> torch.Tensor:
         buf = torch.zeros(size, dtype=torch.uint8, device=dev)
         _WORKSPACES[dev] = buf
         _ERROR_PTRS.pop(dev.index, None)
+        if _binding is not None:
+            _binding.forget()
     return buf
 
 
@@ -251,6 +273,8 @@ def reset_workspace() -> None:
     _RETIRED.clear()
     _ERROR_PTRS.clear()
     _STREAM_SCRATCH.clear()
+    if _binding is not None:
+        _binding.forget()
 
 
 def device_error(dev: torch.device | None = None) -> int:

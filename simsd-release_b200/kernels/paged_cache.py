@@ -87,50 +87,30 @@ def paged_append(qkv: torch.Tensor, heads: int, kv_heads: int, k_cache: torch.Te
     before the rotation (sdar/modeling_sdar.py:197-302), or None.  Computed in
     fp32, rounded once.  bf16 or fp16; D 64 or 128; R a multiple of 16.
     """
+    q = _lib.binding().paged_append(qkv, heads, kv_heads, k_cache, v_cache, slots, positions, cos, sin, q_weight, k_weight,
+                                    eps)
+    if q is not None:
+        return q
     if torch.is_grad_enabled() and (qkv.requires_grad or k_cache.requires_grad or v_cache.requires_grad):
         raise RuntimeError("paged_append is a forward-only inference kernel.")
-    # one test of everything that a good request has; what is wrong with a bad one is said by _check_append
-    dt, dev = qkv.dtype, qkv.get_device()
-    shape, strides = k_cache.shape, k_cache.stride()
-    rows, table = slots.shape, cos.shape
-    if not (dt in _HALF and dev >= 0 and len(shape) == 4 and len(rows) == 1 and len(table) == 2
-            and k_cache.dtype is dt and v_cache.dtype is dt and v_cache.shape == shape and v_cache.stride() == strides
-            and strides[3] == 1 and shape[1] == kv_heads and heads >= 1
-            and qkv.shape == (rows[0], (heads + 2 * kv_heads) * shape[3]) and positions.shape == rows
-            and slots.dtype is torch.int64 and positions.dtype is torch.int64
-            and cos.dtype is torch.float32 and sin.dtype is torch.float32 and sin.shape == table
-            and cos.is_contiguous() and sin.is_contiguous()
-            and (q_weight is None or q_weight.dtype is dt and q_weight.shape == shape[3:] and q_weight.get_device() == dev)
-            and (k_weight is None or k_weight.dtype is dt and k_weight.shape == shape[3:] and k_weight.get_device() == dev)
-            and k_cache.get_device() == v_cache.get_device() == slots.get_device() == positions.get_device()
-            == cos.get_device() == sin.get_device() == dev):
-        _check_append(qkv, heads, kv_heads, k_cache, v_cache, slots, positions, cos, sin, q_weight, k_weight)
+    _check_append(qkv, heads, kv_heads, k_cache, v_cache, slots, positions, cos, sin, q_weight, k_weight)
+    dev, shape, strides = qkv.get_device(), k_cache.shape, k_cache.stride()
     if _current_device() != dev:
         with torch.cuda.device(dev):
             return paged_append(qkv, heads, kv_heads, k_cache, v_cache, slots, positions, cos, sin, q_weight, k_weight, eps)
-    ldq, unit = qkv.stride()
-    if unit != 1:
+    if qkv.stride(1) != 1:
         qkv = qkv.contiguous()
-        ldq = qkv.stride(0)
-    if not slots.is_contiguous():
-        slots = slots.contiguous()
-    if not positions.is_contiguous():
-        positions = positions.contiguous()
-    qw = kw = None
-    if q_weight is not None:
-        q_weight = q_weight.contiguous()
-        qw = q_weight.data_ptr()
-    if k_weight is not None:
-        k_weight = k_weight.contiguous()
-        kw = k_weight.data_ptr()
-    q = qkv.new_empty((rows[0], heads, shape[3]))
+    slots, positions = slots.contiguous(), positions.contiguous()
+    q_weight = q_weight.contiguous() if q_weight is not None else None
+    k_weight = k_weight.contiguous() if k_weight is not None else None
+    q = qkv.new_empty((qkv.shape[0], heads, shape[3]))
     rc = _lib.lib().simsd_paged_append(
-        qkv.data_ptr(), ldq, rows[0], heads, kv_heads, shape[3], 2 * table[1], qw, kw, eps, cos.data_ptr(),
-        sin.data_ptr(), table[0], positions.data_ptr(), slots.data_ptr(), q.data_ptr(), k_cache.data_ptr(),
-        v_cache.data_ptr(), shape[0], shape[2], strides[0], strides[1], strides[2], _HALF[dt], _lib.error_ptr(dev),
-        _current_stream(dev))
-    if rc:
-        _lib.check(rc, "paged_append")
+        qkv.data_ptr(), qkv.stride(0), qkv.shape[0], heads, kv_heads, shape[3], 2 * cos.shape[1],
+        q_weight.data_ptr() if q_weight is not None else None, k_weight.data_ptr() if k_weight is not None else None, eps,
+        cos.data_ptr(), sin.data_ptr(), cos.shape[0], positions.data_ptr(), slots.data_ptr(), q.data_ptr(),
+        k_cache.data_ptr(), v_cache.data_ptr(), shape[0], shape[2], strides[0], strides[1], strides[2], _HALF[qkv.dtype],
+        _lib.error_ptr(dev), _current_stream(dev))
+    _lib.check(rc, "paged_append")
     return q
 
 
@@ -177,61 +157,37 @@ def paged_attention(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tenso
     when None.  Lengths are read on the device, so the call can be captured in a
     CUDA graph and replayed as the sequences grow.
     """
+    o = _lib.binding().paged_attention(q, k_cache, v_cache, page_table, seq_lens, scale, tail_mask, return_lse)
+    if o is not None:
+        return o
     if torch.is_grad_enabled() and (q.requires_grad or k_cache.requires_grad or v_cache.requires_grad):
         raise RuntimeError("paged_attention is a forward-only inference kernel.")
-    # one test of everything that a good request has; what is wrong with a bad one is said by _check_attention
-    dt, dev = q.dtype, q.get_device()
-    qs, shape, strides, ts = q.shape, k_cache.shape, k_cache.stride(), page_table.shape
-    if not (dt in _HALF and dev >= 0 and 3 <= len(qs) <= 4 and len(shape) == 4 and len(ts) == 2
-            and k_cache.dtype is dt and v_cache.dtype is dt and v_cache.shape == shape and v_cache.stride() == strides
-            and strides[3] == 1 and shape[3] == qs[-1] and shape[1] > 0 and qs[-2] > 0 and qs[-2] % shape[1] == 0
-            and page_table.dtype is torch.int32 and seq_lens.dtype is torch.int32 and ts[0] == qs[0]
-            and seq_lens.shape == qs[:1]
-            and k_cache.get_device() == v_cache.get_device() == page_table.get_device() == seq_lens.get_device() == dev
-            and (tail_mask is None or tail_mask.dtype is torch.bool and tail_mask.get_device() == dev and len(qs) == 4
-                 and (tail_mask.shape == (qs[0], qs[1], qs[1]) or tail_mask.shape == (qs[1], qs[1])))):
-        _check_attention(q, k_cache, v_cache, page_table, seq_lens, tail_mask)
+    _check_attention(q, k_cache, v_cache, page_table, seq_lens, tail_mask)
+    dev, shape, strides = q.get_device(), k_cache.shape, k_cache.stride()
     if _current_device() != dev:
         with torch.cuda.device(dev):
             return paged_attention(q, k_cache, v_cache, page_table, seq_lens, scale, tail_mask, return_lse)
-    B, Hq, D = qs[0], qs[-2], qs[-1]
-    L = qs[1] if len(qs) == 4 else 1
-    mask, ldm_b, ldm_t = None, 0, 0
+    B, Hq, D = q.shape[0], q.shape[-2], q.shape[-1]
+    L = q.shape[1] if q.ndim == 4 else 1
+    ldm_b = ldm_t = 0
     if tail_mask is not None:
         if tail_mask.stride(-1) != 1:
             tail_mask = tail_mask.contiguous()
-        mask, ldm_t = tail_mask.data_ptr(), tail_mask.stride(-2)
+        ldm_t = tail_mask.stride(-2)
         ldm_b = tail_mask.stride(0) if tail_mask.ndim == 3 else 0
-    if not q.is_contiguous():
-        q = q.contiguous()
-    ld_table, unit = page_table.stride()
-    if unit != 1:
+    q, seq_lens = q.contiguous(), seq_lens.contiguous()
+    if page_table.stride(1) != 1:
         page_table = page_table.contiguous()
-        ld_table = page_table.stride(0)
-    if not seq_lens.is_contiguous():
-        seq_lens = seq_lens.contiguous()
     o = torch.empty_like(q)
-    lse = q.new_empty(qs[:-1], dtype=torch.float32) if return_lse else None
+    lse = q.new_empty(q.shape[:-1], dtype=torch.float32) if return_lse else None
     lib, stream = _lib.lib(), _current_stream(dev)
-    ws, ws_bytes, owner = _lib.stream_scratch(dev, stream, _workspace_bytes(dev, L, Hq, shape[1], D),
-                                              _lib.PAGED_COUNTER_BYTES)
+    ws, ws_bytes, _owner = _lib.stream_scratch(dev, stream, lib.simsd_paged_attention_workspace_size(L, Hq, shape[1], D),
+                                               _lib.PAGED_COUNTER_BYTES)
     rc = lib.simsd_paged_attention(
         q.data_ptr(), k_cache.data_ptr(), v_cache.data_ptr(), shape[0], shape[2], strides[0], strides[1], strides[2],
-        page_table.data_ptr(), ld_table, ts[1], seq_lens.data_ptr(), mask, ldm_b, ldm_t, B, L, Hq, shape[1], D,
-        D ** -0.5 if scale is None else scale, o.data_ptr(), lse.data_ptr() if return_lse else None, _HALF[dt], ws,
+        page_table.data_ptr(), page_table.stride(0), page_table.shape[1], seq_lens.data_ptr(),
+        tail_mask.data_ptr() if tail_mask is not None else None, ldm_b, ldm_t, B, L, Hq, shape[1], D,
+        D ** -0.5 if scale is None else scale, o.data_ptr(), lse.data_ptr() if return_lse else None, _HALF[q.dtype], ws,
         ws_bytes, _lib.error_ptr(dev), stream)
-    if rc:
-        _lib.check(rc, "paged_attention")
+    _lib.check(rc, "paged_attention")
     return (o, lse) if return_lse else o
-
-
-_WS_SIZES: dict[tuple, int] = {}
-
-
-def _workspace_bytes(dev: int, L: int, Hq: int, Hk: int, D: int) -> int:
-    """simsd_paged_attention_workspace_size, memoised (arithmetic for a device; the batch does not enter)."""
-    key = (dev, L, Hq, Hk, D)
-    size = _WS_SIZES.get(key)
-    if size is None:
-        size = _WS_SIZES[key] = _lib.lib().simsd_paged_attention_workspace_size(L, Hq, Hk, D)
-    return size

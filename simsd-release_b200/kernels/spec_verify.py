@@ -73,80 +73,40 @@ def speculative_verify(target_logits: torch.Tensor, draft_tokens: torch.Tensor, 
     token.  A drafted token outside [0, V) is refused, the next one drawn from p,
     and DEV_ERR_BAD_INDEX raised in `_lib.device_error()`.
     """
+    out = _lib.binding().speculative_verify(target_logits, draft_tokens, uniform, noise, draft_logits, temperature, n_draft)
+    if out is not None:
+        return out
     if torch.is_grad_enabled() and (target_logits.requires_grad
                                     or (draft_logits is not None and draft_logits.requires_grad)):
         raise RuntimeError("speculative_verify is a forward-only inference kernel.")
-    # one test of everything that a good request has; what is wrong with a bad one is said by _check
-    dt, dev, shape, f32 = target_logits.dtype, target_logits.get_device(), target_logits.shape, torch.float32
-    if not (dt in _lib._DTYPE and dev >= 0 and len(shape) == 3 and shape[1] > 0 and shape[2] > 0
-            and draft_tokens.dtype is torch.int64 and uniform.dtype is f32 and noise.dtype is f32
-            and draft_tokens.shape == uniform.shape == (shape[0], shape[1] - 1) and noise.shape == shape[::2]
-            and (draft_logits is None or draft_logits.dtype is dt
-                 and draft_logits.shape == (shape[0], shape[1] - 1, shape[2]) and draft_logits.get_device() == dev)
-            and (temperature is None or temperature.dtype is f32 and temperature.shape == shape[:1]
-                 and temperature.get_device() == dev)
-            and (n_draft is None or n_draft.dtype is torch.int32 and n_draft.shape == shape[:1]
-                 and n_draft.get_device() == dev)
-            and draft_tokens.get_device() == uniform.get_device() == noise.get_device() == dev):
-        _check(target_logits, draft_tokens, uniform, noise, draft_logits, temperature, n_draft)
+    _check(target_logits, draft_tokens, uniform, noise, draft_logits, temperature, n_draft)
+    dev = target_logits.get_device()
     if _current_device() != dev:
         with torch.cuda.device(dev):
             return speculative_verify(target_logits, draft_tokens, uniform, noise, draft_logits, temperature, n_draft)
-    B, R, V = shape
+    B, R, V = target_logits.shape
     K = R - 1
-    ldt_b, ldt_r, unit = target_logits.stride()
-    if unit != 1:
-        target_logits = target_logits.contiguous()
-        ldt_b, ldt_r, _ = target_logits.stride()
-    draft = temp = count = None
-    ldd_b = ldd_r = 0
-    if draft_logits is not None and K > 0:
-        ldd_b, ldd_r, unit = draft_logits.stride()
-        if unit != 1:
-            draft_logits = draft_logits.contiguous()
-            ldd_b, ldd_r, _ = draft_logits.stride()
-        draft = draft_logits.data_ptr()
-    ld_x, unit = draft_tokens.stride()
-    if unit != 1:
-        draft_tokens = draft_tokens.contiguous()
-        ld_x = draft_tokens.stride(0)
-    ld_u, unit = uniform.stride()
-    if unit != 1:
-        uniform = uniform.contiguous()
-        ld_u = uniform.stride(0)
-    ld_n, unit = noise.stride()
-    if unit != 1:
-        noise = noise.contiguous()
-        ld_n = noise.stride(0)
-    if temperature is not None:
-        temperature = temperature.contiguous()
-        temp = temperature.data_ptr()
-    if n_draft is not None:
-        n_draft = n_draft.contiguous()
-        count = n_draft.data_ptr()
+    if K == 0:
+        draft_logits = None
+    unit = lambda t: t if t is None or t.stride(-1) == 1 else t.contiguous()  # noqa: E731
+    target_logits, draft_logits, draft_tokens, uniform, noise, temperature, n_draft = map(
+        unit, (target_logits, draft_logits, draft_tokens, uniform, noise, temperature, n_draft))
     tokens = target_logits.new_empty((B, R), dtype=torch.int64)
     accepted = target_logits.new_empty((B,), dtype=torch.int64)
-    logprobs = target_logits.new_empty((B, R), dtype=f32)
-    stream = _current_stream(dev)
+    logprobs = target_logits.new_empty((B, R), dtype=torch.float32)
+    lib, stream = _lib.lib(), _current_stream(dev)
     # past the counters that paged_attention keeps zero in the stream's scratch
     skip = _lib.PAGED_COUNTER_BYTES
-    ws, ws_bytes, owner = _lib.stream_scratch(dev, stream, _workspace_bytes(dev, B, K, V) + skip, 0)
-    rc = _lib.lib().simsd_speculative_verify(
-        target_logits.data_ptr(), ldt_b, ldt_r, draft, ldd_b, ldd_r, draft_tokens.data_ptr(), ld_x, uniform.data_ptr(),
-        ld_u, noise.data_ptr(), ld_n, temp, count, B, K, V, _lib._DTYPE[dt], tokens.data_ptr(), accepted.data_ptr(),
-        logprobs.data_ptr(), ws + skip, ws_bytes - skip, _lib.error_ptr(dev), stream)
-    if rc:
-        _lib.check(rc, "speculative_verify")
+    ws, ws_bytes, _owner = _lib.stream_scratch(dev, stream,
+                                               lib.simsd_speculative_verify_workspace_size(B, K, V) + skip, 0)
+    rc = lib.simsd_speculative_verify(
+        target_logits.data_ptr(), target_logits.stride(0), target_logits.stride(1),
+        draft_logits.data_ptr() if draft_logits is not None else None,
+        draft_logits.stride(0) if draft_logits is not None else 0,
+        draft_logits.stride(1) if draft_logits is not None else 0, draft_tokens.data_ptr(), draft_tokens.stride(0),
+        uniform.data_ptr(), uniform.stride(0), noise.data_ptr(), noise.stride(0),
+        temperature.data_ptr() if temperature is not None else None, n_draft.data_ptr() if n_draft is not None else None,
+        B, K, V, _lib.dtype_code(target_logits.dtype), tokens.data_ptr(), accepted.data_ptr(), logprobs.data_ptr(),
+        ws + skip, ws_bytes - skip, _lib.error_ptr(dev), stream)
+    _lib.check(rc, "speculative_verify")
     return tokens, accepted, logprobs
-
-
-_WS_SIZES: dict[tuple, int] = {}
-
-
-def _workspace_bytes(dev: int, B: int, K: int, V: int) -> int:
-    """simsd_speculative_verify_workspace_size, memoised (arithmetic for a device)."""
-    key = (dev, B, K, V)
-    size = _WS_SIZES.get(key)
-    if size is None:
-        size = _WS_SIZES[key] = _lib.lib().simsd_speculative_verify_workspace_size(B, K, V)
-    return size
