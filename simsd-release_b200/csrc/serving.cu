@@ -104,7 +104,7 @@ SpecPlan spec_plan(int B, int K, int V) {
   p.parts = (int)cdiv(V, p.blocks * SV_BLOCK);
   p.chunk = (int)std::min<long long>(cdiv(cdiv((long long)B * V, 4 * sms), SV_CHUNK), cdiv(V, SV_CHUNK)) * SV_CHUNK;
   p.chunks = (int)cdiv(V, p.chunk);
-  p.cand_at = align256((size_t)B * (2 * K + 1) * p.parts * sizeof(float2));
+  p.cand_at = align256((size_t)B * (2 * K + 1) * p.parts * sizeof(SpecPart));
   p.done_at = p.cand_at + align256((size_t)B * p.chunks * sizeof(float2));
   p.bytes = p.done_at + align256((size_t)B * sizeof(int));
   return p;
@@ -115,7 +115,7 @@ int verify_drafts(const SpecVerifyArgs& a, void* stream) {
   const dim3 grid((unsigned)cdiv(a.parts, SV_WARPS), (unsigned)a.B, (unsigned)(a.draft ? 2 * a.K + 1 : a.K + 1));
   int rc = launch_on(spec_stat_kernel<DT>, grid, SV_THREADS, 0, stream, false, a);
   if (rc != SIMSD_OK) return rc;
-  return launch_on(spec_draw_kernel<DT>, dim3((unsigned)(a.B * a.chunks)), SV_THREADS, (size_t)(2 * a.K + 1) * 2 * sizeof(float),
+  return launch_on(spec_draw_kernel<DT>, dim3((unsigned)(a.B * a.chunks)), SV_THREADS, (size_t)(2 * a.K + 1) * sizeof(SpecPart),
                    stream, true, a);
 }
 
@@ -283,7 +283,7 @@ int simsd_speculative_verify(const void* target_logits, int64_t ldt_b, int64_t l
   const SpecPlan pl = spec_plan(B, K, V);
   uint8_t* ws = reinterpret_cast<uint8_t*>(workspace);
   if ((long long)B * pl.chunks > 0x7fffffffLL) return SIMSD_ERR_UNSUPPORTED;
-  a.part = reinterpret_cast<float2*>(ws);
+  a.part = reinterpret_cast<SpecPart*>(ws);
   a.cand = reinterpret_cast<float2*>(ws + pl.cand_at);
   a.done = reinterpret_cast<int*>(ws + pl.done_at);
   a.blocks = pl.blocks;

@@ -29,6 +29,15 @@
 
 namespace simsd {
 
+// What a part of a row comes to.  A likely token leaves a sum of 1 and a little,
+// whose logarithm is that little: the sums of lanes and parts are joined in 64 bits
+// (and a lane's run in eight 32-bit ones), so that log p keeps its relative precision.
+struct SpecPart {
+  double s;                 // sum of exp((x - m) / T)
+  float m;                  // maximum
+  int at;                   // greedy sequences: where the maximum is first
+};
+
 struct SpecVerifyArgs {
   const void* target;       // [B, K + 1, V]
   const void* draft;        // [B, K, V] or nullptr
@@ -40,8 +49,7 @@ struct SpecVerifyArgs {
   long long* out_tokens;    // [B, K + 1]
   long long* out_accepted;  // [B]
   float* out_logprobs;      // [B, K + 1]
-  float2* part;             // [B, 2 K + 1, parts]: maximum, sum of exp((x - max) / T) of a part of a row; in
-                            // greedy sequences the place of the maximum instead of the sum
+  SpecPart* part;           // [B, 2 K + 1, parts]
   float2* cand;             // [B, chunks]: best race and its token
   int* done;                // [B]: CTAs of the sequence that have finished, zeroed by the first kernel
   int* err;
@@ -128,11 +136,11 @@ __device__ __forceinline__ float spec_max(const uint4 (&raw)[VL]) {
 // Sum of exp2((x - m) c) over a lane's vectors, two values an instruction but for
 // the exponential
 template <int DT, int VL>
-__device__ __forceinline__ float spec_sum(const uint4 (&raw)[VL], float m, float c) {
-  uint64_t nm, cc, sum = 0;
+__device__ __forceinline__ double spec_sum(const uint4 (&raw)[VL], float m, float c) {
+  uint64_t nm, cc, sum[4] = {0, 0, 0, 0};
   asm("mov.b64 %0, {%1, %1};" : "=l"(nm) : "f"(-m));
   asm("mov.b64 %0, {%1, %1};" : "=l"(cc) : "f"(c));
-  auto see = [&](float a, float b) {
+  auto see = [&](float a, float b, uint64_t& to) {
     uint64_t x;
     asm("mov.b64 %0, {%1, %2};" : "=l"(x) : "f"(a), "f"(b));
     asm("add.rn.f32x2 %0, %0, %1;" : "+l"(x) : "l"(nm));
@@ -140,18 +148,21 @@ __device__ __forceinline__ float spec_sum(const uint4 (&raw)[VL], float m, float
     asm("mov.b64 {%0, %1}, %2;" : "=f"(a), "=f"(b) : "l"(x));
     a = spec_exp2(a), b = spec_exp2(b);
     asm("mov.b64 %0, {%1, %2};" : "=l"(x) : "f"(a), "f"(b));
-    asm("add.rn.f32x2 %0, %0, %1;" : "+l"(sum) : "l"(x));
+    asm("add.rn.f32x2 %0, %0, %1;" : "+l"(to) : "l"(x));
   };
 #pragma unroll
   for (int i = 0; i < VL; ++i) {
     float f[SpecVec<DT>::N];
     SpecVec<DT>::unpack(raw[i], f);
 #pragma unroll
-    for (int e = 0; e < SpecVec<DT>::N; e += 2) see(f[e], f[e + 1]);
+    for (int e = 0; e < SpecVec<DT>::N; e += 2) see(f[e], f[e + 1], sum[(i * SpecVec<DT>::N + e) / 2 % 4]);
   }
-  float a, b;
-  asm("mov.b64 {%0, %1}, %2;" : "=f"(a), "=f"(b) : "l"(sum));
-  return a + b;
+  asm("add.rn.f32x2 %0, %0, %1;" : "+l"(sum[0]) : "l"(sum[1]));
+  asm("add.rn.f32x2 %0, %0, %1;" : "+l"(sum[2]) : "l"(sum[3]));
+  float a, b, c2, d;
+  asm("mov.b64 {%0, %1}, %2;" : "=f"(a), "=f"(b) : "l"(sum[0]));
+  asm("mov.b64 {%0, %1}, %2;" : "=f"(c2), "=f"(d) : "l"(sum[2]));
+  return ((double)a + b) + ((double)c2 + d);
 }
 
 // Where a row of V logits starts to be 16-byte aligned, and its whole vectors.
@@ -178,7 +189,7 @@ __device__ __forceinline__ const void* spec_row_ptr(const SpecVerifyArgs& p, int
 
 // Grid: x parts of a row, y sequences, z rows
 template <int DT>
-__global__ void __launch_bounds__(SV_THREADS, 4) spec_stat_kernel(const SpecVerifyArgs p) {
+__global__ void __launch_bounds__(SV_THREADS, DT == 2 ? 3 : 4) spec_stat_kernel(const SpecVerifyArgs p) {
   griddep_launch_dependents();
   griddep_wait();
   constexpr int N = SpecVec<DT>::N, VL = SV_BLOCK / N / 32;    // vectors per lane
@@ -217,10 +228,11 @@ __global__ void __launch_bounds__(SV_THREADS, 4) spec_stat_kernel(const SpecVeri
     for (int k = 16; k > 0; k >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, k));
     return m;
   };
-  float m = spec_clean(warp_max(fmaxf(extra, extra2))), s = 0.0f;   // s: this lane's
+  float m = spec_clean(warp_max(fmaxf(extra, extra2)));
+  double s = 0.0;                                        // this lane's
   int at = 0x7fffffff;                                   // greedy: the first place of m that this lane saw
   if (m != -INFINITY) {
-    s = spec_exp2((extra - m) * c) + spec_exp2((extra2 - m) * c);
+    s = (double)spec_exp2((extra - m) * c) + spec_exp2((extra2 - m) * c);
     if (extra2 == m) at = tail + lane;
     if (extra == m) at = lane;
   }
@@ -244,9 +256,9 @@ __global__ void __launch_bounds__(SV_THREADS, 4) spec_stat_kernel(const SpecVeri
       }
       continue;
     }
-    float add = spec_sum<DT, VL>(raw, m, c);
+    double add = spec_sum<DT, VL>(raw, m, c);
     if (!(add < INFINITY)) {                             // NaN or +inf among the lane's logits
-      add = 0.0f;
+      add = 0.0;
 #pragma unroll
       for (int i = 0; i < VL; ++i) {
         float f[N];
@@ -263,50 +275,41 @@ __global__ void __launch_bounds__(SV_THREADS, 4) spec_stat_kernel(const SpecVeri
     at = min(at, __shfl_xor_sync(0xffffffffu, at, k));
   }
   if (lane == 0)
-    p.part[((long long)b * (2 * p.K + 1) + r) * p.parts + part] = make_float2(m, c == 0.0f ? __int_as_float(at) : s);
+    p.part[((long long)b * (2 * p.K + 1) + r) * p.parts + part] = {s, m, at};
 }
 
-// Maximum, and sum or, for greedy sequences, first place of the maximum of row r, by one warp
-__device__ __forceinline__ void spec_join_row(const SpecVerifyArgs& p, int b, int r, float c, float& m, float& s) {
+// Row r from its parts, by one warp (every lane has the result)
+__device__ __forceinline__ SpecPart spec_join_row(const SpecVerifyArgs& p, int b, int r, float c) {
   constexpr int HOLD = 3;                          // parts that a lane holds
   const int lane = threadIdx.x & 31;
-  const float2* part = p.part + ((long long)b * (2 * p.K + 1) + r) * p.parts;
-  float2 x[HOLD];
+  const SpecPart* part = p.part + ((long long)b * (2 * p.K + 1) + r) * p.parts;
+  auto get = [&](int i) {
+    const int4 x = __ldcg(reinterpret_cast<const int4*>(part + i));
+    return SpecPart{__hiloint2double(x.y, x.x), __int_as_float(x.z), x.w};
+  };
+  SpecPart x[HOLD];
 #pragma unroll
-  for (int k = 0; k < HOLD; ++k) {
-    const int i = lane + k * 32;
-    x[k] = i < p.parts ? __ldcg(part + i) : make_float2(-INFINITY, 0.0f);
+  for (int k = 0; k < HOLD; ++k) x[k] = lane + k * 32 < p.parts ? get(lane + k * 32) : SpecPart{0.0, -INFINITY, 0x7fffffff};
+  SpecPart y = {0.0, -INFINITY, 0x7fffffff};
+#pragma unroll
+  for (int k = 0; k < HOLD; ++k) y.m = fmaxf(y.m, x[k].m);
+  for (int i = lane + HOLD * 32; i < p.parts; i += 32) y.m = fmaxf(y.m, get(i).m);
+#pragma unroll
+  for (int k = 16; k > 0; k >>= 1) y.m = fmaxf(y.m, __shfl_xor_sync(0xffffffffu, y.m, k));
+  if (y.m == -INFINITY) return y;
+  auto see = [&](const SpecPart& z) {
+    y.s += z.s * spec_exp2((z.m - y.m) * c);
+    if (z.m == y.m) y.at = min(y.at, z.at);
+  };
+#pragma unroll
+  for (int k = 0; k < HOLD; ++k) see(x[k]);
+  for (int i = lane + HOLD * 32; i < p.parts; i += 32) see(get(i));
+#pragma unroll
+  for (int k = 16; k > 0; k >>= 1) {
+    y.s += __shfl_xor_sync(0xffffffffu, y.s, k);
+    y.at = min(y.at, __shfl_xor_sync(0xffffffffu, y.at, k));
   }
-  m = -INFINITY;
-#pragma unroll
-  for (int k = 0; k < HOLD; ++k) m = fmaxf(m, x[k].x);
-  for (int i = lane + HOLD * 32; i < p.parts; i += 32) m = fmaxf(m, __ldcg(part + i).x);
-#pragma unroll
-  for (int k = 16; k > 0; k >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, k));
-  s = 0.0f;
-  if (m == -INFINITY) return;
-  if (c == 0.0f) {
-    int at = 0x7fffffff;
-#pragma unroll
-    for (int k = 0; k < HOLD; ++k)
-      if (x[k].x == m) at = min(at, __float_as_int(x[k].y));
-    for (int i = lane + HOLD * 32; i < p.parts; i += 32) {
-      const float2 y = __ldcg(part + i);
-      if (y.x == m) at = min(at, __float_as_int(y.y));
-    }
-#pragma unroll
-    for (int k = 16; k > 0; k >>= 1) at = min(at, __shfl_xor_sync(0xffffffffu, at, k));
-    s = __int_as_float(at);
-    return;
-  }
-#pragma unroll
-  for (int k = 0; k < HOLD; ++k) s = fmaf(x[k].y, spec_exp2((x[k].x - m) * c), s);
-  for (int i = lane + HOLD * 32; i < p.parts; i += 32) {
-    const float2 y = __ldcg(part + i);
-    s = fmaf(y.y, spec_exp2((y.x - m) * c), s);
-  }
-#pragma unroll
-  for (int k = 16; k > 0; k >>= 1) s += __shfl_xor_sync(0xffffffffu, s, k);
+  return y;
 }
 
 // The best race so far, in ascending order of tokens per thread
@@ -344,7 +347,7 @@ __global__ void __launch_bounds__(SV_THREADS) spec_draw_kernel(const SpecVerifyA
   griddep_launch_dependents();
   griddep_wait();
   constexpr int N = SpecVec<DT>::N;
-  extern __shared__ float sv_rows[];               // [2 K + 1][2]: maximum, sum (greedy: place of the maximum)
+  extern __shared__ SpecPart sv_rows[];            // [2 K + 1]
   __shared__ SpecBest s_best[SV_WARPS];
   __shared__ int s_kept, s_last;
   __shared__ bool s_bad;
@@ -368,17 +371,16 @@ __global__ void __launch_bounds__(SV_THREADS) spec_draw_kernel(const SpecVerifyA
   const int R = d + 1 + (p.draft ? d : 0);
   for (int k = SV_WARPS - 1 - warp; k < R; k += SV_WARPS) {
     const int r = k <= d ? k : p.K + k - d;
-    float m, s;
-    spec_join_row(p, b, r, c, m, s);
-    if (lane == 0) sv_rows[r * 2] = m, sv_rows[r * 2 + 1] = s;
+    const SpecPart y = spec_join_row(p, b, r, c);
+    if (lane == 0) sv_rows[r] = y;
   }
   __syncthreads();
   // the probability of token v, whose logit is x, in row r
   auto prob = [&](int r, float x, int v) {
-    const float m = sv_rows[r * 2], s = sv_rows[r * 2 + 1];
-    if (m == -INFINITY) return 0.0f;
-    if (c == 0.0f) return v == __float_as_int(s) ? 1.0f : 0.0f;
-    return spec_exp2((spec_clean(x) - m) * c) / s;
+    const SpecPart& y = sv_rows[r];
+    if (y.m == -INFINITY) return 0.0f;
+    if (c == 0.0f) return v == y.at ? 1.0f : 0.0f;
+    return spec_exp2((spec_clean(x) - y.m) * c) / (float)y.s;
   };
   if (warp == 0) {
     int kept = d;
@@ -411,8 +413,8 @@ __global__ void __launch_bounds__(SV_THREADS) spec_draw_kernel(const SpecVerifyA
   const int hit = minus && !p.draft ? (int)xs[a] : -1;
   const float* e = p.noise + b * p.ld_n;
   auto law = [&](int r) {
-    const float m = sv_rows[r * 2];
-    return m == -INFINITY ? SpecLaw{0.0f, 0.0f} : SpecLaw{m, 1.0f / sv_rows[r * 2 + 1]};
+    const SpecPart& y = sv_rows[r];
+    return y.m == -INFINITY ? SpecLaw{0.0f, 0.0f} : SpecLaw{y.m, 1.0f / (float)y.s};
   };
   const SpecLaw pt = law(a), pd = dr ? law(p.K + 1 + a) : SpecLaw{0.0f, 0.0f};
   SpecBest best = {-1.0f, 0x7fffffff};
@@ -462,8 +464,8 @@ __global__ void __launch_bounds__(SV_THREADS) spec_draw_kernel(const SpecVerifyA
   __syncthreads();
   if (!s_last) return;
   // the sequence's last CTA: the best of all chunks, and the outputs
-  int drawn = __float_as_int(sv_rows[a * 2 + 1]);
-  if (sv_rows[a * 2] == -INFINITY) {
+  int drawn = sv_rows[a].at;
+  if (sv_rows[a].m == -INFINITY) {
     drawn = 0;
   } else if (c != 0.0f) {
     best = {-1.0f, 0x7fffffff};
@@ -489,13 +491,13 @@ __global__ void __launch_bounds__(SV_THREADS) spec_draw_kernel(const SpecVerifyA
     const int v = i < a ? (int)xs[i] : drawn;
     float lp = 0.0f;
     if (i <= a) {
-      const float m = sv_rows[i * 2], s = sv_rows[i * 2 + 1];
-      if (m == -INFINITY)
+      const SpecPart& y = sv_rows[i];
+      if (y.m == -INFINITY)
         lp = -INFINITY;
       else if (c == 0.0f)
-        lp = v == __float_as_int(s) ? 0.0f : -INFINITY;
+        lp = v == y.at ? 0.0f : -INFINITY;
       else
-        lp = (spec_logit(spec_row_ptr(p, b, i), v, DT) - m) / fmaxf(T, 1e-30f) - logf(s);
+        lp = (spec_logit(spec_row_ptr(p, b, i), v, DT) - y.m) / fmaxf(T, 1e-30f) - log1pf((float)(y.s - 1.0));
     }
     p.out_tokens[(long long)b * (p.K + 1) + i] = i <= a ? v : -1;
     p.out_logprobs[(long long)b * (p.K + 1) + i] = lp;
