@@ -43,65 +43,90 @@ struct PagedAppendArgs {
   float eps;
 };
 
-constexpr int PA_THREADS = 256, PA_UNROLL = 4;
+constexpr int PA_THREADS = 128, PA_UNROLL = 3;
 
+// Two fp32 values in a 64-bit register, worked on by one instruction
+__device__ __forceinline__ uint64_t f2_pack(float a, float b) {
+  uint64_t r;
+  asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(a), "f"(b));
+  return r;
+}
+__device__ __forceinline__ float2 f2_unpack(uint64_t v) {
+  float2 r;
+  asm("mov.b64 {%0, %1}, %2;" : "=f"(r.x), "=f"(r.y) : "l"(v));
+  return r;
+}
+__device__ __forceinline__ uint64_t f2_mul(uint64_t a, uint64_t b) {
+  uint64_t r;
+  asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+  return r;
+}
+__device__ __forceinline__ uint64_t f2_fma(uint64_t a, uint64_t b, uint64_t c) {
+  uint64_t r;
+  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(a), "l"(b), "l"(c));
+  return r;
+}
+
+// 8 16-bit elements as four pairs of fp32, and back
 template <bool BF>
-__device__ __forceinline__ void paged_unpack4(uint2 u, float (&v)[4]) {
-  const uint32_t w[2] = {u.x, u.y};
+__device__ __forceinline__ void paged_unpack8(uint4 u, uint64_t (&v)[4]) {
+  const uint32_t w[4] = {u.x, u.y, u.z, u.w};
 #pragma unroll
-  for (int i = 0; i < 2; ++i) {
+  for (int i = 0; i < 4; ++i) {
     if constexpr (BF) {
-      v[2 * i] = __uint_as_float(w[i] << 16);
-      v[2 * i + 1] = __uint_as_float(w[i] & 0xffff0000u);
+      v[i] = f2_pack(__uint_as_float(w[i] << 16), __uint_as_float(w[i] & 0xffff0000u));
     } else {
       const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&w[i]));
-      v[2 * i] = f.x;
-      v[2 * i + 1] = f.y;
+      v[i] = f2_pack(f.x, f.y);
     }
   }
 }
 template <bool BF>
-__device__ __forceinline__ uint2 paged_pack4(const float (&f)[4]) {
-  uint2 r;
-  if constexpr (BF) {
-    asm("cvt.rn.bf16x2.f32 %0, %1, %2;" : "=r"(r.x) : "f"(f[1]), "f"(f[0]));
-    asm("cvt.rn.bf16x2.f32 %0, %1, %2;" : "=r"(r.y) : "f"(f[3]), "f"(f[2]));
-  } else {
-    asm("cvt.rn.f16x2.f32 %0, %1, %2;" : "=r"(r.x) : "f"(f[1]), "f"(f[0]));
-    asm("cvt.rn.f16x2.f32 %0, %1, %2;" : "=r"(r.y) : "f"(f[3]), "f"(f[2]));
+__device__ __forceinline__ uint4 paged_pack8(const uint64_t (&v)[4]) {
+  uint32_t w[4];
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    const float2 f = f2_unpack(v[i]);
+    if constexpr (BF)
+      asm("cvt.rn.bf16x2.f32 %0, %1, %2;" : "=r"(w[i]) : "f"(f.y), "f"(f.x));
+    else
+      asm("cvt.rn.f16x2.f32 %0, %1, %2;" : "=r"(w[i]) : "f"(f.y), "f"(f.x));
   }
-  return r;
+  return make_uint4(w[0], w[1], w[2], w[3]);
 }
 
-// One CTA per token.  D / 8 neighbouring threads share a head; PA_THREADS is a
+// One CTA per token.  D / 16 neighbouring threads share a head; PA_THREADS is a
 // multiple of that, so a thread keeps its place in the head over its heads and its
-// rotary row and weights stay in registers.  The first R / 8 of them hold elements
-// 4 j .. 4 j + 3 and their pairs R / 2 further, so the rotation needs no exchange
-// (8-byte loads and stores; a warp's are still whole 128-byte lines); the others
-// hold the 8 next elements of the unrotated rest.  HBM bounds it: the row's loads
-// (PA_UNROLL heads a thread at a time) are issued before the slot, the position and
-// the rotary row are known, so that one round of latency covers them all.
+// rotary row and weights stay in registers.  The first R / 16 of them hold elements
+// 8 j .. 8 j + 7 and their pairs R / 2 further, so the rotation needs no exchange;
+// the others hold the 16 next elements of the unrotated rest.
+//
+// HBM bounds it, with the issue of instructions close behind (16 elements a thread
+// and two a multiplication, against 8 and one: 55 -> @ us for 8192 tokens of 48 heads
+// x 128).  The row's loads, PA_UNROLL heads a thread at a time, are issued before
+// the slot, the position and the rotary row are known, so that one round of latency
+// covers them all.
 template <int D, bool BF>
-__global__ void __launch_bounds__(PA_THREADS, 4) paged_append_kernel(const PagedAppendArgs p) {
+__global__ void __launch_bounds__(PA_THREADS, 5) paged_append_kernel(const PagedAppendArgs p) {
   griddep_launch_dependents();
   griddep_wait();
-  constexpr int LANES = D / 8, HEADS = PA_THREADS / LANES;    // threads of a head, heads at a time
+  constexpr int LANES = D / 16, HEADS = PA_THREADS / LANES;   // threads of a head, heads at a time
   const int t = blockIdx.x;
   const int tid = threadIdx.x, lane = tid & 31;
   const int j = tid % LANES, h_at = tid / LANES;
   const int H = p.Hq + 2 * p.Hk;
-  const bool pair = 8 * j < p.R;                 // this thread's elements are rotated
-  const int e0 = pair ? 4 * j : 8 * j, e1 = pair ? p.R / 2 + 4 * j : 8 * j + 4;
+  const bool pair = 16 * j < p.R;                // this thread's elements are rotated
+  const int e0 = pair ? 8 * j : 16 * j, e1 = pair ? p.R / 2 + 8 * j : 16 * j + 8;
   const uint16_t* row = reinterpret_cast<const uint16_t*>(p.qkv) + t * p.ldqkv;
-  uint2 lo[PA_UNROLL], hi[PA_UNROLL];
+  uint4 lo[PA_UNROLL], hi[PA_UNROLL];
   auto fetch = [&](int h0) {
 #pragma unroll
     for (int u = 0; u < PA_UNROLL; ++u) {
       const int h = h0 + u * HEADS + h_at;
-      lo[u] = hi[u] = make_uint2(0, 0);
+      lo[u] = hi[u] = make_uint4(0, 0, 0, 0);
       if (h < H) {
-        lo[u] = __ldg(reinterpret_cast<const uint2*>(row + h * D + e0));
-        hi[u] = __ldg(reinterpret_cast<const uint2*>(row + h * D + e1));
+        lo[u] = __ldg(reinterpret_cast<const uint4*>(row + h * D + e0));
+        hi[u] = __ldg(reinterpret_cast<const uint4*>(row + h * D + e1));
       }
     }
   };
@@ -111,17 +136,26 @@ __global__ void __launch_bounds__(PA_THREADS, 4) paged_append_kernel(const Paged
   const bool bad = slot >= p.n_slots || (slot >= 0 && (pos < 0 || pos >= p.n_pos));
   if (bad && tid == 0 && p.err) atomicOr(p.err, SIMSD_DEV_ERR_BAD_INDEX);
   const bool live = slot >= 0 && !bad;
-  float4 c = make_float4(1.0f, 1.0f, 1.0f, 1.0f), s = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+  uint64_t c[4], s[4], ns[4];
+#pragma unroll
+  for (int e = 0; e < 4; ++e) c[e] = s[e] = ns[e] = 0;
   if (pair && live) {
-    const long long at = pos * (p.R / 2) + 4 * j;
-    c = __ldg(reinterpret_cast<const float4*>(p.cos + at));
-    s = __ldg(reinterpret_cast<const float4*>(p.sin + at));
+    const long long at = pos * (p.R / 2) + 8 * j;
+#pragma unroll
+    for (int e = 0; e < 2; ++e) {
+      const float4 cv = __ldg(reinterpret_cast<const float4*>(p.cos + at) + e);
+      const float4 sv = __ldg(reinterpret_cast<const float4*>(p.sin + at) + e);
+      c[2 * e] = f2_pack(cv.x, cv.y), c[2 * e + 1] = f2_pack(cv.z, cv.w);
+      s[2 * e] = f2_pack(sv.x, sv.y), s[2 * e + 1] = f2_pack(sv.z, sv.w);
+      ns[2 * e] = f2_pack(-sv.x, -sv.y), ns[2 * e + 1] = f2_pack(-sv.z, -sv.w);
+    }
   }
   long long base = 0;
   if (live) {
     const long long page = p.n_slots <= 0x7fffffffLL ? p.page_div((int)slot) : slot / p.page_size;
     base = page * p.ld_page + (slot - page * p.page_size) * p.ld_tok;
   }
+  const uint32_t mask = ((1u << LANES) - 1u) << (lane & ~(LANES - 1));
   uint16_t* q = reinterpret_cast<uint16_t*>(p.q_out) + (long long)t * p.Hq * D;
   for (int h0 = 0; h0 < H; h0 += HEADS * PA_UNROLL) {
     if (h0 > 0) fetch(h0);
@@ -130,47 +164,50 @@ __global__ void __launch_bounds__(PA_THREADS, 4) paged_append_kernel(const Paged
       const int h = h0 + u * HEADS + h_at;
       if (h0 + u * HEADS >= H) break;              // the whole CTA
       const int kv = h - p.Hq;
-      uint2 a = lo[u], b = hi[u];
+      uint4 a = lo[u], b = hi[u];
       if (kv < p.Hk) {                             // q and k; all of a head's threads take the same side
-        float x[4], y[4];
-        paged_unpack4<BF>(a, x);
-        paged_unpack4<BF>(b, y);
+        uint64_t x[4], y[4];
+        paged_unpack8<BF>(a, x);
+        paged_unpack8<BF>(b, y);
         const uint16_t* w = reinterpret_cast<const uint16_t*>(kv < 0 ? p.qw : p.kw);
         if (w != nullptr) {
-          float ss = 0.0f;
+          uint64_t sx = 0, sy = 0;
 #pragma unroll
-          for (int e = 0; e < 4; ++e) ss = fmaf(x[e], x[e], fmaf(y[e], y[e], ss));
-          const uint32_t mask = ((1u << LANES) - 1u) << (lane & ~(LANES - 1));
+          for (int e = 0; e < 4; ++e) sx = f2_fma(x[e], x[e], sx), sy = f2_fma(y[e], y[e], sy);
+          const float2 s0 = f2_unpack(sx), s1 = f2_unpack(sy);
+          float ss = (s0.x + s0.y) + (s1.x + s1.y);
 #pragma unroll
           for (int m = LANES / 2; m > 0; m >>= 1) ss += __shfl_xor_sync(mask, ss, m);
           const float inv = rsqrtf(fmaf(ss, 1.0f / D, p.eps));
-          float wx[4], wy[4];
-          paged_unpack4<BF>(__ldg(reinterpret_cast<const uint2*>(w + e0)), wx);
-          paged_unpack4<BF>(__ldg(reinterpret_cast<const uint2*>(w + e1)), wy);
+          const uint64_t inv2 = f2_pack(inv, inv);
+          uint64_t wx[4], wy[4];
+          paged_unpack8<BF>(__ldg(reinterpret_cast<const uint4*>(w + e0)), wx);
+          paged_unpack8<BF>(__ldg(reinterpret_cast<const uint4*>(w + e1)), wy);
 #pragma unroll
-          for (int e = 0; e < 4; ++e) x[e] = x[e] * inv * wx[e], y[e] = y[e] * inv * wy[e];
+          for (int e = 0; e < 4; ++e) x[e] = f2_mul(f2_mul(x[e], inv2), wx[e]), y[e] = f2_mul(f2_mul(y[e], inv2), wy[e]);
         }
-        const float cc[4] = {c.x, c.y, c.z, c.w}, sc[4] = {s.x, s.y, s.z, s.w};
-        float ox[4], oy[4];
+        if (pair) {
 #pragma unroll
-        for (int e = 0; e < 4; ++e) {
-          ox[e] = pair ? fmaf(-y[e], sc[e], x[e] * cc[e]) : x[e];
-          oy[e] = pair ? fmaf(x[e], sc[e], y[e] * cc[e]) : y[e];
+          for (int e = 0; e < 4; ++e) {
+            const uint64_t x0 = x[e];
+            x[e] = f2_fma(y[e], ns[e], f2_mul(x0, c[e]));
+            y[e] = f2_fma(x0, s[e], f2_mul(y[e], c[e]));
+          }
         }
-        a = paged_pack4<BF>(ox);
-        b = paged_pack4<BF>(oy);
+        a = paged_pack8<BF>(x);
+        b = paged_pack8<BF>(y);
       }
       uint16_t* dst;
       if (kv < 0) {
         dst = q + h * D;
-        if (!live) a = b = make_uint2(0, 0);
+        if (!live) a = b = make_uint4(0, 0, 0, 0);
       } else {
         if (!live || h >= H) continue;
         dst = kv < p.Hk ? reinterpret_cast<uint16_t*>(p.k_cache) + base + kv * p.ld_head
                         : reinterpret_cast<uint16_t*>(p.v_cache) + base + (kv - p.Hk) * p.ld_head;
       }
-      *reinterpret_cast<uint2*>(dst + e0) = a;
-      *reinterpret_cast<uint2*>(dst + e1) = b;
+      *reinterpret_cast<uint4*>(dst + e0) = a;
+      *reinterpret_cast<uint4*>(dst + e1) = b;
     }
   }
 }
