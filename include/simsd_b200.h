@@ -511,7 +511,7 @@ int simsd_moe_ep_return(const void* y, int64_t ldy, const int32_t* recv_expert, 
  * caches and a zero q row, and its position is not read.  qkv [T, (Hq + 2 Hk)
  * head_dim] with row stride ldqkv (q heads, k heads, v heads), q_out [T, Hq,
  * head_dim].  Slots of one call are distinct.  rotary_dim: a multiple of 16, <=
- * head_dim.  Replaces, for a batch, the q/k norm, rotary embedding and cache
+ * head_dim.  (Hq + 2 Hk) head_dim <= 36864 (more: SIMSD_ERR_UNSUPPORTED).  Replaces, for a batch, the q/k norm, rotary embedding and cache
  * write of sdar/modeling_sdar.py:197-302.
  */
 int simsd_paged_append(const void* qkv, int64_t ldqkv, int T, int Hq, int Hk, int head_dim, int rotary_dim,

@@ -38,12 +38,12 @@ struct PagedAppendArgs {
   void* v_cache;
   int* err;
   long long ldqkv, n_pos, n_slots, ld_page, ld_head, ld_tok;
-  int Hq, Hk, R, page_size;
+  int T, Hq, Hk, R, page_size;
   PagedDiv page_div;        // by page_size
   float eps;
 };
 
-constexpr int PA_THREADS = 128, PA_UNROLL = 3;
+constexpr int PA_THREADS = 128, PA_STAGES = 3, PA_CTAS_PER_SM = 4;
 
 // Two fp32 values in a 64-bit register, worked on by one instruction
 __device__ __forceinline__ uint64_t f2_pack(float a, float b) {
@@ -95,76 +95,99 @@ __device__ __forceinline__ uint4 paged_pack8(const uint64_t (&v)[4]) {
   return make_uint4(w[0], w[1], w[2], w[3]);
 }
 
-// One CTA per token.  D / 16 neighbouring threads share a head; PA_THREADS is a
-// multiple of that, so a thread keeps its place in the head over its heads and its
-// rotary row and weights stay in registers.  The first R / 16 of them hold elements
-// 8 j .. 8 j + 7 and their pairs R / 2 further, so the rotation needs no exchange;
-// the others hold the 16 next elements of the unrotated rest.
+__device__ __forceinline__ void paged_cp16(uint32_t dst, const void* src) {
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(dst), "l"(src) : "memory");
+}
+
+// A CTA takes tokens blockIdx.x, + gridDim.x, ...  D / 16 neighbouring threads share
+// a head; PA_THREADS is a multiple of that, so a thread keeps its place in the head
+// over its heads and its rotary row stays in registers.  The first R / 16 of them
+// hold elements 8 j .. 8 j + 7 and their pairs R / 2 further, so the rotation needs
+// no exchange; the others hold the 16 next elements of the unrotated rest.
 //
-// HBM bounds it, with the issue of instructions close behind (16 elements a thread
-// and two a multiplication, against 8 and one: 55 -> @ us for 8192 tokens of 48 heads
-// x 128).  The row's loads, PA_UNROLL heads a thread at a time, are issued before
-// the slot, the position and the rotary row are known, so that one round of latency
-// covers them all.
+// HBM bounds it, with the issue of instructions close behind (hence 16 elements a
+// thread and two a multiplication).  Loads run ahead: each thread copies its own
+// elements of the next PA_STAGES - 1 tokens into its own places of a ring (cp.async;
+// no barrier, since no thread reads another's), and the rotary row is fetched one
+// token ahead, the slot and position two.
 template <int D, bool BF>
-__global__ void __launch_bounds__(PA_THREADS, 5) paged_append_kernel(const PagedAppendArgs p) {
+__global__ void __launch_bounds__(PA_THREADS, PA_CTAS_PER_SM) paged_append_kernel(const PagedAppendArgs p) {
   griddep_launch_dependents();
   griddep_wait();
   constexpr int LANES = D / 16, HEADS = PA_THREADS / LANES;   // threads of a head, heads at a time
-  const int t = blockIdx.x;
+  constexpr int PLANE = PA_THREADS * 16;                      // bytes of one half of HEADS heads
+  extern __shared__ __align__(16) uint8_t pa_ring[];          // [PA_STAGES][turns][2][PA_THREADS] x 16 bytes
   const int tid = threadIdx.x, lane = tid & 31;
   const int j = tid % LANES, h_at = tid / LANES;
-  const int H = p.Hq + 2 * p.Hk;
+  const int H = p.Hq + 2 * p.Hk, turns = (H + HEADS - 1) / HEADS;
   const bool pair = 16 * j < p.R;                // this thread's elements are rotated
   const int e0 = pair ? 8 * j : 16 * j, e1 = pair ? p.R / 2 + 8 * j : 16 * j + 8;
-  const uint16_t* row = reinterpret_cast<const uint16_t*>(p.qkv) + t * p.ldqkv;
-  uint4 lo[PA_UNROLL], hi[PA_UNROLL];
-  auto fetch = [&](int h0) {
-#pragma unroll
-    for (int u = 0; u < PA_UNROLL; ++u) {
-      const int h = h0 + u * HEADS + h_at;
-      lo[u] = hi[u] = make_uint4(0, 0, 0, 0);
-      if (h < H) {
-        lo[u] = __ldg(reinterpret_cast<const uint4*>(row + h * D + e0));
-        hi[u] = __ldg(reinterpret_cast<const uint4*>(row + h * D + e1));
+  const int stage_bytes = turns * 2 * PLANE;
+  const uint32_t place = smem_u32(pa_ring) + tid * 16;
+
+  int ahead = blockIdx.x;                        // the token whose loads come next, and its stage
+  uint32_t ahead_at = place;
+  auto fetch = [&]() {
+    if (ahead < p.T) {
+      const uint16_t* src = reinterpret_cast<const uint16_t*>(p.qkv) + ahead * p.ldqkv + h_at * D;
+      uint32_t dst = ahead_at;
+      for (int h = h_at; h < H; h += HEADS) {
+        paged_cp16(dst, src + e0);
+        paged_cp16(dst + PLANE, src + e1);
+        src += HEADS * D;
+        dst += 2 * PLANE;
       }
+      ahead += gridDim.x;
+      ahead_at += stage_bytes;
+      if (ahead_at == place + PA_STAGES * stage_bytes) ahead_at = place;
+    }
+    asm volatile("cp.async.commit_group;" ::: "memory");
+  };
+#pragma unroll
+  for (int s = 0; s < PA_STAGES - 1; ++s) fetch();
+
+  struct Place {
+    long long slot, pos;
+  };
+  auto where = [&](int x) { return x < p.T ? Place{p.slots[x], p.positions[x]} : Place{-1, 0}; };
+  auto good = [&](const Place& x) { return x.slot >= 0 && x.slot < p.n_slots && x.pos >= 0 && x.pos < p.n_pos; };
+  float4 row[4];                                 // the next token's cos and sin
+  auto table = [&](const Place& x) {
+    if (pair && good(x)) {
+      const long long at = x.pos * (p.R / 2) + 8 * j;
+      row[0] = __ldg(reinterpret_cast<const float4*>(p.cos + at)), row[1] = __ldg(reinterpret_cast<const float4*>(p.cos + at) + 1);
+      row[2] = __ldg(reinterpret_cast<const float4*>(p.sin + at)), row[3] = __ldg(reinterpret_cast<const float4*>(p.sin + at) + 1);
     }
   };
-  fetch(0);
-  const long long slot = p.slots[t];
-  const long long pos = p.positions[t];
-  const bool bad = slot >= p.n_slots || (slot >= 0 && (pos < 0 || pos >= p.n_pos));
-  if (bad && tid == 0 && p.err) atomicOr(p.err, SIMSD_DEV_ERR_BAD_INDEX);
-  const bool live = slot >= 0 && !bad;
-  uint64_t c[4], s[4], ns[4];
-#pragma unroll
-  for (int e = 0; e < 4; ++e) c[e] = s[e] = ns[e] = 0;
-  if (pair && live) {
-    const long long at = pos * (p.R / 2) + 8 * j;
+  Place now = where(blockIdx.x), next = where(blockIdx.x + gridDim.x);
+  table(now);
+  const uint32_t mask = ((1u << LANES) - 1u) << (lane & ~(LANES - 1));
+  uint32_t at = 0;                               // this token's stage
+  for (int t = blockIdx.x; t < p.T; t += gridDim.x) {
+    uint64_t c[4], s[4], ns[4];
 #pragma unroll
     for (int e = 0; e < 2; ++e) {
-      const float4 cv = __ldg(reinterpret_cast<const float4*>(p.cos + at) + e);
-      const float4 sv = __ldg(reinterpret_cast<const float4*>(p.sin + at) + e);
-      c[2 * e] = f2_pack(cv.x, cv.y), c[2 * e + 1] = f2_pack(cv.z, cv.w);
-      s[2 * e] = f2_pack(sv.x, sv.y), s[2 * e + 1] = f2_pack(sv.z, sv.w);
-      ns[2 * e] = f2_pack(-sv.x, -sv.y), ns[2 * e + 1] = f2_pack(-sv.z, -sv.w);
+      c[2 * e] = f2_pack(row[e].x, row[e].y), c[2 * e + 1] = f2_pack(row[e].z, row[e].w);
+      s[2 * e] = f2_pack(row[2 + e].x, row[2 + e].y), s[2 * e + 1] = f2_pack(row[2 + e].z, row[2 + e].w);
+      ns[2 * e] = f2_pack(-row[2 + e].x, -row[2 + e].y), ns[2 * e + 1] = f2_pack(-row[2 + e].z, -row[2 + e].w);
     }
-  }
-  long long base = 0;
-  if (live) {
-    const long long page = p.n_slots <= 0x7fffffffLL ? p.page_div((int)slot) : slot / p.page_size;
-    base = page * p.ld_page + (slot - page * p.page_size) * p.ld_tok;
-  }
-  const uint32_t mask = ((1u << LANES) - 1u) << (lane & ~(LANES - 1));
-  uint16_t* q = reinterpret_cast<uint16_t*>(p.q_out) + (long long)t * p.Hq * D;
-  for (int h0 = 0; h0 < H; h0 += HEADS * PA_UNROLL) {
-    if (h0 > 0) fetch(h0);
-#pragma unroll
-    for (int u = 0; u < PA_UNROLL; ++u) {
-      const int h = h0 + u * HEADS + h_at;
-      if (h0 + u * HEADS >= H) break;              // the whole CTA
+    const bool live = good(now);
+    if (!live && now.slot >= 0 && tid == 0 && p.err) atomicOr(p.err, SIMSD_DEV_ERR_BAD_INDEX);
+    long long base = 0;
+    if (live) {
+      const long long page = p.n_slots <= 0x7fffffffLL ? p.page_div((int)now.slot) : now.slot / p.page_size;
+      base = page * p.ld_page + (now.slot - page * p.page_size) * p.ld_tok;
+    }
+    now = next;
+    table(now);
+    next = where(t + 2 * gridDim.x);
+    fetch();
+    asm volatile("cp.async.wait_group %0;" ::"n"(PA_STAGES - 1) : "memory");
+    uint16_t* q = reinterpret_cast<uint16_t*>(p.q_out) + (long long)t * p.Hq * D;
+    const uint8_t* from = pa_ring + at + tid * 16;
+    for (int h = h_at; h < H; h += HEADS, from += 2 * PLANE) {
       const int kv = h - p.Hq;
-      uint4 a = lo[u], b = hi[u];
+      uint4 a = *reinterpret_cast<const uint4*>(from), b = *reinterpret_cast<const uint4*>(from + PLANE);
       if (kv < p.Hk) {                             // q and k; all of a head's threads take the same side
         uint64_t x[4], y[4];
         paged_unpack8<BF>(a, x);
@@ -202,13 +225,15 @@ __global__ void __launch_bounds__(PA_THREADS, 5) paged_append_kernel(const Paged
         dst = q + h * D;
         if (!live) a = b = make_uint4(0, 0, 0, 0);
       } else {
-        if (!live || h >= H) continue;
+        if (!live) continue;
         dst = kv < p.Hk ? reinterpret_cast<uint16_t*>(p.k_cache) + base + kv * p.ld_head
                         : reinterpret_cast<uint16_t*>(p.v_cache) + base + (kv - p.Hk) * p.ld_head;
       }
       *reinterpret_cast<uint4*>(dst + e0) = a;
       *reinterpret_cast<uint4*>(dst + e1) = b;
     }
+    at += stage_bytes;
+    if (at == (uint32_t)(PA_STAGES * stage_bytes)) at = 0;
   }
 }
 

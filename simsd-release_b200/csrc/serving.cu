@@ -17,6 +17,7 @@ using namespace simsd;
 namespace {
 
 constexpr int kMaxDev = 64;
+constexpr int kMaxSmem = 227 * 1024;
 std::mutex g_attr_mu;
 
 inline size_t align256(size_t v) { return (v + 255) & ~size_t(255); }
@@ -119,6 +120,19 @@ int verify_drafts(const SpecVerifyArgs& a, void* stream) {
                    stream, true, a);
 }
 
+template <int D, bool BF>
+int append(const PagedAppendArgs& a, void* stream) {
+  static bool done[kMaxDev];
+  const long long turns = cdiv(a.Hq + 2 * a.Hk, PA_THREADS / (D / 16)), smem = PA_STAGES * turns * 2 * PA_THREADS * 16;
+  if (smem > 48 * 1024) {
+    const int rc = allow_smem(paged_append_kernel<D, BF>, kMaxSmem, done);
+    if (rc != SIMSD_OK) return rc;
+  }
+  const int sms = simsd_device_sm_count();
+  const int grid = std::min(a.T, PA_CTAS_PER_SM * (sms > 0 ? sms : 148));
+  return launch_on(paged_append_kernel<D, BF>, dim3((unsigned)grid), PA_THREADS, (size_t)smem, stream, false, a);
+}
+
 template <int D, int NT, bool BF>
 int attend(const PagedAttnArgs& a, const PagedPlan& pl, void* stream) {
   static bool done[kMaxDev];
@@ -141,6 +155,7 @@ int simsd_paged_append(const void* qkv, int64_t ldqkv, int T, int Hq, int Hk, in
   if (dtype != SIMSD_BF16 && dtype != SIMSD_F16) return SIMSD_ERR_DTYPE;
   if (head_dim != 64 && head_dim != 128) return SIMSD_ERR_UNSUPPORTED;
   if (rotary_dim < 0 || rotary_dim > head_dim || rotary_dim % 16) return SIMSD_ERR_UNSUPPORTED;
+  if ((int64_t)(Hq + 2LL * Hk) * head_dim > 36864) return SIMSD_ERR_UNSUPPORTED;   // its ring in shared memory
   if (T == 0) return SIMSD_OK;
   if (!qkv || (rotary_dim > 0 && (!cos || !sin)) || !positions || !slots || !q_out || !k_cache || !v_cache) return SIMSD_ERR_SHAPE;
   if (ldqkv < (int64_t)(Hq + 2 * Hk) * head_dim) return SIMSD_ERR_SHAPE;
@@ -172,11 +187,9 @@ int simsd_paged_append(const void* qkv, int64_t ldqkv, int T, int Hq, int Hk, in
   a.page_size = page_size;
   a.page_div = paged_div(page_size);
   a.eps = eps;
-  if (dtype == SIMSD_BF16)
-    return head_dim == 64 ? launch_on(paged_append_kernel<64, true>, dim3((unsigned)T), PA_THREADS, 0, stream, false, a)
-                          : launch_on(paged_append_kernel<128, true>, dim3((unsigned)T), PA_THREADS, 0, stream, false, a);
-  return head_dim == 64 ? launch_on(paged_append_kernel<64, false>, dim3((unsigned)T), PA_THREADS, 0, stream, false, a)
-                        : launch_on(paged_append_kernel<128, false>, dim3((unsigned)T), PA_THREADS, 0, stream, false, a);
+  a.T = T;
+  if (dtype == SIMSD_BF16) return head_dim == 64 ? append<64, true>(a, stream) : append<128, true>(a, stream);
+  return head_dim == 64 ? append<64, false>(a, stream) : append<128, false>(a, stream);
 }
 
 size_t simsd_paged_attention_workspace_size(int L, int Hq, int Hk, int head_dim) {
