@@ -10,17 +10,17 @@
 // the work is to keep loads in flight on every SM and to cut any mix of lengths
 // evenly.
 //
-// Split.  A unit is 64 keys of one (sequence, KV head, row tile); the units of the
-// whole call, in that order, are cut into equal contiguous ranges, one per CTA, two
-// CTAs per SM, from the lengths on the device (no host knowledge of them, so a
+// Split.  A unit is TK keys of one (sequence, KV head, row tile); the units of the
+// whole call, in that order, are cut into equal contiguous ranges, one per CTA of
+// what the SMs hold at once, from the lengths on the device (no host knowledge of them, so a
 // graph replays as sequences grow).  A range may hold many short sequences or a
 // slice of a long one; a sequence cut between CTAs leaves each part's (O, max,
 // sum) in the workspace, and the last of its CTAs to finish (a counter per first
 // CTA, zero again afterwards) joins the parts, always in key order.
 //
-// In a CTA each of the 4 warps takes 16 keys of every unit through a ring of its
-// own (cp.async, no barrier between warps until the sequence ends), loading ahead
-// across sequence ends; the next sequence's queries are fetched a sequence ahead.
+// In a CTA each key group (a warp, or one per 16 rows where there are more) takes 16 keys of every unit through a ring of its own (cp.async, no barrier
+// between key groups until the sequence ends), loading ahead across sequence ends;
+// the next sequence's queries are fetched a sequence ahead.
 // Products with the roles swapped, so that few rows waste little: S^T = K Q^T
 // (m16n8k16: 16 keys x 8 rows), P^T turned into the second product's operand with
 // movmatrix, O^T = V^T P^T (16 dims x 8 rows).  Softmax in fp32 with exp2 of
@@ -49,7 +49,7 @@ struct PagedAttnArgs {
   float* lse;               // [B, L, Hq] or nullptr
   int* err;
   int* arrived;             // [grid]: parts written of the cut sequence that starts in that CTA; zero between calls
-  float4* part_o;           // [2 grid][D / 16][NT][32] fragments
+  float4* part_o;           // [2 grid][D / 16][NR / 8][32] fragments
   float2* part_ml;          // [2 grid][NR] (max in log2 units, sum)
   long long ld_page, ld_head, ld_tok, ld_table, ldm_b, ldm_t;
   int B, L, Hq, Hk, G, num_pages, page_size, max_pages, rows, row_tiles;
@@ -58,17 +58,23 @@ struct PagedAttnArgs {
   float scale_log2;         // |scale| log2(e), positive
 };
 
-constexpr int PAT_WARPS = 4, PAT_THREADS = PAT_WARPS * 32, PAT_TK = 16 * PAT_WARPS;
-constexpr int PAT_CTAS_PER_SM = 2;
-
-template <int D, int NT>
-struct PatSmem {
-  static constexpr int STAGES = NT <= 2 ? 3 : 2;
+// A CTA's warps: KG key groups of 16 keys (a unit is one step of all of them, TK
+// keys) x RG row groups of NT 8-row tiles (NR rows in all).  Up to 16 rows one row
+// group holds them, its queries as fragments in registers, in two CTAs of 4 warps
+// per SM.  More rows take more row groups, which share the keys and values of their
+// key group and the queries in shared memory, in one CTA of 12 warps (so that a
+// thread's sums stay in registers).
+template <int D, int NT, int RG>
+struct PatShape {
+  static constexpr int KG = RG == 1 ? 4 : 12 / RG, TK = 16 * KG;
+  static constexpr int THREADS = KG * RG * 32, CTAS_PER_SM = RG == 1 ? 2 : 1;
+  static constexpr int NR = NT * 8 * RG;
+  static constexpr int STAGES = RG == 4 ? 5 : 3;
   static constexpr int MAT = 16 * D * 2;                       // 16 keys (or values)
-  static constexpr int RING = PAT_WARPS * STAGES * 2 * MAT;
-  static constexpr int OBUF = PAT_WARPS * (D / 16) * 32 * 16;  // one 8-row tile of every warp's O
-  static constexpr int Q = NT > 2 ? NT * 8 * D * 2 : 0;
-  static constexpr int ML = 2 * PAT_WARPS * NT * 8 * 4;
+  static constexpr int RING = KG * STAGES * 2 * MAT;
+  static constexpr int OBUF = KG * RG * (D / 16) * 32 * 16;    // one 8-row tile of every warp's O
+  static constexpr int Q = RG > 1 ? NR * D * 2 : 0;
+  static constexpr int ML = 2 * KG * NR * 4;
   static constexpr int BYTES = RING + OBUF + Q + ML;
 };
 
@@ -131,10 +137,14 @@ __device__ __forceinline__ int paged_len(const PagedAttnArgs& p, int b) {
   return n < 0 ? 0 : n > cap ? (int)cap : n;
 }
 // units of one (head, row tile) of a sequence; an empty one has a unit, which writes its rows
-__device__ __forceinline__ int paged_units(int n) { return n <= PAT_TK ? 1 : (n + PAT_TK - 1) / PAT_TK; }
+template <int TK>
+__device__ __forceinline__ int paged_units(int n) {
+  return n <= TK ? 1 : (n + TK - 1) / TK;
+}
 
 // Position in the unit order: sequence b (length n, nu units per KV head and row
 // tile), KV head g, row tile rt, unit of it.
+template <int TK>
 struct PagedPos {
   int b, g, rt, unit, n, nu;
   __device__ __forceinline__ void next(const PagedAttnArgs& p) {
@@ -142,7 +152,7 @@ struct PagedPos {
     unit = 0;
     if (!next_rows(p, b, g, rt) || b >= p.B) return;
     n = paged_len(p, b);
-    nu = paged_units(n);
+    nu = paged_units<TK>(n);
   }
   // the row tile, head or sequence after (b, g, rt); true for another sequence
   __device__ static __forceinline__ bool next_rows(const PagedAttnArgs& p, int& b, int& g, int& rt) {
@@ -197,8 +207,10 @@ __device__ __forceinline__ void paged_store_lse(const PagedAttnArgs& p, int b, i
 
 // This CTA's place in the cut of the call's units and the position of its first
 // unit.  False: this CTA has none.
-__device__ __forceinline__ bool paged_range(const PagedAttnArgs& p, PagedCut& cut, PagedPos& pos) {
-  __shared__ int s_sum[PAT_WARPS], s_more[PAT_WARPS];
+template <int THREADS, int TK>
+__device__ __forceinline__ bool paged_range(const PagedAttnArgs& p, PagedCut& cut, PagedPos<TK>& pos) {
+  constexpr int WARPS = THREADS / 32;
+  __shared__ int s_sum[WARPS], s_more[WARPS];
   __shared__ int s_b, s_first;
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   const int per = p.Hk * p.row_tiles;
@@ -206,11 +218,11 @@ __device__ __forceinline__ bool paged_range(const PagedAttnArgs& p, PagedCut& cu
   auto units = [&](int b) {
     if (b >= p.B) return 0;
     if (flag && p.seq_lens[b] > (long long)p.max_pages * p.page_size) atomicOr(p.err, SIMSD_DEV_ERR_BAD_INDEX);
-    return paged_units(paged_len(p, b)) * per;
+    return paged_units<TK>(paged_len(p, b)) * per;
   };
-  // sequences tid, tid + PAT_THREADS, ...: the first of them scanned, the others summed
+  // sequences tid, tid + THREADS, ...: the first of them scanned, the others summed
   int u = units(tid), incl = u, more = 0;
-  for (int b = tid + PAT_THREADS; b < p.B; b += PAT_THREADS) more += units(b);
+  for (int b = tid + THREADS; b < p.B; b += THREADS) more += units(b);
 #pragma unroll
   for (int m = 1; m < 32; m <<= 1) {
     const int v = __shfl_up_sync(0xffffffffu, incl, m);
@@ -221,7 +233,7 @@ __device__ __forceinline__ bool paged_range(const PagedAttnArgs& p, PagedCut& cu
   __syncthreads();
   int off = 0, head = 0, total = 0;
 #pragma unroll
-  for (int w = 0; w < PAT_WARPS; ++w) {
+  for (int w = 0; w < WARPS; ++w) {
     if (w < warp) off += s_sum[w];
     head += s_sum[w];
     total += s_sum[w] + s_more[w];
@@ -233,7 +245,7 @@ __device__ __forceinline__ bool paged_range(const PagedAttnArgs& p, PagedCut& cu
   cut.extra = total - cut.base * cut.ctas;
   const int w0 = cut.first(c);
   if (off + incl - u <= w0 && w0 < off + incl) s_b = tid, s_first = off + incl - u;
-  for (int base = PAT_THREADS, before = head; before <= w0; base += PAT_THREADS) {   // past the first sequences
+  for (int base = THREADS, before = head; before <= w0; base += THREADS) {   // past the first sequences
     u = incl = units(base + tid);
 #pragma unroll
     for (int m = 1; m < 32; m <<= 1) {
@@ -245,7 +257,7 @@ __device__ __forceinline__ bool paged_range(const PagedAttnArgs& p, PagedCut& cu
     __syncthreads();
     off = before;
 #pragma unroll
-    for (int w = 0; w < PAT_WARPS; ++w) {
+    for (int w = 0; w < WARPS; ++w) {
       if (w < warp) off += s_sum[w];
       before += s_sum[w];
     }
@@ -254,7 +266,7 @@ __device__ __forceinline__ bool paged_range(const PagedAttnArgs& p, PagedCut& cu
   __syncthreads();
   pos.b = s_b;
   pos.n = paged_len(p, pos.b);
-  pos.nu = paged_units(pos.n);
+  pos.nu = paged_units<TK>(pos.n);
   const int rem = w0 - s_first, hr = rem / pos.nu;
   pos.unit = rem - hr * pos.nu;
   pos.g = hr / p.row_tiles;
@@ -270,12 +282,15 @@ struct PagedPart {
 // Joins the parts of a cut sequence (one KV head and row tile of it) that starts
 // in CTA c0: part i's max, sum and O lie in slot 1 of CTA c0 for i = 0, in slot 0
 // of CTA c0 + i for the others.  `buf`: OBUF bytes of shared memory.
-template <int D, int NT, bool BF>
+template <int D, int NT, int RG, bool BF>
 __device__ __noinline__ void paged_join(const PagedAttnArgs& p, int b, int g, int r0, int c0, int parts, float* buf) {
-  constexpr int MT = D / 16, NR = NT * 8, PER = MT * NT * 32 / PAT_THREADS;
-  constexpr int GR = PAT_THREADS / NR, KEEP = 4;              // threads of a row, parts a thread keeps
-  constexpr int CAP = PatSmem<D, NT>::OBUF / 4 / NR;          // parts whose weights fit in buf
+  using S = PatShape<D, NT, RG>;
+  constexpr int MT = D / 16, NR = S::NR, TILES = NR / 8, THREADS = S::THREADS;
+  constexpr int ALL = MT * TILES * 32, PER = (ALL + THREADS - 1) / THREADS;   // fragments, and of a thread
+  constexpr int GR = THREADS / NR, KEEP = 4;                  // threads of a row, parts a thread keeps
+  constexpr int CAP = S::OBUF / 4 / NR;                       // parts whose weights fit in buf
   const int tid = threadIdx.x, lane = tid & 31, r = tid % NR, grp = tid / NR;
+  const bool rows = grp < GR;                                 // this thread looks after row r
   auto slot = [&](int i) { return i == 0 ? 2 * c0 + 1 : 2 * (c0 + i); };
   // the first two parts of O (most sequences are cut once) are on their way while the weights are made
   float4 lead[2][PER];
@@ -283,12 +298,12 @@ __device__ __noinline__ void paged_join(const PagedAttnArgs& p, int b, int g, in
   for (int i = 0; i < 2; ++i)
 #pragma unroll
     for (int k = 0; k < PER; ++k)
-      lead[i][k] = __ldcg(p.part_o + (long long)slot(i) * (MT * NT * 32) + tid + k * PAT_THREADS);
+      lead[i][k] = __ldcg(p.part_o + (long long)slot(i) * ALL + min(tid + k * THREADS, ALL - 1));
   float2 keep[KEEP];
 #pragma unroll
   for (int k = 0; k < KEEP; ++k) {
     const int i = grp + k * GR;
-    keep[k] = i < parts ? __ldcg(p.part_ml + slot(i) * NR + r) : make_float2(-INFINITY, 0.0f);
+    keep[k] = rows && i < parts ? __ldcg(p.part_ml + slot(i) * NR + r) : make_float2(-INFINITY, 0.0f);
   }
   float mm = -INFINITY, ll = 0.0f;
   auto see = [&](float2 x) {
@@ -298,9 +313,9 @@ __device__ __noinline__ void paged_join(const PagedAttnArgs& p, int b, int g, in
   };
 #pragma unroll
   for (int k = 0; k < KEEP; ++k) see(keep[k]);
-  for (int i = grp + KEEP * GR; i < parts; i += GR) see(__ldcg(p.part_ml + slot(i) * NR + r));
+  for (int i = grp + KEEP * GR; rows && i < parts; i += GR) see(__ldcg(p.part_ml + slot(i) * NR + r));
   float* all = buf + GR * NR;
-  buf[grp * NR + r] = mm, all[grp * NR + r] = ll;
+  if (rows) buf[grp * NR + r] = mm, all[grp * NR + r] = ll;
   __syncthreads();
   mm = -INFINITY, ll = 0.0f;
 #pragma unroll
@@ -313,7 +328,7 @@ __device__ __noinline__ void paged_join(const PagedAttnArgs& p, int b, int g, in
   for (int i0 = 0; i0 < parts; i0 += CAP) {
     const int n = min(CAP, parts - i0);
     __syncthreads();
-    for (int i = grp; i < n; i += GR) {
+    for (int i = grp; rows && i < n; i += GR) {
       const int k = (i0 + i) / GR;
       float x = 0.0f;
       if (k < KEEP) {
@@ -326,7 +341,7 @@ __device__ __noinline__ void paged_join(const PagedAttnArgs& p, int b, int g, in
     }
     __syncthreads();
     auto add = [&](int i, int k, float4 v) {
-      const int rr = (tid + k * PAT_THREADS) / 32 % NT * 8 + 2 * (lane & 3);
+      const int rr = (tid + k * THREADS) / 32 % TILES * 8 + 2 * (lane & 3);
       const float f0 = buf[i * NR + rr], f1 = buf[i * NR + rr + 1];
       a[k].x = fmaf(v.x, f0, a[k].x), a[k].y = fmaf(v.y, f1, a[k].y);
       a[k].z = fmaf(v.z, f0, a[k].z), a[k].w = fmaf(v.w, f1, a[k].w);
@@ -340,53 +355,67 @@ __device__ __noinline__ void paged_join(const PagedAttnArgs& p, int b, int g, in
     }
 #pragma unroll 4
     for (; i < n; ++i) {
-      const float4* o = p.part_o + (long long)slot(i0 + i) * (MT * NT * 32);
+      const float4* o = p.part_o + (long long)slot(i0 + i) * ALL;
 #pragma unroll
-      for (int k = 0; k < PER; ++k) add(i, k, __ldcg(o + tid + k * PAT_THREADS));
+      for (int k = 0; k < PER; ++k) add(i, k, __ldcg(o + min(tid + k * THREADS, ALL - 1)));
     }
   }
 #pragma unroll
   for (int k = 0; k < PER; ++k) {
-    const int x = tid + k * PAT_THREADS, rr = r0 + x / 32 % NT * 8 + (lane >> 2);
-    paged_store<BF, D>(p, rr < p.rows ? paged_row(p, b, g, rr) : -1, x / (NT * 32), lane, a[k]);
+    const int x = tid + k * THREADS, rr = r0 + x / 32 % TILES * 8 + (lane >> 2);
+    if (x >= ALL) break;                                      // whole warps
+    paged_store<BF, D>(p, rr < p.rows ? paged_row(p, b, g, rr) : -1, x / (TILES * 32), lane, a[k]);
   }
 }
 
-template <int D, int NT, bool BF>
-__global__ void __launch_bounds__(PAT_THREADS, PAT_CTAS_PER_SM) paged_attention_kernel(const __grid_constant__ PagedAttnArgs p) {
+template <int D, int NT, int RG, bool BF>
+__global__ void __launch_bounds__(PatShape<D, NT, RG>::THREADS, PatShape<D, NT, RG>::CTAS_PER_SM)
+    paged_attention_kernel(const __grid_constant__ PagedAttnArgs p) {
   griddep_launch_dependents();
   griddep_wait();
-  using S = PatSmem<D, NT>;
-  constexpr int MT = D / 16, NR = NT * 8, CH = D / 8;     // 16-byte chunks of a key
+  using S = PatShape<D, NT, RG>;
+  constexpr int THREADS = S::THREADS, KG = S::KG, TK = S::TK, NR = S::NR, TILES = NR / 8;
+  constexpr int MT = D / 16, CH = D / 8;                  // 16-dim tiles, 16-byte chunks of a key
   constexpr int KPI = 32 / CH;                            // keys per cp.async of the warp
-  constexpr bool QREG = NT <= 2;
-  constexpr int QW = QREG ? MT * NT * 2 : NR * CH * 4 / PAT_THREADS;   // words of the queries in a thread
-  extern __shared__ __align__(128) uint8_t pat_smem[];
+  constexpr bool QREG = RG == 1;
+  constexpr int QW = QREG ? MT * NT * 2 : (NR * CH + THREADS - 1) / THREADS * 4;   // words of the queries in a thread
+  extern __shared__ __align__(256) uint8_t pat_smem[];
   __shared__ PagedPart s_cut[2];
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
-  const uint32_t ring = smem_u32(pat_smem) + warp * S::STAGES * 2 * S::MAT;
+  const int kg = warp % KG, rg = warp / KG;       // key group, row group
+  const uint32_t ring = smem_u32(pat_smem) + kg * S::STAGES * 2 * S::MAT;
   float4* obuf = reinterpret_cast<float4*>(pat_smem + S::RING);
   uint8_t* qs = pat_smem + S::RING + S::OBUF;
   float* sm_m = reinterpret_cast<float*>(pat_smem + S::RING + S::OBUF + S::Q);
-  float* sm_l = sm_m + PAT_WARPS * NR;
+  float* sm_l = sm_m + KG * NR;
 
-  PagedCut cut;
-  PagedPos ld;
-  if (!paged_range(p, cut, ld)) return;
+  __shared__ PagedCut s_range;
+  PagedPos<TK> ld;
+  int steps;
+  {
+    PagedCut cut;
+    if (!paged_range<THREADS, TK>(p, cut, ld)) return;
+    steps = cut.first(blockIdx.x + 1) - cut.first(blockIdx.x);
+    if (tid == 0) s_range = cut;
+  }
   if (tid < 2) s_cut[tid].parts = 0;
-  PagedPos at = ld;
-  const int w0 = cut.first(blockIdx.x), steps = cut.first(blockIdx.x + 1) - w0;
+  PagedPos<TK> at = ld;
 
-  // ---- loads: the warp's 16 keys of position `ld` into ring slot `loaded` % STAGES.
+  // ---- loads: the key group's 16 keys of position `ld` into its next ring slot; with
+  // several row groups each of their warps loads a share (keys or values, or half of
+  // the rows of either).
   // Pages of a multiple of 16 tokens hold all sixteen in one page, a fixed distance
   // apart; otherwise every key's place is looked up (by lane key % 16, handed round).
   // The page numbers are fetched a step ahead.
   const bool page16 = p.page_size % 16 == 0;
   const int kc = lane % CH, khi = lane / CH;
   const uint32_t swz = (uint32_t)(khi * (D * 2) + ((kc ^ khi) << 4));
-  auto fetch_page = [&](const PagedPos& x) {
-    const int key = x.unit * PAT_TK + warp * 16 + (page16 ? 0 : lane & 15);
+  auto fetch_page = [&](const PagedPos<TK>& x) {
+    const int key = x.unit * TK + kg * 16 + (page16 ? 0 : lane & 15);
     return key < x.n ? p.page_table[x.b * p.ld_table + p.page_div(key)] : -1;
+  };
+  auto mine = [&](int i, int mat) {
+    return RG == 1 || (RG == 2 ? rg == mat : rg == 2 * mat + (i >= 8 / KPI));
   };
   int page = fetch_page(ld);
   int loaded = 0;
@@ -394,7 +423,7 @@ __global__ void __launch_bounds__(PAT_THREADS, PAT_CTAS_PER_SM) paged_attention_
   auto load = [&]() {
     if (loaded < steps) {
       const uint32_t dst = load_slot + swz;
-      const int key0 = ld.unit * PAT_TK + warp * 16;
+      const int key0 = ld.unit * TK + kg * 16;
       if (key0 < ld.n) {
         const bool fine = page >= 0 && page < p.num_pages;
         if (page16) {
@@ -409,8 +438,8 @@ __global__ void __launch_bounds__(PAT_THREADS, PAT_CTAS_PER_SM) paged_attention_
           for (int i = 0; i < 16 / KPI; ++i) {
             const uint32_t s = (dst ^ ((i * KPI & 7) << 4)) + i * KPI * (D * 2);
             const bool ok = left > i * KPI;
-            pat_cp16(s, ok ? k : reinterpret_cast<const char*>(p.k_cache), ok);
-            pat_cp16(s + S::MAT, ok ? v : reinterpret_cast<const char*>(p.v_cache), ok);
+            if (mine(i, 0)) pat_cp16(s, ok ? k : reinterpret_cast<const char*>(p.k_cache), ok);
+            if (mine(i, 1)) pat_cp16(s + S::MAT, ok ? v : reinterpret_cast<const char*>(p.v_cache), ok);
             k += step;
             v += step;
           }
@@ -429,8 +458,8 @@ __global__ void __launch_bounds__(PAT_THREADS, PAT_CTAS_PER_SM) paged_attention_
             const long long o = __shfl_sync(0xffffffffu, off, i * KPI + khi);
             const uint32_t s = (dst ^ ((i * KPI & 7) << 4)) + i * KPI * (D * 2);
             const long long e = o < 0 ? 0 : o + kc * 8;
-            pat_cp16(s, reinterpret_cast<const uint16_t*>(p.k_cache) + e, o >= 0);
-            pat_cp16(s + S::MAT, reinterpret_cast<const uint16_t*>(p.v_cache) + e, o >= 0);
+            if (mine(i, 0)) pat_cp16(s, reinterpret_cast<const uint16_t*>(p.k_cache) + e, o >= 0);
+            if (mine(i, 1)) pat_cp16(s + S::MAT, reinterpret_cast<const uint16_t*>(p.v_cache) + e, o >= 0);
           }
         }
       }
@@ -449,7 +478,7 @@ __global__ void __launch_bounds__(PAT_THREADS, PAT_CTAS_PER_SM) paged_attention_
   // registers, more through shared memory
   uint32_t qnext[QW];
   auto fetch_queries = [&](int b, int g, int rt) {
-    const int r0 = rt * NR;
+    const int r0 = rt * NR;                                // QREG: the one row group's
     const uint16_t* qb = reinterpret_cast<const uint16_t*>(p.q);
     if constexpr (QREG) {
 #pragma unroll
@@ -464,8 +493,8 @@ __global__ void __launch_bounds__(PAT_THREADS, PAT_CTAS_PER_SM) paged_attention_
     } else {
 #pragma unroll
       for (int k = 0; k < QW / 4; ++k) {
-        const int x = tid + k * PAT_THREADS, r = r0 + x / CH;
-        const bool in = r < p.rows && b < p.B;
+        const int x = tid + k * THREADS, r = r0 + x / CH;
+        const bool in = x < NR * CH && r < p.rows && b < p.B;
         const uint4 v = in ? __ldg(reinterpret_cast<const uint4*>(qb + paged_row(p, b, g, r) * D + x % CH * 8))
                            : make_uint4(0, 0, 0, 0);
         const uint32_t f = in ? p.q_sign : 0u;
@@ -476,6 +505,14 @@ __global__ void __launch_bounds__(PAT_THREADS, PAT_CTAS_PER_SM) paged_attention_
   fetch_queries(at.b, at.g, at.rt);
 #pragma unroll
   for (int s = 0; s < S::STAGES - 1; ++s) load();
+
+  // What a lane reads of a swizzled tile (rows of D * 2 bytes on multiples of that):
+  // chunk c of row r at r * D * 2 + ((c ^ r % 8) << 4), so that stepping by two chunks
+  // is an exclusive or with multiples of 32.
+  const uint32_t k_lane = (lane & 15) * (D * 2) + (((lane >> 4) ^ (lane & 7)) << 4);
+  const uint32_t v_lane = ((lane & 7) + (lane >> 4) * 8) * (D * 2) + ((((lane >> 3) & 1) ^ (lane & 7)) << 4);
+  const uint32_t q_lane = smem_u32(qs) + (rg * NT * 8 + (lane >> 4) * 8 + (lane & 7)) * (D * 2) +
+                          ((((lane >> 3) & 1) ^ (lane & 7)) << 4);
 
   float o[MT][NT][4], m[NT][2], l[NT][2];
   uint32_t bq[QREG ? QW : 1];
@@ -491,15 +528,15 @@ __global__ void __launch_bounds__(PAT_THREADS, PAT_CTAS_PER_SM) paged_attention_
       } else {
 #pragma unroll
         for (int k = 0; k < QW / 4; ++k) {
-          const int x = tid + k * PAT_THREADS, rr = x / CH, c = x % CH;
-          *reinterpret_cast<uint4*>(qs + rr * (D * 2) + ((c ^ (rr & 7)) << 4)) =
+          const int x = tid + k * THREADS, rr = x / CH, c = x % CH;
+          if (x < NR * CH) *reinterpret_cast<uint4*>(qs + rr * (D * 2) + ((c ^ (rr & 7)) << 4)) =
               make_uint4(qnext[4 * k], qnext[4 * k + 1], qnext[4 * k + 2], qnext[4 * k + 3]);
         }
         __syncthreads();
       }
       if (at.nu - at.unit < steps - i) {
         int b = at.b, g = at.g, rt = at.rt;
-        PagedPos::next_rows(p, b, g, rt);
+        PagedPos<TK>::next_rows(p, b, g, rt);
         fetch_queries(b, g, rt);
       }
 #pragma unroll
@@ -512,39 +549,44 @@ __global__ void __launch_bounds__(PAT_THREADS, PAT_CTAS_PER_SM) paged_attention_
           for (int e = 0; e < 4; ++e) o[mt][nt][e] = 0.0f;
       }
     }
-    load();
-    pat_wait<S::STAGES - 1>();
-    __syncwarp();
+    if constexpr (RG == 1) {
+      load();
+      pat_wait<S::STAGES - 1>();
+      __syncwarp();
+    } else {
+      // the slot's loads by all row groups have arrived, and all have left the slot that load() fills
+      pat_wait<S::STAGES - 2>();
+      named_bar_sync(1 + kg, RG * 32);
+      load();
+    }
     const uint32_t ks_base = slot_at, vs_base = ks_base + S::MAT;
     slot_at += 2 * S::MAT;
     if (slot_at == ring + S::STAGES * 2 * S::MAT) slot_at = ring;
-    const int key0 = at.unit * PAT_TK + warp * 16;
+    const int key0 = at.unit * TK + kg * 16;
     if (key0 < at.n) {
       // S^T = K Q^T
       float s[NT][4];
 #pragma unroll
       for (int nt = 0; nt < NT; ++nt) s[nt][0] = s[nt][1] = s[nt][2] = s[nt][3] = 0.0f;
-      const int kr = lane & 15;
 #pragma unroll
       for (int ks = 0; ks < MT; ++ks) {
         uint32_t a[4];
-        pat_ldsm(ks_base + kr * (D * 2) + (((ks * 2 + (lane >> 4)) ^ (kr & 7)) << 4), a);
+        pat_ldsm((ks_base + k_lane) ^ (ks << 5), a);
         if constexpr (QREG) {
 #pragma unroll
           for (int nt = 0; nt < NT; ++nt) pat_mma<BF>(s[nt], a, bq[2 * ks * NT + nt], bq[(2 * ks + 1) * NT + nt]);
         } else {
 #pragma unroll
           for (int nt = 0; nt < NT; nt += 2) {
-            // rows nt * 8 .. + 15, both 8-element halves of this k step
-            const int rr = nt * 8 + (lane >> 4) * 8 + (lane & 7);
+            // 16 rows of the row group, both 8-element halves of this k step
             uint32_t b[4];
-            pat_ldsm(smem_u32(qs) + rr * (D * 2) + (((ks * 2 + ((lane >> 3) & 1)) ^ (rr & 7)) << 4), b);
+            pat_ldsm((q_lane + nt * 8 * (D * 2)) ^ (ks << 5), b);
             pat_mma<BF>(s[nt], a, b[0], b[1]);
             pat_mma<BF>(s[nt + 1], a, b[2], b[3]);
           }
         }
       }
-      const int r0 = at.rt * NR;
+      const int r0 = at.rt * NR + rg * NT * 8;
       const bool edge = key0 + 16 > at.n - p.L;          // some key of the sixteen may be hidden from some row
       if (edge) {
         uint32_t see = 0;
@@ -595,7 +637,6 @@ __global__ void __launch_bounds__(PAT_THREADS, PAT_CTAS_PER_SM) paged_attention_
         pb[nt][1] = pat_transpose(pat_pack<BF>(s[nt][2], s[nt][3]));
       }
       // O^T += V^T P^T
-      const int vr = (lane & 7) + (lane >> 4) * 8, vc = (lane >> 3) & 1;
       bool odd = false;
       if (edge && (p.L > 1 || p.tail)) {   // a value that is not finite, of a key that some row does not see?
         for (int x = lane; x < 16 * CH; x += 32) {
@@ -612,7 +653,7 @@ __global__ void __launch_bounds__(PAT_THREADS, PAT_CTAS_PER_SM) paged_attention_
 #pragma unroll
         for (int mt = 0; mt < MT; ++mt) {
           uint32_t a[4];
-          pat_ldsm_t(vs_base + vr * (D * 2) + (((mt * 2 + vc) ^ (vr & 7)) << 4), a);
+          pat_ldsm_t((vs_base + v_lane) ^ (mt << 5), a);
 #pragma unroll
           for (int nt = 0; nt < NT; ++nt) pat_mma<BF>(o[mt][nt], a, pb[nt][0], pb[nt][1]);
         }
@@ -632,7 +673,7 @@ __global__ void __launch_bounds__(PAT_THREADS, PAT_CTAS_PER_SM) paged_attention_
 #pragma unroll
             for (int mt = 0; mt < MT; ++mt) {
               uint32_t a[4];
-              pat_ldsm_t(vs_base + vr * (D * 2) + (((mt * 2 + vc) ^ (vr & 7)) << 4), a);
+              pat_ldsm_t((vs_base + v_lane) ^ (mt << 5), a);
               a[0] &= keep[0], a[1] &= keep[0], a[2] &= keep[1], a[3] &= keep[1];
               float d[4] = {0.0f, 0.0f, 0.0f, 0.0f};
               pat_mma<BF>(d, a, pb[nt][0], pb[nt][1]);
@@ -645,9 +686,9 @@ __global__ void __launch_bounds__(PAT_THREADS, PAT_CTAS_PER_SM) paged_attention_
     __syncwarp();
     const bool ends = at.unit + 1 == at.nu;
     if (ends || i + 1 == steps) {
-      // join the four warps; a whole sequence is written, a part goes to the workspace
+      // join the key groups; a whole sequence is written, a part goes to the workspace
       const bool whole = ends && first_unit == 0;
-      const int part = first_unit == 0 ? 1 : 0, slot = 2 * blockIdx.x + part, r0 = at.rt * NR;
+      const int part = first_unit == 0 ? 1 : 0, slot = 2 * blockIdx.x + part, r0 = at.rt * NR, w0r = rg * NT * 8;
 #pragma unroll
       for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
@@ -658,58 +699,64 @@ __global__ void __launch_bounds__(PAT_THREADS, PAT_CTAS_PER_SM) paged_attention_
           x += __shfl_xor_sync(0xffffffffu, x, 16);
           m[nt][e] *= p.scale_log2;
           if (lane < 4) {
-            sm_m[warp * NR + nt * 8 + 2 * lane + e] = m[nt][e];
-            sm_l[warp * NR + nt * 8 + 2 * lane + e] = x;
+            sm_m[kg * NR + w0r + nt * 8 + 2 * lane + e] = m[nt][e];
+            sm_l[kg * NR + w0r + nt * 8 + 2 * lane + e] = x;
           }
         }
       __syncthreads();
+      float inv[NT][2];
 #pragma unroll
-      for (int nt = 0; nt < NT; ++nt) {
-        float f[2], inv[2];
+      for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
         for (int e = 0; e < 2; ++e) {
-          const int r = nt * 8 + 2 * (lane & 3) + e;
+          const int r = w0r + nt * 8 + 2 * (lane & 3) + e;
           float mm = -INFINITY, ll = 0.0f;
 #pragma unroll
-          for (int w = 0; w < PAT_WARPS; ++w) mm = fmaxf(mm, sm_m[w * NR + r]);
+          for (int w = 0; w < KG; ++w) mm = fmaxf(mm, sm_m[w * NR + r]);
           const float mu = mm == -INFINITY ? 0.0f : mm;
 #pragma unroll
-          for (int w = 0; w < PAT_WARPS; ++w) ll = fmaf(sm_l[w * NR + r], pat_exp2(sm_m[w * NR + r] - mu), ll);
-          f[e] = pat_exp2(m[nt][e] - mu);
-          inv[e] = !whole ? 1.0f : ll == 0.0f ? 0.0f : 1.0f / ll;
-          if (warp == nt % PAT_WARPS && lane < 4) {
+          for (int w = 0; w < KG; ++w) ll = fmaf(sm_l[w * NR + r], pat_exp2(sm_m[w * NR + r] - mu), ll);
+          const float f = pat_exp2(m[nt][e] - mu);
+          inv[nt][e] = !whole ? 1.0f : ll == 0.0f ? 0.0f : 1.0f / ll;
+#pragma unroll
+          for (int mt = 0; mt < MT; ++mt) o[mt][nt][e] *= f, o[mt][nt][e + 2] *= f;
+          if (kg == 0 && lane < 4) {
             if (whole)
               paged_store_lse(p, at.b, at.g, r0 + r, mm, ll);
             else
               p.part_ml[slot * NR + r] = make_float2(mm, ll);
           }
         }
-        const int r = r0 + nt * 8 + (lane >> 2);
+#pragma unroll
+      for (int nt = 0; nt < NT; ++nt) {
+        const int r = r0 + w0r + nt * 8 + (lane >> 2);
         const long long row = r < p.rows ? paged_row(p, at.b, at.g, r) : -1;
         if (nt > 0) __syncthreads();
 #pragma unroll
         for (int mt = 0; mt < MT; ++mt)
-          obuf[(warp * MT + mt) * 32 + lane] =
-              make_float4(o[mt][nt][0] * f[0], o[mt][nt][1] * f[1], o[mt][nt][2] * f[0], o[mt][nt][3] * f[1]);
+          obuf[(warp * MT + mt) * 32 + lane] = make_float4(o[mt][nt][0], o[mt][nt][1], o[mt][nt][2], o[mt][nt][3]);
         __syncthreads();
 #pragma unroll
-        for (int k = 0; k < MT / PAT_WARPS; ++k) {
-          const int mt = warp + k * PAT_WARPS;
-          float4 a = obuf[mt * 32 + lane];
+        for (int k = 0; k < (MT + KG - 1) / KG; ++k) {
+          const int mt = kg + k * KG;
+          if (mt >= MT) break;
+          const float4* from = obuf + (rg * KG * MT + mt) * 32 + lane;
+          float4 a = from[0];
 #pragma unroll
-          for (int w = 1; w < PAT_WARPS; ++w) {
-            const float4 x = obuf[(w * MT + mt) * 32 + lane];
+          for (int w = 1; w < KG; ++w) {
+            const float4 x = from[w * MT * 32];
             a.x += x.x, a.y += x.y, a.z += x.z, a.w += x.w;
           }
-          a.x *= inv[0], a.y *= inv[1], a.z *= inv[0], a.w *= inv[1];
+          a.x *= inv[nt][0], a.y *= inv[nt][1], a.z *= inv[nt][0], a.w *= inv[nt][1];
           if (whole)
             paged_store<BF, D>(p, row, mt, lane, a);
           else
-            p.part_o[(((long long)slot * MT + mt) * NT + nt) * 32 + lane] = a;
+            p.part_o[(((long long)slot * MT + mt) * TILES + rg * NT + nt) * 32 + lane] = a;
         }
       }
       if (!whole && tid == 0) {
-        const int head = w0 + i - at.unit, c0 = cut.cta_of(head);      // the sequence's first unit and CTA
+        const PagedCut cut = s_range;
+        const int head = cut.first(blockIdx.x) + i - at.unit, c0 = cut.cta_of(head);   // the sequence's first unit and CTA
         s_cut[part] = {at.b, at.g, r0, c0, cut.cta_of(head + at.nu - 1) - c0 + 1};
       }
       __syncthreads();
@@ -730,7 +777,7 @@ __global__ void __launch_bounds__(PAT_THREADS, PAT_CTAS_PER_SM) paged_attention_
   __syncthreads();
   for (int k = 0; k < 2; ++k) {
     const PagedPart x = s_cut[k];
-    if (x.parts > 0) paged_join<D, NT, BF>(p, x.b, x.g, x.r0, x.c0, x.parts, reinterpret_cast<float*>(obuf));
+    if (x.parts > 0) paged_join<D, NT, RG, BF>(p, x.b, x.g, x.r0, x.c0, x.parts, reinterpret_cast<float*>(obuf));
     __syncthreads();
   }
 }

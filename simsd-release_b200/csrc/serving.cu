@@ -51,22 +51,22 @@ int cache_check(const void* k, const void* v, int64_t ld_page, int64_t ld_head, 
   return SIMSD_OK;
 }
 
-// What paged attention does with G L rows per KV head: 8-row tiles per CTA (all
-// rows in one pass over the keys up to 32, more in row tiles of 32), the grid, and
-// the workspace: the arrival counters, then two parts per CTA (the end of a sequence
-// it started inside, the start of one it leaves unfinished).
+// What paged attention does with G L rows per KV head: the rows of a CTA (8, 16, 32
+// or 64; more go in tiles of 64), the grid, and the workspace: the arrival counters,
+// then two parts per CTA (the end of a sequence it started inside, the start of one
+// it leaves unfinished).
 struct PagedPlan {
-  int nt, grid;
+  int nr, grid;
   size_t ml_at, bytes;
 };
 PagedPlan paged_plan(int L, int G, int D) {
   PagedPlan p;
   const long long rows = (long long)L * G;
-  p.nt = rows <= 8 ? 1 : rows <= 16 ? 2 : 4;
+  p.nr = rows <= 8 ? 8 : rows <= 16 ? 16 : rows <= 32 ? 32 : 64;
   const int sms = simsd_device_sm_count();
-  p.grid = std::min(PAT_CTAS_PER_SM * (sms > 0 ? sms : 148), SIMSD_PAGED_COUNTER_BYTES / (int)sizeof(int));
-  p.ml_at = SIMSD_PAGED_COUNTER_BYTES + align256((size_t)2 * p.grid * D * p.nt * 8 * sizeof(float));
-  p.bytes = p.ml_at + align256((size_t)2 * p.grid * p.nt * 8 * sizeof(float2));
+  p.grid = std::min((p.nr <= 16 ? 2 : 1) * (sms > 0 ? sms : 148), SIMSD_PAGED_COUNTER_BYTES / (int)sizeof(int));
+  p.ml_at = SIMSD_PAGED_COUNTER_BYTES + align256((size_t)2 * p.grid * D * p.nr * sizeof(float));
+  p.bytes = p.ml_at + align256((size_t)2 * p.grid * p.nr * sizeof(float2));
   return p;
 }
 
@@ -133,13 +133,22 @@ int append(const PagedAppendArgs& a, void* stream) {
   return launch_on(paged_append_kernel<D, BF>, dim3((unsigned)grid), PA_THREADS, (size_t)smem, stream, false, a);
 }
 
-template <int D, int NT, bool BF>
+template <int D, int NT, int RG, bool BF>
 int attend(const PagedAttnArgs& a, const PagedPlan& pl, void* stream) {
   static bool done[kMaxDev];
-  constexpr int smem = PatSmem<D, NT>::BYTES;
-  int rc = allow_smem(paged_attention_kernel<D, NT, BF>, smem, done);
+  using S = PatShape<D, NT, RG>;
+  const int rc = allow_smem(paged_attention_kernel<D, NT, RG, BF>, S::BYTES, done);
   if (rc != SIMSD_OK) return rc;
-  return launch_on(paged_attention_kernel<D, NT, BF>, dim3((unsigned)pl.grid), PAT_THREADS, smem, stream, false, a);
+  return launch_on(paged_attention_kernel<D, NT, RG, BF>, dim3((unsigned)pl.grid), S::THREADS, S::BYTES, stream, false, a);
+}
+template <int D, bool BF>
+int attend_rows(const PagedAttnArgs& a, const PagedPlan& pl, void* stream) {
+  switch (pl.nr) {
+    case 8: return attend<D, 1, 1, BF>(a, pl, stream);
+    case 16: return attend<D, 2, 1, BF>(a, pl, stream);
+    case 32: return attend<D, 2, 2, BF>(a, pl, stream);
+    default: return attend<D, 2, 4, BF>(a, pl, stream);
+  }
 }
 
 }  // namespace
@@ -245,22 +254,16 @@ int simsd_paged_attention(const void* q, const void* k_cache, const void* v_cach
   a.scale_log2 = std::max(std::fabs(scale) * 1.4426950408889634f, 1e-30f);
   const PagedPlan pl = paged_plan(L, a.G, head_dim);
   a.rows = a.G * L;
-  a.row_tiles = (a.rows + pl.nt * 8 - 1) / (pl.nt * 8);
-  if ((long long)B * Hk * a.row_tiles * ((int64_t)max_pages * page_size / PAT_TK + 1) > 0x7fffffffLL)
+  a.row_tiles = (a.rows + pl.nr - 1) / pl.nr;
+  if ((long long)B * Hk * a.row_tiles * ((int64_t)max_pages * page_size / 48 + 1) > 0x7fffffffLL)
     return SIMSD_ERR_UNSUPPORTED;
   uint8_t* ws = reinterpret_cast<uint8_t*>(workspace);
   a.arrived = reinterpret_cast<int*>(ws);
   a.part_o = reinterpret_cast<float4*>(ws + SIMSD_PAGED_COUNTER_BYTES);
   a.part_ml = reinterpret_cast<float2*>(ws + pl.ml_at);
-  const bool bf = dtype == SIMSD_BF16;
-  switch (pl.nt * 1000 + head_dim) {
-    case 1064: return bf ? attend<64, 1, true>(a, pl, stream) : attend<64, 1, false>(a, pl, stream);
-    case 1128: return bf ? attend<128, 1, true>(a, pl, stream) : attend<128, 1, false>(a, pl, stream);
-    case 2064: return bf ? attend<64, 2, true>(a, pl, stream) : attend<64, 2, false>(a, pl, stream);
-    case 2128: return bf ? attend<128, 2, true>(a, pl, stream) : attend<128, 2, false>(a, pl, stream);
-    case 4064: return bf ? attend<64, 4, true>(a, pl, stream) : attend<64, 4, false>(a, pl, stream);
-    default: return bf ? attend<128, 4, true>(a, pl, stream) : attend<128, 4, false>(a, pl, stream);
-  }
+  if (dtype == SIMSD_BF16)
+    return head_dim == 64 ? attend_rows<64, true>(a, pl, stream) : attend_rows<128, true>(a, pl, stream);
+  return head_dim == 64 ? attend_rows<64, false>(a, pl, stream) : attend_rows<128, false>(a, pl, stream);
 }
 
 size_t simsd_speculative_verify_workspace_size(int B, int K, int V) {
