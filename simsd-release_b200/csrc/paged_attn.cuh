@@ -5,6 +5,8 @@
 // = j - (n - L), a key with jt < 0 is visible to all of them, the others where
 // jt <= t, or where tail_mask[b, t, jt] is set.  No visible key: o = 0, lse = -inf.
 //
+// This file: up to 16 rows (G L) per KV head; more in paged_attn_tc.cuh.
+//
 // What bounds it: every key and value is read once for the G L rows that share it
 // (4 G L operations per 2-byte element), so up to some 64 rows HBM bounds it and
 // the work is to keep loads in flight on every SM and to cut any mix of lengths
@@ -19,7 +21,7 @@
 // CTA, zero again afterwards) joins the parts, always in key order.
 //
 // In a CTA each key group (a warp, or one per 16 rows where there are more) takes 16 keys of every unit through a ring of its own (cp.async, no barrier
-// between key groups until the sequence ends), loading ahead across sequence ends;
+// between warps until the sequence ends), loading ahead across sequence ends;
 // the next sequence's queries are fetched a sequence ahead.
 // Products with the roles swapped, so that few rows waste little: S^T = K Q^T
 // (m16n8k16: 16 keys x 8 rows), P^T turned into the second product's operand with
@@ -58,24 +60,19 @@ struct PagedAttnArgs {
   float scale_log2;         // |scale| log2(e), positive
 };
 
-// A CTA's warps: KG key groups of 16 keys (a unit is one step of all of them, TK
-// keys) x RG row groups of NT 8-row tiles (NR rows in all).  Up to 16 rows one row
-// group holds them, its queries as fragments in registers, in two CTAs of 4 warps
-// per SM.  More rows take more row groups, which share the keys and values of their
-// key group and the queries in shared memory, in one CTA of 12 warps (so that a
-// thread's sums stay in registers).
-template <int D, int NT, int RG>
+// A CTA is 4 warps of 16 keys (a unit is one step of all of them) x NT 8-row tiles.
+constexpr int PAT_WARPS = 4, PAT_THREADS = PAT_WARPS * 32, PAT_TK = 16 * PAT_WARPS;
+constexpr int PAT_CTAS_PER_SM = 2;
+
+template <int D, int NT>
 struct PatShape {
-  static constexpr int KG = RG == 1 ? 4 : 12 / RG, TK = 16 * KG;
-  static constexpr int THREADS = KG * RG * 32, CTAS_PER_SM = RG == 1 ? 2 : 1;
-  static constexpr int NR = NT * 8 * RG;
-  static constexpr int STAGES = RG == 4 ? 5 : 3;
+  static constexpr int NR = NT * 8;
+  static constexpr int STAGES = 3;
   static constexpr int MAT = 16 * D * 2;                       // 16 keys (or values)
-  static constexpr int RING = KG * STAGES * 2 * MAT;
-  static constexpr int OBUF = KG * RG * (D / 16) * 32 * 16;    // one 8-row tile of every warp's O
-  static constexpr int Q = RG > 1 ? NR * D * 2 : 0;
-  static constexpr int ML = 2 * KG * NR * 4;
-  static constexpr int BYTES = RING + OBUF + Q + ML;
+  static constexpr int RING = PAT_WARPS * STAGES * 2 * MAT;
+  static constexpr int OBUF = PAT_WARPS * (D / 16) * 32 * 16;  // one 8-row tile of every warp's O
+  static constexpr int ML = 2 * PAT_WARPS * NR * 4;
+  static constexpr int BYTES = RING + OBUF + ML;
 };
 
 __device__ __forceinline__ void pat_ldsm(uint32_t addr, uint32_t (&r)[4]) {
@@ -282,15 +279,13 @@ struct PagedPart {
 // Joins the parts of a cut sequence (one KV head and row tile of it) that starts
 // in CTA c0: part i's max, sum and O lie in slot 1 of CTA c0 for i = 0, in slot 0
 // of CTA c0 + i for the others.  `buf`: OBUF bytes of shared memory.
-template <int D, int NT, int RG, bool BF>
+template <int D, int NT, bool BF>
 __device__ __noinline__ void paged_join(const PagedAttnArgs& p, int b, int g, int r0, int c0, int parts, float* buf) {
-  using S = PatShape<D, NT, RG>;
-  constexpr int MT = D / 16, NR = S::NR, TILES = NR / 8, THREADS = S::THREADS;
-  constexpr int ALL = MT * TILES * 32, PER = (ALL + THREADS - 1) / THREADS;   // fragments, and of a thread
-  constexpr int GR = THREADS / NR, KEEP = 4;                  // threads of a row, parts a thread keeps
+  using S = PatShape<D, NT>;
+  constexpr int MT = D / 16, NR = S::NR, ALL = MT * NT * 32, PER = ALL / PAT_THREADS;   // fragments, and of a thread
+  constexpr int GR = PAT_THREADS / NR, KEEP = 4;              // threads of a row, parts a thread keeps
   constexpr int CAP = S::OBUF / 4 / NR;                       // parts whose weights fit in buf
   const int tid = threadIdx.x, lane = tid & 31, r = tid % NR, grp = tid / NR;
-  const bool rows = grp < GR;                                 // this thread looks after row r
   auto slot = [&](int i) { return i == 0 ? 2 * c0 + 1 : 2 * (c0 + i); };
   // the first two parts of O (most sequences are cut once) are on their way while the weights are made
   float4 lead[2][PER];
@@ -298,12 +293,12 @@ __device__ __noinline__ void paged_join(const PagedAttnArgs& p, int b, int g, in
   for (int i = 0; i < 2; ++i)
 #pragma unroll
     for (int k = 0; k < PER; ++k)
-      lead[i][k] = __ldcg(p.part_o + (long long)slot(i) * ALL + min(tid + k * THREADS, ALL - 1));
+      lead[i][k] = __ldcg(p.part_o + (long long)slot(i) * ALL + tid + k * PAT_THREADS);
   float2 keep[KEEP];
 #pragma unroll
   for (int k = 0; k < KEEP; ++k) {
     const int i = grp + k * GR;
-    keep[k] = rows && i < parts ? __ldcg(p.part_ml + slot(i) * NR + r) : make_float2(-INFINITY, 0.0f);
+    keep[k] = i < parts ? __ldcg(p.part_ml + slot(i) * NR + r) : make_float2(-INFINITY, 0.0f);
   }
   float mm = -INFINITY, ll = 0.0f;
   auto see = [&](float2 x) {
@@ -313,9 +308,9 @@ __device__ __noinline__ void paged_join(const PagedAttnArgs& p, int b, int g, in
   };
 #pragma unroll
   for (int k = 0; k < KEEP; ++k) see(keep[k]);
-  for (int i = grp + KEEP * GR; rows && i < parts; i += GR) see(__ldcg(p.part_ml + slot(i) * NR + r));
+  for (int i = grp + KEEP * GR; i < parts; i += GR) see(__ldcg(p.part_ml + slot(i) * NR + r));
   float* all = buf + GR * NR;
-  if (rows) buf[grp * NR + r] = mm, all[grp * NR + r] = ll;
+  buf[grp * NR + r] = mm, all[grp * NR + r] = ll;
   __syncthreads();
   mm = -INFINITY, ll = 0.0f;
 #pragma unroll
@@ -328,7 +323,7 @@ __device__ __noinline__ void paged_join(const PagedAttnArgs& p, int b, int g, in
   for (int i0 = 0; i0 < parts; i0 += CAP) {
     const int n = min(CAP, parts - i0);
     __syncthreads();
-    for (int i = grp; rows && i < n; i += GR) {
+    for (int i = grp; i < n; i += GR) {
       const int k = (i0 + i) / GR;
       float x = 0.0f;
       if (k < KEEP) {
@@ -341,7 +336,7 @@ __device__ __noinline__ void paged_join(const PagedAttnArgs& p, int b, int g, in
     }
     __syncthreads();
     auto add = [&](int i, int k, float4 v) {
-      const int rr = (tid + k * THREADS) / 32 % TILES * 8 + 2 * (lane & 3);
+      const int rr = (tid + k * PAT_THREADS) / 32 % NT * 8 + 2 * (lane & 3);
       const float f0 = buf[i * NR + rr], f1 = buf[i * NR + rr + 1];
       a[k].x = fmaf(v.x, f0, a[k].x), a[k].y = fmaf(v.y, f1, a[k].y);
       a[k].z = fmaf(v.z, f0, a[k].z), a[k].w = fmaf(v.w, f1, a[k].w);
@@ -357,65 +352,56 @@ __device__ __noinline__ void paged_join(const PagedAttnArgs& p, int b, int g, in
     for (; i < n; ++i) {
       const float4* o = p.part_o + (long long)slot(i0 + i) * ALL;
 #pragma unroll
-      for (int k = 0; k < PER; ++k) add(i, k, __ldcg(o + min(tid + k * THREADS, ALL - 1)));
+      for (int k = 0; k < PER; ++k) add(i, k, __ldcg(o + tid + k * PAT_THREADS));
     }
   }
 #pragma unroll
   for (int k = 0; k < PER; ++k) {
-    const int x = tid + k * THREADS, rr = r0 + x / 32 % TILES * 8 + (lane >> 2);
-    if (x >= ALL) break;                                      // whole warps
-    paged_store<BF, D>(p, rr < p.rows ? paged_row(p, b, g, rr) : -1, x / (TILES * 32), lane, a[k]);
+    const int x = tid + k * PAT_THREADS, rr = r0 + x / 32 % NT * 8 + (lane >> 2);
+    paged_store<BF, D>(p, rr < p.rows ? paged_row(p, b, g, rr) : -1, x / (NT * 32), lane, a[k]);
   }
 }
 
-template <int D, int NT, int RG, bool BF>
-__global__ void __launch_bounds__(PatShape<D, NT, RG>::THREADS, PatShape<D, NT, RG>::CTAS_PER_SM)
-    paged_attention_kernel(const __grid_constant__ PagedAttnArgs p) {
+template <int D, int NT, bool BF>
+__global__ void __launch_bounds__(PAT_THREADS, PAT_CTAS_PER_SM) paged_attention_kernel(const __grid_constant__ PagedAttnArgs p) {
   griddep_launch_dependents();
   griddep_wait();
-  using S = PatShape<D, NT, RG>;
-  constexpr int THREADS = S::THREADS, KG = S::KG, TK = S::TK, NR = S::NR, TILES = NR / 8;
+  using S = PatShape<D, NT>;
+  constexpr int NR = S::NR;
   constexpr int MT = D / 16, CH = D / 8;                  // 16-dim tiles, 16-byte chunks of a key
   constexpr int KPI = 32 / CH;                            // keys per cp.async of the warp
-  constexpr bool QREG = RG == 1;
-  constexpr int QW = QREG ? MT * NT * 2 : (NR * CH + THREADS - 1) / THREADS * 4;   // words of the queries in a thread
+  constexpr int QW = MT * NT * 2;                         // words of the queries in a thread
   extern __shared__ __align__(256) uint8_t pat_smem[];
   __shared__ PagedPart s_cut[2];
+  __shared__ bool s_join[2];
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
-  const int kg = warp % KG, rg = warp / KG;       // key group, row group
-  const uint32_t ring = smem_u32(pat_smem) + kg * S::STAGES * 2 * S::MAT;
+  const uint32_t ring = smem_u32(pat_smem) + warp * S::STAGES * 2 * S::MAT;
   float4* obuf = reinterpret_cast<float4*>(pat_smem + S::RING);
-  uint8_t* qs = pat_smem + S::RING + S::OBUF;
-  float* sm_m = reinterpret_cast<float*>(pat_smem + S::RING + S::OBUF + S::Q);
-  float* sm_l = sm_m + KG * NR;
+  float* sm_m = reinterpret_cast<float*>(pat_smem + S::RING + S::OBUF);
+  float* sm_l = sm_m + PAT_WARPS * NR;
 
   __shared__ PagedCut s_range;
-  PagedPos<TK> ld;
+  PagedPos<PAT_TK> ld;
   int steps;
   {
     PagedCut cut;
-    if (!paged_range<THREADS, TK>(p, cut, ld)) return;
+    if (!paged_range<PAT_THREADS, PAT_TK>(p, cut, ld)) return;
     steps = cut.first(blockIdx.x + 1) - cut.first(blockIdx.x);
     if (tid == 0) s_range = cut;
   }
   if (tid < 2) s_cut[tid].parts = 0;
-  PagedPos<TK> at = ld;
+  PagedPos<PAT_TK> at = ld;
 
-  // ---- loads: the key group's 16 keys of position `ld` into its next ring slot; with
-  // several row groups each of their warps loads a share (keys or values, or half of
-  // the rows of either).
+  // ---- loads: the warp's 16 keys of position `ld` into its next ring slot.
   // Pages of a multiple of 16 tokens hold all sixteen in one page, a fixed distance
   // apart; otherwise every key's place is looked up (by lane key % 16, handed round).
   // The page numbers are fetched a step ahead.
   const bool page16 = p.page_size % 16 == 0;
   const int kc = lane % CH, khi = lane / CH;
   const uint32_t swz = (uint32_t)(khi * (D * 2) + ((kc ^ khi) << 4));
-  auto fetch_page = [&](const PagedPos<TK>& x) {
-    const int key = x.unit * TK + kg * 16 + (page16 ? 0 : lane & 15);
+  auto fetch_page = [&](const PagedPos<PAT_TK>& x) {
+    const int key = x.unit * PAT_TK + warp * 16 + (page16 ? 0 : lane & 15);
     return key < x.n ? p.page_table[x.b * p.ld_table + p.page_div(key)] : -1;
-  };
-  auto mine = [&](int i, int mat) {
-    return RG == 1 || (RG == 2 ? rg == mat : rg == 2 * mat + (i >= 8 / KPI));
   };
   int page = fetch_page(ld);
   int loaded = 0;
@@ -423,7 +409,7 @@ __global__ void __launch_bounds__(PatShape<D, NT, RG>::THREADS, PatShape<D, NT, 
   auto load = [&]() {
     if (loaded < steps) {
       const uint32_t dst = load_slot + swz;
-      const int key0 = ld.unit * TK + kg * 16;
+      const int key0 = ld.unit * PAT_TK + warp * 16;
       if (key0 < ld.n) {
         const bool fine = page >= 0 && page < p.num_pages;
         if (page16) {
@@ -438,8 +424,8 @@ __global__ void __launch_bounds__(PatShape<D, NT, RG>::THREADS, PatShape<D, NT, 
           for (int i = 0; i < 16 / KPI; ++i) {
             const uint32_t s = (dst ^ ((i * KPI & 7) << 4)) + i * KPI * (D * 2);
             const bool ok = left > i * KPI;
-            if (mine(i, 0)) pat_cp16(s, ok ? k : reinterpret_cast<const char*>(p.k_cache), ok);
-            if (mine(i, 1)) pat_cp16(s + S::MAT, ok ? v : reinterpret_cast<const char*>(p.v_cache), ok);
+            pat_cp16(s, ok ? k : reinterpret_cast<const char*>(p.k_cache), ok);
+            pat_cp16(s + S::MAT, ok ? v : reinterpret_cast<const char*>(p.v_cache), ok);
             k += step;
             v += step;
           }
@@ -458,8 +444,8 @@ __global__ void __launch_bounds__(PatShape<D, NT, RG>::THREADS, PatShape<D, NT, 
             const long long o = __shfl_sync(0xffffffffu, off, i * KPI + khi);
             const uint32_t s = (dst ^ ((i * KPI & 7) << 4)) + i * KPI * (D * 2);
             const long long e = o < 0 ? 0 : o + kc * 8;
-            if (mine(i, 0)) pat_cp16(s, reinterpret_cast<const uint16_t*>(p.k_cache) + e, o >= 0);
-            if (mine(i, 1)) pat_cp16(s + S::MAT, reinterpret_cast<const uint16_t*>(p.v_cache) + e, o >= 0);
+            pat_cp16(s, reinterpret_cast<const uint16_t*>(p.k_cache) + e, o >= 0);
+            pat_cp16(s + S::MAT, reinterpret_cast<const uint16_t*>(p.v_cache) + e, o >= 0);
           }
         }
       }
@@ -474,32 +460,18 @@ __global__ void __launch_bounds__(PatShape<D, NT, RG>::THREADS, PatShape<D, NT, 
     pat_commit();
   };
 
-  // ---- queries of a row tile: up to 16 rows as the first product's fragments in
-  // registers, more through shared memory
+  // ---- queries of a row tile, as the first product's fragments
   uint32_t qnext[QW];
   auto fetch_queries = [&](int b, int g, int rt) {
-    const int r0 = rt * NR;                                // QREG: the one row group's
     const uint16_t* qb = reinterpret_cast<const uint16_t*>(p.q);
-    if constexpr (QREG) {
 #pragma unroll
-      for (int nt = 0; nt < NT; ++nt) {
-        const int r = r0 + nt * 8 + (lane >> 2);
-        const bool in = r < p.rows && b < p.B;
-        const uint16_t* src = qb + (in ? paged_row(p, b, g, r) * D : 0) + 2 * (lane & 3);
+    for (int nt = 0; nt < NT; ++nt) {
+      const int r = rt * NR + nt * 8 + (lane >> 2);
+      const bool in = r < p.rows && b < p.B;
+      const uint16_t* src = qb + (in ? paged_row(p, b, g, r) * D : 0) + 2 * (lane & 3);
 #pragma unroll
-        for (int k = 0; k < MT * 2; ++k)
-          qnext[k * NT + nt] = in ? __ldg(reinterpret_cast<const uint32_t*>(src + k * 8)) ^ p.q_sign : 0u;
-      }
-    } else {
-#pragma unroll
-      for (int k = 0; k < QW / 4; ++k) {
-        const int x = tid + k * THREADS, r = r0 + x / CH;
-        const bool in = x < NR * CH && r < p.rows && b < p.B;
-        const uint4 v = in ? __ldg(reinterpret_cast<const uint4*>(qb + paged_row(p, b, g, r) * D + x % CH * 8))
-                           : make_uint4(0, 0, 0, 0);
-        const uint32_t f = in ? p.q_sign : 0u;
-        qnext[4 * k] = v.x ^ f, qnext[4 * k + 1] = v.y ^ f, qnext[4 * k + 2] = v.z ^ f, qnext[4 * k + 3] = v.w ^ f;
-      }
+      for (int k = 0; k < MT * 2; ++k)
+        qnext[k * NT + nt] = in ? __ldg(reinterpret_cast<const uint32_t*>(src + k * 8)) ^ p.q_sign : 0u;
     }
   };
   fetch_queries(at.b, at.g, at.rt);
@@ -511,32 +483,20 @@ __global__ void __launch_bounds__(PatShape<D, NT, RG>::THREADS, PatShape<D, NT, 
   // is an exclusive or with multiples of 32.
   const uint32_t k_lane = (lane & 15) * (D * 2) + (((lane >> 4) ^ (lane & 7)) << 4);
   const uint32_t v_lane = ((lane & 7) + (lane >> 4) * 8) * (D * 2) + ((((lane >> 3) & 1) ^ (lane & 7)) << 4);
-  const uint32_t q_lane = smem_u32(qs) + (rg * NT * 8 + (lane >> 4) * 8 + (lane & 7)) * (D * 2) +
-                          ((((lane >> 3) & 1) ^ (lane & 7)) << 4);
 
   float o[MT][NT][4], m[NT][2], l[NT][2];
-  uint32_t bq[QREG ? QW : 1];
+  uint32_t bq[QW];
   int first_unit = at.unit;
   uint32_t slot_at = ring;
   for (int i = 0; i < steps; ++i) {
     if (i == 0 || at.unit == 0) {
       // a new sequence, head or row tile: its queries, and empty sums
       first_unit = at.unit;
-      if constexpr (QREG) {
 #pragma unroll
-        for (int k = 0; k < QW; ++k) bq[k] = qnext[k];
-      } else {
-#pragma unroll
-        for (int k = 0; k < QW / 4; ++k) {
-          const int x = tid + k * THREADS, rr = x / CH, c = x % CH;
-          if (x < NR * CH) *reinterpret_cast<uint4*>(qs + rr * (D * 2) + ((c ^ (rr & 7)) << 4)) =
-              make_uint4(qnext[4 * k], qnext[4 * k + 1], qnext[4 * k + 2], qnext[4 * k + 3]);
-        }
-        __syncthreads();
-      }
+      for (int k = 0; k < QW; ++k) bq[k] = qnext[k];
       if (at.nu - at.unit < steps - i) {
         int b = at.b, g = at.g, rt = at.rt;
-        PagedPos<TK>::next_rows(p, b, g, rt);
+        PagedPos<PAT_TK>::next_rows(p, b, g, rt);
         fetch_queries(b, g, rt);
       }
 #pragma unroll
@@ -549,20 +509,13 @@ __global__ void __launch_bounds__(PatShape<D, NT, RG>::THREADS, PatShape<D, NT, 
           for (int e = 0; e < 4; ++e) o[mt][nt][e] = 0.0f;
       }
     }
-    if constexpr (RG == 1) {
-      load();
-      pat_wait<S::STAGES - 1>();
-      __syncwarp();
-    } else {
-      // the slot's loads by all row groups have arrived, and all have left the slot that load() fills
-      pat_wait<S::STAGES - 2>();
-      named_bar_sync(1 + kg, RG * 32);
-      load();
-    }
+    load();
+    pat_wait<S::STAGES - 1>();
+    __syncwarp();
     const uint32_t ks_base = slot_at, vs_base = ks_base + S::MAT;
     slot_at += 2 * S::MAT;
     if (slot_at == ring + S::STAGES * 2 * S::MAT) slot_at = ring;
-    const int key0 = at.unit * TK + kg * 16;
+    const int key0 = at.unit * PAT_TK + warp * 16;
     if (key0 < at.n) {
       // S^T = K Q^T
       float s[NT][4];
@@ -572,21 +525,10 @@ __global__ void __launch_bounds__(PatShape<D, NT, RG>::THREADS, PatShape<D, NT, 
       for (int ks = 0; ks < MT; ++ks) {
         uint32_t a[4];
         pat_ldsm((ks_base + k_lane) ^ (ks << 5), a);
-        if constexpr (QREG) {
 #pragma unroll
-          for (int nt = 0; nt < NT; ++nt) pat_mma<BF>(s[nt], a, bq[2 * ks * NT + nt], bq[(2 * ks + 1) * NT + nt]);
-        } else {
-#pragma unroll
-          for (int nt = 0; nt < NT; nt += 2) {
-            // 16 rows of the row group, both 8-element halves of this k step
-            uint32_t b[4];
-            pat_ldsm((q_lane + nt * 8 * (D * 2)) ^ (ks << 5), b);
-            pat_mma<BF>(s[nt], a, b[0], b[1]);
-            pat_mma<BF>(s[nt + 1], a, b[2], b[3]);
-          }
-        }
+        for (int nt = 0; nt < NT; ++nt) pat_mma<BF>(s[nt], a, bq[2 * ks * NT + nt], bq[(2 * ks + 1) * NT + nt]);
       }
-      const int r0 = at.rt * NR + rg * NT * 8;
+      const int r0 = at.rt * NR;
       const bool edge = key0 + 16 > at.n - p.L;          // some key of the sixteen may be hidden from some row
       if (edge) {
         uint32_t see = 0;
@@ -686,9 +628,9 @@ __global__ void __launch_bounds__(PatShape<D, NT, RG>::THREADS, PatShape<D, NT, 
     __syncwarp();
     const bool ends = at.unit + 1 == at.nu;
     if (ends || i + 1 == steps) {
-      // join the key groups; a whole sequence is written, a part goes to the workspace
+      // join the warps; a whole sequence is written, a part goes to the workspace
       const bool whole = ends && first_unit == 0;
-      const int part = first_unit == 0 ? 1 : 0, slot = 2 * blockIdx.x + part, r0 = at.rt * NR, w0r = rg * NT * 8;
+      const int part = first_unit == 0 ? 1 : 0, slot = 2 * blockIdx.x + part, r0 = at.rt * NR;
 #pragma unroll
       for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
@@ -699,8 +641,8 @@ __global__ void __launch_bounds__(PatShape<D, NT, RG>::THREADS, PatShape<D, NT, 
           x += __shfl_xor_sync(0xffffffffu, x, 16);
           m[nt][e] *= p.scale_log2;
           if (lane < 4) {
-            sm_m[kg * NR + w0r + nt * 8 + 2 * lane + e] = m[nt][e];
-            sm_l[kg * NR + w0r + nt * 8 + 2 * lane + e] = x;
+            sm_m[warp * NR + nt * 8 + 2 * lane + e] = m[nt][e];
+            sm_l[warp * NR + nt * 8 + 2 * lane + e] = x;
           }
         }
       __syncthreads();
@@ -709,18 +651,18 @@ __global__ void __launch_bounds__(PatShape<D, NT, RG>::THREADS, PatShape<D, NT, 
       for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
         for (int e = 0; e < 2; ++e) {
-          const int r = w0r + nt * 8 + 2 * (lane & 3) + e;
+          const int r = nt * 8 + 2 * (lane & 3) + e;
           float mm = -INFINITY, ll = 0.0f;
 #pragma unroll
-          for (int w = 0; w < KG; ++w) mm = fmaxf(mm, sm_m[w * NR + r]);
+          for (int w = 0; w < PAT_WARPS; ++w) mm = fmaxf(mm, sm_m[w * NR + r]);
           const float mu = mm == -INFINITY ? 0.0f : mm;
 #pragma unroll
-          for (int w = 0; w < KG; ++w) ll = fmaf(sm_l[w * NR + r], pat_exp2(sm_m[w * NR + r] - mu), ll);
+          for (int w = 0; w < PAT_WARPS; ++w) ll = fmaf(sm_l[w * NR + r], pat_exp2(sm_m[w * NR + r] - mu), ll);
           const float f = pat_exp2(m[nt][e] - mu);
           inv[nt][e] = !whole ? 1.0f : ll == 0.0f ? 0.0f : 1.0f / ll;
 #pragma unroll
           for (int mt = 0; mt < MT; ++mt) o[mt][nt][e] *= f, o[mt][nt][e + 2] *= f;
-          if (kg == 0 && lane < 4) {
+          if (warp == 0 && lane < 4) {
             if (whole)
               paged_store_lse(p, at.b, at.g, r0 + r, mm, ll);
             else
@@ -729,7 +671,7 @@ __global__ void __launch_bounds__(PatShape<D, NT, RG>::THREADS, PatShape<D, NT, 
         }
 #pragma unroll
       for (int nt = 0; nt < NT; ++nt) {
-        const int r = r0 + w0r + nt * 8 + (lane >> 2);
+        const int r = r0 + nt * 8 + (lane >> 2);
         const long long row = r < p.rows ? paged_row(p, at.b, at.g, r) : -1;
         if (nt > 0) __syncthreads();
 #pragma unroll
@@ -737,13 +679,12 @@ __global__ void __launch_bounds__(PatShape<D, NT, RG>::THREADS, PatShape<D, NT, 
           obuf[(warp * MT + mt) * 32 + lane] = make_float4(o[mt][nt][0], o[mt][nt][1], o[mt][nt][2], o[mt][nt][3]);
         __syncthreads();
 #pragma unroll
-        for (int k = 0; k < (MT + KG - 1) / KG; ++k) {
-          const int mt = kg + k * KG;
-          if (mt >= MT) break;
-          const float4* from = obuf + (rg * KG * MT + mt) * 32 + lane;
+        for (int k = 0; k < MT / PAT_WARPS; ++k) {
+          const int mt = warp + k * PAT_WARPS;
+          const float4* from = obuf + mt * 32 + lane;
           float4 a = from[0];
 #pragma unroll
-          for (int w = 1; w < KG; ++w) {
+          for (int w = 1; w < PAT_WARPS; ++w) {
             const float4 x = from[w * MT * 32];
             a.x += x.x, a.y += x.y, a.z += x.z, a.w += x.w;
           }
@@ -751,7 +692,7 @@ __global__ void __launch_bounds__(PatShape<D, NT, RG>::THREADS, PatShape<D, NT, 
           if (whole)
             paged_store<BF, D>(p, row, mt, lane, a);
           else
-            p.part_o[(((long long)slot * MT + mt) * TILES + rg * NT + nt) * 32 + lane] = a;
+            p.part_o[(((long long)slot * MT + mt) * NT + nt) * 32 + lane] = a;
         }
       }
       if (!whole && tid == 0) {
@@ -765,19 +706,20 @@ __global__ void __launch_bounds__(PatShape<D, NT, RG>::THREADS, PatShape<D, NT, 
   }
   // cut sequences (at most the range's first and last): the last of their CTAs to get here joins the parts
   if (s_cut[0].parts + s_cut[1].parts == 0) return;
-  if (tid < 2 && s_cut[tid].parts > 0) {
-    __threadfence();
-    const int c0 = s_cut[tid].c0;
-    if (atomicAdd(p.arrived + c0, 1) == s_cut[tid].parts - 1)
-      p.arrived[c0] = 0;
-    else
-      s_cut[tid].parts = 0;
-    __threadfence();
+  if (tid < 2) {
+    s_join[tid] = false;
+    if (s_cut[tid].parts > 0) {
+      __threadfence();
+      const int c0 = s_cut[tid].c0;
+      s_join[tid] = atomicAdd(p.arrived + c0, 1) == s_cut[tid].parts - 1;
+      if (s_join[tid]) p.arrived[c0] = 0;
+      __threadfence();
+    }
   }
   __syncthreads();
   for (int k = 0; k < 2; ++k) {
     const PagedPart x = s_cut[k];
-    if (x.parts > 0) paged_join<D, NT, RG, BF>(p, x.b, x.g, x.r0, x.c0, x.parts, reinterpret_cast<float*>(obuf));
+    if (s_join[k]) paged_join<D, NT, BF>(p, x.b, x.g, x.r0, x.c0, x.parts, reinterpret_cast<float*>(obuf));
     __syncthreads();
   }
 }

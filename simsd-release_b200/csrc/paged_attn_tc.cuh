@@ -1,0 +1,561 @@
+// Paged attention for more than 16 rows per KV head (several drafted tokens times
+// the head group), on the 5th-generation tensor cores.  Same operator, cut and
+// workspace scheme as paged_attn.cuh, whose mma.sync products at 32 rows already
+// cost more than reading the keys and values: m16n8k16 runs at about an eighth of the
+// tcgen05 rate here, and 16 x 8 drafted rows x 4 heads took 51 to 57 us against 21
+// of HBM.
+//
+// A unit is 128 keys of one (sequence, KV head, row tile of R = 32, 64 or 128 rows).
+// The products are 128 rows tall whatever R is; the R queries stand in them F = 128 /
+// R times, and copy f of a row keeps only the keys [f R, f R + R) of every unit:
+//   S = Q K^T       [128 x 128 keys], TMEM; a thread per TMEM lane reads its R keys
+//   softmax         per lane (a row's copy is a softmax of its own, joined at the end):
+//                   no exchange between threads, R exponentials each
+//   P               16-bit, in shared memory, zero outside a copy's own keys
+//   O += P V        [128 x D], TMEM, accumulated over the units of the sequence
+// so a unit's softmax is spread over all 128 lanes at 32 rows too.  The running
+// maximum moves only when a score passes it by more than 2^8 (P <= 256 keeps its
+// relative precision in 16 bits), so O is hardly ever rescaled in TMEM.
+//
+// Warps 0-3 softmax and epilogue, 4-7 loads (cp.async into the 128-byte-swizzled
+// operand layout, any page size and stride, a ring of NS operand tiles K, V, K, V,
+// ...; a tile is handed over once its copies have landed and are visible to the
+// tensor cores), 8 issues the products: S of unit n + 1 before O of unit n, so that
+// they overlap its softmax.  One CTA per SM.
+//
+// A value that is not finite, of a key that some rows do not see, is taken out of the
+// product and added to the rows that see it by themselves.  All waits are bounded.
+#pragma once
+#include "paged_attn.cuh"
+
+namespace simsd {
+
+constexpr int PTC_THREADS = 288, PTC_SOFTMAX = 128, PTC_TK = 128;
+
+template <int D, int R>
+struct PtcShape {
+  static constexpr int F = 128 / R;
+  static constexpr int TILE = 128 * D * 2;              // 128 keys, values or rows of queries
+  static constexpr int NS = D == 128 ? 5 : 8;
+  static constexpr int P = 32768;
+  static constexpr int BYTES = 1024 + NS * TILE + TILE + P + 1024 + 512;
+};
+
+__device__ __forceinline__ void ptc_st16(uint32_t taddr, const float (&v)[16]) {
+  asm volatile(
+      "tcgen05.st.sync.aligned.32x32b.x16.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16};" ::"r"(taddr),
+      "r"(__float_as_uint(v[0])), "r"(__float_as_uint(v[1])), "r"(__float_as_uint(v[2])), "r"(__float_as_uint(v[3])),
+      "r"(__float_as_uint(v[4])), "r"(__float_as_uint(v[5])), "r"(__float_as_uint(v[6])), "r"(__float_as_uint(v[7])),
+      "r"(__float_as_uint(v[8])), "r"(__float_as_uint(v[9])), "r"(__float_as_uint(v[10])), "r"(__float_as_uint(v[11])),
+      "r"(__float_as_uint(v[12])), "r"(__float_as_uint(v[13])), "r"(__float_as_uint(v[14])), "r"(__float_as_uint(v[15]))
+      : "memory");
+}
+__device__ __forceinline__ void ptc_wait_st() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
+
+// MN-major operand in the 128-byte swizzle: V as it lies, 16 keys a step
+__device__ __forceinline__ uint64_t ptc_desc_mn(uint32_t addr) {
+  uint64_t d = 0;
+  d |= (uint64_t)((addr >> 4) & 0x3FFF);
+  d |= (uint64_t)(16384 >> 4) << 16;      // to the next 64 dims
+  d |= (uint64_t)(1024 >> 4) << 32;       // to the next 8 keys
+  d |= (uint64_t)1 << 46;
+  d |= (uint64_t)2 << 61;
+  return d;
+}
+
+// 16-byte chunk c of row r of an operand tile (blocks of 64 elements x 128 rows)
+__device__ __forceinline__ uint32_t ptc_off(int r, int c) {
+  return (uint32_t)((c >> 3) * 16384 + r * 128 + (((c ^ r) & 7) << 4));
+}
+
+// Joins the parts of a cut sequence (rows r0 .. r0 + R - 1 of KV head g), as
+// paged_join; parts hold R rows of D.  `buf`: parts * R float2 of shared memory.
+template <int D, int R, bool BF>
+__device__ void ptc_join(const PagedAttnArgs& p, const PagedPart& x, float2* buf) {
+  const int tid = threadIdx.x;
+  auto slot = [&](int i) { return (long long)(i == 0 ? 2 * x.c0 + 1 : 2 * (x.c0 + i)); };
+  for (int k = tid; k < x.parts * R; k += PTC_THREADS) buf[k] = __ldcg(p.part_ml + slot(k / R) * R + k % R);
+  __syncthreads();
+  if (tid < R) {
+    float mm = -INFINITY, ll = 0.0f;
+    for (int i = 0; i < x.parts; ++i) mm = fmaxf(mm, buf[i * R + tid].x);
+    const float mu = mm == -INFINITY ? 0.0f : mm;
+    for (int i = 0; i < x.parts; ++i) {
+      const float w = pat_exp2(buf[i * R + tid].x - mu);
+      ll = fmaf(buf[i * R + tid].y, w, ll);
+      buf[i * R + tid].x = w;
+    }
+    const float inv = ll == 0.0f ? 0.0f : 1.0f / ll;
+    for (int i = 0; i < x.parts; ++i) buf[i * R + tid].x *= inv;
+    paged_store_lse(p, x.b, x.g, x.r0 + tid, mm, ll);
+  }
+  __syncthreads();
+  const float* po = reinterpret_cast<const float*>(p.part_o);
+  for (int k = tid; k < R * (D / 4); k += PTC_THREADS) {
+    const int r = k / (D / 4), c = k % (D / 4);
+    if (x.r0 + r >= p.rows) break;
+    float4 a = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+#pragma unroll 4
+    for (int i = 0; i < x.parts; ++i) {
+      const float4 v = __ldcg(reinterpret_cast<const float4*>(po + (slot(i) * R + r) * D) + c);
+      const float w = buf[i * R + r].x;
+      a.x = fmaf(v.x, w, a.x), a.y = fmaf(v.y, w, a.y), a.z = fmaf(v.z, w, a.z), a.w = fmaf(v.w, w, a.w);
+    }
+    uint2* dst = reinterpret_cast<uint2*>(reinterpret_cast<uint16_t*>(p.o) + paged_row(p, x.b, x.g, x.r0 + r) * D) + c;
+    *dst = make_uint2(pat_pack<BF>(a.x, a.y), pat_pack<BF>(a.z, a.w));
+  }
+  __syncthreads();
+}
+
+template <int D, int R, bool BF>
+__global__ void __launch_bounds__(PTC_THREADS, 1) paged_attention_tc_kernel(const __grid_constant__ PagedAttnArgs p) {
+  using S = PtcShape<D, R>;
+  constexpr int F = S::F, NS = S::NS, CH = D / 8, KPI = 32 / CH;
+  extern __shared__ uint8_t ptc_raw[];
+  uint8_t* ring = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(ptc_raw) + 1023) & ~uintptr_t(1023));
+  uint8_t* Qs = ring + NS * S::TILE;
+  uint8_t* Ps = Qs + S::TILE;
+  float* xm = reinterpret_cast<float*>(Ps + S::P);       // [128] maximum, then [128] sum of a lane
+  float* xl = xm + 128;
+  uint64_t* bars = reinterpret_cast<uint64_t*>(xl + 128);
+  uint64_t *full = bars, *empty = bars + 8, *q_full = bars + 16, *q_empty = bars + 17, *s_full = bars + 18,
+           *p_full = bars + 20, *pv_done = bars + 21, *drained = bars + 22;
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(bars + 23);
+  volatile int* abort_flag = reinterpret_cast<int*>(bars + 23) + 1;
+  uint32_t* bad = reinterpret_cast<uint32_t*>(bars + 24);  // [4] keys of the unit with values that are not finite
+  __shared__ PagedPart s_cut[2];
+  __shared__ PagedCut s_range;
+  __shared__ bool s_join[2];
+  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+
+  if (tid == 0) {
+    for (int s = 0; s < NS; ++s) mbar_init(smem_u32(full + s), 128), mbar_init(smem_u32(empty + s), 1);
+    mbar_init(smem_u32(q_full), 128);
+    mbar_init(smem_u32(q_empty), 1);
+    mbar_init(smem_u32(s_full), 1);
+    mbar_init(smem_u32(s_full + 1), 1);
+    mbar_init(smem_u32(p_full), PTC_SOFTMAX);
+    mbar_init(smem_u32(pv_done), 1);
+    mbar_init(smem_u32(drained), 1);
+    *abort_flag = 0;
+    s_cut[0].parts = s_cut[1].parts = 0;
+    fence_mbar_init();
+  }
+  if (warp == 8) {
+    tmem_alloc(smem_u32(tmem_slot), 512);
+    tmem_relinquish();
+  }
+  griddep_launch_dependents();
+  griddep_wait();
+  PagedPos<PTC_TK> at;
+  PagedCut cut;
+  tc_fence_before();
+  __syncthreads();
+  const bool mine = paged_range<PTC_THREADS, PTC_TK>(p, cut, at);
+  tc_fence_after();
+  const uint32_t tmem = *tmem_slot;
+  const uint32_t o_col = tmem + 256;
+  if (mine) {
+    const int steps = cut.first(blockIdx.x + 1) - cut.first(blockIdx.x);
+    if (tid == 0) s_range = cut;
+    if (warp >= 4 && warp < 8) {
+      // ================= loads
+      const int lt = tid - 128, lw = warp - 4, kc = lane % CH, khi = lane / CH;
+      uint32_t slot = 0, phase = 0, items = 0;
+      // groups of copies that have been issued and not handed over, oldest first
+      uint32_t w0 = 0, w1 = 0, w2 = 0;
+      int waiting = 0;
+      auto flush = [&]() {
+        pat_wait<0>();
+        fence_proxy_async_smem();
+        if (waiting > 0) mbar_arrive(w0);
+        if (waiting > 1) mbar_arrive(w1);
+        if (waiting > 2) mbar_arrive(w2);
+        waiting = 0;
+      };
+      auto issued = [&](uint32_t bar) {
+        pat_commit();
+        if (waiting == 3) {
+          pat_wait<3>();
+          fence_proxy_async_smem();
+          mbar_arrive(w0);
+          w0 = w1, w1 = w2, w2 = bar;
+        } else {
+          if (waiting == 0) w0 = bar;
+          if (waiting == 1) w1 = bar;
+          if (waiting == 2) w2 = bar;
+          ++waiting;
+        }
+      };
+      // nothing waits for a free tile while it holds back one that has been filled
+      auto wait_for = [&](uint32_t bar, uint32_t parity) {
+        bool ok = mbar_try_wait(bar, parity);
+        if (!__all_sync(0xffffffffu, ok)) {
+          flush();
+          ok = mbar_wait(bar, parity, abort_flag, p.err);
+        }
+        return __all_sync(0xffffffffu, ok) != 0;
+      };
+      auto key_page = [&](const PagedPos<PTC_TK>& x) {
+        const int key = x.unit * PTC_TK + lt;
+        return key < x.n ? p.page_table[x.b * p.ld_table + p.page_div(key)] : -1;
+      };
+      int page = key_page(at);
+      for (int n = 0; n < steps; ++n) {
+        const int key = at.unit * PTC_TK + lt;
+        long long off = -1;
+        if (key < at.n) {
+          if (page >= 0 && page < p.num_pages)
+            off = page * p.ld_page + at.g * p.ld_head + (key - p.page_div(key) * p.page_size) * p.ld_tok;
+          else if (p.err)
+            atomicOr(p.err, SIMSD_DEV_ERR_BAD_INDEX);
+        }
+        const PagedPos<PTC_TK> cur = at;
+        if (n + 1 < steps) {
+          at.next(p);
+          page = key_page(at);
+        }
+        auto copy = [&](const void* src) {
+          const uint32_t dst = smem_u32(ring) + slot * S::TILE;
+#pragma unroll
+          for (int i = 0; i < 32 / KPI; ++i) {
+            const long long o = __shfl_sync(0xffffffffu, off, i * KPI + khi);
+            pat_cp16(dst + ptc_off(lw * 32 + i * KPI + khi, kc),
+                     reinterpret_cast<const uint16_t*>(src) + (o < 0 ? 0 : o + kc * 8), o >= 0);
+          }
+          issued(smem_u32(full + slot));
+          if (++slot == NS) slot = 0, phase ^= 1;
+        };
+        if (!wait_for(smem_u32(empty + slot), phase ^ 1)) break;
+        copy(p.k_cache);
+        if (n == 0 || cur.unit == 0) {
+          // the queries of a new sequence, head or row tile, F times
+          if (!wait_for(smem_u32(q_empty), (items & 1) ^ 1)) break;
+          ++items;
+          for (int x = lt; x < 128 * CH; x += 128) {
+            const int row = x / CH, r = cur.rt * R + row % R;
+            const bool in = r < p.rows;
+            pat_cp16(smem_u32(Qs) + ptc_off(row, x % CH),
+                     reinterpret_cast<const uint16_t*>(p.q) + (in ? paged_row(p, cur.b, cur.g, r) * D + x % CH * 8 : 0), in);
+          }
+          issued(smem_u32(q_full));
+        }
+        if (!wait_for(smem_u32(empty + slot), phase ^ 1)) break;
+        copy(p.v_cache);
+      }
+      flush();
+    } else if (warp == 8) {
+      // ================= products
+      if (lane == 0) {
+        const uint32_t idesc_s = make_idesc_f16(BF, 128, 128);
+        const uint32_t idesc_o = make_idesc_f16(BF, 128, D) | (1u << 16);   // V is MN-major
+        uint32_t ks = 0, kph = 0, vs = 1, vph = 0, items = 0;
+        bool ok = true, first = true, prev_first = true, any = false;
+        for (int n = 0; n <= steps && ok; ++n) {
+          if (n < steps) {
+            first = n == 0 || at.unit == 0;
+            if (first && !(ok = mbar_wait(smem_u32(q_full), items++ & 1, abort_flag, p.err))) break;
+            if (!(ok = mbar_wait(smem_u32(full + ks), kph, abort_flag, p.err))) break;
+            tc_fence_after();
+            const uint32_t kt = smem_u32(ring) + ks * S::TILE;
+#pragma unroll
+            for (int kk = 0; kk < D / 16; ++kk) {
+              const uint32_t o = (kk >> 2) * 16384;
+              tc_mma_f16(tmem + (n & 1) * 128, make_sw128_desc(smem_u32(Qs) + o) + 2 * (kk & 3),
+                         make_sw128_desc(kt + o) + 2 * (kk & 3), idesc_s, kk > 0);
+            }
+            any = true;
+            tc_commit(smem_u32(s_full + (n & 1)));
+            tc_commit(smem_u32(empty + ks));
+            if (at.unit + 1 == at.nu) tc_commit(smem_u32(q_empty));
+            ks += 2;
+            if (ks >= NS) ks -= NS, kph ^= 1;
+            at.next(p);
+          }
+          if (n > 0) {
+            if (!(ok = mbar_wait(smem_u32(p_full), (n - 1) & 1, abort_flag, p.err))) break;
+            if (!(ok = mbar_wait(smem_u32(full + vs), vph, abort_flag, p.err))) break;
+            tc_fence_after();
+            const uint32_t vt = smem_u32(ring) + vs * S::TILE;
+#pragma unroll
+            for (int kk = 0; kk < 8; ++kk)
+              tc_mma_f16(o_col, make_sw128_desc(smem_u32(Ps) + (kk >> 2) * 16384) + 2 * (kk & 3), ptc_desc_mn(vt + kk * 2048),
+                         idesc_o, kk > 0 || !prev_first);
+            tc_commit(smem_u32(empty + vs));
+            tc_commit(smem_u32(pv_done));
+            vs += 2;
+            if (vs >= NS) vs -= NS, vph ^= 1;
+          }
+          prev_first = first;
+        }
+        if (any) {   // nothing in flight when the CTA gives its TMEM back
+          tc_commit(smem_u32(drained));
+          mbar_wait_drain(smem_u32(drained), 0, 100000000ull);
+        }
+      }
+      __syncwarp();
+    } else if (warp < 4) {
+      // ================= softmax and epilogue: a thread per TMEM lane, copy f of row `row`
+      const int row = tid % R, f = tid / R;
+      const uint32_t t_lane = (uint32_t)(warp * 32) << 16;
+      uint8_t* own_p = Ps;
+      auto clear_p = [&]() {
+#pragma unroll
+        for (int c = 0; c < 16; ++c) *reinterpret_cast<uint4*>(own_p + ptc_off(tid, c)) = make_uint4(0, 0, 0, 0);
+      };
+      clear_p();
+      float m = -INFINITY, l = 0.0f;       // the maximum in use, unscaled; the sum
+      int first_unit = at.unit;
+      uint32_t vs = 1, vph = 0;
+      bool ok = true;
+      auto wait_all = [&](uint64_t* bar, uint32_t parity) {
+        return named_bar_and(1, PTC_SOFTMAX, mbar_wait(smem_u32(bar), parity, abort_flag, p.err));
+      };
+      for (int n = 0; n < steps && ok; ++n) {
+        if (n == 0 || at.unit == 0) {
+          first_unit = at.unit;
+          m = -INFINITY, l = 0.0f;
+        }
+        if (!(ok = wait_all(s_full + (n & 1), (n >> 1) & 1))) break;
+        tc_fence_after();
+        float v[R];
+#pragma unroll
+        for (int c = 0; c < R / 16; ++c) {
+          float x[16];
+          tmem_ld16(tmem + t_lane + (n & 1) * 128 + f * R + c * 16, x);
+#pragma unroll
+          for (int e = 0; e < 16; ++e) v[c * 16 + e] = x[e];
+        }
+        tmem_wait_ld();
+        if (p.q_sign) {
+#pragma unroll
+          for (int c = 0; c < R; ++c) v[c] = -v[c];
+        }
+        const int k0 = at.unit * PTC_TK, key0 = k0 + f * R, base = at.n - p.L;
+        const bool edge = k0 + PTC_TK > base;
+        uint32_t see[R / 32];
+        bool strange = false;
+        if (edge) {
+          // the lane's keys that its row sees
+          const int t = min(p.g_div(at.rt * R + row), p.L - 1);
+          const int lim = (p.tail ? min(at.n, base) : min(at.n, base + t + 1)) - key0;
+          const uint8_t* tm = p.tail ? p.tail + at.b * p.ldm_b + t * p.ldm_t : nullptr;
+#pragma unroll
+          for (int w = 0; w < R / 32; ++w) {
+            const int k = lim - 32 * w;
+            see[w] = k <= 0 ? 0u : k >= 32 ? 0xffffffffu : (1u << k) - 1u;
+            if (tm) {
+              const int lo = max(0, base - (key0 + 32 * w)), hi = min(32, at.n - (key0 + 32 * w));
+#pragma unroll 8
+              for (int c = lo; c < hi; ++c) see[w] |= (uint32_t)(tm[key0 + 32 * w + c - base] != 0) << c;
+            }
+          }
+#pragma unroll
+          for (int c = 0; c < R; ++c)
+            if (!(see[c / 32] >> (c % 32) & 1)) v[c] = -INFINITY;
+          if (p.L > 1 || p.tail) {
+            // keys that some row may not see: values that are not finite leave the product
+            if (!(ok = wait_all(full + vs, vph))) break;
+            bool odd = false;
+            uint8_t* vt = ring + vs * S::TILE;
+            if (k0 + tid >= base && k0 + tid < at.n) {
+              constexpr uint32_t EXP = BF ? 0x7f80u : 0x7c00u;
+              for (int c = 0; c < CH; ++c) {
+                const uint4 u = *reinterpret_cast<const uint4*>(vt + ptc_off(tid, c));
+                const uint32_t w[4] = {u.x, u.y, u.z, u.w};
+#pragma unroll
+                for (int k = 0; k < 4; ++k) odd |= (w[k] & EXP) == EXP || ((w[k] >> 16) & EXP) == EXP;
+              }
+              if (odd)
+                for (int c = 0; c < CH; ++c) *reinterpret_cast<uint4*>(vt + ptc_off(tid, c)) = make_uint4(0, 0, 0, 0);
+            }
+            const uint32_t b = __ballot_sync(0xffffffffu, odd);
+            if (lane == 0) bad[warp] = b;
+            named_bar_sync(1, PTC_SOFTMAX);
+            strange = (bad[0] | bad[1] | bad[2] | bad[3]) != 0;
+          }
+        }
+        float m4[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+#pragma unroll
+        for (int c = 0; c < R; ++c) m4[c & 3] = fmaxf(m4[c & 3], v[c]);
+        const float mx = fmaxf(fmaxf(m4[0], m4[1]), fmaxf(m4[2], m4[3]));
+        // O of the units before has been summed, P may be written
+        if (n > 0 && !(ok = wait_all(pv_done, (n - 1) & 1))) break;
+        const bool up = m == -INFINITY ? mx > m : (mx - m) * p.scale_log2 > 8.0f;
+        if (__any_sync(0xffffffffu, up)) {
+          const float to = up ? mx : m;
+          const float w = !up ? 1.0f : m == -INFINITY ? 0.0f : pat_exp2((m - to) * p.scale_log2);
+          m = to;
+          l *= w;
+          if (n > 0 && at.unit > first_unit) {
+            tc_fence_after();
+#pragma unroll 1
+            for (int c = 0; c < D / 16; ++c) {
+              float x[16];
+              tmem_ld16(o_col + t_lane + c * 16, x);
+              tmem_wait_ld();
+#pragma unroll
+              for (int e = 0; e < 16; ++e) x[e] *= w;
+              ptc_st16(o_col + t_lane + c * 16, x);
+            }
+            ptc_wait_st();
+          }
+        }
+        const float ms = m == -INFINITY ? 0.0f : m * p.scale_log2;
+        float l4[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+        for (int c = 0; c < R; ++c) {
+          v[c] = pat_exp2(fmaf(v[c], p.scale_log2, -ms));
+          l4[c & 3] += v[c];
+        }
+        l += (l4[0] + l4[1]) + (l4[2] + l4[3]);
+#pragma unroll
+        for (int c = 0; c < R / 8; ++c)
+          *reinterpret_cast<uint4*>(own_p + ptc_off(tid, f * (R / 8) + c)) =
+              make_uint4(pat_pack<BF>(v[8 * c], v[8 * c + 1]), pat_pack<BF>(v[8 * c + 2], v[8 * c + 3]),
+                         pat_pack<BF>(v[8 * c + 4], v[8 * c + 5]), pat_pack<BF>(v[8 * c + 6], v[8 * c + 7]));
+        tc_fence_before();
+        fence_proxy_async_smem();
+        mbar_arrive(smem_u32(p_full));
+        vs += 2;
+        if (vs >= NS) vs -= NS, vph ^= 1;
+        const bool ends = at.unit + 1 == at.nu, leaves = ends || n + 1 == steps;
+        if (strange || leaves) {
+          if (!(ok = wait_all(pv_done, n & 1))) break;
+          tc_fence_after();
+        }
+        if (strange) {
+          // the values that were taken out, for the rows that see them
+#pragma unroll 1
+          for (int k = 0; k < 128; ++k) {
+            if (!(bad[k / 32] >> (k % 32) & 1)) continue;
+            const int j = k0 + k, c = k - f * R;
+            float w = 0.0f;
+            bool on = false;
+#pragma unroll
+            for (int e = 0; e < R; ++e)
+              if (e == c) w = v[e], on = see[e / 32] >> (e % 32) & 1;
+            const int page = p.page_table[at.b * p.ld_table + p.page_div(j)];
+            if (page < 0 || page >= p.num_pages) continue;
+            const long long off = page * p.ld_page + at.g * p.ld_head + (j - p.page_div(j) * p.page_size) * p.ld_tok;
+#pragma unroll 1
+            for (int d = 0; d < D / 16; ++d) {
+              float x[16];
+              tmem_ld16(o_col + t_lane + d * 16, x);
+              tmem_wait_ld();
+#pragma unroll
+              for (int e = 0; e < 16; ++e)
+                if (on) x[e] = fmaf(w, load_f(p.v_cache, off + d * 16 + e, BF ? 0 : 1), x[e]);
+              ptc_st16(o_col + t_lane + d * 16, x);
+            }
+            ptc_wait_st();
+          }
+          named_bar_sync(1, PTC_SOFTMAX);          // `bad` read
+          tc_fence_before();
+        }
+        if (leaves) {
+          // a whole sequence is written, a part goes to the workspace
+          const bool whole = ends && first_unit == 0;
+          const int part = first_unit == 0 ? 1 : 0, r0 = at.rt * R;
+          const long long slot = 2LL * blockIdx.x + part;
+          m *= p.scale_log2;
+          float mm = m, ll = l, w = 1.0f;
+          if constexpr (F > 1) {
+            xm[tid] = m, xl[tid] = l;
+            named_bar_sync(1, PTC_SOFTMAX);
+            mm = -INFINITY, ll = 0.0f;
+#pragma unroll
+            for (int k = 0; k < F; ++k) mm = fmaxf(mm, xm[k * R + row]);
+            const float mu = mm == -INFINITY ? 0.0f : mm;
+#pragma unroll
+            for (int k = 0; k < F; ++k) ll = fmaf(xl[k * R + row], pat_exp2(xm[k * R + row] - mu), ll);
+            w = pat_exp2(m - mu);
+          }
+          if (whole) w *= ll == 0.0f ? 0.0f : 1.0f / ll;
+          if (f == 0) {
+            if (whole)
+              paged_store_lse(p, at.b, at.g, r0 + row, mm, ll);
+            else
+              p.part_ml[slot * R + row] = make_float2(mm, ll);
+          }
+          if (whole && ll == 0.0f) w = 0.0f;
+          float* po = reinterpret_cast<float*>(p.part_o) + slot * R * D;
+          auto put = [&](int r, int q4, float4 a) {          // four dims of a row
+            if (!whole) {
+              *(reinterpret_cast<float4*>(po + r * D) + q4) = a;
+            } else if (r0 + r < p.rows) {
+              *(reinterpret_cast<uint2*>(reinterpret_cast<uint16_t*>(p.o) + paged_row(p, at.b, at.g, r0 + r) * D) + q4) =
+                  make_uint2(pat_pack<BF>(a.x, a.y), pat_pack<BF>(a.z, a.w));
+            }
+          };
+#pragma unroll 1
+          for (int h = 0; h < D / 64; ++h) {
+#pragma unroll
+            for (int c = 0; c < 4; ++c) {
+              float x[16];
+              tmem_ld16(o_col + t_lane + h * 64 + c * 16, x);
+              tmem_wait_ld();
+#pragma unroll
+              for (int e = 0; e < 4; ++e) {
+                const int q4 = c * 4 + e;
+                // nothing was added where the weight is 0 (0 x NaN of another row's keys cannot be: those left)
+                const float4 a = make_float4(x[4 * e] * w, x[4 * e + 1] * w, x[4 * e + 2] * w, x[4 * e + 3] * w);
+                if constexpr (F == 1)
+                  put(row, h * 16 + q4, a);
+                else
+                  *reinterpret_cast<float4*>(own_p + ptc_off(tid, q4)) = a;
+              }
+            }
+            if constexpr (F > 1) {
+              named_bar_sync(1, PTC_SOFTMAX);
+#pragma unroll
+              for (int k = 0; k < R * 16 / PTC_SOFTMAX; ++k) {
+                const int x = tid + k * PTC_SOFTMAX, r = x / 16, q4 = x % 16;
+                float4 a = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+#pragma unroll
+                for (int i = 0; i < F; ++i) {
+                  const float4 y = *reinterpret_cast<const float4*>(own_p + ptc_off(i * R + r, q4));
+                  a.x += y.x, a.y += y.y, a.z += y.z, a.w += y.w;
+                }
+                put(r, h * 16 + q4, a);
+              }
+              named_bar_sync(1, PTC_SOFTMAX);
+            }
+          }
+          if constexpr (F > 1) clear_p();
+          tc_fence_before();
+          if (!whole && tid == 0) {
+            const PagedCut range = s_range;
+            const int head = range.first(blockIdx.x) + n - at.unit, c0 = range.cta_of(head);
+            s_cut[part] = {at.b, at.g, r0, c0, range.cta_of(head + at.nu - 1) - c0 + 1};
+          }
+        }
+        at.next(p);
+      }
+      if (!ok && tid == 0) s_cut[0].parts = s_cut[1].parts = 0;
+    }
+  }
+  tc_fence_before();
+  __syncthreads();
+  if (warp == 8) {
+    tc_fence_after();
+    tmem_dealloc(tmem, 512);
+  }
+  if (!mine || s_cut[0].parts + s_cut[1].parts == 0) return;
+  // cut sequences (at most the range's first and last): the last of their CTAs to get here joins the parts
+  if (tid < 2) {
+    s_join[tid] = false;
+    if (s_cut[tid].parts > 0) {
+      __threadfence();
+      const int c0 = s_cut[tid].c0;
+      s_join[tid] = atomicAdd(p.arrived + c0, 1) == s_cut[tid].parts - 1;
+      if (s_join[tid]) p.arrived[c0] = 0;
+      __threadfence();
+    }
+  }
+  __syncthreads();
+  for (int k = 0; k < 2; ++k)
+    if (s_join[k]) ptc_join<D, R, BF>(p, s_cut[k], reinterpret_cast<float2*>(ring));
+}
+
+}  // namespace simsd

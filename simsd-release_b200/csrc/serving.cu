@@ -9,6 +9,7 @@
 
 #include "paged.cuh"
 #include "paged_attn.cuh"
+#include "paged_attn_tc.cuh"
 #include "simsd_b200.h"
 #include "spec_verify.cuh"
 
@@ -51,10 +52,10 @@ int cache_check(const void* k, const void* v, int64_t ld_page, int64_t ld_head, 
   return SIMSD_OK;
 }
 
-// What paged attention does with G L rows per KV head: the rows of a CTA (8, 16, 32
-// or 64; more go in tiles of 64), the grid, and the workspace: the arrival counters,
-// then two parts per CTA (the end of a sequence it started inside, the start of one
-// it leaves unfinished).
+// What paged attention does with G L rows per KV head: the rows of a CTA (up to 16
+// with mma.sync, 32, 64 or 128 with tcgen05; more go in tiles of 128), the grid, and
+// the workspace: the arrival counters, then two parts per CTA (the end of a sequence
+// it started inside, the start of one it leaves unfinished).
 struct PagedPlan {
   int nr, grid;
   size_t ml_at, bytes;
@@ -62,9 +63,9 @@ struct PagedPlan {
 PagedPlan paged_plan(int L, int G, int D) {
   PagedPlan p;
   const long long rows = (long long)L * G;
-  p.nr = rows <= 8 ? 8 : rows <= 16 ? 16 : rows <= 32 ? 32 : 64;
+  p.nr = rows <= 8 ? 8 : rows <= 16 ? 16 : rows <= 32 ? 32 : rows <= 64 ? 64 : 128;
   const int sms = simsd_device_sm_count();
-  p.grid = std::min((p.nr <= 16 ? 2 : 1) * (sms > 0 ? sms : 148), SIMSD_PAGED_COUNTER_BYTES / (int)sizeof(int));
+  p.grid = std::min((p.nr <= 16 ? PAT_CTAS_PER_SM : 1) * (sms > 0 ? sms : 148), SIMSD_PAGED_COUNTER_BYTES / (int)sizeof(int));
   p.ml_at = SIMSD_PAGED_COUNTER_BYTES + align256((size_t)2 * p.grid * D * p.nr * sizeof(float));
   p.bytes = p.ml_at + align256((size_t)2 * p.grid * p.nr * sizeof(float2));
   return p;
@@ -133,21 +134,30 @@ int append(const PagedAppendArgs& a, void* stream) {
   return launch_on(paged_append_kernel<D, BF>, dim3((unsigned)grid), PA_THREADS, (size_t)smem, stream, false, a);
 }
 
-template <int D, int NT, int RG, bool BF>
+template <int D, int NT, bool BF>
 int attend(const PagedAttnArgs& a, const PagedPlan& pl, void* stream) {
   static bool done[kMaxDev];
-  using S = PatShape<D, NT, RG>;
-  const int rc = allow_smem(paged_attention_kernel<D, NT, RG, BF>, S::BYTES, done);
+  constexpr int smem = PatShape<D, NT>::BYTES;
+  const int rc = allow_smem(paged_attention_kernel<D, NT, BF>, smem, done);
   if (rc != SIMSD_OK) return rc;
-  return launch_on(paged_attention_kernel<D, NT, RG, BF>, dim3((unsigned)pl.grid), S::THREADS, S::BYTES, stream, false, a);
+  return launch_on(paged_attention_kernel<D, NT, BF>, dim3((unsigned)pl.grid), PAT_THREADS, smem, stream, false, a);
+}
+template <int D, int R, bool BF>
+int attend_tc(const PagedAttnArgs& a, const PagedPlan& pl, void* stream) {
+  static bool done[kMaxDev];
+  constexpr int smem = PtcShape<D, R>::BYTES;
+  const int rc = allow_smem(paged_attention_tc_kernel<D, R, BF>, smem, done);
+  if (rc != SIMSD_OK) return rc;
+  return launch_on(paged_attention_tc_kernel<D, R, BF>, dim3((unsigned)pl.grid), PTC_THREADS, smem, stream, false, a);
 }
 template <int D, bool BF>
 int attend_rows(const PagedAttnArgs& a, const PagedPlan& pl, void* stream) {
   switch (pl.nr) {
-    case 8: return attend<D, 1, 1, BF>(a, pl, stream);
-    case 16: return attend<D, 2, 1, BF>(a, pl, stream);
-    case 32: return attend<D, 2, 2, BF>(a, pl, stream);
-    default: return attend<D, 2, 4, BF>(a, pl, stream);
+    case 8: return attend<D, 1, BF>(a, pl, stream);
+    case 16: return attend<D, 2, BF>(a, pl, stream);
+    case 32: return attend_tc<D, 32, BF>(a, pl, stream);
+    case 64: return attend_tc<D, 64, BF>(a, pl, stream);
+    default: return attend_tc<D, 128, BF>(a, pl, stream);
   }
 }
 
@@ -255,7 +265,7 @@ int simsd_paged_attention(const void* q, const void* k_cache, const void* v_cach
   const PagedPlan pl = paged_plan(L, a.G, head_dim);
   a.rows = a.G * L;
   a.row_tiles = (a.rows + pl.nr - 1) / pl.nr;
-  if ((long long)B * Hk * a.row_tiles * ((int64_t)max_pages * page_size / 48 + 1) > 0x7fffffffLL)
+  if ((long long)B * Hk * a.row_tiles * ((int64_t)max_pages * page_size / PAT_TK + 1) > 0x7fffffffLL)
     return SIMSD_ERR_UNSUPPORTED;
   uint8_t* ws = reinterpret_cast<uint8_t*>(workspace);
   a.arrived = reinterpret_cast<int*>(ws);
