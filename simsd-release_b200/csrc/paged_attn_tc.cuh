@@ -17,11 +17,13 @@
 // maximum moves only when a score passes it by more than 2^8 (P <= 256 keeps its
 // relative precision in 16 bits), so O is hardly ever rescaled in TMEM.
 //
-// Warps 0-3 softmax and epilogue, 4-7 loads (cp.async into the 128-byte-swizzled
-// operand layout, any page size and stride, a ring of NS operand tiles K, V, K, V,
-// ...; a tile is handed over once its copies have landed and are visible to the
-// tensor cores), 8 issues the products: S of unit n + 1 before O of unit n, so that
-// they overlap its softmax.  One CTA per SM.
+// Warps 0-3 softmax and epilogue, 4-7 loads into a ring of NS operand tiles K, V, K,
+// V, ..., 8 issues the products: S of unit n + 1 before O of unit n, so that they
+// overlap its softmax.  One CTA per SM.  Pages of a multiple of 8 tokens are loaded
+// with TMA, a lane per run of `block` tokens that lies in one page (warp 4; warps
+// 5-7 then only fetch queries); other pages with cp.async into the same swizzled
+// layout, where handing a tile to the tensor cores waits for the copies behind it
+// too, about half the rate.
 //
 // A value that is not finite, of a key that some rows do not see, is taken out of the
 // product and added to the rows that see it by themselves.  All waits are bounded.
@@ -68,6 +70,21 @@ __device__ __forceinline__ uint32_t ptc_off(int r, int c) {
   return (uint32_t)((c >> 3) * 16384 + r * 128 + (((c ^ r) & 7) << 4));
 }
 
+struct PtcArgs {
+  PagedAttnArgs a;
+  CUtensorMap k, v;        // [pages, Hk, page size, D], box {64 dims, block tokens, 1, 1}; where block > 0
+  int block;               // tokens of a TMA load: the largest power of two <= 128 in the page size, or 0
+};
+
+__device__ __forceinline__ void ptc_tma(uint32_t dst, const void* map, uint32_t bar, int x, int tok, int head, int page,
+                                        uint64_t policy) {
+  asm volatile(
+      "cp.async.bulk.tensor.4d.shared::cluster.global.mbarrier::complete_tx::bytes.L2::cache_hint"
+      " [%0], [%1, {%3, %4, %5, %6}], [%2], %7;" ::"r"(dst),
+      "l"(reinterpret_cast<uint64_t>(map)), "r"(bar), "r"(x), "r"(tok), "r"(head), "r"(page), "l"(policy)
+      : "memory");
+}
+
 // Joins the parts of a cut sequence (rows r0 .. r0 + R - 1 of KV head g), as
 // paged_join; parts hold R rows of D.  `buf`: parts * R float2 of shared memory.
 template <int D, int R, bool BF>
@@ -76,39 +93,54 @@ __device__ void ptc_join(const PagedAttnArgs& p, const PagedPart& x, float2* buf
   auto slot = [&](int i) { return (long long)(i == 0 ? 2 * x.c0 + 1 : 2 * (x.c0 + i)); };
   for (int k = tid; k < x.parts * R; k += PTC_THREADS) buf[k] = __ldcg(p.part_ml + slot(k / R) * R + k % R);
   __syncthreads();
-  if (tid < R) {
+  // (maximum, 1 / sum) of a row from its parts, in order
+  auto law = [&](int r, bool lse) {
     float mm = -INFINITY, ll = 0.0f;
-    for (int i = 0; i < x.parts; ++i) mm = fmaxf(mm, buf[i * R + tid].x);
+    for (int i = 0; i < x.parts; ++i) mm = fmaxf(mm, buf[i * R + r].x);
     const float mu = mm == -INFINITY ? 0.0f : mm;
-    for (int i = 0; i < x.parts; ++i) {
-      const float w = pat_exp2(buf[i * R + tid].x - mu);
-      ll = fmaf(buf[i * R + tid].y, w, ll);
-      buf[i * R + tid].x = w;
-    }
-    const float inv = ll == 0.0f ? 0.0f : 1.0f / ll;
-    for (int i = 0; i < x.parts; ++i) buf[i * R + tid].x *= inv;
-    paged_store_lse(p, x.b, x.g, x.r0 + tid, mm, ll);
-  }
-  __syncthreads();
+    for (int i = 0; i < x.parts; ++i) ll = fmaf(buf[i * R + r].y, pat_exp2(buf[i * R + r].x - mu), ll);
+    if (lse) paged_store_lse(p, x.b, x.g, x.r0 + r, mm, ll);
+    return make_float2(mu, ll == 0.0f ? 0.0f : 1.0f / ll);
+  };
   const float* po = reinterpret_cast<const float*>(p.part_o);
-  for (int k = tid; k < R * (D / 4); k += PTC_THREADS) {
-    const int r = k / (D / 4), c = k % (D / 4);
-    if (x.r0 + r >= p.rows) break;
-    float4 a = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-#pragma unroll 4
-    for (int i = 0; i < x.parts; ++i) {
-      const float4 v = __ldcg(reinterpret_cast<const float4*>(po + (slot(i) * R + r) * D) + c);
-      const float w = buf[i * R + r].x;
-      a.x = fmaf(v.x, w, a.x), a.y = fmaf(v.y, w, a.y), a.z = fmaf(v.z, w, a.z), a.w = fmaf(v.w, w, a.w);
+  // four dims of IT rows a thread at a time, so that several parts of each are on their way
+  constexpr int IT = 4, ALL = R * (D / 4), C4 = D / 4;
+  for (int k0 = 0; k0 < ALL; k0 += IT * PTC_THREADS) {
+    float4 a[IT];
+    float2 lw[IT];
+    int r[IT], c[IT];
+#pragma unroll
+    for (int u = 0; u < IT; ++u) {
+      const int k = k0 + u * PTC_THREADS + tid;
+      r[u] = min(k / C4, R - 1), c[u] = k % C4;
+      a[u] = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+      lw[u] = law(r[u], k < ALL && c[u] == 0);
     }
-    uint2* dst = reinterpret_cast<uint2*>(reinterpret_cast<uint16_t*>(p.o) + paged_row(p, x.b, x.g, x.r0 + r) * D) + c;
-    *dst = make_uint2(pat_pack<BF>(a.x, a.y), pat_pack<BF>(a.z, a.w));
+#pragma unroll 2
+    for (int i = 0; i < x.parts; ++i) {
+      const float* from = po + slot(i) * R * D;
+      float4 v[IT];
+#pragma unroll
+      for (int u = 0; u < IT; ++u) v[u] = __ldcg(reinterpret_cast<const float4*>(from + r[u] * D) + c[u]);
+#pragma unroll
+      for (int u = 0; u < IT; ++u) {
+        const float w = pat_exp2(buf[i * R + r[u]].x - lw[u].x) * lw[u].y;
+        a[u].x = fmaf(v[u].x, w, a[u].x), a[u].y = fmaf(v[u].y, w, a[u].y);
+        a[u].z = fmaf(v[u].z, w, a[u].z), a[u].w = fmaf(v[u].w, w, a[u].w);
+      }
+    }
+#pragma unroll
+    for (int u = 0; u < IT; ++u)
+      if (k0 + u * PTC_THREADS + tid < ALL && x.r0 + r[u] < p.rows)
+        *(reinterpret_cast<uint2*>(reinterpret_cast<uint16_t*>(p.o) + paged_row(p, x.b, x.g, x.r0 + r[u]) * D) + c[u]) =
+            make_uint2(pat_pack<BF>(a[u].x, a[u].y), pat_pack<BF>(a[u].z, a[u].w));
   }
   __syncthreads();
 }
 
 template <int D, int R, bool BF>
-__global__ void __launch_bounds__(PTC_THREADS, 1) paged_attention_tc_kernel(const __grid_constant__ PagedAttnArgs p) {
+__global__ void __launch_bounds__(PTC_THREADS, 1) paged_attention_tc_kernel(const __grid_constant__ PtcArgs args) {
+  const PagedAttnArgs& p = args.a;
   using S = PtcShape<D, R>;
   constexpr int F = S::F, NS = S::NS, CH = D / 8, KPI = 32 / CH;
   extern __shared__ uint8_t ptc_raw[];
@@ -129,8 +161,8 @@ __global__ void __launch_bounds__(PTC_THREADS, 1) paged_attention_tc_kernel(cons
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
 
   if (tid == 0) {
-    for (int s = 0; s < NS; ++s) mbar_init(smem_u32(full + s), 128), mbar_init(smem_u32(empty + s), 1);
-    mbar_init(smem_u32(q_full), 128);
+    for (int s = 0; s < NS; ++s) mbar_init(smem_u32(full + s), args.block ? 1 : 128), mbar_init(smem_u32(empty + s), 1);
+    mbar_init(smem_u32(q_full), args.block ? 96 : 128);
     mbar_init(smem_u32(q_empty), 1);
     mbar_init(smem_u32(s_full), 1);
     mbar_init(smem_u32(s_full + 1), 1);
@@ -158,8 +190,72 @@ __global__ void __launch_bounds__(PTC_THREADS, 1) paged_attention_tc_kernel(cons
   if (mine) {
     const int steps = cut.first(blockIdx.x + 1) - cut.first(blockIdx.x);
     if (tid == 0) s_range = cut;
-    if (warp >= 4 && warp < 8) {
-      // ================= loads
+    if (args.block && warp == 4) {
+      // ================= loads of keys and values by TMA: a lane per `block` tokens of the unit
+      uint32_t slot = 0, phase = 0;
+      const int runs = PTC_TK / args.block, first_key = lane * args.block;
+      const uint64_t policy = policy_evict_first();
+      if (lane == 0) prefetch_tmap(&args.k), prefetch_tmap(&args.v);
+      // the page of the lane's run; one past the last (which loads zeros) where it holds no key
+      auto run_page = [&](const PagedPos<PTC_TK>& x) {
+        const int key = x.unit * PTC_TK + first_key;
+        return lane < runs && key < x.n ? p.page_table[x.b * p.ld_table + p.page_div(key)] : p.num_pages;
+      };
+      int page = run_page(at);
+      uint32_t filled = 0, parity = 0;           // tiles with a load in flight, and its phase
+      bool ok = true;
+      for (int n = 0; n < steps && ok; ++n) {
+        if (page < 0 || page > p.num_pages || (page == p.num_pages && lane < runs && at.unit * PTC_TK + first_key < at.n)) {
+          if (p.err) atomicOr(p.err, SIMSD_DEV_ERR_BAD_INDEX);
+          page = p.num_pages;
+        }
+        const int now = page, head = at.g, key = at.unit * PTC_TK + first_key, tok = key - p.page_div(key) * p.page_size;
+        if (n + 1 < steps) {
+          at.next(p);
+          page = run_page(at);
+        }
+        for (int kv = 0; kv < 2; ++kv) {
+          ok = __all_sync(0xffffffffu, mbar_wait(smem_u32(empty + slot), phase ^ 1, abort_flag, p.err));
+          if (!ok) break;
+          const uint32_t bar = smem_u32(full + slot), dst = smem_u32(ring) + slot * S::TILE + first_key * 128;
+          if (lane == 0) mbar_arrive_expect_tx(bar, S::TILE);
+          __syncwarp();
+          if (lane < runs) {
+            const void* map = kv ? &args.v : &args.k;
+#pragma unroll
+            for (int x = 0; x < D / 64; ++x) ptc_tma(dst + x * 16384, map, bar, x * 64, tok, head, now, policy);
+          }
+          filled |= 1u << slot;
+          parity = (parity & ~(1u << slot)) | (phase << slot);
+          if (++slot == NS) slot = 0, phase ^= 1;
+        }
+      }
+      if (!ok && lane == 0)                      // giving up: no copy may land after the CTA has left
+        for (int s = 0; s < NS; ++s)
+          if (filled >> s & 1) mbar_wait_drain(smem_u32(full + s), parity >> s & 1, 100000000ull);
+      __syncwarp();
+    } else if (args.block && warp >= 5 && warp < 8) {
+      // ================= queries, for the TMA loads
+      uint32_t items = 0;
+      for (int n = 0; n < steps; ++n) {
+        if (n == 0 || at.unit == 0) {
+          if (!__all_sync(0xffffffffu, mbar_wait(smem_u32(q_empty), (items & 1) ^ 1, abort_flag, p.err))) break;
+          ++items;
+          for (int x = tid - 160; x < 128 * CH; x += 96) {
+            const int row = x / CH, r = at.rt * R + row % R;
+            const bool in = r < p.rows;
+            pat_cp16(smem_u32(Qs) + ptc_off(row, x % CH),
+                     reinterpret_cast<const uint16_t*>(p.q) + (in ? paged_row(p, at.b, at.g, r) * D + x % CH * 8 : 0), in);
+          }
+          pat_commit();
+          pat_wait<0>();
+          fence_proxy_async_smem();
+          mbar_arrive(smem_u32(q_full));
+        }
+        at.next(p);
+      }
+    } else if (warp >= 4 && warp < 8) {
+      // ================= loads by cp.async
       const int lt = tid - 128, lw = warp - 4, kc = lane % CH, khi = lane / CH;
       uint32_t slot = 0, phase = 0, items = 0;
       // groups of copies that have been issued and not handed over, oldest first
@@ -201,6 +297,10 @@ __global__ void __launch_bounds__(PTC_THREADS, 1) paged_attention_tc_kernel(cons
         return key < x.n ? p.page_table[x.b * p.ld_table + p.page_div(key)] : -1;
       };
       int page = key_page(at);
+      // Pages of a multiple of 16 tokens: the warp's keys 0 - 15 and 16 - 31 each lie a
+      // fixed distance apart; otherwise each key's place is handed round.
+      const bool page16 = p.page_size % 16 == 0;
+      const uint32_t lane_dst = ptc_off(lw * 32 + khi, kc);
       for (int n = 0; n < steps; ++n) {
         const int key = at.unit * PTC_TK + lt;
         long long off = -1;
@@ -215,13 +315,34 @@ __global__ void __launch_bounds__(PTC_THREADS, 1) paged_attention_tc_kernel(cons
           at.next(p);
           page = key_page(at);
         }
-        auto copy = [&](const void* src) {
-          const uint32_t dst = smem_u32(ring) + slot * S::TILE;
+        long long half[2];                       // keys khi and 16 + khi of the warp, chunk kc
+        int live[2];                             // keys of that half that exist, from khi on
 #pragma unroll
-          for (int i = 0; i < 32 / KPI; ++i) {
-            const long long o = __shfl_sync(0xffffffffu, off, i * KPI + khi);
-            pat_cp16(dst + ptc_off(lw * 32 + i * KPI + khi, kc),
-                     reinterpret_cast<const uint16_t*>(src) + (o < 0 ? 0 : o + kc * 8), o >= 0);
+        for (int h = 0; h < 2; ++h) {
+          const long long o = __shfl_sync(0xffffffffu, off, 16 * h);
+          half[h] = o < 0 ? 0 : o + khi * p.ld_tok + kc * 8;
+          live[h] = o < 0 ? 0 : cur.n - (cur.unit * PTC_TK + lw * 32 + 16 * h) - khi;
+        }
+        auto copy = [&](const void* src) {
+          const uint32_t dst = smem_u32(ring) + slot * S::TILE + lane_dst;
+          const uint16_t* from = reinterpret_cast<const uint16_t*>(src);
+          if (page16) {
+#pragma unroll
+            for (int h = 0; h < 2; ++h) {
+              const uint16_t* k = from + half[h];
+#pragma unroll
+              for (int i = 0; i < 16 / KPI; ++i) {
+                const bool ok = live[h] > i * KPI;
+                pat_cp16((dst ^ ((i * KPI & 7) << 4)) + (16 * h + i * KPI) * 128, ok ? k : from, ok);
+                k += KPI * p.ld_tok;
+              }
+            }
+          } else {
+#pragma unroll
+            for (int i = 0; i < 32 / KPI; ++i) {
+              const long long o = __shfl_sync(0xffffffffu, off, i * KPI + khi);
+              pat_cp16((dst ^ ((i * KPI & 7) << 4)) + i * KPI * 128, from + (o < 0 ? 0 : o + kc * 8), o >= 0);
+            }
           }
           issued(smem_u32(full + slot));
           if (++slot == NS) slot = 0, phase ^= 1;
@@ -320,12 +441,8 @@ __global__ void __launch_bounds__(PTC_THREADS, 1) paged_attention_tc_kernel(cons
         tc_fence_after();
         float v[R];
 #pragma unroll
-        for (int c = 0; c < R / 16; ++c) {
-          float x[16];
-          tmem_ld16(tmem + t_lane + (n & 1) * 128 + f * R + c * 16, x);
-#pragma unroll
-          for (int e = 0; e < 16; ++e) v[c * 16 + e] = x[e];
-        }
+        for (int c = 0; c < R / 16; ++c)
+          tmem_ld16(tmem + t_lane + (n & 1) * 128 + f * R + c * 16, *reinterpret_cast<float(*)[16]>(v + c * 16));
         tmem_wait_ld();
         if (p.q_sign) {
 #pragma unroll
@@ -353,53 +470,39 @@ __global__ void __launch_bounds__(PTC_THREADS, 1) paged_attention_tc_kernel(cons
 #pragma unroll
           for (int c = 0; c < R; ++c)
             if (!(see[c / 32] >> (c % 32) & 1)) v[c] = -INFINITY;
-          if (p.L > 1 || p.tail) {
-            // keys that some row may not see: values that are not finite leave the product
-            if (!(ok = wait_all(full + vs, vph))) break;
-            bool odd = false;
-            uint8_t* vt = ring + vs * S::TILE;
-            if (k0 + tid >= base && k0 + tid < at.n) {
-              constexpr uint32_t EXP = BF ? 0x7f80u : 0x7c00u;
-              for (int c = 0; c < CH; ++c) {
-                const uint4 u = *reinterpret_cast<const uint4*>(vt + ptc_off(tid, c));
-                const uint32_t w[4] = {u.x, u.y, u.z, u.w};
+          // Values past the sequence's end are whatever the page holds: zero.  Of keys that
+          // some row may not see, values that are not finite leave the product.
+          if (!(ok = wait_all(full + vs, vph))) break;
+          uint8_t* vt = ring + vs * S::TILE;
+          bool odd = false;
+          if (k0 + tid >= base && k0 + tid < at.n) {
+            constexpr uint32_t EXP = BF ? 0x7f80u : 0x7c00u;
 #pragma unroll
-                for (int k = 0; k < 4; ++k) odd |= (w[k] & EXP) == EXP || ((w[k] >> 16) & EXP) == EXP;
-              }
-              if (odd)
-                for (int c = 0; c < CH; ++c) *reinterpret_cast<uint4*>(vt + ptc_off(tid, c)) = make_uint4(0, 0, 0, 0);
+            for (int c = 0; c < CH; ++c) {
+              const uint4 u = *reinterpret_cast<const uint4*>(vt + ptc_off(tid, c));
+              const uint32_t w[4] = {u.x, u.y, u.z, u.w};
+#pragma unroll
+              for (int k = 0; k < 4; ++k) odd |= (w[k] & EXP) == EXP || ((w[k] >> 16) & EXP) == EXP;
             }
-            const uint32_t b = __ballot_sync(0xffffffffu, odd);
-            if (lane == 0) bad[warp] = b;
-            named_bar_sync(1, PTC_SOFTMAX);
-            strange = (bad[0] | bad[1] | bad[2] | bad[3]) != 0;
           }
+          if (odd || k0 + tid >= at.n) {
+#pragma unroll
+            for (int c = 0; c < CH; ++c) *reinterpret_cast<uint4*>(vt + ptc_off(tid, c)) = make_uint4(0, 0, 0, 0);
+          }
+          const uint32_t b = __ballot_sync(0xffffffffu, odd);
+          if (lane == 0) bad[warp] = b;
+          named_bar_sync(1, PTC_SOFTMAX);
+          strange = (bad[0] | bad[1] | bad[2] | bad[3]) != 0;
         }
         float m4[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
 #pragma unroll
         for (int c = 0; c < R; ++c) m4[c & 3] = fmaxf(m4[c & 3], v[c]);
         const float mx = fmaxf(fmaxf(m4[0], m4[1]), fmaxf(m4[2], m4[3]));
-        // O of the units before has been summed, P may be written
-        if (n > 0 && !(ok = wait_all(pv_done, (n - 1) & 1))) break;
         const bool up = m == -INFINITY ? mx > m : (mx - m) * p.scale_log2 > 8.0f;
-        if (__any_sync(0xffffffffu, up)) {
-          const float to = up ? mx : m;
-          const float w = !up ? 1.0f : m == -INFINITY ? 0.0f : pat_exp2((m - to) * p.scale_log2);
-          m = to;
-          l *= w;
-          if (n > 0 && at.unit > first_unit) {
-            tc_fence_after();
-#pragma unroll 1
-            for (int c = 0; c < D / 16; ++c) {
-              float x[16];
-              tmem_ld16(o_col + t_lane + c * 16, x);
-              tmem_wait_ld();
-#pragma unroll
-              for (int e = 0; e < 16; ++e) x[e] *= w;
-              ptc_st16(o_col + t_lane + c * 16, x);
-            }
-            ptc_wait_st();
-          }
+        float w_old = 1.0f;                      // what the sums so far are scaled by
+        if (up) {
+          w_old = m == -INFINITY ? 0.0f : pat_exp2((m - mx) * p.scale_log2);
+          m = mx;
         }
         const float ms = m == -INFINITY ? 0.0f : m * p.scale_log2;
         float l4[4] = {0.0f, 0.0f, 0.0f, 0.0f};
@@ -408,7 +511,22 @@ __global__ void __launch_bounds__(PTC_THREADS, 1) paged_attention_tc_kernel(cons
           v[c] = pat_exp2(fmaf(v[c], p.scale_log2, -ms));
           l4[c & 3] += v[c];
         }
-        l += (l4[0] + l4[1]) + (l4[2] + l4[3]);
+        l = fmaf(l, w_old, (l4[0] + l4[1]) + (l4[2] + l4[3]));
+        // O of the units before has been summed, P may be written
+        if (n > 0 && !(ok = wait_all(pv_done, (n - 1) & 1))) break;
+        if (n > 0 && at.unit > first_unit && __any_sync(0xffffffffu, up)) {
+          tc_fence_after();
+#pragma unroll 1
+          for (int c = 0; c < D / 16; ++c) {
+            float x[16];
+            tmem_ld16(o_col + t_lane + c * 16, x);
+            tmem_wait_ld();
+#pragma unroll
+            for (int e = 0; e < 16; ++e) x[e] *= w_old;
+            ptc_st16(o_col + t_lane + c * 16, x);
+          }
+          ptc_wait_st();
+        }
 #pragma unroll
         for (int c = 0; c < R / 8; ++c)
           *reinterpret_cast<uint4*>(own_p + ptc_off(tid, f * (R / 8) + c)) =
@@ -490,16 +608,16 @@ __global__ void __launch_bounds__(PTC_THREADS, 1) paged_attention_tc_kernel(cons
           };
 #pragma unroll 1
           for (int h = 0; h < D / 64; ++h) {
+            float x[4][16];
+#pragma unroll
+            for (int c = 0; c < 4; ++c) tmem_ld16(o_col + t_lane + h * 64 + c * 16, x[c]);
+            tmem_wait_ld();
 #pragma unroll
             for (int c = 0; c < 4; ++c) {
-              float x[16];
-              tmem_ld16(o_col + t_lane + h * 64 + c * 16, x);
-              tmem_wait_ld();
 #pragma unroll
               for (int e = 0; e < 4; ++e) {
                 const int q4 = c * 4 + e;
-                // nothing was added where the weight is 0 (0 x NaN of another row's keys cannot be: those left)
-                const float4 a = make_float4(x[4 * e] * w, x[4 * e + 1] * w, x[4 * e + 2] * w, x[4 * e + 3] * w);
+                const float4 a = make_float4(x[c][4 * e] * w, x[c][4 * e + 1] * w, x[c][4 * e + 2] * w, x[c][4 * e + 3] * w);
                 if constexpr (F == 1)
                   put(row, h * 16 + q4, a);
                 else

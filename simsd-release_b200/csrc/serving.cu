@@ -1,6 +1,9 @@
 // extern "C" entry points of the batched serving operators (declared in
 // include/simsd_b200.h): the paged key-value cache and draft verification.
+#include <cudaTypedefs.h>
 #include <cuda_runtime.h>
+
+#include <cstring>
 
 #include <algorithm>
 #include <cmath>
@@ -142,13 +145,42 @@ int attend(const PagedAttnArgs& a, const PagedPlan& pl, void* stream) {
   if (rc != SIMSD_OK) return rc;
   return launch_on(paged_attention_kernel<D, NT, BF>, dim3((unsigned)pl.grid), PAT_THREADS, smem, stream, false, a);
 }
+// A TMA map of a cache for loads of `block` tokens of one page and head; false where
+// the driver will not describe it (a stride of 0, say).
+bool cache_map(CUtensorMap* m, const void* base, const PagedAttnArgs& a, int D, int block, bool bf) {
+  static const PFN_cuTensorMapEncodeTiled_v12000 encode = [] {
+    void* fn = nullptr;
+    cudaDriverEntryPointQueryResult q;
+    if (cudaGetDriverEntryPointByVersion("cuTensorMapEncodeTiled", &fn, 12000, cudaEnableDefault, &q) != cudaSuccess ||
+        q != cudaDriverEntryPointSuccess) {
+      (void)cudaGetLastError();
+      fn = nullptr;
+    }
+    return reinterpret_cast<PFN_cuTensorMapEncodeTiled_v12000>(fn);
+  }();
+  if (encode == nullptr) return false;
+  const cuuint64_t dims[4] = {(cuuint64_t)D, (cuuint64_t)a.page_size, (cuuint64_t)a.Hk, (cuuint64_t)a.num_pages};
+  const cuuint64_t strides[3] = {(cuuint64_t)a.ld_tok * 2, (cuuint64_t)a.ld_head * 2, (cuuint64_t)a.ld_page * 2};
+  const cuuint32_t box[4] = {64, (cuuint32_t)block, 1, 1}, step[4] = {1, 1, 1, 1};
+  if (a.ld_tok <= 0 || a.ld_head <= 0 || a.ld_page <= 0) return false;
+  return encode(m, bf ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16, 4, const_cast<void*>(base), dims,
+                strides, box, step, CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B,
+                CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+}
+
 template <int D, int R, bool BF>
 int attend_tc(const PagedAttnArgs& a, const PagedPlan& pl, void* stream) {
   static bool done[kMaxDev];
   constexpr int smem = PtcShape<D, R>::BYTES;
   const int rc = allow_smem(paged_attention_tc_kernel<D, R, BF>, smem, done);
   if (rc != SIMSD_OK) return rc;
-  return launch_on(paged_attention_tc_kernel<D, R, BF>, dim3((unsigned)pl.grid), PTC_THREADS, smem, stream, false, a);
+  PtcArgs t;
+  std::memset(&t, 0, sizeof(t));
+  t.a = a;
+  t.block = std::min(a.page_size & -a.page_size, PTC_TK);
+  if (t.block < 8 || !cache_map(&t.k, a.k_cache, a, D, t.block, BF) || !cache_map(&t.v, a.v_cache, a, D, t.block, BF))
+    t.block = 0;
+  return launch_on(paged_attention_tc_kernel<D, R, BF>, dim3((unsigned)pl.grid), PTC_THREADS, smem, stream, false, t);
 }
 template <int D, bool BF>
 int attend_rows(const PagedAttnArgs& a, const PagedPlan& pl, void* stream) {

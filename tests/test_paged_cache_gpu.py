@@ -179,6 +179,11 @@ ATT = [
     ([64, 200, 1500], 8, 32, 8, 128, 16, "nhd", BF, "each"), ([90, 130], 5, 40, 8, 128, 32, "hnd", FP, "one"),
     ([300, 37, 16], 16, 16, 2, 64, 24, "both", BF, "each"), ([777, 12], 3, 12, 1, 64, 8, "nhd", FP, "each"),
     ([513, 40], 40, 8, 8, 128, 16, "hnd", BF, "one"), ([257, 31], 33, 6, 2, 64, 16, "hnd", BF, None),
+    # 17 to 128 rows and more, pages of other than 8 tokens among them
+    ([200, 65, 5, 0], 8, 16, 2, 128, 7, "hnd", BF, "each"), ([130, 300], 6, 32, 8, 64, 1, "nhd", FP, None),
+    ([1000, 129, 128, 127], 32, 32, 8, 128, 16, "hnd", BF, "each"), ([2500, 12], 20, 20, 4, 128, 40, "both", FP, "one"),
+    ([260, 3], 70, 2, 1, 128, 64, "nhd", BF, "one"), ([6000], 4, 32, 4, 128, 128, "hnd", BF, None),
+    ([9000, 8000], 17, 8, 2, 64, 8, "nhd", BF, None), ([640] * 9, 1, 24, 1, 128, 16, "hnd", BF, None),
     ([10] * 200, 1, 8, 4, 64, 16, "hnd", BF, None), ([0] * 5, 2, 4, 2, 128, 16, "hnd", BF, None),
 ]
 
