@@ -11,19 +11,20 @@
 //   S = Q K^T       [128 x 128 keys], TMEM; a thread per TMEM lane reads its R keys
 //   softmax         per lane (a row's copy is a softmax of its own, joined at the end):
 //                   no exchange between threads, R exponentials each
-//   P               16-bit, in shared memory, zero outside a copy's own keys
+//   P               16-bit, in TMEM, zero outside a copy's own keys
 //   O += P V        [128 x D], TMEM, accumulated over the units of the sequence
-// so a unit's softmax is spread over all 128 lanes at 32 rows too.  The running
+// so a unit's softmax is spread over all 128 lanes at 32 rows too.  Q and P are read
+// from TMEM: with both operands in shared memory a product of 128 x 128 x 16 took 141
+// cycles, its 8 KB at about half of what shared memory delivers.  The running
 // maximum moves only when a score passes it by more than 2^8 (P <= 256 keeps its
 // relative precision in 16 bits), so O is hardly ever rescaled in TMEM.
 //
 // Warps 0-3 softmax and epilogue, 4-7 loads into a ring of NS operand tiles K, V, K,
 // V, ..., 8 issues the products: S of unit n + 1 before O of unit n, so that they
 // overlap its softmax.  One CTA per SM.  Pages of a multiple of 8 tokens are loaded
-// with TMA, a lane per run of `block` tokens that lies in one page (warp 4; warps
-// 5-7 then only fetch queries); other pages with cp.async into the same swizzled
-// layout, where handing a tile to the tensor cores waits for the copies behind it
-// too, about half the rate.
+// with TMA, a lane per run of `block` tokens that lies in one page (warp 4); other
+// pages with cp.async into the same swizzled layout (warps 4-7), where handing a tile
+// to the tensor cores waits for the copies behind it too, about half the rate.
 //
 // A value that is not finite, of a key that some rows do not see, is taken out of the
 // product and added to the rows that see it by themselves.  All waits are bounded.
@@ -37,12 +38,24 @@ constexpr int PTC_THREADS = 288, PTC_SOFTMAX = 128, PTC_TK = 128;
 template <int D, int R>
 struct PtcShape {
   static constexpr int F = 128 / R;
-  static constexpr int TILE = 128 * D * 2;              // 128 keys, values or rows of queries
-  static constexpr int NS = D == 128 ? 5 : 8;
-  static constexpr int P = 32768;
-  static constexpr int BYTES = 1024 + NS * TILE + TILE + P + 1024 + 512;
+  static constexpr int TILE = 128 * D * 2;              // 128 keys or values
+  static constexpr int NS = D == 128 ? 6 : 8;
+  static constexpr int X = 32768;                       // 64 dims of every lane's O, where copies are joined
+  static constexpr int BYTES = 1024 + NS * TILE + X + 1024 + 512;
+  // TMEM columns: S of even and odd units, O, then Q and P, two 16-bit values a column
+  static constexpr int O = 256, Q = O + D, P = Q + D / 2;
+  static_assert(P + 64 <= 512);
 };
 
+// D (+)= A B^T with A in TMEM (a lane per row, two 16-bit values a column)
+__device__ __forceinline__ void ptc_mma(uint32_t d, uint32_t a, uint64_t bdesc, uint32_t idesc, uint32_t accumulate) {
+  asm volatile(
+      "{\n\t.reg .pred p;\n\t"
+      "setp.ne.b32 p, %4, 0;\n\t"
+      "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t}" ::"r"(d),
+      "r"(a), "l"(bdesc), "r"(idesc), "r"(accumulate)
+      : "memory");
+}
 __device__ __forceinline__ void ptc_st16(uint32_t taddr, const float (&v)[16]) {
   asm volatile(
       "tcgen05.st.sync.aligned.32x32b.x16.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16};" ::"r"(taddr),
@@ -145,12 +158,11 @@ __global__ void __launch_bounds__(PTC_THREADS, 1) paged_attention_tc_kernel(cons
   constexpr int F = S::F, NS = S::NS, CH = D / 8, KPI = 32 / CH;
   extern __shared__ uint8_t ptc_raw[];
   uint8_t* ring = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(ptc_raw) + 1023) & ~uintptr_t(1023));
-  uint8_t* Qs = ring + NS * S::TILE;
-  uint8_t* Ps = Qs + S::TILE;
-  float* xm = reinterpret_cast<float*>(Ps + S::P);       // [128] maximum, then [128] sum of a lane
+  uint8_t* own_x = ring + NS * S::TILE;
+  float* xm = reinterpret_cast<float*>(own_x + S::X);    // [128] maximum, then [128] sum of a lane
   float* xl = xm + 128;
   uint64_t* bars = reinterpret_cast<uint64_t*>(xl + 128);
-  uint64_t *full = bars, *empty = bars + 8, *q_full = bars + 16, *q_empty = bars + 17, *s_full = bars + 18,
+  uint64_t *full = bars, *empty = bars + 8, *q_full = bars + 16, *s_full = bars + 18,
            *p_full = bars + 20, *pv_done = bars + 21, *drained = bars + 22;
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(bars + 23);
   volatile int* abort_flag = reinterpret_cast<int*>(bars + 23) + 1;
@@ -162,8 +174,7 @@ __global__ void __launch_bounds__(PTC_THREADS, 1) paged_attention_tc_kernel(cons
 
   if (tid == 0) {
     for (int s = 0; s < NS; ++s) mbar_init(smem_u32(full + s), args.block ? 1 : 128), mbar_init(smem_u32(empty + s), 1);
-    mbar_init(smem_u32(q_full), args.block ? 96 : 128);
-    mbar_init(smem_u32(q_empty), 1);
+    mbar_init(smem_u32(q_full), PTC_SOFTMAX);
     mbar_init(smem_u32(s_full), 1);
     mbar_init(smem_u32(s_full + 1), 1);
     mbar_init(smem_u32(p_full), PTC_SOFTMAX);
@@ -186,7 +197,7 @@ __global__ void __launch_bounds__(PTC_THREADS, 1) paged_attention_tc_kernel(cons
   const bool mine = paged_range<PTC_THREADS, PTC_TK>(p, cut, at);
   tc_fence_after();
   const uint32_t tmem = *tmem_slot;
-  const uint32_t o_col = tmem + 256;
+  const uint32_t o_col = tmem + S::O;
   if (mine) {
     const int steps = cut.first(blockIdx.x + 1) - cut.first(blockIdx.x);
     if (tid == 0) s_range = cut;
@@ -234,30 +245,12 @@ __global__ void __launch_bounds__(PTC_THREADS, 1) paged_attention_tc_kernel(cons
         for (int s = 0; s < NS; ++s)
           if (filled >> s & 1) mbar_wait_drain(smem_u32(full + s), parity >> s & 1, 100000000ull);
       __syncwarp();
-    } else if (args.block && warp >= 5 && warp < 8) {
-      // ================= queries, for the TMA loads
-      uint32_t items = 0;
-      for (int n = 0; n < steps; ++n) {
-        if (n == 0 || at.unit == 0) {
-          if (!__all_sync(0xffffffffu, mbar_wait(smem_u32(q_empty), (items & 1) ^ 1, abort_flag, p.err))) break;
-          ++items;
-          for (int x = tid - 160; x < 128 * CH; x += 96) {
-            const int row = x / CH, r = at.rt * R + row % R;
-            const bool in = r < p.rows;
-            pat_cp16(smem_u32(Qs) + ptc_off(row, x % CH),
-                     reinterpret_cast<const uint16_t*>(p.q) + (in ? paged_row(p, at.b, at.g, r) * D + x % CH * 8 : 0), in);
-          }
-          pat_commit();
-          pat_wait<0>();
-          fence_proxy_async_smem();
-          mbar_arrive(smem_u32(q_full));
-        }
-        at.next(p);
-      }
+    } else if (args.block && warp > 4 && warp < 8) {
+      // warps 5-7 load only where TMA does not
     } else if (warp >= 4 && warp < 8) {
       // ================= loads by cp.async
       const int lt = tid - 128, lw = warp - 4, kc = lane % CH, khi = lane / CH;
-      uint32_t slot = 0, phase = 0, items = 0;
+      uint32_t slot = 0, phase = 0;
       // groups of copies that have been issued and not handed over, oldest first
       uint32_t w0 = 0, w1 = 0, w2 = 0;
       int waiting = 0;
@@ -349,18 +342,6 @@ __global__ void __launch_bounds__(PTC_THREADS, 1) paged_attention_tc_kernel(cons
         };
         if (!wait_for(smem_u32(empty + slot), phase ^ 1)) break;
         copy(p.k_cache);
-        if (n == 0 || cur.unit == 0) {
-          // the queries of a new sequence, head or row tile, F times
-          if (!wait_for(smem_u32(q_empty), (items & 1) ^ 1)) break;
-          ++items;
-          for (int x = lt; x < 128 * CH; x += 128) {
-            const int row = x / CH, r = cur.rt * R + row % R;
-            const bool in = r < p.rows;
-            pat_cp16(smem_u32(Qs) + ptc_off(row, x % CH),
-                     reinterpret_cast<const uint16_t*>(p.q) + (in ? paged_row(p, cur.b, cur.g, r) * D + x % CH * 8 : 0), in);
-          }
-          issued(smem_u32(q_full));
-        }
         if (!wait_for(smem_u32(empty + slot), phase ^ 1)) break;
         copy(p.v_cache);
       }
@@ -372,43 +353,47 @@ __global__ void __launch_bounds__(PTC_THREADS, 1) paged_attention_tc_kernel(cons
         const uint32_t idesc_o = make_idesc_f16(BF, 128, D) | (1u << 16);   // V is MN-major
         uint32_t ks = 0, kph = 0, vs = 1, vph = 0, items = 0;
         bool ok = true, first = true, prev_first = true, any = false;
-        for (int n = 0; n <= steps && ok; ++n) {
-          if (n < steps) {
-            first = n == 0 || at.unit == 0;
-            if (first && !(ok = mbar_wait(smem_u32(q_full), items++ & 1, abort_flag, p.err))) break;
-            if (!(ok = mbar_wait(smem_u32(full + ks), kph, abort_flag, p.err))) break;
-            tc_fence_after();
-            const uint32_t kt = smem_u32(ring) + ks * S::TILE;
+        auto product_s = [&](int n) {
+          if (first && !mbar_wait(smem_u32(q_full), items++ & 1, abort_flag, p.err)) return false;
+          if (!mbar_wait(smem_u32(full + ks), kph, abort_flag, p.err)) return false;
+          tc_fence_after();
+          const uint32_t kt = smem_u32(ring) + ks * S::TILE;
 #pragma unroll
-            for (int kk = 0; kk < D / 16; ++kk) {
-              const uint32_t o = (kk >> 2) * 16384;
-              tc_mma_f16(tmem + (n & 1) * 128, make_sw128_desc(smem_u32(Qs) + o) + 2 * (kk & 3),
-                         make_sw128_desc(kt + o) + 2 * (kk & 3), idesc_s, kk > 0);
-            }
-            any = true;
-            tc_commit(smem_u32(s_full + (n & 1)));
-            tc_commit(smem_u32(empty + ks));
-            if (at.unit + 1 == at.nu) tc_commit(smem_u32(q_empty));
-            ks += 2;
-            if (ks >= NS) ks -= NS, kph ^= 1;
-            at.next(p);
-          }
-          if (n > 0) {
-            if (!(ok = mbar_wait(smem_u32(p_full), (n - 1) & 1, abort_flag, p.err))) break;
-            if (!(ok = mbar_wait(smem_u32(full + vs), vph, abort_flag, p.err))) break;
-            tc_fence_after();
-            const uint32_t vt = smem_u32(ring) + vs * S::TILE;
+          for (int kk = 0; kk < D / 16; ++kk)
+            ptc_mma(tmem + (n & 1) * 128, tmem + S::Q + kk * 8, make_sw128_desc(kt + (kk >> 2) * 16384) + 2 * (kk & 3), idesc_s,
+                    kk > 0);
+          any = true;
+          tc_commit(smem_u32(s_full + (n & 1)));
+          tc_commit(smem_u32(empty + ks));
+          ks += 2;
+          if (ks >= NS) ks -= NS, kph ^= 1;
+          return true;
+        };
+        auto product_o = [&](int n, bool start) {
+          if (!mbar_wait(smem_u32(p_full), n & 1, abort_flag, p.err)) return false;
+          if (!mbar_wait(smem_u32(full + vs), vph, abort_flag, p.err)) return false;
+          tc_fence_after();
+          const uint32_t vt = smem_u32(ring) + vs * S::TILE;
 #pragma unroll
-            for (int kk = 0; kk < 8; ++kk)
-              tc_mma_f16(o_col, make_sw128_desc(smem_u32(Ps) + (kk >> 2) * 16384) + 2 * (kk & 3), ptc_desc_mn(vt + kk * 2048),
-                         idesc_o, kk > 0 || !prev_first);
-            tc_commit(smem_u32(empty + vs));
-            tc_commit(smem_u32(pv_done));
-            vs += 2;
-            if (vs >= NS) vs -= NS, vph ^= 1;
-          }
+          for (int kk = 0; kk < 8; ++kk)
+            ptc_mma(o_col, tmem + S::P + kk * 8, ptc_desc_mn(vt + kk * 2048), idesc_o, kk > 0 || !start);
+          tc_commit(smem_u32(empty + vs));
+          tc_commit(smem_u32(pv_done));
+          vs += 2;
+          if (vs >= NS) vs -= NS, vph ^= 1;
+          return true;
+        };
+        // S of a unit goes before O of the one before it, except where a new sequence's
+        // queries are still on their way
+        for (int n = 0; n < steps && ok; ++n) {
+          first = n == 0 || at.unit == 0;
+          if (first && n > 0) ok = product_o(n - 1, prev_first);
+          ok = ok && product_s(n);
+          if (!first && ok) ok = product_o(n - 1, prev_first);
           prev_first = first;
+          at.next(p);
         }
+        if (ok) ok = product_o(steps - 1, prev_first);
         if (any) {   // nothing in flight when the CTA gives its TMEM back
           tc_commit(smem_u32(drained));
           mbar_wait_drain(smem_u32(drained), 0, 100000000ull);
@@ -419,12 +404,38 @@ __global__ void __launch_bounds__(PTC_THREADS, 1) paged_attention_tc_kernel(cons
       // ================= softmax and epilogue: a thread per TMEM lane, copy f of row `row`
       const int row = tid % R, f = tid / R;
       const uint32_t t_lane = (uint32_t)(warp * 32) << 16;
-      uint8_t* own_p = Ps;
-      auto clear_p = [&]() {
+      {
+        float zero[16];
 #pragma unroll
-        for (int c = 0; c < 16; ++c) *reinterpret_cast<uint4*>(own_p + ptc_off(tid, c)) = make_uint4(0, 0, 0, 0);
+        for (int e = 0; e < 16; ++e) zero[e] = 0.0f;
+#pragma unroll
+        for (int c = 0; c < 4; ++c) ptc_st16(tmem + S::P + t_lane + c * 16, zero);
+      }
+      // the queries of a sequence, head and row tile into TMEM, the copies alike
+      auto put_queries = [&](int b, int g, int rt) {
+        const int r = rt * R + row;
+        const bool in = r < p.rows && b < p.B;
+        const uint4* src = reinterpret_cast<const uint4*>(reinterpret_cast<const uint16_t*>(p.q) +
+                                                          (in ? paged_row(p, b, g, r) * D : 0));
+        uint4 u[D / 8];
+#pragma unroll
+        for (int c = 0; c < D / 8; ++c) u[c] = in ? __ldg(src + c) : make_uint4(0, 0, 0, 0);
+#pragma unroll
+        for (int c = 0; c < D / 32; ++c) {
+          float x[16];
+#pragma unroll
+          for (int e = 0; e < 4; ++e) {
+            const uint4 y = u[4 * c + e];
+            x[4 * e] = __uint_as_float(y.x), x[4 * e + 1] = __uint_as_float(y.y);
+            x[4 * e + 2] = __uint_as_float(y.z), x[4 * e + 3] = __uint_as_float(y.w);
+          }
+          ptc_st16(tmem + S::Q + t_lane + c * 16, x);
+        }
+        ptc_wait_st();
+        tc_fence_before();
+        mbar_arrive(smem_u32(q_full));
       };
-      clear_p();
+      put_queries(at.b, at.g, at.rt);
       float m = -INFINITY, l = 0.0f;       // the maximum in use, unscaled; the sum
       int first_unit = at.unit;
       uint32_t vs = 1, vph = 0;
@@ -528,16 +539,24 @@ __global__ void __launch_bounds__(PTC_THREADS, 1) paged_attention_tc_kernel(cons
           ptc_wait_st();
         }
 #pragma unroll
-        for (int c = 0; c < R / 8; ++c)
-          *reinterpret_cast<uint4*>(own_p + ptc_off(tid, f * (R / 8) + c)) =
-              make_uint4(pat_pack<BF>(v[8 * c], v[8 * c + 1]), pat_pack<BF>(v[8 * c + 2], v[8 * c + 3]),
-                         pat_pack<BF>(v[8 * c + 4], v[8 * c + 5]), pat_pack<BF>(v[8 * c + 6], v[8 * c + 7]));
+        for (int c = 0; c < R / 32; ++c) {
+          float x[16];
+#pragma unroll
+          for (int e = 0; e < 16; ++e) x[e] = __uint_as_float(pat_pack<BF>(v[32 * c + 2 * e], v[32 * c + 2 * e + 1]));
+          ptc_st16(tmem + S::P + t_lane + f * (R / 2) + c * 16, x);
+        }
+        ptc_wait_st();
         tc_fence_before();
-        fence_proxy_async_smem();
+        if (edge) fence_proxy_async_smem();      // values that were zeroed
         mbar_arrive(smem_u32(p_full));
         vs += 2;
         if (vs >= NS) vs -= NS, vph ^= 1;
         const bool ends = at.unit + 1 == at.nu, leaves = ends || n + 1 == steps;
+        if (ends && n + 1 < steps) {
+          int b = at.b, g = at.g, rt = at.rt;
+          PagedPos<PTC_TK>::next_rows(p, b, g, rt);
+          put_queries(b, g, rt);
+        }
         if (strange || leaves) {
           if (!(ok = wait_all(pv_done, n & 1))) break;
           tc_fence_after();
@@ -621,7 +640,7 @@ __global__ void __launch_bounds__(PTC_THREADS, 1) paged_attention_tc_kernel(cons
                 if constexpr (F == 1)
                   put(row, h * 16 + q4, a);
                 else
-                  *reinterpret_cast<float4*>(own_p + ptc_off(tid, q4)) = a;
+                  *reinterpret_cast<float4*>(own_x + ptc_off(tid, q4)) = a;
               }
             }
             if constexpr (F > 1) {
@@ -632,7 +651,7 @@ __global__ void __launch_bounds__(PTC_THREADS, 1) paged_attention_tc_kernel(cons
                 float4 a = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
 #pragma unroll
                 for (int i = 0; i < F; ++i) {
-                  const float4 y = *reinterpret_cast<const float4*>(own_p + ptc_off(i * R + r, q4));
+                  const float4 y = *reinterpret_cast<const float4*>(own_x + ptc_off(i * R + r, q4));
                   a.x += y.x, a.y += y.y, a.z += y.z, a.w += y.w;
                 }
                 put(r, h * 16 + q4, a);
@@ -640,7 +659,6 @@ __global__ void __launch_bounds__(PTC_THREADS, 1) paged_attention_tc_kernel(cons
               named_bar_sync(1, PTC_SOFTMAX);
             }
           }
-          if constexpr (F > 1) clear_p();
           tc_fence_before();
           if (!whole && tid == 0) {
             const PagedCut range = s_range;
