@@ -67,6 +67,18 @@ __device__ __forceinline__ void ptc_st16(uint32_t taddr, const float (&v)[16]) {
 }
 __device__ __forceinline__ void ptc_wait_st() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
 
+// One lane of a converged warp.  The product warp runs its loop with all lanes, so
+// that what the instructions take stays in uniform registers.
+__device__ __forceinline__ bool ptc_elect() {
+  uint32_t r;
+  asm volatile(
+      "{\n\t.reg .pred p;\n\t"
+      "elect.sync _|p, 0xffffffff;\n\t"
+      "selp.u32 %0, 1, 0, p;\n\t}"
+      : "=r"(r));
+  return r != 0;
+}
+
 // MN-major operand in the 128-byte swizzle: V as it lies, 16 keys a step
 __device__ __forceinline__ uint64_t ptc_desc_mn(uint32_t addr) {
   uint64_t d = 0;
@@ -348,37 +360,46 @@ __global__ void __launch_bounds__(PTC_THREADS, 1) paged_attention_tc_kernel(cons
       flush();
     } else if (warp == 8) {
       // ================= products
-      if (lane == 0) {
+      {
         const uint32_t idesc_s = make_idesc_f16(BF, 128, 128);
         const uint32_t idesc_o = make_idesc_f16(BF, 128, D) | (1u << 16);   // V is MN-major
         uint32_t ks = 0, kph = 0, vs = 1, vph = 0, items = 0;
         bool ok = true, first = true, prev_first = true, any = false;
+        // operand descriptors of the ring's first tile; addresses in them count 16 bytes
+        const uint64_t desc_k = make_sw128_desc(smem_u32(ring)), desc_v = ptc_desc_mn(smem_u32(ring));
+        auto wait = [&](uint64_t* bar, uint32_t parity) {
+          return __all_sync(0xffffffffu, mbar_wait(smem_u32(bar), parity, abort_flag, p.err)) != 0;
+        };
         auto product_s = [&](int n) {
-          if (first && !mbar_wait(smem_u32(q_full), items++ & 1, abort_flag, p.err)) return false;
-          if (!mbar_wait(smem_u32(full + ks), kph, abort_flag, p.err)) return false;
+          if (first && !wait(q_full, items++ & 1)) return false;
+          if (!wait(full + ks, kph)) return false;
           tc_fence_after();
-          const uint32_t kt = smem_u32(ring) + ks * S::TILE;
+          const uint64_t kt = desc_k + ks * (S::TILE >> 4);
+          if (ptc_elect()) {
 #pragma unroll
-          for (int kk = 0; kk < D / 16; ++kk)
-            ptc_mma(tmem + (n & 1) * 128, tmem + S::Q + kk * 8, make_sw128_desc(kt + (kk >> 2) * 16384) + 2 * (kk & 3), idesc_s,
-                    kk > 0);
+            for (int kk = 0; kk < D / 16; ++kk)
+              ptc_mma(tmem + (n & 1) * 128, tmem + S::Q + kk * 8, kt + (kk >> 2) * 1024 + 2 * (kk & 3), idesc_s, kk > 0);
+            tc_commit(smem_u32(s_full + (n & 1)));
+            tc_commit(smem_u32(empty + ks));
+          }
+          __syncwarp();
           any = true;
-          tc_commit(smem_u32(s_full + (n & 1)));
-          tc_commit(smem_u32(empty + ks));
           ks += 2;
           if (ks >= NS) ks -= NS, kph ^= 1;
           return true;
         };
         auto product_o = [&](int n, bool start) {
-          if (!mbar_wait(smem_u32(p_full), n & 1, abort_flag, p.err)) return false;
-          if (!mbar_wait(smem_u32(full + vs), vph, abort_flag, p.err)) return false;
+          if (!wait(p_full, n & 1) || !wait(full + vs, vph)) return false;
           tc_fence_after();
-          const uint32_t vt = smem_u32(ring) + vs * S::TILE;
+          const uint64_t vt = desc_v + vs * (S::TILE >> 4);
+          if (ptc_elect()) {
 #pragma unroll
-          for (int kk = 0; kk < 8; ++kk)
-            ptc_mma(o_col, tmem + S::P + kk * 8, ptc_desc_mn(vt + kk * 2048), idesc_o, kk > 0 || !start);
-          tc_commit(smem_u32(empty + vs));
-          tc_commit(smem_u32(pv_done));
+            for (int kk = 0; kk < 8; ++kk)
+              ptc_mma(o_col, tmem + S::P + kk * 8, vt + kk * 128, idesc_o, kk > 0 || !start);
+            tc_commit(smem_u32(empty + vs));
+            tc_commit(smem_u32(pv_done));
+          }
+          __syncwarp();
           vs += 2;
           if (vs >= NS) vs -= NS, vph ^= 1;
           return true;
@@ -395,7 +416,8 @@ __global__ void __launch_bounds__(PTC_THREADS, 1) paged_attention_tc_kernel(cons
         }
         if (ok) ok = product_o(steps - 1, prev_first);
         if (any) {   // nothing in flight when the CTA gives its TMEM back
-          tc_commit(smem_u32(drained));
+          if (ptc_elect()) tc_commit(smem_u32(drained));
+          __syncwarp();
           mbar_wait_drain(smem_u32(drained), 0, 100000000ull);
         }
       }
