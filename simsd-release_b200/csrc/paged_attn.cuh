@@ -276,6 +276,15 @@ struct PagedPart {
   int b, g, r0, c0, parts;
 };
 
+// Counts a part that its CTA has written (and a barrier has followed) in; by one thread.  True for the last.
+__device__ __forceinline__ bool paged_arrive(const PagedAttnArgs& p, const PagedPart& x) {
+  __threadfence();
+  const bool last = atomicAdd(p.arrived + x.c0, 1) == x.parts - 1;
+  if (last) p.arrived[x.c0] = 0;
+  __threadfence();
+  return last;
+}
+
 // Joins the parts of a cut sequence (one KV head and row tile of it) that starts
 // in CTA c0: part i's max, sum and O lie in slot 1 of CTA c0 for i = 0, in slot 0
 // of CTA c0 + i for the others.  `buf`: OBUF bytes of shared memory.
@@ -389,7 +398,7 @@ __global__ void __launch_bounds__(PAT_THREADS, PAT_CTAS_PER_SM) paged_attention_
     steps = cut.first(blockIdx.x + 1) - cut.first(blockIdx.x);
     if (tid == 0) s_range = cut;
   }
-  if (tid < 2) s_cut[tid].parts = 0;
+  if (tid < 2) s_cut[tid].parts = 0, s_join[tid] = false;
   PagedPos<PAT_TK> at = ld;
 
   // ---- loads: the warp's 16 keys of position `ld` into its next ring slot.
@@ -695,27 +704,19 @@ __global__ void __launch_bounds__(PAT_THREADS, PAT_CTAS_PER_SM) paged_attention_
             p.part_o[(((long long)slot * MT + mt) * NT + nt) * 32 + lane] = a;
         }
       }
+      __syncthreads();
       if (!whole && tid == 0) {
         const PagedCut cut = s_range;
         const int head = cut.first(blockIdx.x) + i - at.unit, c0 = cut.cta_of(head);   // the sequence's first unit and CTA
         s_cut[part] = {at.b, at.g, r0, c0, cut.cta_of(head + at.nu - 1) - c0 + 1};
+        // the first part at once, so that it is not this CTA that everyone else waits for in the end
+        if (part == 0) s_join[0] = paged_arrive(p, s_cut[0]);
       }
-      __syncthreads();
     }
     at.next(p);
   }
   // cut sequences (at most the range's first and last): the last of their CTAs to get here joins the parts
-  if (s_cut[0].parts + s_cut[1].parts == 0) return;
-  if (tid < 2) {
-    s_join[tid] = false;
-    if (s_cut[tid].parts > 0) {
-      __threadfence();
-      const int c0 = s_cut[tid].c0;
-      s_join[tid] = atomicAdd(p.arrived + c0, 1) == s_cut[tid].parts - 1;
-      if (s_join[tid]) p.arrived[c0] = 0;
-      __threadfence();
-    }
-  }
+  if (tid == 0 && s_cut[1].parts > 0) s_join[1] = paged_arrive(p, s_cut[1]);
   __syncthreads();
   for (int k = 0; k < 2; ++k) {
     const PagedPart x = s_cut[k];

@@ -194,6 +194,7 @@ __global__ void __launch_bounds__(PTC_THREADS, 1) paged_attention_tc_kernel(cons
     mbar_init(smem_u32(drained), 1);
     *abort_flag = 0;
     s_cut[0].parts = s_cut[1].parts = 0;
+    s_join[0] = s_join[1] = false;
     fence_mbar_init();
   }
   if (warp == 8) {
@@ -682,15 +683,20 @@ __global__ void __launch_bounds__(PTC_THREADS, 1) paged_attention_tc_kernel(cons
             }
           }
           tc_fence_before();
-          if (!whole && tid == 0) {
-            const PagedCut range = s_range;
-            const int head = range.first(blockIdx.x) + n - at.unit, c0 = range.cta_of(head);
-            s_cut[part] = {at.b, at.g, r0, c0, range.cta_of(head + at.nu - 1) - c0 + 1};
+          if (!whole) {
+            if (part == 0) named_bar_sync(1, PTC_SOFTMAX);
+            if (tid == 0) {
+              const PagedCut range = s_range;
+              const int head = range.first(blockIdx.x) + n - at.unit, c0 = range.cta_of(head);
+              s_cut[part] = {at.b, at.g, r0, c0, range.cta_of(head + at.nu - 1) - c0 + 1};
+              // the first part at once, so that it is not this CTA that everyone else waits for in the end
+              if (part == 0) s_join[0] = paged_arrive(p, s_cut[0]);
+            }
           }
         }
         at.next(p);
       }
-      if (!ok && tid == 0) s_cut[0].parts = s_cut[1].parts = 0;
+      if (!ok && tid == 0) s_join[0] = false, s_cut[1].parts = 0;
     }
   }
   tc_fence_before();
@@ -699,18 +705,8 @@ __global__ void __launch_bounds__(PTC_THREADS, 1) paged_attention_tc_kernel(cons
     tc_fence_after();
     tmem_dealloc(tmem, 512);
   }
-  if (!mine || s_cut[0].parts + s_cut[1].parts == 0) return;
   // cut sequences (at most the range's first and last): the last of their CTAs to get here joins the parts
-  if (tid < 2) {
-    s_join[tid] = false;
-    if (s_cut[tid].parts > 0) {
-      __threadfence();
-      const int c0 = s_cut[tid].c0;
-      s_join[tid] = atomicAdd(p.arrived + c0, 1) == s_cut[tid].parts - 1;
-      if (s_join[tid]) p.arrived[c0] = 0;
-      __threadfence();
-    }
-  }
+  if (tid == 0 && s_cut[1].parts > 0) s_join[1] = paged_arrive(p, s_cut[1]);
   __syncthreads();
   for (int k = 0; k < 2; ++k)
     if (s_join[k]) ptc_join<D, R, BF>(p, s_cut[k], reinterpret_cast<float2*>(ring));
