@@ -139,13 +139,19 @@ __device__ __forceinline__ int paged_units(int n) {
   return n <= TK ? 1 : (n + TK - 1) / TK;
 }
 
+// The end of a sequence's row tile (joining the warps, writing, the next queries) takes
+// a CTA about as long as a unit does, and is weighed as one in the cut.
+constexpr int PAGED_END = 1;
+
 // Position in the unit order: sequence b (length n, nu units per KV head and row
-// tile), KV head g, row tile rt, unit of it.
+// tile), KV head g, row tile rt, unit of it; w counts units and ends before it.
 template <int TK>
 struct PagedPos {
-  int b, g, rt, unit, n, nu;
+  int b, g, rt, unit, n, nu, w;
   __device__ __forceinline__ void next(const PagedAttnArgs& p) {
+    ++w;
     if (++unit < nu) return;
+    w += PAGED_END;
     unit = 0;
     if (!next_rows(p, b, g, rt) || b >= p.B) return;
     n = paged_len(p, b);
@@ -162,7 +168,7 @@ struct PagedPos {
   }
 };
 
-// The equal cut of `total` units over `ctas` CTAs, the first `extra` of which have one more
+// The equal cut of `total` units and ends over `ctas` CTAs, the first `extra` of which have one more
 struct PagedCut {
   int ctas, base, extra;
   __device__ __forceinline__ int first(int c) const { return c * base + min(c, extra); }
@@ -202,8 +208,8 @@ __device__ __forceinline__ void paged_store_lse(const PagedAttnArgs& p, int b, i
   p.lse[paged_row(p, b, g, r)] = l == 0.0f ? -INFINITY : fmaf(0.69314718055994531f, m, logf(l));
 }
 
-// This CTA's place in the cut of the call's units and the position of its first
-// unit.  False: this CTA has none.
+// This CTA's place in the cut of the call's units and ends, and the position of its
+// first unit.  False: this CTA has none.
 template <int THREADS, int TK>
 __device__ __forceinline__ bool paged_range(const PagedAttnArgs& p, PagedCut& cut, PagedPos<TK>& pos) {
   constexpr int WARPS = THREADS / 32;
@@ -215,7 +221,7 @@ __device__ __forceinline__ bool paged_range(const PagedAttnArgs& p, PagedCut& cu
   auto units = [&](int b) {
     if (b >= p.B) return 0;
     if (flag && p.seq_lens[b] > (long long)p.max_pages * p.page_size) atomicOr(p.err, SIMSD_DEV_ERR_BAD_INDEX);
-    return paged_units<TK>(paged_len(p, b)) * per;
+    return (paged_units<TK>(paged_len(p, b)) + PAGED_END) * per;
   };
   // sequences tid, tid + THREADS, ...: the first of them scanned, the others summed
   int u = units(tid), incl = u, more = 0;
@@ -264,11 +270,18 @@ __device__ __forceinline__ bool paged_range(const PagedAttnArgs& p, PagedCut& cu
   pos.b = s_b;
   pos.n = paged_len(p, pos.b);
   pos.nu = paged_units<TK>(pos.n);
-  const int rem = w0 - s_first, hr = rem / pos.nu;
-  pos.unit = rem - hr * pos.nu;
+  const int rem = w0 - s_first, hr = rem / (pos.nu + PAGED_END);
+  pos.unit = rem - hr * (pos.nu + PAGED_END);
+  pos.w = w0;
   pos.g = hr / p.row_tiles;
   pos.rt = hr - pos.g * p.row_tiles;
-  return true;
+  if (pos.unit >= pos.nu) {          // an end: the unit after it
+    pos.w += PAGED_END - (pos.unit - pos.nu) - 1;
+    pos.unit = pos.nu - 1;
+    pos.w -= PAGED_END;
+    pos.next(p);
+  }
+  return pos.w < cut.first(c + 1);
 }
 
 // A cut sequence (one KV head and row tile, rows from r0): its first CTA and how many it lies in
@@ -391,11 +404,11 @@ __global__ void __launch_bounds__(PAT_THREADS, PAT_CTAS_PER_SM) paged_attention_
 
   __shared__ PagedCut s_range;
   PagedPos<PAT_TK> ld;
-  int steps;
+  int end;
   {
     PagedCut cut;
     if (!paged_range<PAT_THREADS, PAT_TK>(p, cut, ld)) return;
-    steps = cut.first(blockIdx.x + 1) - cut.first(blockIdx.x);
+    end = cut.first(blockIdx.x + 1);
     if (tid == 0) s_range = cut;
   }
   if (tid < 2) s_cut[tid].parts = 0, s_join[tid] = false;
@@ -413,10 +426,9 @@ __global__ void __launch_bounds__(PAT_THREADS, PAT_CTAS_PER_SM) paged_attention_
     return key < x.n ? p.page_table[x.b * p.ld_table + p.page_div(key)] : -1;
   };
   int page = fetch_page(ld);
-  int loaded = 0;
   uint32_t load_slot = ring;
   auto load = [&]() {
-    if (loaded < steps) {
+    if (ld.w < end) {
       const uint32_t dst = load_slot + swz;
       const int key0 = ld.unit * PAT_TK + warp * 16;
       if (key0 < ld.n) {
@@ -458,13 +470,10 @@ __global__ void __launch_bounds__(PAT_THREADS, PAT_CTAS_PER_SM) paged_attention_
           }
         }
       }
-      ++loaded;
       load_slot += 2 * S::MAT;
       if (load_slot == ring + S::STAGES * 2 * S::MAT) load_slot = ring;
-      if (loaded < steps) {
-        ld.next(p);
-        page = fetch_page(ld);
-      }
+      ld.next(p);
+      if (ld.w < end) page = fetch_page(ld);
     }
     pat_commit();
   };
@@ -497,13 +506,13 @@ __global__ void __launch_bounds__(PAT_THREADS, PAT_CTAS_PER_SM) paged_attention_
   uint32_t bq[QW];
   int first_unit = at.unit;
   uint32_t slot_at = ring;
-  for (int i = 0; i < steps; ++i) {
-    if (i == 0 || at.unit == 0) {
+  for (bool start = true; at.w < end; start = false) {
+    if (start || at.unit == 0) {
       // a new sequence, head or row tile: its queries, and empty sums
       first_unit = at.unit;
 #pragma unroll
       for (int k = 0; k < QW; ++k) bq[k] = qnext[k];
-      if (at.nu - at.unit < steps - i) {
+      if (at.w + at.nu - at.unit + PAGED_END < end) {
         int b = at.b, g = at.g, rt = at.rt;
         PagedPos<PAT_TK>::next_rows(p, b, g, rt);
         fetch_queries(b, g, rt);
@@ -636,7 +645,7 @@ __global__ void __launch_bounds__(PAT_THREADS, PAT_CTAS_PER_SM) paged_attention_
     }
     __syncwarp();
     const bool ends = at.unit + 1 == at.nu;
-    if (ends || i + 1 == steps) {
+    if (ends || at.w + 1 >= end) {
       // join the warps; a whole sequence is written, a part goes to the workspace
       const bool whole = ends && first_unit == 0;
       const int part = first_unit == 0 ? 1 : 0, slot = 2 * blockIdx.x + part, r0 = at.rt * NR;
@@ -707,7 +716,7 @@ __global__ void __launch_bounds__(PAT_THREADS, PAT_CTAS_PER_SM) paged_attention_
       __syncthreads();
       if (!whole && tid == 0) {
         const PagedCut cut = s_range;
-        const int head = cut.first(blockIdx.x) + i - at.unit, c0 = cut.cta_of(head);   // the sequence's first unit and CTA
+        const int head = at.w - at.unit, c0 = cut.cta_of(head);   // the sequence's first unit and CTA
         s_cut[part] = {at.b, at.g, r0, c0, cut.cta_of(head + at.nu - 1) - c0 + 1};
         // the first part at once, so that it is not this CTA that everyone else waits for in the end
         if (part == 0) s_join[0] = paged_arrive(p, s_cut[0]);

@@ -212,7 +212,7 @@ __global__ void __launch_bounds__(PTC_THREADS, 1) paged_attention_tc_kernel(cons
   const uint32_t tmem = *tmem_slot;
   const uint32_t o_col = tmem + S::O;
   if (mine) {
-    const int steps = cut.first(blockIdx.x + 1) - cut.first(blockIdx.x);
+    const int end = cut.first(blockIdx.x + 1);
     if (tid == 0) s_range = cut;
     if (args.block && warp == 4) {
       // ================= loads of keys and values by TMA: a lane per `block` tokens of the unit
@@ -228,16 +228,14 @@ __global__ void __launch_bounds__(PTC_THREADS, 1) paged_attention_tc_kernel(cons
       int page = run_page(at);
       uint32_t filled = 0, parity = 0;           // tiles with a load in flight, and its phase
       bool ok = true;
-      for (int n = 0; n < steps && ok; ++n) {
+      while (ok && at.w < end) {
         if (page < 0 || page > p.num_pages || (page == p.num_pages && lane < runs && at.unit * PTC_TK + first_key < at.n)) {
           if (p.err) atomicOr(p.err, SIMSD_DEV_ERR_BAD_INDEX);
           page = p.num_pages;
         }
         const int now = page, head = at.g, key = at.unit * PTC_TK + first_key, tok = key - p.page_div(key) * p.page_size;
-        if (n + 1 < steps) {
-          at.next(p);
-          page = run_page(at);
-        }
+        at.next(p);
+        if (at.w < end) page = run_page(at);
         for (int kv = 0; kv < 2; ++kv) {
           ok = __all_sync(0xffffffffu, mbar_wait(smem_u32(empty + slot), phase ^ 1, abort_flag, p.err));
           if (!ok) break;
@@ -307,7 +305,7 @@ __global__ void __launch_bounds__(PTC_THREADS, 1) paged_attention_tc_kernel(cons
       // fixed distance apart; otherwise each key's place is handed round.
       const bool page16 = p.page_size % 16 == 0;
       const uint32_t lane_dst = ptc_off(lw * 32 + khi, kc);
-      for (int n = 0; n < steps; ++n) {
+      while (at.w < end) {
         const int key = at.unit * PTC_TK + lt;
         long long off = -1;
         if (key < at.n) {
@@ -317,10 +315,8 @@ __global__ void __launch_bounds__(PTC_THREADS, 1) paged_attention_tc_kernel(cons
             atomicOr(p.err, SIMSD_DEV_ERR_BAD_INDEX);
         }
         const PagedPos<PTC_TK> cur = at;
-        if (n + 1 < steps) {
-          at.next(p);
-          page = key_page(at);
-        }
+        at.next(p);
+        if (at.w < end) page = key_page(at);
         long long half[2];                       // keys khi and 16 + khi of the warp, chunk kc
         int live[2];                             // keys of that half that exist, from khi on
 #pragma unroll
@@ -407,7 +403,8 @@ __global__ void __launch_bounds__(PTC_THREADS, 1) paged_attention_tc_kernel(cons
         };
         // S of a unit goes before O of the one before it, except where a new sequence's
         // queries are still on their way
-        for (int n = 0; n < steps && ok; ++n) {
+        int n = 0;
+        for (; ok && at.w < end; ++n) {
           first = n == 0 || at.unit == 0;
           if (first && n > 0) ok = product_o(n - 1, prev_first);
           ok = ok && product_s(n);
@@ -415,7 +412,7 @@ __global__ void __launch_bounds__(PTC_THREADS, 1) paged_attention_tc_kernel(cons
           prev_first = first;
           at.next(p);
         }
-        if (ok) ok = product_o(steps - 1, prev_first);
+        if (ok) ok = product_o(n - 1, prev_first);
         if (any) {   // nothing in flight when the CTA gives its TMEM back
           if (ptc_elect()) tc_commit(smem_u32(drained));
           __syncwarp();
@@ -466,7 +463,7 @@ __global__ void __launch_bounds__(PTC_THREADS, 1) paged_attention_tc_kernel(cons
       auto wait_all = [&](uint64_t* bar, uint32_t parity) {
         return named_bar_and(1, PTC_SOFTMAX, mbar_wait(smem_u32(bar), parity, abort_flag, p.err));
       };
-      for (int n = 0; n < steps && ok; ++n) {
+      for (int n = 0; ok && at.w < end; ++n) {
         if (n == 0 || at.unit == 0) {
           first_unit = at.unit;
           m = -INFINITY, l = 0.0f;
@@ -574,8 +571,8 @@ __global__ void __launch_bounds__(PTC_THREADS, 1) paged_attention_tc_kernel(cons
         mbar_arrive(smem_u32(p_full));
         vs += 2;
         if (vs >= NS) vs -= NS, vph ^= 1;
-        const bool ends = at.unit + 1 == at.nu, leaves = ends || n + 1 == steps;
-        if (ends && n + 1 < steps) {
+        const bool ends = at.unit + 1 == at.nu, leaves = ends || at.w + 1 >= end;
+        if (ends && at.w + 1 + PAGED_END < end) {
           int b = at.b, g = at.g, rt = at.rt;
           PagedPos<PTC_TK>::next_rows(p, b, g, rt);
           put_queries(b, g, rt);
@@ -687,7 +684,7 @@ __global__ void __launch_bounds__(PTC_THREADS, 1) paged_attention_tc_kernel(cons
             if (part == 0) named_bar_sync(1, PTC_SOFTMAX);
             if (tid == 0) {
               const PagedCut range = s_range;
-              const int head = range.first(blockIdx.x) + n - at.unit, c0 = range.cta_of(head);
+              const int head = at.w - at.unit, c0 = range.cta_of(head);
               s_cut[part] = {at.b, at.g, r0, c0, range.cta_of(head + at.nu - 1) - c0 + 1};
               // the first part at once, so that it is not this CTA that everyone else waits for in the end
               if (part == 0) s_join[0] = paged_arrive(p, s_cut[0]);
