@@ -531,7 +531,7 @@ int simsd_paged_append(const void* qkv, int64_t ldqkv, int T, int Hq, int Hk, in
  * tail_mask[b * ldm_b + t * ldm_t + jt] != 0.  A query without a visible key: o =
  * 0, lse = -inf.  q, o [B, L, Hq, head_dim] contiguous, lse [B, L, Hq] or NULL.
  * The lengths are read on the device only.  B Hk ceil(G L / 128) (max_pages
- * page_size / 64 + 2) < 2^31 (more: SIMSD_ERR_UNSUPPORTED).
+ * page_size / 64 + 3) < 2^31 (more: SIMSD_ERR_UNSUPPORTED).
  */
 size_t simsd_paged_attention_workspace_size(int L, int Hq, int Hk, int head_dim);
 int simsd_paged_attention(const void* q, const void* k_cache, const void* v_cache, int num_pages, int page_size,

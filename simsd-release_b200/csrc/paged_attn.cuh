@@ -140,18 +140,26 @@ __device__ __forceinline__ int paged_units(int n) {
 }
 
 // The end of a sequence's row tile (joining the warps, writing, the next queries) takes
-// a CTA about as long as a unit does, and is weighed as one in the cut.
-constexpr int PAGED_END = 1;
+// a CTA as long as one or two units do, and is weighed as that many in the cut: with
+// 64-key units 64 sequences of 0.1 - 2k tokens take 50 us at 0, 44 at 1, 40 at 2 and 32
+// of 0.3 - 4k 41, 38, 38; with the 128-key units of paged_attn_tc.cuh 16 x 8 rows take
+// 41, 39.5, 41.
+template <int TK>
+struct PagedEnd {
+  static constexpr int UNITS = TK == 64 ? 2 : 1;
+};
+constexpr int PAGED_END_MAX = 2;
 
 // Position in the unit order: sequence b (length n, nu units per KV head and row
 // tile), KV head g, row tile rt, unit of it; w counts units and ends before it.
 template <int TK>
 struct PagedPos {
+  static constexpr int END = PagedEnd<TK>::UNITS;
   int b, g, rt, unit, n, nu, w;
   __device__ __forceinline__ void next(const PagedAttnArgs& p) {
     ++w;
     if (++unit < nu) return;
-    w += PAGED_END;
+    w += END;
     unit = 0;
     if (!next_rows(p, b, g, rt) || b >= p.B) return;
     n = paged_len(p, b);
@@ -221,7 +229,7 @@ __device__ __forceinline__ bool paged_range(const PagedAttnArgs& p, PagedCut& cu
   auto units = [&](int b) {
     if (b >= p.B) return 0;
     if (flag && p.seq_lens[b] > (long long)p.max_pages * p.page_size) atomicOr(p.err, SIMSD_DEV_ERR_BAD_INDEX);
-    return (paged_units<TK>(paged_len(p, b)) + PAGED_END) * per;
+    return (paged_units<TK>(paged_len(p, b)) + PagedEnd<TK>::UNITS) * per;
   };
   // sequences tid, tid + THREADS, ...: the first of them scanned, the others summed
   int u = units(tid), incl = u, more = 0;
@@ -270,16 +278,16 @@ __device__ __forceinline__ bool paged_range(const PagedAttnArgs& p, PagedCut& cu
   pos.b = s_b;
   pos.n = paged_len(p, pos.b);
   pos.nu = paged_units<TK>(pos.n);
-  const int rem = w0 - s_first, hr = rem / (pos.nu + PAGED_END);
-  pos.unit = rem - hr * (pos.nu + PAGED_END);
+  const int rem = w0 - s_first, hr = rem / (pos.nu + PagedEnd<TK>::UNITS);
+  pos.unit = rem - hr * (pos.nu + PagedEnd<TK>::UNITS);
   pos.w = w0;
   pos.g = hr / p.row_tiles;
   pos.rt = hr - pos.g * p.row_tiles;
   if (pos.unit >= pos.nu) {          // an end: the unit after it
-    pos.w += PAGED_END - (pos.unit - pos.nu) - 1;
+    const int w = w0 + pos.nu + PagedEnd<TK>::UNITS - pos.unit;
     pos.unit = pos.nu - 1;
-    pos.w -= PAGED_END;
     pos.next(p);
+    pos.w = w;
   }
   return pos.w < cut.first(c + 1);
 }
@@ -512,7 +520,7 @@ __global__ void __launch_bounds__(PAT_THREADS, PAT_CTAS_PER_SM) paged_attention_
       first_unit = at.unit;
 #pragma unroll
       for (int k = 0; k < QW; ++k) bq[k] = qnext[k];
-      if (at.w + at.nu - at.unit + PAGED_END < end) {
+      if (at.w + at.nu - at.unit + at.END < end) {
         int b = at.b, g = at.g, rt = at.rt;
         PagedPos<PAT_TK>::next_rows(p, b, g, rt);
         fetch_queries(b, g, rt);

@@ -572,7 +572,7 @@ __global__ void __launch_bounds__(PTC_THREADS, 1) paged_attention_tc_kernel(cons
         vs += 2;
         if (vs >= NS) vs -= NS, vph ^= 1;
         const bool ends = at.unit + 1 == at.nu, leaves = ends || at.w + 1 >= end;
-        if (ends && at.w + 1 + PAGED_END < end) {
+        if (ends && at.w + 1 + at.END < end) {
           int b = at.b, g = at.g, rt = at.rt;
           PagedPos<PTC_TK>::next_rows(p, b, g, rt);
           put_queries(b, g, rt);

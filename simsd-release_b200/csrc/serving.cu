@@ -297,7 +297,7 @@ int simsd_paged_attention(const void* q, const void* k_cache, const void* v_cach
   const PagedPlan pl = paged_plan(L, a.G, head_dim);
   a.rows = a.G * L;
   a.row_tiles = (a.rows + pl.nr - 1) / pl.nr;
-  if ((long long)B * Hk * a.row_tiles * ((int64_t)max_pages * page_size / PAT_TK + 1 + PAGED_END) > 0x7fffffffLL)
+  if ((long long)B * Hk * a.row_tiles * ((int64_t)max_pages * page_size / PAT_TK + 1 + PAGED_END_MAX) > 0x7fffffffLL)
     return SIMSD_ERR_UNSUPPORTED;
   uint8_t* ws = reinterpret_cast<uint8_t*>(workspace);
   a.arrived = reinterpret_cast<int*>(ws);
