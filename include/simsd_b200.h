@@ -497,8 +497,9 @@ int simsd_moe_ep_return(const void* y, int64_t ldy, const int32_t* recv_expert, 
  * written for it.  The workspaces of these calls have no header; they are scratch
  * that is not read after the call's kernels, except that simsd_paged_attention
  * keeps counters in the first SIMSD_PAGED_COUNTER_BYTES of its own: zero before the
- * first call with it, zero again after every call.  Calls that share a workspace
- * must be ordered on one stream. */
+ * first call with it, zero again after every call but one that ended with
+ * SIMSD_DEV_ERR_TIMEOUT, after which the caller zeroes them.  Calls that share a
+ * workspace must be ordered on one stream. */
 #define SIMSD_PAGED_COUNTER_BYTES 4096
 
 /*

@@ -291,8 +291,13 @@ def device_error(dev: torch.device | None = None) -> int:
 
 
 def clear_device_error(dev: torch.device | None = None) -> None:
-    """Zero `dev`'s workspace header (error word and tile counters), stream-ordered."""
+    """Zero `dev`'s workspace header (error word and tile counters), stream-ordered.  The
+    streams' scratch is dropped: a launch that gave up may have left counters in it."""
     dev = torch.device("cuda", torch.cuda.current_device()) if dev is None else dev
+    for key in [k for k in _STREAM_SCRATCH if dev.index in (None, k[0])]:
+        del _STREAM_SCRATCH[key]
+    if _binding is not None:
+        _binding.forget()
     buf = _WORKSPACES.get(dev)
     if buf is None:
         return
