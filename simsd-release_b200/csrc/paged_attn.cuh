@@ -35,6 +35,10 @@
 // holds.  A tail key that some rows of the unit see and others do not takes part
 // with weight 0 in the second product; where its value is not finite (0 x inf), the
 // unit's product runs row by row with the hidden keys zeroed instead.
+//
+// Measured (B200, 8 KV heads x 128, 4 query heads each, bf16): 2 x 120-128k tokens 172
+// us, 6.2 TB/s, 94 % of the measured copy rate; 32 x 0.3-4k 38 us, 4.8 TB/s, 73 %; 1 x 100
+// 7.6 us.
 #pragma once
 #include "paged.cuh"
 

@@ -23,7 +23,8 @@
 // rest of its arithmetic is packed: the maximum in the 16-bit type itself, the
 // differences and sums two at a time.  Rows
 // are read last to first, so that the rows drawn from, mostly early ones, are the
-// ones left in L2.
+// ones left in L2.  64 x 7 drafts of 151936 tokens, bf16: 76 us, 4.3 TB/s (statistics 58
+// at 5.0 TB/s under ncu); 1 x 4 of 32000 8.4 us, the latency of two kernels.
 #pragma once
 #include "sm100.cuh"
 
