@@ -549,7 +549,7 @@ int simsd_paged_attention(const void* q, const void* k_cache, const void* v_cach
  *   x_i is kept while uniform[b, i] q_i(x_i) < p_i(x_i); at the first one refused
  *   the next token is argmax_v max(p - q, 0)(v) / noise[b, v], after d kept ones
  *   argmax_v p_d(v) / noise[b, v]  (noise positive, exponentially distributed;
- *   ties to the lowest v; a residual that is nowhere positive draws from p).
+ *   ties to the lowest v; a residual nowhere over 2^-21 of p draws from p).
  * tokens [B, K + 1]: the kept ones, the drawn one, then -1; accepted [B]: how many
  * were kept; logprobs [B, K + 1]: log p of each, 0 after them.  target_logits
  * [B, K + 1, V] (strides ldt_b, ldt_r, unit last), draft_logits [B, K, V],

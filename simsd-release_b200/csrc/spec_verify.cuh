@@ -11,7 +11,7 @@
 // T = 0: p and q are one at their first maximum.  NaN logits count as -inf,
 // +inf as the largest finite number; a row without any finite logit has p = 0.
 // Ties go to the lowest token.  A residual that is nowhere positive (p <= q
-// everywhere) draws from p.
+// everywhere, to 2^-21 of p) draws from p.
 //
 // Two kernels.  spec_stat_kernel reads every row once: a warp takes `blocks` times
 // 1024 logits, keeps each block in registers between its maximum and the sum of its
@@ -61,6 +61,10 @@ struct SpecVerifyArgs {
 constexpr int SV_THREADS = 256, SV_WARPS = SV_THREADS / 32;
 constexpr int SV_BLOCK = 1024;                     // logits that a warp holds at a time
 constexpr int SV_CHUNK = 2048;                     // tokens that a CTA races at a time
+// p - q counts where it is more than p's rounding: the same logits in two rows give p and
+// q apart by a rounding of the sum, of its reciprocal and of the product each, at most
+// 2^-22 of p.  Without it two equal rows leave noise for a residual, which is drawn from.
+constexpr float SV_OVER = 1.0f - 0x1p-21f;
 
 __device__ __forceinline__ float spec_clean(float v) { return fminf(fmaxf(v, -INFINITY), 3.402823466e+38f); }
 __device__ __forceinline__ float spec_logit(const void* p, long long i, int dtype) {
@@ -417,7 +421,9 @@ __global__ void __launch_bounds__(SV_THREADS) spec_draw_kernel(const SpecVerifyA
     const SpecPart& y = sv_rows[r];
     return y.m == -INFINITY ? SpecLaw{0.0f, 0.0f} : SpecLaw{y.m, 1.0f / (float)y.s};
   };
-  const SpecLaw pt = law(a), pd = dr ? law(p.K + 1 + a) : SpecLaw{0.0f, 0.0f};
+  SpecLaw pt = law(a);
+  const SpecLaw pd = dr ? law(p.K + 1 + a) : SpecLaw{0.0f, 0.0f};
+  if (dr) pt.inv *= SV_OVER;
   SpecBest best = {-1.0f, 0x7fffffff};
   // tokens lo .. hi - 1, a thread's in ascending order
   auto race = [&](int lo, int hi, bool less) {
