@@ -15,17 +15,19 @@
 //
 // Two kernels.  spec_stat_kernel reads every row once: a warp takes `blocks` times
 // 1024 logits, keeps each block in registers between its maximum and the sum of its
-// exponentials, the next one on its way, and leaves (max, sum) as the row's part.  spec_draw_kernel joins the partials,
-// decides how many drafts are kept (every CTA of the sequence for itself: a few KB
-// from L2) and races the one row that is drawn from; the sequence's last CTA to
+// exponentials, the next one on its way, and leaves (max, sum) as the row's part.
+// spec_draw_kernel joins the parts, decides how many drafts are kept (every CTA of the
+// sequence for itself: a few KB from L2) and races the one row that is drawn from; the sequence's last CTA to
 // finish writes its outputs.  HBM bounds both; the first also runs one exponential
 // per 2 bytes, about 0.7 of what the SMs' exponential units do in that time, so the
 // rest of its arithmetic is packed: the maximum in the 16-bit type itself, the
 // differences and sums two at a time.  Rows
 // are read last to first, so that the rows drawn from, mostly early ones, are the
-// ones left in L2.  64 x 7 drafts of 151936 tokens, bf16: 76 us, 4.3 TB/s (statistics 58
-// at 5.0 TB/s under ncu); 1 x 4 of 32000 8.4 us, the latency of two kernels.
+// ones left in L2.  64 x 7 drafts of 151936 tokens, bf16: 72 us, 4.6 TB/s (statistics 58
+// at 5.0 TB/s under ncu); 1 x 4 of 32000 8.1 us, the latency of two kernels.
 #pragma once
+#include <type_traits>
+
 #include "sm100.cuh"
 
 namespace simsd {
@@ -195,8 +197,8 @@ __device__ __forceinline__ const void* spec_row_ptr(const SpecVerifyArgs& p, int
 // Grid: x parts of a row, y sequences, z rows
 template <int DT>
 __global__ void __launch_bounds__(SV_THREADS, DT == 2 ? 3 : 4) spec_stat_kernel(const SpecVerifyArgs p) {
-  griddep_launch_dependents();
   griddep_wait();
+  griddep_launch_dependents();             // after it: the second kernel reads inputs before its own wait
   constexpr int N = SpecVec<DT>::N, VL = SV_BLOCK / N / 32;    // vectors per lane
   const int lane = threadIdx.x & 31, b = blockIdx.y, back = blockIdx.z;
   const int part = blockIdx.x * SV_WARPS + (threadIdx.x >> 5);
@@ -335,22 +337,50 @@ struct SpecBest {
 
 __device__ __forceinline__ float spec_rcp(float x) {
   float y;
-  asm("rcp.approx.f32 %0, %1;" : "=f"(y) : "f"(x));
+  asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
   return y;
 }
 
 // A row's probabilities: exp2((x - m) c) inv, 0 for an empty row (inv = 0)
 struct SpecLaw {
   float m, inv;
-  __device__ __forceinline__ float of(float x, float c) const {
-    return spec_exp2((spec_clean(x) - m) * c) * inv;
-  }
 };
 
+// p / e, or max(p - q, 0) / e, of a lane's run of N tokens.  The differences are taken two
+// at a time; the exponential is clamped to [0, 1], which makes NaN 0 and the +inf of a
+// row whose maximum is the largest finite number 1, as the cleaned logit would.
+template <int N, bool MINUS>
+__device__ __forceinline__ void spec_race(const float (&x)[N], const float (&y)[N], const float (&e)[N], SpecLaw pt,
+                                          SpecLaw pd, float c, float (&out)[N]) {
+  uint64_t cc, nt, nd;
+  asm("mov.b64 %0, {%1, %1};" : "=l"(cc) : "f"(c));
+  asm("mov.b64 %0, {%1, %1};" : "=l"(nt) : "f"(-pt.m));
+  asm("mov.b64 %0, {%1, %1};" : "=l"(nd) : "f"(-pd.m));
+  auto weight = [&](float a, float b, uint64_t nm, float& wa, float& wb) {
+    uint64_t d;
+    asm("mov.b64 %0, {%1, %2};" : "=l"(d) : "f"(a), "f"(b));
+    asm("add.rn.f32x2 %0, %0, %1;" : "+l"(d) : "l"(nm));
+    asm("mul.rn.f32x2 %0, %0, %1;" : "+l"(d) : "l"(cc));
+    asm("mov.b64 {%0, %1}, %2;" : "=f"(a), "=f"(b) : "l"(d));
+    wa = __saturatef(spec_exp2(a)), wb = __saturatef(spec_exp2(b));
+  };
+#pragma unroll
+  for (int k = 0; k < N; k += 2) {
+    float p[2], q[2];
+    weight(x[k], x[k + 1], nt, p[0], p[1]);
+    if constexpr (MINUS) weight(y[k], y[k + 1], nd, q[0], q[1]);
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+      float w = p[h] * pt.inv;
+      if constexpr (MINUS) w = fmaxf(w - q[h] * pd.inv, 0.0f);
+      out[k + h] = w * spec_rcp(e[k + h]);
+    }
+  }
+}
+
 template <int DT>
-__global__ void __launch_bounds__(SV_THREADS) spec_draw_kernel(const SpecVerifyArgs p) {
+__global__ void __launch_bounds__(SV_THREADS, 4) spec_draw_kernel(const SpecVerifyArgs p) {
   griddep_launch_dependents();
-  griddep_wait();
   constexpr int N = SpecVec<DT>::N;
   extern __shared__ SpecPart sv_rows[];            // [2 K + 1]
   __shared__ SpecBest s_best[SV_WARPS];
@@ -373,6 +403,9 @@ __global__ void __launch_bounds__(SV_THREADS) spec_draw_kernel(const SpecVerifyA
     }
   };
   if (warp == 0) fetch(lane);
+  // all that was read so far is input: the first kernel lets this one start after its own wait
+  const int lo = chunk * p.chunk, hi = min(p.V, lo + p.chunk);
+  griddep_wait();
   const int R = d + 1 + (p.draft ? d : 0);
   for (int k = SV_WARPS - 1 - warp; k < R; k += SV_WARPS) {
     const int r = k <= d ? k : p.K + k - d;
@@ -425,36 +458,56 @@ __global__ void __launch_bounds__(SV_THREADS) spec_draw_kernel(const SpecVerifyA
   const SpecLaw pd = dr ? law(p.K + 1 + a) : SpecLaw{0.0f, 0.0f};
   if (dr) pt.inv *= SV_OVER;
   SpecBest best = {-1.0f, 0x7fffffff};
+  const bool vectors = ((reinterpret_cast<uintptr_t>(tr) | reinterpret_cast<uintptr_t>(e) | reinterpret_cast<uintptr_t>(dr)) & 15) == 0;
   // tokens lo .. hi - 1, a thread's in ascending order
-  auto race = [&](int lo, int hi, bool less) {
-    auto see = [&](float x, float y, float noise, int v) {
-      const float q = less ? (dr ? pd.of(y, c) : v == hit ? 1.0f : 0.0f) : 0.0f;
-      best.see(fmaxf(pt.of(x, c) - q, 0.0f) * spec_rcp(noise), v);
-    };
-    auto aligned = [](const void* q) { return (reinterpret_cast<uintptr_t>(q) & 15) == 0; };
+  auto run = [&](int lo, int hi, int skip, auto minus_q) {
+    constexpr bool MINUS = decltype(minus_q)::value;
     int vec_hi = lo;
-    if (aligned(tr) && aligned(e) && (!dr || aligned(dr))) {
+    if (vectors) {
       vec_hi = hi - (hi - lo) % N;
-#pragma unroll 2
+#pragma unroll 1
       for (int v0 = lo + tid * N; v0 < vec_hi; v0 += SV_THREADS * N) {
-        float x[N], y[N], z[N];
-        SpecVec<DT>::unpack(__ldg(reinterpret_cast<const uint4*>(reinterpret_cast<const char*>(tr) + (long long)v0 * (16 / N))), x);
-        SpecVec<DT>::unpack(dr ? __ldg(reinterpret_cast<const uint4*>(reinterpret_cast<const char*>(dr) + (long long)v0 * (16 / N)))
-                               : make_uint4(0, 0, 0, 0), y);
+        float x[N], y[N], z[N], w[N];
+        const uint4 xr = __ldg(reinterpret_cast<const uint4*>(reinterpret_cast<const char*>(tr) + (long long)v0 * (16 / N)));
+        uint4 yr;
+        if constexpr (MINUS) yr = __ldg(reinterpret_cast<const uint4*>(reinterpret_cast<const char*>(dr) + (long long)v0 * (16 / N)));
 #pragma unroll
         for (int k = 0; k < N / 4; ++k) {
           const float4 f = __ldg(reinterpret_cast<const float4*>(e + v0) + k);
           z[4 * k] = f.x, z[4 * k + 1] = f.y, z[4 * k + 2] = f.z, z[4 * k + 3] = f.w;
         }
+        SpecVec<DT>::unpack(xr, x);
+        if constexpr (MINUS) SpecVec<DT>::unpack(yr, y);
+        spec_race<N, MINUS>(x, y, z, pt, pd, c, w);
+        if (!MINUS && (unsigned)(skip - v0) < (unsigned)N) {
 #pragma unroll
-        for (int k = 0; k < N; ++k) see(x[k], y[k], z[k], v0 + k);
+          for (int k = 0; k < N; ++k)
+            if (v0 + k == skip) w[k] = 0.0f;
+        }
+#pragma unroll
+        for (int k = 0; k < N; ++k) best.see(w[k], v0 + k);
       }
     }
-#pragma unroll 8
-    for (int v = vec_hi + tid; v < hi; v += SV_THREADS) see(load_f(tr, v, DT), dr ? load_f(dr, v, DT) : 0.0f, e[v], v);
+#pragma unroll 4
+    for (int v = vec_hi + tid; v < hi; v += 2 * SV_THREADS) {
+      const int v2 = v + SV_THREADS < hi ? v + SV_THREADS : v;
+      const float x[2] = {load_f(tr, v, DT), load_f(tr, v2, DT)}, z[2] = {e[v], e[v2]};
+      float y[2], w[2];
+      if constexpr (MINUS) y[0] = load_f(dr, v, DT), y[1] = load_f(dr, v2, DT);
+      spec_race<2, MINUS>(x, y, z, pt, pd, c, w);
+      best.see(v == skip ? 0.0f : w[0], v);
+      best.see(v2 == skip ? 0.0f : w[1], v2);
+    }
+  };
+  // p, p without the refused token (q one there: max(p - q, 0) is 0), or p - q
+  auto race = [&](int lo, int hi, bool less) {
+    if (less && dr)
+      run(lo, hi, -1, std::true_type());
+    else
+      run(lo, hi, less ? hit : -1, std::false_type());
   };
   if (c != 0.0f) {
-    race(chunk * p.chunk, min(p.V, (chunk + 1) * p.chunk), minus);
+    race(lo, hi, minus);
     best.join_warp();
     if (lane == 0) s_best[warp] = best;
     __syncthreads();
