@@ -20,17 +20,18 @@
 // Warps 0-3 softmax and epilogue, 4-7 loads into a ring of NS operand tiles K, V, K,
 // V, ..., 8 issues the products: S of unit n + 1 before O of unit n, so that they
 // overlap its softmax.  One CTA per SM.  Pages of a multiple of 8 tokens are loaded
-// with TMA, a lane per run of `block` tokens that lies in one page (warp 4); other
-// pages with cp.async into the same swizzled layout (warps 4-7), where handing a tile
-// to the tensor cores waits for the copies behind it too (58 us against 47 with TMA).
+// with TMA, a lane per run of `block` tokens that lies in one page, spread over warps
+// 4-7 (by one warp alone 16 x 8 rows take 54 us with pages of 8, 39.5 with 16; by four
+// 37 each); other pages with cp.async into the same swizzled layout (41 us, pages of 1,
+// 4 and 12).  At 2 x 64k x 8 rows TMA takes 91-92 us and cp.async 95 with pages of 8 to
+// 128; with 64 dims and pages of 8 TMA is behind, 120 against 117 at 4 x 64k.
 //
 // A value that is not finite, of a key that some rows do not see, is taken out of the
 // product and added to the rows that see it by themselves.  All waits are bounded.
 //
 // Measured (B200, 8 KV heads x 128, 4 query heads each, bf16): 16 x 1-3k tokens x 8 rows
-// 39.5 us, 3.5 TB/s; 2 x 64k x 8 rows 103 us, 5.0 TB/s with pages of 16 tokens; in an
-// earlier state 109 with 16, 97.5 with 32, fewer TMA boxes.  64 and 128 rows, with R keys
-// a softmax thread: 16 x 1-3k 50 and 88 us.
+// 36.5 us, 3.8 TB/s; 2 x 64k x 8 rows 91 us, 5.6 TB/s, 86 % of the measured copy rate.
+// 64 and 128 rows, with R keys a softmax thread: 16 x 1-3k 50 and 76 us.
 #pragma once
 #include "paged_attn.cuh"
 
@@ -186,9 +187,10 @@ __global__ void __launch_bounds__(PTC_THREADS, 1) paged_attention_tc_kernel(cons
   __shared__ PagedCut s_range;
   __shared__ bool s_join[2];
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+  const int runs = args.block ? PTC_TK / args.block : 0, loaders = min(4, runs);   // powers of two
 
   if (tid == 0) {
-    for (int s = 0; s < NS; ++s) mbar_init(smem_u32(full + s), args.block ? 1 : 128), mbar_init(smem_u32(empty + s), 1);
+    for (int s = 0; s < NS; ++s) mbar_init(smem_u32(full + s), args.block ? loaders : 128), mbar_init(smem_u32(empty + s), 1);
     mbar_init(smem_u32(q_full), PTC_SOFTMAX);
     mbar_init(smem_u32(s_full), 1);
     mbar_init(smem_u32(s_full + 1), 1);
@@ -217,22 +219,24 @@ __global__ void __launch_bounds__(PTC_THREADS, 1) paged_attention_tc_kernel(cons
   if (mine) {
     const int end = cut.first(blockIdx.x + 1);
     if (tid == 0) s_range = cut;
-    if (args.block && warp == 4) {
-      // ================= loads of keys and values by TMA: a lane per `block` tokens of the unit
+    if (args.block && warp >= 4 && warp < 4 + loaders) {
+      // ================= loads of keys and values by TMA: a lane per `block` tokens of the
+      // unit, its runs spread over up to four warps (a warp issues its lanes' boxes one
+      // after the other)
       uint32_t slot = 0, phase = 0;
-      const int runs = PTC_TK / args.block, first_key = lane * args.block;
+      const int own = runs / loaders, first_key = ((warp - 4) * own + lane) * args.block;
       const uint64_t policy = policy_evict_first();
       if (lane == 0) prefetch_tmap(&args.k), prefetch_tmap(&args.v);
       // the page of the lane's run; one past the last (which loads zeros) where it holds no key
       auto run_page = [&](const PagedPos<PTC_TK>& x) {
         const int key = x.unit * PTC_TK + first_key;
-        return lane < runs && key < x.n ? p.page_table[x.b * p.ld_table + p.page_div(key)] : p.num_pages;
+        return lane < own && key < x.n ? p.page_table[x.b * p.ld_table + p.page_div(key)] : p.num_pages;
       };
       int page = run_page(at);
       uint32_t filled = 0, parity = 0;           // tiles with a load in flight, and its phase
       bool ok = true;
       while (ok && at.w < end) {
-        if (page < 0 || page > p.num_pages || (page == p.num_pages && lane < runs && at.unit * PTC_TK + first_key < at.n)) {
+        if (page < 0 || page > p.num_pages || (page == p.num_pages && lane < own && at.unit * PTC_TK + first_key < at.n)) {
           if (p.err) atomicOr(p.err, SIMSD_DEV_ERR_BAD_INDEX);
           page = p.num_pages;
         }
@@ -243,9 +247,9 @@ __global__ void __launch_bounds__(PTC_THREADS, 1) paged_attention_tc_kernel(cons
           ok = __all_sync(0xffffffffu, mbar_wait(smem_u32(empty + slot), phase ^ 1, abort_flag, p.err));
           if (!ok) break;
           const uint32_t bar = smem_u32(full + slot), dst = smem_u32(ring) + slot * S::TILE + first_key * 128;
-          if (lane == 0) mbar_arrive_expect_tx(bar, S::TILE);
+          if (lane == 0) mbar_arrive_expect_tx(bar, S::TILE / loaders);
           __syncwarp();
-          if (lane < runs) {
+          if (lane < own) {
             const void* map = kv ? &args.v : &args.k;
 #pragma unroll
             for (int x = 0; x < D / 64; ++x) ptc_tma(dst + x * 16384, map, bar, x * 64, tok, head, now, policy);
@@ -255,12 +259,14 @@ __global__ void __launch_bounds__(PTC_THREADS, 1) paged_attention_tc_kernel(cons
           if (++slot == NS) slot = 0, phase ^= 1;
         }
       }
-      if (!ok && lane == 0)                      // giving up: no copy may land after the CTA has left
+      // giving up: no copy may land after the CTA has left (where another warp gave up
+      // first, the tile's phase stays open and the wait's limit outlasts the copies)
+      if (!ok && lane == 0)
         for (int s = 0; s < NS; ++s)
           if (filled >> s & 1) mbar_wait_drain(smem_u32(full + s), parity >> s & 1, 100000000ull);
       __syncwarp();
-    } else if (args.block && warp > 4 && warp < 8) {
-      // warps 5-7 load only where TMA does not
+    } else if (args.block && warp >= 4 && warp < 8) {
+      // no run left for this warp
     } else if (warp >= 4 && warp < 8) {
       // ================= loads by cp.async
       const int lt = tid - 128, lw = warp - 4, kc = lane % CH, khi = lane / CH;
