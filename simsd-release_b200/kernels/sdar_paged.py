@@ -28,19 +28,23 @@ from .thin_linear_fused import thin_linear_cat
 
 
 class PagedBatch:
-    """`sequences` sequences of up to `max_len` tokens over one model.
+    """`sequences` sequences of up to `max_len` tokens (rounded up to whole pages) over one model.
 
-    Pages are handed out at construction, `max_len` tokens' worth to each sequence;
-    `page_table` may be edited between steps by a caller that allocates as it goes.
+    Pages are handed out at construction, `max_len` + `max_drafts` tokens' worth to each
+    sequence: the places after `max_len` take the keys of drafted tokens that a step near
+    the end has no room to keep, so that its queries and keys stay aligned.
+    `page_table` may be edited between steps by a caller that allocates as it goes, as long
+    as it covers `lens` + K + 1 tokens of every sequence that a step moves on.
     `lens` counts the tokens whose keys and values are in the cache; `last` is each
     sequence's newest token, which is not there yet.
     """
 
     def __init__(self, model: SDARVerifyModel, sequences: int, max_len: int, page_size: int = 16,
-                 tail_mask: torch.Tensor | None = None):
+                 tail_mask: torch.Tensor | None = None, max_drafts: int = 31):
         s, p = model.s, next(model.parameters())
         self.model, self.page_size, self.tail_mask = model, page_size, tail_mask
-        per = -(-max_len // page_size)
+        self.max_len = -(-max_len // page_size) * page_size
+        per = -(-(self.max_len + max_drafts) // page_size)
         self.page_table = torch.arange(sequences * per, dtype=torch.int32, device=p.device).view(sequences, per)
         shape = (sequences * per, s.kv_heads, page_size, s.head_dim)
         self.caches = [(torch.zeros(shape, dtype=p.dtype, device=p.device), torch.zeros(shape, dtype=p.dtype, device=p.device))
@@ -86,7 +90,7 @@ class PagedBatch:
         dev = self.lens.device
         if len(prompts) != self.lens.numel() or min(map(len, prompts)) < 1:
             raise ValueError(f"{self.lens.numel()} prompts of at least one token each")
-        if max(map(len, prompts)) > self.page_table.shape[1] * self.page_size:
+        if max(map(len, prompts)) > self.max_len:
             raise ValueError("a prompt is longer than max_len")
         self.lens.zero_()
         with torch.inference_mode():
@@ -103,16 +107,28 @@ class PagedBatch:
              draft_logits: torch.Tensor | None = None, temperature: torch.Tensor | None = None,
              n_draft: torch.Tensor | None = None):
         """Verify drafts [B, K] (int64; see `speculative_verify` for the rest) and move on:
-        (tokens [B, K + 1], accepted [B], logprobs [B, K + 1]).  K = 0 decodes plainly."""
+        (tokens [B, K + 1], accepted [B], logprobs [B, K + 1]).  K = 0 decodes plainly.
+
+        A sequence keeps no more drafts than `max_len` leaves room for.  One that is full
+        (lens = max_len, or fewer than K + 1 places left in the table, which only K >
+        `max_drafts` brings about) stays as it is: its tokens are -1, accepted and logprobs 0."""
         with torch.inference_mode():
             ids = torch.cat([self.last[:, None], drafts.clamp(min=0)], 1)
             B, L = ids.shape
-            x = self.hidden(ids, tail_mask=self.tail_mask)
+            if n_draft is not None and n_draft.shape != (B,):
+                raise ValueError(f"n_draft must be [{B}]")
+            room = self.max_len - self.lens
+            full = (room <= 0) | (self.lens + L > self.page_table.shape[1] * self.page_size)
+            keep = (room - 1).clamp(0, L - 1)
+            keep = keep if n_draft is None else torch.minimum(keep, n_draft)
+            x = self.hidden(ids, torch.where(full, 0, L), self.tail_mask)
             logits = self.model.lm_head(x.view(B * L, -1)).view(B, L, -1)
-            tokens, accepted, logprobs = speculative_verify(logits, drafts, uniform, noise, draft_logits, temperature,
-                                                            n_draft)
-            self.last.copy_(tokens.gather(1, accepted[:, None])[:, 0])
-            self.lens += (accepted + 1).to(torch.int32)
+            tokens, accepted, logprobs = speculative_verify(logits, drafts, uniform, noise, draft_logits, temperature, keep)
+            self.last.copy_(torch.where(full, self.last, tokens.gather(1, accepted[:, None])[:, 0]))
+            self.lens += torch.where(full, 0, accepted + 1).to(torch.int32)
+            tokens.masked_fill_(full[:, None], -1)
+            accepted.masked_fill_(full, 0)
+            logprobs.masked_fill_(full[:, None], 0.0)
         return tokens, accepted, logprobs
 
 
