@@ -545,7 +545,8 @@ int simsd_paged_attention(const void* q, const void* k_cache, const void* v_cach
  * Speculative sampling's verification from given random numbers.  For sequence b
  * with d = n_draft[b] (K when NULL) drafted tokens x_i, p_i = softmax(target row i
  * / T) and q_i = softmax(draft row i / T) (draft_logits NULL: one at x_i), T =
- * temperature[b] (1 when NULL; 0: one at the row's first maximum):
+ * temperature[b] (1 when NULL; 0: one at the row's first maximum; inf: uniform over the
+ * logits that are not -inf):
  *   x_i is kept while uniform[b, i] q_i(x_i) < p_i(x_i); at the first one refused
  *   the next token is argmax_v max(p - q, 0)(v) / noise[b, v], after d kept ones
  *   argmax_v p_d(v) / noise[b, v]  (noise positive, exponentially distributed;

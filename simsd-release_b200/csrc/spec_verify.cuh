@@ -8,7 +8,7 @@
 //   argmax_v p_d(v) / e(v), with e exponential noise: of independent exponential
 //   variables e(v) / w(v) the smallest is v's with probability w(v) / sum w, so
 //   this draws from the (residual) distribution without a running sum.
-// T = 0: p and q are one at their first maximum.  NaN logits count as -inf,
+// T = 0: p and q are one at their first maximum; T = inf: alike at every logit over -inf.  NaN logits count as -inf,
 // +inf as the largest finite number; a row without any finite logit has p = 0.
 // Ties go to the lowest token.  A residual that is nowhere positive (p <= q
 // everywhere, to 2^-21 of p) draws from p.
@@ -79,8 +79,12 @@ __device__ __forceinline__ int spec_count(const SpecVerifyArgs& p, int b) {
 __device__ __forceinline__ float spec_temperature(const SpecVerifyArgs& p, int b) {
   return p.temperature ? p.temperature[b] : 1.0f;
 }
-// log2(e) / T, what a difference of logits is multiplied with; 0 for greedy sequences
-__device__ __forceinline__ float spec_scale(float T) { return T > 0.0f ? 1.4426950408889634f / fmaxf(T, 1e-30f) : 0.0f; }
+// log2(e) / T, what a difference of logits is multiplied with; 0 for greedy sequences only
+// (an infinite T takes the smallest positive number: differences of finite logits come to
+// nothing, -inf stays)
+__device__ __forceinline__ float spec_scale(float T) {
+  return T > 0.0f ? fmaxf(1.4426950408889634f / fmaxf(T, 1e-30f), 1.4e-45f) : 0.0f;
+}
 __device__ __forceinline__ float spec_exp2(float x) {
   float y;
   asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));

@@ -63,7 +63,8 @@ def speculative_verify(target_logits: torch.Tensor, draft_tokens: torch.Tensor, 
     probabilities (greedy ones).  uniform [B, K] fp32 in [0, 1): accepts token i
     where uniform * q_i < p_i.  noise [B, V] fp32, positive, exponentially
     distributed: draws the token after the accepted ones from max(p - q, 0), or
-    from p after the last one.  temperature [B] fp32: 1 when None, 0 = greedy.
+    from p after the last one.  temperature [B] fp32: 1 when None, 0 = greedy,
+    inf = uniform over the tokens whose logit is not -inf.
     n_draft [B] int32: drafted tokens of each sequence (<= K; K when None); the
     rows after them are not read.
 
