@@ -27,7 +27,10 @@
 // 128; with 64 dims and pages of 8 TMA is behind, 120 against 117 at 4 x 64k.
 //
 // A value that is not finite, of a key that some rows do not see, is taken out of the
-// product and added to the rows that see it by themselves.  All waits are bounded.
+// product and added to the rows that see it by themselves.  One that all rows see stays,
+// and makes NaN of the sums of the copies that do not keep its key (P = 0 there): where the
+// copies of a row join to no finite number, what the row's keys hold says which it is.
+// All waits are bounded.
 //
 // Measured (B200, 8 KV heads x 128, 4 query heads each, bf16): 16 x 1-3k tokens x 8 rows
 // 36.5 us, 3.8 TB/s; 2 x 64k x 8 rows 91 us, 5.6 TB/s, 86 % of the measured copy rate.
@@ -165,6 +168,31 @@ __device__ void ptc_join(const PagedAttnArgs& p, const PagedPart& x, float2* buf
             make_uint2(pat_pack<BF>(a[u].x, a[u].y), pat_pack<BF>(a[u].z, a[u].w));
   }
   __syncthreads();
+}
+
+// What four dims (from d) of row `row` come to where a sum of its copies is not finite: by the
+// values of its visible keys lo .. hi - 1, which weigh in with positive numbers.  +inf or
+// -inf where they hold no other value that is not finite, else NaN; `a` where they hold
+// none.  Off the product's path, and slow (a key at a time).
+template <int D, bool BF>
+__device__ __noinline__ float4 ptc_settle(const PagedAttnArgs& p, int b, int g, int n, int row, int lo, int hi, int d, float4 a) {
+  float v[4] = {a.x, a.y, a.z, a.w}, sum[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+  if (isfinite((v[0] + v[1]) + (v[2] + v[3]))) return a;
+  for (int j = lo; j < hi; ++j) {
+    if (!paged_visible(p, b, n, j, row)) continue;
+    const int page = p.page_table[b * p.ld_table + p.page_div(j)];
+    if (page < 0 || page >= p.num_pages) continue;
+    const long long off = page * p.ld_page + g * p.ld_head + (j - p.page_div(j) * p.page_size) * p.ld_tok + d;
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+      const float x = load_f(p.v_cache, off + e, BF ? 0 : 1);
+      if (!isfinite(x)) sum[e] += x;
+    }
+  }
+#pragma unroll
+  for (int e = 0; e < 4; ++e)
+    if (!isfinite(v[e]) && sum[e] != 0.0f) v[e] = sum[e];
+  return make_float4(v[0], v[1], v[2], v[3]);
 }
 
 template <int D, int R, bool BF>
@@ -674,17 +702,37 @@ __global__ void __launch_bounds__(PTC_THREADS, 1) paged_attention_tc_kernel(cons
             }
             if constexpr (F > 1) {
               named_bar_sync(1, PTC_SOFTMAX);
-#pragma unroll
-              for (int k = 0; k < R * 16 / PTC_SOFTMAX; ++k) {
-                const int x = tid + k * PTC_SOFTMAX, r = x / 16, q4 = x % 16;
+              auto joined = [&](int r, int q4) {
                 float4 a = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
 #pragma unroll
                 for (int i = 0; i < F; ++i) {
                   const float4 y = *reinterpret_cast<const float4*>(own_x + ptc_off(i * R + r, q4));
                   a.x += y.x, a.y += y.y, a.z += y.z, a.w += y.w;
                 }
+                return a;
+              };
+              float4 nul = make_float4(0.0f, 0.0f, 0.0f, 0.0f);   // NaN where a sum is not finite
+#pragma unroll
+              for (int k = 0; k < R * 16 / PTC_SOFTMAX; ++k) {
+                const int x = tid + k * PTC_SOFTMAX, r = x / 16, q4 = x % 16;
+                const float4 a = joined(r, q4);
+                nul.x = fmaf(a.x, 0.0f, nul.x), nul.y = fmaf(a.y, 0.0f, nul.y);
+                nul.z = fmaf(a.z, 0.0f, nul.z), nul.w = fmaf(a.w, 0.0f, nul.w);
                 put(r, h * 16 + q4, a);
               }
+              if (isnan((nul.x + nul.y) + (nul.z + nul.w))) {
+#pragma unroll 1
+                for (int x = tid; x < R * 16; x += PTC_SOFTMAX) {
+                  const int r = x / 16, q4 = x % 16;
+                  bool scored = r0 + r < p.rows;           // NaN scores leave NaN
+                  for (int i = 0; i < F; ++i) scored &= !isnan(xl[i * R + r]);
+                  if (scored)
+                    put(r, h * 16 + q4,
+                        ptc_settle<D, BF>(p, at.b, at.g, at.n, r0 + r, first_unit * PTC_TK, min(at.n, (at.unit + 1) * PTC_TK),
+                                          h * 64 + q4 * 4, joined(r, q4)));
+                }
+              }
+              __syncwarp();
               named_bar_sync(1, PTC_SOFTMAX);
             }
           }
