@@ -34,7 +34,9 @@ namespace simsd {
 
 // What a part of a row comes to.  A likely token leaves a sum of 1 and a little,
 // whose logarithm is that little: the sums of lanes and parts are joined in 64 bits
-// (and a lane's run in eight 32-bit ones), so that log p keeps its relative precision.
+// (a lane's own, in eight 32-bit runs, are taken apart where the 1 outweighs the rest), so
+// that log p keeps its relative precision: the exponentials' arguments, 2^-23 of the
+// difference to the maximum, and 2^-16 at most of the runs.
 struct SpecPart {
   double s;                 // sum of exp((x - m) / T)
   float m;                  // maximum
@@ -145,9 +147,9 @@ __device__ __forceinline__ float spec_max(const uint4 (&raw)[VL]) {
 }
 
 // Sum of exp2((x - m) c) over a lane's vectors, two values an instruction but for
-// the exponential
+// the exponential; `near` is the same in 32 bits
 template <int DT, int VL>
-__device__ __forceinline__ double spec_sum(const uint4 (&raw)[VL], float m, float c) {
+__device__ __forceinline__ double spec_sum(const uint4 (&raw)[VL], float m, float c, float& near) {
   uint64_t nm, cc, sum[4] = {0, 0, 0, 0};
   asm("mov.b64 %0, {%1, %1};" : "=l"(nm) : "f"(-m));
   asm("mov.b64 %0, {%1, %1};" : "=l"(cc) : "f"(c));
@@ -173,6 +175,7 @@ __device__ __forceinline__ double spec_sum(const uint4 (&raw)[VL], float m, floa
   float a, b, c2, d;
   asm("mov.b64 {%0, %1}, %2;" : "=f"(a), "=f"(b) : "l"(sum[0]));
   asm("mov.b64 {%0, %1}, %2;" : "=f"(c2), "=f"(d) : "l"(sum[2]));
+  near = (a + b) + (c2 + d);
   return ((double)a + b) + ((double)c2 + d);
 }
 
@@ -204,6 +207,7 @@ __global__ void __launch_bounds__(SV_THREADS, DT == 2 ? 3 : 4) spec_stat_kernel(
   griddep_wait();
   griddep_launch_dependents();             // after it: the second kernel reads inputs before its own wait
   constexpr int N = SpecVec<DT>::N, VL = SV_BLOCK / N / 32;    // vectors per lane
+  static_assert(VL * N == 32);
   const int lane = threadIdx.x & 31, b = blockIdx.y, back = blockIdx.z;
   const int part = blockIdx.x * SV_WARPS + (threadIdx.x >> 5);
   // rows last to first: target K, then target and draft K - 1, ...
@@ -267,7 +271,8 @@ __global__ void __launch_bounds__(SV_THREADS, DT == 2 ? 3 : 4) spec_stat_kernel(
       }
       continue;
     }
-    double add = spec_sum<DT, VL>(raw, m, c);
+    float near;
+    double add = spec_sum<DT, VL>(raw, m, c, near);
     if (!(add < INFINITY)) {                             // NaN or +inf among the lane's logits
       add = 0.0;
 #pragma unroll
@@ -276,6 +281,18 @@ __global__ void __launch_bounds__(SV_THREADS, DT == 2 ? 3 : 4) spec_stat_kernel(
         SpecVec<DT>::unpack(raw[i], f);
 #pragma unroll
         for (int e = 0; e < N; ++e) add += spec_exp2((spec_clean(f[e]) - m) * c);
+      }
+    }
+    if (m2 == m) {
+      // A likely token: in the run of the maximum's 1 the others, of little weight beside it,
+      // lose their last bits (four roundings of 2^-24), which log p is made of.  Where they
+      // come to less than 2^-6, the lanes share that lane's logits out, one each (read
+      // again: kept in registers they cost 17 us at 64 x 7; up to 2^-3 2 us more).
+      for (uint32_t likely = __ballot_sync(0xffffffffu, near >= 1.0f && near < 1.015625f); likely; likely &= likely - 1) {
+        const int other = __ffs(likely) - 1, vi = v + lane / N * 32 + other;
+        if (lane == other) add = 0.0;
+        const float one = vi < row.nvec ? spec_logit(x, row.head + (long long)vi * N + lane % N, DT) : -INFINITY;
+        s += spec_exp2((one - m) * c);
       }
     }
     s += add;
