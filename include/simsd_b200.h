@@ -557,6 +557,8 @@ int simsd_paged_attention(const void* q, const void* k_cache, const void* v_cach
  * draft_tokens [B, K] (ld_x), uniform [B, K] (ld_u), noise [B, V] (ld_n).  NaN
  * logits count as -inf, +inf as the largest finite number.  A drafted token
  * outside [0, V) is refused (SIMSD_DEV_ERR_BAD_INDEX), the next one drawn from p.
+ * Noise that no token wins with (NaN throughout) gives token 0 and
+ * SIMSD_DEV_ERR_BAD_INDEX.
  * B <= 65535, K <= 1024 (more: SIMSD_ERR_UNSUPPORTED).  Replaces mrs_verify
  * (speculative_decoding/mrs.py:14-108) for a batch.
  */

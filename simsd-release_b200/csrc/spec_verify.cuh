@@ -566,6 +566,11 @@ __global__ void __launch_bounds__(SV_THREADS, 4) spec_draw_kernel(const SpecVeri
       for (int w = 0; w < SV_WARPS; ++w) best.join(s_best[w].v, s_best[w].at);
     }
     drawn = best.at;
+    // no token won (noise that is NaN throughout, say): nothing is read for such an index
+    if ((unsigned)drawn >= (unsigned)p.V) {
+      drawn = 0;
+      if (tid == 0 && p.err) atomicOr(p.err, SIMSD_DEV_ERR_BAD_INDEX);
+    }
   }
   if (warp != 0) return;
   for (int i = lane; i <= p.K; i += 32) {

@@ -72,7 +72,8 @@ def speculative_verify(target_logits: torch.Tensor, draft_tokens: torch.Tensor, 
     target's log probability of each, 0 after them.  Logits bf16, fp16 or fp32;
     NaN counts as -inf, +inf as the largest finite number; ties go to the lowest
     token.  A drafted token outside [0, V) is refused, the next one drawn from p,
-    and DEV_ERR_BAD_INDEX raised in `_lib.device_error()`.
+    and DEV_ERR_BAD_INDEX raised in `_lib.device_error()`; so it is, with token 0, where
+    no token wins (a noise row of NaN).
     """
     out = _lib.binding().speculative_verify(target_logits, draft_tokens, uniform, noise, draft_logits, temperature, n_draft)
     if out is not None:
