@@ -92,6 +92,8 @@ class PagedBatch:
             raise ValueError(f"{self.lens.numel()} prompts of at least one token each")
         if max(map(len, prompts)) > self.max_len:
             raise ValueError("a prompt is longer than max_len")
+        if not all(0 <= t < self.model.s.vocab for p in prompts for t in p):
+            raise ValueError(f"a prompt has a token outside the vocabulary of {self.model.s.vocab}")
         self.lens.zero_()
         with torch.inference_mode():
             for c in range(0, max(map(len, prompts)) - 1, chunk):
@@ -113,7 +115,8 @@ class PagedBatch:
         (lens = max_len, or fewer than K + 1 places left in the table, which only K >
         `max_drafts` brings about) stays as it is: its tokens are -1, accepted and logprobs 0."""
         with torch.inference_mode():
-            ids = torch.cat([self.last[:, None], drafts.clamp(min=0)], 1)
+            # ids outside the vocabulary are speculative_verify's to refuse, not the embedding's to read
+            ids = torch.cat([self.last[:, None], drafts.clamp(0, self.model.s.vocab - 1)], 1)
             B, L = ids.shape
             if n_draft is not None and n_draft.shape != (B,):
                 raise ValueError(f"n_draft must be [{B}]")
