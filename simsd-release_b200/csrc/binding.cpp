@@ -40,17 +40,29 @@ struct {
   PyObject* stream_scratch = nullptr;   // _lib.stream_scratch
 } g;
 
+// Scratch of a stream; holds its owner
 struct Scratch {
-  char* at;
-  size_t bytes;
-  PyObject* owner;
+  char* at = nullptr;
+  size_t bytes = 0;
+  PyObject* owner = nullptr;
+  Scratch() = default;
+  Scratch(char* a, size_t n, PyObject* o) : at(a), bytes(n), owner(o) { Py_XINCREF(owner); }
+  Scratch(const Scratch& s) : Scratch(s.at, s.bytes, s.owner) {}
+  Scratch& operator=(Scratch s) {
+    std::swap(at, s.at);
+    std::swap(bytes, s.bytes);
+    std::swap(owner, s.owner);
+    return *this;
+  }
+  ~Scratch() { Py_XDECREF(owner); }
 };
-std::map<std::pair<int, cudaStream_t>, Scratch> g_scratch;
+using ScratchMap = std::map<std::pair<int, cudaStream_t>, Scratch>;
+ScratchMap& g_scratch = *new ScratchMap;   // never destroyed: the interpreter may be gone by then
 int* g_error[64];
 
 void forget_all() {
-  for (auto& s : g_scratch) Py_DECREF(s.second.owner);
-  g_scratch.clear();
+  ScratchMap old;                          // owners go once nothing refers to them
+  old.swap(g_scratch);
   for (auto& e : g_error) e = nullptr;
 }
 
@@ -66,22 +78,19 @@ int* error_word(int dev) {
   return g_error[dev];
 }
 
-// Scratch of the stream; nullptr with a Python error set
-const Scratch* scratch(int dev, cudaStream_t stream, size_t bytes) {
-  auto it = g_scratch.find({dev, stream});
-  if (it != g_scratch.end() && it->second.bytes >= bytes) return &it->second;
+// Scratch of the stream; without an address, and with a Python error set, where there is
+// none.  The Python function may let other threads in, and they ask for scratch or forget
+// it: nothing of the map is kept over the call.
+Scratch scratch(int dev, cudaStream_t stream, size_t bytes) {
+  const auto it = g_scratch.find({dev, stream});
+  if (it != g_scratch.end() && it->second.bytes >= bytes) return it->second;
   PyObject* r = PyObject_CallFunction(g.stream_scratch, "iKni", dev, (unsigned long long)(uintptr_t)stream,
                                       (Py_ssize_t)bytes, SIMSD_PAGED_COUNTER_BYTES);
-  if (r == nullptr) return nullptr;
-  if (it != g_scratch.end()) {
-    Py_DECREF(it->second.owner);
-    g_scratch.erase(it);
-  }
-  Scratch s;
-  s.at = reinterpret_cast<char*>(PyLong_AsVoidPtr(PyTuple_GetItem(r, 0)));
-  s.bytes = PyLong_AsSize_t(PyTuple_GetItem(r, 1));
-  s.owner = r;
-  return &(g_scratch[{dev, stream}] = s);
+  if (r == nullptr) return {};
+  const Scratch s(reinterpret_cast<char*>(PyLong_AsVoidPtr(PyTuple_GetItem(r, 0))), PyLong_AsSize_t(PyTuple_GetItem(r, 1)), r);
+  Py_DECREF(r);
+  g_scratch[{dev, stream}] = s;
+  return s;
 }
 
 // A request's tensors and numbers, and whether all of them are what is wanted
@@ -214,14 +223,14 @@ PyObject* attention(PyObject*, PyObject* const* args, Py_ssize_t n) {
   if (!r.here(stream) || c10::cuda::currentStreamCaptureStatusMayInitCtx() != c10::cuda::CaptureStatus::None) return none();
   int* err = error_word(r.dev);
   if (err == nullptr) return PyErr_Occurred() ? nullptr : none();
-  const Scratch* ws = scratch(r.dev, stream, g.attention_bytes((int)L, (int)Hq, (int)Hk, (int)D));
-  if (ws == nullptr) return nullptr;
+  const Scratch ws = scratch(r.dev, stream, g.attention_bytes((int)L, (int)Hq, (int)Hk, (int)D));
+  if (ws.at == nullptr) return nullptr;
   at::Tensor o = at::empty(q->sizes(), q->options()), lse;
   if (with_lse) lse = at::empty(q->sizes().slice(0, q->dim() - 1), q->options().dtype(at::kFloat));
   const int rc = g.attention(ptr(q), ptr(k), ptr(v), (int)k->size(0), (int)k->size(2), k->stride(0), k->stride(1), k->stride(2),
                              ptr<int32_t>(table), table->stride(0), (int)table->size(1), ptr<int32_t>(lens),
                              ptr<uint8_t>(tail), ldm_b, ldm_t, (int)B, (int)L, (int)Hq, (int)Hk, (int)D, (float)scale,
-                             o.data_ptr(), with_lse ? lse.data_ptr<float>() : nullptr, code, ws->at, ws->bytes, err, stream);
+                             o.data_ptr(), with_lse ? lse.data_ptr<float>() : nullptr, code, ws.at, ws.bytes, err, stream);
   if (rc != SIMSD_OK) return none();
   if (!with_lse) return THPVariable_Wrap(std::move(o));
   PyObject* out = PyTuple_New(2);
@@ -254,8 +263,8 @@ PyObject* verify(PyObject*, PyObject* const* args, Py_ssize_t n) {
   int* err = error_word(r.dev);
   if (err == nullptr) return PyErr_Occurred() ? nullptr : none();
   const size_t skip = SIMSD_PAGED_COUNTER_BYTES;       // the attention's counters
-  const Scratch* ws = scratch(r.dev, stream, g.verify_bytes((int)B, (int)K, (int)V) + skip);
-  if (ws == nullptr) return nullptr;
+  const Scratch ws = scratch(r.dev, stream, g.verify_bytes((int)B, (int)K, (int)V) + skip);
+  if (ws.at == nullptr) return nullptr;
   if (K == 0) draft = nullptr;
   at::Tensor tokens = at::empty({B, R}, target->options().dtype(at::kLong)),
              accepted = at::empty({B}, target->options().dtype(at::kLong)),
@@ -263,8 +272,8 @@ PyObject* verify(PyObject*, PyObject* const* args, Py_ssize_t n) {
   const int rc = g.verify(ptr(target), target->stride(0), target->stride(1), ptr(draft), draft ? draft->stride(0) : 0,
                           draft ? draft->stride(1) : 0, ptr<int64_t>(x), x->stride(0), ptr<float>(u), u->stride(0),
                           ptr<float>(e), e->stride(0), ptr<float>(temp), ptr<int32_t>(count), (int)B, (int)K, (int)V, code,
-                          tokens.data_ptr<int64_t>(), accepted.data_ptr<int64_t>(), logprobs.data_ptr<float>(), ws->at + skip,
-                          ws->bytes - skip, err, stream);
+                          tokens.data_ptr<int64_t>(), accepted.data_ptr<int64_t>(), logprobs.data_ptr<float>(), ws.at + skip,
+                          ws.bytes - skip, err, stream);
   if (rc != SIMSD_OK) return none();
   PyObject* out = PyTuple_New(3);
   if (out == nullptr) return nullptr;
@@ -303,9 +312,21 @@ PyObject* forget(PyObject*, PyObject*) {
   Py_RETURN_NONE;
 }
 
+// scratch(device, stream, bytes) -> (address, bytes) that the operators would get
+PyObject* scratch_of(PyObject*, PyObject* args) {
+  int dev;
+  unsigned long long stream;
+  Py_ssize_t bytes;
+  if (!PyArg_ParseTuple(args, "iKn", &dev, &stream, &bytes)) return nullptr;
+  const Scratch s = scratch(dev, reinterpret_cast<cudaStream_t>((uintptr_t)stream), (size_t)bytes);
+  if (s.at == nullptr) return nullptr;
+  return Py_BuildValue("Kn", (unsigned long long)reinterpret_cast<uintptr_t>(s.at), (Py_ssize_t)s.bytes);
+}
+
 PyMethodDef methods[] = {
     {"bind", bind, METH_VARARGS, nullptr},
     {"forget", forget, METH_NOARGS, nullptr},
+    {"scratch", scratch_of, METH_VARARGS, nullptr},
     {"paged_append", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(append)), METH_FASTCALL, nullptr},
     {"paged_attention", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(attention)), METH_FASTCALL, nullptr},
     {"speculative_verify", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(verify)), METH_FASTCALL, nullptr},
