@@ -116,6 +116,13 @@ def lib() -> ctypes.CDLL:
             fn = getattr(L, name)
             fn.restype = res
             fn.argtypes = args
+        # Over the streams' scratch, the GIL orders one thread's calls with another's (the
+        # native binding holds it too): a verification is two launches on the same bytes.
+        held = ctypes.PyDLL(str(LIB_PATH))
+        for name in ("simsd_paged_attention", "simsd_speculative_verify"):
+            fn = getattr(held, name)
+            fn.restype, fn.argtypes = SIGNATURES[name]
+            setattr(L, name, fn)
         _lib = L
     return _lib
 
