@@ -5,14 +5,16 @@
 
 The library lands next to the Python package (kernels/libsimsd_b200.so), where
 kernels/_lib.py loads it, and beside it kernels/_binding.so, the short way from
-Python to the serving operators (host code only, against torch's headers).  nvcc
-cross-compiles without a GPU.
+Python to the serving operators (host code only, against torch's and CPython's headers;
+where it cannot be built they are called through ctypes).  nvcc cross-compiles without a
+GPU.
 """
 from __future__ import annotations
 
 import argparse
 import importlib.util
 import os
+import re
 import subprocess
 import sys
 import sysconfig
@@ -24,6 +26,7 @@ CSRC = PKG / "csrc"
 OUT = PKG / "kernels" / "libsimsd_b200.so"
 OBJ = PKG / "_build"
 BINDING = PKG / "kernels" / "_binding.so"
+STAMP = OBJ / "binding.stamp"          # what the binding was built for
 ARCH = ["-gencode", "arch=compute_100a,code=sm_100a"]
 
 
@@ -47,17 +50,33 @@ def build(force: bool = False, verbose: bool = False) -> Path:
              for u, o in zip(units, objs)], verbose)
         run([[nvcc(), *ARCH, "-shared", "-Xcompiler", "-fPIC", "-o", str(OUT) + ".tmp", *objs]], verbose)
         os.replace(str(OUT) + ".tmp", OUT)
-    source = CSRC / "binding.cpp"
-    if force or stale(BINDING, [source, REPO / "include" / "simsd_b200.h"]):
-        torch = Path(importlib.util.find_spec("torch").submodule_search_locations[0])
-        cuda = Path(nvcc()).resolve().parents[1]
-        run([[os.environ.get("CXX", "g++"), "-O2", "-std=c++17", "-fPIC", "-shared", "-I", str(REPO / "include"),
-              "-I", sysconfig.get_paths()["include"], "-I", str(torch / "include"),
-              "-I", str(torch / "include" / "torch" / "csrc" / "api" / "include"), "-I", str(cuda / "include"),
-              "-o", str(BINDING) + ".tmp", str(source), "-L", str(torch / "lib"), "-L", str(cuda / "lib64"),
-              "-ltorch_python", "-ltorch_cpu", "-ltorch_cuda", "-lc10", "-lc10_cuda", "-lcudart"]], verbose)
-        os.replace(str(BINDING) + ".tmp", BINDING)
+    try:
+        build_binding(force, verbose)
+    except (OSError, RuntimeError) as e:
+        # the library is complete without it: kernels/_lib.py then calls through ctypes
+        BINDING.unlink(missing_ok=True)
+        sys.stderr.write(f"{BINDING.name} was not built, the serving operators go through ctypes: {e}\n")
     return OUT
+
+
+def build_binding(force: bool = False, verbose: bool = False) -> None:
+    source = CSRC / "binding.cpp"
+    torch = Path(importlib.util.find_spec("torch").submodule_search_locations[0])
+    # torch's C++ interface changes with its version, CPython's with the minor one; _lib.py checks the same text
+    version = re.search(r"^__version__ = ['\"](.+)['\"]", (torch / "version.py").read_text(), re.M).group(1)
+    built_for = "torch %s, Python %d.%d" % (version, *sys.version_info[:2])
+    if not (force or stale(BINDING, [source, REPO / "include" / "simsd_b200.h"])
+            or not STAMP.exists() or STAMP.read_text() != built_for):
+        return
+    cuda = Path(nvcc()).resolve().parents[1]
+    run([[os.environ.get("CXX", "g++"), "-O2", "-std=c++17", "-fPIC", "-shared", f'-DSIMSD_BUILT_FOR="{built_for}"',
+          "-I", str(REPO / "include"), "-I", sysconfig.get_paths()["include"], "-I", str(torch / "include"),
+          "-I", str(torch / "include" / "torch" / "csrc" / "api" / "include"), "-I", str(cuda / "include"),
+          "-o", str(BINDING) + ".tmp", str(source), "-L", str(torch / "lib"), "-L", str(cuda / "lib64"),
+          "-ltorch_python", "-ltorch_cpu", "-ltorch_cuda", "-lc10", "-lc10_cuda", "-lcudart"]], verbose)
+    os.replace(str(BINDING) + ".tmp", BINDING)
+    STAMP.parent.mkdir(exist_ok=True)
+    STAMP.write_text(built_for)
 
 
 def stale(out: Path, srcs: list[Path]) -> bool:

@@ -336,4 +336,15 @@ PyModuleDef module = {PyModuleDef_HEAD_INIT, "_binding", nullptr, -1, methods, n
 
 }  // namespace
 
-PyMODINIT_FUNC PyInit__binding(void) { return PyModule_Create(&module); }
+#ifndef SIMSD_BUILT_FOR
+#define SIMSD_BUILT_FOR "an unknown version"
+#endif
+// built_for: the torch and Python whose headers this was compiled against (build.py)
+PyMODINIT_FUNC PyInit__binding(void) {
+  PyObject* m = PyModule_Create(&module);
+  if (m != nullptr && PyModule_AddStringConstant(m, "built_for", SIMSD_BUILT_FOR) != 0) {
+    Py_DECREF(m);
+    return nullptr;
+  }
+  return m;
+}

@@ -10,6 +10,8 @@ from __future__ import annotations
 
 import contextlib
 import ctypes
+import sys
+import warnings
 from pathlib import Path
 
 import torch
@@ -132,18 +134,42 @@ _BOUND = ("simsd_paged_append", "simsd_paged_attention", "simsd_paged_attention_
 _binding = None
 
 
+class _CtypesOnly:
+    """Stands in for the native binding where there is none: every request takes the Python way."""
+
+    @staticmethod
+    def paged_append(*_):
+        return None
+
+    paged_attention = speculative_verify = paged_append
+
+    @staticmethod
+    def forget():
+        pass
+
+
 def binding():
-    """The native short way to the serving operators (csrc/binding.cpp), bound to this library."""
+    """The native short way to the serving operators (csrc/binding.cpp), bound to this library.
+
+    Where it has not been built, or was built for another torch or Python, the operators are
+    called through ctypes (some 8 us a call more), with one warning."""
     global _binding
     if _binding is None:
+        L = lib()
+        wanted = "torch %s, Python %d.%d" % (torch.__version__, *sys.version_info[:2])
         try:
             from . import _binding as native
+            found = getattr(native, "built_for", "another version")
+            why = None if found == wanted else f"it was built for {found}"
         except ImportError as e:
-            raise RuntimeError("kernels/_binding.so is not built for this Python and torch; run "
-                               "`python simsd-release_b200/build.py`") from e
-        L = lib()
-        native.bind({n: ctypes.cast(getattr(L, n), ctypes.c_void_p).value for n in _BOUND}, error_ptr, stream_scratch)
-        _binding = native
+            why = str(e)
+        if why is None:
+            native.bind({n: ctypes.cast(getattr(L, n), ctypes.c_void_p).value for n in _BOUND}, error_ptr, stream_scratch)
+            _binding = native
+        else:
+            warnings.warn(f"kernels/_binding.so is not used with {wanted} ({why}): the serving operators go through "
+                          "ctypes. `python simsd-release_b200/build.py` builds it.", RuntimeWarning, stacklevel=3)
+            _binding = _CtypesOnly()
     return _binding
 
 
