@@ -14,6 +14,9 @@ The reference keeps one static cache per sequence
 
 Forward-only; CUDA tensors only (no CPU fallback).  Every stream has scratch of its
 own, so calls on several streams share none.
+Inputs of other strides than the kernels read, or that do not start on 16 bytes, are
+copied; the caches, which are written in place, have to start on 16 bytes and have page,
+head and token strides of multiples of 8 elements.
 Indices that the device finds out of range raise DEV_ERR_BAD_INDEX in
 `_lib.device_error()`; nothing is read or written for them.
 """
@@ -44,6 +47,11 @@ def _check_cache(what: str, k_cache: torch.Tensor, v_cache: torch.Tensor, kv_hea
                          f"{tuple(k_cache.shape)} / {tuple(v_cache.shape)}")
     if k_cache.stride() != v_cache.stride() or k_cache.stride(3) != 1:
         raise ValueError(f"{what}: k_cache and v_cache must have the same strides, the last one 1")
+
+
+def _on_16_bytes(t: torch.Tensor | None) -> torch.Tensor | None:
+    """t, copied where the kernels' 16-byte loads cannot start at its first element."""
+    return t if t is None or t.data_ptr() % 16 == 0 else t.clone()
 
 
 def _check_append(qkv, heads, kv_heads, k_cache, v_cache, slots, positions, cos, sin, q_weight, k_weight) -> None:
@@ -98,11 +106,11 @@ def paged_append(qkv: torch.Tensor, heads: int, kv_heads: int, k_cache: torch.Te
     if _current_device() != dev:
         with torch.cuda.device(dev):
             return paged_append(qkv, heads, kv_heads, k_cache, v_cache, slots, positions, cos, sin, q_weight, k_weight, eps)
-    if qkv.stride(1) != 1:
-        qkv = qkv.contiguous()
+    if qkv.stride(1) != 1 or qkv.stride(0) % 8 or qkv.stride(0) < qkv.shape[1]:
+        qkv = qkv.clone(memory_format=torch.contiguous_format)
     slots, positions = slots.contiguous(), positions.contiguous()
-    q_weight = q_weight.contiguous() if q_weight is not None else None
-    k_weight = k_weight.contiguous() if k_weight is not None else None
+    qkv, cos, sin, q_weight, k_weight = map(_on_16_bytes, (
+        qkv, cos, sin, *(w.contiguous() if w is not None else None for w in (q_weight, k_weight))))
     q = qkv.new_empty((qkv.shape[0], heads, shape[3]))
     rc = _lib.lib().simsd_paged_append(
         qkv.data_ptr(), qkv.stride(0), qkv.shape[0], heads, kv_heads, shape[3], 2 * cos.shape[1],
@@ -175,7 +183,7 @@ def paged_attention(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tenso
             tail_mask = tail_mask.contiguous()
         ldm_t = tail_mask.stride(-2)
         ldm_b = tail_mask.stride(0) if tail_mask.ndim == 3 else 0
-    q, seq_lens = q.contiguous(), seq_lens.contiguous()
+    q, seq_lens = _on_16_bytes(q.contiguous()), seq_lens.contiguous()
     if page_table.stride(1) != 1:
         page_table = page_table.contiguous()
     o = torch.empty_like(q)
