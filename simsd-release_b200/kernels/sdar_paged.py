@@ -120,17 +120,18 @@ class PagedBatch:
             B, L = ids.shape
             if n_draft is not None and n_draft.shape != (B,):
                 raise ValueError(f"n_draft must be [{B}]")
-            room = self.max_len - self.lens
-            full = (room <= 0) | (self.lens + L > self.page_table.shape[1] * self.page_size)
-            keep = (room - 1).clamp(0, L - 1)
+            # with at most max_drafts drafts every sequence short of max_len has L places in the table
+            full = self.lens >= min(self.max_len, self.page_table.shape[1] * self.page_size - L + 1)
+            keep = self.max_len - 1 - self.lens              # speculative_verify takes 0 .. K of it
             keep = keep if n_draft is None else torch.minimum(keep, n_draft)
             x = self.hidden(ids, torch.where(full, 0, L), self.tail_mask)
             logits = self.model.lm_head(x.view(B * L, -1)).view(B, L, -1)
             tokens, accepted, logprobs = speculative_verify(logits, drafts, uniform, noise, draft_logits, temperature, keep)
             self.last.copy_(torch.where(full, self.last, tokens.gather(1, accepted[:, None])[:, 0]))
-            self.lens += torch.where(full, 0, accepted + 1).to(torch.int32)
+            accepted.masked_fill_(full, -1)
+            self.lens += (accepted + 1).to(torch.int32)
+            accepted.clamp_(min=0)
             tokens.masked_fill_(full[:, None], -1)
-            accepted.masked_fill_(full, 0)
             logprobs.masked_fill_(full[:, None], 0.0)
         return tokens, accepted, logprobs
 

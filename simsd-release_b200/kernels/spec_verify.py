@@ -65,7 +65,7 @@ def speculative_verify(target_logits: torch.Tensor, draft_tokens: torch.Tensor, 
     distributed: draws the token after the accepted ones from max(p - q, 0), or
     from p after the last one.  temperature [B] fp32: 1 when None, 0 = greedy,
     inf = uniform over the tokens whose logit is not -inf.
-    n_draft [B] int32: drafted tokens of each sequence (<= K; K when None); the
+    n_draft [B] int32: drafted tokens of each sequence (K when None; cut to 0 .. K); the
     rows after them are not read.
 
     tokens: the accepted drafts, then the drawn token, then -1.  logprobs: the
