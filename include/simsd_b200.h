@@ -512,8 +512,8 @@ int simsd_moe_ep_return(const void* y, int64_t ldy, const int32_t* recv_expert, 
  * caches and a zero q row, and its position is not read.  qkv [T, (Hq + 2 Hk)
  * head_dim] with row stride ldqkv (q heads, k heads, v heads), q_out [T, Hq,
  * head_dim].  Slots of one call are distinct.  rotary_dim: a multiple of 16, <=
- * head_dim.  (Hq + 2 Hk) head_dim <= 36864 (more: SIMSD_ERR_UNSUPPORTED).  Replaces, for a batch, the q/k norm, rotary embedding and cache
- * write of sdar/modeling_sdar.py:197-302.
+ * head_dim.  (Hq + 2 Hk) head_dim <= 36864 (more: SIMSD_ERR_UNSUPPORTED).  Replaces, for
+ * a batch, the q/k norm, rotary embedding and cache write of sdar/modeling_sdar.py:197-302.
  */
 int simsd_paged_append(const void* qkv, int64_t ldqkv, int T, int Hq, int Hk, int head_dim, int rotary_dim,
                        const void* q_weight, const void* k_weight, float eps, const float* cos, const float* sin,
@@ -531,6 +531,8 @@ int simsd_paged_append(const void* qkv, int64_t ldqkv, int T, int Hq, int Hk, in
  * are visible to every query, the others where jt <= t, or, with tail_mask, where
  * tail_mask[b * ldm_b + t * ldm_t + jt] != 0.  A query without a visible key: o =
  * 0, lse = -inf.  q, o [B, L, Hq, head_dim] contiguous, lse [B, L, Hq] or NULL.
+ * A length over max_pages * page_size is cut there, the newest L keys being those of the
+ * cut length (SIMSD_DEV_ERR_BAD_INDEX); a negative one counts as 0.
  * The lengths are read on the device only.  B Hk ceil(G L / 128) (max_pages
  * page_size / 64 + 3) < 2^31 (more: SIMSD_ERR_UNSUPPORTED).
  */
@@ -543,7 +545,7 @@ int simsd_paged_attention(const void* q, const void* k_cache, const void* v_cach
 
 /*
  * Speculative sampling's verification from given random numbers.  For sequence b
- * with d = n_draft[b] (K when NULL) drafted tokens x_i, p_i = softmax(target row i
+ * with d = n_draft[b] (K when NULL; cut to 0 .. K) drafted tokens x_i, p_i = softmax(target row i
  * / T) and q_i = softmax(draft row i / T) (draft_logits NULL: one at x_i), T =
  * temperature[b] (1 when NULL; 0: one at the row's first maximum; inf: uniform over the
  * logits that are not -inf):

@@ -20,25 +20,30 @@
 // sum) in the workspace, and the last of its CTAs to finish (a counter per first
 // CTA, zero again afterwards) joins the parts, always in key order.
 //
-// In a CTA each key group (a warp, or one per 16 rows where there are more) takes 16 keys of every unit through a ring of its own (cp.async, no barrier
-// between warps until the sequence ends), loading ahead across sequence ends;
-// the next sequence's queries are fetched a sequence ahead.
+// In a CTA each of four warps takes 16 keys of every unit through a ring of its own
+// (cp.async, no barrier between warps until the sequence ends), loading ahead across
+// sequence ends; the next sequence's queries are fetched a sequence ahead.
 // Products with the roles swapped, so that few rows waste little: S^T = K Q^T
 // (m16n8k16: 16 keys x 8 rows), P^T turned into the second product's operand with
 // movmatrix, O^T = V^T P^T (16 dims x 8 rows).  Softmax in fp32 with exp2 of
 // log2-scaled scores; the running maximum moves (and O is rescaled) only when a
 // score exceeds it.  P is rounded to the 16-bit type for the second product: the
 // weights are <= 1 and their sum, kept in fp32, is of the unrounded ones, so the
-// rounding errs by at most half a step per weight.
+// rounding errs by at most half a step per weight (bf16: error 1.8e-3 of the output in the
+// 2-norm against 1.7e-3 for its own rounding alone).  A second product of what the rounding
+// leaves would double the tensor work for that.
 //
 // Masked keys: keys past n are zero-filled in shared memory, whatever stale memory
 // holds.  A tail key that some rows of the unit see and others do not takes part
 // with weight 0 in the second product; where its value is not finite (0 x inf), the
-// unit's product runs row by row with the hidden keys zeroed instead.
+// unit's product runs row by row with the hidden keys zeroed instead.  An infinite value
+// that a row sees gives an infinite output, but NaN in fp16 where its weight is under 2^-25
+// and rounds to 0.
 //
-// Measured (B200, 8 KV heads x 128, 4 query heads each, bf16): 2 x 120-128k tokens 172
-// us, 6.2 TB/s, 94 % of the measured copy rate; 32 x 0.3-4k 38 us, 4.8 TB/s, 73 %; 1 x 100
-// 7.6 us.
+// Measured (B200, 8 KV heads x 128, 4 query heads each, bf16; device time in a graph of
+// calls, in brackets calls one after the other on a stream): 2 x 120-128k tokens 173 us
+// (177), 6.2 TB/s, 94 % of the measured copy rate; 32 x 0.3-4k 38 us (40), 4.7 TB/s, 72 %;
+// 1 x 100 7.9 us (10.2, the host's time for a call).
 #pragma once
 #include "paged.cuh"
 

@@ -15,7 +15,9 @@
 // so a unit's softmax is spread over all 128 lanes at 32 rows too.  Q and P are read
 // from TMEM, which leaves 64 KB of shared memory to the ring (47 -> 44 us).  The running
 // maximum moves only when a score passes it by more than 2^8 (P <= 256 keeps its
-// relative precision in 16 bits), so O is hardly ever rescaled in TMEM.
+// relative precision in 16 bits), so O is hardly ever rescaled in TMEM.  P is rounded to
+// the 16-bit type as there, the largest weight too: error 2.2e-3 of the output in the
+// 2-norm against 1.7e-3 for its own rounding alone.
 //
 // Warps 0-3 softmax and epilogue, 4-7 loads into a ring of NS operand tiles K, V, K,
 // V, ..., 8 issues the products: S of unit n + 1 before O of unit n, so that they
@@ -32,9 +34,11 @@
 // copies of a row join to no finite number, what the row's keys hold says which it is.
 // All waits are bounded.
 //
-// Measured (B200, 8 KV heads x 128, 4 query heads each, bf16): 16 x 1-3k tokens x 8 rows
-// 36.5 us, 3.8 TB/s; 2 x 64k x 8 rows 91 us, 5.6 TB/s, 86 % of the measured copy rate.
-// 64 and 128 rows, with R keys a softmax thread: 16 x 1-3k 50 and 76 us.
+// Measured (B200, 8 KV heads x 128, 4 query heads each, bf16; device time in a graph of
+// calls): 16 x 1-3k tokens x 8 rows 37 us (39 one after the other on a stream), 3.8 TB/s;
+// 2 x 64k x 8 rows 91-93 us, 5.5 TB/s, 85 % of the measured copy rate.  64 and 128 rows,
+// with R keys a softmax thread: 16 x 1-3k 51.5 and 76 us.  Looking for values that are not
+// finite in every unit instead of in the joined sums took 40 and 54 us at 32 and 64 rows.
 #pragma once
 #include "paged_attn.cuh"
 

@@ -23,8 +23,9 @@
 // rest of its arithmetic is packed: the maximum in the 16-bit type itself, the
 // differences and sums two at a time.  Rows
 // are read last to first, so that the rows drawn from, mostly early ones, are the
-// ones left in L2.  64 x 7 drafts of 151936 tokens, bf16: 72 us, 4.6 TB/s (statistics 58
-// at 5.0 TB/s under ncu); 1 x 4 of 32000 8.1 us, the latency of two kernels.
+// ones left in L2.  64 x 7 drafts of 151936 tokens, bf16: 74 us on the device in a graph of
+// calls, 4.5 TB/s (82 us one after the other on a stream); 1 x 4 of 32000 8.4 us, the
+// latency of two kernels.
 #pragma once
 #include <type_traits>
 
@@ -65,9 +66,12 @@ struct SpecVerifyArgs {
 constexpr int SV_THREADS = 256, SV_WARPS = SV_THREADS / 32;
 constexpr int SV_BLOCK = 1024;                     // logits that a warp holds at a time
 constexpr int SV_CHUNK = 2048;                     // tokens that a CTA races at a time
-// p - q counts where it is more than p's rounding: the same logits in two rows give p and
-// q apart by a rounding of the sum, of its reciprocal and of the product each, at most
-// 2^-22 of p.  Without it two equal rows leave noise for a residual, which is drawn from.
+// p - q counts where it is more than p's rounding.  The same logits in two rows, split into
+// parts at the same places (rows alike modulo 16 bytes), have the same sum, and p and q
+// differ by a rounding of its reciprocal and of the product each, at most 2^-22 of p.
+// Rows that start elsewhere split the sum otherwise and may be further apart: the margin
+// does not cover them.  Without it two equal rows leave noise for a residual, which is
+// drawn from.
 constexpr float SV_OVER = 1.0f - 0x1p-21f;
 
 __device__ __forceinline__ float spec_clean(float v) { return fminf(fmaxf(v, -INFINITY), 3.402823466e+38f); }

@@ -157,7 +157,8 @@ def paged_attention(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tenso
     page_table [B, max_pages] int32: sequence b's key j is token j % page_size of
     page page_table[b, j // page_size]; entries past its last page are not read.
     seq_lens [B] int32: its keys, the L queries' own included (they are the
-    newest L).  Keys before those are visible to all of its queries; among them
+    newest L); a negative one counts as 0, one past the table is cut to its end (and
+    raises DEV_ERR_BAD_INDEX).  Keys before those are visible to all of its queries; among them
     query t sees key i where i <= t, or where tail_mask [L, L] or [B, L, L] (bool)
     is set.  A query that sees no key (an empty sequence, a mask without any) gets
     o = 0 and lse = -inf.  Only visible keys count: what stale cache memory or a
