@@ -37,7 +37,7 @@
 // Measured (B200, 8 KV heads x 128, 4 query heads each, bf16; device time in a graph of
 // calls): 16 x 1-3k tokens x 8 rows 37 us (39 one after the other on a stream), 3.8 TB/s;
 // 2 x 64k x 8 rows 91-93 us, 5.5 TB/s, 85 % of the measured copy rate.  64 and 128 rows,
-// with R keys a softmax thread: 16 x 1-3k 51.5 and 76 us.  Looking for values that are not
+// with R keys a softmax thread: 16 x 1-3k 51 and 76 us.  Looking for values that are not
 // finite in every unit instead of in the joined sums took 40 and 54 us at 32 and 64 rows.
 #pragma once
 #include "paged_attn.cuh"
@@ -174,29 +174,39 @@ __device__ void ptc_join(const PagedAttnArgs& p, const PagedPart& x, float2* buf
   __syncthreads();
 }
 
-// What four dims (from d) of row `row` come to where a sum of its copies is not finite: by the
-// values of its visible keys lo .. hi - 1, which weigh in with positive numbers.  +inf or
-// -inf where they hold no other value that is not finite, else NaN; `a` where they hold
-// none.  Off the product's path, and slow (a key at a time).
+// Sum of the values that are not finite, of four dims (from d) of keys lo .. hi - 1, of those
+// that row `row` sees or (row < 0) of all: what the dims come to where their sum is not
+// finite, since weights are positive (+inf or -inf, NaN where both occur or NaN does; 0:
+// there are none).  Off the product's path: eight keys at a time.
 template <int D, bool BF>
-__device__ __noinline__ float4 ptc_settle(const PagedAttnArgs& p, int b, int g, int n, int row, int lo, int hi, int d, float4 a) {
-  float v[4] = {a.x, a.y, a.z, a.w}, sum[4] = {0.0f, 0.0f, 0.0f, 0.0f};
-  if (isfinite((v[0] + v[1]) + (v[2] + v[3]))) return a;
-  for (int j = lo; j < hi; ++j) {
-    if (!paged_visible(p, b, n, j, row)) continue;
-    const int page = p.page_table[b * p.ld_table + p.page_div(j)];
-    if (page < 0 || page >= p.num_pages) continue;
-    const long long off = page * p.ld_page + g * p.ld_head + (j - p.page_div(j) * p.page_size) * p.ld_tok + d;
+__device__ __noinline__ float4 ptc_odd_values(const PagedAttnArgs& p, int b, int g, int n, int row, int lo, int hi, int d) {
+  constexpr int AT = 8;
+  float sum[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+  for (int j0 = lo; j0 < hi; j0 += AT) {
+    int page[AT];
 #pragma unroll
-    for (int e = 0; e < 4; ++e) {
-      const float x = load_f(p.v_cache, off + e, BF ? 0 : 1);
-      if (!isfinite(x)) sum[e] += x;
+    for (int k = 0; k < AT; ++k) page[k] = j0 + k < hi ? p.page_table[b * p.ld_table + p.page_div(j0 + k)] : -1;
+    uint2 u[AT];
+#pragma unroll
+    for (int k = 0; k < AT; ++k) {
+      const int j = j0 + k;
+      const long long off = page[k] * p.ld_page + g * p.ld_head + (j - p.page_div(j) * p.page_size) * p.ld_tok + d;
+      const bool ok = page[k] >= 0 && page[k] < p.num_pages;
+      u[k] = ok ? __ldg(reinterpret_cast<const uint2*>(reinterpret_cast<const uint16_t*>(p.v_cache) + off)) : make_uint2(0, 0);
+    }
+#pragma unroll
+    for (int k = 0; k < AT; ++k) {
+      const uint32_t w[2] = {u[k].x, u[k].y};
+      const bool see = row < 0 || paged_visible(p, b, n, j0 + k, row);
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        const uint32_t h = w[e / 2] >> (16 * (e & 1)) & 0xffffu;
+        const float x = BF ? __uint_as_float(h << 16) : __half2float(__ushort_as_half((unsigned short)h));
+        if (see && !isfinite(x)) sum[e] += x;
+      }
     }
   }
-#pragma unroll
-  for (int e = 0; e < 4; ++e)
-    if (!isfinite(v[e]) && sum[e] != 0.0f) v[e] = sum[e];
-  return make_float4(v[0], v[1], v[2], v[3]);
+  return make_float4(sum[0], sum[1], sum[2], sum[3]);
 }
 
 template <int D, int R, bool BF>
@@ -725,15 +735,21 @@ __global__ void __launch_bounds__(PTC_THREADS, 1) paged_attention_tc_kernel(cons
                 put(r, h * 16 + q4, a);
               }
               if (isnan((nul.x + nul.y) + (nul.z + nul.w))) {
+                // the thread's sums are all of the same four dims: keys before the tail count
+                // for every row
+                const int d = h * 64 + tid % 16 * 4, lo = first_unit * PTC_TK, hi = min(at.n, (at.unit + 1) * PTC_TK);
+                const float4 old = ptc_odd_values<D, BF>(p, at.b, at.g, at.n, -1, lo, min(hi, base), d);
 #pragma unroll 1
-                for (int x = tid; x < R * 16; x += PTC_SOFTMAX) {
-                  const int r = x / 16, q4 = x % 16;
+                for (int r = tid / 16; r < R; r += PTC_SOFTMAX / 16) {
                   bool scored = r0 + r < p.rows;           // NaN scores leave NaN
                   for (int i = 0; i < F; ++i) scored &= !isnan(xl[i * R + r]);
-                  if (scored)
-                    put(r, h * 16 + q4,
-                        ptc_settle<D, BF>(p, at.b, at.g, at.n, r0 + r, first_unit * PTC_TK, min(at.n, (at.unit + 1) * PTC_TK),
-                                          h * 64 + q4 * 4, joined(r, q4)));
+                  if (!scored) continue;
+                  const float4 odd = ptc_odd_values<D, BF>(p, at.b, at.g, at.n, r0 + r, max(lo, base), hi, d);
+                  const float x[4] = {old.x + odd.x, old.y + odd.y, old.z + odd.z, old.w + odd.w};
+                  float4 a = joined(r, tid % 16);
+                  a.x = isfinite(a.x) || x[0] == 0.0f ? a.x : x[0], a.y = isfinite(a.y) || x[1] == 0.0f ? a.y : x[1];
+                  a.z = isfinite(a.z) || x[2] == 0.0f ? a.z : x[2], a.w = isfinite(a.w) || x[3] == 0.0f ? a.w : x[3];
+                  put(r, h * 16 + tid % 16, a);
                 }
               }
               __syncwarp();
