@@ -61,10 +61,15 @@ def build(force: bool = False, verbose: bool = False) -> Path:
 
 def build_binding(force: bool = False, verbose: bool = False) -> None:
     source = CSRC / "binding.cpp"
-    torch = Path(importlib.util.find_spec("torch").submodule_search_locations[0])
+    spec = importlib.util.find_spec("torch")
+    if spec is None:
+        raise RuntimeError("torch is not installed")
+    torch = Path(spec.submodule_search_locations[0])
     # torch's C++ interface changes with its version, CPython's with the minor one; _lib.py checks the same text
-    version = re.search(r"^__version__ = ['\"](.+)['\"]", (torch / "version.py").read_text(), re.M).group(1)
-    built_for = "torch %s, Python %d.%d" % (version, *sys.version_info[:2])
+    version = re.search(r"^__version__ = ['\"](.+)['\"]", (torch / "version.py").read_text(), re.M)
+    if version is None:
+        raise RuntimeError(f"no version in {torch / 'version.py'}")
+    built_for = "torch %s, Python %d.%d" % (version.group(1), *sys.version_info[:2])
     if not (force or stale(BINDING, [source, REPO / "include" / "simsd_b200.h"])
             or not STAMP.exists() or STAMP.read_text() != built_for):
         return

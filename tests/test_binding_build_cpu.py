@@ -61,6 +61,12 @@ def test_library_builds_without_the_binding(build, monkeypatch, capsys, error):
     assert str(error) in capsys.readouterr().err
 
 
+def test_library_builds_without_torch(build, monkeypatch, capsys):
+    monkeypatch.setattr(build.importlib.util, "find_spec", lambda name: None)
+    assert build.build() == build.OUT and not build.calls and not build.BINDING.exists()
+    assert "torch is not installed" in capsys.readouterr().err
+
+
 def refuse_all():
     for f, args in ((_paged().paged_append, append_args()), (_paged().paged_attention, attention_args()),
                     (_verify().speculative_verify, verify_args())):
