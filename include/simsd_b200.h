@@ -544,6 +544,113 @@ int simsd_paged_attention(const void* q, const void* k_cache, const void* v_cach
                           void* workspace, size_t workspace_bytes, int* err_word, void* stream);
 
 /*
+ * The same through a window: the query at position x = n - L + t sees a key j only where
+ * also j > x - window or j < sinks (window 0: no window, every key).  Keys that no query of
+ * the call sees are not read, and the pages that hold nothing else may be any.
+ */
+int simsd_paged_attention_window(const void* q, const void* k_cache, const void* v_cache, int num_pages, int page_size,
+                                 int64_t ld_page, int64_t ld_head, int64_t ld_tok, const int32_t* page_table,
+                                 int64_t ld_table, int max_pages, const int32_t* seq_lens, const uint8_t* tail_mask,
+                                 int64_t ldm_b, int64_t ldm_t, int B, int L, int Hq, int Hk, int head_dim, float scale,
+                                 int window, int sinks, void* o, float* lse, int dtype, void* workspace,
+                                 size_t workspace_bytes, int* err_word, void* stream);
+
+/*
+ * The paged cache held in 8 bits: k_cache / v_cache [num_pages, Hk, page_size, head_dim]
+ * e4m3 with strides of multiples of 16, and k_scale / v_scale [num_pages, Hk, page_size /
+ * block] fp32 (strides lds_page, lds_head, lds_block): a stored number stands for its block's
+ * scale times itself.  block divides page_size.
+ *
+ * simsd_paged_append8: sequence b's new tokens are the last c = count[b] (L when NULL; cut to
+ * 0 .. min(L, n)) of its L rows of qkv [B, L, (Hq + 2 Hk) head_dim] (strides ldq_b, ldq_t)
+ * and go to positions n - c .. n - 1 with n = seq_lens[b], the length with them, in the pages
+ * of page_table.  Row by row q_out [B, L, Hq, head_dim] = r(n(q)) as simsd_paged_append has
+ * it, zero in the rows before the new tokens; keys r(n(k)) and values v are stored in
+ * 8 bits.  Per block and head with new tokens, a the largest finite magnitude among them:
+ *   want = the smallest 2^e with a <= 448 2^e, e from -64 to 64
+ *   scale = want where the block's first token is new, else max(scale, want)
+ * where it grows the block's tokens before the new ones are rounded anew to it; tokens after
+ * them are left as they are.  Numbers that are not finite are stored as NaN.  A position past the page
+ * table or cos / sin, or a page outside the cache, is flagged (SIMSD_DEV_ERR_BAD_INDEX): the
+ * keys and values are not written, and q is zero for a position past the tables.  No page
+ * is written by two sequences of a call.
+ */
+int simsd_paged_append8(const void* qkv, int64_t ldq_b, int64_t ldq_t, int B, int L, int Hq, int Hk, int head_dim,
+                        int rotary_dim, const void* q_weight, const void* k_weight, float eps, const float* cos,
+                        const float* sin, int64_t n_positions, const int32_t* page_table, int64_t ld_table, int max_pages,
+                        const int32_t* seq_lens, const int32_t* count, void* q_out, void* k_cache, void* v_cache,
+                        float* k_scale, float* v_scale, int num_pages, int page_size, int block, int64_t ld_page,
+                        int64_t ld_head, int64_t ld_tok, int64_t lds_page, int64_t lds_head, int64_t lds_block, int dtype,
+                        int* err_word, void* stream);
+
+/*
+ * simsd_paged_attention_window over that cache (window 0: none).  Any positive scales up to
+ * 2^64 do, not only powers of two; sums are fp32 and weights fp16 (11 bits down to 2^-22 of
+ * the largest).  The workspace as for simsd_paged_attention, of a size of its own.
+ */
+size_t simsd_paged_attention8_workspace_size(int L, int Hq, int Hk, int head_dim);
+int simsd_paged_attention8(const void* q, const void* k_cache, const void* v_cache, const float* k_scale,
+                           const float* v_scale, int num_pages, int page_size, int block, int64_t ld_page, int64_t ld_head,
+                           int64_t ld_tok, int64_t lds_page, int64_t lds_head, int64_t lds_block,
+                           const int32_t* page_table, int64_t ld_table, int max_pages, const int32_t* seq_lens,
+                           const uint8_t* tail_mask, int64_t ldm_b, int64_t ldm_t, int B, int L, int Hq, int Hk,
+                           int head_dim, float scale, int window, int sinks, void* o, float* lse, int dtype,
+                           void* workspace, size_t workspace_bytes, int* err_word, void* stream);
+
+/*
+ * Page tables and slot maps from lengths.  free_pages [pool_pages] is a stack of which the
+ * lowest free_count[0] entries are free pages; held[b] pages of sequence b's row of
+ * page_table are its own.
+ *
+ * simsd_paged_reserve: room for c = count[b] (L when NULL; cut to 0 .. L) more tokens after
+ * the lens[b] of every sequence.  It takes max(0, ceil((lens + c) / page_size) - h) pages, h =
+ * max(held, ceil(lens / page_size)), from the top of the stack, sequence by sequence, into the
+ * row's places from h on.  Row b of slots and positions [B, L] ends in its c tokens (slot
+ * page * page_size + place, position lens .. lens + c - 1); before them slot -1, position 0.
+ * total[b] = lens[b] + c.  From the first sequence that the stack cannot serve on, those that
+ * need a page get no tokens (all -1, total = lens) and SIMSD_DEV_ERR_CAPACITY is raised; so
+ * it is with one whose pages would not fit its row.  A negative length (SIMSD_DEV_ERR_BAD_INDEX)
+ * gets none, total 0.
+ * simsd_paged_release: sequence b keeps the pages of keep[b] tokens (negative: none), and its
+ * other held ones go back onto the stack, sequence by sequence, each one's in its order; a stack
+ * without room for them takes none of a sequence's (SIMSD_DEV_ERR_CAPACITY).
+ * The workspace is SIMSD_PAGED_COUNTER_BYTES of counters, zero before the first call and after
+ * every one (simsd_paged_attention's may be shared).
+ */
+int simsd_paged_reserve(int32_t* page_table, int64_t ld_table, int max_pages, const int32_t* lens, const int32_t* count,
+                        int32_t* held, int32_t* free_pages, int pool_pages, int32_t* free_count, int B, int L,
+                        int page_size, int64_t* slots, int64_t* positions, int32_t* total, void* workspace,
+                        size_t workspace_bytes, int* err_word, void* stream);
+int simsd_paged_release(const int32_t* page_table, int64_t ld_table, int max_pages, int32_t* held, int32_t* free_pages,
+                        int pool_pages, int32_t* free_count, const int32_t* keep, int B, int page_size, void* workspace,
+                        size_t workspace_bytes, int* err_word, void* stream);
+
+/*
+ * Rules on logits [B, R, V] (strides ld_b, ld_r, unit last; out ldo_b, ldo_r, the same memory
+ * with the same strides or other memory): row i of sequence b is what follows i drafted tokens, token v, c =
+ * counts[b, v] + the number of j < i with drafts[b, j] = v (each NULL: none):
+ *   x > 0 ? x / repetition[b] : x repetition[b]    where c > 0 or seen[b] has v
+ *   - frequency[b] c - presence[b]                 where c > 0
+ *   + the sum of bias_values[b, k] over bias_ids[b, k] = v
+ *   -inf                                           where allowed[b, i] lacks v
+ * one after the other in fp32, rounded once.  seen and allowed are bit lists of ceil(V / 32)
+ * words (token v: bit v % 32 of word v / 32; NULL: nothing seen, everything allowed).  Drafts
+ * outside [0, V) count nowhere; bias ids below 0 are none, those from V on raise
+ * SIMSD_DEV_ERR_BAD_INDEX.  dtype: all three.  B <= 65535 (more: SIMSD_ERR_UNSUPPORTED).
+ *
+ * simsd_count_tokens: counts[b, v] += how often v is among tokens[b, 0 .. N - 1]; negative
+ * ones are none, those from V on raise SIMSD_DEV_ERR_BAD_INDEX.
+ */
+int simsd_adjust_logits(const void* logits, int64_t ld_b, int64_t ld_r, void* out, int64_t ldo_b, int64_t ldo_r, int B,
+                        int R, int V, int dtype, const int32_t* counts, int64_t ld_counts, const int64_t* drafts,
+                        int64_t ld_drafts, const uint32_t* seen, int64_t ld_seen, const float* repetition,
+                        const float* presence, const float* frequency, const int32_t* bias_ids, int64_t ld_ids,
+                        const float* bias_values, int64_t ld_values, int n_bias, const uint32_t* allowed,
+                        int64_t ld_allowed_b, int64_t ld_allowed_r, int* err_word, void* stream);
+int simsd_count_tokens(int32_t* counts, int64_t ld_counts, const int64_t* tokens, int64_t ld_tokens, int B, int N, int V,
+                       int* err_word, void* stream);
+
+/*
  * Speculative sampling's verification from given random numbers.  For sequence b
  * with d = n_draft[b] (K when NULL; cut to 0 .. K) drafted tokens x_i, p_i = softmax(target row i
  * / T) and q_i = softmax(draft row i / T) (draft_logits NULL: one at x_i), T =

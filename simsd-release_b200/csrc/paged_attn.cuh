@@ -65,6 +65,7 @@ struct PagedAttnArgs {
   long long ld_page, ld_head, ld_tok, ld_table, ldm_b, ldm_t;
   int B, L, Hq, Hk, G, num_pages, page_size, max_pages, rows, row_tiles;
   PagedDiv page_div, g_div; // by page_size, by G
+  int window, sinks;        // a query at position x sees j > x - window and j < sinks; read where WIN
   uint32_t q_sign;          // 0x80008000 flips the queries' signs (a negative scale)
   float scale_log2;         // |scale| log2(e), positive
 };
@@ -159,20 +160,44 @@ struct PagedEnd {
 };
 constexpr int PAGED_END_MAX = 2;
 
+// Through a window, the first key after the sinks that some row of a sequence of n sees
+__device__ __forceinline__ int paged_first(const PagedAttnArgs& p, int n) {
+  return (int)max(0LL, (long long)n - p.L + 1 - p.window);
+}
+// units of TK keys between those of the sinks and that key's: no row sees any of their keys
+template <int TK>
+__device__ __forceinline__ int paged_skip(const PagedAttnArgs& p, int n) {
+  return max(0, paged_first(p, n) / TK - (p.sinks / TK + (p.sinks % TK != 0)));
+}
+
+// whether a window hides one of `keys` keys from key0 on from a row of the last token, at n - 1
+__device__ __forceinline__ bool paged_out(const PagedAttnArgs& p, int n, int key0, int keys) {
+  return key0 < n - p.window && key0 + keys > p.sinks;
+}
+
 // Position in the unit order: sequence b (length n, nu units per KV head and row
 // tile), KV head g, row tile rt, unit of it; w counts units and ends before it.
-template <int TK>
+// WIN: through a window, whose units are the sequence's but the `skip` ones in its middle.
+template <int TK, bool WIN = false>
 struct PagedPos {
   static constexpr int END = PagedEnd<TK>::UNITS;
-  int b, g, rt, unit, n, nu, w;
+  int b, g, rt, unit, n, nu, w, skip;
   __device__ __forceinline__ void next(const PagedAttnArgs& p) {
     ++w;
     if (++unit < nu) return;
     w += END;
     unit = 0;
     if (!next_rows(p, b, g, rt) || b >= p.B) return;
+    measure(p);
+  }
+  __device__ __forceinline__ void measure(const PagedAttnArgs& p) {
     n = paged_len(p, b);
-    nu = paged_units<TK>(n);
+    skip = WIN ? paged_skip<TK>(p, n) : 0;
+    nu = paged_units<TK>(n) - skip;
+  }
+  // the unit's first key
+  __device__ __forceinline__ int key(const PagedAttnArgs& p) const {
+    return (WIN && unit >= p.sinks / TK + (p.sinks % TK != 0) ? unit + skip : unit) * TK;
   }
   // the row tile, head or sequence after (b, g, rt); true for another sequence
   __device__ static __forceinline__ bool next_rows(const PagedAttnArgs& p, int& b, int& g, int& rt) {
@@ -197,10 +222,12 @@ struct PagedCut {
 
 // Whether query row r (token t = r / G) sees key j, j < n or not; rows past the last
 // one count as the last token's.  No branch around the mask's byte, so that several are fetched at once.
+template <bool WIN = false>
 __device__ __forceinline__ bool paged_visible(const PagedAttnArgs& p, int b, int n, int j, int r) {
   const int t = min(p.g_div(r), p.L - 1), jt = j - (n - p.L);
   bool see = jt <= t;
   if (p.tail) see = jt < 0 || p.tail[b * p.ldm_b + t * p.ldm_t + max(0, min(jt, p.L - 1))] != 0;
+  if (WIN) see = see && (j < p.sinks || jt > t - p.window);
   return see && j < n;
 }
 
@@ -210,12 +237,18 @@ __device__ __forceinline__ long long paged_row(const PagedAttnArgs& p, int b, in
   return ((long long)b * p.L + t) * p.Hq + g * p.G + (r - t * p.G);
 }
 // 16 dims (from mt * 16) of 8 rows (from r8) out of a fragment of O^T (v: dims d, d
-// + 8 of two rows): packed and transposed, so that a lane holds two dims of row
-// lane / 4 and stores 4 bytes twice.  `row`: the lane's row's place, or -1.
-template <bool BF, int D>
+// + 8 of two rows; with PAIRS dims 2 d, 2 d + 1): packed and transposed, so that a lane
+// holds two dims of row lane / 4 and stores 4 bytes twice (with PAIRS four dims, 8 bytes).
+// `row`: the lane's row's place, or -1.
+template <bool BF, int D, bool PAIRS = false>
 __device__ __forceinline__ void paged_store(const PagedAttnArgs& p, long long row, int mt, int lane, float4 v) {
   const uint32_t lo = pat_transpose(pat_pack<BF>(v.x, v.y)), hi = pat_transpose(pat_pack<BF>(v.z, v.w));
   if (row < 0) return;
+  if constexpr (PAIRS) {
+    reinterpret_cast<uint2*>(reinterpret_cast<uint16_t*>(p.o) + row * D + mt * 16)[lane & 3] =
+        make_uint2(__byte_perm(lo, hi, 0x5410), __byte_perm(lo, hi, 0x7632));
+    return;
+  }
   uint32_t* dst = reinterpret_cast<uint32_t*>(reinterpret_cast<uint16_t*>(p.o) + row * D + mt * 16) + (lane & 3);
   dst[0] = lo;
   dst[4] = hi;
@@ -227,8 +260,8 @@ __device__ __forceinline__ void paged_store_lse(const PagedAttnArgs& p, int b, i
 
 // This CTA's place in the cut of the call's units and ends, and the position of its
 // first unit.  False: this CTA has none.
-template <int THREADS, int TK>
-__device__ __forceinline__ bool paged_range(const PagedAttnArgs& p, PagedCut& cut, PagedPos<TK>& pos) {
+template <int THREADS, int TK, bool WIN = false>
+__device__ __forceinline__ bool paged_range(const PagedAttnArgs& p, PagedCut& cut, PagedPos<TK, WIN>& pos) {
   constexpr int WARPS = THREADS / 32;
   __shared__ int s_sum[WARPS], s_more[WARPS];
   __shared__ int s_b, s_first;
@@ -238,7 +271,8 @@ __device__ __forceinline__ bool paged_range(const PagedAttnArgs& p, PagedCut& cu
   auto units = [&](int b) {
     if (b >= p.B) return 0;
     if (flag && p.seq_lens[b] > (long long)p.max_pages * p.page_size) atomicOr(p.err, SIMSD_DEV_ERR_BAD_INDEX);
-    return (paged_units<TK>(paged_len(p, b)) + PagedEnd<TK>::UNITS) * per;
+    const int n = paged_len(p, b), skip = WIN ? paged_skip<TK>(p, n) : 0;
+    return (paged_units<TK>(n) - skip + PagedEnd<TK>::UNITS) * per;
   };
   // sequences tid, tid + THREADS, ...: the first of them scanned, the others summed
   int u = units(tid), incl = u, more = 0;
@@ -285,8 +319,7 @@ __device__ __forceinline__ bool paged_range(const PagedAttnArgs& p, PagedCut& cu
   }
   __syncthreads();
   pos.b = s_b;
-  pos.n = paged_len(p, pos.b);
-  pos.nu = paged_units<TK>(pos.n);
+  pos.measure(p);
   const int rem = w0 - s_first, hr = rem / (pos.nu + PagedEnd<TK>::UNITS);
   pos.unit = rem - hr * (pos.nu + PagedEnd<TK>::UNITS);
   pos.w = w0;
@@ -318,7 +351,7 @@ __device__ __forceinline__ bool paged_arrive(const PagedAttnArgs& p, const Paged
 // Joins the parts of a cut sequence (one KV head and row tile of it) that starts
 // in CTA c0: part i's max, sum and O lie in slot 1 of CTA c0 for i = 0, in slot 0
 // of CTA c0 + i for the others.  `buf`: OBUF bytes of shared memory.
-template <int D, int NT, bool BF>
+template <int D, int NT, bool BF, bool PAIRS = false>
 __device__ __noinline__ void paged_join(const PagedAttnArgs& p, int b, int g, int r0, int c0, int parts, float* buf) {
   using S = PatShape<D, NT>;
   constexpr int MT = D / 16, NR = S::NR, ALL = MT * NT * 32, PER = ALL / PAT_THREADS;   // fragments, and of a thread
@@ -397,11 +430,114 @@ __device__ __noinline__ void paged_join(const PagedAttnArgs& p, int b, int g, in
 #pragma unroll
   for (int k = 0; k < PER; ++k) {
     const int x = tid + k * PAT_THREADS, rr = r0 + x / 32 % NT * 8 + (lane >> 2);
-    paged_store<BF, D>(p, rr < p.rows ? paged_row(p, b, g, rr) : -1, x / (NT * 32), lane, a[k]);
+    paged_store<BF, D, PAIRS>(p, rr < p.rows ? paged_row(p, b, g, rr) : -1, x / (NT * 32), lane, a[k]);
   }
 }
 
-template <int D, int NT, bool BF>
+// The end of a sequence's row tile, or of the CTA's range inside it (whole: neither end was
+// cut): the warps are joined, a whole sequence is written, a part goes to the workspace.
+// o, m (in log2 units), l: a warp's fragments; l is not summed over the lanes yet.
+template <int D, int NT, bool BF, bool PAIRS, typename Pos>
+__device__ __forceinline__ void paged_finish(const PagedAttnArgs& p, const Pos& at, bool whole, int part, float (&o)[D / 16][NT][4],
+                                             const float (&m)[NT][2], const float (&l)[NT][2], float4* obuf, float* sm_m,
+                                             float* sm_l, const PagedCut& range, PagedPart* cuts, bool* joins) {
+  constexpr int MT = D / 16, NR = NT * 8;
+  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+  const int slot = 2 * blockIdx.x + part, r0 = at.rt * NR;
+#pragma unroll
+  for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+    for (int e = 0; e < 2; ++e) {
+      float x = l[nt][e];
+      x += __shfl_xor_sync(0xffffffffu, x, 4);
+      x += __shfl_xor_sync(0xffffffffu, x, 8);
+      x += __shfl_xor_sync(0xffffffffu, x, 16);
+      if (lane < 4) {
+        sm_m[warp * NR + nt * 8 + 2 * lane + e] = m[nt][e];
+        sm_l[warp * NR + nt * 8 + 2 * lane + e] = x;
+      }
+    }
+  __syncthreads();
+  float inv[NT][2];
+#pragma unroll
+  for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+    for (int e = 0; e < 2; ++e) {
+      const int r = nt * 8 + 2 * (lane & 3) + e;
+      float mm = -INFINITY, ll = 0.0f;
+#pragma unroll
+      for (int w = 0; w < PAT_WARPS; ++w) mm = fmaxf(mm, sm_m[w * NR + r]);
+      const float mu = mm == -INFINITY ? 0.0f : mm;
+#pragma unroll
+      for (int w = 0; w < PAT_WARPS; ++w) ll = fmaf(sm_l[w * NR + r], pat_exp2(sm_m[w * NR + r] - mu), ll);
+      const float f = pat_exp2(m[nt][e] - mu);
+      inv[nt][e] = !whole ? 1.0f : ll == 0.0f ? 0.0f : 1.0f / ll;
+#pragma unroll
+      for (int mt = 0; mt < MT; ++mt) o[mt][nt][e] *= f, o[mt][nt][e + 2] *= f;
+      if (warp == 0 && lane < 4) {
+        if (whole)
+          paged_store_lse(p, at.b, at.g, r0 + r, mm, ll);
+        else
+          p.part_ml[slot * NR + r] = make_float2(mm, ll);
+      }
+    }
+#pragma unroll
+  for (int nt = 0; nt < NT; ++nt) {
+    const int r = r0 + nt * 8 + (lane >> 2);
+    const long long row = r < p.rows ? paged_row(p, at.b, at.g, r) : -1;
+    if (nt > 0) __syncthreads();
+#pragma unroll
+    for (int mt = 0; mt < MT; ++mt)
+      obuf[(warp * MT + mt) * 32 + lane] = make_float4(o[mt][nt][0], o[mt][nt][1], o[mt][nt][2], o[mt][nt][3]);
+    __syncthreads();
+#pragma unroll
+    for (int k = 0; k < MT / PAT_WARPS; ++k) {
+      const int mt = warp + k * PAT_WARPS;
+      const float4* from = obuf + mt * 32 + lane;
+      float4 a = from[0];
+#pragma unroll
+      for (int w = 1; w < PAT_WARPS; ++w) {
+        const float4 x = from[w * MT * 32];
+        a.x += x.x, a.y += x.y, a.z += x.z, a.w += x.w;
+      }
+      a.x *= inv[nt][0], a.y *= inv[nt][1], a.z *= inv[nt][0], a.w *= inv[nt][1];
+      if (whole)
+        paged_store<BF, D, PAIRS>(p, row, mt, lane, a);
+      else
+        p.part_o[(((long long)slot * MT + mt) * NT + nt) * 32 + lane] = a;
+    }
+  }
+  __syncthreads();
+  if (!whole && tid == 0) {
+    const int head = at.w - at.unit, c0 = range.cta_of(head);   // the sequence's first unit and CTA
+    cuts[part] = {at.b, at.g, r0, c0, range.cta_of(head + at.nu - 1) - c0 + 1};
+    // the first part at once, so that it is not this CTA that everyone else waits for in the end
+    if (part == 0) joins[0] = paged_arrive(p, cuts[0]);
+  }
+}
+// Cut sequences (at most the range's first and last): the last of their CTAs to get here joins the parts.
+template <int D, int NT, bool BF, bool PAIRS>
+__device__ __forceinline__ void paged_leave(const PagedAttnArgs& p, const PagedPart* cuts, bool* joins, float4* obuf) {
+  if (threadIdx.x == 0 && cuts[1].parts > 0) joins[1] = paged_arrive(p, cuts[1]);
+  __syncthreads();
+  for (int k = 0; k < 2; ++k) {
+    const PagedPart x = cuts[k];
+    if (joins[k]) paged_join<D, NT, BF, PAIRS>(p, x.b, x.g, x.r0, x.c0, x.parts, reinterpret_cast<float*>(obuf));
+    __syncthreads();
+  }
+}
+
+// Page of `keys` keys (of one page, from `key` on) through a window; PAGED_UNSEEN where no row
+// sees any of them: their pages may have been given back.
+constexpr int PAGED_UNSEEN = -0x7fffffff;
+template <typename Pos>
+__device__ __forceinline__ int paged_page(const PagedAttnArgs& p, const Pos& x, int key, int keys) {
+  if (key >= x.n) return -1;
+  if (key >= p.sinks && key + keys <= paged_first(p, x.n)) return PAGED_UNSEEN;
+  return p.page_table[x.b * p.ld_table + p.page_div(key)];
+}
+
+template <int D, int NT, bool BF, bool WIN>
 __global__ void __launch_bounds__(PAT_THREADS, PAT_CTAS_PER_SM) paged_attention_kernel(const __grid_constant__ PagedAttnArgs p) {
   griddep_launch_dependents();
   griddep_wait();
@@ -420,16 +556,16 @@ __global__ void __launch_bounds__(PAT_THREADS, PAT_CTAS_PER_SM) paged_attention_
   float* sm_l = sm_m + PAT_WARPS * NR;
 
   __shared__ PagedCut s_range;
-  PagedPos<PAT_TK> ld;
+  PagedPos<PAT_TK, WIN> ld;
   int end;
   {
     PagedCut cut;
-    if (!paged_range<PAT_THREADS, PAT_TK>(p, cut, ld)) return;
+    if (!paged_range<PAT_THREADS, PAT_TK, WIN>(p, cut, ld)) return;
     end = cut.first(blockIdx.x + 1);
     if (tid == 0) s_range = cut;
   }
   if (tid < 2) s_cut[tid].parts = 0, s_join[tid] = false;
-  PagedPos<PAT_TK> at = ld;
+  PagedPos<PAT_TK, WIN> at = ld;
 
   // ---- loads: the warp's 16 keys of position `ld` into its next ring slot.
   // Pages of a multiple of 16 tokens hold all sixteen in one page, a fixed distance
@@ -438,20 +574,21 @@ __global__ void __launch_bounds__(PAT_THREADS, PAT_CTAS_PER_SM) paged_attention_
   const bool page16 = p.page_size % 16 == 0;
   const int kc = lane % CH, khi = lane / CH;
   const uint32_t swz = (uint32_t)(khi * (D * 2) + ((kc ^ khi) << 4));
-  auto fetch_page = [&](const PagedPos<PAT_TK>& x) {
-    const int key = x.unit * PAT_TK + warp * 16 + (page16 ? 0 : lane & 15);
-    return key < x.n ? p.page_table[x.b * p.ld_table + p.page_div(key)] : -1;
+  auto fetch_page = [&](const PagedPos<PAT_TK, WIN>& x) {
+    const int key = x.key(p) + warp * 16 + (page16 ? 0 : lane & 15);
+    return WIN ? paged_page(p, x, key, page16 ? 16 : 1) : key < x.n ? p.page_table[x.b * p.ld_table + p.page_div(key)] : -1;
   };
   int page = fetch_page(ld);
   uint32_t load_slot = ring;
   auto load = [&]() {
     if (ld.w < end) {
       const uint32_t dst = load_slot + swz;
-      const int key0 = ld.unit * PAT_TK + warp * 16;
+      const int key0 = ld.key(p) + warp * 16;
       if (key0 < ld.n) {
         const bool fine = page >= 0 && page < p.num_pages;
+        const int from = WIN ? paged_first(p, ld.n) : 0;      // keys from the sinks' end on that no row sees
         if (page16) {
-          if (!fine && p.err) atomicOr(p.err, SIMSD_DEV_ERR_BAD_INDEX);
+          if (!fine && p.err && !(WIN && page == PAGED_UNSEEN)) atomicOr(p.err, SIMSD_DEV_ERR_BAD_INDEX);
           const int in = key0 - p.page_div(key0) * p.page_size;
           const long long off = fine ? page * p.ld_page + ld.g * p.ld_head + (in + khi) * p.ld_tok + kc * 8 : 0;
           const char* k = reinterpret_cast<const char*>(p.k_cache) + off * 2;
@@ -461,7 +598,8 @@ __global__ void __launch_bounds__(PAT_THREADS, PAT_CTAS_PER_SM) paged_attention_
 #pragma unroll
           for (int i = 0; i < 16 / KPI; ++i) {
             const uint32_t s = (dst ^ ((i * KPI & 7) << 4)) + i * KPI * (D * 2);
-            const bool ok = left > i * KPI;
+            const int key = key0 + khi + i * KPI;
+            const bool ok = left > i * KPI && !(WIN && key >= p.sinks && key < from);
             pat_cp16(s, ok ? k : reinterpret_cast<const char*>(p.k_cache), ok);
             pat_cp16(s + S::MAT, ok ? v : reinterpret_cast<const char*>(p.v_cache), ok);
             k += step;
@@ -474,7 +612,7 @@ __global__ void __launch_bounds__(PAT_THREADS, PAT_CTAS_PER_SM) paged_attention_
             if (fine)
               off = page * p.ld_page + ld.g * p.ld_head +
                     (key - p.page_div(key) * p.page_size) * p.ld_tok;
-            else if (p.err)
+            else if (p.err && !(WIN && page == PAGED_UNSEEN))
               atomicOr(p.err, SIMSD_DEV_ERR_BAD_INDEX);
           }
 #pragma unroll
@@ -531,7 +669,7 @@ __global__ void __launch_bounds__(PAT_THREADS, PAT_CTAS_PER_SM) paged_attention_
       for (int k = 0; k < QW; ++k) bq[k] = qnext[k];
       if (at.w + at.nu - at.unit + at.END < end) {
         int b = at.b, g = at.g, rt = at.rt;
-        PagedPos<PAT_TK>::next_rows(p, b, g, rt);
+        PagedPos<PAT_TK, WIN>::next_rows(p, b, g, rt);
         fetch_queries(b, g, rt);
       }
 #pragma unroll
@@ -550,7 +688,7 @@ __global__ void __launch_bounds__(PAT_THREADS, PAT_CTAS_PER_SM) paged_attention_
     const uint32_t ks_base = slot_at, vs_base = ks_base + S::MAT;
     slot_at += 2 * S::MAT;
     if (slot_at == ring + S::STAGES * 2 * S::MAT) slot_at = ring;
-    const int key0 = at.unit * PAT_TK + warp * 16;
+    const int key0 = at.key(p) + warp * 16;
     if (key0 < at.n) {
       // S^T = K Q^T
       float s[NT][4];
@@ -564,12 +702,13 @@ __global__ void __launch_bounds__(PAT_THREADS, PAT_CTAS_PER_SM) paged_attention_
         for (int nt = 0; nt < NT; ++nt) pat_mma<BF>(s[nt], a, bq[2 * ks * NT + nt], bq[(2 * ks + 1) * NT + nt]);
       }
       const int r0 = at.rt * NR;
-      const bool edge = key0 + 16 > at.n - p.L;          // some key of the sixteen may be hidden from some row
+      // some key of the sixteen may be hidden from some row
+      const bool edge = key0 + 16 > at.n - p.L || (WIN && paged_out(p, at.n, key0, 16));
       if (edge) {
         uint32_t see = 0;
 #pragma unroll
         for (int x = 0; x < NT * 4; ++x)
-          see |= (uint32_t)paged_visible(p, at.b, at.n, key0 + (lane >> 2) + (x & 2) * 4,
+          see |= (uint32_t)paged_visible<WIN>(p, at.b, at.n, key0 + (lane >> 2) + (x & 2) * 4,
                                          r0 + (x >> 2) * 8 + 2 * (lane & 3) + (x & 1)) << x;
 #pragma unroll
         for (int nt = 0; nt < NT; ++nt)
@@ -643,8 +782,8 @@ __global__ void __launch_bounds__(PAT_THREADS, PAT_CTAS_PER_SM) paged_attention_
 #pragma unroll
             for (int e = 0; e < 2; ++e) {
               const int j = key0 + 2 * (lane & 3) + e * 8, row = r0 + nt * 8 + r;
-              keep[e] = (paged_visible(p, at.b, at.n, j, row) ? 0xffffu : 0u) |
-                        (paged_visible(p, at.b, at.n, j + 1, row) ? 0xffff0000u : 0u);
+              keep[e] = (paged_visible<WIN>(p, at.b, at.n, j, row) ? 0xffffu : 0u) |
+                        (paged_visible<WIN>(p, at.b, at.n, j + 1, row) ? 0xffff0000u : 0u);
             }
             const bool mine = (r >> 1) == (lane & 3);
 #pragma unroll
@@ -664,91 +803,16 @@ __global__ void __launch_bounds__(PAT_THREADS, PAT_CTAS_PER_SM) paged_attention_
     const bool ends = at.unit + 1 == at.nu;
     if (ends || at.w + 1 >= end) {
       // join the warps; a whole sequence is written, a part goes to the workspace
-      const bool whole = ends && first_unit == 0;
-      const int part = first_unit == 0 ? 1 : 0, slot = 2 * blockIdx.x + part, r0 = at.rt * NR;
 #pragma unroll
       for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
-        for (int e = 0; e < 2; ++e) {
-          float x = l[nt][e];
-          x += __shfl_xor_sync(0xffffffffu, x, 4);
-          x += __shfl_xor_sync(0xffffffffu, x, 8);
-          x += __shfl_xor_sync(0xffffffffu, x, 16);
-          m[nt][e] *= p.scale_log2;
-          if (lane < 4) {
-            sm_m[warp * NR + nt * 8 + 2 * lane + e] = m[nt][e];
-            sm_l[warp * NR + nt * 8 + 2 * lane + e] = x;
-          }
-        }
-      __syncthreads();
-      float inv[NT][2];
-#pragma unroll
-      for (int nt = 0; nt < NT; ++nt)
-#pragma unroll
-        for (int e = 0; e < 2; ++e) {
-          const int r = nt * 8 + 2 * (lane & 3) + e;
-          float mm = -INFINITY, ll = 0.0f;
-#pragma unroll
-          for (int w = 0; w < PAT_WARPS; ++w) mm = fmaxf(mm, sm_m[w * NR + r]);
-          const float mu = mm == -INFINITY ? 0.0f : mm;
-#pragma unroll
-          for (int w = 0; w < PAT_WARPS; ++w) ll = fmaf(sm_l[w * NR + r], pat_exp2(sm_m[w * NR + r] - mu), ll);
-          const float f = pat_exp2(m[nt][e] - mu);
-          inv[nt][e] = !whole ? 1.0f : ll == 0.0f ? 0.0f : 1.0f / ll;
-#pragma unroll
-          for (int mt = 0; mt < MT; ++mt) o[mt][nt][e] *= f, o[mt][nt][e + 2] *= f;
-          if (warp == 0 && lane < 4) {
-            if (whole)
-              paged_store_lse(p, at.b, at.g, r0 + r, mm, ll);
-            else
-              p.part_ml[slot * NR + r] = make_float2(mm, ll);
-          }
-        }
-#pragma unroll
-      for (int nt = 0; nt < NT; ++nt) {
-        const int r = r0 + nt * 8 + (lane >> 2);
-        const long long row = r < p.rows ? paged_row(p, at.b, at.g, r) : -1;
-        if (nt > 0) __syncthreads();
-#pragma unroll
-        for (int mt = 0; mt < MT; ++mt)
-          obuf[(warp * MT + mt) * 32 + lane] = make_float4(o[mt][nt][0], o[mt][nt][1], o[mt][nt][2], o[mt][nt][3]);
-        __syncthreads();
-#pragma unroll
-        for (int k = 0; k < MT / PAT_WARPS; ++k) {
-          const int mt = warp + k * PAT_WARPS;
-          const float4* from = obuf + mt * 32 + lane;
-          float4 a = from[0];
-#pragma unroll
-          for (int w = 1; w < PAT_WARPS; ++w) {
-            const float4 x = from[w * MT * 32];
-            a.x += x.x, a.y += x.y, a.z += x.z, a.w += x.w;
-          }
-          a.x *= inv[nt][0], a.y *= inv[nt][1], a.z *= inv[nt][0], a.w *= inv[nt][1];
-          if (whole)
-            paged_store<BF, D>(p, row, mt, lane, a);
-          else
-            p.part_o[(((long long)slot * MT + mt) * NT + nt) * 32 + lane] = a;
-        }
-      }
-      __syncthreads();
-      if (!whole && tid == 0) {
-        const PagedCut cut = s_range;
-        const int head = at.w - at.unit, c0 = cut.cta_of(head);   // the sequence's first unit and CTA
-        s_cut[part] = {at.b, at.g, r0, c0, cut.cta_of(head + at.nu - 1) - c0 + 1};
-        // the first part at once, so that it is not this CTA that everyone else waits for in the end
-        if (part == 0) s_join[0] = paged_arrive(p, s_cut[0]);
-      }
+        for (int e = 0; e < 2; ++e) m[nt][e] *= p.scale_log2;
+      paged_finish<D, NT, BF, false>(p, at, ends && first_unit == 0, first_unit == 0 ? 1 : 0, o, m, l, obuf, sm_m, sm_l, s_range,
+                                     s_cut, s_join);
     }
     at.next(p);
   }
-  // cut sequences (at most the range's first and last): the last of their CTAs to get here joins the parts
-  if (tid == 0 && s_cut[1].parts > 0) s_join[1] = paged_arrive(p, s_cut[1]);
-  __syncthreads();
-  for (int k = 0; k < 2; ++k) {
-    const PagedPart x = s_cut[k];
-    if (s_join[k]) paged_join<D, NT, BF>(p, x.b, x.g, x.r0, x.c0, x.parts, reinterpret_cast<float*>(obuf));
-    __syncthreads();
-  }
+  paged_leave<D, NT, BF, false>(p, s_cut, s_join, obuf);
 }
 
 }  // namespace simsd

@@ -7,12 +7,11 @@
 
 #include <algorithm>
 #include <cmath>
-#include <mutex>
-#include <utility>
 
 #include "paged.cuh"
 #include "paged_attn.cuh"
 #include "paged_attn_tc.cuh"
+#include "serving_host.cuh"
 #include "simsd_b200.h"
 #include "spec_verify.cuh"
 
@@ -20,77 +19,17 @@ using namespace simsd;
 
 namespace {
 
-constexpr int kMaxDev = 64;
-constexpr int kMaxSmem = 227 * 1024;
-std::mutex g_attr_mu;
-
-inline size_t align256(size_t v) { return (v + 255) & ~size_t(255); }
-inline long long cdiv(long long a, long long b) { return (a + b - 1) / b; }
-inline bool al16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15) == 0; }
-
-// Launch on `s`; as a programmatic dependent of the kernel before it on the
-// stream when `dependent` (the second kernel of one call) or SIMSD_LAUNCH_PDL is
-// set.  Every kernel here starts with griddepcontrol.wait.
-template <typename... KArgs, typename... Args>
-int launch_on(void (*kern)(KArgs...), dim3 grid, int block, size_t smem, void* s, bool dependent, Args&&... args) {
-  cudaLaunchConfig_t cfg = {};
-  cfg.gridDim = grid;
-  cfg.blockDim = dim3((unsigned)block);
-  cfg.dynamicSmemBytes = smem;
-  cfg.stream = (cudaStream_t)s;
-  cudaLaunchAttribute attr[1];
-  if (dependent || (simsd_get_launch_flags() & SIMSD_LAUNCH_PDL)) {
-    attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
-    attr[0].val.programmaticStreamSerializationAllowed = 1;
-    cfg.attrs = attr;
-    cfg.numAttrs = 1;
-  }
-  if (cudaLaunchKernelEx(&cfg, kern, std::forward<Args>(args)...) != cudaSuccess) return SIMSD_ERR_LAUNCH;
-  return cudaGetLastError() == cudaSuccess ? SIMSD_OK : SIMSD_ERR_LAUNCH;
-}
-
 // 16-byte rows of a paged cache
 int cache_check(const void* k, const void* v, int64_t ld_page, int64_t ld_head, int64_t ld_tok) {
   if (!al16(k) || !al16(v) || (ld_page & 7) || (ld_head & 7) || (ld_tok & 7)) return SIMSD_ERR_ALIGN;
   return SIMSD_OK;
 }
 
-// What paged attention does with G L rows per KV head: the rows of a CTA (up to 16
-// with mma.sync, 32, 64 or 128 with tcgen05; more go in tiles of 128), the grid, and
-// the workspace: the arrival counters, then two parts per CTA (the end of a sequence
-// it started inside, the start of one it leaves unfinished).
-struct PagedPlan {
-  int nr, grid;
-  size_t ml_at, bytes;
-};
+// Up to 16 rows per KV head with mma.sync, 32, 64 or 128 with tcgen05; more go in tiles of 128.
 PagedPlan paged_plan(int L, int G, int D) {
-  PagedPlan p;
   const long long rows = (long long)L * G;
-  p.nr = rows <= 8 ? 8 : rows <= 16 ? 16 : rows <= 32 ? 32 : rows <= 64 ? 64 : 128;
-  const int sms = simsd_device_sm_count();
-  p.grid = std::min((p.nr <= 16 ? PAT_CTAS_PER_SM : 1) * (sms > 0 ? sms : 148), SIMSD_PAGED_COUNTER_BYTES / (int)sizeof(int));
-  p.ml_at = SIMSD_PAGED_COUNTER_BYTES + align256((size_t)2 * p.grid * D * p.nr * sizeof(float));
-  p.bytes = p.ml_at + align256((size_t)2 * p.grid * p.nr * sizeof(float2));
-  return p;
-}
-
-PagedDiv paged_div(int d) {
-  int sh = 0;
-  while ((1LL << sh) < d) ++sh;
-  return {(uint32_t)(((1ULL << (31 + sh)) + d - 1) / d), 31 + sh};
-}
-
-// Raise a kernel's shared-memory limit once per device.
-template <typename F>
-int allow_smem(F* kern, int bytes, bool* done) {
-  int dev = -1;
-  if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= kMaxDev) return SIMSD_ERR_DEVICE;
-  std::lock_guard<std::mutex> lk(g_attr_mu);
-  if (done[dev]) return SIMSD_OK;
-  if (cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes) != cudaSuccess)
-    return SIMSD_ERR_LAUNCH;
-  done[dev] = true;
-  return SIMSD_OK;
+  if (rows <= 16) return paged_plan_tiles(rows, D);
+  return paged_plan_of(rows <= 32 ? 32 : rows <= 64 ? 64 : 128, 1, D);
 }
 
 // How verification splits its rows.  A warp takes 4 blocks of 1024 logits where that
@@ -103,7 +42,7 @@ struct SpecPlan {
 };
 SpecPlan spec_plan(int B, int K, int V) {
   SpecPlan p;
-  const int sms = simsd_device_sm_count() > 0 ? simsd_device_sm_count() : 148;
+  const int sms = sm_count();
   const long long all = (long long)B * (2 * K + 1) * V;
   p.blocks = all >= (long long)sms * 32 * 4 * SV_BLOCK ? 4 : 1;
   p.parts = (int)cdiv(V, p.blocks * SV_BLOCK);
@@ -132,18 +71,22 @@ int append(const PagedAppendArgs& a, void* stream) {
     const int rc = allow_smem(paged_append_kernel<D, BF>, kMaxSmem, done);
     if (rc != SIMSD_OK) return rc;
   }
-  const int sms = simsd_device_sm_count();
-  const int grid = std::min(a.T, PA_CTAS_PER_SM * (sms > 0 ? sms : 148));
+  const int grid = std::min(a.T, PA_CTAS_PER_SM * sm_count());
   return launch_on(paged_append_kernel<D, BF>, dim3((unsigned)grid), PA_THREADS, (size_t)smem, stream, false, a);
 }
 
-template <int D, int NT, bool BF>
+template <int D, int NT, bool BF, bool WIN>
 int attend(const PagedAttnArgs& a, const PagedPlan& pl, void* stream) {
   static bool done[kMaxDev];
   constexpr int smem = PatShape<D, NT>::BYTES;
-  const int rc = allow_smem(paged_attention_kernel<D, NT, BF>, smem, done);
+  const int rc = allow_smem(paged_attention_kernel<D, NT, BF, WIN>, smem, done);
   if (rc != SIMSD_OK) return rc;
-  return launch_on(paged_attention_kernel<D, NT, BF>, dim3((unsigned)pl.grid), PAT_THREADS, smem, stream, false, a);
+  return launch_on(paged_attention_kernel<D, NT, BF, WIN>, dim3((unsigned)pl.grid), PAT_THREADS, smem, stream, false, a);
+}
+// A window leaves few keys, so its rows go in tiles of 16 at most, each reading them again.
+template <int D, bool BF>
+int attend_window(const PagedAttnArgs& a, const PagedPlan& pl, void* stream) {
+  return pl.nr == 8 ? attend<D, 1, BF, true>(a, pl, stream) : attend<D, 2, BF, true>(a, pl, stream);
 }
 // A TMA map of a cache for loads of `block` tokens of one page and head; false where
 // the driver will not describe it (a stride of 0, say).
@@ -185,8 +128,8 @@ int attend_tc(const PagedAttnArgs& a, const PagedPlan& pl, void* stream) {
 template <int D, bool BF>
 int attend_rows(const PagedAttnArgs& a, const PagedPlan& pl, void* stream) {
   switch (pl.nr) {
-    case 8: return attend<D, 1, BF>(a, pl, stream);
-    case 16: return attend<D, 2, BF>(a, pl, stream);
+    case 8: return attend<D, 1, BF, false>(a, pl, stream);
+    case 16: return attend<D, 2, BF, false>(a, pl, stream);
     case 32: return attend_tc<D, 32, BF>(a, pl, stream);
     case 64: return attend_tc<D, 64, BF>(a, pl, stream);
     default: return attend_tc<D, 128, BF>(a, pl, stream);
@@ -253,59 +196,36 @@ int simsd_paged_attention(const void* q, const void* k_cache, const void* v_cach
                           int max_pages, const int32_t* seq_lens, const uint8_t* tail_mask, int64_t ldm_b, int64_t ldm_t,
                           int B, int L, int Hq, int Hk, int head_dim, float scale, void* o, float* lse, int dtype,
                           void* workspace, size_t workspace_bytes, int* err_word, void* stream) {
-  if (B < 0 || L < 0 || Hq < 1 || Hk < 1 || Hq % Hk || num_pages < 1 || page_size < 1 || max_pages < 0)
-    return SIMSD_ERR_SHAPE;
-  if (dtype != SIMSD_BF16 && dtype != SIMSD_F16) return SIMSD_ERR_DTYPE;
-  if (head_dim != 64 && head_dim != 128) return SIMSD_ERR_UNSUPPORTED;
-  if (B == 0 || L == 0) return SIMSD_OK;
-  if ((int64_t)max_pages * page_size > 0x7fff0000LL) return SIMSD_ERR_UNSUPPORTED;
-  if (!q || !k_cache || !v_cache || (max_pages > 0 && !page_table) || !seq_lens || !o || ld_table < 0)
-    return SIMSD_ERR_SHAPE;
-  if (!al16(q) || !al16(o)) return SIMSD_ERR_ALIGN;
-  int rc = cache_check(k_cache, v_cache, ld_page, ld_head, ld_tok);
-  if (rc != SIMSD_OK) return rc;
-  if (workspace == nullptr || workspace_bytes < simsd_paged_attention_workspace_size(L, Hq, Hk, head_dim))
-    return SIMSD_ERR_WORKSPACE;
+  return simsd_paged_attention_window(q, k_cache, v_cache, num_pages, page_size, ld_page, ld_head, ld_tok, page_table, ld_table,
+                                      max_pages, seq_lens, tail_mask, ldm_b, ldm_t, B, L, Hq, Hk, head_dim, scale, 0, 0, o, lse,
+                                      dtype, workspace, workspace_bytes, err_word, stream);
+}
+
+int simsd_paged_attention_window(const void* q, const void* k_cache, const void* v_cache, int num_pages, int page_size,
+                                 int64_t ld_page, int64_t ld_head, int64_t ld_tok, const int32_t* page_table,
+                                 int64_t ld_table, int max_pages, const int32_t* seq_lens, const uint8_t* tail_mask,
+                                 int64_t ldm_b, int64_t ldm_t, int B, int L, int Hq, int Hk, int head_dim, float scale,
+                                 int window, int sinks, void* o, float* lse, int dtype, void* workspace,
+                                 size_t workspace_bytes, int* err_word, void* stream) {
   PagedAttnArgs a;
-  a.q = q;
-  a.k_cache = k_cache;
-  a.v_cache = v_cache;
-  a.page_table = page_table;
-  a.seq_lens = seq_lens;
-  a.tail = tail_mask;
-  a.o = o;
-  a.lse = lse;
-  a.err = err_word;
+  int rc = paged_attn_request(a, q, k_cache, v_cache, num_pages, page_size, page_table, ld_table, max_pages, seq_lens, tail_mask,
+                              ldm_b, ldm_t, B, L, Hq, Hk, head_dim, scale, window, sinks, o, lse, dtype, err_word);
+  if (rc != SIMSD_OK || B == 0 || L == 0) return rc;
+  rc = cache_check(k_cache, v_cache, ld_page, ld_head, ld_tok);
+  if (rc != SIMSD_OK) return rc;
   a.ld_page = ld_page;
   a.ld_head = ld_head;
   a.ld_tok = ld_tok;
-  a.ld_table = ld_table;
-  a.ldm_b = ldm_b;
-  a.ldm_t = ldm_t;
-  a.B = B;
-  a.L = L;
-  a.Hq = Hq;
-  a.Hk = Hk;
-  a.G = Hq / Hk;
-  a.num_pages = num_pages;
-  a.page_size = page_size;
-  a.max_pages = max_pages;
-  a.page_div = paged_div(page_size);
-  a.g_div = paged_div(a.G);
-  a.q_sign = scale < 0.0f ? 0x80008000u : 0u;
-  a.scale_log2 = std::max(std::fabs(scale) * 1.4426950408889634f, 1e-30f);
-  const PagedPlan pl = paged_plan(L, a.G, head_dim);
-  a.rows = a.G * L;
-  a.row_tiles = (a.rows + pl.nr - 1) / pl.nr;
-  if ((long long)B * Hk * a.row_tiles * ((int64_t)max_pages * page_size / PAT_TK + 1 + PAGED_END_MAX) > 0x7fffffffLL)
-    return SIMSD_ERR_UNSUPPORTED;
-  uint8_t* ws = reinterpret_cast<uint8_t*>(workspace);
-  a.arrived = reinterpret_cast<int*>(ws);
-  a.part_o = reinterpret_cast<float4*>(ws + SIMSD_PAGED_COUNTER_BYTES);
-  a.part_ml = reinterpret_cast<float2*>(ws + pl.ml_at);
-  if (dtype == SIMSD_BF16)
-    return head_dim == 64 ? attend_rows<64, true>(a, pl, stream) : attend_rows<128, true>(a, pl, stream);
-  return head_dim == 64 ? attend_rows<64, false>(a, pl, stream) : attend_rows<128, false>(a, pl, stream);
+  const PagedPlan pl = window ? paged_plan_tiles(a.rows, head_dim) : paged_plan(L, a.G, head_dim);
+  rc = paged_attn_plan(a, pl, workspace, workspace_bytes);
+  if (rc != SIMSD_OK) return rc;
+  const bool bf = dtype == SIMSD_BF16;
+  if (window) {
+    if (head_dim == 64) return bf ? attend_window<64, true>(a, pl, stream) : attend_window<64, false>(a, pl, stream);
+    return bf ? attend_window<128, true>(a, pl, stream) : attend_window<128, false>(a, pl, stream);
+  }
+  if (head_dim == 64) return bf ? attend_rows<64, true>(a, pl, stream) : attend_rows<64, false>(a, pl, stream);
+  return bf ? attend_rows<128, true>(a, pl, stream) : attend_rows<128, false>(a, pl, stream);
 }
 
 size_t simsd_speculative_verify_workspace_size(int B, int K, int V) {

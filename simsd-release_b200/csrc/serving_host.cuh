@@ -1,0 +1,142 @@
+// What the translation units of the batched serving operators share on the host.
+#pragma once
+#include <cuda_runtime.h>
+
+#include <algorithm>
+#include <cmath>
+#include <mutex>
+#include <utility>
+
+#include "paged_attn.cuh"
+#include "simsd_b200.h"
+
+namespace simsd {
+
+constexpr int kMaxDev = 64;
+constexpr int kMaxSmem = 227 * 1024;
+
+inline size_t align256(size_t v) { return (v + 255) & ~size_t(255); }
+inline long long cdiv(long long a, long long b) { return (a + b - 1) / b; }
+inline bool al16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15) == 0; }
+inline int sm_count() {
+  const int n = simsd_device_sm_count();
+  return n > 0 ? n : 148;
+}
+
+// Launch on `s`; as a programmatic dependent of the kernel before it on the
+// stream when `dependent` (the second kernel of one call) or SIMSD_LAUNCH_PDL is
+// set.  Every kernel here starts with griddepcontrol.wait.
+template <typename... KArgs, typename... Args>
+int launch_on(void (*kern)(KArgs...), dim3 grid, int block, size_t smem, void* s, bool dependent, Args&&... args) {
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = grid;
+  cfg.blockDim = dim3((unsigned)block);
+  cfg.dynamicSmemBytes = smem;
+  cfg.stream = (cudaStream_t)s;
+  cudaLaunchAttribute attr[1];
+  if (dependent || (simsd_get_launch_flags() & SIMSD_LAUNCH_PDL)) {
+    attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr[0].val.programmaticStreamSerializationAllowed = 1;
+    cfg.attrs = attr;
+    cfg.numAttrs = 1;
+  }
+  if (cudaLaunchKernelEx(&cfg, kern, std::forward<Args>(args)...) != cudaSuccess) return SIMSD_ERR_LAUNCH;
+  return cudaGetLastError() == cudaSuccess ? SIMSD_OK : SIMSD_ERR_LAUNCH;
+}
+
+inline PagedDiv paged_div(int d) {
+  int sh = 0;
+  while ((1LL << sh) < d) ++sh;
+  return {(uint32_t)(((1ULL << (31 + sh)) + d - 1) / d), 31 + sh};
+}
+
+// Raise a kernel's shared-memory limit once per device.
+template <typename F>
+int allow_smem(F* kern, int bytes, bool* done) {
+  int dev = -1;
+  if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= kMaxDev) return SIMSD_ERR_DEVICE;
+  static std::mutex mu;
+  std::lock_guard<std::mutex> lk(mu);
+  if (done[dev]) return SIMSD_OK;
+  if (cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes) != cudaSuccess)
+    return SIMSD_ERR_LAUNCH;
+  done[dev] = true;
+  return SIMSD_OK;
+}
+
+// How paged attention runs the G L rows of a KV head: `nr` rows a CTA, the grid, and the
+// workspace: the arrival counters, then two parts per CTA (the end of a sequence
+// it started inside, the start of one it leaves unfinished).
+struct PagedPlan {
+  int nr, grid;
+  size_t ml_at, bytes;
+};
+inline PagedPlan paged_plan_of(int nr, int ctas_per_sm, int D) {
+  PagedPlan p;
+  p.nr = nr;
+  p.grid = std::min(ctas_per_sm * sm_count(), SIMSD_PAGED_COUNTER_BYTES / (int)sizeof(int));
+  p.ml_at = SIMSD_PAGED_COUNTER_BYTES + align256((size_t)2 * p.grid * D * p.nr * sizeof(float));
+  p.bytes = p.ml_at + align256((size_t)2 * p.grid * p.nr * sizeof(float2));
+  return p;
+}
+// with mma.sync: tiles of 8 or 16 rows
+inline PagedPlan paged_plan_tiles(long long rows, int D) { return paged_plan_of(rows <= 8 ? 8 : 16, PAT_CTAS_PER_SM, D); }
+
+// A request of paged attention, the sizes that every form of it refuses, and its arguments
+// but for what goes by the form: the caches' strides and the plan's part.
+inline int paged_attn_request(PagedAttnArgs& a, const void* q, const void* k_cache, const void* v_cache, int num_pages,
+                              int page_size, const int32_t* page_table, int64_t ld_table, int max_pages, const int32_t* seq_lens,
+                              const uint8_t* tail_mask, int64_t ldm_b, int64_t ldm_t, int B, int L, int Hq, int Hk, int head_dim,
+                              float scale, int window, int sinks, void* o, float* lse, int dtype, int* err_word) {
+  if (B < 0 || L < 0 || Hq < 1 || Hk < 1 || Hq % Hk || num_pages < 1 || page_size < 1 || max_pages < 0 || window < 0 || sinks < 0)
+    return SIMSD_ERR_SHAPE;
+  if (dtype != SIMSD_BF16 && dtype != SIMSD_F16) return SIMSD_ERR_DTYPE;
+  if (head_dim != 64 && head_dim != 128) return SIMSD_ERR_UNSUPPORTED;
+  if (B == 0 || L == 0) return SIMSD_OK;
+  if ((int64_t)max_pages * page_size > 0x7fff0000LL) return SIMSD_ERR_UNSUPPORTED;
+  if (!q || !k_cache || !v_cache || (max_pages > 0 && !page_table) || !seq_lens || !o || ld_table < 0)
+    return SIMSD_ERR_SHAPE;
+  if (!al16(q) || !al16(o)) return SIMSD_ERR_ALIGN;
+  a.q = q;
+  a.k_cache = k_cache;
+  a.v_cache = v_cache;
+  a.page_table = page_table;
+  a.seq_lens = seq_lens;
+  a.tail = tail_mask;
+  a.o = o;
+  a.lse = lse;
+  a.err = err_word;
+  a.ld_table = ld_table;
+  a.ldm_b = ldm_b;
+  a.ldm_t = ldm_t;
+  a.B = B;
+  a.L = L;
+  a.Hq = Hq;
+  a.Hk = Hk;
+  a.G = Hq / Hk;
+  a.num_pages = num_pages;
+  a.page_size = page_size;
+  a.max_pages = max_pages;
+  a.page_div = paged_div(page_size);
+  a.g_div = paged_div(a.G);
+  // more than any length of either counts as that
+  a.window = std::min(window, 0x40000000);
+  a.sinks = std::min(sinks, 0x40000000);
+  a.q_sign = scale < 0.0f ? 0x80008000u : 0u;
+  a.scale_log2 = std::max(std::fabs(scale) * 1.4426950408889634f, 1e-30f);
+  a.rows = a.G * L;
+  return SIMSD_OK;
+}
+inline int paged_attn_plan(PagedAttnArgs& a, const PagedPlan& pl, void* workspace, size_t workspace_bytes) {
+  if (workspace == nullptr || workspace_bytes < pl.bytes) return SIMSD_ERR_WORKSPACE;
+  a.row_tiles = (a.rows + pl.nr - 1) / pl.nr;
+  if ((long long)a.B * a.Hk * a.row_tiles * ((int64_t)a.max_pages * a.page_size / PAT_TK + 1 + PAGED_END_MAX) > 0x7fffffffLL)
+    return SIMSD_ERR_UNSUPPORTED;
+  uint8_t* ws = reinterpret_cast<uint8_t*>(workspace);
+  a.arrived = reinterpret_cast<int*>(ws);
+  a.part_o = reinterpret_cast<float4*>(ws + SIMSD_PAGED_COUNTER_BYTES);
+  a.part_ml = reinterpret_cast<float2*>(ws + pl.ml_at);
+  return SIMSD_OK;
+}
+
+}  // namespace simsd

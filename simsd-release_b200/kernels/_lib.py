@@ -89,6 +89,18 @@ SIGNATURES: dict[str, tuple] = {
     "simsd_paged_attention_workspace_size": (_S, [_I, _I, _I, _I]),
     "simsd_paged_attention": (_I, [_P, _P, _P, _I, _I, _L, _L, _L, _P, _L, _I, _P, _P, _L, _L, _I, _I, _I, _I, _I, _F,
                                    _P, _P, _I, _P, _S, _P, _P]),
+    "simsd_paged_attention_window": (_I, [_P, _P, _P, _I, _I, _L, _L, _L, _P, _L, _I, _P, _P, _L, _L, _I, _I, _I, _I, _I,
+                                          _F, _I, _I, _P, _P, _I, _P, _S, _P, _P]),
+    "simsd_paged_append8": (_I, [_P, _L, _L, _I, _I, _I, _I, _I, _I, _P, _P, _F, _P, _P, _L, _P, _L, _I, _P, _P, _P, _P, _P,
+                                 _P, _P, _I, _I, _I, _L, _L, _L, _L, _L, _L, _I, _P, _P]),
+    "simsd_paged_attention8_workspace_size": (_S, [_I, _I, _I, _I]),
+    "simsd_paged_attention8": (_I, [_P, _P, _P, _P, _P, _I, _I, _I, _L, _L, _L, _L, _L, _L, _P, _L, _I, _P, _P, _L, _L, _I,
+                                    _I, _I, _I, _I, _F, _I, _I, _P, _P, _I, _P, _S, _P, _P]),
+    "simsd_paged_reserve": (_I, [_P, _L, _I, _P, _P, _P, _P, _I, _P, _I, _I, _I, _P, _P, _P, _P, _S, _P, _P]),
+    "simsd_paged_release": (_I, [_P, _L, _I, _P, _P, _I, _P, _P, _I, _I, _P, _S, _P, _P]),
+    "simsd_adjust_logits": (_I, [_P, _L, _L, _P, _L, _L, _I, _I, _I, _I, _P, _L, _P, _L, _P, _L, _P, _P, _P, _P, _L, _P, _L,
+                                 _I, _P, _L, _L, _P, _P]),
+    "simsd_count_tokens": (_I, [_P, _L, _P, _L, _I, _I, _I, _P, _P]),
     "simsd_speculative_verify_workspace_size": (_S, [_I, _I, _I]),
     "simsd_speculative_verify": (_I, [_P, _L, _L, _P, _L, _L, _P, _L, _P, _L, _P, _L, _P, _P, _I, _I, _I, _I, _P, _P,
                                       _P, _P, _S, _P, _P]),
@@ -121,7 +133,8 @@ def lib() -> ctypes.CDLL:
         # Over the streams' scratch, the GIL orders one thread's calls with another's (the
         # native binding holds it too): a verification is two launches on the same bytes.
         held = ctypes.PyDLL(str(LIB_PATH))
-        for name in ("simsd_paged_attention", "simsd_speculative_verify"):
+        for name in ("simsd_paged_attention", "simsd_paged_attention_window", "simsd_paged_attention8", "simsd_paged_reserve",
+                     "simsd_paged_release", "simsd_speculative_verify"):
             fn = getattr(held, name)
             fn.restype, fn.argtypes = SIGNATURES[name]
             setattr(L, name, fn)
@@ -129,8 +142,10 @@ def lib() -> ctypes.CDLL:
     return _lib
 
 
-_BOUND = ("simsd_paged_append", "simsd_paged_attention", "simsd_paged_attention_workspace_size",
-          "simsd_speculative_verify", "simsd_speculative_verify_workspace_size")
+_BOUND = ("simsd_paged_append", "simsd_paged_attention_window", "simsd_paged_attention_workspace_size",
+          "simsd_speculative_verify", "simsd_speculative_verify_workspace_size", "simsd_paged_append8",
+          "simsd_paged_attention8", "simsd_paged_attention8_workspace_size", "simsd_paged_reserve", "simsd_paged_release",
+          "simsd_adjust_logits", "simsd_count_tokens")
 _binding = None
 
 
@@ -142,6 +157,7 @@ class _CtypesOnly:
         return None
 
     paged_attention = speculative_verify = paged_append
+    paged_append8 = paged_attention8 = paged_reserve = paged_release = adjust_logits = count_tokens = paged_append
 
     @staticmethod
     def forget():

@@ -3,12 +3,13 @@
 * `paged_append(qkv, ...)` — q/k RMSNorm (optional), rotary embedding and the
   write of each token's key and value into its cache slot.
 * `paged_attention(q, ...)` — attention of each sequence's newest token, or of
-  its L drafted ones, over its pages.
+  its L drafted ones, over its pages, or through a sliding window over them.
 * `rope_table(n, dim, theta)` — the fp32 cos/sin rows `paged_append` reads.
 
 The cache is a pair of tensors [pages, kv_heads, page_size, head_dim] with a unit
 last stride; a token-major cache [pages, page_size, kv_heads, head_dim] is passed
-as its `.transpose(1, 2)`.  Slot s is token s % page_size of page s // page_size.
+as its `.transpose(1, 2)`.  Slot s is token s % page_size of page s // page_size (`kernels/paged_tables.py` makes
+slots and page tables on the device; `kernels/paged_cache8.py` holds the cache in 8 bits).
 The reference keeps one static cache per sequence
 (speculative_decoding/cache_aware.py:195-215); it has no paged form.
 
@@ -41,7 +42,7 @@ _current_device = torch._C._cuda_getDevice
 
 def _check_cache(what: str, k_cache: torch.Tensor, v_cache: torch.Tensor, kv_heads: int, dtype: torch.dtype) -> None:
     if k_cache.dtype != dtype or v_cache.dtype != dtype:
-        raise TypeError(f"{what}: the caches must have the activations' type {dtype}, got {k_cache.dtype} / {v_cache.dtype}")
+        raise TypeError(f"{what}: the caches must be {dtype}, got {k_cache.dtype} / {v_cache.dtype}")
     if k_cache.ndim != 4 or k_cache.shape != v_cache.shape or k_cache.shape[1] != kv_heads:
         raise ValueError(f"{what}: k_cache and v_cache must both be [pages, {kv_heads}, page_size, head_dim], got "
                          f"{tuple(k_cache.shape)} / {tuple(v_cache.shape)}")
@@ -52,6 +53,20 @@ def _check_cache(what: str, k_cache: torch.Tensor, v_cache: torch.Tensor, kv_hea
 def _on_16_bytes(t: torch.Tensor | None) -> torch.Tensor | None:
     """t, copied where the kernels' 16-byte loads cannot start at its first element."""
     return t if t is None or t.data_ptr() % 16 == 0 else t.clone()
+
+
+def _mask_strides(tail_mask: torch.Tensor | None):
+    """(tail_mask with a unit last stride, its strides of a sequence and of a query)."""
+    if tail_mask is None:
+        return None, 0, 0
+    if tail_mask.stride(-1) != 1:
+        tail_mask = tail_mask.contiguous()
+    return tail_mask, tail_mask.stride(0) if tail_mask.ndim == 3 else 0, tail_mask.stride(-2)
+
+
+def _window(window: int | None, sinks: int) -> tuple[int, int]:
+    """What the library takes: 0 for no window; numbers past any length count as the largest."""
+    return 0 if window is None else min(window, 0x7fffffff), min(sinks, 0x7fffffff)
 
 
 def _check_append(qkv, heads, kv_heads, k_cache, v_cache, slots, positions, cos, sin, q_weight, k_weight) -> None:
@@ -122,34 +137,39 @@ def paged_append(qkv: torch.Tensor, heads: int, kv_heads: int, k_cache: torch.Te
     return q
 
 
-def _check_attention(q, k_cache, v_cache, page_table, seq_lens, tail_mask) -> None:
-    """Raise what is wrong with a request of paged_attention."""
+def _check_attention(q, k_cache, v_cache, page_table, seq_lens, tail_mask, window, sinks, what="paged_attention",
+                     cache_dtype=None) -> None:
+    """Raise what is wrong with a request of paged_attention (or, as `what`, of paged_attention8)."""
     if q.dtype not in _HALF:
-        raise TypeError(f"paged_attention takes bf16 or fp16 queries, got {q.dtype}")
+        raise TypeError(f"{what} takes bf16 or fp16 queries, got {q.dtype}")
     if q.ndim not in (3, 4):
         raise ValueError(f"q must be [B, L, heads, D] or [B, heads, D], got {tuple(q.shape)}")
     B, Hq, D = q.shape[0], q.shape[-2], q.shape[-1]
     L = q.shape[1] if q.ndim == 4 else 1
     Hk = k_cache.shape[1] if k_cache.ndim == 4 else 0
-    _check_cache("paged_attention", k_cache, v_cache, Hk, q.dtype)
+    _check_cache(what, k_cache, v_cache, Hk, cache_dtype or q.dtype)
     if k_cache.shape[3] != D or Hk < 1 or Hq < 1 or Hq % Hk:
         raise ValueError(f"q heads {Hq} x {D} do not go with the cache's {Hk} x {k_cache.shape[3]}")
     if page_table.dtype != torch.int32 or seq_lens.dtype != torch.int32:
-        raise TypeError("paged_attention: page_table and seq_lens are int32")
+        raise TypeError(f"{what}: page_table and seq_lens are int32")
     if page_table.ndim != 2 or page_table.shape[0] != B or seq_lens.shape != (B,):
         raise ValueError(f"page_table must be [{B}, max_pages] and seq_lens [{B}], got {tuple(page_table.shape)} / "
                          f"{tuple(seq_lens.shape)}")
     if tail_mask is not None:
         if tail_mask.dtype != torch.bool:
-            raise TypeError("paged_attention: tail_mask is bool")
+            raise TypeError(f"{what}: tail_mask is bool")
         if tail_mask.shape != (L, L) and tail_mask.shape != (B, L, L):
             raise ValueError(f"tail_mask must be [{L}, {L}] or [{B}, {L}, {L}], got {tuple(tail_mask.shape)}")
+    if window is not None and window < 1:
+        raise ValueError(f"window must be at least 1 (None: no window), got {window}")
+    if sinks < 0:
+        raise ValueError(f"sinks must not be negative, got {sinks}")
     _lib.require_cuda(q, k_cache, v_cache, page_table, seq_lens, tail_mask)
 
 
 def paged_attention(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor, page_table: torch.Tensor,
                     seq_lens: torch.Tensor, scale: float | None = None, tail_mask: torch.Tensor | None = None,
-                    return_lse: bool = False):
+                    return_lse: bool = False, window: int | None = None, sinks: int = 0):
     """Attention of q [B, L, heads, D] (or [B, heads, D], L = 1) over each
     sequence's pages -> o of q's shape, or (o, lse) with lse [B, L, heads] (fp32,
     natural log of the softmax's denominator).
@@ -163,27 +183,25 @@ def paged_attention(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tenso
     is set.  A query that sees no key (an empty sequence, a mask without any) gets
     o = 0 and lse = -inf.  Only visible keys count: what stale cache memory or a
     masked key holds, NaN included, does not reach the output.  scale: D ** -0.5
-    when None.  Lengths are read on the device, so the call can be captured in a
+    when None.  window: query t, at position x = seq_lens[b] - L + t, sees key j only where
+    also j > x - window or j < sinks: the newest `window` keys and the first `sinks`.  Keys
+    that no query sees are not read, and pages that hold nothing else may have been given
+    back (their entries are not read).  Lengths are read on the device, so the call can be captured in a
     CUDA graph and replayed as the sequences grow.
     """
-    o = _lib.binding().paged_attention(q, k_cache, v_cache, page_table, seq_lens, scale, tail_mask, return_lse)
+    o = _lib.binding().paged_attention(q, k_cache, v_cache, page_table, seq_lens, scale, tail_mask, return_lse, window, sinks)
     if o is not None:
         return o
     if torch.is_grad_enabled() and (q.requires_grad or k_cache.requires_grad or v_cache.requires_grad):
         raise RuntimeError("paged_attention is a forward-only inference kernel.")
-    _check_attention(q, k_cache, v_cache, page_table, seq_lens, tail_mask)
+    _check_attention(q, k_cache, v_cache, page_table, seq_lens, tail_mask, window, sinks)
     dev, shape, strides = q.get_device(), k_cache.shape, k_cache.stride()
     if _current_device() != dev:
         with torch.cuda.device(dev):
-            return paged_attention(q, k_cache, v_cache, page_table, seq_lens, scale, tail_mask, return_lse)
+            return paged_attention(q, k_cache, v_cache, page_table, seq_lens, scale, tail_mask, return_lse, window, sinks)
     B, Hq, D = q.shape[0], q.shape[-2], q.shape[-1]
     L = q.shape[1] if q.ndim == 4 else 1
-    ldm_b = ldm_t = 0
-    if tail_mask is not None:
-        if tail_mask.stride(-1) != 1:
-            tail_mask = tail_mask.contiguous()
-        ldm_t = tail_mask.stride(-2)
-        ldm_b = tail_mask.stride(0) if tail_mask.ndim == 3 else 0
+    tail_mask, ldm_b, ldm_t = _mask_strides(tail_mask)
     q, seq_lens = _on_16_bytes(q.contiguous()), seq_lens.contiguous()
     if page_table.stride(1) != 1:
         page_table = page_table.contiguous()
@@ -192,11 +210,11 @@ def paged_attention(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tenso
     lib, stream = _lib.lib(), _current_stream(dev)
     ws, ws_bytes, _owner = _lib.stream_scratch(dev, stream, lib.simsd_paged_attention_workspace_size(L, Hq, shape[1], D),
                                                _lib.PAGED_COUNTER_BYTES)
-    rc = lib.simsd_paged_attention(
+    rc = lib.simsd_paged_attention_window(
         q.data_ptr(), k_cache.data_ptr(), v_cache.data_ptr(), shape[0], shape[2], strides[0], strides[1], strides[2],
         page_table.data_ptr(), page_table.stride(0), page_table.shape[1], seq_lens.data_ptr(),
         tail_mask.data_ptr() if tail_mask is not None else None, ldm_b, ldm_t, B, L, Hq, shape[1], D,
-        D ** -0.5 if scale is None else scale, o.data_ptr(), lse.data_ptr() if return_lse else None, _HALF[q.dtype], ws,
+        D ** -0.5 if scale is None else scale, *_window(window, sinks), o.data_ptr(), lse.data_ptr() if return_lse else None, _HALF[q.dtype], ws,
         ws_bytes, _lib.error_ptr(dev), stream)
     _lib.check(rc, "paged_attention")
     return (o, lse) if return_lse else o
