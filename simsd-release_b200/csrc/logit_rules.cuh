@@ -6,13 +6,14 @@
 //   x = x - frequency[b] c - presence[b]                where c > 0
 //   x = x + the biases of v in sequence b's list, summed in the list's order
 //   x = -inf                                            where allowed[b, i] lacks v
-// in fp32, rounded once to the logits' type.
+// in fp32 (x times a factor plus one number, the division as a product with the reciprocal),
+// rounded once to the logits' type.
 //
 // HBM bounds it: every logit read and written once.  A CTA takes 2048 tokens of one
 // sequence through all its rows, so that counts, the prompt's bits and the biases are
-// read once a sequence and stay in registers; after row i the thread that owns drafted
-// token i counts it.  The next row is on its way while one is worked on, and tokens
-// without a rule (nearly all) cost a conversion there and back.
+// read once a sequence; what stays of them in registers is a number to add and a bit for each token.
+// After row i the thread that owns drafted token i counts it.  Several rows are on their way at a time.
+// Its threads look through the bias list, an entry each, for those on the CTA's tokens.
 #pragma once
 #include "spec_verify.cuh"
 
@@ -36,20 +37,21 @@ struct LogitRulesArgs {
   bool penal;               // one of the penalties is there
 };
 
-constexpr int LR_THREADS = 256, LR_EACH = 8, LR_TOKENS = LR_THREADS * LR_EACH;
+constexpr int LR_THREADS = 256, LR_EACH = 8, LR_TOKENS = LR_THREADS * LR_EACH, LR_LIST = 1024;
 
 // VEC: a thread owns 8 tokens in a row (16-byte loads and stores), else 8 tokens 32
 // apart, a warp's next to each other (rows that start anywhere).
 template <int DT, bool VEC>
-__global__ void __launch_bounds__(LR_THREADS) logit_rules_kernel(const LogitRulesArgs p) {
+__global__ void __launch_bounds__(LR_THREADS, 4) logit_rules_kernel(const LogitRulesArgs p) {
   griddep_launch_dependents();
   griddep_wait();
   constexpr int VECS = DT == 2 ? 2 : 1;           // 16-byte loads of 8 logits
-  __shared__ int s_id[LR_THREADS], s_n[LR_THREADS / 32];
-  __shared__ float s_val[LR_THREADS];
+  constexpr int ROWS = VEC && DT != 2 ? 4 : 2;    // rows in registers
+  constexpr int SIZE = DT == 2 ? 4 : 2;
+  __shared__ int s_draft[LR_THREADS], s_hit[LR_LIST], s_order[LR_LIST], s_hits;
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, b = blockIdx.y;
-  const int v0 = blockIdx.x * LR_TOKENS;
-  const int first = VEC ? v0 + tid * LR_EACH : v0 + warp * 32 * LR_EACH + lane;   // the thread's tokens: first + k step
+  const int v0 = blockIdx.x * LR_TOKENS, w0 = v0 + warp * 32 * LR_EACH;
+  const int first = VEC ? w0 + lane * LR_EACH : w0 + lane;   // the thread's tokens: first + k step
   constexpr int step = VEC ? 1 : 32;
   // the thread's place for a token of the CTA (0 .. LR_TOKENS - 1), or -1
   auto mine = [&](int at) {
@@ -69,89 +71,103 @@ __global__ void __launch_bounds__(LR_THREADS) logit_rules_kernel(const LogitRule
     return m;
   };
 
-  uint4 raw[2][VECS];                             // VEC: this row and the next
-  float val[2][VEC ? 1 : LR_EACH];                // else
-  uint32_t ok[2] = {0xffu, 0xffu};
-  long long draft[2] = {-1, -1};
-  auto fetch = [&](int i, int at) {
-    if (i >= p.R) return;
-    const long long off = b * p.ld_b + i * p.ld_r + first;
+  // rows that are on their way; the next one's places
+  uint4 raw[VEC ? ROWS : 1][VECS];
+  float val[VEC ? 1 : ROWS][LR_EACH];
+  uint32_t ok[ROWS];
+  const char* src = static_cast<const char*>(p.logits) + (b * p.ld_b + first) * SIZE;
+  const uint32_t* mask = p.allowed ? p.allowed + b * p.lda_b : nullptr;
+  int fetched = 0;
+  auto fetch = [&](int at) {
+    ok[at] = 0xffu;
+    if (fetched >= p.R) return;
     if constexpr (VEC) {
       if (first < p.V) {
-        const uint4* src = reinterpret_cast<const uint4*>(static_cast<const char*>(p.logits) + off * (DT == 2 ? 4 : 2));
 #pragma unroll
-        for (int x = 0; x < VECS; ++x) raw[at][x] = src[x];
+        for (int x = 0; x < VECS; ++x) raw[at][x] = reinterpret_cast<const uint4*>(src)[x];
       }
     } else {
 #pragma unroll
       for (int k = 0; k < LR_EACH; ++k)
-        if (first + k * step < p.V) val[at][k] = load_f(p.logits, off + k * step, DT);
+        if (first + k * step < p.V) val[at][k] = load_f(src, k * step, DT);
     }
-    if (p.allowed) ok[at] = bits(p.allowed + b * p.lda_b + i * p.lda_r);
-    draft[at] = p.drafts && i + 1 < p.R ? p.drafts[b * p.ld_d + i] : -1;
+    if (mask) ok[at] = bits(mask), mask += p.lda_r;
+    src += p.ld_r * SIZE;
+    ++fetched;
   };
-  fetch(0, 0);
+#pragma unroll
+  for (int x = 0; x < ROWS; ++x) fetch(x);
 
+  // what the sequence has, all of it sent for before any is waited for
+  float rep = 1.0f, pres = 0.0f, freq = 0.0f;
+  uint32_t again = 0;                             // tokens that the repetition penalty holds for
+  const int* counts = p.counts ? p.counts + b * p.ld_c + first : nullptr;
   int c[LR_EACH];
-  uint32_t met = 0, again = 0;                    // tokens counted, and those or in the prompt
 #pragma unroll
   for (int k = 0; k < LR_EACH; ++k) c[k] = 0;
-  float rep = 1.0f, pres = 0.0f, freq = 0.0f;
   if (p.penal) {
-    if (p.counts) {
-      const int* src = p.counts + b * p.ld_c + first;
+    if (counts) {
       if (VEC) {
         if (first < p.V) {
-          const int4 a = reinterpret_cast<const int4*>(src)[0], d = reinterpret_cast<const int4*>(src)[1];
+          const int4 a = reinterpret_cast<const int4*>(counts)[0], d = reinterpret_cast<const int4*>(counts)[1];
           c[0] = a.x, c[1] = a.y, c[2] = a.z, c[3] = a.w, c[4] = d.x, c[5] = d.y, c[6] = d.z, c[7] = d.w;
         }
       } else {
 #pragma unroll
         for (int k = 0; k < LR_EACH; ++k)
-          if (first + k * step < p.V) c[k] = src[k * step];
+          if (first + k * step < p.V) c[k] = counts[k * step];
       }
     }
     if (p.seen) again = bits(p.seen + b * p.ld_s);
-#pragma unroll
-    for (int k = 0; k < LR_EACH; ++k) met |= (uint32_t)(c[k] > 0) << k;
-    again |= met;
     if (p.repetition) rep = p.repetition[b];
     if (p.presence) pres = p.presence[b];
     if (p.frequency) freq = p.frequency[b];
   }
-  float bias[LR_EACH];
-  bool biased = false;
-#pragma unroll
-  for (int k = 0; k < LR_EACH; ++k) bias[k] = 0.0f;
-  for (int base = 0; base < p.n_bias; base += LR_THREADS) {
-    // the list's entries that fall on the CTA's tokens, in its order
-    const int n = base + tid;
-    const int id = n < p.n_bias ? p.bias_ids[b * p.ld_i + n] : -1;
-    if (id >= p.V && blockIdx.x == 0 && p.err) atomicOr(p.err, SIMSD_DEV_ERR_BAD_INDEX);
-    const bool in = id >= v0 && id < v0 + LR_TOKENS && id < p.V;
-    const uint32_t who = __ballot_sync(0xffffffffu, in);
-    if (lane == 0) s_n[warp] = __popc(who);
-    __syncthreads();
-    int at = __popc(who & ((1u << lane) - 1)), all = 0;
-#pragma unroll
-    for (int w = 0; w < LR_THREADS / 32; ++w) {
-      if (w < warp) at += s_n[w];
-      all += s_n[w];
-    }
-    if (in) s_id[at] = id - v0, s_val[at] = p.bias[b * p.ld_v + n];
-    __syncthreads();
-    for (int e = 0; e < all; ++e) {
-      const int k = mine(s_id[e]);
-      if (k < 0) continue;
-      biased = true;
-#pragma unroll
-      for (int x = 0; x < LR_EACH; ++x) bias[x] += x == k ? s_val[e] : 0.0f;
-    }
-    __syncthreads();
-  }
+  auto stage_drafts = [&](int i) {                // rows i on: their drafted tokens that are the CTA's
+    const long long v = p.drafts && i + tid + 1 < p.R ? p.drafts[b * p.ld_d + i + tid] : -1;
+    s_draft[tid] = v >= v0 && v < min(v0 + LR_TOKENS, p.V) ? (int)(v - v0) : -1;
+  };
+  if (p.penal) stage_drafts(0);
 
+  // per token: what is added
+  float add[LR_EACH];
+#pragma unroll
+  for (int k = 0; k < LR_EACH; ++k) add[k] = 0.0f;
+  const int* ids = p.bias_ids + b * p.ld_i;
+  const float* values = p.bias + b * p.ld_v;
+  for (int base = 0; base < p.n_bias; base += LR_LIST) {
+    // the list's entries that are the CTA's, as (place in the list, token), in the list's order: found in any, then ranked
+    const int n = min(LR_LIST, p.n_bias - base);
+    if (tid == 0) s_hits = 0;
+    __syncthreads();
+    for (int x = tid; x < n; x += LR_THREADS) {
+      const int id = ids[base + x];
+      if (id >= p.V && blockIdx.x == 0 && p.err) atomicOr(p.err, SIMSD_DEV_ERR_BAD_INDEX);
+      if ((uint32_t)(id - v0) < (uint32_t)LR_TOKENS && id < p.V) s_hit[atomicAdd(&s_hits, 1)] = x * LR_TOKENS + id - v0;
+    }
+    __syncthreads();
+    const int hits = s_hits;
+    for (int x = tid; x < hits; x += LR_THREADS) {
+      int rank = 0;
+      for (int y = 0; y < hits; ++y) rank += s_hit[y] < s_hit[x];
+      s_order[rank] = s_hit[x];
+    }
+    __syncthreads();
+    for (int x = 0; x < hits; ++x) {
+      const int hit = s_order[x], k = mine(hit % LR_TOKENS);
+      if (k < 0) continue;
+      const float v = values[base + hit / LR_TOKENS];
+#pragma unroll
+      for (int y = 0; y < LR_EACH; ++y) add[y] += y == k ? v : 0.0f;
+    }
+  }
+  const float inv = 1.0f / rep;
+#pragma unroll
+  for (int k = 0; k < LR_EACH; ++k)
+    if (c[k] > 0) add[k] -= fmaf(freq, (float)c[k], pres), again |= 1u << k;
+
+  char* dst = static_cast<char*>(p.out) + (b * p.ldo_b + first) * SIZE;
   auto row = [&](int i, int at) {
-    fetch(i + 1, at ^ 1);
     float x[LR_EACH];
     if constexpr (VEC) {
 #pragma unroll
@@ -165,53 +181,81 @@ __global__ void __launch_bounds__(LR_THREADS) logit_rules_kernel(const LogitRule
 #pragma unroll
       for (int k = 0; k < LR_EACH; ++k) x[k] = val[at][k];
     }
-    if (again != 0) {
 #pragma unroll
-      for (int k = 0; k < LR_EACH; ++k) {
-        if (again >> k & 1) x[k] = x[k] > 0.0f ? x[k] / rep : x[k] * rep;
-        if (met >> k & 1) x[k] = fmaf(-freq, (float)c[k], x[k]) - pres;
-      }
+    for (int k = 0; k < LR_EACH; ++k) x[k] = fmaf(x[k], again >> k & 1 ? x[k] > 0.0f ? inv : rep : 1.0f, add[k]);
+    if ((!VEC || DT == 2) && ok[at] != 0xffu) {
+#pragma unroll
+      for (int k = 0; k < LR_EACH; ++k)
+        if (!(ok[at] >> k & 1)) x[k] = -INFINITY;
     }
-    if (biased) {
-#pragma unroll
-      for (int k = 0; k < LR_EACH; ++k) x[k] += bias[k];
-    }
-#pragma unroll
-    for (int k = 0; k < LR_EACH; ++k)
-      if (!(ok[at] >> k & 1)) x[k] = -INFINITY;
-    const long long off = b * p.ldo_b + i * p.ldo_r + first;
     if constexpr (VEC) {
       if (first < p.V) {
-        uint4* dst = reinterpret_cast<uint4*>(static_cast<char*>(p.out) + off * (DT == 2 ? 4 : 2));
+        uint4* to = reinterpret_cast<uint4*>(dst);
         if constexpr (DT == 2) {
-          dst[0] = make_uint4(__float_as_uint(x[0]), __float_as_uint(x[1]), __float_as_uint(x[2]), __float_as_uint(x[3]));
-          dst[1] = make_uint4(__float_as_uint(x[4]), __float_as_uint(x[5]), __float_as_uint(x[6]), __float_as_uint(x[7]));
+          to[0] = make_uint4(__float_as_uint(x[0]), __float_as_uint(x[1]), __float_as_uint(x[2]), __float_as_uint(x[3]));
+          to[1] = make_uint4(__float_as_uint(x[4]), __float_as_uint(x[5]), __float_as_uint(x[6]), __float_as_uint(x[7]));
         } else {
           uint32_t w[4];
 #pragma unroll
-          for (int k = 0; k < 4; ++k)
-            w[k] = (uint32_t)f32_to_16bit(x[2 * k], DT) | (uint32_t)f32_to_16bit(x[2 * k + 1], DT) << 16;
-          dst[0] = make_uint4(w[0], w[1], w[2], w[3]);
+          for (int k = 0; k < 4; ++k) {
+            if constexpr (DT == 0)
+              asm("cvt.rn.bf16x2.f32 %0, %1, %2;" : "=r"(w[k]) : "f"(x[2 * k + 1]), "f"(x[2 * k]));
+            else
+              asm("cvt.rn.f16x2.f32 %0, %1, %2;" : "=r"(w[k]) : "f"(x[2 * k + 1]), "f"(x[2 * k]));
+          }
+          if (ok[at] != 0xffu) {
+            // four bits to the top bits of four bytes, and those over the two halves of two words
+            constexpr uint32_t LOW = DT == 0 ? 0xff80ff80u : 0xfc00fc00u;      // two -inf
+#pragma unroll
+            for (int h = 0; h < 2; ++h) {
+              const uint32_t t = (ok[at] >> 4 * h & 15u) * 0x10204080u;
+              uint32_t m0, m1;
+              asm("prmt.b32 %0, %1, 0, 0x9988;" : "=r"(m0) : "r"(t));          // a byte's top bit, eight times
+              asm("prmt.b32 %0, %1, 0, 0xbbaa;" : "=r"(m1) : "r"(t));
+              w[2 * h] = (w[2 * h] & m0) | (LOW & ~m0), w[2 * h + 1] = (w[2 * h + 1] & m1) | (LOW & ~m1);
+            }
+          }
+          to[0] = make_uint4(w[0], w[1], w[2], w[3]);
         }
       }
     } else {
 #pragma unroll
       for (int k = 0; k < LR_EACH; ++k)
-        if (first + k * step < p.V) store_f(p.out, off + k * step, x[k], DT);
+        if (first + k * step < p.V) store_f(dst, k * step, x[k], DT);
     }
-    const long long d = draft[at];
-    if (p.penal && d >= v0 && d < min(v0 + LR_TOKENS, p.V)) {     // the rows after this one count it
-      const int k = mine((int)(d - v0));
+    dst += p.ldo_r * SIZE;
+    const int d = p.penal ? s_draft[i % LR_THREADS] : -1;
+    if (d >= 0 && d / (32 * LR_EACH) == warp) {   // the rows after this one count it
+      float sum = 0.0f;                           // its biases once more
+#pragma unroll 4
+      for (int y = 0; y < p.n_bias; y += 32) {
+        const int id = y + lane < p.n_bias ? ids[y + lane] : -1;
+        for (uint32_t who = __ballot_sync(0xffffffffu, id == v0 + d); who != 0; who &= who - 1) sum += values[y + __ffs(who) - 1];
+      }
+      const int k = mine(d);
       if (k >= 0) {
-        met |= 1u << k, again |= 1u << k;
+        int c = counts ? counts[k * step] : 0;
+        for (int y = 0; y <= i; ++y) c += p.drafts[b * p.ld_d + y] == v0 + d;
+        const float now = c > 0 ? sum - fmaf(freq, (float)c, pres) : sum;
+        if (c > 0) again |= 1u << k;
 #pragma unroll
-        for (int y = 0; y < LR_EACH; ++y) c[y] += y == k;
+        for (int y = 0; y < LR_EACH; ++y) add[y] = y == k ? now : add[y];
       }
     }
   };
-  for (int i = 0; i < p.R; i += 2) {
-    row(i, 0);
-    if (i + 1 < p.R) row(i + 1, 1);
+  for (int i = 0; i < p.R; i += ROWS) {
+    if (p.penal && i % LR_THREADS == 0) {
+      if (i > 0) {
+        __syncthreads();
+        stage_drafts(i);
+      }
+      __syncthreads();
+    }
+#pragma unroll
+    for (int x = 0; x < ROWS; ++x) {
+      if (i + x < p.R) row(i + x, x);
+      fetch(x);
+    }
   }
 }
 

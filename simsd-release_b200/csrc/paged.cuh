@@ -67,6 +67,12 @@ __device__ __forceinline__ uint64_t f2_fma(uint64_t a, uint64_t b, uint64_t c) {
   return r;
 }
 
+__device__ __forceinline__ uint64_t f2_add(uint64_t a, uint64_t b) {
+  uint64_t r;
+  asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+  return r;
+}
+
 // 8 16-bit elements as four pairs of fp32, and back
 template <bool BF>
 __device__ __forceinline__ void paged_unpack8(uint4 u, uint64_t (&v)[4]) {

@@ -36,13 +36,14 @@ struct PagedAppend8Args {
   float* v_scale;
   int* err;
   long long ldq_b, ldq_t, n_pos, ld_table, ld_page, ld_head, ld_tok, lds_page, lds_head, lds_block;
-  int kv_tasks, tasks;      // warps' tasks: blocks of keys and values, then rows of queries
-  int B, L, Hq, Hk, R, page_size, block, num_pages, max_pages, blocks, chunks;   // blocks of a sequence, row chunks
+  int kv_tasks, tasks;      // warps' tasks: blocks of a key or value head, then rows of some query heads
+  int B, L, Hq, Hk, R, page_size, block, num_pages, max_pages, blocks;   // blocks that a sequence's rows can touch
+  int q_heads, q_groups, q_chunks;   // query heads of a task, groups of them, groups of rows
   float eps;
 };
 
 constexpr int PA8_WARPS = 4, PA8_THREADS = PA8_WARPS * 32;
-constexpr int PA8_ROWS = 16;          // rows that a warp holds in registers
+constexpr int PA8_ROWS = 16;          // rows that a warp holds
 
 // 2^e as a float, e from -126 to 127
 __device__ __forceinline__ float p8_power(int e) { return __int_as_float((e + 127) << 23); }
@@ -64,8 +65,53 @@ __device__ __forceinline__ uint32_t p8_half2(uint32_t two) {
   return r;
 }
 
+// A lane's 8 elements x and 8 more y of a row: the norm, over all lanes of the row, and the rotation
+// of pairs (x, y)
 template <int D, bool BF>
-__global__ void __launch_bounds__(PA8_THREADS) paged_append8_kernel(const PagedAppend8Args p) {
+__device__ __forceinline__ void p8_norm(uint64_t (&x)[4], uint64_t (&y)[4], uint32_t row_mask, float eps, const uint64_t (&wx)[4],
+                                        const uint64_t (&wy)[4]) {
+  uint64_t sx = 0, sy = 0;
+#pragma unroll
+  for (int e = 0; e < 4; ++e) sx = f2_fma(x[e], x[e], sx), sy = f2_fma(y[e], y[e], sy);
+  const float2 s0 = f2_unpack(sx), s1 = f2_unpack(sy);
+  float ss = (s0.x + s0.y) + (s1.x + s1.y);
+#pragma unroll
+  for (int m = D / 32; m > 0; m >>= 1) ss += __shfl_xor_sync(row_mask, ss, m);
+  const float inv = rsqrtf(fmaf(ss, 1.0f / D, eps));
+  const uint64_t inv2 = f2_pack(inv, inv);
+#pragma unroll
+  for (int e = 0; e < 4; ++e) x[e] = f2_mul(f2_mul(x[e], inv2), wx[e]), y[e] = f2_mul(f2_mul(y[e], inv2), wy[e]);
+}
+__device__ __forceinline__ void p8_rotate(uint64_t (&x)[4], uint64_t (&y)[4], const uint64_t (&cs)[4], const uint64_t (&sn)[4],
+                                          const uint64_t (&ns)[4]) {
+#pragma unroll
+  for (int e = 0; e < 4; ++e) {
+    const uint64_t x0 = x[e];
+    x[e] = f2_fma(y[e], ns[e], f2_mul(x0, cs[e]));
+    y[e] = f2_fma(x0, sn[e], f2_mul(y[e], cs[e]));
+  }
+}
+struct P8Turn {               // a lane's cos, sin and -sin
+  uint64_t c[4], s[4], n[4];
+  __device__ __forceinline__ void load(const float* cos, const float* sin, long long at) {
+#pragma unroll
+    for (int q = 0; q < 2; ++q) {
+      const float4 a = __ldg(reinterpret_cast<const float4*>(cos + at) + q), b = __ldg(reinterpret_cast<const float4*>(sin + at) + q);
+      c[2 * q] = f2_pack(a.x, a.y), c[2 * q + 1] = f2_pack(a.z, a.w);
+      s[2 * q] = f2_pack(b.x, b.y), s[2 * q + 1] = f2_pack(b.z, b.w);
+      n[2 * q] = f2_pack(-b.x, -b.y), n[2 * q + 1] = f2_pack(-b.z, -b.w);
+    }
+  }
+};
+
+// D / 16 lanes share a row of a head, each with elements 8 j .. 8 j + 7 and their pairs R / 2 further
+// (or 16 next to each other of the unrotated rest), so that the rotation needs no exchange.
+//
+// A task of keys or values is one (sequence, block, head): 16 rows in shared memory (longer blocks
+// twice over: for the largest magnitude, then to be stored).  A task of queries is four (D
+// 128) or eight rows of some neighbouring heads: the rotary row and the weight stay in registers over these.
+template <int D, bool BF>
+__global__ void __launch_bounds__(PA8_THREADS, 4) paged_append8_kernel(const PagedAppend8Args p) {
   griddep_launch_dependents();
   griddep_wait();
   constexpr int LANES = D / 16, ROWS = 32 / LANES, TURNS = PA8_ROWS / ROWS;   // threads of a row, rows of a warp at a time
@@ -74,112 +120,125 @@ __global__ void __launch_bounds__(PA8_THREADS) paged_append8_kernel(const PagedA
   const bool pair = 16 * j < p.R;                // this thread's elements are rotated
   const int e0 = pair ? 8 * j : 16 * j, e1 = pair ? p.R / 2 + 8 * j : 16 * j + 8;
   const uint16_t* qkv = reinterpret_cast<const uint16_t*>(p.qkv);
+  __shared__ float4 rows[PA8_WARPS][TURNS * 4 * 32];   // a warp's rows in fp32, every lane's its own
+  float4* own = rows[threadIdx.x >> 5] + lane;
 
   for (uint32_t task = blockIdx.x * PA8_WARPS + (threadIdx.x >> 5); task < (uint32_t)p.tasks; task += gridDim.x * PA8_WARPS) {
-    // ---- which rows of which head: keys first, then values, then queries
+    // ---- which rows of which heads: keys first, then values, then queries
     const bool kv = task < (uint32_t)p.kv_tasks;
-    const uint32_t at = kv ? task : task - p.kv_tasks, heads = kv ? 2 * p.Hk : p.Hq, per = kv ? p.blocks : p.chunks;
+    const uint32_t at = kv ? task : task - p.kv_tasks, heads = kv ? 2 * p.Hk : p.q_groups, per = kv ? p.blocks : p.q_chunks;
     const int h = (int)(at % heads), k = (int)(at / heads % per), b = (int)(at / heads / per);
-    const int head = kv ? p.Hq + h : h;
-    const bool key = kv && h < p.Hk, turned = !kv || key;
+    const bool key = kv && h < p.Hk;
     const int n = max(0, p.seq_lens[b]);
     const int c = min(n, p.count ? max(0, min(p.count[b], p.L)) : p.L);
     // positions past the tables are no places: flagged, not written
     const long long cap = min((long long)p.max_pages * p.page_size, p.n_pos);
     const int top = (int)min((long long)n, cap), old = n - c;
-    if (n > top && c > 0 && k == 0 && h == 0 && lane == 0 && p.err) atomicOr(p.err, SIMSD_DEV_ERR_BAD_INDEX);
     const int shift = n - p.L;                   // position of row 0
-    int lo, hi, block_at = 0;                    // rows t, lo <= t < hi
-    if (kv) {
-      block_at = (old / p.block + k) * p.block;
-      if (block_at >= top || c == 0) continue;
-      lo = max(old, block_at) - shift, hi = min(top, block_at + p.block) - shift;
-      if (lo >= hi) continue;
-    } else {
-      lo = k * PA8_ROWS, hi = min(p.L, lo + PA8_ROWS);
-    }
-    const uint16_t* src = qkv + b * p.ldq_b + (long long)head * D;
     const uint16_t* weight = reinterpret_cast<const uint16_t*>(key ? p.kw : p.qw);
-    // rows base .. base + 15 of the head: normed, rotated
-    float x[TURNS][16];
-    auto fill = [&](int base) {
+    uint4 w0 = make_uint4(0, 0, 0, 0), w1 = w0;
+    if (weight != nullptr && (key || !kv))
+      w0 = __ldg(reinterpret_cast<const uint4*>(weight + e0)), w1 = __ldg(reinterpret_cast<const uint4*>(weight + e1));
+    if (!kv) {
+      uint64_t wx[4], wy[4];
+      paged_unpack8<BF>(w0, wx);
+      paged_unpack8<BF>(w1, wy);
+      const int t = k * ROWS + sub;
+      if (n > top && c > 0 && k == 0 && h == 0 && lane == 0 && p.err) atomicOr(p.err, SIMSD_DEV_ERR_BAD_INDEX);
+      const bool in = t < p.L, real = in && t + shift >= old && t + shift < top;
+      P8Turn turn;
+      if (pair && real) turn.load(p.cos, p.sin, (long long)(t + shift) * (p.R / 2) + 8 * j);
+      const int h0 = h * p.q_heads, h1 = min(p.Hq, h0 + p.q_heads);
+      const uint16_t* src = qkv + b * p.ldq_b + (real ? t : 0) * p.ldq_t + h0 * D;
+      uint16_t* dst = reinterpret_cast<uint16_t*>(p.q_out) + (((long long)b * p.L + (in ? t : 0)) * p.Hq + h0) * D;
+      // AHEAD heads' loads are on their way
+      constexpr int AHEAD = 4;
+      uint4 u[AHEAD][2];
+      auto fetch = [&](int i, int head) {
+        u[i][0] = u[i][1] = make_uint4(0, 0, 0, 0);
+        if (real && head < h1) {
+          u[i][0] = __ldg(reinterpret_cast<const uint4*>(src + e0)), u[i][1] = __ldg(reinterpret_cast<const uint4*>(src + e1));
+        }
+        src += D;
+      };
+#pragma unroll
+      for (int i = 0; i < AHEAD; ++i) fetch(i, h0 + i);
+      for (int head = h0; head < h1; head += AHEAD) {
+#pragma unroll
+        for (int i = 0; i < AHEAD; ++i) {
+          if (head + i >= h1) break;
+          uint64_t x[4], y[4];
+          paged_unpack8<BF>(u[i][0], x);
+          paged_unpack8<BF>(u[i][1], y);
+          fetch(i, head + i + AHEAD);
+          if (weight != nullptr) p8_norm<D, BF>(x, y, row_mask, p.eps, wx, wy);
+          if (pair) p8_rotate(x, y, turn.c, turn.s, turn.n);
+          if (in) {
+            const uint4 nul = make_uint4(0, 0, 0, 0);
+            *reinterpret_cast<uint4*>(dst + e0) = real ? paged_pack8<BF>(x) : nul;
+            *reinterpret_cast<uint4*>(dst + e1) = real ? paged_pack8<BF>(y) : nul;
+          }
+          dst += D;
+        }
+      }
+      continue;
+    }
+    // ---- keys or values: the block's rows t, lo <= t < hi, its page and scale
+    const int block_at = (old / p.block + k) * p.block;
+    if (block_at >= top || c == 0) continue;
+    const int lo = max(old, block_at) - shift, hi = min(top, block_at + p.block) - shift;
+    if (lo >= hi) continue;
+    const uint16_t* src = qkv + b * p.ldq_b + (long long)(p.Hq + h) * D;
+    // rows base .. base + 15 into the lane's places of shared memory; their largest magnitude, infinities
+    // among them or not (NaN never)
+    auto fill = [&](int base, bool all) {
       uint4 u[TURNS][2];
 #pragma unroll
       for (int i = 0; i < TURNS; ++i) {
         const int t = base + i * ROWS + sub;
-        const bool real = t < hi && t + shift >= old && t + shift < top;
         u[i][0] = u[i][1] = make_uint4(0, 0, 0, 0);
-        if (real) {
+        if (t < hi) {
           u[i][0] = __ldg(reinterpret_cast<const uint4*>(src + t * p.ldq_t + e0));
           u[i][1] = __ldg(reinterpret_cast<const uint4*>(src + t * p.ldq_t + e1));
         }
       }
+      float a = 0.0f;
 #pragma unroll
       for (int i = 0; i < TURNS; ++i) {
-        uint64_t v[4], y[4];
-        paged_unpack8<BF>(u[i][0], v);
+        uint64_t x[4], y[4];
+        paged_unpack8<BF>(u[i][0], x);
         paged_unpack8<BF>(u[i][1], y);
-        if (turned) {
+        if (key) {
           if (weight != nullptr) {
-            uint64_t sx = 0, sy = 0;
-#pragma unroll
-            for (int e = 0; e < 4; ++e) sx = f2_fma(v[e], v[e], sx), sy = f2_fma(y[e], y[e], sy);
-            const float2 s0 = f2_unpack(sx), s1 = f2_unpack(sy);
-            float ss = (s0.x + s0.y) + (s1.x + s1.y);
-#pragma unroll
-            for (int m = LANES / 2; m > 0; m >>= 1) ss += __shfl_xor_sync(row_mask, ss, m);
-            const float inv = rsqrtf(fmaf(ss, 1.0f / D, p.eps));
-            const uint64_t inv2 = f2_pack(inv, inv);
             uint64_t wx[4], wy[4];
-            paged_unpack8<BF>(__ldg(reinterpret_cast<const uint4*>(weight + e0)), wx);
-            paged_unpack8<BF>(__ldg(reinterpret_cast<const uint4*>(weight + e1)), wy);
-#pragma unroll
-            for (int e = 0; e < 4; ++e) v[e] = f2_mul(f2_mul(v[e], inv2), wx[e]), y[e] = f2_mul(f2_mul(y[e], inv2), wy[e]);
+            paged_unpack8<BF>(w0, wx);
+            paged_unpack8<BF>(w1, wy);
+            p8_norm<D, BF>(x, y, row_mask, p.eps, wx, wy);
           }
           const int t = base + i * ROWS + sub;
-          if (pair && t < hi && t + shift >= old && t + shift < top) {
-            const long long row = (long long)(t + shift) * (p.R / 2) + 8 * j;
-#pragma unroll
-            for (int q = 0; q < 2; ++q) {
-              const float4 cs = __ldg(reinterpret_cast<const float4*>(p.cos + row) + q);
-              const float4 sn = __ldg(reinterpret_cast<const float4*>(p.sin + row) + q);
-              const uint64_t c2[2] = {f2_pack(cs.x, cs.y), f2_pack(cs.z, cs.w)};
-              const uint64_t s2[2] = {f2_pack(sn.x, sn.y), f2_pack(sn.z, sn.w)};
-              const uint64_t n2[2] = {f2_pack(-sn.x, -sn.y), f2_pack(-sn.z, -sn.w)};
-#pragma unroll
-              for (int e = 0; e < 2; ++e) {
-                const uint64_t v0 = v[2 * q + e];
-                v[2 * q + e] = f2_fma(y[2 * q + e], n2[e], f2_mul(v0, c2[e]));
-                y[2 * q + e] = f2_fma(v0, s2[e], f2_mul(y[2 * q + e], c2[e]));
-              }
-            }
+          if (pair && t < hi) {
+            P8Turn turn;
+            turn.load(p.cos, p.sin, (long long)(t + shift) * (p.R / 2) + 8 * j);
+            p8_rotate(x, y, turn.c, turn.s, turn.n);
           }
         }
 #pragma unroll
-        for (int e = 0; e < 4; ++e) {
-          const float2 a = f2_unpack(v[e]), d = f2_unpack(y[e]);
-          x[i][2 * e] = a.x, x[i][2 * e + 1] = a.y, x[i][8 + 2 * e] = d.x, x[i][8 + 2 * e + 1] = d.y;
+        for (int e = 0; e < 4; e += 2) {
+          const float2 x0 = f2_unpack(x[e]), x1 = f2_unpack(x[e + 1]), y0 = f2_unpack(y[e]), y1 = f2_unpack(y[e + 1]);
+          own[(i * 4 + e / 2) * 32] = make_float4(x0.x, x0.y, x1.x, x1.y);
+          own[(i * 4 + 2 + e / 2) * 32] = make_float4(y0.x, y0.y, y1.x, y1.y);
+          if (all) {
+            a = fmaxf(fmaxf(a, fabsf(x0.x)), fabsf(x0.y)), a = fmaxf(fmaxf(a, fabsf(x1.x)), fabsf(x1.y));
+            a = fmaxf(fmaxf(a, fabsf(y0.x)), fabsf(y0.y)), a = fmaxf(fmaxf(a, fabsf(y1.x)), fabsf(y1.y));
+          } else {
+            const float w[8] = {x0.x, x0.y, x1.x, x1.y, y0.x, y0.y, y1.x, y1.y};
+#pragma unroll
+            for (int z = 0; z < 8; ++z) a = fmaxf(a, fabsf(w[z]) < INFINITY ? fabsf(w[z]) : 0.0f);
+          }
         }
       }
+      return a;
     };
-    if (!kv) {
-      fill(lo);
-#pragma unroll
-      for (int i = 0; i < TURNS; ++i) {
-        const int t = lo + i * ROWS + sub;
-        if (t >= hi) continue;
-        const bool real = t + shift >= old && t + shift < top;
-        uint16_t* dst = reinterpret_cast<uint16_t*>(p.q_out) + (((long long)b * p.L + t) * p.Hq + h) * D;
-        uint64_t v[4], y[4];
-#pragma unroll
-        for (int e = 0; e < 4; ++e) v[e] = f2_pack(x[i][2 * e], x[i][2 * e + 1]), y[e] = f2_pack(x[i][8 + 2 * e], x[i][8 + 2 * e + 1]);
-        const uint4 nul = make_uint4(0, 0, 0, 0);
-        *reinterpret_cast<uint4*>(dst + e0) = real ? paged_pack8<BF>(v) : nul;
-        *reinterpret_cast<uint4*>(dst + e1) = real ? paged_pack8<BF>(y) : nul;
-      }
-      continue;
-    }
-    // ---- keys or values: the block's page and scale
     const int page = p.page_table[b * p.ld_table + block_at / p.page_size];
     if (page < 0 || page >= p.num_pages) {
       if (h == 0 && lane == 0 && p.err) atomicOr(p.err, SIMSD_DEV_ERR_BAD_INDEX);
@@ -190,25 +249,24 @@ __global__ void __launch_bounds__(PA8_THREADS) paged_append8_kernel(const PagedA
     float* scale = (key ? p.k_scale : p.v_scale) + page * p.lds_page + g * p.lds_head + in / p.block * p.lds_block;
     const bool fresh = block_at >= old;
     const float had = fresh ? 0.0f : *scale;
-    float a = 0.0f;
+    // the largest magnitude; where an infinity is it, once more without those
     const int last = lo + (hi - lo - 1) / PA8_ROWS * PA8_ROWS;
-    for (int base = lo; base <= last; base += PA8_ROWS) {
-      fill(base);
+    auto largest = [&](bool all) {
+      float a = 0.0f;
+      for (int base = lo; base <= last; base += PA8_ROWS) a = fmaxf(a, fill(base, all));
 #pragma unroll
-      for (int i = 0; i < TURNS; ++i)
-#pragma unroll
-        for (int e = 0; e < 16; ++e) {
-          const float y = fabsf(x[i][e]);
-          a = fmaxf(a, y < INFINITY ? y : 0.0f);
-        }
-    }
-#pragma unroll
-    for (int m = 16; m > 0; m >>= 1) a = fmaxf(a, __shfl_xor_sync(0xffffffffu, a, m));
+      for (int m = 16; m > 0; m >>= 1) a = fmaxf(a, __shfl_xor_sync(0xffffffffu, a, m));
+      return a;
+    };
+    float a = largest(true);
+    const bool infinite = a == INFINITY;
+    if (infinite) a = largest(false);
     const float s = fmaxf(had, p8_power(p8_exponent(a))), inv = 1.0f / s;
+    const uint64_t inv2 = f2_pack(inv, inv);
     if (lane == 0) *scale = s;
-    // the new tokens; the last rows are still in registers
+    // the new tokens; the last rows are still at hand
     for (int base = last; base >= lo; base -= PA8_ROWS) {
-      if (base != last) fill(base);
+      if (base != last) fill(base, true);
 #pragma unroll
       for (int i = 0; i < TURNS; ++i) {
         const int t = base + i * ROWS + sub;
@@ -216,13 +274,10 @@ __global__ void __launch_bounds__(PA8_THREADS) paged_append8_kernel(const PagedA
         uint32_t w[4];
 #pragma unroll
         for (int q = 0; q < 4; ++q) {
-          float y[4];
-#pragma unroll
-          for (int e = 0; e < 4; ++e) {
-            const float z = x[i][4 * q + e];
-            y[e] = fabsf(z) < INFINITY ? z * inv : __int_as_float(0x7fffffff);
-          }
-          w[q] = p8_pack2(y[0], y[1]) | p8_pack2(y[2], y[3]) << 16;
+          const float4 z = own[(i * 4 + q) * 32];
+          float2 u = f2_unpack(f2_mul(f2_pack(z.x, z.y), inv2)), v = f2_unpack(f2_mul(f2_pack(z.z, z.w), inv2));
+          if (infinite) u.x -= u.x - u.x, u.y -= u.y - u.y, v.x -= v.x - v.x, v.y -= v.y - v.y;   // infinities become NaN
+          w[q] = p8_pack2(u.x, u.y) | p8_pack2(v.x, v.y) << 16;
         }
         uint8_t* dst = cache + (t + shift - block_at) * p.ld_tok;
         *reinterpret_cast<uint2*>(dst + e0) = make_uint2(w[0], w[1]);

@@ -85,6 +85,8 @@ struct PatShape {
   static constexpr int BYTES = RING + OBUF + ML;
 };
 
+// the warps that hold O; another one of the CTA may be loading
+__device__ __forceinline__ void pat_sync() { named_bar_sync(1, PAT_THREADS); }
 __device__ __forceinline__ void pat_ldsm(uint32_t addr, uint32_t (&r)[4]) {
   asm volatile("ldmatrix.sync.aligned.m8n8.x4.shared.b16 {%0, %1, %2, %3}, [%4];"
                : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]) : "r"(addr) : "memory");
@@ -237,18 +239,12 @@ __device__ __forceinline__ long long paged_row(const PagedAttnArgs& p, int b, in
   return ((long long)b * p.L + t) * p.Hq + g * p.G + (r - t * p.G);
 }
 // 16 dims (from mt * 16) of 8 rows (from r8) out of a fragment of O^T (v: dims d, d
-// + 8 of two rows; with PAIRS dims 2 d, 2 d + 1): packed and transposed, so that a lane
-// holds two dims of row lane / 4 and stores 4 bytes twice (with PAIRS four dims, 8 bytes).
-// `row`: the lane's row's place, or -1.
-template <bool BF, int D, bool PAIRS = false>
+// + 8 of two rows): packed and transposed, so that a lane holds two dims of row
+// lane / 4 and stores 4 bytes twice.  `row`: the lane's row's place, or -1.
+template <bool BF, int D>
 __device__ __forceinline__ void paged_store(const PagedAttnArgs& p, long long row, int mt, int lane, float4 v) {
   const uint32_t lo = pat_transpose(pat_pack<BF>(v.x, v.y)), hi = pat_transpose(pat_pack<BF>(v.z, v.w));
   if (row < 0) return;
-  if constexpr (PAIRS) {
-    reinterpret_cast<uint2*>(reinterpret_cast<uint16_t*>(p.o) + row * D + mt * 16)[lane & 3] =
-        make_uint2(__byte_perm(lo, hi, 0x5410), __byte_perm(lo, hi, 0x7632));
-    return;
-  }
   uint32_t* dst = reinterpret_cast<uint32_t*>(reinterpret_cast<uint16_t*>(p.o) + row * D + mt * 16) + (lane & 3);
   dst[0] = lo;
   dst[4] = hi;
@@ -350,94 +346,83 @@ __device__ __forceinline__ bool paged_arrive(const PagedAttnArgs& p, const Paged
 
 // Joins the parts of a cut sequence (one KV head and row tile of it) that starts
 // in CTA c0: part i's max, sum and O lie in slot 1 of CTA c0 for i = 0, in slot 0
-// of CTA c0 + i for the others.  `buf`: OBUF bytes of shared memory.
-template <int D, int NT, bool BF, bool PAIRS = false>
-__device__ __noinline__ void paged_join(const PagedAttnArgs& p, int b, int g, int r0, int c0, int parts, float* buf) {
-  using S = PatShape<D, NT>;
-  constexpr int MT = D / 16, NR = S::NR, ALL = MT * NT * 32, PER = ALL / PAT_THREADS;   // fragments, and of a thread
-  constexpr int GR = PAT_THREADS / NR, KEEP = 4;              // threads of a row, parts a thread keeps
-  constexpr int CAP = S::OBUF / 4 / NR;                       // parts whose weights fit in buf
+// of CTA c0 + i for the others.  `buf`: `room` bytes of shared memory, at least
+// a part's O and its weights and 2 KB.  The parts of O come in by cp.async, as many at a time as there is room
+// for (28 parts one after the other, four on their way, took 7 us at the end of a kernel).
+template <int D, int NT, bool BF>
+__device__ __noinline__ void paged_join(const PagedAttnArgs& p, int b, int g, int r0, int c0, int parts, uint8_t* buf, int room) {
+  constexpr int NR = NT * 8, THREADS = PAT_THREADS, PART = D * NR * 4;
+  constexpr int ALL = PART / 16, PER = ALL / THREADS;                    // fragments, and of a thread
+  constexpr int GR = THREADS / NR;                                       // threads of a row
   const int tid = threadIdx.x, lane = tid & 31, r = tid % NR, grp = tid / NR;
-  auto slot = [&](int i) { return i == 0 ? 2 * c0 + 1 : 2 * (c0 + i); };
-  // the first two parts of O (most sequences are cut once) are on their way while the weights are made
-  float4 lead[2][PER];
+  auto slot = [&](int i) { return (long long)(i == 0 ? 2 * c0 + 1 : 2 * (c0 + i)); };
+  float* red = reinterpret_cast<float*>(buf);                            // [2][GR][NR]
+  float* weight = red + 2 * GR * NR;                                     // [parts of a batch][NR]
+  const int batch = min(parts, (room - 2 * GR * NR * 4) / (PART + NR * 4));
+  const uint32_t stage = smem_u32(weight + batch * NR);
+  auto fetch = [&](int i0) {
+    const int n = min(batch, parts - i0);
+    for (int i = 0; i < n; ++i) {
+      const float4* o = p.part_o + slot(i0 + i) * ALL;
 #pragma unroll
-  for (int i = 0; i < 2; ++i)
-#pragma unroll
-    for (int k = 0; k < PER; ++k)
-      lead[i][k] = __ldcg(p.part_o + (long long)slot(i) * ALL + tid + k * PAT_THREADS);
-  float2 keep[KEEP];
-#pragma unroll
-  for (int k = 0; k < KEEP; ++k) {
-    const int i = grp + k * GR;
-    keep[k] = i < parts ? __ldcg(p.part_ml + slot(i) * NR + r) : make_float2(-INFINITY, 0.0f);
-  }
+      for (int k = 0; k < PER; ++k)
+        paged_cp16(stage + i * PART + (tid + k * THREADS) * 16, o + tid + k * THREADS);
+    }
+    asm volatile("cp.async.commit_group;" ::: "memory");
+  };
+  fetch(0);
   float mm = -INFINITY, ll = 0.0f;
   auto see = [&](float2 x) {
     const float mn = fmaxf(mm, x.x), mu = mn == -INFINITY ? 0.0f : mn;
     ll = fmaf(ll, pat_exp2(mm - mu), x.y * pat_exp2(x.x - mu));
     mm = mn;
   };
-#pragma unroll
-  for (int k = 0; k < KEEP; ++k) see(keep[k]);
-  for (int i = grp + KEEP * GR; i < parts; i += GR) see(__ldcg(p.part_ml + slot(i) * NR + r));
-  float* all = buf + GR * NR;
-  buf[grp * NR + r] = mm, all[grp * NR + r] = ll;
-  __syncthreads();
+#pragma unroll 4
+  for (int i = grp; i < parts; i += GR) see(__ldcg(p.part_ml + slot(i) * NR + r));
+  red[grp * NR + r] = mm, red[(GR + grp) * NR + r] = ll;
+  pat_sync();
   mm = -INFINITY, ll = 0.0f;
 #pragma unroll
-  for (int k = 0; k < GR; ++k) see(make_float2(buf[k * NR + r], all[k * NR + r]));
+  for (int k = 0; k < GR; ++k) see(make_float2(red[k * NR + r], red[(GR + k) * NR + r]));
   if (grp == 0) paged_store_lse(p, b, g, r0 + r, mm, ll);
   const float mu = mm == -INFINITY ? 0.0f : mm, inv = ll == 0.0f ? 0.0f : 1.0f / ll;
   float4 a[PER];
 #pragma unroll
   for (int k = 0; k < PER; ++k) a[k] = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-  for (int i0 = 0; i0 < parts; i0 += CAP) {
-    const int n = min(CAP, parts - i0);
-    __syncthreads();
-    for (int i = grp; i < n; i += GR) {
-      const int k = (i0 + i) / GR;
-      float x = 0.0f;
-      if (k < KEEP) {
-#pragma unroll
-        for (int q = 0; q < KEEP; ++q) x = k == q ? keep[q].x : x;
-      } else {
-        x = __ldcg(p.part_ml + slot(i0 + i) * NR + r).x;
-      }
-      buf[i * NR + r] = pat_exp2(x - mu) * inv;
-    }
-    __syncthreads();
-    auto add = [&](int i, int k, float4 v) {
-      const int rr = (tid + k * PAT_THREADS) / 32 % NT * 8 + 2 * (lane & 3);
-      const float f0 = buf[i * NR + rr], f1 = buf[i * NR + rr + 1];
-      a[k].x = fmaf(v.x, f0, a[k].x), a[k].y = fmaf(v.y, f1, a[k].y);
-      a[k].z = fmaf(v.z, f0, a[k].z), a[k].w = fmaf(v.w, f1, a[k].w);
-    };
-    int i = 0;
-    if (i0 == 0) {
-#pragma unroll
-      for (; i < 2; ++i)
-#pragma unroll
-        for (int k = 0; k < PER; ++k) add(i, k, lead[i][k]);
-    }
+  for (int i0 = 0; i0 < parts; i0 += batch) {
+    const int n = min(batch, parts - i0);
+    for (int i = grp; i < n; i += GR) weight[i * NR + r] = pat_exp2(__ldcg(p.part_ml + slot(i0 + i) * NR + r).x - mu) * inv;
+    pat_wait<0>();
+    pat_sync();
 #pragma unroll 4
-    for (; i < n; ++i) {
-      const float4* o = p.part_o + (long long)slot(i0 + i) * ALL;
+    for (int i = 0; i < n; ++i) {
 #pragma unroll
-      for (int k = 0; k < PER; ++k) add(i, k, __ldcg(o + tid + k * PAT_THREADS));
+      for (int k = 0; k < PER; ++k) {
+        const int x = tid + k * THREADS;
+        const int rr = x / 32 % NT * 8 + 2 * (lane & 3);
+        const float f0 = weight[i * NR + rr], f1 = weight[i * NR + rr + 1];
+        float4 v;
+        asm volatile("ld.shared.v4.f32 {%0, %1, %2, %3}, [%4];"
+                     : "=f"(v.x), "=f"(v.y), "=f"(v.z), "=f"(v.w) : "r"(stage + i * PART + x * 16) : "memory");
+        a[k].x = fmaf(v.x, f0, a[k].x), a[k].y = fmaf(v.y, f1, a[k].y);
+        a[k].z = fmaf(v.z, f0, a[k].z), a[k].w = fmaf(v.w, f1, a[k].w);
+      }
     }
+    pat_sync();
+    if (i0 + batch < parts) fetch(i0 + batch);
   }
 #pragma unroll
   for (int k = 0; k < PER; ++k) {
-    const int x = tid + k * PAT_THREADS, rr = r0 + x / 32 % NT * 8 + (lane >> 2);
-    paged_store<BF, D, PAIRS>(p, rr < p.rows ? paged_row(p, b, g, rr) : -1, x / (NT * 32), lane, a[k]);
+    const int x = tid + k * THREADS, rr = r0 + x / 32 % NT * 8 + (lane >> 2);
+    paged_store<BF, D>(p, rr < p.rows ? paged_row(p, b, g, rr) : -1, x / (NT * 32), lane, a[k]);
   }
 }
 
 // The end of a sequence's row tile, or of the CTA's range inside it (whole: neither end was
 // cut): the warps are joined, a whole sequence is written, a part goes to the workspace.
-// o, m (in log2 units), l: a warp's fragments; l is not summed over the lanes yet.
-template <int D, int NT, bool BF, bool PAIRS, typename Pos>
+// o, m (in log2 units), l: a warp's fragments; l is not summed over the lanes yet.  obuf: room
+// for one 8-row tile of O of every warp.
+template <int D, int NT, bool BF, typename Pos>
 __device__ __forceinline__ void paged_finish(const PagedAttnArgs& p, const Pos& at, bool whole, int part, float (&o)[D / 16][NT][4],
                                              const float (&m)[NT][2], const float (&l)[NT][2], float4* obuf, float* sm_m,
                                              float* sm_l, const PagedCut& range, PagedPart* cuts, bool* joins) {
@@ -457,7 +442,7 @@ __device__ __forceinline__ void paged_finish(const PagedAttnArgs& p, const Pos& 
         sm_l[warp * NR + nt * 8 + 2 * lane + e] = x;
       }
     }
-  __syncthreads();
+  pat_sync();
   float inv[NT][2];
 #pragma unroll
   for (int nt = 0; nt < NT; ++nt)
@@ -485,11 +470,11 @@ __device__ __forceinline__ void paged_finish(const PagedAttnArgs& p, const Pos& 
   for (int nt = 0; nt < NT; ++nt) {
     const int r = r0 + nt * 8 + (lane >> 2);
     const long long row = r < p.rows ? paged_row(p, at.b, at.g, r) : -1;
-    if (nt > 0) __syncthreads();
+    if (nt > 0) pat_sync();
 #pragma unroll
     for (int mt = 0; mt < MT; ++mt)
       obuf[(warp * MT + mt) * 32 + lane] = make_float4(o[mt][nt][0], o[mt][nt][1], o[mt][nt][2], o[mt][nt][3]);
-    __syncthreads();
+    pat_sync();
 #pragma unroll
     for (int k = 0; k < MT / PAT_WARPS; ++k) {
       const int mt = warp + k * PAT_WARPS;
@@ -502,12 +487,12 @@ __device__ __forceinline__ void paged_finish(const PagedAttnArgs& p, const Pos& 
       }
       a.x *= inv[nt][0], a.y *= inv[nt][1], a.z *= inv[nt][0], a.w *= inv[nt][1];
       if (whole)
-        paged_store<BF, D, PAIRS>(p, row, mt, lane, a);
+        paged_store<BF, D>(p, row, mt, lane, a);
       else
         p.part_o[(((long long)slot * MT + mt) * NT + nt) * 32 + lane] = a;
     }
   }
-  __syncthreads();
+  pat_sync();
   if (!whole && tid == 0) {
     const int head = at.w - at.unit, c0 = range.cta_of(head);   // the sequence's first unit and CTA
     cuts[part] = {at.b, at.g, r0, c0, range.cta_of(head + at.nu - 1) - c0 + 1};
@@ -516,17 +501,16 @@ __device__ __forceinline__ void paged_finish(const PagedAttnArgs& p, const Pos& 
   }
 }
 // Cut sequences (at most the range's first and last): the last of their CTAs to get here joins the parts.
-template <int D, int NT, bool BF, bool PAIRS>
-__device__ __forceinline__ void paged_leave(const PagedAttnArgs& p, const PagedPart* cuts, bool* joins, float4* obuf) {
+template <int D, int NT, bool BF>
+__device__ __forceinline__ void paged_leave(const PagedAttnArgs& p, const PagedPart* cuts, bool* joins, uint8_t* buf, int room) {
   if (threadIdx.x == 0 && cuts[1].parts > 0) joins[1] = paged_arrive(p, cuts[1]);
-  __syncthreads();
+  pat_sync();
   for (int k = 0; k < 2; ++k) {
     const PagedPart x = cuts[k];
-    if (joins[k]) paged_join<D, NT, BF, PAIRS>(p, x.b, x.g, x.r0, x.c0, x.parts, reinterpret_cast<float*>(obuf));
-    __syncthreads();
+    if (joins[k]) paged_join<D, NT, BF>(p, x.b, x.g, x.r0, x.c0, x.parts, buf, room);
+    pat_sync();
   }
 }
-
 // Page of `keys` keys (of one page, from `key` on) through a window; PAGED_UNSEEN where no row
 // sees any of them: their pages may have been given back.
 constexpr int PAGED_UNSEEN = -0x7fffffff;
@@ -807,12 +791,13 @@ __global__ void __launch_bounds__(PAT_THREADS, PAT_CTAS_PER_SM) paged_attention_
       for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
         for (int e = 0; e < 2; ++e) m[nt][e] *= p.scale_log2;
-      paged_finish<D, NT, BF, false>(p, at, ends && first_unit == 0, first_unit == 0 ? 1 : 0, o, m, l, obuf, sm_m, sm_l, s_range,
-                                     s_cut, s_join);
+      paged_finish<D, NT, BF>(p, at, ends && first_unit == 0, first_unit == 0 ? 1 : 0, o, m, l, obuf, sm_m, sm_l,
+                                         s_range, s_cut, s_join);
     }
     at.next(p);
   }
-  paged_leave<D, NT, BF, false>(p, s_cut, s_join, obuf);
+  pat_wait<0>();
+  paged_leave<D, NT, BF>(p, s_cut, s_join, pat_smem, S::RING + S::OBUF);
 }
 
 }  // namespace simsd

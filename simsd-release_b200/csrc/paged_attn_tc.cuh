@@ -123,11 +123,11 @@ __device__ __forceinline__ void ptc_tma(uint32_t dst, const void* map, uint32_t 
 
 // Joins the parts of a cut sequence (rows r0 .. r0 + R - 1 of KV head g), as
 // paged_join; parts hold R rows of D.  `buf`: parts * R float2 of shared memory.
-template <int D, int R, bool BF>
+template <int D, int R, bool BF, int THREADS = PTC_THREADS>
 __device__ void ptc_join(const PagedAttnArgs& p, const PagedPart& x, float2* buf) {
   const int tid = threadIdx.x;
   auto slot = [&](int i) { return (long long)(i == 0 ? 2 * x.c0 + 1 : 2 * (x.c0 + i)); };
-  for (int k = tid; k < x.parts * R; k += PTC_THREADS) buf[k] = __ldcg(p.part_ml + slot(k / R) * R + k % R);
+  for (int k = tid; k < x.parts * R; k += THREADS) buf[k] = __ldcg(p.part_ml + slot(k / R) * R + k % R);
   __syncthreads();
   // (maximum, 1 / sum) of a row from its parts, in order
   auto law = [&](int r, bool lse) {
@@ -141,13 +141,13 @@ __device__ void ptc_join(const PagedAttnArgs& p, const PagedPart& x, float2* buf
   const float* po = reinterpret_cast<const float*>(p.part_o);
   // four dims of IT rows a thread at a time, so that several parts of each are on their way
   constexpr int IT = 4, ALL = R * (D / 4), C4 = D / 4;
-  for (int k0 = 0; k0 < ALL; k0 += IT * PTC_THREADS) {
+  for (int k0 = 0; k0 < ALL; k0 += IT * THREADS) {
     float4 a[IT];
     float2 lw[IT];
     int r[IT], c[IT];
 #pragma unroll
     for (int u = 0; u < IT; ++u) {
-      const int k = k0 + u * PTC_THREADS + tid;
+      const int k = k0 + u * THREADS + tid;
       r[u] = min(k / C4, R - 1), c[u] = k % C4;
       a[u] = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
       lw[u] = law(r[u], k < ALL && c[u] == 0);
@@ -167,7 +167,7 @@ __device__ void ptc_join(const PagedAttnArgs& p, const PagedPart& x, float2* buf
     }
 #pragma unroll
     for (int u = 0; u < IT; ++u)
-      if (k0 + u * PTC_THREADS + tid < ALL && x.r0 + r[u] < p.rows)
+      if (k0 + u * THREADS + tid < ALL && x.r0 + r[u] < p.rows)
         *(reinterpret_cast<uint2*>(reinterpret_cast<uint16_t*>(p.o) + paged_row(p, x.b, x.g, x.r0 + r[u]) * D) + c[u]) =
             make_uint2(pat_pack<BF>(a[u].x, a[u].y), pat_pack<BF>(a[u].z, a[u].w));
   }

@@ -88,27 +88,10 @@ template <int D, bool BF>
 int attend_window(const PagedAttnArgs& a, const PagedPlan& pl, void* stream) {
   return pl.nr == 8 ? attend<D, 1, BF, true>(a, pl, stream) : attend<D, 2, BF, true>(a, pl, stream);
 }
-// A TMA map of a cache for loads of `block` tokens of one page and head; false where
-// the driver will not describe it (a stride of 0, say).
+// Loads of `block` tokens of one page and head, 64 dims at a time.
 bool cache_map(CUtensorMap* m, const void* base, const PagedAttnArgs& a, int D, int block, bool bf) {
-  static const PFN_cuTensorMapEncodeTiled_v12000 encode = [] {
-    void* fn = nullptr;
-    cudaDriverEntryPointQueryResult q;
-    if (cudaGetDriverEntryPointByVersion("cuTensorMapEncodeTiled", &fn, 12000, cudaEnableDefault, &q) != cudaSuccess ||
-        q != cudaDriverEntryPointSuccess) {
-      (void)cudaGetLastError();
-      fn = nullptr;
-    }
-    return reinterpret_cast<PFN_cuTensorMapEncodeTiled_v12000>(fn);
-  }();
-  if (encode == nullptr) return false;
-  const cuuint64_t dims[4] = {(cuuint64_t)D, (cuuint64_t)a.page_size, (cuuint64_t)a.Hk, (cuuint64_t)a.num_pages};
-  const cuuint64_t strides[3] = {(cuuint64_t)a.ld_tok * 2, (cuuint64_t)a.ld_head * 2, (cuuint64_t)a.ld_page * 2};
-  const cuuint32_t box[4] = {64, (cuuint32_t)block, 1, 1}, step[4] = {1, 1, 1, 1};
-  if (a.ld_tok <= 0 || a.ld_head <= 0 || a.ld_page <= 0) return false;
-  return encode(m, bf ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16, 4, const_cast<void*>(base), dims,
-                strides, box, step, CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B,
-                CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+  return paged_cache_map(m, base, a, bf ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16, 2, D, 64, block,
+                         CU_TENSOR_MAP_SWIZZLE_128B);
 }
 
 template <int D, int R, bool BF>

@@ -3,9 +3,10 @@
 #include <cuda_runtime.h>
 
 #include <algorithm>
+#include <cstring>
 
 #include "paged8.cuh"
-#include "paged_attn8.cuh"
+#include "paged_attn8_run.cuh"
 #include "serving_host.cuh"
 #include "simsd_b200.h"
 
@@ -24,20 +25,6 @@ template <int D, bool BF>
 int append8(const PagedAppend8Args& a, void* stream) {
   const int grid = (int)std::min<long long>(cdiv(a.tasks, PA8_WARPS), 32LL * sm_count());
   return launch_on(paged_append8_kernel<D, BF>, dim3((unsigned)grid), PA8_THREADS, 0, stream, false, a);
-}
-
-template <int D, int NT, bool BF, bool WIN>
-int attend8(const PagedAttn8Args& a, const PagedPlan& pl, void* stream) {
-  static bool done[kMaxDev];
-  constexpr int smem = Pat8Shape<D, NT>::BYTES;
-  const int rc = allow_smem(paged_attention8_kernel<D, NT, BF, WIN>, smem, done);
-  if (rc != SIMSD_OK) return rc;
-  return launch_on(paged_attention8_kernel<D, NT, BF, WIN>, dim3((unsigned)pl.grid), PAT_THREADS, smem, stream, false, a);
-}
-template <int D, bool BF>
-int attend8_rows(const PagedAttn8Args& a, const PagedPlan& pl, void* stream) {
-  if (a.a.window) return pl.nr == 8 ? attend8<D, 1, BF, true>(a, pl, stream) : attend8<D, 2, BF, true>(a, pl, stream);
-  return pl.nr == 8 ? attend8<D, 1, BF, false>(a, pl, stream) : attend8<D, 2, BF, false>(a, pl, stream);
 }
 
 }  // namespace
@@ -101,9 +88,13 @@ int simsd_paged_append8(const void* qkv, int64_t ldq_b, int64_t ldq_t, int B, in
   a.num_pages = num_pages;
   a.max_pages = max_pages;
   a.blocks = (int)(((long long)L + block - 2) / block + 1);   // that L neighbouring tokens can touch
-  a.chunks = (int)cdiv(L, PA8_ROWS);
+  // queries: as many heads a task, up to 8, as leave every SM 16 warps of them
+  a.q_chunks = (int)cdiv(L, 32 / (head_dim / 16));
+  a.q_heads = 8;
+  while (a.q_heads > 1 && (long long)B * a.q_chunks * cdiv(Hq, a.q_heads) < 16LL * sm_count()) a.q_heads /= 2;
+  a.q_groups = (int)cdiv(Hq, a.q_heads);
   a.eps = eps;
-  const long long kv = (long long)B * a.blocks * 2 * Hk, all = kv + (long long)B * a.chunks * Hq;
+  const long long kv = (long long)B * a.blocks * 2 * Hk, all = kv + (long long)B * a.q_chunks * a.q_groups;
   if (all > 0x7fffffffLL) return SIMSD_ERR_UNSUPPORTED;
   a.kv_tasks = (int)kv;
   a.tasks = (int)all;
@@ -113,7 +104,7 @@ int simsd_paged_append8(const void* qkv, int64_t ldq_b, int64_t ldq_t, int B, in
 
 size_t simsd_paged_attention8_workspace_size(int L, int Hq, int Hk, int head_dim) {
   if (L < 1 || Hq < 1 || Hk < 1 || Hq % Hk || head_dim < 1) return 256;
-  return paged_plan_tiles((long long)L * (Hq / Hk), head_dim).bytes;
+  return paged_plan8((long long)L * (Hq / Hk), head_dim).bytes;
 }
 
 int simsd_paged_attention8(const void* q, const void* k_cache, const void* v_cache, const float* k_scale,
@@ -124,6 +115,7 @@ int simsd_paged_attention8(const void* q, const void* k_cache, const void* v_cac
                            int head_dim, float scale, int window, int sinks, void* o, float* lse, int dtype,
                            void* workspace, size_t workspace_bytes, int* err_word, void* stream) {
   PagedAttn8Args t;
+  std::memset(&t, 0, sizeof(t));
   PagedAttnArgs& a = t.a;
   int rc = paged_attn_request(a, q, k_cache, v_cache, num_pages, page_size, page_table, ld_table, max_pages, seq_lens, tail_mask,
                               ldm_b, ldm_t, B, L, Hq, Hk, head_dim, scale, window, sinks, o, lse, dtype, err_word);
@@ -141,7 +133,7 @@ int simsd_paged_attention8(const void* q, const void* k_cache, const void* v_cac
   t.lds_head = lds_head;
   t.lds_block = lds_block;
   t.block_div = paged_div(block);
-  const PagedPlan pl = paged_plan_tiles(a.rows, head_dim);
+  const PagedPlan pl = paged_plan8(a.rows, head_dim);
   rc = paged_attn_plan(a, pl, workspace, workspace_bytes);
   if (rc != SIMSD_OK) return rc;
   if (dtype == SIMSD_BF16)

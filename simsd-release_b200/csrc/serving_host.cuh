@@ -1,5 +1,6 @@
 // What the translation units of the batched serving operators share on the host.
 #pragma once
+#include <cudaTypedefs.h>
 #include <cuda_runtime.h>
 
 #include <algorithm>
@@ -81,6 +82,11 @@ inline PagedPlan paged_plan_of(int nr, int ctas_per_sm, int D) {
 }
 // with mma.sync: tiles of 8 or 16 rows
 inline PagedPlan paged_plan_tiles(long long rows, int D) { return paged_plan_of(rows <= 8 ? 8 : 16, PAT_CTAS_PER_SM, D); }
+// over the 8-bit cache: up to 8 rows with mma.sync, three CTAs an SM, else tcgen05
+inline PagedPlan paged_plan8(long long rows, int D) {
+  if (rows <= 8) return paged_plan_of(8, 3, D);
+  return paged_plan_of(rows <= 32 ? 32 : rows <= 64 ? 64 : 128, 1, D);
+}
 
 // A request of paged attention, the sizes that every form of it refuses, and its arguments
 // but for what goes by the form: the caches' strides and the plan's part.
@@ -126,6 +132,28 @@ inline int paged_attn_request(PagedAttnArgs& a, const void* q, const void* k_cac
   a.scale_log2 = std::max(std::fabs(scale) * 1.4426950408889634f, 1e-30f);
   a.rows = a.G * L;
   return SIMSD_OK;
+}
+// A TMA map of a cache for loads of `dims` dims of `block` tokens of one page and head; false
+// where the driver will not describe it (a stride of 0, say).
+inline bool paged_cache_map(CUtensorMap* m, const void* base, const PagedAttnArgs& a, CUtensorMapDataType type, int size, int D,
+                            int dims, int block, CUtensorMapSwizzle swizzle) {
+  static const PFN_cuTensorMapEncodeTiled_v12000 encode = [] {
+    void* fn = nullptr;
+    cudaDriverEntryPointQueryResult q;
+    if (cudaGetDriverEntryPointByVersion("cuTensorMapEncodeTiled", &fn, 12000, cudaEnableDefault, &q) != cudaSuccess ||
+        q != cudaDriverEntryPointSuccess) {
+      (void)cudaGetLastError();
+      fn = nullptr;
+    }
+    return reinterpret_cast<PFN_cuTensorMapEncodeTiled_v12000>(fn);
+  }();
+  if (encode == nullptr) return false;
+  const cuuint64_t extent[4] = {(cuuint64_t)D, (cuuint64_t)a.page_size, (cuuint64_t)a.Hk, (cuuint64_t)a.num_pages};
+  const cuuint64_t strides[3] = {(cuuint64_t)a.ld_tok * size, (cuuint64_t)a.ld_head * size, (cuuint64_t)a.ld_page * size};
+  const cuuint32_t box[4] = {(cuuint32_t)dims, (cuuint32_t)block, 1, 1}, step[4] = {1, 1, 1, 1};
+  if (a.ld_tok <= 0 || a.ld_head <= 0 || a.ld_page <= 0) return false;
+  return encode(m, type, 4, const_cast<void*>(base), extent, strides, box, step, CU_TENSOR_MAP_INTERLEAVE_NONE, swizzle,
+                CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
 }
 inline int paged_attn_plan(PagedAttnArgs& a, const PagedPlan& pl, void* workspace, size_t workspace_bytes) {
   if (workspace == nullptr || workspace_bytes < pl.bytes) return SIMSD_ERR_WORKSPACE;

@@ -363,6 +363,9 @@ ATT = [
     ([1000, 129, 128, 127], 32, 32, 8, 128, 16, 16, "hnd", BF, "each"), ([260, 3], 70, 2, 1, 128, 64, 16, "nhd", BF, "one"),
     ([6000], 4, 32, 4, 128, 128, 128, "hnd", BF, None), ([10] * 200, 1, 8, 4, 64, 16, 8, "hnd", BF, None),
     ([0] * 5, 2, 4, 2, 128, 16, 16, "hnd", BF, None), ([640] * 9, 1, 24, 1, 128, 16, 16, "hnd", BF, None),
+    # many units a CTA: every ring goes round, with and without TMA
+    ([2500 + 97 * i for i in range(12)], 4, 32, 8, 128, 16, 16, "hnd", BF, None), ([3000, 1, 5000, 900] * 4, 3, 28, 4, 64, 4, 2, "nhd", FP, "each"),
+    ([4000] * 6, 20, 32, 8, 128, 64, 64, "hnd", BF, "one"), ([40000, 30000], 2, 64, 8, 128, 1, 1, "hnd", BF, None),
 ]
 
 
