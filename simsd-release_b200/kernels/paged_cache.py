@@ -55,6 +55,17 @@ def _on_16_bytes(t: torch.Tensor | None) -> torch.Tensor | None:
     return t if t is None or t.data_ptr() % 16 == 0 else t.clone()
 
 
+def _check_scales(what: str, k_cache, k_scale, v_scale) -> None:
+    if k_scale.dtype != torch.float32 or v_scale.dtype != torch.float32:
+        raise TypeError(f"{what}: the scales are fp32")
+    if (k_scale.ndim != 3 or k_scale.shape != v_scale.shape or k_scale.shape[:2] != k_cache.shape[:2] or k_scale.shape[2] < 1
+            or k_cache.shape[2] % k_scale.shape[2]):
+        raise ValueError(f"{what}: k_scale and v_scale must both be [{k_cache.shape[0]}, {k_cache.shape[1]}, page_size / block] "
+                         f"for pages of {k_cache.shape[2]}, got {tuple(k_scale.shape)} / {tuple(v_scale.shape)}")
+    if k_scale.stride() != v_scale.stride():
+        raise ValueError(f"{what}: k_scale and v_scale must have the same strides")
+
+
 def _mask_strides(tail_mask: torch.Tensor | None):
     """(tail_mask with a unit last stride, its strides of a sequence and of a query)."""
     if tail_mask is None:
@@ -138,7 +149,7 @@ def paged_append(qkv: torch.Tensor, heads: int, kv_heads: int, k_cache: torch.Te
 
 
 def _check_attention(q, k_cache, v_cache, page_table, seq_lens, tail_mask, window, sinks, what="paged_attention",
-                     cache_dtype=None) -> None:
+                     cache_dtype=None, scales=()) -> None:
     """Raise what is wrong with a request of paged_attention (or, as `what`, of paged_attention8)."""
     if q.dtype not in _HALF:
         raise TypeError(f"{what} takes bf16 or fp16 queries, got {q.dtype}")
@@ -150,6 +161,8 @@ def _check_attention(q, k_cache, v_cache, page_table, seq_lens, tail_mask, windo
     _check_cache(what, k_cache, v_cache, Hk, cache_dtype or q.dtype)
     if k_cache.shape[3] != D or Hk < 1 or Hq < 1 or Hq % Hk:
         raise ValueError(f"q heads {Hq} x {D} do not go with the cache's {Hk} x {k_cache.shape[3]}")
+    if scales:
+        _check_scales(what, k_cache, *scales)
     if page_table.dtype != torch.int32 or seq_lens.dtype != torch.int32:
         raise TypeError(f"{what}: page_table and seq_lens are int32")
     if page_table.ndim != 2 or page_table.shape[0] != B or seq_lens.shape != (B,):
@@ -164,7 +177,7 @@ def _check_attention(q, k_cache, v_cache, page_table, seq_lens, tail_mask, windo
         raise ValueError(f"window must be at least 1 (None: no window), got {window}")
     if sinks < 0:
         raise ValueError(f"sinks must not be negative, got {sinks}")
-    _lib.require_cuda(q, k_cache, v_cache, page_table, seq_lens, tail_mask)
+    _lib.require_cuda(q, k_cache, v_cache, page_table, seq_lens, tail_mask, *scales)
 
 
 def paged_attention(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor, page_table: torch.Tensor,

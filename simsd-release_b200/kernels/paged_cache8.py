@@ -23,7 +23,7 @@ from __future__ import annotations
 import torch
 
 from . import _lib
-from .paged_cache import (_HALF, _check_attention, _check_cache, _current_device, _current_stream, _mask_strides, _on_16_bytes,
+from .paged_cache import (_HALF, _check_attention, _check_cache, _check_scales, _current_device, _current_stream, _mask_strides, _on_16_bytes,
                           _window)
 
 F8 = torch.float8_e4m3fn
@@ -36,17 +36,6 @@ def cache8(pages: int, kv_heads: int, page_size: int, head_dim: int, block: int 
     shape, scales = (pages, kv_heads, page_size, head_dim), (pages, kv_heads, page_size // block)
     return (*(torch.zeros(shape, dtype=F8, device=device) for _ in range(2)),
             *(torch.zeros(scales, dtype=torch.float32, device=device) for _ in range(2)))
-
-
-def _check_scales(what: str, k_cache, k_scale, v_scale) -> None:
-    if k_scale.dtype != torch.float32 or v_scale.dtype != torch.float32:
-        raise TypeError(f"{what}: the scales are fp32")
-    if (k_scale.ndim != 3 or k_scale.shape != v_scale.shape or k_scale.shape[:2] != k_cache.shape[:2] or k_scale.shape[2] < 1
-            or k_cache.shape[2] % k_scale.shape[2]):
-        raise ValueError(f"{what}: k_scale and v_scale must both be [{k_cache.shape[0]}, {k_cache.shape[1]}, page_size / block] "
-                         f"for pages of {k_cache.shape[2]}, got {tuple(k_scale.shape)} / {tuple(v_scale.shape)}")
-    if k_scale.stride() != v_scale.stride():
-        raise ValueError(f"{what}: k_scale and v_scale must have the same strides")
 
 
 def _check_append8(qkv, heads, kv_heads, k_cache, v_cache, k_scale, v_scale, page_table, seq_lens, cos, sin, q_weight, k_weight,
@@ -153,9 +142,7 @@ def paged_attention8(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tens
         return o
     if torch.is_grad_enabled() and (q.requires_grad or k_scale.requires_grad or v_scale.requires_grad):
         raise RuntimeError("paged_attention8 is a forward-only inference kernel.")
-    _check_attention(q, k_cache, v_cache, page_table, seq_lens, tail_mask, window, sinks, "paged_attention8", F8)
-    _check_scales("paged_attention8", k_cache, k_scale, v_scale)
-    _lib.require_cuda(q, k_scale, v_scale)
+    _check_attention(q, k_cache, v_cache, page_table, seq_lens, tail_mask, window, sinks, "paged_attention8", F8, (k_scale, v_scale))
     dev, shape, strides = q.get_device(), k_cache.shape, k_cache.stride()
     if _current_device() != dev:
         with torch.cuda.device(dev):

@@ -67,9 +67,9 @@ def paged_reserve(page_table: torch.Tensor, lens: torch.Tensor, held: torch.Tens
     out = _lib.binding().paged_reserve(page_table, lens, held, free_pages, free_count, L, page_size, count)
     if out is not None:
         return out
-    _check_state("paged_reserve", page_table, free_pages, free_count, page_size, lens=lens, held=held, count=count)
     if L < 0:
         raise ValueError(f"paged_reserve: L must not be negative, got {L}")
+    _check_state("paged_reserve", page_table, free_pages, free_count, page_size, lens=lens, held=held, count=count)
     dev = page_table.get_device()
     if _current_device() != dev:
         with torch.cuda.device(dev):
