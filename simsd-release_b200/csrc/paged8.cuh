@@ -39,6 +39,7 @@ struct PagedAppend8Args {
   int kv_tasks, tasks;      // warps' tasks: blocks of a key or value head, then rows of some query heads
   int B, L, Hq, Hk, R, page_size, block, num_pages, max_pages, blocks;   // blocks that a sequence's rows can touch
   int q_heads, q_groups, q_chunks;   // query heads of a task, groups of them, groups of rows
+  int span;                 // tokens of a task of keys or values: a block, or 16 where blocks are smaller and divide that
   float eps;
 };
 
@@ -108,7 +109,8 @@ struct P8Turn {               // a lane's cos, sin and -sin
 // (or 16 next to each other of the unrotated rest), so that the rotation needs no exchange.
 //
 // A task of keys or values is one (sequence, block, head): 16 rows in shared memory (longer blocks
-// twice over: for the largest magnitude, then to be stored).  A task of queries is four (D
+// twice over: for the largest magnitude, then to be stored); blocks of 1, 2, 4 or 8 tokens go 16
+// tokens a task.  A task of queries is four (D
 // 128) or eight rows of some neighbouring heads: the rotary row and the weight stay in registers over these.
 template <int D, bool BF>
 __global__ void __launch_bounds__(PA8_THREADS, 4) paged_append8_kernel(const PagedAppend8Args p) {
@@ -121,7 +123,9 @@ __global__ void __launch_bounds__(PA8_THREADS, 4) paged_append8_kernel(const Pag
   const int e0 = pair ? 8 * j : 16 * j, e1 = pair ? p.R / 2 + 8 * j : 16 * j + 8;
   const uint16_t* qkv = reinterpret_cast<const uint16_t*>(p.qkv);
   __shared__ float4 rows[PA8_WARPS][TURNS * 4 * 32];   // a warp's rows in fp32, every lane's its own
+  __shared__ float row_tops[PA8_WARPS][PA8_ROWS];
   float4* own = rows[threadIdx.x >> 5] + lane;
+  float* tops = row_tops[threadIdx.x >> 5];
 
   for (uint32_t task = blockIdx.x * PA8_WARPS + (threadIdx.x >> 5); task < (uint32_t)p.tasks; task += gridDim.x * PA8_WARPS) {
     // ---- which rows of which heads: keys first, then values, then queries
@@ -184,27 +188,28 @@ __global__ void __launch_bounds__(PA8_THREADS, 4) paged_append8_kernel(const Pag
       continue;
     }
     // ---- keys or values: the block's rows t, lo <= t < hi, its page and scale
-    const int block_at = (old / p.block + k) * p.block;
+    const int block_at = (old / p.span + k) * p.span;
     if (block_at >= top || c == 0) continue;
-    const int lo = max(old, block_at) - shift, hi = min(top, block_at + p.block) - shift;
+    const int lo = max(old, block_at) - shift, hi = min(top, block_at + p.span) - shift;
     if (lo >= hi) continue;
     const uint16_t* src = qkv + b * p.ldq_b + (long long)(p.Hq + h) * D;
-    // rows base .. base + 15 into the lane's places of shared memory; their largest magnitude, infinities
-    // among them or not (NaN never)
+    // rows base .. base + 15 into the lane's places of shared memory; the largest magnitudes of its part of
+    // each, infinities among them or not (NaN never)
+    float peak[TURNS];
     auto fill = [&](int base, bool all) {
       uint4 u[TURNS][2];
 #pragma unroll
       for (int i = 0; i < TURNS; ++i) {
         const int t = base + i * ROWS + sub;
         u[i][0] = u[i][1] = make_uint4(0, 0, 0, 0);
-        if (t < hi) {
+        if (t >= lo && t < hi) {
           u[i][0] = __ldg(reinterpret_cast<const uint4*>(src + t * p.ldq_t + e0));
           u[i][1] = __ldg(reinterpret_cast<const uint4*>(src + t * p.ldq_t + e1));
         }
       }
-      float a = 0.0f;
 #pragma unroll
       for (int i = 0; i < TURNS; ++i) {
+        float a = 0.0f;
         uint64_t x[4], y[4];
         paged_unpack8<BF>(u[i][0], x);
         paged_unpack8<BF>(u[i][1], y);
@@ -216,7 +221,7 @@ __global__ void __launch_bounds__(PA8_THREADS, 4) paged_append8_kernel(const Pag
             p8_norm<D, BF>(x, y, row_mask, p.eps, wx, wy);
           }
           const int t = base + i * ROWS + sub;
-          if (pair && t < hi) {
+          if (pair && t >= lo && t < hi) {
             P8Turn turn;
             turn.load(p.cos, p.sin, (long long)(t + shift) * (p.R / 2) + 8 * j);
             p8_rotate(x, y, turn.c, turn.s, turn.n);
@@ -236,24 +241,105 @@ __global__ void __launch_bounds__(PA8_THREADS, 4) paged_append8_kernel(const Pag
             for (int z = 0; z < 8; ++z) a = fmaxf(a, fabsf(w[z]) < INFINITY ? fabsf(w[z]) : 0.0f);
           }
         }
+        peak[i] = a;
       }
-      return a;
     };
+    // a row's stored numbers from its fp32 ones
+    auto put = [&](int i, uint8_t* dst, float inv, bool infinite) {
+      const uint64_t inv2 = f2_pack(inv, inv);
+      uint32_t w[4];
+#pragma unroll
+      for (int q = 0; q < 4; ++q) {
+        const float4 z = own[(i * 4 + q) * 32];
+        float2 u = f2_unpack(f2_mul(f2_pack(z.x, z.y), inv2)), v = f2_unpack(f2_mul(f2_pack(z.z, z.w), inv2));
+        if (infinite) u.x -= u.x - u.x, u.y -= u.y - u.y, v.x -= v.x - v.x, v.y -= v.y - v.y;   // infinities become NaN
+        w[q] = p8_pack2(u.x, u.y) | p8_pack2(v.x, v.y) << 16;
+      }
+      *reinterpret_cast<uint2*>(dst + e0) = make_uint2(w[0], w[1]);
+      *reinterpret_cast<uint2*>(dst + e1) = make_uint2(w[2], w[3]);
+    };
+    // a stored row, rounded anew
+    auto again = [&](uint8_t* row, float ratio) {
+      uint4* at16 = reinterpret_cast<uint4*>(row + 16 * j);
+      const uint4 u = *at16;
+      uint32_t w[4] = {u.x, u.y, u.z, u.w};
+#pragma unroll
+      for (int q = 0; q < 4; ++q) {
+        const uint32_t h0 = p8_half2(w[q] & 0xffffu), h1 = p8_half2(w[q] >> 16);
+        const float2 f0 = __half22float2(*reinterpret_cast<const __half2*>(&h0));
+        const float2 f1 = __half22float2(*reinterpret_cast<const __half2*>(&h1));
+        w[q] = p8_pack2(f0.x * ratio, f0.y * ratio) | p8_pack2(f1.x * ratio, f1.y * ratio) << 16;
+      }
+      *at16 = make_uint4(w[0], w[1], w[2], w[3]);
+    };
+    const int g = key ? h : h - p.Hk;
+    uint8_t* caches = (key ? p.k_cache : p.v_cache) + g * p.ld_head;
+    float* scales = (key ? p.k_scale : p.v_scale) + g * p.lds_head;
+    if (p.span != p.block) {
+      // ---- blocks of less than 16 tokens: those of 16 neighbouring tokens together
+      const int base = block_at - shift;             // row of the first of them; rows lo .. hi - 1 are new
+      fill(base, false);
+#pragma unroll
+      for (int i = 0; i < TURNS; ++i) {
+        float a = peak[i];
+#pragma unroll
+        for (int m = LANES / 2; m > 0; m >>= 1) a = fmaxf(a, __shfl_xor_sync(row_mask, a, m));
+        if (j == 0) tops[i * ROWS + sub] = a;        // 0 for a row that is none
+      }
+      __syncwarp();
+      float s[TURNS], had[TURNS];
+      long long at_page[TURNS];                      // the row's page, or -1
+#pragma unroll
+      for (int i = 0; i < TURNS; ++i) {
+        const int r = i * ROWS + sub, t = base + r, pos = t + shift, first = r / p.block * p.block;
+        at_page[i] = -1, s[i] = had[i] = 0.0f;
+        if (t < lo || t >= hi) continue;
+        const int page = p.page_table[b * p.ld_table + pos / p.page_size];
+        if (page < 0 || page >= p.num_pages) {
+          if (h == 0 && j == 0 && p.err) atomicOr(p.err, SIMSD_DEV_ERR_BAD_INDEX);
+          continue;
+        }
+        at_page[i] = page;
+        float a = 0.0f;
+        for (int q = 0; q < p.block; ++q) a = fmaxf(a, tops[first + q]);
+        if (block_at + first < old) had[i] = scales[page * p.lds_page + pos % p.page_size / p.block * p.lds_block];
+        s[i] = fmaxf(had[i], p8_power(p8_exponent(a)));
+      }
+      __syncwarp();                                  // the scales have been read
+#pragma unroll
+      for (int i = 0; i < TURNS; ++i) {
+        const int r = i * ROWS + sub, t = base + r, pos = t + shift, first = r / p.block * p.block, in = pos % p.page_size;
+        if (at_page[i] < 0) continue;
+        uint8_t* row = caches + at_page[i] * p.ld_page + in * p.ld_tok;
+        put(i, row, 1.0f / s[i], true);
+        if (t != max(lo, base + first)) continue;
+        // the block's first new row: its scale, and where that has grown the older tokens
+        if (j == 0) scales[at_page[i] * p.lds_page + in / p.block * p.lds_block] = s[i];
+        if (block_at + first < old && s[i] != had[i])
+          for (int x = block_at + first; x < old; ++x) again(row - (pos - x) * p.ld_tok, had[i] / s[i]);
+      }
+      __syncwarp();                                  // `tops` has been read
+      continue;
+    }
     const int page = p.page_table[b * p.ld_table + block_at / p.page_size];
     if (page < 0 || page >= p.num_pages) {
       if (h == 0 && lane == 0 && p.err) atomicOr(p.err, SIMSD_DEV_ERR_BAD_INDEX);
       continue;
     }
-    const int g = key ? h : h - p.Hk, in = block_at % p.page_size;
-    uint8_t* cache = (key ? p.k_cache : p.v_cache) + page * p.ld_page + g * p.ld_head + in * p.ld_tok;
-    float* scale = (key ? p.k_scale : p.v_scale) + page * p.lds_page + g * p.lds_head + in / p.block * p.lds_block;
+    const int in = block_at % p.page_size;
+    uint8_t* cache = caches + page * p.ld_page + in * p.ld_tok;
+    float* scale = scales + page * p.lds_page + in / p.block * p.lds_block;
     const bool fresh = block_at >= old;
     const float had = fresh ? 0.0f : *scale;
     // the largest magnitude; where an infinity is it, once more without those
     const int last = lo + (hi - lo - 1) / PA8_ROWS * PA8_ROWS;
     auto largest = [&](bool all) {
       float a = 0.0f;
-      for (int base = lo; base <= last; base += PA8_ROWS) a = fmaxf(a, fill(base, all));
+      for (int base = lo; base <= last; base += PA8_ROWS) {
+        fill(base, all);
+#pragma unroll
+        for (int i = 0; i < TURNS; ++i) a = fmaxf(a, peak[i]);
+      }
 #pragma unroll
       for (int m = 16; m > 0; m >>= 1) a = fmaxf(a, __shfl_xor_sync(0xffffffffu, a, m));
       return a;
@@ -262,7 +348,6 @@ __global__ void __launch_bounds__(PA8_THREADS, 4) paged_append8_kernel(const Pag
     const bool infinite = a == INFINITY;
     if (infinite) a = largest(false);
     const float s = fmaxf(had, p8_power(p8_exponent(a))), inv = 1.0f / s;
-    const uint64_t inv2 = f2_pack(inv, inv);
     if (lane == 0) *scale = s;
     // the new tokens; the last rows are still at hand
     for (int base = last; base >= lo; base -= PA8_ROWS) {
@@ -270,37 +355,12 @@ __global__ void __launch_bounds__(PA8_THREADS, 4) paged_append8_kernel(const Pag
 #pragma unroll
       for (int i = 0; i < TURNS; ++i) {
         const int t = base + i * ROWS + sub;
-        if (t >= hi) continue;
-        uint32_t w[4];
-#pragma unroll
-        for (int q = 0; q < 4; ++q) {
-          const float4 z = own[(i * 4 + q) * 32];
-          float2 u = f2_unpack(f2_mul(f2_pack(z.x, z.y), inv2)), v = f2_unpack(f2_mul(f2_pack(z.z, z.w), inv2));
-          if (infinite) u.x -= u.x - u.x, u.y -= u.y - u.y, v.x -= v.x - v.x, v.y -= v.y - v.y;   // infinities become NaN
-          w[q] = p8_pack2(u.x, u.y) | p8_pack2(v.x, v.y) << 16;
-        }
-        uint8_t* dst = cache + (t + shift - block_at) * p.ld_tok;
-        *reinterpret_cast<uint2*>(dst + e0) = make_uint2(w[0], w[1]);
-        *reinterpret_cast<uint2*>(dst + e1) = make_uint2(w[2], w[3]);
+        if (t < hi) put(i, cache + (t + shift - block_at) * p.ld_tok, inv, infinite);
       }
     }
     // the block's older tokens, where the scale has grown
-    if (!fresh && s != had) {
-      const float ratio = had * inv;
-      for (int t = sub; t < old - block_at; t += ROWS) {
-        uint4* at16 = reinterpret_cast<uint4*>(cache + t * p.ld_tok + 16 * j);
-        const uint4 u = *at16;
-        uint32_t w[4] = {u.x, u.y, u.z, u.w};
-#pragma unroll
-        for (int q = 0; q < 4; ++q) {
-          const uint32_t h0 = p8_half2(w[q] & 0xffffu), h1 = p8_half2(w[q] >> 16);
-          const float2 f0 = __half22float2(*reinterpret_cast<const __half2*>(&h0));
-          const float2 f1 = __half22float2(*reinterpret_cast<const __half2*>(&h1));
-          w[q] = p8_pack2(f0.x * ratio, f0.y * ratio) | p8_pack2(f1.x * ratio, f1.y * ratio) << 16;
-        }
-        *at16 = make_uint4(w[0], w[1], w[2], w[3]);
-      }
-    }
+    if (!fresh && s != had)
+      for (int t = sub; t < old - block_at; t += ROWS) again(cache + t * p.ld_tok, had * inv);
   }
 }
 

@@ -87,7 +87,8 @@ int simsd_paged_append8(const void* qkv, int64_t ldq_b, int64_t ldq_t, int B, in
   a.block = block;
   a.num_pages = num_pages;
   a.max_pages = max_pages;
-  a.blocks = (int)(((long long)L + block - 2) / block + 1);   // that L neighbouring tokens can touch
+  a.span = block < PA8_ROWS && PA8_ROWS % block == 0 ? PA8_ROWS : block;
+  a.blocks = (int)(((long long)L + a.span - 2) / a.span + 1);   // that L neighbouring tokens can touch
   // queries: as many heads a task, up to 8, as leave every SM 16 warps of them
   a.q_chunks = (int)cdiv(L, 32 / (head_dim / 16));
   a.q_heads = 8;

@@ -161,6 +161,9 @@ APPEND = [
     ([17] * 3, [1000, 18, 17], 4, 2, 128, 112, 16, 1, "hnd", FP, True, [17, 1, -3]), ([9], [9], 3, 1, 64, 16, 7, 7, "hnd", BF, False, [50]),
     ([3] * 2, [4, 50], 16, 4, 128, 64, 1, 1, "nhd", BF, True, None), ([300], [300], 2, 1, 128, 128, 48, 24, "both", BF, True, None),
     ([16] * 2, [32, 31], 8, 2, 64, 64, 32, 2, "hnd", BF, True, None),
+    # blocks of less than 16 tokens that start, end and were begun before the call, over pages of less than 16 too
+    ([21] * 4, [21, 22, 530, 100], 6, 2, 128, 128, 8, 8, "hnd", BF, True, [21, 9, 20, 1]), ([50] * 2, [77, 51], 4, 4, 64, 32, 4, 4, "nhd", FP, False, None),
+    ([100], [131], 2, 2, 128, 64, 24, 8, "both", BF, True, None), ([70], [75], 3, 3, 64, 64, 12, 3, "hnd", BF, True, None),
 ]
 
 
