@@ -586,7 +586,8 @@ int simsd_paged_append8(const void* qkv, int64_t ldq_b, int64_t ldq_t, int B, in
 /*
  * simsd_paged_attention_window over that cache (window 0: none).  Any positive scales up to
  * 2^64 do, not only powers of two; sums are fp32 and weights fp16 (11 bits down to 2^-22 of
- * the largest).  The workspace as for simsd_paged_attention, of a size of its own.
+ * the largest).  The workspace as for simsd_paged_attention, of a size of its own; + 4 in the
+ * place of + 3 in the limit there.
  */
 size_t simsd_paged_attention8_workspace_size(int L, int Hq, int Hk, int head_dim);
 int simsd_paged_attention8(const void* q, const void* k_cache, const void* v_cache, const float* k_scale,

@@ -180,9 +180,9 @@ __device__ __forceinline__ bool paged_out(const PagedAttnArgs& p, int n, int key
 // Position in the unit order: sequence b (length n, nu units per KV head and row
 // tile), KV head g, row tile rt, unit of it; w counts units and ends before it.
 // WIN: through a window, whose units are the sequence's but the `skip` ones in its middle.
-template <int TK, bool WIN = false>
+template <int TK, bool WIN = false, int ENDS = PagedEnd<TK>::UNITS>
 struct PagedPos {
-  static constexpr int END = PagedEnd<TK>::UNITS;
+  static constexpr int END = ENDS;
   int b, g, rt, unit, n, nu, w, skip;
   __device__ __forceinline__ void next(const PagedAttnArgs& p) {
     ++w;
@@ -256,8 +256,8 @@ __device__ __forceinline__ void paged_store_lse(const PagedAttnArgs& p, int b, i
 
 // This CTA's place in the cut of the call's units and ends, and the position of its
 // first unit.  False: this CTA has none.
-template <int THREADS, int TK, bool WIN = false>
-__device__ __forceinline__ bool paged_range(const PagedAttnArgs& p, PagedCut& cut, PagedPos<TK, WIN>& pos) {
+template <int THREADS, int TK, bool WIN = false, int ENDS>
+__device__ __forceinline__ bool paged_range(const PagedAttnArgs& p, PagedCut& cut, PagedPos<TK, WIN, ENDS>& pos) {
   constexpr int WARPS = THREADS / 32;
   __shared__ int s_sum[WARPS], s_more[WARPS];
   __shared__ int s_b, s_first;
@@ -268,7 +268,7 @@ __device__ __forceinline__ bool paged_range(const PagedAttnArgs& p, PagedCut& cu
     if (b >= p.B) return 0;
     if (flag && p.seq_lens[b] > (long long)p.max_pages * p.page_size) atomicOr(p.err, SIMSD_DEV_ERR_BAD_INDEX);
     const int n = paged_len(p, b), skip = WIN ? paged_skip<TK>(p, n) : 0;
-    return (paged_units<TK>(n) - skip + PagedEnd<TK>::UNITS) * per;
+    return (paged_units<TK>(n) - skip + ENDS) * per;
   };
   // sequences tid, tid + THREADS, ...: the first of them scanned, the others summed
   int u = units(tid), incl = u, more = 0;
@@ -316,13 +316,13 @@ __device__ __forceinline__ bool paged_range(const PagedAttnArgs& p, PagedCut& cu
   __syncthreads();
   pos.b = s_b;
   pos.measure(p);
-  const int rem = w0 - s_first, hr = rem / (pos.nu + PagedEnd<TK>::UNITS);
-  pos.unit = rem - hr * (pos.nu + PagedEnd<TK>::UNITS);
+  const int rem = w0 - s_first, hr = rem / (pos.nu + ENDS);
+  pos.unit = rem - hr * (pos.nu + ENDS);
   pos.w = w0;
   pos.g = hr / p.row_tiles;
   pos.rt = hr - pos.g * p.row_tiles;
   if (pos.unit >= pos.nu) {          // an end: the unit after it
-    const int w = w0 + pos.nu + PagedEnd<TK>::UNITS - pos.unit;
+    const int w = w0 + pos.nu + ENDS - pos.unit;
     pos.unit = pos.nu - 1;
     pos.next(p);
     pos.w = w;

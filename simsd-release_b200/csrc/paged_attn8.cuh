@@ -46,6 +46,12 @@ struct PagedAttn8Args {
   int run;                  // tokens of a TMA load: the largest power of two <= 32 in the page size, or 0
 };
 
+// Positions in units of 128 keys; a sequence's end weighs as three of them in the cut: at 1, 2, 3, 4 and 6
+// 32 x 0.3 - 4k tokens take 28.5, 27, 26.3, 27.4 and 29 us; 19 windowed rows of 5 take 28.3 at 2 and 29 at 3.
+constexpr int P8_END = 3;
+template <bool WIN>
+using P8Pos = PagedPos<128, WIN, P8_END>;
+
 template <int D>
 struct Pat8Shape {
   static constexpr int NR = 8;
@@ -113,11 +119,11 @@ __device__ __forceinline__ void p8_cp_arrive(uint32_t bar) {
 // unit ahead.  TMA: a lane per run; one without a key that is read loads zeros, from past the
 // last page.  Else the lane's keys are lane, 32 + lane, ...: their places are handed round.
 template <int D, bool WIN, bool TMA>
-__device__ __forceinline__ void p8_load(const PagedAttn8Args& args, PagedPos<Pat8Shape<D>::TK, WIN> ld, int end, uint32_t ring, uint32_t scales,
+__device__ __forceinline__ void p8_load(const PagedAttn8Args& args, P8Pos<WIN> ld, int end, uint32_t ring, uint32_t scales,
                                         uint32_t full, uint32_t empty, volatile int* abort_flag) {
   using S = Pat8Shape<D>;
   constexpr int TK = S::TK;
-  using Pos = PagedPos<TK, WIN>;
+  using Pos = P8Pos<WIN>;
   constexpr int CH = D / 16, KPI = 32 / CH, EACH = TK / 32;      // chunks of a key, keys of a copy, keys of a lane
   const PagedAttnArgs& p = args.a;
   const int lane = threadIdx.x & 31, kc = lane % CH, khi = lane / CH;
@@ -207,7 +213,7 @@ __global__ void __launch_bounds__(Pat8Shape<D>::THREADS, Pat8Shape<D>::CTAS) pag
   using S = Pat8Shape<D>;
   constexpr int NR = S::NR;
   constexpr int MT = D / 16, CH = D / 16;                 // 16-dim tiles, 16-byte chunks of a key
-  using Pos = PagedPos<S::TK, WIN>;
+  using Pos = P8Pos<WIN>;
   extern __shared__ uint8_t pat8_raw[];
   __shared__ PagedPart s_cut[2];
   __shared__ bool s_join[2];

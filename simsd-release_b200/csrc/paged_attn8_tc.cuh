@@ -46,7 +46,7 @@ struct P8tShape {
 // the lane's keys are lane, 32 + lane, ...: their places are handed round.  The page numbers are
 // fetched a unit ahead.
 template <int D, bool TMA, typename S>
-__device__ __forceinline__ void p8t_load(const PagedAttn8Args& args, PagedPos<PTC_TK, true> ld, int end, int kv, uint32_t raw,
+__device__ __forceinline__ void p8t_load(const PagedAttn8Args& args, P8Pos<true> ld, int end, int kv, uint32_t raw,
                                          uint32_t full, uint32_t empty, volatile int* abort_flag) {
   constexpr int CH = D / 16, KPI = 32 / CH, EACH = PTC_TK / 32, PAGES = TMA ? 1 : EACH;
   const PagedAttnArgs& p = args.a;
@@ -57,7 +57,7 @@ __device__ __forceinline__ void p8t_load(const PagedAttn8Args& args, PagedPos<PT
   const uint8_t* base = reinterpret_cast<const uint8_t*>(kv ? p.v_cache : p.k_cache);
   if (TMA && lane == 0) prefetch_tmap(map);
   int page[PAGES];
-  auto fetch_pages = [&](const PagedPos<PTC_TK, true>& x) {
+  auto fetch_pages = [&](const P8Pos<true>& x) {
 #pragma unroll
     for (int i = 0; i < PAGES; ++i)
       page[i] = !TMA || lane < runs ? paged_page(p, x, x.key(p) + (TMA ? lane * run : i * 32 + lane), run) : -1;
@@ -113,7 +113,7 @@ __device__ __forceinline__ void p8t_load(const PagedAttn8Args& args, PagedPos<PT
 // The warp that brings the scales: lane, 32 + lane, ... of every unit, loaded a unit ahead of
 // their use, their pages two.
 template <typename S>
-__device__ __forceinline__ void p8t_scales(const PagedAttn8Args& args, PagedPos<PTC_TK, true> ld, int end, float* sc, uint32_t full,
+__device__ __forceinline__ void p8t_scales(const PagedAttn8Args& args, P8Pos<true> ld, int end, float* sc, uint32_t full,
                                            uint32_t empty, volatile int* abort_flag) {
   constexpr int EACH = PTC_TK / 32;
   const PagedAttnArgs& p = args.a;
@@ -201,7 +201,7 @@ __global__ void __launch_bounds__(P8T_THREADS, 1) paged_attention8_tc_kernel(con
   }
   griddep_launch_dependents();
   griddep_wait();
-  PagedPos<PTC_TK, true> at;
+  P8Pos<true> at;
   PagedCut cut;
   tc_fence_before();
   __syncthreads();
@@ -529,7 +529,7 @@ __global__ void __launch_bounds__(P8T_THREADS, 1) paged_attention8_tc_kernel(con
         const bool ends = at.unit + 1 == at.nu, leaves = ends || at.w + 1 >= end;
         if (ends && at.w + 1 + at.END < end) {
           int b = at.b, g = at.g, rt = at.rt;
-          PagedPos<PTC_TK, true>::next_rows(p, b, g, rt);
+          P8Pos<true>::next_rows(p, b, g, rt);
           put_queries(b, g, rt);
         }
         if (strange || leaves) {

@@ -135,7 +135,7 @@ int simsd_paged_attention8(const void* q, const void* k_cache, const void* v_cac
   t.lds_block = lds_block;
   t.block_div = paged_div(block);
   const PagedPlan pl = paged_plan8(a.rows, head_dim);
-  rc = paged_attn_plan(a, pl, workspace, workspace_bytes);
+  rc = paged_attn_plan(a, pl, workspace, workspace_bytes, P8_END);
   if (rc != SIMSD_OK) return rc;
   if (dtype == SIMSD_BF16)
     return head_dim == 64 ? attend8_rows<64, true>(t, pl, stream) : attend8_rows<128, true>(t, pl, stream);

@@ -155,10 +155,11 @@ inline bool paged_cache_map(CUtensorMap* m, const void* base, const PagedAttnArg
   return encode(m, type, 4, const_cast<void*>(base), extent, strides, box, step, CU_TENSOR_MAP_INTERLEAVE_NONE, swizzle,
                 CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
 }
-inline int paged_attn_plan(PagedAttnArgs& a, const PagedPlan& pl, void* workspace, size_t workspace_bytes) {
+// `end`: what a sequence's end weighs in the cut
+inline int paged_attn_plan(PagedAttnArgs& a, const PagedPlan& pl, void* workspace, size_t workspace_bytes, int end = PAGED_END_MAX) {
   if (workspace == nullptr || workspace_bytes < pl.bytes) return SIMSD_ERR_WORKSPACE;
   a.row_tiles = (a.rows + pl.nr - 1) / pl.nr;
-  if ((long long)a.B * a.Hk * a.row_tiles * ((int64_t)a.max_pages * a.page_size / PAT_TK + 1 + PAGED_END_MAX) > 0x7fffffffLL)
+  if ((long long)a.B * a.Hk * a.row_tiles * ((int64_t)a.max_pages * a.page_size / PAT_TK + 1 + end) > 0x7fffffffLL)
     return SIMSD_ERR_UNSUPPORTED;
   uint8_t* ws = reinterpret_cast<uint8_t*>(workspace);
   a.arrived = reinterpret_cast<int*>(ws);
