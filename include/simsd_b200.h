@@ -546,7 +546,8 @@ int simsd_paged_attention(const void* q, const void* k_cache, const void* v_cach
 /*
  * The same through a window: the query at position x = n - L + t sees a key j only where
  * also j > x - window or j < sinks (window 0: no window, every key).  Keys that no query of
- * the call sees are not read, and the pages that hold nothing else may be any.
+ * the call sees are not read, and the pages that hold nothing else may be any.  With a
+ * window max_pages page_size <= 2^30 (more: SIMSD_ERR_UNSUPPORTED).
  */
 int simsd_paged_attention_window(const void* q, const void* k_cache, const void* v_cache, int num_pages, int page_size,
                                  int64_t ld_page, int64_t ld_head, int64_t ld_tok, const int32_t* page_table,
@@ -573,7 +574,7 @@ int simsd_paged_attention_window(const void* q, const void* k_cache, const void*
  * them are left as they are.  Numbers that are not finite are stored as NaN.  A position past the page
  * table or cos / sin, or a page outside the cache, is flagged (SIMSD_DEV_ERR_BAD_INDEX): the
  * keys and values are not written, and q is zero for a position past the tables.  No page
- * is written by two sequences of a call.
+ * is written by two sequences of a call, and the caches' and scales' elements share no memory.
  */
 int simsd_paged_append8(const void* qkv, int64_t ldq_b, int64_t ldq_t, int B, int L, int Hq, int Hk, int head_dim,
                         int rotary_dim, const void* q_weight, const void* k_weight, float eps, const float* cos,
@@ -587,7 +588,7 @@ int simsd_paged_append8(const void* qkv, int64_t ldq_b, int64_t ldq_t, int B, in
  * simsd_paged_attention_window over that cache (window 0: none).  Any positive scales up to
  * 2^64 do, not only powers of two; sums are fp32 and weights fp16 (11 bits down to 2^-22 of
  * the largest).  The workspace as for simsd_paged_attention, of a size of its own; + 4 in the
- * place of + 3 in the limit there.
+ * place of + 3 in the limit there, and max_pages page_size <= 2^30.
  */
 size_t simsd_paged_attention8_workspace_size(int L, int Hq, int Hk, int head_dim);
 int simsd_paged_attention8(const void* q, const void* k_cache, const void* v_cache, const float* k_scale,
@@ -616,7 +617,8 @@ int simsd_paged_attention8(const void* q, const void* k_cache, const void* v_cac
  * other held ones go back onto the stack, sequence by sequence, each one's in its order; a stack
  * without room for them takes none of a sequence's (SIMSD_DEV_ERR_CAPACITY).
  * The workspace is SIMSD_PAGED_COUNTER_BYTES of counters, zero before the first call and after
- * every one (simsd_paged_attention's may be shared).
+ * every one (simsd_paged_attention's may be shared).  What is written is no input's memory, and
+ * calls on one pool are ordered.
  */
 int simsd_paged_reserve(int32_t* page_table, int64_t ld_table, int max_pages, const int32_t* lens, const int32_t* count,
                         int32_t* held, int32_t* free_pages, int pool_pages, int32_t* free_count, int B, int L,
@@ -634,10 +636,10 @@ int simsd_paged_release(const int32_t* page_table, int64_t ld_table, int max_pag
  *   - frequency[b] c - presence[b]                 where c > 0
  *   + the sum of bias_values[b, k] over bias_ids[b, k] = v
  *   -inf                                           where allowed[b, i] lacks v
- * one after the other in fp32, rounded once.  seen and allowed are bit lists of ceil(V / 32)
+ * in fp32, what is added summed first, rounded once.  seen and allowed are bit lists of ceil(V / 32)
  * words (token v: bit v % 32 of word v / 32; NULL: nothing seen, everything allowed).  Drafts
  * outside [0, V) count nowhere; bias ids below 0 are none, those from V on raise
- * SIMSD_DEV_ERR_BAD_INDEX.  dtype: all three.  B <= 65535 (more: SIMSD_ERR_UNSUPPORTED).
+ * SIMSD_DEV_ERR_BAD_INDEX.  dtype: all three.  out's rows share no memory.  B <= 65535 (more: SIMSD_ERR_UNSUPPORTED).
  *
  * simsd_count_tokens: counts[b, v] += how often v is among tokens[b, 0 .. N - 1]; negative
  * ones are none, those from V on raise SIMSD_DEV_ERR_BAD_INDEX.

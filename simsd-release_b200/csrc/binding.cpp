@@ -318,8 +318,9 @@ PyObject* append8(PyObject*, PyObject* const* args, Py_ssize_t n) {
   if (!r.good || code < 0 || !cache_good(*k, *v, at::kFloat8_e4m3fn) || heads < 1 || heads > 65536 || kv_heads != k->size(1) ||
       !scales_good(*k, *ks, *vs))
     return none();
+  if (qkv->dim() != 3) return none();
   const int64_t D = k->size(3), B = qkv->size(0);
-  if (qkv->dim() != 3 || qkv->size(2) != (heads + 2 * kv_heads) * D || qkv->stride(2) != 1) return none();
+  if (qkv->size(2) != (heads + 2 * kv_heads) * D || qkv->stride(2) != 1) return none();
   const int64_t L = qkv->size(1);
   if (B > INT_MAX || L > INT_MAX || table->dim() != 2 || table->size(0) != B || table->stride(1) != 1 ||
       table->size(1) > INT_MAX || !is_shape(*lens, {B}) || !lens->is_contiguous() || cos->dim() != 2 ||

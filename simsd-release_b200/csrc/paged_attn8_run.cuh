@@ -23,7 +23,7 @@ int attend8_tc(PagedAttn8Args& a, const PagedPlan& pl, void* stream) {
   constexpr int smem = P8tShape<D, R>::BYTES;
   const int rc = allow_smem(paged_attention8_tc_kernel<D, R, BF>, smem, done);
   if (rc != SIMSD_OK) return rc;
-  if (a.a.window == 0) a.a.window = 0x40000000, a.a.sinks = 0;       // this form has a window always
+  if (a.a.window == 0) a.a.window = PAGED_WINDOW_MAX, a.a.sinks = 0;       // this form has a window always
   return launch_on(paged_attention8_tc_kernel<D, R, BF>, dim3((unsigned)pl.grid), P8T_THREADS, smem, stream, false, a);
 }
 template <int D, bool BF>

@@ -3,7 +3,7 @@
 // free_count of them free, taken from the top.
 //
 // Reserve.  Sequence b has n = lens[b] tokens in h = max(held[b], ceil(n / ps)) pages
-// and is to get c = count[b] (0 .. L) more: t = max(0, ceil((n + c) / ps) - h) pages.
+// (held[b] where the row has not so many) and is to get c = count[b] (0 .. L) more: t = max(0, ceil((n + c) / ps) - h) pages.
 //   T_b = t_0 + .. + t_b;   b is served where t = 0 or T_b <= free_count
 // (from the first one that the stack does not reach on, only those that need no page).
 // Its i-th new page is free_pages[free_count - 1 - (T_b - t) - i].  Row b of slots and
@@ -116,7 +116,8 @@ __global__ void __launch_bounds__(PT_THREADS) paged_reserve_kernel(const PagedRe
       w.len = max(n, 0);
       w.fresh = max(0, min(c, p.L));
       const int mine = (w.len + (long long)p.page_size - 1) / p.page_size;
-      w.have = max(max(0, min(p.held[b], p.max_pages)), mine);
+      const int held = max(0, min(p.held[b], p.max_pages));
+      w.have = mine > p.max_pages ? held : max(held, mine);       // tokens past the row: no pages that it has
       const long long need = ((long long)w.len + w.fresh + p.page_size - 1) / p.page_size;
       bad = n < 0;
       short_of = need > p.max_pages;

@@ -53,6 +53,9 @@ int simsd_paged_append8(const void* qkv, int64_t ldq_b, int64_t ldq_t, int B, in
     return SIMSD_ERR_ALIGN;
   const int rc = cache8_check(k_cache, v_cache, ld_page, ld_head, ld_tok, page_size, block);
   if (rc != SIMSD_OK) return rc;
+  if (!rows_apart(head_dim, {{ld_page, num_pages}, {ld_head, Hk}, {ld_tok, page_size}}) ||
+      !rows_apart(1, {{lds_page, num_pages}, {lds_head, Hk}, {lds_block, page_size / block}}))
+    return SIMSD_ERR_SHAPE;
   PagedAppend8Args a;
   a.qkv = qkv;
   a.qw = q_weight;
@@ -122,6 +125,7 @@ int simsd_paged_attention8(const void* q, const void* k_cache, const void* v_cac
                               ldm_b, ldm_t, B, L, Hq, Hk, head_dim, scale, window, sinks, o, lse, dtype, err_word);
   if (rc != SIMSD_OK || B == 0 || L == 0) return rc;
   if (!k_scale || !v_scale) return SIMSD_ERR_SHAPE;
+  if ((int64_t)max_pages * page_size > PAGED_WINDOW_MAX) return SIMSD_ERR_UNSUPPORTED;
   rc = cache8_check(k_cache, v_cache, ld_page, ld_head, ld_tok, page_size, block);
   if (rc != SIMSD_OK) return rc;
   a.ld_page = ld_page;

@@ -65,6 +65,21 @@ int allow_smem(F* kern, int bytes, bool* done) {
   return SIMSD_OK;
 }
 
+// Whether no two elements of a tensor that is written meet: rows of `row` elements along
+// dimensions of (stride, size), each one reaching past all of the smaller strides together.
+inline bool rows_apart(int64_t row, std::initializer_list<std::pair<int64_t, int64_t>> dims) {
+  std::pair<int64_t, int64_t> d[4];
+  int n = 0;
+  for (const auto& x : dims)
+    if (x.second > 1) d[n++] = x;
+  std::sort(d, d + n);
+  for (int i = 0; i < n; ++i) {
+    if (d[i].first < row) return false;
+    row += (d[i].second - 1) * d[i].first;
+  }
+  return true;
+}
+
 // How paged attention runs the G L rows of a KV head: `nr` rows a CTA, the grid, and the
 // workspace: the arrival counters, then two parts per CTA (the end of a sequence
 // it started inside, the start of one it leaves unfinished).
@@ -88,6 +103,10 @@ inline PagedPlan paged_plan8(long long rows, int D) {
   return paged_plan_of(rows <= 32 ? 32 : rows <= 64 ? 64 : 128, 1, D);
 }
 
+// The longest sequence, and the largest window, where there is one (or the form always has one):
+// a position less a window, or plus some tokens, stays in 32 bits.
+constexpr int PAGED_WINDOW_MAX = 0x40000000;
+
 // A request of paged attention, the sizes that every form of it refuses, and its arguments
 // but for what goes by the form: the caches' strides and the plan's part.
 inline int paged_attn_request(PagedAttnArgs& a, const void* q, const void* k_cache, const void* v_cache, int num_pages,
@@ -99,7 +118,7 @@ inline int paged_attn_request(PagedAttnArgs& a, const void* q, const void* k_cac
   if (dtype != SIMSD_BF16 && dtype != SIMSD_F16) return SIMSD_ERR_DTYPE;
   if (head_dim != 64 && head_dim != 128) return SIMSD_ERR_UNSUPPORTED;
   if (B == 0 || L == 0) return SIMSD_OK;
-  if ((int64_t)max_pages * page_size > 0x7fff0000LL) return SIMSD_ERR_UNSUPPORTED;
+  if ((int64_t)max_pages * page_size > (window > 0 ? PAGED_WINDOW_MAX : 0x7fff0000LL)) return SIMSD_ERR_UNSUPPORTED;
   if (!q || !k_cache || !v_cache || (max_pages > 0 && !page_table) || !seq_lens || !o || ld_table < 0)
     return SIMSD_ERR_SHAPE;
   if (!al16(q) || !al16(o)) return SIMSD_ERR_ALIGN;
@@ -126,8 +145,8 @@ inline int paged_attn_request(PagedAttnArgs& a, const void* q, const void* k_cac
   a.page_div = paged_div(page_size);
   a.g_div = paged_div(a.G);
   // more than any length of either counts as that
-  a.window = std::min(window, 0x40000000);
-  a.sinks = std::min(sinks, 0x40000000);
+  a.window = std::min(window, PAGED_WINDOW_MAX);
+  a.sinks = std::min(sinks, PAGED_WINDOW_MAX);
   a.q_sign = scale < 0.0f ? 0x80008000u : 0u;
   a.scale_log2 = std::max(std::fabs(scale) * 1.4426950408889634f, 1e-30f);
   a.rows = a.G * L;

@@ -31,9 +31,10 @@ int simsd_paged_reserve(int32_t* page_table, int64_t ld_table, int max_pages, co
   if (B < 0 || L < 0 || page_size < 1 || max_pages < 0 || pool_pages < 0 || ld_table < 0) return SIMSD_ERR_SHAPE;
   if (B == 0) return SIMSD_OK;
   if (!lens || !held || !free_count || !total || (max_pages > 0 && !page_table) || (pool_pages > 0 && !free_pages) ||
-      (L > 0 && (!slots || !positions)))
+      (L > 0 && (!slots || !positions)) || !rows_apart(max_pages, {{ld_table, B}}))
     return SIMSD_ERR_SHAPE;
-  if ((int64_t)max_pages * page_size > 0x7fff0000LL || (int64_t)L * PT_THREADS > 0x7fff0000LL) return SIMSD_ERR_UNSUPPORTED;
+  // places of a block of sequences, and a grid's more, in 32 bits
+  if ((int64_t)max_pages * page_size > 0x7fff0000LL || (int64_t)L * PT_THREADS > 0x7f000000LL) return SIMSD_ERR_UNSUPPORTED;
   if (workspace == nullptr || workspace_bytes < SIMSD_PAGED_COUNTER_BYTES) return SIMSD_ERR_WORKSPACE;
   PagedReserveArgs a;
   a.table = page_table;
@@ -94,7 +95,8 @@ int simsd_adjust_logits(const void* logits, int64_t ld_b, int64_t ld_r, void* ou
   if (dtype != SIMSD_BF16 && dtype != SIMSD_F16 && dtype != SIMSD_F32) return SIMSD_ERR_DTYPE;
   if (B > 65535 || V > 0x7fff0000) return SIMSD_ERR_UNSUPPORTED;
   if (B == 0 || R == 0) return SIMSD_OK;
-  if (!logits || !out || (n_bias > 0 && (!bias_ids || !bias_values))) return SIMSD_ERR_SHAPE;
+  if (!logits || !out || (n_bias > 0 && (!bias_ids || !bias_values)) || !rows_apart(V, {{ldo_b, B}, {ldo_r, R}}))
+    return SIMSD_ERR_SHAPE;
   LogitRulesArgs a;
   a.logits = logits;
   a.out = out;
@@ -138,7 +140,7 @@ int simsd_count_tokens(int32_t* counts, int64_t ld_counts, const int64_t* tokens
                        int* err_word, void* stream) {
   if (B < 0 || N < 0 || V < 1) return SIMSD_ERR_SHAPE;
   if (B == 0 || N == 0) return SIMSD_OK;
-  if (!counts || !tokens) return SIMSD_ERR_SHAPE;
+  if (!counts || !tokens || !rows_apart(V, {{ld_counts, B}})) return SIMSD_ERR_SHAPE;
   const int grid = (int)std::min<long long>(cdiv((long long)B * N, 256), 8LL * sm_count());
   return launch_on(count_tokens_kernel, dim3((unsigned)grid), 256, 0, stream, false, counts, ld_counts,
                    reinterpret_cast<const long long*>(tokens), ld_tokens, B, N, V, err_word);

@@ -13,7 +13,7 @@ from __future__ import annotations
 import torch
 
 from . import _lib
-from .paged_cache import _current_device, _current_stream
+from .paged_cache import _check_apart, _current_device, _current_stream
 
 
 def token_bits(tokens: torch.Tensor, vocab: int) -> torch.Tensor:
@@ -32,6 +32,8 @@ def _check_rules(logits, counts, drafts, repetition, presence, frequency, seen, 
     if logits.ndim != 3 or logits.shape[2] < 1:
         raise ValueError(f"logits must be [B, R, V], got {tuple(logits.shape)}")
     B, R, V = logits.shape
+    if max(R, V) > 0x7fff0000:
+        raise ValueError(f"adjust_logits: at most {0x7fff0000} rows and tokens, got {tuple(logits.shape)}")
     W = -(-V // 32)
     for name, t in (("repetition", repetition), ("presence", presence), ("frequency", frequency)):
         if t is not None:
@@ -65,6 +67,7 @@ def _check_rules(logits, counts, drafts, repetition, presence, frequency, seen, 
             raise TypeError(f"dtype mismatch: logits {logits.dtype} out {out.dtype}")
         if out.shape != logits.shape or (V > 1 and out.stride(2) != 1):
             raise ValueError(f"out must be {tuple(logits.shape)} with a unit last stride")
+        _check_apart("adjust_logits", out=out)
     _lib.require_cuda(logits, counts, drafts, repetition, presence, frequency, seen, bias_ids, bias_values, allowed, out)
 
 
@@ -74,8 +77,8 @@ def adjust_logits(logits: torch.Tensor, counts: torch.Tensor | None = None, draf
                   bias_ids: torch.Tensor | None = None, bias_values: torch.Tensor | None = None,
                   allowed: torch.Tensor | None = None, out: torch.Tensor | None = None) -> torch.Tensor:
     """logits [B, R, V] (bf16, fp16 or fp32) with the rules applied; row i of a sequence follows
-    i drafted tokens (R = K + 1, as `speculative_verify` takes them).  For token v, one after
-    the other in fp32, rounded once:
+    i drafted tokens (R = K + 1, as `speculative_verify` takes them).  For token v, in fp32
+    (what is added summed first), rounded once:
 
     * repetition [B] fp32 (positive): a logit over 0 is divided by it, another one multiplied,
       where v was answered, drafted before row i, or stands in the prompt;
@@ -134,6 +137,7 @@ def count_tokens(counts: torch.Tensor, tokens: torch.Tensor) -> None:
         raise ValueError(f"counts must be [B, V] and tokens [B, N], got {tuple(counts.shape)} / {tuple(tokens.shape)}")
     if counts.shape[1] > 1 and counts.stride(1) != 1:
         raise ValueError("counts, which are written in place, must have a unit last stride")
+    _check_apart("count_tokens", counts=counts)
     _lib.require_cuda(counts, tokens)
     dev = counts.get_device()
     if _current_device() != dev:

@@ -66,6 +66,16 @@ def _check_scales(what: str, k_cache, k_scale, v_scale) -> None:
         raise ValueError(f"{what}: k_scale and v_scale must have the same strides")
 
 
+def _check_apart(what: str, **written: torch.Tensor) -> None:
+    """Raise where two elements of a tensor that is written may be the same memory."""
+    for name, t in written.items():
+        reach = 1
+        for stride, n in sorted((s, n) for s, n in zip(t.stride(), t.shape) if n > 1):
+            if stride < reach and t.numel():
+                raise ValueError(f"{what}: {name}, which is written, has elements that share memory (strides {t.stride()})")
+            reach += (n - 1) * stride
+
+
 def _mask_strides(tail_mask: torch.Tensor | None):
     """(tail_mask with a unit last stride, its strides of a sequence and of a query)."""
     if tail_mask is None:

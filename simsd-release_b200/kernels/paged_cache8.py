@@ -23,8 +23,8 @@ from __future__ import annotations
 import torch
 
 from . import _lib
-from .paged_cache import (_HALF, _check_attention, _check_cache, _check_scales, _current_device, _current_stream, _mask_strides, _on_16_bytes,
-                          _window)
+from .paged_cache import (_HALF, _check_apart, _check_attention, _check_cache, _check_scales, _current_device, _current_stream,
+                          _mask_strides, _on_16_bytes, _window)
 
 F8 = torch.float8_e4m3fn
 
@@ -45,6 +45,7 @@ def _check_append8(qkv, heads, kv_heads, k_cache, v_cache, k_scale, v_scale, pag
         raise TypeError(f"paged_append8 takes bf16 or fp16 activations, got {qkv.dtype}")
     _check_cache("paged_append8", k_cache, v_cache, kv_heads, F8)
     _check_scales("paged_append8", k_cache, k_scale, v_scale)
+    _check_apart("paged_append8", k_cache=k_cache, k_scale=k_scale)
     D = k_cache.shape[3]
     if qkv.ndim not in (2, 3) or heads < 1 or kv_heads < 1 or qkv.shape[-1] != (heads + 2 * kv_heads) * D:
         raise ValueError(f"qkv must be [B, L, {(heads + 2 * kv_heads) * D}] or [B, ..], got {tuple(qkv.shape)}")

@@ -18,7 +18,7 @@ from __future__ import annotations
 import torch
 
 from . import _lib
-from .paged_cache import _current_device, _current_stream
+from .paged_cache import _check_apart, _current_device, _current_stream
 
 
 def page_pool(sequences: int, max_pages: int, pages: int, device=None):
@@ -39,12 +39,13 @@ def _check_state(what: str, page_table, free_pages, free_count, page_size, **row
     for name, t in rows.items():
         if t is not None and t.shape != (B,):
             raise ValueError(f"{what}: {name} must be [{B}], got {tuple(t.shape)}")
-    if page_size < 1:
-        raise ValueError(f"{what}: page_size must be at least 1")
+    if not 1 <= page_size <= 0x7fffffff:
+        raise ValueError(f"{what}: page_size must be at least 1 and below 2^31, got {page_size}")
     written = {"page_table": page_table, "free_pages": free_pages, "held": rows["held"]}
     for name, t in written.items():
         if t.numel() > 1 and t.stride(-1) != 1:
             raise ValueError(f"{what}: {name}, which is written in place, must have a unit last stride")
+    _check_apart(what, **written)
     _lib.require_cuda(*given)
 
 
@@ -67,8 +68,8 @@ def paged_reserve(page_table: torch.Tensor, lens: torch.Tensor, held: torch.Tens
     out = _lib.binding().paged_reserve(page_table, lens, held, free_pages, free_count, L, page_size, count)
     if out is not None:
         return out
-    if L < 0:
-        raise ValueError(f"paged_reserve: L must not be negative, got {L}")
+    if not 0 <= L <= 0x7fffffff:
+        raise ValueError(f"paged_reserve: L must be at least 0 and below 2^31, got {L}")
     _check_state("paged_reserve", page_table, free_pages, free_count, page_size, lens=lens, held=held, count=count)
     dev = page_table.get_device()
     if _current_device() != dev:

@@ -233,3 +233,27 @@ def test_streams_and_graphs():
             want = adjust_logits(x, **k)
             graph.replay()
             assert torch.equal(held, want)
+
+
+@pytest.mark.parametrize("B,R,V,dtype,kw", [(1, 300, 2056, BF, {}), (2, 520, 37, FL, dict(bias=3)), (2, 3, 4096, FP, dict(bias=1500)),
+                                            (1, 2, 50, FL, dict(bias=2100))])
+def test_many_drafts_and_long_bias_lists(B, R, V, dtype, kw):
+    g = gen(B + R + V)
+    x = (torch.randn(B, R, V, generator=g, device=DEV) * 3).to(dtype)
+    rules = rules_of(g, B, R, V, **kw)
+    with torch.inference_mode():
+        check(adjust_logits(x, **rules), x, rules["bias_ids"].shape[1], **rules)
+
+
+def test_rows_in_another_order_and_the_same_row_for_all():
+    g = gen(5)
+    B, R, V = 3, 4, 2048
+    rules = rules_of(g, B, R, V)
+    with torch.inference_mode():
+        x = torch.randn(1, R, V, generator=g, device=DEV).to(BF).expand(B, R, V)
+        y = adjust_logits(x.contiguous(), **rules)
+        assert torch.equal(adjust_logits(x, **rules), y)
+        turned = torch.empty(R, B, V, dtype=BF, device=DEV).transpose(0, 1)
+        assert adjust_logits(x, **rules, out=turned) is turned and torch.equal(turned, y)
+        with pytest.raises(ValueError, match="share memory"):
+            adjust_logits(x.contiguous(), **rules, out=x)

@@ -658,3 +658,26 @@ def test_inputs_at_odd_addresses_and_strides():
             q.copy_(want)
             assert torch.equal(paged_attention8(q, c[0], c[2], ks, vs, wide[:, ::2], ints([50, 0, 20, 0])[::2]), ref)
     assert _lib.device_error() == 0
+
+
+@pytest.mark.parametrize("L", [1, 8])
+@pytest.mark.parametrize("window", [None, 60])
+def test_one_scale_for_all_and_pages_that_sequences_share(L, window):
+    """Scales of stride 0; a prefix's pages in several rows, and one page many times in a row."""
+    g = gen(L)
+    k, _ = cache_of(g, 9, 2, 16, 64, 16, "hnd", BF)
+    v, _ = cache_of(g, 9, 2, 16, 64, 16, "hnd", BF)
+    one, two = (torch.full((1, 1, 1), s, device=DEV).expand(9, 2, 1) for s in (0.125, 0.5))
+    table = ints([[0, 1, 2, 3, 4, 5], [0, 1, 2, 6, 7, 8], [3, 3, 3, 3, 3, 3]])
+    lens = [95, 81, 96]
+    q = randn(g, 3, L, 8, 64, dtype=BF)
+    with torch.inference_mode():
+        o, lse = paged_attention8(q, k, v, one, two, table, ints(lens), return_lse=True, window=window, sinks=3)
+        apart = [table[b].long() for b in range(3)]
+        k2, v2 = (torch.cat([c.view(torch.uint8)[t] for t in apart]).view(F8) for c in (k, v))
+        own = torch.arange(18, dtype=torch.int32, device=DEV).view(3, 6)
+        o2, lse2 = paged_attention8(q, k2, v2, one[:1].expand(18, 2, 1).contiguous(), two[:1].expand(18, 2, 1).contiguous(), own,
+                                    ints(lens), return_lse=True, window=window, sinks=3)
+    assert torch.equal(o, o2) and torch.equal(lse, lse2)
+    check_attention(q, values(k, one), values(v, two), spread_scales(two, 16), table, lens, 64 ** -0.5, None, o, lse, window, 3)
+    assert _lib.device_error() == 0

@@ -200,3 +200,14 @@ def test_nothing():
     slots, _, total = paged_reserve(table, ints([0, 0]), held, free, count, 2, 16)
     assert bool((slots == -1).all()) and total.tolist() == [0, 0]
     assert errors() == (True, False)
+
+
+def test_a_length_past_its_row_takes_and_keeps_nothing():
+    """Two pages of 16 a row: 40 tokens are not in the row, and what it holds stays its own."""
+    table, held, free, count = ints([[5, -1], [6, 7]]), ints([1, 2]), ints([0, 1, 2, 3, 4, -1, -1, -1]), ints([5])
+    slots, positions, total = paged_reserve(table, ints([40, 20]), held, free, count, 3, 16)
+    assert slots.tolist() == [[-1] * 3, [7 * 16 + 4 + i for i in range(3)]] and total.tolist() == [40, 23]
+    assert held.tolist() == [1, 2] and count.tolist() == [5] and errors() == (True, False)
+    paged_release(table, held, free, count, ints([0, 0]), 16)
+    assert held.tolist() == [0, 0] and free.tolist() == [0, 1, 2, 3, 4, 5, 6, 7] and count.tolist() == [8]
+    assert errors() == (False, False)

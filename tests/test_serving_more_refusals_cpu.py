@@ -185,6 +185,63 @@ def test_c_entry_points_refuse():
     assert L.simsd_count_tokens(p, 8, p, 1, 1, 0, 8, None, None) == _lib.SIMSD_OK
 
 
+def test_written_tensors_whose_elements_share_memory_are_refused():
+    shared = torch.zeros(4, 1, 1).expand(4, 2, 1)
+    with pytest.raises(ValueError, match="share memory"):
+        paged_append8(**{**append_args(), "k_scale": shared, "v_scale": shared})
+    wide = torch.zeros(1, 2, 16, 64).to(F8).expand(4, 2, 16, 64)
+    with pytest.raises(ValueError, match="share memory"):
+        paged_append8(**{**append_args(), "k_cache": wide, "v_cache": wide})
+    with pytest.raises(ValueError, match="share memory"):
+        paged_reserve(**{**reserve_args(), "page_table": ints(1, 4).expand(3, 4)})
+    with pytest.raises(ValueError, match="share memory"):
+        adjust_logits(torch.zeros(2, 3, 40), out=torch.zeros(2, 1, 40).expand(2, 3, 40))
+    with pytest.raises(ValueError, match="share memory"):
+        count_tokens(ints(1, 5).expand(2, 5), ints(2, 3).long())
+    # rows in another order, rows with room between them and heads of a wider tensor are fine
+    for out in (torch.zeros(3, 2, 40).transpose(0, 1), torch.zeros(2, 6, 48)[:, ::2, :40]):
+        with pytest.raises(RuntimeError):                          # no CUDA tensors
+            adjust_logits(torch.zeros(2, 3, 40), out=out)
+
+
+def test_c_entry_points_refuse_shared_memory_and_lengths_past_30_bits():
+    L = _lib.lib()
+    buf = ctypes.create_string_buffer(64)
+    p = (ctypes.addressof(buf) + 15) & ~15
+    S, U = _lib.SIMSD_ERR_SHAPE, _lib.SIMSD_ERR_UNSUPPORTED
+
+    def append(strides=(2048, 1024, 64), scales=(2, 1, 1)):
+        return L.simsd_paged_append8(p, 512, 512, 1, 1, 4, 2, 64, 64, None, None, 1e-6, p, p, 32, p, 2, 2, p, None, p, p, p, p, p, 4, 16,
+                                     16, *strides, *scales, 0, None, None)
+    for strides in ((2048, 0, 64), (0, 1024, 64), (2048, 1024, 48), (1024, 1024, 64), (1984, 1024, 64)):
+        assert append(strides=strides) == S
+    assert append(scales=(1, 1, 1)) == append(scales=(0, 1, 1)) == append(scales=(2, 0, 1)) == S
+
+    def attend(f, pages, window):
+        cache = (p, p, p, p, 4, 16, 16, 2048, 1024, 64, 2, 1, 1) if f is L.simsd_paged_attention8 else (p, p, 4, 16, 2048, 1024, 64)
+        return f(p, *cache, p, pages, pages, p, None, 0, 0, 1, 1, 4, 2, 64, 0.125, window, 0, p, None, 0, p, 0, None, None)
+    over, fits = (1 << 26) + 1, 1 << 26                            # pages of 16: 2^30 tokens
+    assert attend(L.simsd_paged_attention8, over, 0) == attend(L.simsd_paged_attention8, over, 5) == U
+    assert attend(L.simsd_paged_attention_window, over, 5) == U
+    for f, pages, window in ((L.simsd_paged_attention8, fits, 0), (L.simsd_paged_attention_window, fits, 5),
+                             (L.simsd_paged_attention_window, over, 0)):
+        assert attend(f, pages, window) == _lib.SIMSD_ERR_WORKSPACE
+    rows = lambda ld: L.simsd_paged_reserve(p, ld, 4, p, None, p, p, 4, p, 2, 1, 16, p, p, p, p, 0, None, None)  # noqa: E731
+    assert rows(3) == S and rows(4) == _lib.SIMSD_ERR_WORKSPACE
+    out = lambda b, r: L.simsd_adjust_logits(p, 8, 8, p, b, r, 2, 2, 8, 0, *[None, 0] * 3, None, None, None, *[None, 0] * 2, 0, None, 0, 0,  # noqa: E731
+                                             None, None)
+    assert out(8, 8) == out(16, 0) == out(8, 7) == S
+    assert L.simsd_count_tokens(p, 7, p, 1, 2, 1, 8, None, None) == S
+
+
+def test_numbers_past_32_bits_are_refused():
+    for change in (dict(L=1 << 31), dict(page_size=1 << 31)):
+        with pytest.raises(ValueError, match="2\\^31"):
+            paged_reserve(**{**reserve_args(), **change})
+    with pytest.raises(ValueError):
+        paged_append8(**{**append_args(), "qkv": torch.zeros((), dtype=BF)})
+
+
 @pytest.mark.parametrize("name", ["simsd_paged_attention_window", "simsd_paged_attention8", "simsd_paged_reserve", "simsd_paged_release"])
 def test_calls_that_share_scratch_hold_the_gil(name):
     fn = getattr(_lib.lib(), name)
