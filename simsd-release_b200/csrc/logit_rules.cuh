@@ -9,12 +9,20 @@
 // in fp32 (x times a factor plus one number, the division as a product with the reciprocal),
 // rounded once to the logits' type.
 //
-// HBM bounds it: every logit read and written once.  A CTA takes 2048 tokens of one
-// sequence through all its rows, so that counts, the prompt's bits and the biases are
-// read once a sequence; what stays of them in registers is a number to add and a bit for each token.
-// After row i the thread that owns drafted token i counts it.  Several rows are on their way at a time.
-// Its threads look through the bias list, an entry each, for those on the CTA's tokens.
+// HBM bounds it: every logit read and written once.  A warp takes 256 tokens of one sequence
+// through all its rows, so that counts, the prompt's bits and the biases are read once a sequence; what
+// stays of them in registers is two factors and a number to add for each token.  Several rows are on
+// their way at a time.  After row i the lane that owns drafted token i counts it.  Each warp looks through
+// the bias list itself, an entry a lane, and needs no barrier.
+//
+// Measured (B200, device time in a graph of calls; bf16, 151936 tokens, counts, prompt bits, 300 biases and a mask a
+// row): 64 x 8 rows 83.6 us, 4.3 TB/s (66 % of the bytes' time at the copy rate), without biases 73.5, with no
+// rule at all 52 (91 %); 64 x 1 row 35.  A CTA for 2048 tokens with the biases and drafts in shared memory took
+// 117, 101, 61 and 45: some 100 instructions a warp's row instead of 150, and no waits for the CTA.  What is left is the
+// setup, 570 instructions a warp and its loads' latency, at 60 % of the issue slots.  Rows whose 8 tokens do not lie
+// on 16 bytes take 2.8 times their bytes' time (64 x 4 x 151937: 86 us), 2-byte loads and stores.
 #pragma once
+#include "paged.cuh"
 #include "spec_verify.cuh"
 
 namespace simsd {
@@ -37,97 +45,99 @@ struct LogitRulesArgs {
   bool penal;               // one of the penalties is there
 };
 
-constexpr int LR_THREADS = 256, LR_EACH = 8, LR_TOKENS = LR_THREADS * LR_EACH, LR_LIST = 1024;
+constexpr int LR_THREADS = 128, LR_EACH = 8, LR_TOKENS = 32 * LR_EACH;   // tokens of a warp
+constexpr int LR_CTAS = 8;                        // CTAs that an SM holds; 9, with spills: 90 us at 64 x 8, not 84
 
-// VEC: a thread owns 8 tokens in a row (16-byte loads and stores), else 8 tokens 32
-// apart, a warp's next to each other (rows that start anywhere).
-template <int DT, bool VEC>
-__global__ void __launch_bounds__(LR_THREADS, 4) logit_rules_kernel(const LogitRulesArgs p) {
+// VEC: a lane owns 8 tokens in a row (16-byte loads and stores), else 8 tokens 32 apart, a warp's next to
+// each other (rows that start anywhere).  PENAL: one of the penalties is there.
+template <int DT, bool VEC, bool PENAL>
+__global__ void __launch_bounds__(LR_THREADS, LR_CTAS) logit_rules_kernel(const LogitRulesArgs p) {
   griddep_launch_dependents();
   griddep_wait();
   constexpr int VECS = DT == 2 ? 2 : 1;           // 16-byte loads of 8 logits
-  constexpr int ROWS = VEC && DT != 2 ? 4 : 2;    // rows in registers
+  // rows in registers: with penalties 4 take 98 us at 64 x 8 at best where 2 took 89.5; without, 52 and 54
+  constexpr int ROWS = VEC && DT != 2 && !PENAL ? 4 : 2;
   constexpr int SIZE = DT == 2 ? 4 : 2;
-  __shared__ int s_draft[LR_THREADS], s_hit[LR_LIST], s_order[LR_LIST], s_hits;
-  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, b = blockIdx.y;
-  const int v0 = blockIdx.x * LR_TOKENS, w0 = v0 + warp * 32 * LR_EACH;
-  const int first = VEC ? w0 + lane * LR_EACH : w0 + lane;   // the thread's tokens: first + k step
   constexpr int step = VEC ? 1 : 32;
-  // the thread's place for a token of the CTA (0 .. LR_TOKENS - 1), or -1
-  auto mine = [&](int at) {
-    if (VEC) return at / LR_EACH == tid ? at % LR_EACH : -1;
-    return at / (32 * LR_EACH) == warp && at % 32 == lane ? at / 32 % LR_EACH : -1;
-  };
-  // 8 bits of a word list, the thread's tokens'
+  const int lane = threadIdx.x & 31, b = blockIdx.y;
+  const int w0 = (blockIdx.x * (LR_THREADS / 32) + (threadIdx.x >> 5)) * LR_TOKENS;
+  if (w0 >= p.V) return;
+  const int first = VEC ? w0 + lane * LR_EACH : w0 + lane;   // the lane's tokens: first + k step
+  const bool in = first < p.V;
+  // who owns token w0 + at, and as which of its own
+  auto owner = [](int at) { return VEC ? at / LR_EACH : at % 32; };
+  auto place = [](int at) { return VEC ? at % LR_EACH : at / 32; };
+  // 8 bits of a word list, the lane's tokens'
   auto bits = [&](const uint32_t* w) {
+    if (VEC) return w[first / 32] >> first % 32 & 0xffu;
     const int words = (p.V + 31) / 32;
-    if (VEC) return first < p.V ? w[first / 32] >> first % 32 & 0xffu : 0u;
     uint32_t m = 0;
 #pragma unroll
     for (int k = 0; k < LR_EACH; ++k) {
-      const int at = first / 32 + k;
+      const int at = w0 / 32 + k;
       m |= (at < words ? w[at] >> lane & 1u : 0u) << k;
     }
     return m;
   };
 
-  // rows that are on their way; the next one's places
+  // rows that are on their way
   uint4 raw[VEC ? ROWS : 1][VECS];
   float val[VEC ? 1 : ROWS][LR_EACH];
   uint32_t ok[ROWS];
   const char* src = static_cast<const char*>(p.logits) + (b * p.ld_b + first) * SIZE;
   const uint32_t* mask = p.allowed ? p.allowed + b * p.lda_b : nullptr;
-  int fetched = 0;
-  auto fetch = [&](int at) {
+  auto fetch = [&](int at, int row) {
     ok[at] = 0xffu;
-    if (fetched >= p.R) return;
-    if constexpr (VEC) {
-      if (first < p.V) {
+    if (in && row < p.R) {
+      if constexpr (VEC) {
 #pragma unroll
         for (int x = 0; x < VECS; ++x) raw[at][x] = reinterpret_cast<const uint4*>(src)[x];
-      }
-    } else {
+      } else {
 #pragma unroll
-      for (int k = 0; k < LR_EACH; ++k)
-        if (first + k * step < p.V) val[at][k] = load_f(src, k * step, DT);
+        for (int k = 0; k < LR_EACH; ++k)
+          if (first + k * step < p.V) val[at][k] = load_f(src, k * step, DT);
+      }
+      if (mask) ok[at] = bits(mask);
     }
-    if (mask) ok[at] = bits(mask), mask += p.lda_r;
     src += p.ld_r * SIZE;
-    ++fetched;
+    if (mask) mask += p.lda_r;
   };
 #pragma unroll
-  for (int x = 0; x < ROWS; ++x) fetch(x);
+  for (int x = 0; x < ROWS; ++x) fetch(x, x);
 
   // what the sequence has, all of it sent for before any is waited for
   float rep = 1.0f, pres = 0.0f, freq = 0.0f;
   uint32_t again = 0;                             // tokens that the repetition penalty holds for
-  const int* counts = p.counts ? p.counts + b * p.ld_c + first : nullptr;
+  const int* counts = PENAL && p.counts ? p.counts + b * p.ld_c + first : nullptr;
+  const long long* drafts = PENAL && p.drafts ? p.drafts + b * p.ld_d : nullptr;
   int c[LR_EACH];
 #pragma unroll
   for (int k = 0; k < LR_EACH; ++k) c[k] = 0;
-  if (p.penal) {
-    if (counts) {
+  int d = -1;                                     // drafted token of row 32 i + lane, where it is the warp's
+  uint32_t drafted = 0;                           // the rows that have one
+  auto draft_of = [&](int row) { return drafts && row + lane + 1 < p.R ? drafts[row + lane] : -1; };
+  auto stage_drafts = [&](long long v) {
+    d = v >= w0 && v < min((long long)w0 + LR_TOKENS, (long long)p.V) ? (int)(v - w0) : -1;
+    drafted = __ballot_sync(0xffffffffu, d >= 0);
+  };
+  long long draft = -1;
+  if constexpr (PENAL) {
+    draft = draft_of(0);
+    if (counts && in) {
       if (VEC) {
-        if (first < p.V) {
-          const int4 a = reinterpret_cast<const int4*>(counts)[0], d = reinterpret_cast<const int4*>(counts)[1];
-          c[0] = a.x, c[1] = a.y, c[2] = a.z, c[3] = a.w, c[4] = d.x, c[5] = d.y, c[6] = d.z, c[7] = d.w;
-        }
+        const int4 x = reinterpret_cast<const int4*>(counts)[0], y = reinterpret_cast<const int4*>(counts)[1];
+        c[0] = x.x, c[1] = x.y, c[2] = x.z, c[3] = x.w, c[4] = y.x, c[5] = y.y, c[6] = y.z, c[7] = y.w;
       } else {
 #pragma unroll
         for (int k = 0; k < LR_EACH; ++k)
           if (first + k * step < p.V) c[k] = counts[k * step];
       }
     }
-    if (p.seen) again = bits(p.seen + b * p.ld_s);
+    if (p.seen && in) again = bits(p.seen + b * p.ld_s);
     if (p.repetition) rep = p.repetition[b];
     if (p.presence) pres = p.presence[b];
     if (p.frequency) freq = p.frequency[b];
   }
-  auto stage_drafts = [&](int i) {                // rows i on: their drafted tokens that are the CTA's
-    const long long v = p.drafts && i + tid + 1 < p.R ? p.drafts[b * p.ld_d + i + tid] : -1;
-    s_draft[tid] = v >= v0 && v < min(v0 + LR_TOKENS, p.V) ? (int)(v - v0) : -1;
-  };
-  if (p.penal) stage_drafts(0);
 
   // per token: what is added
   float add[LR_EACH];
@@ -135,36 +145,47 @@ __global__ void __launch_bounds__(LR_THREADS, 4) logit_rules_kernel(const LogitR
   for (int k = 0; k < LR_EACH; ++k) add[k] = 0.0f;
   const int* ids = p.bias_ids + b * p.ld_i;
   const float* values = p.bias + b * p.ld_v;
-  for (int base = 0; base < p.n_bias; base += LR_LIST) {
-    // the list's entries that are the CTA's, as (place in the list, token), in the list's order: found in any, then ranked
-    const int n = min(LR_LIST, p.n_bias - base);
-    if (tid == 0) s_hits = 0;
-    __syncthreads();
-    for (int x = tid; x < n; x += LR_THREADS) {
-      const int id = ids[base + x];
-      if (id >= p.V && blockIdx.x == 0 && p.err) atomicOr(p.err, SIMSD_DEV_ERR_BAD_INDEX);
-      if ((uint32_t)(id - v0) < (uint32_t)LR_TOKENS && id < p.V) s_hit[atomicAdd(&s_hits, 1)] = x * LR_TOKENS + id - v0;
-    }
-    __syncthreads();
-    const int hits = s_hits;
-    for (int x = tid; x < hits; x += LR_THREADS) {
-      int rank = 0;
-      for (int y = 0; y < hits; ++y) rank += s_hit[y] < s_hit[x];
-      s_order[rank] = s_hit[x];
-    }
-    __syncthreads();
-    for (int x = 0; x < hits; ++x) {
-      const int hit = s_order[x], k = mine(hit % LR_TOKENS);
-      if (k < 0) continue;
-      const float v = values[base + hit / LR_TOKENS];
+  // entries of a lane at a time; hardly ever is one of them the warp's
+  constexpr int LIST = 4;
+  const uint32_t mine = min(LR_TOKENS, p.V - w0);
+  for (int base = 0; base < p.n_bias; base += 32 * LIST) {
+    int id[LIST];
+    bool any = false;
 #pragma unroll
-      for (int y = 0; y < LR_EACH; ++y) add[y] += y == k ? v : 0.0f;
+    for (int q = 0; q < LIST; ++q) {
+      id[q] = base + q * 32 + lane < p.n_bias ? ids[base + q * 32 + lane] : -1;
+      any |= (uint32_t)id[q] - (uint32_t)w0 < mine;
+    }
+    if (w0 == 0 && p.err) {
+#pragma unroll
+      for (int q = 0; q < LIST; ++q)
+        if (id[q] >= p.V) atomicOr(p.err, SIMSD_DEV_ERR_BAD_INDEX);
+    }
+    if (!__any_sync(0xffffffffu, any)) continue;
+#pragma unroll
+    for (int q = 0; q < LIST; ++q) {
+      // in the list's order
+      uint32_t who = __ballot_sync(0xffffffffu, (uint32_t)id[q] - (uint32_t)w0 < mine);
+      for (; who != 0; who &= who - 1) {
+        const int from = __ffs(who) - 1, at = __shfl_sync(0xffffffffu, id[q], from) - w0;
+        const float v = owner(at) == lane ? values[base + q * 32 + from] : 0.0f;
+#pragma unroll
+        for (int k = 0; k < LR_EACH; ++k) add[k] += place(at) == k ? v : 0.0f;
+      }
     }
   }
   const float inv = 1.0f / rep;
+  float up[LR_EACH], down[LR_EACH];               // factors of a logit over 0 and of another one
+  if constexpr (PENAL) {
+    stage_drafts(draft);
+    if (c[0] | c[1] | c[2] | c[3] | c[4] | c[5] | c[6] | c[7]) {
 #pragma unroll
-  for (int k = 0; k < LR_EACH; ++k)
-    if (c[k] > 0) add[k] -= fmaf(freq, (float)c[k], pres), again |= 1u << k;
+      for (int k = 0; k < LR_EACH; ++k)
+        if (c[k] > 0) add[k] -= fmaf(freq, (float)c[k], pres), again |= 1u << k;
+    }
+#pragma unroll
+    for (int k = 0; k < LR_EACH; ++k) up[k] = again >> k & 1 ? inv : 1.0f, down[k] = again >> k & 1 ? rep : 1.0f;
+  }
 
   char* dst = static_cast<char*>(p.out) + (b * p.ldo_b + first) * SIZE;
   auto row = [&](int i, int at) {
@@ -182,41 +203,50 @@ __global__ void __launch_bounds__(LR_THREADS, 4) logit_rules_kernel(const LogitR
       for (int k = 0; k < LR_EACH; ++k) x[k] = val[at][k];
     }
 #pragma unroll
-    for (int k = 0; k < LR_EACH; ++k) x[k] = fmaf(x[k], again >> k & 1 ? x[k] > 0.0f ? inv : rep : 1.0f, add[k]);
+    for (int k = 0; k < LR_EACH; k += 2) {
+      uint64_t z = f2_pack(x[k], x[k + 1]);
+      const uint64_t y = f2_pack(add[k], add[k + 1]);
+      if (PENAL)
+        z = f2_fma(z, f2_pack(x[k] > 0.0f ? up[k] : down[k], x[k + 1] > 0.0f ? up[k + 1] : down[k + 1]), y);
+      else
+        z = f2_add(z, y);
+      const float2 w = f2_unpack(z);
+      x[k] = w.x, x[k + 1] = w.y;
+    }
     if ((!VEC || DT == 2) && ok[at] != 0xffu) {
 #pragma unroll
       for (int k = 0; k < LR_EACH; ++k)
         if (!(ok[at] >> k & 1)) x[k] = -INFINITY;
     }
     if constexpr (VEC) {
-      if (first < p.V) {
-        uint4* to = reinterpret_cast<uint4*>(dst);
-        if constexpr (DT == 2) {
+      uint4* to = reinterpret_cast<uint4*>(dst);
+      if constexpr (DT == 2) {
+        if (in) {
           to[0] = make_uint4(__float_as_uint(x[0]), __float_as_uint(x[1]), __float_as_uint(x[2]), __float_as_uint(x[3]));
           to[1] = make_uint4(__float_as_uint(x[4]), __float_as_uint(x[5]), __float_as_uint(x[6]), __float_as_uint(x[7]));
-        } else {
-          uint32_t w[4];
-#pragma unroll
-          for (int k = 0; k < 4; ++k) {
-            if constexpr (DT == 0)
-              asm("cvt.rn.bf16x2.f32 %0, %1, %2;" : "=r"(w[k]) : "f"(x[2 * k + 1]), "f"(x[2 * k]));
-            else
-              asm("cvt.rn.f16x2.f32 %0, %1, %2;" : "=r"(w[k]) : "f"(x[2 * k + 1]), "f"(x[2 * k]));
-          }
-          if (ok[at] != 0xffu) {
-            // four bits to the top bits of four bytes, and those over the two halves of two words
-            constexpr uint32_t LOW = DT == 0 ? 0xff80ff80u : 0xfc00fc00u;      // two -inf
-#pragma unroll
-            for (int h = 0; h < 2; ++h) {
-              const uint32_t t = (ok[at] >> 4 * h & 15u) * 0x10204080u;
-              uint32_t m0, m1;
-              asm("prmt.b32 %0, %1, 0, 0x9988;" : "=r"(m0) : "r"(t));          // a byte's top bit, eight times
-              asm("prmt.b32 %0, %1, 0, 0xbbaa;" : "=r"(m1) : "r"(t));
-              w[2 * h] = (w[2 * h] & m0) | (LOW & ~m0), w[2 * h + 1] = (w[2 * h + 1] & m1) | (LOW & ~m1);
-            }
-          }
-          to[0] = make_uint4(w[0], w[1], w[2], w[3]);
         }
+      } else {
+        uint32_t w[4];
+#pragma unroll
+        for (int k = 0; k < 4; ++k) {
+          if constexpr (DT == 0)
+            asm("cvt.rn.bf16x2.f32 %0, %1, %2;" : "=r"(w[k]) : "f"(x[2 * k + 1]), "f"(x[2 * k]));
+          else
+            asm("cvt.rn.f16x2.f32 %0, %1, %2;" : "=r"(w[k]) : "f"(x[2 * k + 1]), "f"(x[2 * k]));
+        }
+        if (p.allowed) {
+          // four bits to the top bits of four bytes, and those over the two halves of two words
+          constexpr uint32_t LOW = DT == 0 ? 0xff80ff80u : 0xfc00fc00u;      // two -inf
+#pragma unroll
+          for (int h = 0; h < 2; ++h) {
+            const uint32_t t = (ok[at] >> 4 * h & 15u) * 0x10204080u;
+            uint32_t m0, m1;
+            asm("prmt.b32 %0, %1, 0, 0x9988;" : "=r"(m0) : "r"(t));          // a byte's top bit, eight times
+            asm("prmt.b32 %0, %1, 0, 0xbbaa;" : "=r"(m1) : "r"(t));
+            w[2 * h] = (w[2 * h] & m0) | (LOW & ~m0), w[2 * h + 1] = (w[2 * h + 1] & m1) | (LOW & ~m1);
+          }
+        }
+        if (in) to[0] = make_uint4(w[0], w[1], w[2], w[3]);
       }
     } else {
 #pragma unroll
@@ -224,37 +254,34 @@ __global__ void __launch_bounds__(LR_THREADS, 4) logit_rules_kernel(const LogitR
         if (first + k * step < p.V) store_f(dst, k * step, x[k], DT);
     }
     dst += p.ldo_r * SIZE;
-    const int d = p.penal ? s_draft[i % LR_THREADS] : -1;
-    if (d >= 0 && d / (32 * LR_EACH) == warp) {   // the rows after this one count it
+    if (PENAL && drafted >> (i & 31) & 1) {       // the rows after this one count it
+      const int at = __shfl_sync(0xffffffffu, d, i & 31), token = w0 + at;
       float sum = 0.0f;                           // its biases once more
-#pragma unroll 4
       for (int y = 0; y < p.n_bias; y += 32) {
         const int id = y + lane < p.n_bias ? ids[y + lane] : -1;
-        for (uint32_t who = __ballot_sync(0xffffffffu, id == v0 + d); who != 0; who &= who - 1) sum += values[y + __ffs(who) - 1];
+        for (uint32_t who = __ballot_sync(0xffffffffu, id == token); who != 0; who &= who - 1) sum += values[y + __ffs(who) - 1];
       }
-      const int k = mine(d);
-      if (k >= 0) {
-        int c = counts ? counts[k * step] : 0;
-        for (int y = 0; y <= i; ++y) c += p.drafts[b * p.ld_d + y] == v0 + d;
-        const float now = c > 0 ? sum - fmaf(freq, (float)c, pres) : sum;
-        if (c > 0) again |= 1u << k;
+      int n = 0;
+      for (int y = lane; y <= i; y += 32) n += drafts[y] == token;
+      n = __reduce_add_sync(0xffffffffu, n);
+      if (owner(at) == lane) {
+        const int k = place(at), all = n + (counts ? counts[k * step] : 0);
+        const float now = all > 0 ? sum - fmaf(freq, (float)all, pres) : sum;
 #pragma unroll
-        for (int y = 0; y < LR_EACH; ++y) add[y] = y == k ? now : add[y];
+        for (int y = 0; y < LR_EACH; ++y)
+          if (y == k) {
+            add[y] = now;
+            if (all > 0) up[y] = inv, down[y] = rep;
+          }
       }
     }
   };
   for (int i = 0; i < p.R; i += ROWS) {
-    if (p.penal && i % LR_THREADS == 0) {
-      if (i > 0) {
-        __syncthreads();
-        stage_drafts(i);
-      }
-      __syncthreads();
-    }
+    if (PENAL && i % 32 == 0 && i > 0) stage_drafts(draft_of(i));
 #pragma unroll
     for (int x = 0; x < ROWS; ++x) {
       if (i + x < p.R) row(i + x, x);
-      fetch(x);
+      fetch(x, i + x + ROWS);
     }
   }
 }

@@ -17,7 +17,8 @@
 // Other loads change little: one warp for all of them 126 us at 2 x 64k x 8 rows, the
 // converting warps for themselves by cp.async 134, this 133.
 // Measured (B200, 8 KV heads x 128, 4 query heads each, pages of 16, bf16; device time in a graph of
-// calls): 16 x 1-3k tokens x 8 rows 54 us, x 16 rows 75; with mma.sync in tiles of 16 rows 53 and 89.
+// calls): 16 x 1-3k tokens x 8 rows 50 us, x 16 rows 65; with mma.sync in tiles of 16 rows 53 and 89 (its sequences' ends
+// weighed as one unit, as here then: 54 and 75).  2 x 64k tokens x 8 rows 130 us; 19 x 0-9k in a window of 1000, 5 rows, 29.
 //
 // Hidden keys as there: a key that no row sees becomes zeros in the fp16 tile, as does one that
 // some rows do not see where its values hold NaN; the rows that see that one add it by

@@ -20,6 +20,10 @@
 // one launch each: every CTA scans all sequences (a block of 256 at a time) and writes
 // its share of the places, and the last one to finish moves the state on that the
 // others were reading (held, free_count).
+//
+// Measured (B200, device time in a graph of calls): reserve and release together 8 - 9.5 us for 32
+// sequences x 4 tokens, 12 for 64 prompts of up to 2048 tokens; 13 issued from Python, which is
+// the time of the two calls on the host.
 #pragma once
 #include "paged.cuh"
 

@@ -15,9 +15,10 @@ namespace {
 
 template <int DT>
 int adjust(const LogitRulesArgs& a, bool vec, void* stream) {
-  const dim3 grid((unsigned)cdiv(a.V, LR_TOKENS), (unsigned)a.B);
-  return vec ? launch_on(logit_rules_kernel<DT, true>, grid, LR_THREADS, 0, stream, false, a)
-             : launch_on(logit_rules_kernel<DT, false>, grid, LR_THREADS, 0, stream, false, a);
+  const dim3 grid((unsigned)cdiv(a.V, LR_TOKENS * (LR_THREADS / 32)), (unsigned)a.B);
+  auto launch = [&](auto kernel) { return launch_on(kernel, grid, LR_THREADS, 0, stream, false, a); };
+  if (a.penal) return vec ? launch(logit_rules_kernel<DT, true, true>) : launch(logit_rules_kernel<DT, false, true>);
+  return vec ? launch(logit_rules_kernel<DT, true, false>) : launch(logit_rules_kernel<DT, false, false>);
 }
 
 }  // namespace

@@ -138,7 +138,8 @@ class PagedBatch:
         return x.view(B, L, -1), new
 
     def finish(self, done: torch.Tensor) -> None:
-        """Sequences with done[b] (bool) end: their length becomes 0 and, with a pool, their pages go back to it."""
+        """Sequences with done[b] (bool) end: their length becomes 0 and, with a pool, their pages go back to it.
+        The next step starts such a sequence anew, with its `last`."""
         with torch.inference_mode():
             self.lens.masked_fill_(done, 0)
             self._give_back()
