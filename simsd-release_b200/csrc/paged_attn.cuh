@@ -44,6 +44,8 @@
 // calls, in brackets calls one after the other on a stream): 2 x 120-128k tokens 173 us
 // (177), 6.2 TB/s, 94 % of the measured copy rate; 32 x 0.3-4k 38 us (40), 4.7 TB/s, 72 %;
 // 1 x 100 7.9 us (10.2, the host's time for a call).
+// With a window only the units that some row sees are cut up: 16 x 8-32k tokens in a window of 4096 and 4
+// first keys 52 us, 5.2 TB/s, 79 %.
 #pragma once
 #include "paged.cuh"
 

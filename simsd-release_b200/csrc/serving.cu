@@ -83,7 +83,9 @@ int attend(const PagedAttnArgs& a, const PagedPlan& pl, void* stream) {
   if (rc != SIMSD_OK) return rc;
   return launch_on(paged_attention_kernel<D, NT, BF, WIN>, dim3((unsigned)pl.grid), PAT_THREADS, smem, stream, false, a);
 }
-// A window leaves few keys, so its rows go in tiles of 16 at most, each reading them again.
+// The tcgen05 form has no window: its rows go in tiles of 16 at most, each reading the keys again.  16 x 8 - 32k
+// tokens, window 4096, 4 query heads on each of 8: 52 us for a token, 101 for 8, 358 for 32; 4096 keys without a
+// window 53 and 101 us for 8 and 32.
 template <int D, bool BF>
 int attend_window(const PagedAttnArgs& a, const PagedPlan& pl, void* stream) {
   return pl.nr == 8 ? attend<D, 1, BF, true>(a, pl, stream) : attend<D, 2, BF, true>(a, pl, stream);

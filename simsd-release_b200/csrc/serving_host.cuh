@@ -97,7 +97,9 @@ inline PagedPlan paged_plan_of(int nr, int ctas_per_sm, int D) {
 }
 // with mma.sync: tiles of 8 or 16 rows
 inline PagedPlan paged_plan_tiles(long long rows, int D) { return paged_plan_of(rows <= 8 ? 8 : 16, PAT_CTAS_PER_SM, D); }
-// over the 8-bit cache: up to 8 rows with mma.sync, three CTAs an SM, else tcgen05
+// over the 8-bit cache: up to 8 rows with mma.sync, three CTAs an SM, else tcgen05.  2 x 120-128k keys for 4 rows
+// take 90 us with mma.sync, 2 x 64k for 32 rows 130 with tcgen05, near three times that a key; at 32 and 64 rows x 16 x 1-3k
+// tcgen05 takes 50 and 65 us, mma.sync in tiles of 16 53 and 89.
 inline PagedPlan paged_plan8(long long rows, int D) {
   if (rows <= 8) return paged_plan_of(8, 3, D);
   return paged_plan_of(rows <= 32 ? 32 : rows <= 64 ? 64 : 128, 1, D);
