@@ -23,6 +23,7 @@
 // shared memory); blocks of 64 tokens 43, of 8 and of 1 51 and 52, 16 tokens a task.  4 tokens 4.1.
 #pragma once
 #include "paged.cuh"
+#include "paged8_rows.cuh"
 
 namespace simsd {
 
@@ -194,9 +195,8 @@ __global__ void __launch_bounds__(PA8_THREADS, 4) paged_append8_kernel(const Pag
       continue;
     }
     // ---- keys or values: the block's rows t, lo <= t < hi, its page and scale
-    const int block_at = (old / p.span + k) * p.span;
-    if (block_at >= top || c == 0) continue;
-    const int lo = max(old, block_at) - shift, hi = min(top, block_at + p.span) - shift;
+    const PagedRows8 own_rows = paged_rows8(n, c, top, p.L, p.span, k);
+    const int block_at = own_rows.at, lo = own_rows.lo, hi = own_rows.hi;
     if (lo >= hi) continue;
     const uint16_t* src = qkv + b * p.ldq_b + (long long)(p.Hq + h) * D;
     // rows base .. base + 15 into the lane's places of shared memory; the largest magnitudes of its part of
