@@ -500,9 +500,11 @@ __global__ void __launch_bounds__(P8T_THREADS, 1) paged_attention8_tc_kernel(con
         if (lane == 0) mbar_arrive(smem_u32(sc_empty + unit));
         if (++unit == S::NU) unit = 0, uph ^= 1;
         // O of the units before has been summed, P may be written
-        if (n > 0 && !(ok = wait_all(pv_done, (n - 1) & 1))) break;
-        if (n > 0 && at.unit > first_unit && __any_sync(0xffffffffu, up)) {
+        if (n > 0) {
+          if (!(ok = wait_all(pv_done, (n - 1) & 1))) break;
           tc_fence_after();
+        }
+        if (n > 0 && at.unit > first_unit && __any_sync(0xffffffffu, up)) {
 #pragma unroll 1
           for (int c = 0; c < D / 16; ++c) {
             float x[16];

@@ -595,9 +595,11 @@ __global__ void __launch_bounds__(PTC_THREADS, 1) paged_attention_tc_kernel(cons
         }
         l = fmaf(l, w_old, (l4[0] + l4[1]) + (l4[2] + l4[3]));
         // O of the units before has been summed, P may be written
-        if (n > 0 && !(ok = wait_all(pv_done, (n - 1) & 1))) break;
-        if (n > 0 && at.unit > first_unit && __any_sync(0xffffffffu, up)) {
+        if (n > 0) {
+          if (!(ok = wait_all(pv_done, (n - 1) & 1))) break;
           tc_fence_after();
+        }
+        if (n > 0 && at.unit > first_unit && __any_sync(0xffffffffu, up)) {
 #pragma unroll 1
           for (int c = 0; c < D / 16; ++c) {
             float x[16];
