@@ -201,11 +201,11 @@ int simsd_paged_attention_window(const void* q, const void* k_cache, const void*
   a.ld_page = ld_page;
   a.ld_head = ld_head;
   a.ld_tok = ld_tok;
-  const PagedPlan pl = window ? paged_plan_tiles(a.rows, head_dim) : paged_plan(L, a.G, head_dim);
+  const PagedPlan pl = a.window ? paged_plan_tiles(a.rows, head_dim) : paged_plan(L, a.G, head_dim);
   rc = paged_attn_plan(a, pl, workspace, workspace_bytes);
   if (rc != SIMSD_OK) return rc;
   const bool bf = dtype == SIMSD_BF16;
-  if (window) {
+  if (a.window) {
     if (head_dim == 64) return bf ? attend_window<64, true>(a, pl, stream) : attend_window<64, false>(a, pl, stream);
     return bf ? attend_window<128, true>(a, pl, stream) : attend_window<128, false>(a, pl, stream);
   }
