@@ -609,7 +609,7 @@ int simsd_paged_attention8(const void* q, const void* k_cache, const void* v_cac
  * max(held, ceil(lens / page_size)), from the top of the stack, sequence by sequence, into the
  * row's places from h on.  Row b of slots and positions [B, L] ends in its c tokens (slot
  * page * page_size + place, position lens .. lens + c - 1); before them slot -1, position 0.
- * total[b] = lens[b] + c.  From the first sequence that the stack cannot serve on, those that
+ * total[b] = lens[b] + c, and total - lens is the count that simsd_paged_append8 takes.  From the first sequence that the stack cannot serve on, those that
  * need a page get no tokens (all -1, total = lens) and SIMSD_DEV_ERR_CAPACITY is raised; so
  * it is with one whose pages would not fit its row.  A negative length (SIMSD_DEV_ERR_BAD_INDEX)
  * gets none, total 0.

@@ -79,7 +79,9 @@ def paged_append8(qkv: torch.Tensor, heads: int, kv_heads: int, k_cache: torch.T
     of sequence b is the token at position seq_lens[b] - L + t.  count [B] int32: only the last
     count[b] rows are tokens, those before them padding (None: all L; positions before
     the sequence's start are padding anyway): their q is zero, nothing else of them is
-    used.  page_table [B, max_pages] int32 as for `paged_attention`; no page is
+    used.  After `paged_reserve` it is the tokens that were served, total - lens, not those that
+    were asked for: seq_lens counts no others, and rows too many would be written over a
+    sequence's older tokens.  page_table [B, max_pages] int32 as for `paged_attention`; no page is
     written by two sequences.  cos, sin, q_weight, k_weight, eps: as for `paged_append`.
 
     Where a call writes a block's first token, the block's scale is the smallest power of two

@@ -58,7 +58,8 @@ def paged_reserve(page_table: torch.Tensor, lens: torch.Tensor, held: torch.Tens
     stack, sequence by sequence; page_table, held and free_count move on with that, lens
     does not.  Row b of slots and positions ends in the sequence's new tokens; before them stand
     slot -1, which `paged_append` skips, and position 0.  total: lens + count, the lengths that
-    attention over the new tokens takes.
+    attention over the new tokens takes; total - lens is what was served, the `count` of
+    `paged_append8`.
 
     From the first sequence on that the stack cannot serve, those that need a page get no tokens
     (slots -1, total = lens), and DEV_ERR_CAPACITY is raised in `_lib.device_error()`; so it
