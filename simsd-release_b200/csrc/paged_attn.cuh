@@ -75,6 +75,9 @@ struct PagedAttnArgs {
 // A CTA is 4 warps of 16 keys (a unit is one step of all of them) x NT 8-row tiles.
 constexpr int PAT_WARPS = 4, PAT_THREADS = PAT_WARPS * 32, PAT_TK = 16 * PAT_WARPS;
 constexpr int PAT_CTAS_PER_SM = 2;
+// CTAs of the forms with tcgen05 at most: a sequence may be cut between all of them, and who joins its parts holds a
+// maximum and a sum of every part's rows in shared memory (their shapes assert it; a B200 has 148 SMs).
+constexpr int PTC_MAX_PARTS = 156;
 
 template <int D, int NT>
 struct PatShape {

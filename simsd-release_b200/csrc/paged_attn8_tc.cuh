@@ -39,6 +39,7 @@ struct P8tShape {
   static constexpr int SC = 3 * 512;                           // a unit's scales: of keys, of values, log2 of these
   static constexpr int X = 16384;                              // 32 dims of every lane's O, where copies are joined
   static constexpr int BYTES = 1024 + NS * TILE + NR * RAW + X + 1024 + NU * SC + 512;
+  static_assert(PTC_MAX_PARTS * R * 8 <= BYTES - 1024 - 512);  // ptc_join, in front of the barriers
   using Tmem = PtcShape<D, R>;
 };
 

@@ -56,6 +56,7 @@ struct PtcShape {
   // TMEM columns: S of even and odd units, O, then Q and P, two 16-bit values a column
   static constexpr int O = 256, Q = O + D, P = Q + D / 2;
   static_assert(P + 64 <= 512);
+  static_assert(PTC_MAX_PARTS * R * 8 <= BYTES - 1024 - 512);    // ptc_join, in front of the barriers
 };
 
 // D (+)= A B^T with A in TMEM (a lane per row, two 16-bit values a column)
@@ -122,7 +123,8 @@ __device__ __forceinline__ void ptc_tma(uint32_t dst, const void* map, uint32_t 
 }
 
 // Joins the parts of a cut sequence (rows r0 .. r0 + R - 1 of KV head g), as
-// paged_join; parts hold R rows of D.  `buf`: parts * R float2 of shared memory.
+// paged_join; parts hold R rows of D.  `buf`: parts * R float2 of shared memory, from the first operand
+// tile on, over all that lies in front of the barriers: nothing of it is in use by then.
 template <int D, int R, bool BF, int THREADS = PTC_THREADS>
 __device__ void ptc_join(const PagedAttnArgs& p, const PagedPart& x, float2* buf) {
   const int tid = threadIdx.x;

@@ -90,7 +90,7 @@ struct PagedPlan {
 inline PagedPlan paged_plan_of(int nr, int ctas_per_sm, int D) {
   PagedPlan p;
   p.nr = nr;
-  p.grid = std::min(ctas_per_sm * sm_count(), SIMSD_PAGED_COUNTER_BYTES / (int)sizeof(int));
+  p.grid = std::min(ctas_per_sm * sm_count(), nr > 16 ? PTC_MAX_PARTS : SIMSD_PAGED_COUNTER_BYTES / (int)sizeof(int));
   p.ml_at = SIMSD_PAGED_COUNTER_BYTES + align256((size_t)2 * p.grid * D * p.nr * sizeof(float));
   p.bytes = p.ml_at + align256((size_t)2 * p.grid * p.nr * sizeof(float2));
   return p;
