@@ -571,7 +571,8 @@ int simsd_paged_attention_window(const void* q, const void* k_cache, const void*
  *   want = the smallest 2^e with a <= 448 2^e, e from -64 to 64
  *   scale = want where the block's first token is new, else max(scale, want)
  * where it grows the block's tokens before the new ones are rounded anew to it; tokens after
- * them are left as they are.  Numbers that are not finite are stored as NaN.  A position past the page
+ * them are left as they are.  It does not come down before the block's first token is written again, also
+ * where the tokens that it grew for are taken back.  Numbers that are not finite are stored as NaN.  A position past the page
  * table or cos / sin, or a page outside the cache, is flagged (SIMSD_DEV_ERR_BAD_INDEX): the
  * keys and values are not written, and q is zero for a position past the tables.  No page
  * is written by two sequences of a call, and the caches' and scales' elements share no memory.
