@@ -51,8 +51,10 @@ class PagedBatch:
     one, and DEV_ERR_CAPACITY is raised in `_lib.device_error()`.
     cache_dtype: torch.float8_e4m3fn holds the cache in 8 bits, with a scale for each `block` tokens
     of a head (a divisor of page_size; all of a page up to 16 tokens, 16 of a larger one where
-    that divides it, when None).  window, sinks: each token sees the newest `window` tokens and the
-    first `sinks` only.
+    that divides it, when None).  Drafts that a step does not keep may leave a larger scale in the
+    block that they reached, for its kept tokens too (`paged_append8`): what such a cache holds goes by
+    them as well.  window, sinks: each token sees the newest `window` tokens and the first `sinks`
+    only; the pages of the others stay the sequence's.
     """
 
     def __init__(self, model: SDARVerifyModel, sequences: int, max_len: int, page_size: int = 16,
@@ -108,7 +110,8 @@ class PagedBatch:
                tail_mask: torch.Tensor | None = None) -> torch.Tensor:
         """Final-norm hidden states [B, L, H] of ids [B, L], which go to the cache after the
         `lens` tokens that are there (`lens` itself is not moved).  count [B]: only the last
-        count[b] of a row are tokens, those before them padding."""
+        count[b] of a row are tokens, those before them padding.  The rows of a sequence that the pool has
+        no page for (DEV_ERR_CAPACITY) say nothing."""
         return self._hidden(ids, count, tail_mask)[0]
 
     def _hidden(self, ids, count, tail_mask):
@@ -225,7 +228,7 @@ def main(sequences: int = 8, drafts: int = 3, steps: int = 20) -> None:
         u = torch.rand(sequences, drafts, generator=g, device=dev)
         e = torch.empty(sequences, shape.vocab, device=dev).exponential_(generator=g).clamp_(min=1e-20)
         guess = torch.randint(0, shape.vocab, (sequences, drafts), generator=g, device=dev)
-        if i % 2:   # what the model itself would say, from a dry run without moving on
+        if i % 2:   # what the model itself would say, from steps that are taken back but for the scales they leave
             lens, last, answered = batch.lens.clone(), batch.last.clone(), counts.clone()
             none = torch.empty(sequences, 0, dtype=torch.int64, device=dev)
             for k in range(drafts):
