@@ -546,8 +546,10 @@ int simsd_paged_attention(const void* q, const void* k_cache, const void* v_cach
 /*
  * The same through a window: the query at position x = n - L + t sees a key j only where
  * also j > x - window or j < sinks (window 0: no window, every key).  Keys that no query of
- * the call sees are not read, and the pages that hold nothing else may be any.  With a
- * window max_pages page_size <= 2^30 (more: SIMSD_ERR_UNSUPPORTED).
+ * the call sees are not read, and the pages that hold nothing else may be any.  A window
+ * of max_pages page_size or more hides nothing and is none.  With one max_pages page_size <=
+ * 2^30, and ceil(G L / 16) takes the place of ceil(G L / 128) in the limit there (more:
+ * SIMSD_ERR_UNSUPPORTED).
  */
 int simsd_paged_attention_window(const void* q, const void* k_cache, const void* v_cache, int num_pages, int page_size,
                                  int64_t ld_page, int64_t ld_head, int64_t ld_tok, const int32_t* page_table,
@@ -589,7 +591,7 @@ int simsd_paged_append8(const void* qkv, int64_t ldq_b, int64_t ldq_t, int B, in
  * simsd_paged_attention_window over that cache (window 0: none).  Any positive scales up to
  * 2^64 do, not only powers of two; sums are fp32 and weights fp16 (11 bits down to 2^-22 of
  * the largest).  The workspace as for simsd_paged_attention, of a size of its own; + 4 in the
- * place of + 3 in the limit there, and max_pages page_size <= 2^30.
+ * place of + 3 in the limit there, and 2 in that of ceil(G L / 128) for 9 to 16 rows G L; max_pages page_size <= 2^30.
  */
 size_t simsd_paged_attention8_workspace_size(int L, int Hq, int Hk, int head_dim);
 int simsd_paged_attention8(const void* q, const void* k_cache, const void* v_cache, const float* k_scale,

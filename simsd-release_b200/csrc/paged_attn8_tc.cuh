@@ -1,4 +1,4 @@
-// Attention over the 8-bit paged cache for more than 8 rows per KV head, on the 5th-generation
+// Attention over the 8-bit paged cache for more than 16 rows per KV head, on the 5th-generation
 // tensor cores: the operator and arithmetic of paged_attn8.cuh with the products of
 // paged_attn_tc.cuh (a unit of 128 keys; the R queries stand 128 / R times in a product of 128
 // rows, copy f of a row keeping the unit's keys f R .. f R + R - 1).

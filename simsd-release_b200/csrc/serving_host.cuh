@@ -97,11 +97,13 @@ inline PagedPlan paged_plan_of(int nr, int ctas_per_sm, int D) {
 }
 // with mma.sync: tiles of 8 or 16 rows
 inline PagedPlan paged_plan_tiles(long long rows, int D) { return paged_plan_of(rows <= 8 ? 8 : 16, PAT_CTAS_PER_SM, D); }
-// over the 8-bit cache: up to 8 rows with mma.sync, three CTAs an SM, else tcgen05.  2 x 120-128k keys for 4 rows
-// take 90 us with mma.sync, 2 x 64k for 32 rows 130 with tcgen05, near three times that a key; at 32 and 64 rows x 16 x 1-3k
-// tcgen05 takes 50 and 65 us, mma.sync in tiles of 16 53 and 89.
+// over the 8-bit cache: up to 16 rows with mma.sync in tiles of 8, three CTAs an SM, else tcgen05, whose time hardly goes
+// by the rows.  Two tiles and tcgen05 at 9 to 16 rows (us; 128 dims, 8 KV heads): 16 x 1-3k tokens 31 and 46, 32 x
+// 0.3-4k 40 and 60, 2 x 64k 79 and 112, 19 x 0-9k in a window of 1000 24 and 31, pages of one token 52 and 59, 1 x 100
+// 8.3 and 11.5.  Three at 17 to 24: 41 and 47, 59 and 61, 125 and 113, 34 and 32, 70 and 60, 8.3 and 12.  Four at 32: 51
+// and 48, 68 and 63, 141 and 115, 36 and 34, 85 and 61, 8.4 and 13.
 inline PagedPlan paged_plan8(long long rows, int D) {
-  if (rows <= 8) return paged_plan_of(8, 3, D);
+  if (rows <= 16) return paged_plan_of(8, 3, D);
   return paged_plan_of(rows <= 32 ? 32 : rows <= 64 ? 64 : 128, 1, D);
 }
 
