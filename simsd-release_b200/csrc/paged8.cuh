@@ -354,6 +354,7 @@ __global__ void __launch_bounds__(PA8_THREADS, 4) paged_append8_kernel(const Pag
     const bool infinite = a == INFINITY;
     if (infinite) a = largest(false);
     const float s = fmaxf(had, p8_power(p8_exponent(a))), inv = 1.0f / s;
+    __syncwarp();                                    // every lane has read the scale
     if (lane == 0) *scale = s;
     // the new tokens; the last rows are still at hand
     for (int base = last; base >= lo; base -= PA8_ROWS) {
