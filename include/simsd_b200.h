@@ -533,8 +533,9 @@ int simsd_paged_append(const void* qkv, int64_t ldqkv, int T, int Hq, int Hk, in
  * 0, lse = -inf.  q, o [B, L, Hq, head_dim] contiguous, lse [B, L, Hq] or NULL.
  * A length over max_pages * page_size is cut there, the newest L keys being those of the
  * cut length (SIMSD_DEV_ERR_BAD_INDEX); a negative one counts as 0.
- * The lengths are read on the device only.  B Hk ceil(G L / 128) (max_pages
- * page_size / 64 + 3) < 2^31 (more: SIMSD_ERR_UNSUPPORTED).
+ * Scores and sums are fp32, the weights of the second product q's type.  The lengths are
+ * read on the device only.  B Hk ceil(G L / 128) (max_pages page_size / 64 + 3) < 2^31 (more:
+ * SIMSD_ERR_UNSUPPORTED).
  */
 size_t simsd_paged_attention_workspace_size(int L, int Hq, int Hk, int head_dim);
 int simsd_paged_attention(const void* q, const void* k_cache, const void* v_cache, int num_pages, int page_size,
@@ -562,7 +563,8 @@ int simsd_paged_attention_window(const void* q, const void* k_cache, const void*
  * The paged cache held in 8 bits: k_cache / v_cache [num_pages, Hk, page_size, head_dim]
  * e4m3 with strides of multiples of 16, and k_scale / v_scale [num_pages, Hk, page_size /
  * block] fp32 (strides lds_page, lds_head, lds_block): a stored number stands for its block's
- * scale times itself.  block divides page_size.
+ * scale times itself.  block divides page_size.  Numbers are scaled in fp32, by a factor 1 / scale that is exact
+ * for powers of two, and rounded to e4m3.
  *
  * simsd_paged_append8: sequence b's new tokens are the last c = count[b] (L when NULL; cut to
  * 0 .. min(L, n)) of its L rows of qkv [B, L, (Hq + 2 Hk) head_dim] (strides ldq_b, ldq_t)
@@ -612,9 +614,9 @@ int simsd_paged_attention8(const void* q, const void* k_cache, const void* v_cac
  * max(held, ceil(lens / page_size)), from the top of the stack, sequence by sequence, into the
  * row's places from h on.  Row b of slots and positions [B, L] ends in its c tokens (slot
  * page * page_size + place, position lens .. lens + c - 1); before them slot -1, position 0.
- * total[b] = lens[b] + c, and total - lens is the count that simsd_paged_append8 takes.  From the first sequence that the stack cannot serve on, those that
- * need a page get no tokens (all -1, total = lens) and SIMSD_DEV_ERR_CAPACITY is raised; so
- * it is with one whose pages would not fit its row.  A negative length (SIMSD_DEV_ERR_BAD_INDEX)
+ * total[b] = lens[b] + c, and total - lens is the count that simsd_paged_append8 takes.
+ * From the first sequence that the stack cannot serve on, those that need a page get no tokens
+ * (all -1, total = lens) and SIMSD_DEV_ERR_CAPACITY is raised; so it is with one whose pages would not fit its row.  A negative length (SIMSD_DEV_ERR_BAD_INDEX)
  * gets none, total 0.
  * simsd_paged_release: sequence b keeps the pages of keep[b] tokens (negative: none), and its
  * other held ones go back onto the stack, sequence by sequence, each one's in its order; a stack
@@ -639,7 +641,8 @@ int simsd_paged_release(const int32_t* page_table, int64_t ld_table, int max_pag
  *   - frequency[b] c - presence[b]                 where c > 0
  *   + the sum of bias_values[b, k] over bias_ids[b, k] = v
  *   -inf                                           where allowed[b, i] lacks v
- * in fp32, what is added summed first, rounded once.  seen and allowed are bit lists of ceil(V / 32)
+ * in fp32, what is added summed first, rounded once; the division is a product with 1 / repetition[b] in
+ * fp32, 2^-23 off at most.  seen and allowed are bit lists of ceil(V / 32)
  * words (token v: bit v % 32 of word v / 32; NULL: nothing seen, everything allowed).  Drafts
  * outside [0, V) count nowhere; bias ids below 0 are none, those from V on raise
  * SIMSD_DEV_ERR_BAD_INDEX.  dtype: all three.  out's rows share no memory.  B <= 65535 (more: SIMSD_ERR_UNSUPPORTED).

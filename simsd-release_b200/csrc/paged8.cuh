@@ -2,13 +2,15 @@
 // is in paged_attn8.cuh).
 //
 // Keys and values are e4m3 with a scale for each block of `block` tokens and head: the
-// number that is stored for x is rn(x / s), and stands for s times that.  Sequence b's
+// number that is stored for x is rn(x (1 / s)), and stands for s times that.  The product and the
+// reciprocal are fp32: exact for the powers of two that appends make, 2^-23 off at most for an older
+// block's other scale, against e4m3's 2^-4.  Sequence b's
 // new tokens are its newest, at positions n - c .. n - 1 (n = seq_lens[b], c = count[b]),
 // in the last c of its L rows.  Per block and head that they touch, with a the largest
 // finite |x| among the block's new tokens (x: the normed and rotated key, the value; fp32):
 //   want = 2^e, the smallest with a <= 448 2^e, e from -64 to 64
 //   s    = want where the block's first token is new, else max(the block's scale, want)
-// and where s has grown, the block's older tokens are stored anew, rn(stored s_old / s).
+// and where s has grown, the block's older tokens are stored anew, rn(stored (s_old / s)).
 // A power of two costs e4m3 no precision but near its smallest numbers, and makes that
 // step exact there too.  Values that are not finite are stored as NaN and do not take
 // part in a; finite ones past 448 2^64 are stored as 448.

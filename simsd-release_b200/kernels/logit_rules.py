@@ -80,7 +80,7 @@ def adjust_logits(logits: torch.Tensor, counts: torch.Tensor | None = None, draf
     i drafted tokens (R = K + 1, as `speculative_verify` takes them).  For token v, in fp32
     (what is added summed first), rounded once:
 
-    * repetition [B] fp32 (positive): a logit over 0 is divided by it, another one multiplied,
+    * repetition [B] fp32 (positive): a logit over 0 is divided by it (multiplied by its fp32 reciprocal), another one multiplied,
       where v was answered, drafted before row i, or stands in the prompt;
     * frequency [B], presence [B] fp32: subtracted, times how often and once, where v was
       answered or drafted before row i;

@@ -206,7 +206,8 @@ def paged_attention(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tenso
     is set.  A query that sees no key (an empty sequence, a mask without any) gets
     o = 0 and lse = -inf.  Only visible keys count: what stale cache memory or a
     masked key holds, NaN included, does not reach the output.  scale: D ** -0.5
-    when None.  window: query t, at position x = seq_lens[b] - L + t, sees key j only where
+    when None.  Scores, sums and sums of products are fp32; the weights are rounded to q's type
+    for the second product.  window: query t, at position x = seq_lens[b] - L + t, sees key j only where
     also j > x - window or j < sinks: the newest `window` keys and the first `sinks`.  Keys
     that no query sees are not read, and pages that hold nothing else may have been given
     back (their entries are not read).  Lengths are read on the device, so the call can be captured in a

@@ -90,7 +90,8 @@ def paged_append8(qkv: torch.Tensor, heads: int, kv_heads: int, k_cache: torch.T
     down before the block's first token is written again: where tokens are taken back (rejected drafts, a step
     undone by its lengths), the block that they ended in may keep a scale that only they needed, and the
     kept tokens' numbers under 2^-6 of it are 2^-9 of it apart.  Numbers that are not finite are
-    stored as NaN and leave the scale alone.  Computed in
+    stored as NaN and leave the scale alone.  Numbers are multiplied by the scale's reciprocal in fp32, which is
+    exact for powers of two (a block may have another scale from elsewhere).  Computed in
     fp32, rounded once.  bf16 or fp16; D 64 or 128; R a multiple of 16.
     """
     q = _lib.binding().paged_append8(qkv, heads, kv_heads, k_cache, v_cache, k_scale, v_scale, page_table, seq_lens, cos, sin,
