@@ -19,8 +19,10 @@
 // row): 64 x 8 rows 83.6 us, 4.3 TB/s (66 % of the bytes' time at the copy rate), without biases 73.5, with no
 // rule at all 52 (91 %); 64 x 1 row 35.  A CTA for 2048 tokens with the biases and drafts in shared memory took
 // 117, 101, 61 and 45: some 100 instructions a warp's row instead of 150, and no waits for the CTA.  What is left is the
-// setup, 570 instructions a warp and its loads' latency, at 60 % of the issue slots.  Rows whose 8 tokens do not lie
-// on 16 bytes take 2.8 times their bytes' time (64 x 4 x 151937: 86 us), 2-byte loads and stores.
+// setup, 570 instructions a warp and its loads' latency, at 60 % of the issue slots.  A list of n biases is read by each
+// of the V / 256 warps of a sequence: 3000 take 194 us, 10000 518, most of it the lists.  fp32, 32 x 4 rows 41 us (66 %).
+// Rows whose 8 tokens do not lie on 16 bytes take 2.8 times their bytes' time (64 x 4 x 151937: 86 us; fp32, 32 x 4 x
+// 50021: 22, 2.5 times), loads and stores of single numbers.
 #pragma once
 #include "paged.cuh"
 #include "spec_verify.cuh"

@@ -22,7 +22,7 @@
 // tables: each element is widened, normed, rotated, compared, scaled and narrowed.  Measured (B200, 32 + 2 x
 // 8 heads x 128, bf16, device time in a graph of calls): 4 x 2048 tokens in blocks of 16 41 us, 63 % of
 // the bytes' time at the copy rate (51 with a block's rows in registers, of which some spilled, instead of in
-// shared memory); blocks of 64 tokens 43, of 8 and of 1 51 and 52, 16 tokens a task.  4 tokens 4.1.
+// shared memory); blocks of 64 tokens 43, of 8 and of 1 51 and 52, 16 tokens a task.  4 tokens 4.1.  64 dims, blocks of 16 28 (floor 14.4).
 #pragma once
 #include "paged.cuh"
 #include "paged8_rows.cuh"

@@ -25,7 +25,9 @@
 // 120-128k tokens 90 us, 6.0 TB/s, 90 % of the bytes' time at the copy rate (101 with each warp loading for itself by
 // cp.async); 32 x 0.3-4k 26 us, 53 %, of which the first units' lengths, pages and data take 5; 1 x
 // 100 7.8.  16 x 8-16k tokens with pages of one token,
-// by cp.async, take 112 us (floor 56).
+// by cp.async, take 112 us (floor 56).  16 x 8-32k in a window of 4096 and 4 first keys 35 us (floor 20.5).
+// Up to 16 rows a KV head, 9 to 16 in two tiles that each read the keys (paged_plan8 has the figures); more in
+// paged_attn8_tc.cuh.
 //
 // In an operand of the first product a lane's four bytes are four
 // neighbouring dims of a key (the queries' dims are ordered alike).  For the second,

@@ -12,13 +12,16 @@
 // maximum goes by, so that the softmax takes none.
 //
 // What bounds it is not HBM but the chain of a unit: S (some 1000 cycles with its waits), the
-// softmax of 32 keys a thread (1100 - 1300), the weights' way back into TMEM and O, some 3200
-// cycles a unit as in paged_attn_tc.cuh, where that is what a unit of 16-bit keys takes to be read.
+// softmax of 32 keys a thread (1100 - 1300), the weights' way back into TMEM and O, 2.1 us a unit at 2 x 64k
+// tokens x 8 rows x 4 heads (8192 units on 148 CTAs).  paged_attn_tc.cuh, the same chain without a conversion before it, takes
+// 1.7 there, on twice the bytes; what the 0.4 consist of has not been taken apart (the fp16 ring holds two
+// units, its ring three).  The 16-bit cache is therefore the faster one for more than 16 rows without a window.
 // Other loads change little: one warp for all of them 126 us at 2 x 64k x 8 rows, the
-// converting warps for themselves by cp.async 134, this 133.
+// converting warps for themselves by cp.async 134, this 133 (on one box then).
 // Measured (B200, 8 KV heads x 128, 4 query heads each, pages of 16, bf16; device time in a graph of
-// calls): 16 x 1-3k tokens x 8 rows 50 us, x 16 rows 65; with mma.sync in tiles of 16 rows 53 and 89 (its sequences' ends
-// weighed as one unit, as here then: 54 and 75).  2 x 64k tokens x 8 rows 130 us; 19 x 0-9k in a window of 1000, 5 rows, 29.
+// calls, in brackets over the 16-bit cache): 16 x 1-3k tokens x 8 rows 49 us (37), x 16 rows 64 (51); with mma.sync in tiles of
+// 16 rows 53 and 89 (its sequences' ends weighed as one unit, as here then: 54 and 75).  2 x 64k tokens x 8 rows 115 us (95); 19 x
+// 0-9k in a window of 1000, 5 rows x 7 heads, 29; 16 x 8-32k in a window of 4096 x 8 and 32 rows 81 (101) and 249 (360).
 //
 // Hidden keys as there: a key that no row sees becomes zeros in the fp16 tile, as does one that
 // some rows do not see where its values hold NaN; the rows that see that one add it by

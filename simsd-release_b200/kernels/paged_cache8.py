@@ -1,5 +1,9 @@
 """A paged key-value cache held in 8 bits, on libsimsd_b200: half the bytes that a
-decoding step reads.
+decoding step reads, and room for twice the tokens.
+
+Attention over it is faster than over the 16-bit cache up to 16 rows (query heads of a KV head times
+tokens) and through a window, slower beyond that without one: 16 sequences of 1000 to 3000 tokens with 8 KV
+heads take 32 us at 16 rows and 49 at 32 (16 bits: 36 and 37).
 
 * `paged_append8(qkv, ...)` — q/k RMSNorm (optional), rotary embedding and the write of
   each sequence's new keys and values, quantised with a scale for each block of tokens
