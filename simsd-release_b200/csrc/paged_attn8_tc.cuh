@@ -17,7 +17,7 @@
 // 1.7 there, on twice the bytes; what the 0.4 consist of has not been taken apart (the fp16 ring holds two
 // units, its ring three).  The 16-bit cache is therefore the faster one for more than 16 rows without a window.
 // Other loads change little: one warp for all of them 126 us at 2 x 64k x 8 rows, the
-// converting warps for themselves by cp.async 134, this 133 (on one box then).
+// converting warps for themselves by cp.async 134, this 133 (in one run then).
 // Measured (B200, 8 KV heads x 128, 4 query heads each, pages of 16, bf16; device time in a graph of
 // calls, in brackets over the 16-bit cache): 16 x 1-3k tokens x 8 rows 49 us (37), x 16 rows 64 (51); with mma.sync in tiles of
 // 16 rows 53 and 89 (its sequences' ends weighed as one unit, as here then: 54 and 75).  2 x 64k tokens x 8 rows 115 us (95); 19 x
